@@ -193,7 +193,7 @@ def _route(logits, k, renormalize):
         w = w / torch.where(used[:, :1], w.sum(1, keepdim=True), 1)
     else:
         w = torch.gather(p, 1, index)
-    w = torch.where(used, w, 0)
+    w = torch.where(torch.isnan(l).any(1, keepdim=True), math.nan, torch.where(used, w, 0))
     expert = torch.where(used, index, E).reshape(-1)
     expert, order = torch.sort(expert, stable=True)
     slot = torch.arange(T * k, device=l.device)
