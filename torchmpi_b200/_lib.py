@@ -214,6 +214,21 @@ _CUDA_PROTOS = {
     "tmpi_gemm_bf16_ex": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _i, _vp]),
     "tmpi_linear_bwd_plan": (_i, [_i, _i, _i, _i, _i, C.POINTER(_sz), _ip]),
     "tmpi_linear_bwd": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp, _i, _vp]),
+    "tmpi_act8_quantize": (_i, [_vp, _vp, _vp, _i64, _i, _i, _vp]),
+    "tmpi_act8_restore": (_i, [_vp, _vp, _vp, _i64, _i, _i, _vp]),
+    "tmpi_act8_gelu_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _vp]),
+    "tmpi_route_limits": (_i, [_ip, _ip]),
+    "tmpi_route_workspace_bytes": (_sz, [_i, _i, _i]),
+    "tmpi_route": (_i, [_vp, _i64, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tmpi_route_gradient": (_i, [_vp, _i64, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "tmpi_expert_dispatch": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "tmpi_expert_dispatch8": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "tmpi_expert_combine": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "tmpi_expert_combine_gradient": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "tmpi_expert_gelu_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "tmpi_grouped_max_experts": (_i, []),
+    "tmpi_grouped_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "tmpi_grouped_weight_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "tmpi_gemm_status": (_i, []),
     "tmpi_gemm_failures": (_i, []),
     "tmpi_gemm_report": (_i, [_i]),

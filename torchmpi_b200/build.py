@@ -64,7 +64,7 @@ def is_current() -> bool:
 
 
 # ---- C++ autograd functions: compiled against PyTorch's headers, resolved against the native library at load time
-BINDINGS_SRC = CSRC / "bindings" / "autograd.cpp"
+BINDINGS_SRC = [CSRC / "bindings" / "autograd.cpp", CSRC / "bindings" / "experts.cpp"]
 BINDINGS = PKG / "lib" / "_autograd.so"
 BINDINGS_STAMP = PKG / "lib" / "bindings.stamp"
 
@@ -73,7 +73,7 @@ def bindings_hash() -> str:
     import hashlib
     import torch
     h = hashlib.sha256(torch.__version__.encode() + sys.version.encode())
-    for f in (BINDINGS_SRC, CSRC / "include" / "tmpi_c_api.h"):
+    for f in (*BINDINGS_SRC, CSRC / "bindings" / "common.h", CSRC / "include" / "tmpi_c_api.h"):
         h.update(f.read_bytes())
     return h.hexdigest()
 
@@ -99,14 +99,21 @@ def build_bindings(force: bool = False) -> Path:
         cc = nvcc()
         cuda = Path(cc).resolve().parent.parent / "include" if cc else Path("/usr/local/cuda/include")
         tmp = BINDINGS.with_suffix(".tmp")
-        cmd = [cxx, "-O2", "-fPIC", "-shared", "-std=c++17", "-DTORCH_EXTENSION_NAME=_autograd", "-DTORCH_API_INCLUDE_EXTENSION_H",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", str(CSRC / "include"),
-               "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda),
-               "-I", sysconfig.get_paths()["include"], str(BINDINGS_SRC), "-o", str(tmp), "-L", str(root / "lib"),
-               "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root / 'lib'}"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"g++ failed for {BINDINGS_SRC.name}:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+        flags = ["-O2", "-fPIC", "-std=c++17", "-DTORCH_EXTENSION_NAME=_autograd", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", str(CSRC / "include"),
+                 "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda),
+                 "-I", sysconfig.get_paths()["include"]]
+        objs = [OBJ / f"bindings_{src.stem}.o" for src in BINDINGS_SRC]
+
+        def run(cmd, name):
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if r.returncode != 0:
+                raise RuntimeError(f"g++ failed for {name}:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+
+        with cf.ThreadPoolExecutor(max_workers=len(objs)) as ex:
+            list(ex.map(lambda so: run([cxx, *flags, "-c", str(so[0]), "-o", str(so[1])], so[0].name), zip(BINDINGS_SRC, objs)))
+        run([cxx, "-shared", *map(str, objs), "-o", str(tmp), "-L", str(root / "lib"),
+             "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root / 'lib'}"], BINDINGS.name)
         tmp.replace(BINDINGS)
         BINDINGS_STAMP.write_text(bindings_hash())
     return BINDINGS

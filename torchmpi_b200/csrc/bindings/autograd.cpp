@@ -7,61 +7,15 @@
 // Scratch memory is allocated per call from PyTorch's caching allocator on the calling stream; the buffers that are kept
 // (KeptZeros) belong to one stream each.  A non-zero status is raised through torchmpi_b200._lib.check, so callers see the usual exceptions.
 // The reference has no counterpart (its layers are Torch7's).
-#include <torch/extension.h>
+#include "common.h"
 #include <c10/cuda/CUDAGraphsC10Utils.h>
-#include <c10/cuda/CUDAStream.h>
-#include <atomic>
 #include <cmath>
 #include <map>
 #include <mutex>
-#include <string>
-#include "tmpi_c_api.h"
 
-namespace {
+namespace tmpi_bind {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-enum { LINEAR, LAYERNORM, ATTENTION, XENT, ATTENTION_BACKWARD, BATCHNORM, CONV, STEM, KINDS };
-std::atomic<long long> g_launches[KINDS];      // attention: calls, and those of the backward alone
 enum { EPI_BIAS = 1 };
-
-void* stream() { return (void*)c10::cuda::getCurrentCUDAStream().stream(); }
-void launched(int what, int n) { g_launches[what].fetch_add(n, std::memory_order_relaxed); }
-
-void check(int status) {
-  if (!status) return;
-  pybind11::gil_scoped_acquire gil;
-  pybind11::module_::import("torchmpi_b200._lib").attr("check")(status);
-}
-
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kHalf: return TMPI_F16;
-    case at::kBFloat16: return TMPI_BF16;
-    case at::kFloat: return TMPI_F32;
-    case at::kDouble: return TMPI_F64;                           // what a kernel does not take, its entry point refuses
-    case at::kByte: return TMPI_U8;
-    case at::kChar: return TMPI_I8;
-    case at::kShort: return TMPI_I16;
-    case at::kInt: return TMPI_I32;
-    case at::kLong: return TMPI_I64;
-    default: throw pybind11::type_error(std::string("torchmpi_b200: unsupported dtype ") + c10::toString(t));
-  }
-}
-
-// Contiguous and on a 16-byte boundary, which the elementwise kernels' loads need: a view into a larger buffer may start
-// anywhere.
-Tensor packed(const Tensor& t, at::MemoryFormat format = at::MemoryFormat::Contiguous) {
-  if (t.is_contiguous(format) && (uintptr_t)t.data_ptr() % 16 == 0) return t;
-  Tensor c = t.contiguous(format);
-  if ((uintptr_t)c.data_ptr() % 16) c = c.clone(format);
-  return c;
-}
-
-// A saved tensor as it was saved: hooks (torch.autograd.graph.save_on_cpu, say) may hand it back in another layout.
-Tensor as_saved(const Tensor& t, at::MemoryFormat format = at::MemoryFormat::Contiguous) { return t.defined() ? packed(t, format) : t; }
 
 // Buffers of arrival counters, which a kernel finds zero and leaves zero.  Two calls may share one only if one ends before the
 // other starts, so there is one per stream, grown to the next power of two.  A call that is being captured gets its own, cleared
@@ -600,7 +554,9 @@ struct StemFn : public torch::autograd::Function<StemFn> {
   }
 };
 
-}  // namespace
+}  // namespace tmpi_bind
+
+using namespace tmpi_bind;
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", [](const Tensor& x, const Tensor& w, const c10::optional<Tensor>& bias, bool gelu) {
@@ -636,5 +592,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("cross_entropy_scratch", xent_scratch);
   m.def("arrival_counters", arrival_counters);
+  register_experts(m);
   m.def("launches", [](int what) { return g_launches[what].load(std::memory_order_relaxed); });
 }

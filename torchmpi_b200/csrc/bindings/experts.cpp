@@ -1,0 +1,308 @@
+// Autograd functions of layers of experts and of 8-bit activation checkpoints (ops/experts.py, ops/act8.py), which make the checks.  Rows
+// are flattened by the callers: x is [rows, width] here.  Scratch memory comes from PyTorch's allocator on the calling stream, per call.
+#include "common.h"
+#include <initializer_list>
+
+namespace tmpi_bind {
+namespace {
+
+enum { PLAIN = 0, GELU = 1, GELU_AND_Z = 2, GELU_AND_Z8 = 3 };      // tmpi_grouped_gemm's modes
+
+using OptTensor = c10::optional<Tensor>;
+Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const int* ints(const Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
+bool wants_grad(std::initializer_list<Tensor> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor& t : inputs)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+struct Kept { Tensor q, scale; };                                   // an 8-bit checkpoint
+
+Kept empty_kept(const Tensor& like, int64_t rows, int64_t cols) {
+  const auto bytes = like.options().dtype(at::kByte);
+  return {at::empty({rows, cols}, bytes), at::empty({rows, (cols + 31) / 32}, bytes)};
+}
+Kept quantize(const Tensor& x) {
+  Kept k = empty_kept(x, x.size(0), x.size(1));
+  check(tmpi_act8_quantize(x.data_ptr(), k.q.data_ptr(), k.scale.data_ptr(), x.size(0), (int)x.size(1), dtype_code(x.scalar_type()), stream()));
+  launched(ACT8, 1);
+  return k;
+}
+Tensor restore(const Kept& k, at::ScalarType type) {
+  Tensor x = at::empty(k.q.sizes(), k.q.options().dtype(type));
+  check(tmpi_act8_restore(k.q.data_ptr(), k.scale.data_ptr(), x.data_ptr(), x.size(0), (int)x.size(1), dtype_code(type), stream()));
+  launched(ACT8, 1);
+  return x;
+}
+std::pair<Tensor, Tensor> gelu_gradient(const Tensor& dy, const Kept& k) {
+  Tensor dz = at::empty_like(dy), h = at::empty_like(dy);
+  check(tmpi_act8_gelu_gradient(dy.data_ptr(), k.q.data_ptr(), k.scale.data_ptr(), dz.data_ptr(), h.data_ptr(), dy.size(0), (int)dy.size(1),
+                                dtype_code(dy.scalar_type()), stream()));
+  launched(ACT8, 1);
+  return {dz, h};
+}
+
+// ---------------------------------------------------------------- products grouped by expert
+// offsets undefined: one expert (w [N, K]) with all rows.  z, scale: see tmpi_grouped_gemm.
+Tensor grouped(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& offsets, bool w_is_kn, int mode, const Tensor& z, const Tensor& scale) {
+  const int experts = offsets.defined() ? (int)w.size(0) : 1, d = (int)w.dim();
+  const int N = (int)w.size(w_is_kn ? d - 1 : d - 2), K = (int)x.size(1);
+  Tensor y = at::empty({x.size(0), N}, x.options());
+  check(tmpi_grouped_gemm(x.data_ptr(), w.data_ptr(), ptr(bias), ints(offsets), y.data_ptr(), z.defined() ? z.data_ptr() : nullptr,
+                          scale.defined() ? scale.data_ptr() : nullptr, (int)x.size(0), experts, K, N, w_is_kn ? 1 : 0, mode, stream()));
+  launched(EXPERTS, 1);
+  return y;
+}
+// dw and, where asked for, db
+void grouped_weight_gradient(const Tensor& dy, const Tensor& x, const Tensor& offsets, const Tensor& row_weights, int64_t experts, Tensor* dw, Tensor* db) {
+  *dw = at::empty({experts, dy.size(1), x.size(1)}, x.options());
+  if (db) *db = at::empty({experts, dy.size(1)}, x.options());
+  check(tmpi_grouped_weight_gradient(dy.data_ptr(), x.data_ptr(), ints(offsets), row_weights.defined() ? row_weights.data_ptr<float>() : nullptr,
+                                     dw->data_ptr(), db ? db->data_ptr() : nullptr, (int)x.size(0), (int)experts, (int)x.size(1), (int)dy.size(1), stream()));
+  launched(EXPERTS, 1);
+}
+
+struct GroupedLinearFn : public torch::autograd::Function<GroupedLinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const OptTensor& bias_, const Tensor& offsets_, bool with_gelu) {
+    const Tensor x = packed(x_), w = packed(w_), bias = bias_.has_value() ? packed(*bias_) : Tensor(), offsets = offsets_.contiguous();
+    Tensor z;
+    if (with_gelu) z = at::empty({x.size(0), w.size(1)}, x.options());
+    const Tensor y = grouped(x, w, bias, offsets, false, with_gelu ? GELU_AND_Z : PLAIN, z, Tensor());
+    ctx->save_for_backward({x, w, offsets, z});
+    ctx->saved_data["bias"] = bias.defined();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor x = as_saved(saved[0]), w = as_saved(saved[1]), offsets = as_saved(saved[2]), z = as_saved(saved[3]);
+    Tensor dy = packed(grads[0]), dx, dw, db;
+    if (z.defined() && dy.numel()) {
+      Tensor dz = at::empty_like(dy);
+      check(tmpi_gelu_bwd(dy.data_ptr(), z.data_ptr(), dz.data_ptr(), (size_t)dy.numel(), dtype_code(dy.scalar_type()), stream()));
+      launched(EXPERTS, 1);
+      dy = dz;
+    }
+    const bool need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+    if (ctx->needs_input_grad(0)) dx = grouped(dy, w, Tensor(), offsets, true, PLAIN, Tensor(), Tensor());
+    if (ctx->needs_input_grad(1) || need_b) grouped_weight_gradient(dy, x, offsets, Tensor(), w.size(0), &dw, need_b ? &db : nullptr);
+    if (!ctx->needs_input_grad(1)) dw = Tensor();
+    return {dx, dw, db, Tensor(), Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------- an MLP with 8-bit checkpoints
+struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w1_, const OptTensor& b1_, const Tensor& w2_, const OptTensor& b2_) {
+    const Tensor x = packed(x_), w1 = packed(w1_), w2 = packed(w2_), b1 = b1_.has_value() ? packed(*b1_) : Tensor(), b2 = b2_.has_value() ? packed(*b2_) : Tensor();
+    const Kept kx = quantize(x), kz = empty_kept(x, x.size(0), w1.size(0));
+    const Tensor h = grouped(x, w1, b1, Tensor(), false, GELU_AND_Z8, kz.q, kz.scale);
+    const Tensor y = matmul_nt(h, w2, b2);
+    ctx->save_for_backward({kx.q, kx.scale, kz.q, kz.scale, w1, w2});
+    ctx->saved_data["b1"] = b1.defined();
+    ctx->saved_data["b2"] = b2.defined();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Kept kx{as_saved(saved[0]), as_saved(saved[1])}, kz{as_saved(saved[2]), as_saved(saved[3])};
+    const Tensor w1 = as_saved(saved[4]), w2 = as_saved(saved[5]), dy = packed(grads[0]);
+    const bool has_b1 = ctx->saved_data["b1"].toBool(), has_b2 = ctx->saved_data["b2"].toBool();         // an absent bias has no number among the inputs
+    const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(1), need_w2 = ctx->needs_input_grad(2 + has_b1);
+    const bool need_b1 = has_b1 && ctx->needs_input_grad(2), need_b2 = has_b2 && ctx->needs_input_grad(3 + has_b1);
+    Tensor dx, dw1, db1, dw2, db2, dh;
+    if (need_x || need_w1 || need_b1 || need_w2) {
+      linear_gradients(dy, kz.q, w2, &dh, nullptr, nullptr);      // kz.q: for its extents alone
+      const auto both = gelu_gradient(dh, kz);
+      const Tensor dz = both.first;
+      if (need_w2) linear_gradients(dy, both.second, w2, nullptr, &dw2, need_b2 ? &db2 : nullptr);
+      if (need_w1) linear_gradients(dz, restore(kx, dz.scalar_type()), w1, need_x ? &dx : nullptr, &dw1, need_b1 ? &db1 : nullptr);
+      else if (need_x) linear_gradients(dz, kx.q, w1, &dx, nullptr, need_b1 ? &db1 : nullptr);
+      else if (need_b1) db1 = dz.sum(0);
+    }
+    if (need_b2 && !db2.defined()) db2 = dy.sum(0);
+    return {dx, dw1, db1, dw2, db2};
+  }
+};
+
+// ---------------------------------------------------------------- routing
+struct RouteFn : public torch::autograd::Function<RouteFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits_, int64_t k, bool renormalize) {
+    const Tensor logits = logits_.stride(1) == 1 && (logits_.size(0) < 2 || logits_.stride(0) >= logits_.size(1)) ? logits_ : logits_.contiguous();
+    const int T = (int)logits.size(0), E = (int)logits.size(1);
+    const auto i32 = logits.options().dtype(at::kInt);
+    Tensor weights = at::empty({T, k}, logits.options().dtype(at::kFloat)), chosen = at::empty({T, k}, i32), order = at::empty({T * k}, i32),
+           place = at::empty({T, k}, i32), offsets = at::empty({E + 1}, i32), ws;
+    const size_t need = tmpi_route_workspace_bytes(T, E, (int)k);
+    if (need) ws = at::empty({(int64_t)need}, logits.options().dtype(at::kByte));
+    check(tmpi_route(logits.data_ptr(), T > 1 ? logits.stride(0) : E, T, E, (int)k, renormalize, dtype_code(logits.scalar_type()), weights.data_ptr<float>(),
+                     chosen.data_ptr<int>(), order.data_ptr<int>(), place.data_ptr<int>(), offsets.data_ptr<int>(), need ? ws.data_ptr() : nullptr, need, stream()));
+    launched(EXPERTS, need ? 2 : 1);
+    ctx->save_for_backward({logits, weights, chosen});
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->mark_non_differentiable({chosen, order, place, offsets});
+    return {weights, chosen, order, place, offsets};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor logits = saved[0].stride(1) == 1 && (saved[0].size(0) < 2 || saved[0].stride(0) >= saved[0].size(1)) ? saved[0] : saved[0].contiguous();
+    const Tensor weights = as_saved(saved[1]), chosen = as_saved(saved[2]), dw = packed(grads[0].to(at::kFloat));
+    const int T = (int)logits.size(0), E = (int)logits.size(1);
+    Tensor dl = at::empty({T, E}, logits.options());
+    check(tmpi_route_gradient(logits.data_ptr(), T > 1 ? logits.stride(0) : E, T, E, (int)ctx->saved_data["k"].toInt(), ctx->saved_data["renormalize"].toBool(),
+                              dtype_code(logits.scalar_type()), weights.data_ptr<float>(), chosen.data_ptr<int>(), dw.data_ptr<float>(), dl.data_ptr(), stream()));
+    launched(EXPERTS, 1);
+    return {dl, Tensor(), Tensor()};
+  }
+};
+
+Tensor dispatch(const Tensor& x, const Tensor& order, int64_t tokens, int64_t k) {
+  Tensor out = at::empty({tokens * k, x.size(1)}, x.options());
+  check(tmpi_expert_dispatch(x.data_ptr(), order.data_ptr<int>(), out.data_ptr(), (int)tokens, (int)k, (int)x.size(1), dtype_code(x.scalar_type()), stream()));
+  launched(EXPERTS, 1);
+  return out;
+}
+Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place) {
+  Tensor y = at::empty({place.size(0), rows.size(1)}, rows.options());
+  check(tmpi_expert_combine(rows.data_ptr(), weights.defined() ? weights.data_ptr<float>() : nullptr, place.data_ptr<int>(), y.data_ptr(), (int)place.size(0),
+                            (int)place.size(1), (int)rows.size(1), dtype_code(rows.scalar_type()), stream()));
+  launched(EXPERTS, 1);
+  return y;
+}
+
+struct DispatchFn : public torch::autograd::Function<DispatchFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& order_, const Tensor& place_) {
+    const Tensor order = order_.contiguous(), place = place_.contiguous();
+    ctx->save_for_backward({place});
+    return dispatch(packed(x), order, place.size(0), place.size(1));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    return {combine(packed(grads[0]), Tensor(), as_saved(saved[0])), Tensor(), Tensor()};
+  }
+};
+
+struct CombineFn : public torch::autograd::Function<CombineFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows_, const Tensor& weights_, const Tensor& order_, const Tensor& place_) {
+    const Tensor rows = packed(rows_), weights = weights_.contiguous(), order = order_.contiguous(), place = place_.contiguous();
+    ctx->save_for_backward({rows, weights, order});
+    return combine(rows, weights, place);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor rows = as_saved(saved[0]), weights = as_saved(saved[1]), order = as_saved(saved[2]), dy = packed(grads[0]);
+    const bool need_w = ctx->needs_input_grad(1);
+    Tensor drows = at::empty_like(rows), dw;
+    if (need_w) dw = at::zeros_like(weights);
+    check(tmpi_expert_combine_gradient(dy.data_ptr(), need_w ? rows.data_ptr() : nullptr, weights.data_ptr<float>(), 1, order.data_ptr<int>(), nullptr,
+                                       drows.data_ptr(), need_w ? dw.data_ptr<float>() : nullptr, nullptr, (int)weights.size(0), (int)weights.size(1),
+                                       (int)rows.size(1), 0, dtype_code(rows.scalar_type()), stream()));
+    launched(EXPERTS, 1);
+    return {drows, dw, Tensor(), Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------- a layer of experts
+// y_t = sum over j of weights_tj (gelu(x_t w1_e^T + b1_e) w2_e^T + b2_e), e = chosen_tj.  Kept for backward: x and the pre-activation,
+// in bf16 or (act8) in 8 bits, and neither the dispatched rows nor what the experts returned: the rows are gathered again, and the weight's gradient
+// dy . (w2 h + b2) is (w2^T dy) . h + dy . b2, of which the first product is there anyway.
+struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weights_, const Tensor& chosen_, const Tensor& order_, const Tensor& place_,
+                        const Tensor& offsets_, const Tensor& w1_, const OptTensor& b1_, const Tensor& w2_, const OptTensor& b2_, bool act8, bool keep) {
+    const Tensor x = packed(x_), weights = weights_.contiguous(), chosen = chosen_.contiguous(), order = order_.contiguous(), place = place_.contiguous(),
+                 offsets = offsets_.contiguous(), w1 = packed(w1_), w2 = packed(w2_), b1 = b1_.has_value() ? packed(*b1_) : Tensor(),
+                 b2 = b2_.has_value() ? packed(*b2_) : Tensor();
+    const int64_t T = place.size(0), k = place.size(1), H = w1.size(1);
+    const Tensor xs = dispatch(x, order, T, k);
+    Kept kx, kz;
+    if (keep && act8) {
+      kx = quantize(x);
+      kz = empty_kept(x, T * k, H);
+    } else if (keep) {
+      kx.q = x;
+      kz.q = at::empty({T * k, H}, x.options());
+    }
+    const Tensor h = grouped(xs, w1, b1, offsets, false, !keep ? GELU : act8 ? GELU_AND_Z8 : GELU_AND_Z, kz.q, kz.scale);
+    const Tensor y = combine(grouped(h, w2, b2, offsets, false, PLAIN, Tensor(), Tensor()), weights, place);
+    if (keep) {
+      ctx->save_for_backward({kx.q, kx.scale, kz.q, kz.scale, weights, chosen, order, place, offsets, w1, w2, b2});
+      ctx->saved_data["b1"] = b1.defined();
+    }
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Kept kx{as_saved(saved[0]), as_saved(saved[1])}, kz{as_saved(saved[2]), as_saved(saved[3])};
+    const Tensor weights = as_saved(saved[4]), chosen = as_saved(saved[5]), order = as_saved(saved[6]), place = as_saved(saved[7]), offsets = as_saved(saved[8]),
+                 w1 = as_saved(saved[9]), w2 = as_saved(saved[10]), b2 = as_saved(saved[11]), dy = packed(grads[0]);
+    const int64_t T = place.size(0), k = place.size(1), C = dy.size(1), H = w1.size(1), E = w1.size(0);
+    const bool has_b1 = ctx->saved_data["b1"].toBool();                 // an absent bias has no number among the inputs
+    const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(6), need_b1 = has_b1 && ctx->needs_input_grad(7),
+               need_w2 = ctx->needs_input_grad(7 + has_b1), need_b2 = b2.defined() && ctx->needs_input_grad(8 + has_b1);
+    const auto f32 = dy.options().dtype(at::kFloat);
+    Tensor dwt = at::zeros({T, k}, f32), by_place = at::empty({T * k}, f32), g = at::empty({T * k, C}, dy.options());
+    check(tmpi_expert_combine_gradient(dy.data_ptr(), ptr(b2), weights.data_ptr<float>(), 0, order.data_ptr<int>(), b2.defined() ? chosen.data_ptr<int>() : nullptr,
+                                       g.data_ptr(), b2.defined() ? dwt.data_ptr<float>() : nullptr, by_place.data_ptr<float>(), (int)T, (int)k, (int)C, (int)E,
+                                       dtype_code(dy.scalar_type()), stream()));
+    const Tensor dh = grouped(g, w2, Tensor(), offsets, true, PLAIN, Tensor(), Tensor());
+    Tensor dz = at::empty_like(dh), hw = at::empty_like(dh);
+    check(tmpi_expert_gelu_gradient(dh.data_ptr(), kz.q.data_ptr(), kz.scale.defined() ? kz.scale.data_ptr() : nullptr, weights.data_ptr<float>(),
+                                    order.data_ptr<int>(), dz.data_ptr(), hw.data_ptr(), dwt.data_ptr<float>(), (int)T, (int)k, (int)H, stream()));
+    launched(EXPERTS, 2);
+    Tensor dx, dw1, db1, dw2, db2;
+    if (need_w2 || need_b2) grouped_weight_gradient(g, hw, offsets, by_place, E, &dw2, need_b2 ? &db2 : nullptr);
+    if (need_w1 || need_b1) {
+      Tensor xs;
+      if (kx.scale.defined()) {
+        xs = at::empty({T * k, C}, dy.options());
+        check(tmpi_expert_dispatch8(kx.q.data_ptr(), kx.scale.data_ptr(), order.data_ptr<int>(), xs.data_ptr(), (int)T, (int)k, (int)C, stream()));
+        launched(EXPERTS, 1);
+      } else {
+        xs = dispatch(kx.q, order, T, k);
+      }
+      grouped_weight_gradient(dz, xs, offsets, Tensor(), E, &dw1, need_b1 ? &db1 : nullptr);
+    }
+    if (need_x) dx = combine(grouped(dz, w1, Tensor(), offsets, true, PLAIN, Tensor(), Tensor()), Tensor(), place);
+    const Tensor none;
+    return {dx, ctx->needs_input_grad(1) ? dwt : none, none, none, none, none, need_w1 ? dw1 : none, db1, need_w2 ? dw2 : none, db2, none, none};
+  }
+};
+
+}  // namespace
+
+void register_experts(pybind11::module_& m) {
+  m.def("act8_quantize", [](const Tensor& x) {
+    const Kept k = quantize(packed(x));
+    return std::make_pair(k.q, k.scale);
+  });
+  m.def("act8_restore", [](const Tensor& q, const Tensor& scale, int code) {
+    return restore({packed(q), packed(scale)}, code == TMPI_F32 ? at::kFloat : code == TMPI_F16 ? at::kHalf : at::kBFloat16);
+  });
+  m.def("act8_gelu_gradient", [](const Tensor& dy, const Tensor& q, const Tensor& scale) { return gelu_gradient(packed(dy), {packed(q), packed(scale)}); });
+  m.def("act8_mlp", [](const Tensor& x, const Tensor& w1, const OptTensor& b1, const Tensor& w2, const OptTensor& b2) -> Tensor {
+    if (wants_grad({x, w1, w2, or_none(b1), or_none(b2)})) return Mlp8Fn::apply(x, w1, b1, w2, b2);
+    const Tensor h = grouped(packed(x), packed(w1), b1.has_value() ? packed(*b1) : Tensor(), Tensor(), false, GELU, Tensor(), Tensor());
+    return matmul_nt(h, packed(w2), b2.has_value() ? packed(*b2) : Tensor());
+  });
+  m.def("grouped_linear", [](const Tensor& x, const Tensor& w, const OptTensor& bias, const Tensor& offsets, bool gelu) -> Tensor {
+    if (wants_grad({x, w, or_none(bias)})) return GroupedLinearFn::apply(x, w, bias, offsets, gelu);
+    return grouped(packed(x), packed(w), bias.has_value() ? packed(*bias) : Tensor(), offsets.contiguous(), false, gelu ? GELU : PLAIN, Tensor(), Tensor());
+  });
+  m.def("expert_route", [](const Tensor& logits, int64_t k, bool renormalize) {
+    const variable_list r = RouteFn::apply(logits, k, renormalize);
+    return std::make_tuple(r[0], r[1], r[2], r[3], r[4]);
+  });
+  m.def("expert_dispatch", [](const Tensor& x, const Tensor& order, const Tensor& place) { return DispatchFn::apply(x, order, place); });
+  m.def("expert_combine", [](const Tensor& rows, const Tensor& weights, const Tensor& order, const Tensor& place) {
+    return CombineFn::apply(rows, weights, order, place);
+  });
+  m.def("expert_mlp", [](const Tensor& x, const Tensor& weights, const Tensor& chosen, const Tensor& order, const Tensor& place, const Tensor& offsets,
+                         const Tensor& w1, const OptTensor& b1, const Tensor& w2, const OptTensor& b2, bool act8) {
+    return ExpertsFn::apply(x, weights, chosen, order, place, offsets, w1, b1, w2, b2, act8, wants_grad({x, weights, w1, w2, or_none(b1), or_none(b2)}));
+  });
+}
+
+}  // namespace tmpi_bind

@@ -374,6 +374,36 @@ int tmpi_linear_bwd_plan(int rows, int in, int out, int want, int form, size_t* 
 int tmpi_linear_bwd(const void* dy, int64_t ld_dy, const void* x, const void* w, void* dx, void* dw, void* db, int rows, int in, int out, int form,
                     void* workspace, size_t workspace_bytes, void* counters, int ncounters, void* stream);
 
+// ---------------------------------------------------------------- 8-bit activation checkpoints (act8.cu)
+// x [rows, cols] <-> q [rows, cols] e4m3, scale [rows, ceil(cols / 32)]: a power of two 2^(byte - 127) for 32 elements of a row
+int tmpi_act8_quantize(const void* x, void* q, void* scale, int64_t rows, int cols, int dtype, void* stream);
+int tmpi_act8_restore(const void* q, const void* scale, void* x, int64_t rows, int cols, int dtype, void* stream);
+// dz = dy gelu'(z~) and, where h is given, h = gelu(z~) for the checkpoint z~ of z
+int tmpi_act8_gelu_gradient(const void* dy, const void* q, const void* scale, void* dz, void* h, int64_t rows, int cols, int dtype, void* stream);
+
+// ---------------------------------------------------------------- layers of experts (route.cu, experts.cu, grouped.cu)
+// The k largest logits of each token (ties: the lowest index; -inf and NaN never), their weights, and all entries token * k + j in the order of the
+// experts: entry order[s] is at place s, place[entry] = s (-1: not used), the places of expert e from offsets[e] to offsets[e + 1].
+int tmpi_route_limits(int* experts, int* k);
+size_t tmpi_route_workspace_bytes(int tokens, int experts, int k);
+int tmpi_route(const void* logits, int64_t ld, int tokens, int experts, int k, int renormalize, int dtype, float* weights, int* chosen, int* order,
+               int* place, int* offsets, void* workspace, size_t workspace_bytes, void* stream);
+int tmpi_route_gradient(const void* logits, int64_t ld, int tokens, int experts, int k, int renormalize, int dtype, const float* weights, const int* chosen,
+                        const float* dweights, void* dlogits, void* stream);
+int tmpi_expert_dispatch(const void* x, const int* order, void* out, int tokens, int k, int cols, int dtype, void* stream);
+int tmpi_expert_dispatch8(const void* q, const void* scale, const int* order, void* out, int tokens, int k, int cols, void* stream);
+int tmpi_expert_combine(const void* rows, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream);
+int tmpi_expert_combine_gradient(const void* dy, const void* other, const float* weights, int scaled, const int* order, const int* chosen, void* drows,
+                                 float* dweights, float* place_weights, int tokens, int k, int cols, int nexperts, int dtype, void* stream);
+int tmpi_expert_gelu_gradient(const void* dh, const void* z, const void* scale, const float* weights, const int* order, void* dz, void* hw, float* dweights,
+                              int tokens, int k, int cols, void* stream);
+// Products grouped by expert: rows offsets[e] <= r < offsets[e + 1] (on the device) of x belong to expert e
+int tmpi_grouped_max_experts(void);
+int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,
+                      int w_is_kn, int mode, void* stream);
+int tmpi_grouped_weight_gradient(const void* dy, const void* x, const int* offsets, const float* row_weights, void* dw, void* db, int rows, int nexperts, int K,
+                                 int N, void* stream);
+
 // ---------------------------------------------------------------- tracing
 // ring buffer of (op, algo, bytes, microseconds) records per process
 int tmpi_trace_enable(int on);

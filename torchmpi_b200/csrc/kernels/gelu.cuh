@@ -48,4 +48,15 @@ __device__ __forceinline__ void gelu_value2(float z0, float z1, float* y0, float
   unpack2(mul2(z, cdf), *y0, *y1);
 }
 
+// both, from one pass over the normal distribution's parts
+__device__ __forceinline__ void gelu_both2(float z0, float z1, float* y0, float* y1, float* g0, float* g1) {
+  using namespace attn_util;
+  const unsigned long long z = pack2(__float_as_uint(z0), __float_as_uint(z1));
+  const unsigned long long c = pack2(__float_as_uint(0.3989422804014327f), __float_as_uint(0.3989422804014327f));
+  unsigned long long cdf, e;
+  normal_parts2(z, &cdf, &e);
+  unpack2(mul2(z, cdf), *y0, *y1);
+  unpack2(fma2(mul2(z, c), e, cdf), *g0, *g1);
+}
+
 }  // namespace tmpi

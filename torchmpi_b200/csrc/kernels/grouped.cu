@@ -1,0 +1,800 @@
+// Matrix products grouped by expert, on CTA pairs (gemm_pair.cuh): the rows offsets[e] <= r < offsets[e + 1] of x belong to expert e.
+//   y_r = x_r w_e^T + b_e      (w [experts, N, K] as it lies; backward's dx_r = dy_r w_e reads it MN-major)
+//   dw_e = sum of dy_r^T x_r,  db_e = sum of dy_r
+// The offsets are read on the device: nothing is known of the groups on the host, and no call waits for it.
+//
+// Rows products.  A group is cut into tiles of 256 rows x bn columns, counted by every CTA for itself (a prefix sum over the experts in shared memory);
+// the tiles of all groups form one list, dealt to persistent clusters in turn.  A tile's rows may start anywhere: the row coordinate of a TMA
+// load has no alignment rule, and rows beyond the group's end, of other experts, only reach accumulator rows that are not stored.  A CTA
+// whose part of the tile has at most 32 rows loads 32, and none without rows, so that few rows cost little beside the weights.  Whole parts are
+// stored through TMA tiles, others row by row.  The weight is a 3-D tensor: what a box reads beyond the matrix of its expert is zero, not the next
+// expert's, whose infinities would come back as NaN.
+//
+// The weights' gradient has the rows as its K.  The last 64 rows of a group may hold rows of the next one: a warp of each CTA waits
+// for that block's loads and overwrites those rows with zeros in both operands (zero times infinity is not zero) before the MMAs may read it.  db is
+// summed by the epilogue warps under the tile's MMAs, in fp32 and in short chains, as in linear_bwd.cu.  Experts without rows get zeros.
+#include "act8.cuh"
+#include "attn_util.cuh"
+#include "gemm_pair.cuh"
+#include "pdl.cuh"
+#include "../include/tmpi_c_api.h"
+#include "../runtime/common.h"
+#include <algorithm>
+#include <mutex>
+
+namespace tmpi {
+
+int make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows);
+int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows);
+int gemm_sm_count();
+int* gemm_status_word();
+
+namespace grouped {
+
+using namespace gemm2;
+constexpr int MAX_EXPERTS = 256;
+constexpr int FEW = 32;                                 // rows of the smaller box of x
+constexpr int EPI_THREADS = GROUPS * 128;
+constexpr int SLICE = 64, SLICE_BYTES = BM * SLICE * 2;
+
+enum { PLAIN = 0, GELU_ONLY = 1, WITH_GELU = 2, KEEP8 = 3 };
+
+struct Problem {
+  const int* offsets;        // [experts + 1]; null: one expert with all rows
+  int rows, experts, K, N;   // of x; N: columns of the result
+  int bn, tiles_n, k_blocks;
+  const __nv_bfloat16* bias; // [experts, N] or null
+  __nv_bfloat16* y;          // [rows, N]
+  __nv_bfloat16* z;          // WITH_GELU: the pre-activation
+  uint8_t *q, *scale;        // KEEP8: its 8-bit checkpoint
+  int* status;
+};
+
+struct Sh {
+  Shared s;
+  int warp_sums[8];
+  int tile_end[MAX_EXPERTS];                            // tiles of the experts up to and with this one
+};
+constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + gemm::EPI_STAGING_BYTES + 1024 + 1280;
+static_assert(sizeof(Sh) <= 1280 && SMEM <= 232448, "shared memory of one CTA");
+
+// Offsets as given, but inside the tensor and not before the group's start: wrong ones give wrong results, never an access outside.
+struct Group { int r0, r1; };
+__device__ __forceinline__ Group group_of(const int* __restrict__ offsets, int rows, int e) {
+  if (!offsets) return {0, rows};
+  const int r0 = min(max(__ldg(offsets + e), 0), rows);
+  return {r0, min(max(__ldg(offsets + e + 1), r0), rows)};
+}
+
+struct Unit {
+  int e, n_blk;
+  int row0, end;             // of the pair's tile: first row, end of the group
+  __device__ __forceinline__ int part_rows(uint32_t rank) const { return min(max(end - row0 - (int)rank * BM, 0), BM); }
+};
+
+__device__ __forceinline__ void give_up(Shared* sh, int* status, int where) {
+  atomicExch(&sh->error, where);
+  if (status) atomicCAS(status, 0, 1000 + where);
+}
+
+// All threads of the CTA; ends with a barrier.
+__device__ __forceinline__ void count_tiles(Sh* sh, const Problem& p, const int* offsets) {
+  const int e = threadIdx.x, lane = e & 31, warp = e >> 5;
+  int tiles = 0;
+  if (e < p.experts) {
+    const Group g = group_of(offsets, p.rows, e);
+    tiles = (g.r1 - g.r0 + 2 * BM - 1) / (2 * BM) * p.tiles_n;
+  }
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int v = __shfl_up_sync(~0u, tiles, d);
+    if (lane >= d) tiles += v;
+  }
+  if (lane == 31 && warp < 8) sh->warp_sums[warp] = tiles;
+  __syncthreads();
+  if (e < p.experts) {
+    for (int w = 0; w < warp; ++w) tiles += sh->warp_sums[w];
+    sh->tile_end[e] = tiles;
+  }
+  __syncthreads();
+}
+
+// f(unit, number in this cluster's list) for each tile of this cluster until it returns false
+template <typename F>
+__device__ __forceinline__ void for_tiles(const Sh* sh, const Problem& p, const int* offsets, F f) {
+  const int total = sh->tile_end[p.experts - 1], step = (int)(gridDim.x >> 1);
+  int e = 0, it = 0;
+  for (int t = (int)(blockIdx.x >> 1); t < total; t += step, ++it) {
+    if (sh->tile_end[e] <= t) {                          // the first expert that ends behind t, which is behind e
+      int hi = p.experts - 1;
+      ++e;
+      while (e < hi) {
+        const int mid = (e + hi) >> 1;
+        if (sh->tile_end[mid] > t) hi = mid;
+        else e = mid + 1;
+      }
+    }
+    const int begin = e ? sh->tile_end[e - 1] : 0;
+    const Group g = group_of(offsets, p.rows, e);
+    Unit u;
+    int m_tile;
+    band_order(t - begin, (sh->tile_end[e] - begin) / p.tiles_n, p.tiles_n, &m_tile, &u.n_blk);
+    u.e = e;
+    u.row0 = g.r0 + m_tile * 2 * BM;
+    u.end = g.r1;
+    if (!f(u, it)) return;
+  }
+}
+
+// bytes of x that a part with this many rows loads for one K block
+__device__ __forceinline__ uint32_t a_bytes(int rows) { return rows > FEW ? A_BYTES : rows > 0 ? FEW * BK * 2 : 0; }
+
+struct Ring { int stage; uint32_t phase; };
+template <int NST>
+__device__ __forceinline__ void advance(Ring* r) { if (++r->stage == NST) { r->stage = 0; r->phase ^= 1; } }
+
+// One thread in each CTA.
+template <int NST, bool B_MN>
+__device__ __forceinline__ void produce(Sh* shl, unsigned char* tiles, const Problem& p, const int* offsets, const CUtensorMap* ma, const CUtensorMap* ma_few,
+                                        const CUtensorMap* mb, uint32_t rank) {
+  Shared* sh = &shl->s;
+  const int half = p.bn / 2;
+  const bool two = half > 64;
+  const uint32_t b_tx = 2 * (B_MN ? (two ? B_BYTES : B_BYTES / 2) : half * BK * 2);
+  Ring ring{0, 0};
+  for_tiles(shl, p, offsets, [&](const Unit& u, int) -> bool {
+    const int mine = u.part_rows(rank), a_row0 = u.row0 + (int)rank * BM, n0 = u.n_blk * p.bn + (int)rank * half;
+    const uint32_t tx = b_tx + a_bytes(u.part_rows(0)) + a_bytes(u.part_rows(1));
+    for (int kb = 0; kb < p.k_blocks; ++kb) {
+      const int stage = ring.stage;
+      if (!sm100::mbar_wait(&sh->empty[stage], ring.phase ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 31); return false; }
+      unsigned char* dst = tiles + (size_t)stage * STAGE_BYTES;
+      const uint32_t full0 = sm100::map_to_cta(&sh->full[stage], 0);
+      if (rank == 0) sm100::mbar_expect_tx(&sh->full[stage], tx);              // both CTAs' bytes
+      if (mine > 0) sm100::tma_load_2d_pair(dst, mine > FEW ? ma : ma_few, kb * BK, a_row0, full0);
+      if (!B_MN) {
+        sm100::tma_load_3d_pair(dst + A_BYTES, mb, kb * BK, n0, u.e, full0);
+      } else {
+        sm100::tma_load_3d_pair(dst + A_BYTES, mb, n0, kb * BK, u.e, full0);
+        if (two) sm100::tma_load_3d_pair(dst + A_BYTES + B_BYTES / 2, mb, n0 + 64, kb * BK, u.e, full0);
+      }
+      advance<NST>(&ring);
+    }
+    return true;
+  });
+}
+
+// One thread of the even CTA.
+template <int NST, bool B_MN>
+__device__ __forceinline__ void issue(Sh* shl, unsigned char* tiles, const Problem& p, const int* offsets) {
+  Shared* sh = &shl->s;
+  const uint32_t idesc = sm100::make_idesc_f16(2 * BM, p.bn, true, B_MN, false);
+  Ring ring{0, 0};
+  for_tiles(shl, p, offsets, [&](const Unit&, int it) -> bool {
+    const int acc = it & 1;
+    if (!sm100::mbar_wait(&sh->acc_empty[acc], ((it >> 1) & 1) ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 32); return false; }
+    sm100::tc_fence_after();
+    const uint32_t d = sh->tmem_base + (uint32_t)acc * BN;
+    for (int kb = 0; kb < p.k_blocks; ++kb) {
+      const int stage = ring.stage;
+      if (!sm100::mbar_wait(&sh->full[stage], ring.phase, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 33); return false; }
+      sm100::tc_fence_after();
+      const uint32_t a = sm100::smem_u32(tiles + (size_t)stage * STAGE_BYTES), b = a + A_BYTES;
+#pragma unroll
+      for (int k = 0; k < BK / UMMA_K; ++k) {
+        const uint64_t da = sm100::make_desc_sw128(a + k * UMMA_K * 2);
+        const uint64_t db = B_MN ? sm100::make_desc_sw128_mn(b + k * UMMA_K * 128, B_BYTES / 2, 1024) : sm100::make_desc_sw128(b + k * UMMA_K * 2);
+        sm100::umma_f16_pair(d, da, db, idesc, (uint32_t)kb | (uint32_t)k);
+      }
+      sm100::umma_commit_pair(sm100::map_to_cta(&sh->empty[stage], 0));
+      sm100::umma_commit_pair(sm100::map_to_cta(&sh->empty[stage], 1));
+      advance<NST>(&ring);
+    }
+    sm100::umma_commit_pair(sm100::map_to_cta(&sh->acc_full[acc], 0));
+    sm100::umma_commit_pair(sm100::map_to_cta(&sh->acc_full[acc], 1));
+    return true;
+  });
+}
+
+// Whether the wait succeeded for all `threads` threads that share the named barrier: they go on, or leave, together.
+template <int THREADS_>
+__device__ __forceinline__ bool all_of(uint32_t ok, int barrier) {
+  uint32_t all;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(all) : "r"(ok), "r"(barrier), "n"(THREADS_) : "memory");
+  return all != 0;
+}
+
+// 64 columns of a row as bf16
+__device__ __forceinline__ void to_bf16(const uint32_t (&r)[2][32], uint32_t (&w)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) w[j] = attn_util::pack_bf16(r[j >> 4][2 * (j & 15)], r[j >> 4][2 * (j & 15) + 1]);
+}
+__device__ __forceinline__ void stage_row(unsigned char* stg_row, int row, const uint32_t (&w)[32]) {
+#pragma unroll
+  for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(stg_row + ((u ^ (row & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+}
+
+// The eight epilogue warps of each CTA: two groups of four take the 64-column slices of a tile in turn, as in gemm_pair.cuh.  The GELU is that of
+// the fp32 sum.  KEEP8: a thread has whole blocks of 32 columns of its row, so the checkpoint of the fp32 sum takes no exchange between threads.
+template <int MODE>
+__device__ __forceinline__ void finish(Sh* shl, unsigned char* staging, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const CUtensorMap* map_y,
+                                       const CUtensorMap* map_z, uint32_t rank, int group, int quarter, int lane) {
+  Shared* sh = &shl->s;
+  constexpr bool TWO = MODE == WITH_GELU;
+  const int row = quarter * 32 + lane, N = p.N, bn = p.bn;
+  const bool leader = quarter == 0 && lane == 0;
+  unsigned char* stg0 = staging + group * SLICE_BYTES;
+  for_tiles(shl, p, offsets, [&](const Unit& u, int it) -> bool {
+    const int acc = it & 1, rows = u.part_rows(rank);
+    const long long row_at = (long long)u.row0 + (int)rank * BM + row;
+    const __nv_bfloat16* bias = bias_all ? bias_all + (long long)u.e * N : nullptr;
+    const uint32_t ok = sm100::mbar_wait(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs) && !sh->error;
+    if (!all_of<128>(ok, 1 + group)) { give_up(sh, p.status, 34); return false; }
+    sm100::tc_fence_after();
+    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * BN;
+    if (rows > 0) {
+#pragma unroll 1
+      for (int c0 = group * SLICE; c0 < bn; c0 += GROUPS * SLICE) {
+        const int col0 = u.n_blk * bn + c0;
+        if (col0 >= N) break;
+        uint32_t r[2][32], w[32];
+        sm100::tmem_ld_32x32(t_base + c0, r[0]);
+        sm100::tmem_ld_32x32(t_base + c0 + 32, r[1]);
+        sm100::tmem_ld_wait();
+        if (bias) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {                  // N is a multiple of 8
+            if (col0 + 8 * j >= N) break;
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(bias + col0) + j);
+            const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t* x = &r[j >> 2][(j & 3) * 8 + 2 * q];
+              x[0] = __float_as_uint(__uint_as_float(x[0]) + __uint_as_float(b[q] << 16));
+              x[1] = __float_as_uint(__uint_as_float(x[1]) + __uint_as_float(b[q] & 0xffff0000u));
+            }
+          }
+        }
+        auto put = [&](const CUtensorMap* map, __nv_bfloat16* to, int which) {
+          if (rows == BM) {
+            unsigned char* stg = stg0 + which * GROUPS * SLICE_BYTES;
+            if (leader) {                                // the store that used this staging tile before must have read it
+              if (TWO) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+              else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+            group_sync(group);
+            stage_row(stg + row * 128, row, w);
+            sm100::fence_proxy_async_smem();
+            group_sync(group);
+            if (leader) {
+              sm100::tma_store_2d(map, stg, col0, u.row0 + (int)rank * BM);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else if (row < rows) {
+            uint4* at = reinterpret_cast<uint4*>(to + row_at * N + col0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col0 + 8 * j < N) at[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+          }
+        };
+        if (TWO) {
+          to_bf16(r, w);
+          put(map_z, p.z, 1);
+        }
+        if (MODE == KEEP8) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int col = col0 + 32 * h;
+            uint32_t a = 0;                              // columns behind N: zeros (the weight's rows there read as zero, and have no bias)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a = max(a, act8::magnitude(__uint_as_float(r[h][j])));
+            const uint32_t byte = act8::scale_byte(a);
+            const float inv = act8::inverse(byte);
+            if (row < rows && col < N) {
+              p.scale[row_at * ((N + 31) / 32) + col / 32] = (uint8_t)byte;
+              uint2* at = reinterpret_cast<uint2*>(p.q + row_at * N + col);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[h][8 * j + i]);
+                if (col + 8 * j < N) at[j] = act8::pack8(x, inv);
+              }
+            }
+          }
+        }
+        if (MODE != PLAIN) {
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            float y0, y1;
+            uint32_t* x = &r[j >> 5][j & 31];
+            gelu_value2(__uint_as_float(x[0]), __uint_as_float(x[1]), &y0, &y1);
+            x[0] = __float_as_uint(y0);
+            x[1] = __float_as_uint(y1);
+          }
+        }
+        to_bf16(r, w);
+        put(map_y, p.y, 0);
+      }
+    }
+    sm100::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&sh->acc_empty[acc], 0));
+    return true;
+  });
+  // rows behind the last group
+  const long long used = group_of(offsets, p.rows, p.experts - 1).r1;
+  const long long chunks = (p.rows - used) * (N / 8);
+  uint4* rest = reinterpret_cast<uint4*>(p.y + used * N);
+  for (long long i = (long long)blockIdx.x * EPI_THREADS + (threadIdx.x - 64); i < chunks; i += (long long)gridDim.x * EPI_THREADS) rest[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
+template <int MODE, bool B_MN>
+__global__ void __launch_bounds__(GROUP_THREADS, 1)
+grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_few, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z, const __grid_constant__ Problem p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *tiles, *staging;
+  Shared* sh0;
+  constexpr int NST = MODE == WITH_GELU ? STAGES - 1 : STAGES;
+  carve<NST>(smem_raw, &tiles, &sh0, &staging);
+  Sh* sh = reinterpret_cast<Sh*>(sh0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = sm100::cluster_ctarank();
+  setup(sh0, warp, &map_a, &map_b, 4 * GROUPS);
+  const int* offsets = p.offsets;
+  const __nv_bfloat16* bias = p.bias;
+  wait_previous(offsets, bias);
+  count_tiles(sh, p, p.offsets ? offsets : nullptr);
+  if (!p.offsets) offsets = nullptr;
+  if (!p.bias) bias = nullptr;
+  if (warp == 0) {
+    if (sm100::elect_one()) produce<NST, B_MN>(sh, tiles, p, offsets, &map_a, &map_a_few, &map_b, rank);
+  } else if (warp == 1) {
+    if (rank == 0 && sm100::elect_one()) issue<NST, B_MN>(sh, tiles, p, offsets);
+  } else {
+    finish<MODE>(sh, staging, p, offsets, bias, &map_y, &map_z, rank, (warp - 2) >> 2, warp & 3, lane);
+  }
+  __syncwarp();
+  teardown(sh0, warp);
+}
+
+// ---------------------------------------------------------------- the weights' gradient
+struct DwProblem {
+  const int* offsets;
+  int rows, experts, K, N;   // dw [experts, N, K]
+  int bn, tiles_m, tiles_n;  // tiles of 256 rows of N x bn columns of K
+  const __nv_bfloat16* dy;   // [rows, N]
+  const float* row_weights;  // db_e = sum of row_weights[r] dy_r; null: ones
+  __nv_bfloat16* db;         // [experts, N] or null
+  int* status;
+};
+
+constexpr int DW_THREADS = GROUP_THREADS + 32;          // and the warp that clears rows of other groups
+constexpr int DB_GROUPS = EPI_THREADS / (BM / 8);
+
+struct DwSh {
+  Shared s;
+  uint64_t tail[STAGES];                                // a block with rows of another group: its loads, one barrier per CTA
+};
+static_assert(sizeof(DwSh) <= 1280, "barriers");
+
+struct DwUnit { int e, m_blk, n_blk, r0, r1, k_blocks; };
+
+template <typename F>
+__device__ __forceinline__ void for_units(const DwProblem& p, const int* offsets, uint32_t rank, F f) {
+  const int per = p.tiles_m * p.tiles_n, total = p.experts * per, step = (int)(gridDim.x >> 1);
+  for (int t = (int)(blockIdx.x >> 1); t < total; t += step) {
+    DwUnit u;
+    u.e = t / per;
+    int m_tile;
+    band_order(t - u.e * per, p.tiles_m, p.tiles_n, &m_tile, &u.n_blk);
+    u.m_blk = m_tile * 2 + (int)rank;
+    const Group g = group_of(offsets, p.rows, u.e);
+    u.r0 = g.r0;
+    u.r1 = g.r1;
+    u.k_blocks = (g.r1 - g.r0 + BK - 1) / BK;
+    if (!f(u)) return;
+  }
+}
+
+__device__ __forceinline__ void dw_setup(DwSh* sh, int warp, const CUtensorMap* ma, const CUtensorMap* mb) {
+  if (warp == 0 && sm100::elect_one()) {
+    sm100::tma_prefetch_desc(ma);
+    sm100::tma_prefetch_desc(mb);
+    for (int s = 0; s < STAGES; ++s) {
+      sm100::mbar_init(&sh->s.full[s], 2);              // one arrival of each CTA: its producer's, or its clearing warp's
+      sm100::mbar_init(&sh->s.empty[s], 1);
+      sm100::mbar_init(&sh->tail[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) { sm100::mbar_init(&sh->s.acc_full[a], 1); sm100::mbar_init(&sh->s.acc_empty[a], 8 * GROUPS); }
+    sh->s.error = 0;
+    sm100::fence_barrier_init();
+  }
+  if (warp == 1) {
+    sm100::tmem_alloc_pair(&sh->s.tmem_base, TMEM_COLS);
+    sm100::tmem_relinquish_pair();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::cluster_sync();
+  sm100::tc_fence_after();
+}
+
+// One thread in each CTA.
+__device__ __forceinline__ void dw_produce(DwSh* shl, unsigned char* tiles, const DwProblem& p, const int* offsets, const CUtensorMap* ma, const CUtensorMap* mb,
+                                           uint32_t rank) {
+  Shared* sh = &shl->s;
+  const int half = p.bn / 2;
+  const bool two = half > 64;
+  const uint32_t tx = A_BYTES + (two ? B_BYTES : B_BYTES / 2);               // of this CTA
+  Ring ring{0, 0};
+  for_units(p, offsets, rank, [&](const DwUnit& u) -> bool {
+    const int m0 = u.m_blk * BM, n0 = u.n_blk * p.bn + (int)rank * half;
+    for (int kb = 0; kb < u.k_blocks; ++kb) {
+      const int stage = ring.stage, k0 = u.r0 + kb * BK;
+      if (!sm100::mbar_wait(&sh->empty[stage], ring.phase ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 41); return false; }
+      unsigned char* dst = tiles + (size_t)stage * STAGE_BYTES;
+      uint32_t bar = sm100::map_to_cta(&sh->full[stage], 0);
+      if (k0 + BK > u.r1) {
+        bar = sm100::map_to_cta(&shl->tail[stage], rank);
+        sm100::mbar_expect_tx(&shl->tail[stage], tx);
+      } else {
+        sm100::mbar_expect_tx_cluster(bar, tx);
+      }
+      sm100::tma_load_2d_pair(dst, ma, m0, k0, bar);
+      sm100::tma_load_2d_pair(dst + A_BYTES / 2, ma, m0 + 64, k0, bar);
+      sm100::tma_load_2d_pair(dst + A_BYTES, mb, n0, k0, bar);
+      if (two) sm100::tma_load_2d_pair(dst + A_BYTES + B_BYTES / 2, mb, n0 + 64, k0, bar);
+      advance<STAGES>(&ring);
+    }
+    return true;
+  });
+}
+
+// One warp in each CTA: rows of other groups in the last block of a group become zeros.  A row of 64 elements is 128 bytes at row * 128 of its box, which
+// the swizzle permutes within themselves.
+__device__ __forceinline__ void dw_clear(DwSh* shl, unsigned char* tiles, const DwProblem& p, const int* offsets, uint32_t rank, int lane) {
+  Shared* sh = &shl->s;
+  const int boxes = p.bn / 2 > 64 ? 4 : 3;
+  int stage = 0;
+  uint32_t phases = 0;
+  for_units(p, offsets, rank, [&](const DwUnit& u) -> bool {
+    const int rem = (u.r1 - u.r0) % BK;
+    if (rem) {
+      const int at = (stage + u.k_blocks - 1) % STAGES;
+      if (!sm100::mbar_wait_warp(&shl->tail[at], phases >> at & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 45); return false; }
+      phases ^= 1u << at;
+      unsigned char* box = tiles + (size_t)at * STAGE_BYTES;
+      for (int b = 0; b < boxes; ++b)
+        for (int c = rem * 8 + lane; c < BK * 8; c += 32) *reinterpret_cast<uint4*>(box + b * (BK * 128) + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&sh->full[at], 0));
+    }
+    stage = (stage + u.k_blocks) % STAGES;
+    return true;
+  });
+}
+
+// One thread of the even CTA.
+__device__ __forceinline__ void dw_issue(DwSh* shl, unsigned char* tiles, const DwProblem& p, const int* offsets) {
+  Shared* sh = &shl->s;
+  const uint32_t idesc = sm100::make_idesc_f16(2 * BM, p.bn, true, true, true);
+  Ring ring{0, 0};
+  int it = 0;
+  for_units(p, offsets, 0, [&](const DwUnit& u) -> bool {
+    if (!u.k_blocks) return true;
+    const int acc = it & 1;
+    if (!sm100::mbar_wait(&sh->acc_empty[acc], ((it >> 1) & 1) ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 42); return false; }
+    ++it;
+    sm100::tc_fence_after();
+    const uint32_t d = sh->tmem_base + (uint32_t)acc * BN;
+    for (int kb = 0; kb < u.k_blocks; ++kb) {
+      const int stage = ring.stage;
+      if (!sm100::mbar_wait(&sh->full[stage], ring.phase, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 43); return false; }
+      sm100::tc_fence_after();
+      const uint32_t a = sm100::smem_u32(tiles + (size_t)stage * STAGE_BYTES), b = a + A_BYTES;
+#pragma unroll
+      for (int k = 0; k < BK / UMMA_K; ++k) {
+        const uint64_t da = sm100::make_desc_sw128_mn(a + k * UMMA_K * 128, A_BYTES / 2, 1024);
+        const uint64_t db = sm100::make_desc_sw128_mn(b + k * UMMA_K * 128, B_BYTES / 2, 1024);
+        sm100::umma_f16_pair(d, da, db, idesc, (uint32_t)kb | (uint32_t)k);
+      }
+      sm100::umma_commit_pair(sm100::map_to_cta(&sh->empty[stage], 0));
+      sm100::umma_commit_pair(sm100::map_to_cta(&sh->empty[stage], 1));
+      advance<STAGES>(&ring);
+    }
+    sm100::umma_commit_pair(sm100::map_to_cta(&sh->acc_full[acc], 0));
+    sm100::umma_commit_pair(sm100::map_to_cta(&sh->acc_full[acc], 1));
+    return true;
+  });
+}
+
+__device__ __forceinline__ void all_sync() { asm volatile("bar.sync 3, %0;" ::"n"(EPI_THREADS) : "memory"); }
+
+// The sums of 128 columns of dY from col0 over the rows [r0, r1), by all epilogue threads; thread `row` of group 0 has column col0 + row.  Sixteen threads
+// share eight columns, each with 16-byte loads of every 16th row, eight in flight, which are added as a tree; a value passes 3 additions in its batch, one
+// for every 128 rows and 4 among the threads.  part: 8 KB of group 0's staging, which its last store has read.
+template <bool WEIGHTS>
+__device__ __forceinline__ float column_sums(const DwProblem& p, const __nv_bfloat16* dy, const float* weights, float* part, int col0, int r0, int r1, int group, int row) {
+  constexpr int U = 8, STEP = DB_GROUPS;
+  const int e = threadIdx.x - 64, col = col0 + (e % (BM / 8)) * 8, mine = e / (BM / 8);
+  const int end = col < p.N ? r1 : r0;                  // N is a multiple of 8
+  unsigned long long acc[4] = {0ull, 0ull, 0ull, 0ull};                      // two columns each
+  for (long long r = (long long)r0 + mine; r < end; r += U * STEP) {
+    uint4 v[U];
+    float wt[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const bool in = r + i * STEP < end;
+      v[i] = in ? __ldcg(reinterpret_cast<const uint4*>(dy + (r + i * STEP) * p.N + col)) : make_uint4(0u, 0u, 0u, 0u);
+      if (WEIGHTS) wt[i] = in ? __ldg(weights + r + i * STEP) : 0.f;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      unsigned long long t[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const uint32_t b = w == 0 ? v[i].x : w == 1 ? v[i].y : w == 2 ? v[i].z : v[i].w;
+        t[i] = attn_util::pack2(b << 16, b & 0xffff0000u);
+        if (WEIGHTS) t[i] = attn_util::mul2(t[i], attn_util::pack2(__float_as_uint(wt[i]), __float_as_uint(wt[i])));
+      }
+#pragma unroll
+      for (int n = U / 2; n; n /= 2)
+#pragma unroll
+        for (int i = 0; i < n; ++i) t[i] = attn_util::add2(t[i], t[i + n]);
+      acc[w] = attn_util::add2(acc[w], t[0]);
+    }
+  }
+  float s[8];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) attn_util::unpack2(acc[w], s[2 * w], s[2 * w + 1]);
+  if (e == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // thread 0 is group 0's leader only where it issued the stores (see finish)
+  all_sync();                          // and the sums of the unit before have been read
+  float4* to = reinterpret_cast<float4*>(part + e * 8);
+  to[0] = make_float4(s[0], s[1], s[2], s[3]);
+  to[1] = make_float4(s[4], s[5], s[6], s[7]);
+  all_sync();
+  if (group) return 0.f;
+  float t[DB_GROUPS];
+#pragma unroll
+  for (int g = 0; g < DB_GROUPS; ++g) t[g] = part[g * BM + row];
+#pragma unroll
+  for (int n = DB_GROUPS / 2; n; n /= 2)
+#pragma unroll
+    for (int g = 0; g < n; ++g) t[g] += t[g + n];
+  return t[0];
+}
+
+__device__ __forceinline__ void dw_finish(DwSh* shl, unsigned char* staging, const DwProblem& p, const int* offsets, const CUtensorMap* mdw, const __nv_bfloat16* dy,
+                                          const float* row_weights, uint32_t rank, int group, int quarter, int lane) {
+  Shared* sh = &shl->s;
+  const int row = quarter * 32 + lane, bn = p.bn;
+  const bool leader = (int)threadIdx.x - 64 == group * 128;
+  unsigned char* stg = staging + group * SLICE_BYTES;
+  int it = 0;
+  for_units(p, offsets, rank, [&](const DwUnit& u) -> bool {
+    const int row0 = u.m_blk * BM;
+    if (p.db && u.n_blk == 0) {
+      const float sum = row_weights ? column_sums<true>(p, dy, row_weights, reinterpret_cast<float*>(staging), row0, u.r0, u.r1, group, row)
+                                    : column_sums<false>(p, dy, row_weights, reinterpret_cast<float*>(staging), row0, u.r0, u.r1, group, row);
+      if (group == 0 && row0 + row < p.N) p.db[(long long)u.e * p.N + row0 + row] = __float2bfloat16_rn(sum);
+    }
+    const int acc = it & 1;
+    if (u.k_blocks) {
+      const uint32_t ok = sm100::mbar_wait(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs) && !sh->error;
+      if (!all_of<EPI_THREADS>(ok, 3)) { give_up(sh, p.status, 44); return false; }
+      ++it;
+      sm100::tc_fence_after();
+    }
+    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * BN;
+#pragma unroll 1
+    for (int c0 = group * SLICE; c0 < bn && u.n_blk * bn + c0 < p.K; c0 += GROUPS * SLICE) {
+      uint32_t w[32];
+      if (u.k_blocks) {
+        uint32_t r[2][32];
+        sm100::tmem_ld_32x32(t_base + c0, r[0]);
+        sm100::tmem_ld_32x32(t_base + c0 + 32, r[1]);
+        sm100::tmem_ld_wait();
+        to_bf16(r, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) w[j] = 0u;
+      }
+      if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      group_sync(group);
+      stage_row(stg + row * 128, row, w);
+      sm100::fence_proxy_async_smem();
+      group_sync(group);
+      if (leader) {
+        const int col0 = u.n_blk * bn + c0;
+        if (row0 < p.N) sm100::tma_store_3d(mdw, stg, col0, row0, u.e);
+        if (row0 + 64 < p.N) sm100::tma_store_3d(mdw, stg + SLICE_BYTES / 2, col0, row0 + 64, u.e);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    }
+    if (u.k_blocks) {
+      sm100::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&sh->acc_empty[acc], 0));
+    }
+    return true;
+  });
+  if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(DW_THREADS, 1)
+grouped_dw_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dw,
+                  const __grid_constant__ DwProblem p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *tiles, *staging;
+  Shared* sh0;
+  carve(smem_raw, &tiles, &sh0, &staging);
+  DwSh* sh = reinterpret_cast<DwSh*>(sh0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = sm100::cluster_ctarank();
+  dw_setup(sh, warp, &map_dy, &map_x);
+  const int* offsets = p.offsets;
+  const __nv_bfloat16* dy = p.dy;
+  const float* row_weights = p.row_weights;
+  wait_previous(offsets, dy, row_weights);
+  if (!p.offsets) offsets = nullptr;
+  if (!p.row_weights) row_weights = nullptr;
+  if (warp == 0) {
+    if (sm100::elect_one()) dw_produce(sh, tiles, p, offsets, &map_dy, &map_x, rank);
+  } else if (warp == 1) {
+    if (rank == 0 && sm100::elect_one()) dw_issue(sh, tiles, p, offsets);
+  } else if (warp < 2 + 4 * GROUPS) {
+    dw_finish(sh, staging, p, offsets, &map_dw, dy, row_weights, rank, (warp - 2) >> 2, warp & 3, lane);
+  } else {
+    dw_clear(sh, tiles, p, offsets, rank, lane);
+  }
+  __syncwarp();
+  teardown(sh0, warp);
+}
+
+// ---------------------------------------------------------------- host side
+static void allow(const void* kernel) { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM); }
+
+static int max_clusters() {
+  static int n = 0;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    allow((const void*)grouped_kernel<PLAIN, false>);
+    allow((const void*)grouped_kernel<GELU_ONLY, false>);
+    allow((const void*)grouped_kernel<WITH_GELU, false>);
+    allow((const void*)grouped_kernel<KEEP8, false>);
+    allow((const void*)grouped_kernel<PLAIN, true>);
+    allow((const void*)grouped_dw_kernel);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(2 * (gemm_sm_count() / 2)); cfg.blockDim = dim3(DW_THREADS);
+    cfg.dynamicSmemBytes = SMEM; cfg.attrs = at; cfg.numAttrs = 1;
+    int c = 0;
+    if (cudaOccupancyMaxActiveClusters(&c, (void*)grouped_dw_kernel, &cfg) == cudaSuccess && c > 0) n = c;
+    else { cudaGetLastError(); n = gemm_sm_count() / 2; }
+  });
+  return n;
+}
+
+// Columns of a tile, for `tiles_m` tiles of rows: whichever takes less time in whole rounds (gemm_pair.cu has the reasons and the costs).
+static int tile_columns(long long tiles_m, int N, int clusters) {
+  auto cost = [&](int bn, int cycles) { return (tiles_m * ((N + bn - 1) / bn) + clusters - 1) / clusters * cycles; };
+  const long long c256 = cost(256, 512), c192 = cost(192, 448), c128 = cost(128, 384);
+  if (100 * c128 < 95 * std::min(c256, c192)) return 128;
+  return 100 * c192 < 95 * c256 ? 192 : 256;
+}
+
+static cudaError_t launch(const void* kernel, long long clusters, int threads, void** args, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // see pdl.cuh
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)(2 * clusters)); cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = SMEM; cfg.stream = stream; cfg.attrs = at; cfg.numAttrs = 2;
+  return cudaLaunchKernelExC(&cfg, kernel, args);
+}
+
+static int checked(const int* offsets, int rows, int nexperts, int K, int N, const char* what) {
+  if (rows < 0 || nexperts < 1 || K < 1 || N < 1) return fail(TMPI_ERR_INVALID, "%s: empty problem", what);
+  if (K % 8 || N % 8) return fail(TMPI_ERR_INVALID, "%s: stored rows must be multiples of 16 bytes (TMA)", what);
+  if (nexperts > MAX_EXPERTS || (!offsets && nexperts != 1)) return fail(TMPI_ERR_UNSUPPORTED, "%s: at most %d experts", what, MAX_EXPERTS);
+  // wrong offsets may ask for this many tiles, which are counted in 32 bits
+  if (((long long)rows / (2 * BM) + 1) * nexperts * ((std::max(K, N) + 127) / 128) > 0x7fffffffLL - 2 * BM)
+    return fail(TMPI_ERR_UNSUPPORTED, "%s: %d rows, %d experts of %d x %d", what, rows, nexperts, N, K);
+  return TMPI_OK;
+}
+
+}  // namespace grouped
+}  // namespace tmpi
+
+using namespace tmpi;
+
+extern "C" {
+
+int tmpi_grouped_max_experts(void) { return grouped::MAX_EXPERTS; }
+
+// y [rows, N] = act(x w_e^T + b_e) for x [rows, K] and w [experts, N, K] (w_is_kn: [experts, K, N], without activation), zeros behind the
+// last group; offsets [experts + 1] on the device, or null for one expert.  mode: 0 none; 1 GELU; 2 GELU, and the pre-activation in z; 3 GELU, and
+// the pre-activation's 8-bit checkpoint in z and scale [rows, ceil(N / 32)].  All bf16 but those, on 16-byte boundaries.
+int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,
+                      int w_is_kn, int mode, void* stream) {
+  int st = grouped::checked(offsets, rows, nexperts, K, N, "grouped_gemm");
+  if (st) return st;
+  if (mode < grouped::PLAIN || mode > grouped::KEEP8 || (w_is_kn && mode) || (mode >= grouped::WITH_GELU && !z) || (mode == grouped::KEEP8 && !scale))
+    return fail(TMPI_ERR_INVALID, "grouped_gemm: mode %d", mode);
+  if (!all_aligned16({x, w, bias, y, z})) return fail(TMPI_ERR_INVALID, "grouped_gemm: tensors must be 16-byte aligned");
+  if (!rows) return TMPI_OK;
+  const int clusters = grouped::max_clusters();
+  const long long tiles_m = rows / (2 * gemm2::BM) + std::min(nexperts, rows);        // at most
+  grouped::Problem p{};
+  p.offsets = offsets; p.rows = rows; p.experts = nexperts; p.K = K; p.N = N;
+  p.bn = grouped::tile_columns(tiles_m, N, clusters);
+  p.tiles_n = (N + p.bn - 1) / p.bn;
+  p.k_blocks = (K + gemm2::BK - 1) / gemm2::BK;
+  p.bias = (const __nv_bfloat16*)bias;
+  p.y = (__nv_bfloat16*)y;
+  p.z = mode == grouped::WITH_GELU ? (__nv_bfloat16*)z : nullptr;
+  p.q = mode == grouped::KEEP8 ? (uint8_t*)z : nullptr;
+  p.scale = (uint8_t*)scale;
+  p.status = gemm_status_word();
+  CUtensorMap ma, ma_few, mb, my, mz;
+  if ((st = make_tmap_bf16(&ma, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, gemm2::BM))) return st;
+  if ((st = make_tmap_bf16(&ma_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, grouped::FEW))) return st;
+  if (w_is_kn) st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, gemm2::BK);
+  else st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, p.bn / 2);
+  if (st) return st;
+  if ((st = make_tmap_bf16(&my, y, (uint64_t)rows, (uint64_t)N, (uint64_t)N, gemm2::BM))) return st;
+  mz = my;
+  if (p.z && (st = make_tmap_bf16(&mz, z, (uint64_t)rows, (uint64_t)N, (uint64_t)N, gemm2::BM))) return st;
+  const void* kernel = w_is_kn ? (const void*)grouped::grouped_kernel<grouped::PLAIN, true>
+                       : mode == grouped::PLAIN ? (const void*)grouped::grouped_kernel<grouped::PLAIN, false>
+                       : mode == grouped::GELU_ONLY ? (const void*)grouped::grouped_kernel<grouped::GELU_ONLY, false>
+                       : mode == grouped::WITH_GELU ? (const void*)grouped::grouped_kernel<grouped::WITH_GELU, false>
+                                                    : (const void*)grouped::grouped_kernel<grouped::KEEP8, false>;
+  void* args[] = {&ma, &ma_few, &mb, &my, &mz, &p};
+  const cudaError_t e = grouped::launch(kernel, std::min<long long>(tiles_m * p.tiles_n, clusters), gemm2::GROUP_THREADS, args, (cudaStream_t)stream);
+  return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_gemm launch: %s", cudaGetErrorString(e));
+}
+
+// dw [experts, N, K] = dy_e^T x_e and, where given, db [experts, N] = the column sums of dy_e, each row times row_weights[row] where given
+// (fp32 [rows]); dy [rows, N], x [rows, K], bf16 on 16-byte boundaries.
+int tmpi_grouped_weight_gradient(const void* dy, const void* x, const int* offsets, const float* row_weights, void* dw, void* db, int rows, int nexperts, int K,
+                                 int N, void* stream) {
+  int st = grouped::checked(offsets, rows, nexperts, K, N, "grouped_weight_gradient");
+  if (st) return st;
+  if (!all_aligned16({dy, x, dw})) return fail(TMPI_ERR_INVALID, "grouped_weight_gradient: tensors must be 16-byte aligned");
+  if (!rows) {
+    const size_t n = (size_t)nexperts * N;
+    cudaError_t e = cudaMemsetAsync(dw, 0, 2 * n * K, (cudaStream_t)stream);
+    if (e == cudaSuccess && db) e = cudaMemsetAsync(db, 0, 2 * n, (cudaStream_t)stream);
+    return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_weight_gradient: %s", cudaGetErrorString(e));
+  }
+  const int clusters = grouped::max_clusters();
+  grouped::DwProblem p{};
+  p.offsets = offsets; p.rows = rows; p.experts = nexperts; p.K = K; p.N = N;
+  p.tiles_m = (N + 2 * gemm2::BM - 1) / (2 * gemm2::BM);
+  p.bn = grouped::tile_columns((long long)p.tiles_m * nexperts, K, clusters);
+  p.tiles_n = (K + p.bn - 1) / p.bn;
+  p.dy = (const __nv_bfloat16*)dy;
+  p.row_weights = row_weights;
+  p.db = (__nv_bfloat16*)db;
+  p.status = gemm_status_word();
+  CUtensorMap mdy, mx, mdw;
+  if ((st = make_tmap_bf16(&mdy, dy, (uint64_t)rows, (uint64_t)N, (uint64_t)N, gemm2::BK))) return st;
+  if ((st = make_tmap_bf16(&mx, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, gemm2::BK))) return st;
+  if ((st = make_tmap_bf16_3d(&mdw, dw, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, 64))) return st;
+  void* args[] = {&mdy, &mx, &mdw, &p};
+  const cudaError_t e = grouped::launch((const void*)grouped::grouped_dw_kernel, std::min<long long>((long long)p.tiles_m * p.tiles_n * nexperts, clusters),
+                                        grouped::DW_THREADS, args, (cudaStream_t)stream);
+  return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_weight_gradient launch: %s", cudaGetErrorString(e));
+}
+
+}  // extern "C"

@@ -1,0 +1,371 @@
+// Routing of tokens to experts: the choice of k experts by a token's logits, its weights, the order of all choices by expert, and the
+// weights' gradient.
+//
+// A warp takes a token; a lane holds the logits of experts lane, lane + 32, ... as integers that compare like the values, so that a round of the
+// choice is a maximum over the lane's own, and two warp-wide reductions (largest value, then the lowest index that has it).  The order by expert is a
+// counting sort in two launches: the first counts the choices of a block of tokens per expert, the second adds the counts of the blocks in front and
+// walks the block's choices in their order, one thread per expert, so entries of an expert keep their order and no atomic decides about a place.
+// Both launches are bound by latency (a few dependent passes over little data).  Up to SMALL choices one block does both.
+#include "pdl.cuh"
+#include "vec.cuh"
+#include "../include/tmpi_c_api.h"
+#include "../runtime/common.h"
+#include <algorithm>
+
+namespace tmpi {
+namespace route {
+
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int MAX_EXPERTS = 256, MAX_K = 32;
+constexpr int MAX_BLOCKS = 148;
+constexpr int SMALL = 512;                 // choices that one block counts and places
+constexpr int CHUNK = 4096;                // choices in shared memory at a time
+constexpr uint32_t KEY_NONE = 0x007fffffu; // the key of -inf
+
+struct Problem {
+  const void* logits;
+  long long ld;                            // elements between rows of the logits
+  int tokens, experts, k, renormalize;
+  int per_block;                           // tokens of a block
+  float* weights;                          // [tokens, k]
+  int* chosen;                             // [tokens, k], -1: none
+  int* order;                              // [tokens * k], behind the last entry -1
+  int* place;                              // [tokens, k], -1: none
+  int* offsets;                            // [experts + 1]
+  int* counts;                             // [blocks, experts]
+};
+
+// Larger values have larger keys; -0 is 0 and NaN is -inf.  0 is no key of a value.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t u = __float_as_uint(x != x ? __uint_as_float(0xff800000u) : x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
+  return x;
+}
+
+// One token by one warp: chosen and weights of lane j < k.
+template <typename T, int NREG>
+__device__ __forceinline__ void choose(const Problem& p, const T* logits, int token, int lane, int* chosen, float* weight) {
+  float l[NREG];
+  uint32_t key[NREG];
+  bool nan = false;
+#pragma unroll
+  for (int r = 0; r < NREG; ++r) {
+    const int e = lane + 32 * r;
+    l[r] = e < p.experts ? (float)to_acc<T>(logits[(long long)token * p.ld + e]) : 0.f;
+    key[r] = e < p.experts ? key_of(l[r]) : 0u;
+    nan |= l[r] != l[r];
+  }
+  nan = __any_sync(~0u, nan);
+  int mine = -1;
+  uint32_t my_key = KEY_NONE, top_key = KEY_NONE;
+  for (int j = 0; j < p.k; ++j) {
+    uint32_t best = 0;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int r = 0; r < NREG; ++r)
+      if (key[r] > best) { best = key[r]; at = lane + 32 * r; }
+    const uint32_t m = __reduce_max_sync(~0u, best);
+    if (m <= KEY_NONE) break;                                      // nothing left that may be used
+    if (!j) top_key = m;
+    const int i = (int)__reduce_min_sync(~0u, (unsigned)(best == m ? at : 0x7fffffff));
+    if (lane == j) { mine = i; my_key = m; }
+#pragma unroll
+    for (int r = 0; r < NREG; ++r)
+      if (i == lane + 32 * r) key[r] = 0;
+  }
+  const float top = of_key(top_key);
+  const bool any = top_key > KEY_NONE;
+  const float e_mine = mine >= 0 ? expf(of_key(my_key) - top) : 0.f;
+  float sum = 0.f;
+  if (p.renormalize) {
+    sum = e_mine;
+  } else if (any) {
+#pragma unroll
+    for (int r = 0; r < NREG; ++r)
+      if (lane + 32 * r < p.experts) sum += expf(l[r] - top);
+  }
+  sum = warp_sum(sum);
+  *chosen = mine;
+  *weight = nan ? __uint_as_float(0x7fffffffu) : mine >= 0 ? e_mine / sum : 0.f;
+}
+
+// The tokens of this block: choices and weights to memory, counts per expert to shared memory (cleared by the caller).
+template <typename T, int NREG>
+__device__ __forceinline__ void choose_block(const Problem& p, const T* logits, int* counts) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t0 = (long long)blockIdx.x * p.per_block;
+  const int t1 = (int)min((long long)p.tokens, t0 + p.per_block);
+  for (int t = (int)t0 + warp; t < t1; t += WARPS) {
+    int c;
+    float w;
+    choose<T, NREG>(p, logits, t, lane, &c, &w);
+    if (lane < p.k) {
+      p.chosen[(long long)t * p.k + lane] = c;
+      p.weights[(long long)t * p.k + lane] = w;
+      if (c >= 0) atomicAdd(&counts[c], 1);                        // a count: the order of the additions does not matter
+    }
+  }
+}
+
+struct Place {
+  int start[MAX_EXPERTS];                  // the next place of an expert's entries
+  int warp_sums[WARPS];
+  alignas(16) short list[CHUNK];
+};
+static_assert(MAX_EXPERTS <= THREADS, "an expert per thread");
+
+// before, total: of this thread's expert (threads beyond the experts: 0).  All threads.
+__device__ __forceinline__ void place_block(const Problem& p, Place& s, int before, int total) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int sum = total;                                                 // inclusive prefix over the experts
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int v = __shfl_up_sync(~0u, sum, d);
+    if (lane >= d) sum += v;
+  }
+  if (lane == 31) s.warp_sums[warp] = sum;
+  __syncthreads();
+  int used = 0, front = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) front += s.warp_sums[w];
+    used += s.warp_sums[w];
+  }
+  const int begin = front + sum - total;
+  if (blockIdx.x == 0 && tid < p.experts) {
+    p.offsets[tid] = begin;
+    if (tid == p.experts - 1) p.offsets[p.experts] = used;
+  }
+  int next = begin + before;
+  const long long e0 = (long long)blockIdx.x * p.per_block * p.k, e1 = min((long long)p.tokens * p.k, e0 + (long long)p.per_block * p.k);
+  for (long long c0 = e0; c0 < e1; c0 += CHUNK) {
+    const int n = (int)min((long long)CHUNK, e1 - c0);
+    __syncthreads();                                               // the list before has been read
+    for (int i = tid; i < (n + 7) / 8 * 8; i += THREADS) {
+      const int c = i < n ? p.chosen[c0 + i] : -1;
+      s.list[i] = (short)c;
+      if (i < n && c < 0) p.place[c0 + i] = -1;
+    }
+    __syncthreads();
+    if (tid < p.experts)
+      for (int i = 0; i < n; i += 8) {
+        const uint4 v = *reinterpret_cast<const uint4*>(&s.list[i]);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if ((int)(short)(w[k >> 1] >> (16 * (k & 1))) == tid) {
+            p.place[c0 + i + k] = next;
+            p.order[next++] = (int)(c0 + i + k);
+          }
+      }
+  }
+  for (long long i = used + (long long)blockIdx.x * THREADS + tid; i < (long long)p.tokens * p.k; i += (long long)gridDim.x * THREADS) p.order[i] = -1;
+}
+
+template <typename T, int NREG>
+__global__ void __launch_bounds__(THREADS) choose_kernel(const Problem p) {
+  __shared__ int counts[MAX_EXPERTS];
+  const T* logits = (const T*)p.logits;
+  wait_previous(logits);
+  for (int e = threadIdx.x; e < p.experts; e += THREADS) counts[e] = 0;
+  __syncthreads();
+  choose_block<T, NREG>(p, logits, counts);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.experts; e += THREADS) p.counts[(long long)blockIdx.x * p.experts + e] = counts[e];
+}
+
+__global__ void __launch_bounds__(THREADS) place_kernel(const Problem p) {
+  __shared__ Place s;
+  const int* counts = p.counts;
+  wait_previous(counts);
+  int before = 0, total = 0;
+  if (threadIdx.x < p.experts) {
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+      const int c = __ldcg(&counts[(long long)b * p.experts + threadIdx.x]);
+      if (b < (int)blockIdx.x) before += c;
+      total += c;
+    }
+  }
+  place_block(p, s, before, total);
+}
+
+template <typename T, int NREG>
+__global__ void __launch_bounds__(THREADS) small_kernel(const Problem p) {
+  __shared__ Place s;
+  __shared__ int counts[MAX_EXPERTS];
+  const T* logits = (const T*)p.logits;
+  wait_previous(logits);
+  counts[threadIdx.x] = 0;
+  __syncthreads();
+  choose_block<T, NREG>(p, logits, counts);
+  __syncthreads();                                                 // the choices, which this block has written, are read again
+  place_block(p, s, 0, counts[threadIdx.x]);
+}
+
+// dl of one token: over the chosen, w_j (dw_j - sum w dw); with weights over all experts, the others get -p_e sum w dw.
+template <typename T, int NREG>
+__global__ void __launch_bounds__(THREADS) gradient_kernel(const Problem p, const float* dweights, T* dlogits) {
+  const T* logits = (const T*)p.logits;
+  wait_previous(logits, dweights);
+  const int lane = threadIdx.x & 31;
+  for (long long t = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); t < p.tokens; t += (long long)gridDim.x * WARPS) {
+    int c = -1;
+    float w = 0.f, wd = 0.f;
+    if (lane < p.k) {
+      c = p.chosen[t * p.k + lane];
+      w = p.weights[t * p.k + lane];                               // NaN in a row with a NaN among its logits, whether used or not
+      if (c >= 0) wd = w * dweights[t * p.k + lane];
+    }
+    const float inner = warp_sum(wd);
+    float l[NREG], d[NREG];
+    bool nan = false;
+    float top = __uint_as_float(0xff800000u), sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < NREG; ++r) {
+      const int e = lane + 32 * r;
+      d[r] = 0.f;
+      l[r] = __uint_as_float(0xff800000u);
+      if (!p.renormalize && e < p.experts) {
+        l[r] = (float)to_acc<T>(logits[t * p.ld + e]);
+        nan |= l[r] != l[r];
+        top = fmaxf(top, l[r]);
+      }
+    }
+    if (!p.renormalize) {
+#pragma unroll
+      for (int k = 16; k; k /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
+      nan = __any_sync(~0u, nan);
+      if (top > __uint_as_float(0xff800000u)) {                    // warp-uniform
+#pragma unroll
+        for (int r = 0; r < NREG; ++r) {
+          d[r] = expf(l[r] - top);
+          if (lane + 32 * r < p.experts) sum += d[r];
+        }
+        sum = warp_sum(sum);
+        const float scale = nan ? __uint_as_float(0x7fffffffu) : -inner / sum;
+#pragma unroll
+        for (int r = 0; r < NREG; ++r) d[r] *= scale;
+      } else if (nan) {
+#pragma unroll
+        for (int r = 0; r < NREG; ++r) d[r] = __uint_as_float(0x7fffffffu);
+      }
+    }
+    for (int j = 0; j < p.k; ++j) {
+      const int i = __shfl_sync(~0u, c, j);
+      const float g = __shfl_sync(~0u, p.renormalize ? wd - w * inner : wd, j);
+#pragma unroll
+      for (int r = 0; r < NREG; ++r)
+        if (i == lane + 32 * r) d[r] += g;
+    }
+#pragma unroll
+    for (int r = 0; r < NREG; ++r)
+      if (lane + 32 * r < p.experts) dlogits[t * p.experts + lane + 32 * r] = from_acc<T>((typename AccOf<T>::type)d[r]);
+  }
+}
+
+static int blocks_of(int tokens, int k) {
+  if ((long long)tokens * k <= SMALL) return 1;
+  return (int)std::min<long long>(MAX_BLOCKS, ((long long)tokens + 31) / 32);
+}
+
+// f(template arguments) for the smallest number of registers that holds the experts
+template <typename F>
+static cudaError_t by_experts(int experts, F f) {
+  if (experts <= 32) return f(std::integral_constant<int, 1>());
+  if (experts <= 64) return f(std::integral_constant<int, 2>());
+  if (experts <= 128) return f(std::integral_constant<int, 4>());
+  return f(std::integral_constant<int, 8>());
+}
+
+template <typename T>
+static cudaError_t forward_t(Problem p, cudaStream_t s) {
+  const int blocks = blocks_of(p.tokens, p.k);
+  p.per_block = (p.tokens + blocks - 1) / blocks;
+  return by_experts(p.experts, [&](auto n) {
+    if (blocks == 1) return launch_overlapped(small_kernel<T, decltype(n)::value>, 1, THREADS, 0, s, p);
+    const cudaError_t e = launch_overlapped(choose_kernel<T, decltype(n)::value>, blocks, THREADS, 0, s, p);
+    return e == cudaSuccess ? launch_overlapped(place_kernel, blocks, THREADS, 0, s, p) : e;
+  });
+}
+
+template <typename T>
+static cudaError_t gradient_t(const Problem& p, const float* dweights, void* dlogits, cudaStream_t s) {
+  const int blocks = (int)std::min<long long>(148 * 8, ((long long)p.tokens + WARPS - 1) / WARPS);
+  return by_experts(p.experts, [&](auto n) {
+    return launch_overlapped(gradient_kernel<T, decltype(n)::value>, blocks, THREADS, 0, s, p, dweights, (T*)dlogits);
+  });
+}
+
+static int checked(int tokens, int experts, int k, int64_t ld, const char* what) {
+  if (tokens < 0 || experts < 1 || k < 1 || k > experts || ld < experts) return fail(TMPI_ERR_INVALID, "%s: %d of %d experts for %d tokens", what, k, experts, tokens);
+  if (experts > MAX_EXPERTS || k > MAX_K) return fail(TMPI_ERR_UNSUPPORTED, "%s: at most %d experts, %d for a token", what, MAX_EXPERTS, MAX_K);
+  if ((long long)tokens * k > 1LL << 30) return fail(TMPI_ERR_UNSUPPORTED, "%s: %d tokens of %d experts", what, tokens, k);
+  return TMPI_OK;
+}
+
+}  // namespace route
+}  // namespace tmpi
+
+using namespace tmpi;
+
+extern "C" {
+
+int tmpi_route_limits(int* experts, int* k) {
+  *experts = route::MAX_EXPERTS;
+  *k = route::MAX_K;
+  return TMPI_OK;
+}
+
+// ints of workspace
+size_t tmpi_route_workspace_bytes(int tokens, int experts, int k) {
+  const int blocks = route::blocks_of(tokens, k);
+  return blocks > 1 ? sizeof(int) * (size_t)blocks * experts : 0;
+}
+
+// logits [tokens, experts] of `dtype`, rows ld elements apart -> weights, chosen, place [tokens, k], order [tokens * k], offsets [experts + 1]
+int tmpi_route(const void* logits, int64_t ld, int tokens, int experts, int k, int renormalize, int dtype, float* weights, int* chosen, int* order,
+               int* place, int* offsets, void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = route::checked(tokens, experts, k, ld, "route");
+  if (st) return st;
+  if (workspace_bytes < tmpi_route_workspace_bytes(tokens, experts, k)) return fail(TMPI_ERR_INVALID, "route: workspace too small");
+  route::Problem p{};
+  p.logits = logits; p.ld = ld; p.tokens = tokens; p.experts = experts; p.k = k; p.renormalize = renormalize;
+  p.weights = weights; p.chosen = chosen; p.order = order; p.place = place; p.offsets = offsets; p.counts = (int*)workspace;
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e;
+  switch (dtype) {
+    case TMPI_BF16: e = route::forward_t<__nv_bfloat16>(p, s); break;
+    case TMPI_F16: e = route::forward_t<__half>(p, s); break;
+    case TMPI_F32: e = route::forward_t<float>(p, s); break;
+    default: return fail(TMPI_ERR_UNSUPPORTED, "route: dtype %d", dtype);
+  }
+  return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "route launch: %s", cudaGetErrorString(e));
+}
+
+// dlogits [tokens, experts] of `dtype`, dense, from dweights [tokens, k] and what the forward gave
+int tmpi_route_gradient(const void* logits, int64_t ld, int tokens, int experts, int k, int renormalize, int dtype, const float* weights, const int* chosen,
+                        const float* dweights, void* dlogits, void* stream) {
+  const int st = route::checked(tokens, experts, k, ld, "route_gradient");
+  if (st || !tokens) return st;
+  route::Problem p{};
+  p.logits = logits; p.ld = ld; p.tokens = tokens; p.experts = experts; p.k = k; p.renormalize = renormalize;
+  p.weights = const_cast<float*>(weights); p.chosen = const_cast<int*>(chosen);
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e;
+  switch (dtype) {
+    case TMPI_BF16: e = route::gradient_t<__nv_bfloat16>(p, dweights, dlogits, s); break;
+    case TMPI_F16: e = route::gradient_t<__half>(p, dweights, dlogits, s); break;
+    case TMPI_F32: e = route::gradient_t<float>(p, dweights, dlogits, s); break;
+    default: return fail(TMPI_ERR_UNSUPPORTED, "route_gradient: dtype %d", dtype);
+  }
+  return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "route_gradient launch: %s", cudaGetErrorString(e));
+}
+
+}  // extern "C"
