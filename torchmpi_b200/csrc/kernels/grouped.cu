@@ -11,7 +11,8 @@
 // expert's, whose infinities would come back as NaN.
 //
 // The weights' gradient has the rows as its K.  The last 64 rows of a group may hold rows of the next one: a warp of each CTA waits
-// for that block's loads and overwrites those rows with zeros in both operands (zero times infinity is not zero) before the MMAs may read it.  db is
+// for that block's loads and overwrites those rows with zeros in both operands (zero times infinity is not zero); the even CTA's, once both are done,
+// lets the MMAs read the block.  db is
 // summed by the epilogue warps under the tile's MMAs, in fp32 and in short chains, as in linear_bwd.cu.  Experts without rows get zeros.
 #include "act8.cuh"
 #include "attn_util.cuh"
@@ -378,6 +379,7 @@ constexpr int DB_GROUPS = EPI_THREADS / (BM / 8);
 struct DwSh {
   Shared s;
   uint64_t tail[STAGES];                                // a block with rows of another group: its loads, one barrier per CTA
+  uint64_t cleared[STAGES];                             // in the even CTA: the odd one's part of such a block is cleared
 };
 static_assert(sizeof(DwSh) <= 1280, "barriers");
 
@@ -405,9 +407,10 @@ __device__ __forceinline__ void dw_setup(DwSh* sh, int warp, const CUtensorMap* 
     sm100::tma_prefetch_desc(ma);
     sm100::tma_prefetch_desc(mb);
     for (int s = 0; s < STAGES; ++s) {
-      sm100::mbar_init(&sh->s.full[s], 2);              // one arrival of each CTA: its producer's, or its clearing warp's
+      sm100::mbar_init(&sh->s.full[s], 1);
       sm100::mbar_init(&sh->s.empty[s], 1);
       sm100::mbar_init(&sh->tail[s], 1);
+      sm100::mbar_init(&sh->cleared[s], 1);
     }
     for (int a = 0; a < 2; ++a) { sm100::mbar_init(&sh->s.acc_full[a], 1); sm100::mbar_init(&sh->s.acc_empty[a], 8 * GROUPS); }
     sh->s.error = 0;
@@ -438,11 +441,11 @@ __device__ __forceinline__ void dw_produce(DwSh* shl, unsigned char* tiles, cons
       if (!sm100::mbar_wait(&sh->empty[stage], ring.phase ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 41); return false; }
       unsigned char* dst = tiles + (size_t)stage * STAGE_BYTES;
       uint32_t bar = sm100::map_to_cta(&sh->full[stage], 0);
-      if (k0 + BK > u.r1) {
+      if (k0 + BK > u.r1) {                             // the clearing warp arrives at full
         bar = sm100::map_to_cta(&shl->tail[stage], rank);
         sm100::mbar_expect_tx(&shl->tail[stage], tx);
-      } else {
-        sm100::mbar_expect_tx_cluster(bar, tx);
+      } else if (rank == 0) {
+        sm100::mbar_expect_tx(&sh->full[stage], 2 * tx);                       // both CTAs' bytes
       }
       sm100::tma_load_2d_pair(dst, ma, m0, k0, bar);
       sm100::tma_load_2d_pair(dst + A_BYTES / 2, ma, m0 + 64, k0, bar);
@@ -465,14 +468,20 @@ __device__ __forceinline__ void dw_clear(DwSh* shl, unsigned char* tiles, const 
     const int rem = (u.r1 - u.r0) % BK;
     if (rem) {
       const int at = (stage + u.k_blocks - 1) % STAGES;
-      if (!sm100::mbar_wait_warp(&shl->tail[at], phases >> at & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 45); return false; }
+      const uint32_t phase = phases >> at & 1;
+      if (!sm100::mbar_wait_warp(&shl->tail[at], phase, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 45); return false; }
       phases ^= 1u << at;
       unsigned char* box = tiles + (size_t)at * STAGE_BYTES;
       for (int b = 0; b < boxes; ++b)
         for (int c = rem * 8 + lane; c < BK * 8; c += 32) *reinterpret_cast<uint4*>(box + b * (BK * 128) + c * 16) = make_uint4(0u, 0u, 0u, 0u);
       sm100::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&sh->full[at], 0));
+      if (rank) {
+        if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&shl->cleared[at], 0));
+      } else {
+        if (!sm100::mbar_wait_warp(&shl->cleared[at], phase, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 46); return false; }
+        if (lane == 0) sm100::mbar_arrive(&sh->full[at]);
+      }
     }
     stage = (stage + u.k_blocks) % STAGES;
     return true;
