@@ -6,7 +6,7 @@
 namespace tmpi_bind {
 namespace {
 
-enum { PLAIN = 0, GELU = 1, GELU_AND_Z = 2, GELU_AND_Z8 = 3 };      // tmpi_grouped_gemm's modes
+enum { PLAIN = 0, GELU = 1, GELU_AND_Z = 2, GELU_AND_Z8 = 3, FP32 = 4 };      // tmpi_grouped_gemm's modes
 
 using OptTensor = c10::optional<Tensor>;
 Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
@@ -50,11 +50,21 @@ std::pair<Tensor, Tensor> gelu_gradient(const Tensor& dy, const Kept& k) {
 Tensor grouped(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& offsets, bool w_is_kn, int mode, const Tensor& z, const Tensor& scale) {
   const int experts = offsets.defined() ? (int)w.size(0) : 1, d = (int)w.dim();
   const int N = (int)w.size(w_is_kn ? d - 1 : d - 2), K = (int)x.size(1);
-  Tensor y = at::empty({x.size(0), N}, x.options());
+  Tensor y = at::empty({x.size(0), N}, mode == FP32 ? x.options().dtype(at::kFloat) : x.options());
   check(tmpi_grouped_gemm(x.data_ptr(), w.data_ptr(), ptr(bias), ints(offsets), y.data_ptr(), z.defined() ? z.data_ptr() : nullptr,
                           scale.defined() ? scale.data_ptr() : nullptr, (int)x.size(0), experts, K, N, w_is_kn ? 1 : 0, mode, stream()));
   launched(EXPERTS, 1);
   return y;
+}
+// (dz, h) of tmpi_grouped_gelu_gradient; dots: an empty tensor of its sums, or undefined
+std::pair<Tensor, Tensor> grouped_gelu_gradient(const Tensor& dy, const Tensor& w, const Tensor& offsets, const Kept& z, const Tensor& row_weights, const Tensor& dots) {
+  const int experts = offsets.defined() ? (int)w.size(0) : 1, N = (int)w.size(-1);
+  Tensor dz = at::empty({dy.size(0), N}, dy.options()), h = at::empty_like(dz);
+  check(tmpi_grouped_gelu_gradient(dy.data_ptr(), w.data_ptr(), ints(offsets), z.q.data_ptr(), z.scale.defined() ? z.scale.data_ptr() : nullptr,
+                                   row_weights.defined() ? row_weights.data_ptr<float>() : nullptr, dz.data_ptr(), h.data_ptr(),
+                                   dots.defined() ? dots.data_ptr<float>() : nullptr, (int)dy.size(0), experts, (int)dy.size(1), N, stream()));
+  launched(EXPERTS, 1);
+  return {dz, h};
 }
 // dw and, where asked for, db
 void grouped_weight_gradient(const Tensor& dy, const Tensor& x, const Tensor& offsets, const Tensor& row_weights, int64_t experts, Tensor* dw, Tensor* db) {
@@ -112,14 +122,13 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
     const bool has_b1 = ctx->saved_data["b1"].toBool(), has_b2 = ctx->saved_data["b2"].toBool();         // an absent bias has no number among the inputs
     const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(1), need_w2 = ctx->needs_input_grad(2 + has_b1);
     const bool need_b1 = has_b1 && ctx->needs_input_grad(2), need_b2 = has_b2 && ctx->needs_input_grad(3 + has_b1);
-    Tensor dx, dw1, db1, dw2, db2, dh;
+    Tensor dx, dw1, db1, dw2, db2;
     if (need_x || need_w1 || need_b1 || need_w2) {
-      linear_gradients(dy, kz.q, w2, &dh, nullptr, nullptr);      // kz.q: for its extents alone
-      const auto both = gelu_gradient(dh, kz);
+      const auto both = grouped_gelu_gradient(dy, w2, Tensor(), kz, Tensor(), Tensor());
       const Tensor dz = both.first;
       if (need_w2) linear_gradients(dy, both.second, w2, nullptr, &dw2, need_b2 ? &db2 : nullptr);
       if (need_w1) linear_gradients(dz, restore(kx, dz.scalar_type()), w1, need_x ? &dx : nullptr, &dw1, need_b1 ? &db1 : nullptr);
-      else if (need_x) linear_gradients(dz, kx.q, w1, &dx, nullptr, need_b1 ? &db1 : nullptr);
+      else if (need_x) linear_gradients(dz, kx.q, w1, &dx, nullptr, need_b1 ? &db1 : nullptr);      // kx.q: for its extents alone
       else if (need_b1) db1 = dz.sum(0);
     }
     if (need_b2 && !db2.defined()) db2 = dy.sum(0);
@@ -165,10 +174,12 @@ Tensor dispatch(const Tensor& x, const Tensor& order, int64_t tokens, int64_t k)
   launched(EXPERTS, 1);
   return out;
 }
-Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place) {
-  Tensor y = at::empty({place.size(0), rows.size(1)}, rows.options());
-  check(tmpi_expert_combine(rows.data_ptr(), weights.defined() ? weights.data_ptr<float>() : nullptr, place.data_ptr<int>(), y.data_ptr(), (int)place.size(0),
-                            (int)place.size(1), (int)rows.size(1), dtype_code(rows.scalar_type()), stream()));
+// rows of `type`, or in fp32 for bf16
+Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place, at::ScalarType type) {
+  const bool fp32 = type == at::kBFloat16 && rows.scalar_type() == at::kFloat;
+  Tensor y = at::empty({place.size(0), rows.size(1)}, rows.options().dtype(type));
+  check(tmpi_expert_combine(rows.data_ptr(), fp32, weights.defined() ? weights.data_ptr<float>() : nullptr, place.data_ptr<int>(), y.data_ptr(), (int)place.size(0),
+                            (int)place.size(1), (int)rows.size(1), dtype_code(type), stream()));
   launched(EXPERTS, 1);
   return y;
 }
@@ -181,7 +192,7 @@ struct DispatchFn : public torch::autograd::Function<DispatchFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    return {combine(packed(grads[0]), Tensor(), as_saved(saved[0])), Tensor(), Tensor()};
+    return {combine(packed(grads[0]), Tensor(), as_saved(saved[0]), grads[0].scalar_type()), Tensor(), Tensor()};
   }
 };
 
@@ -189,7 +200,7 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows_, const Tensor& weights_, const Tensor& order_, const Tensor& place_) {
     const Tensor rows = packed(rows_), weights = weights_.contiguous(), order = order_.contiguous(), place = place_.contiguous();
     ctx->save_for_backward({rows, weights, order});
-    return combine(rows, weights, place);
+    return combine(rows, weights, place, rows.scalar_type());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
@@ -208,7 +219,8 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
 // ---------------------------------------------------------------- a layer of experts
 // y_t = sum over j of weights_tj (gelu(x_t w1_e^T + b1_e) w2_e^T + b2_e), e = chosen_tj.  Kept for backward: x and the pre-activation,
 // in bf16 or (act8) in 8 bits, and neither the dispatched rows nor what the experts returned: the rows are gathered again, and the weight's gradient
-// dy . (w2 h + b2) is (w2^T dy) . h + dy . b2, of which the first product is there anyway.
+// dy . (w2 h + b2) is (w2^T dy) . h + dy . b2, of which the first product is there anyway.  What a token's experts return, and the gradients
+// that they return to it, are handed over in fp32 and rounded once, as their sum.
 struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weights_, const Tensor& chosen_, const Tensor& order_, const Tensor& place_,
                         const Tensor& offsets_, const Tensor& w1_, const OptTensor& b1_, const Tensor& w2_, const OptTensor& b2_, bool act8, bool keep) {
@@ -226,7 +238,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
       kz.q = at::empty({T * k, H}, x.options());
     }
     const Tensor h = grouped(xs, w1, b1, offsets, false, !keep ? GELU : act8 ? GELU_AND_Z8 : GELU_AND_Z, kz.q, kz.scale);
-    const Tensor y = combine(grouped(h, w2, b2, offsets, false, PLAIN, Tensor(), Tensor()), weights, place);
+    const Tensor y = combine(grouped(h, w2, b2, offsets, false, FP32, Tensor(), Tensor()), weights, place, x.scalar_type());
     if (keep) {
       ctx->save_for_backward({kx.q, kx.scale, kz.q, kz.scale, weights, chosen, order, place, offsets, w1, w2, b2});
       ctx->saved_data["b1"] = b1.defined();
@@ -247,11 +259,17 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     check(tmpi_expert_combine_gradient(dy.data_ptr(), ptr(b2), weights.data_ptr<float>(), 0, order.data_ptr<int>(), b2.defined() ? chosen.data_ptr<int>() : nullptr,
                                        g.data_ptr(), b2.defined() ? dwt.data_ptr<float>() : nullptr, by_place.data_ptr<float>(), (int)T, (int)k, (int)C, (int)E,
                                        dtype_code(dy.scalar_type()), stream()));
-    const Tensor dh = grouped(g, w2, Tensor(), offsets, true, PLAIN, Tensor(), Tensor());
-    Tensor dz = at::empty_like(dh), hw = at::empty_like(dh);
-    check(tmpi_expert_gelu_gradient(dh.data_ptr(), kz.q.data_ptr(), kz.scale.defined() ? kz.scale.data_ptr() : nullptr, weights.data_ptr<float>(),
-                                    order.data_ptr<int>(), dz.data_ptr(), hw.data_ptr(), dwt.data_ptr<float>(), (int)T, (int)k, (int)H, stream()));
-    launched(EXPERTS, 2);
+    launched(EXPERTS, 1);
+    const bool need_wt = ctx->needs_input_grad(1);
+    const int64_t slices = (H + 63) / 64;
+    Tensor dots;
+    if (need_wt) dots = at::empty({T * k, slices}, f32);
+    const auto both = grouped_gelu_gradient(g, w2, offsets, kz, by_place, dots);
+    const Tensor dz = both.first, hw = both.second;
+    if (need_wt) {
+      check(tmpi_expert_dots(dots.data_ptr<float>(), order.data_ptr<int>(), dwt.data_ptr<float>(), (int)T, (int)k, (int)slices, stream()));
+      launched(EXPERTS, 1);
+    }
     Tensor dx, dw1, db1, dw2, db2;
     if (need_w2 || need_b2) grouped_weight_gradient(g, hw, offsets, by_place, E, &dw2, need_b2 ? &db2 : nullptr);
     if (need_w1 || need_b1) {
@@ -265,9 +283,9 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
       }
       grouped_weight_gradient(dz, xs, offsets, Tensor(), E, &dw1, need_b1 ? &db1 : nullptr);
     }
-    if (need_x) dx = combine(grouped(dz, w1, Tensor(), offsets, true, PLAIN, Tensor(), Tensor()), Tensor(), place);
+    if (need_x) dx = combine(grouped(dz, w1, Tensor(), offsets, true, FP32, Tensor(), Tensor()), Tensor(), place, dy.scalar_type());
     const Tensor none;
-    return {dx, ctx->needs_input_grad(1) ? dwt : none, none, none, none, none, need_w1 ? dw1 : none, db1, need_w2 ? dw2 : none, db2, none, none};
+    return {dx, need_wt ? dwt : none, none, none, none, none, need_w1 ? dw1 : none, db1, need_w2 ? dw2 : none, db2, none, none};
   }
 };
 

@@ -392,15 +392,16 @@ int tmpi_route_gradient(const void* logits, int64_t ld, int tokens, int experts,
                         const float* dweights, void* dlogits, void* stream);
 int tmpi_expert_dispatch(const void* x, const int* order, void* out, int tokens, int k, int cols, int dtype, void* stream);
 int tmpi_expert_dispatch8(const void* q, const void* scale, const int* order, void* out, int tokens, int k, int cols, void* stream);
-int tmpi_expert_combine(const void* rows, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream);
+int tmpi_expert_combine(const void* rows, int rows_fp32, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream);
 int tmpi_expert_combine_gradient(const void* dy, const void* other, const float* weights, int scaled, const int* order, const int* chosen, void* drows,
                                  float* dweights, float* place_weights, int tokens, int k, int cols, int nexperts, int dtype, void* stream);
-int tmpi_expert_gelu_gradient(const void* dh, const void* z, const void* scale, const float* weights, const int* order, void* dz, void* hw, float* dweights,
-                              int tokens, int k, int cols, void* stream);
+int tmpi_expert_dots(const float* dots, const int* order, float* dweights, int tokens, int k, int slices, void* stream);
 // Products grouped by expert: rows offsets[e] <= r < offsets[e + 1] (on the device) of x belong to expert e
 int tmpi_grouped_max_experts(void);
 int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,
                       int w_is_kn, int mode, void* stream);
+int tmpi_grouped_gelu_gradient(const void* dy, const void* w, const int* offsets, const void* z, const void* scale, const float* row_weights, void* dz, void* h,
+                               float* dots, int rows, int nexperts, int K, int N, void* stream);
 int tmpi_grouped_weight_gradient(const void* dy, const void* x, const int* offsets, const float* row_weights, void* dw, void* db, int rows, int nexperts, int K,
                                  int N, void* stream);
 

@@ -10,6 +10,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include "attn_util.cuh"
 
 namespace tmpi {
 namespace act8 {
@@ -43,6 +44,44 @@ __device__ __forceinline__ void unpack2(uint32_t q, float scale, float* x0, floa
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
   *x0 = f.x * scale;
   *x1 = f.y * scale;
+}
+
+// A whole block by one thread; returns its scale byte.  Where all are finite, which the maximum tells, the elements need no look of their own.
+__device__ __forceinline__ uint32_t pack_block(const float (&x)[32], uint32_t (&q)[8]) {
+  float a = fabsf(x[0]), b = fabsf(x[1]);
+#pragma unroll
+  for (int j = 2; j < 32; j += 4) {
+    a = attn_util::max3_nan(a, fabsf(x[j]), fabsf(x[j + 1]));
+    if (j + 3 < 32) b = attn_util::max3_nan(b, fabsf(x[j + 2]), fabsf(x[j + 3]));
+  }
+  a = attn_util::max_nan(a, b);
+  uint32_t top = __float_as_uint(a);
+  const bool finite = top < 0x7f800000u;
+  if (!finite) {
+    top = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) top = max(top, magnitude(x[j]));
+  }
+  const uint32_t byte = scale_byte(top);
+  const float inv = inverse(byte);
+  if (finite) {
+    const unsigned long long inv2 = attn_util::pack2(__float_as_uint(inv), __float_as_uint(inv));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t h[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float2 v;
+        attn_util::unpack2(attn_util::mul2(attn_util::pack2(__float_as_uint(x[4 * j + 2 * i]), __float_as_uint(x[4 * j + 2 * i + 1])), inv2), v.x, v.y);
+        h[i] = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
+      }
+      q[j] = h[0] | h[1] << 16;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = pack2(x[4 * j], x[4 * j + 1], inv) | pack2(x[4 * j + 2], x[4 * j + 3], inv) << 16;
+  }
+  return byte;
 }
 
 // 8 elements of a checkpoint

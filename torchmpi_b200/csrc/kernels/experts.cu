@@ -1,12 +1,11 @@
 // Rows on their way to the experts and back: dispatch (a token's row to each of its experts' places), combine (the weighted sum of
-// what the experts made of it), their gradients, and the GELU backward between an expert's two products.
+// what the experts made of it) and their gradients.
 //
 // `order` (route.cu) gives the entry token * k + j at each place, `place` the place of each entry.  All passes read and write each element once
 // and are bound by memory.  Passes without a sum over a row give a thread one 16-byte piece of a row, so that one token of a long row is
 // spread over many blocks; those with one give a warp a row.  Sums are in fp32, in one order whatever the launch: nothing is accumulated
 // by atomics.
 #include "act8.cuh"
-#include "gelu.cuh"
 #include "pdl.cuh"
 #include "vec.cuh"
 #include "../include/tmpi_c_api.h"
@@ -121,8 +120,8 @@ __global__ void __launch_bounds__(THREADS) dispatch8_kernel(const uint8_t* __res
 
 // y[t] = sum over j of weights[t, j] rows[place[t, j]], added in the order of j and rounded once; weights null: ones.  An entry without a
 // place adds its weight times zero: nothing, or NaN where the weight is.
-template <typename T, int V>
-__global__ void __launch_bounds__(THREADS) combine_kernel(const T* __restrict__ rows, const float* __restrict__ weights, const int* __restrict__ place,
+template <typename R, typename T, int V>
+__global__ void __launch_bounds__(THREADS) combine_kernel(const R* __restrict__ rows, const float* __restrict__ weights, const int* __restrict__ place,
                                                           T* __restrict__ y, int tokens, int places, int k, int cols) {
   wait_previous(rows, weights, place);
   const int parts = cols / V;
@@ -136,7 +135,7 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const T* __restrict__ 
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
     constexpr int U = 4;                                  // entries in flight
     for (int j0 = 0; j0 < k; j0 += U) {
-      Pack<T, V> v[U];
+      Pack<R, V> v[U];
       float w[U];
       bool there[U];
 #pragma unroll
@@ -147,12 +146,12 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const T* __restrict__ 
         const int s = place[t * k + j0 + u];
         w[u] = weights ? weights[t * k + j0 + u] : 1.f;
         there[u] = s >= 0 && s < places;
-        if (there[u]) v[u] = ld_pack<T, V>(rows + (long long)s * cols + part * V);
+        if (there[u]) v[u] = ld_pack<R, V>(rows + (long long)s * cols + part * V);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum[e] += w[u] * (there[u] ? (float)to_acc<T>(v[u].v[e]) : 0.f);
+        for (int e = 0; e < V; ++e) sum[e] += w[u] * (there[u] ? (float)to_acc<R>(v[u].v[e]) : 0.f);
     }
     Pack<T, V> o;
 #pragma unroll
@@ -215,70 +214,17 @@ __global__ void __launch_bounds__(THREADS) combine_gradient_kernel(const T* __re
   }
 }
 
-// Between an expert's products, a warp to a place: with z~ the checkpoint of the pre-activation (8 bits, or bf16), h = gelu(z~) and w the
-// entry's weight,  dz = w dh gelu'(z~),  hw = w h,  dweights[entry] += dh . h.  (dh is the gradient that the unweighted output would get; so
-// the weight's gradient needs no second look at what the experts returned.)
-template <bool KEPT8>
-__global__ void __launch_bounds__(THREADS, 4) expert_gelu_kernel(const __nv_bfloat16* __restrict__ dh, const void* z, const uint8_t* __restrict__ scale,
-                                                                 const float* __restrict__ weights, const int* __restrict__ order,
-                                                                 __nv_bfloat16* __restrict__ dz, __nv_bfloat16* __restrict__ hw, float* __restrict__ dweights,
-                                                                 int places, int tokens, int k, int cols) {
-  const uint8_t* zq = (const uint8_t*)z;
-  wait_previous(dh, zq, scale, weights, order);
-  const int lane = threadIdx.x & 31, parts = cols / 8, blocks = (cols + act8::BLOCK - 1) / act8::BLOCK;
+// dweights[entry] += the sum of the entry's row of `dots` (grouped.cu: a number for 64 columns), a warp to a place
+__global__ void __launch_bounds__(THREADS) dots_kernel(const float* __restrict__ dots, const int* __restrict__ order, float* __restrict__ dweights, int places, int tokens,
+                                                       int k, int slices) {
+  wait_previous(dots, order);
+  const int lane = threadIdx.x & 31;
   for (long long s = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); s < places; s += (long long)gridDim.x * WARPS) {
-    if (token_at(order, (int)s, k, tokens) < 0) continue;            // nothing reads these rows
-    const int entry = order[s];
-    const float w = weights[entry];
-    float dot = 0.f;
-    constexpr int U = 2;
-    for (int c0 = lane; c0 < parts; c0 += U * 32) {
-      uint4 g[U], zb[U];
-      uint2 q[U];
-      uint32_t e[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = c0 + 32 * u;
-        if (c >= parts) break;
-        g[u] = *reinterpret_cast<const uint4*>(dh + s * cols + c * 8);
-        if (KEPT8) {
-          q[u] = *reinterpret_cast<const uint2*>(zq + s * cols + c * 8);
-          e[u] = scale[s * blocks + (c >> 2)];
-        } else {
-          zb[u] = *reinterpret_cast<const uint4*>(zq + (s * cols + c * 8) * 2);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = c0 + 32 * u;
-        if (c >= parts) break;
-        float v[8], f[8];
-        auto widen = [](const uint4& a, float (&x)[8]) {
-          const uint32_t b[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(b[i] << 16); x[2 * i + 1] = __uint_as_float(b[i] & 0xffff0000u); }
-        };
-        if (KEPT8) act8::unpack8(q[u], act8::value(e[u]), v);
-        else widen(zb[u], v);
-        widen(g[u], f);
-        Pack<__nv_bfloat16, 8> a, b;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          float y[2], d[2];
-          gelu_both2(v[i], v[i + 1], &y[0], &y[1], &d[0], &d[1]);
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            dot += f[i + n] * y[n];
-            a.v[i + n] = __float2bfloat16_rn(w * f[i + n] * d[n]);
-            b.v[i + n] = __float2bfloat16_rn(w * y[n]);
-          }
-        }
-        st_pack<__nv_bfloat16, 8>(dz + s * cols + c * 8, a);
-        st_pack<__nv_bfloat16, 8>(hw + s * cols + c * 8, b);
-      }
-    }
-    dot = warp_sum(dot);
-    if (lane == 0) dweights[entry] += dot;
+    if (token_at(order, (int)s, k, tokens) < 0) continue;
+    float sum = 0.f;
+    for (int i = lane; i < slices; i += 32) sum += dots[s * slices + i];
+    sum = warp_sum(sum);
+    if (lane == 0) dweights[order[s]] += sum;
   }
 }
 
@@ -340,16 +286,24 @@ int tmpi_expert_dispatch8(const void* q, const void* scale, const int* order, vo
                                            (const uint8_t*)q, (const uint8_t*)scale, order, (__nv_bfloat16*)out, places, tokens, k, cols), "expert_dispatch8");
 }
 
-// y [tokens, cols] from rows [tokens * k, cols]; weights [tokens, k] or null
-int tmpi_expert_combine(const void* rows, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream) {
+// y [tokens, cols] of `dtype` from rows [tokens * k, cols] of `dtype`, or in fp32 (rows_fp32: y bf16); weights [tokens, k] or null
+int tmpi_expert_combine(const void* rows, int rows_fp32, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream) {
   const int st = experts::checked(tokens, k, cols, dtype, "expert_combine");
   if (st || !tokens) return st;
-  return experts::finish(experts::by_type(dtype, cols, {rows, y}, [&](auto t, auto v) {
+  if (rows_fp32 && dtype != TMPI_BF16) return fail(TMPI_ERR_UNSUPPORTED, "expert_combine: fp32 rows to dtype %d", dtype);
+  auto go = [&](auto r, auto t, auto v) {
+    using R = decltype(r);
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
-    return launch_overlapped(experts::combine_kernel<T, V>, experts::grid_items((long long)tokens * (cols / V), 1, 8), experts::THREADS, 0, (cudaStream_t)stream,
-                             (const T*)rows, weights, place, (T*)y, tokens, tokens * k, k, cols);
-  }), "expert_combine");
+    return launch_overlapped(experts::combine_kernel<R, T, V>, experts::grid_items((long long)tokens * (cols / V), 1, 8), experts::THREADS, 0, (cudaStream_t)stream,
+                             (const R*)rows, weights, place, (T*)y, tokens, tokens * k, k, cols);
+  };
+  if (rows_fp32) {
+    const bool wide = cols % 4 == 0 && all_aligned16({rows, y});
+    return experts::finish(wide ? go(float(), __nv_bfloat16(), std::integral_constant<int, 4>()) : go(float(), __nv_bfloat16(), std::integral_constant<int, 1>()),
+                           "expert_combine");
+  }
+  return experts::finish(experts::by_type(dtype, cols, {rows, y}, [&](auto t, auto v) { return go(t, t, v); }), "expert_combine");
 }
 
 // drows [tokens * k, cols] and, where given, dweights [tokens * k] (of the entries that have a place) from dy [tokens, cols].  other: rows
@@ -368,17 +322,12 @@ int tmpi_expert_combine_gradient(const void* dy, const void* other, const float*
   }), "expert_combine_gradient");
 }
 
-// dz, hw [tokens * k, cols] bf16 and dweights [tokens * k] (added to) from dh and the checkpoint of z: e4m3 with `scale`, or bf16 without.
-// cols a multiple of 8, tensors on 16-byte boundaries.
-int tmpi_expert_gelu_gradient(const void* dh, const void* z, const void* scale, const float* weights, const int* order, void* dz, void* hw, float* dweights,
-                              int tokens, int k, int cols, void* stream) {
-  const int st = experts::checked(tokens, k, cols, TMPI_BF16, "expert_gelu_gradient");
+// dweights [tokens * k] += the sums of the rows of dots [tokens * k, slices], for the entries that have a place
+int tmpi_expert_dots(const float* dots, const int* order, float* dweights, int tokens, int k, int slices, void* stream) {
+  const int st = experts::checked(tokens, k, slices, TMPI_F32, "expert_dots");
   if (st || !tokens) return st;
-  if (cols % 8 || !all_aligned16({dh, z, dz, hw})) return fail(TMPI_ERR_INVALID, "expert_gelu_gradient: rows must be multiples of 16 bytes, on 16-byte boundaries");
-  const auto kernel = scale ? experts::expert_gelu_kernel<true> : experts::expert_gelu_kernel<false>;
-  return experts::finish(launch_overlapped(kernel, experts::grid_rows(tokens * k, 4), experts::THREADS, 0, (cudaStream_t)stream, (const __nv_bfloat16*)dh, z,
-                                           (const uint8_t*)scale, weights, order, (__nv_bfloat16*)dz, (__nv_bfloat16*)hw, dweights, tokens * k, tokens, k, cols),
-                         "expert_gelu_gradient");
+  return experts::finish(launch_overlapped(experts::dots_kernel, experts::grid_rows(tokens * k, 8), experts::THREADS, 0, (cudaStream_t)stream, dots, order, dweights,
+                                           tokens * k, tokens, k, slices), "expert_dots");
 }
 
 }  // extern "C"

@@ -38,25 +38,39 @@ constexpr int FEW = 32;                                 // rows of the smaller b
 constexpr int EPI_THREADS = GROUPS * 128;
 constexpr int SLICE = 64, SLICE_BYTES = BM * SLICE * 2;
 
-enum { PLAIN = 0, GELU_ONLY = 1, WITH_GELU = 2, KEEP8 = 3 };
+// PLAIN32: the sum in fp32.  GRADIENT8 / 16: the sum is the gradient of a GELU's value, whose input z was kept in 8 bits or in bf16.
+enum { PLAIN = 0, GELU_ONLY = 1, WITH_GELU = 2, KEEP8 = 3, PLAIN32 = 4, GRADIENT8 = 5, GRADIENT16 = 6 };
 
 struct Problem {
   const int* offsets;        // [experts + 1]; null: one expert with all rows
   int rows, experts, K, N;   // of x; N: columns of the result
   int bn, tiles_n, k_blocks;
   const __nv_bfloat16* bias; // [experts, N] or null
-  __nv_bfloat16* y;          // [rows, N]
-  __nv_bfloat16* z;          // WITH_GELU: the pre-activation
-  uint8_t *q, *scale;        // KEEP8: its 8-bit checkpoint
+  __nv_bfloat16* y;          // [rows, N]; GRADIENT: dz
+  float* y32;                // PLAIN32
+  void* z;                   // WITH_GELU, GRADIENT16: the pre-activation [rows, N]; KEEP8, GRADIENT8: its e4m3 numbers
+  uint8_t* scale;            // and their scales
+  __nv_bfloat16* h;          // GRADIENT: weight times gelu(z)
+  const float* row_weights;  // GRADIENT: [rows] or null (ones)
+  float* dots;               // GRADIENT: [rows, slices], the sum over 64 columns of gradient times gelu(z); or null
+  int wide;                  // every row of y, z, h starts on a 32-byte boundary
   int* status;
 };
 
+// Four groups of four epilogue warps: a group takes 64 columns of a tile.  With two groups, whose warps met at barriers around TMA stores, a GELU
+// epilogue ran at 1.1 instructions per cycle and SM and was longer than its tile's MMAs: 16384 x 4096 x 1024 127 us with a GELU, 176 with an
+// 8-bit checkpoint beside it, 103 plain.
+constexpr int ROW_GROUPS = 4, ROW_THREADS = 64 + ROW_GROUPS * 128;
+constexpr int NST = 7;                                  // stages of the operand ring: no staging for the epilogue beside them
+
 struct Sh {
-  Shared s;
+  uint64_t full[NST], empty[NST], acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int error;
   int warp_sums[8];
   int tile_end[MAX_EXPERTS];                            // tiles of the experts up to and with this one
 };
-constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + gemm::EPI_STAGING_BYTES + 1024 + 1280;
+constexpr size_t SMEM = (size_t)NST * STAGE_BYTES + 1024 + 1280;
 static_assert(sizeof(Sh) <= 1280 && SMEM <= 232448, "shared memory of one CTA");
 
 // Offsets as given, but inside the tensor and not before the group's start: wrong ones give wrong results, never an access outside.
@@ -73,7 +87,8 @@ struct Unit {
   __device__ __forceinline__ int part_rows(uint32_t rank) const { return min(max(end - row0 - (int)rank * BM, 0), BM); }
 };
 
-__device__ __forceinline__ void give_up(Shared* sh, int* status, int where) {
+template <typename S>
+__device__ __forceinline__ void give_up(S* sh, int* status, int where) {
   atomicExch(&sh->error, where);
   if (status) atomicCAS(status, 0, 1000 + where);
 }
@@ -131,19 +146,18 @@ __device__ __forceinline__ void for_tiles(const Sh* sh, const Problem& p, const 
 __device__ __forceinline__ uint32_t a_bytes(int rows) { return rows > FEW ? A_BYTES : rows > 0 ? FEW * BK * 2 : 0; }
 
 struct Ring { int stage; uint32_t phase; };
-template <int NST>
-__device__ __forceinline__ void advance(Ring* r) { if (++r->stage == NST) { r->stage = 0; r->phase ^= 1; } }
+template <int N>
+__device__ __forceinline__ void advance(Ring* r) { if (++r->stage == N) { r->stage = 0; r->phase ^= 1; } }
 
 // One thread in each CTA.
-template <int NST, bool B_MN>
-__device__ __forceinline__ void produce(Sh* shl, unsigned char* tiles, const Problem& p, const int* offsets, const CUtensorMap* ma, const CUtensorMap* ma_few,
+template <bool B_MN>
+__device__ __forceinline__ void produce(Sh* sh, unsigned char* tiles, const Problem& p, const int* offsets, const CUtensorMap* ma, const CUtensorMap* ma_few,
                                         const CUtensorMap* mb, uint32_t rank) {
-  Shared* sh = &shl->s;
   const int half = p.bn / 2;
   const bool two = half > 64;
   const uint32_t b_tx = 2 * (B_MN ? (two ? B_BYTES : B_BYTES / 2) : half * BK * 2);
   Ring ring{0, 0};
-  for_tiles(shl, p, offsets, [&](const Unit& u, int) -> bool {
+  for_tiles(sh, p, offsets, [&](const Unit& u, int) -> bool {
     const int mine = u.part_rows(rank), a_row0 = u.row0 + (int)rank * BM, n0 = u.n_blk * p.bn + (int)rank * half;
     const uint32_t tx = b_tx + a_bytes(u.part_rows(0)) + a_bytes(u.part_rows(1));
     for (int kb = 0; kb < p.k_blocks; ++kb) {
@@ -166,12 +180,11 @@ __device__ __forceinline__ void produce(Sh* shl, unsigned char* tiles, const Pro
 }
 
 // One thread of the even CTA.
-template <int NST, bool B_MN>
-__device__ __forceinline__ void issue(Sh* shl, unsigned char* tiles, const Problem& p, const int* offsets) {
-  Shared* sh = &shl->s;
+template <bool B_MN>
+__device__ __forceinline__ void issue(Sh* sh, unsigned char* tiles, const Problem& p, const int* offsets) {
   const uint32_t idesc = sm100::make_idesc_f16(2 * BM, p.bn, true, B_MN, false);
   Ring ring{0, 0};
-  for_tiles(shl, p, offsets, [&](const Unit&, int it) -> bool {
+  for_tiles(sh, p, offsets, [&](const Unit&, int it) -> bool {
     const int acc = it & 1;
     if (!sm100::mbar_wait(&sh->acc_empty[acc], ((it >> 1) & 1) ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 32); return false; }
     sm100::tc_fence_after();
@@ -206,160 +219,247 @@ __device__ __forceinline__ bool all_of(uint32_t ok, int barrier) {
   return all != 0;
 }
 
-// 64 columns of a row as bf16
-__device__ __forceinline__ void to_bf16(const uint32_t (&r)[2][32], uint32_t (&w)[32]) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j) w[j] = attn_util::pack_bf16(r[j >> 4][2 * (j & 15)], r[j >> 4][2 * (j & 15) + 1]);
+// n 32-bit words to or from consecutive addresses: 32 bytes at once where rows start on such a boundary (a whole sector of L2 per lane), else 16 or 8.
+__device__ __forceinline__ void store32(void* to, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
-__device__ __forceinline__ void stage_row(unsigned char* stg_row, int row, const uint32_t (&w)[32]) {
+__device__ __forceinline__ void load32(const void* from, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(from));
+}
+// 32 bf16 columns of a row, `left` of them inside it (a multiple of 8)
+__device__ __forceinline__ void store_row(__nv_bfloat16* to, const uint32_t (&w)[16], int left, bool wide) {
+  if (wide && left >= 32) {
+    store32(to, w);
+    store32(to + 16, w + 8);
+  } else {
 #pragma unroll
-  for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(stg_row + ((u ^ (row & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+    for (int j = 0; j < 4; ++j)
+      if (8 * j < left) reinterpret_cast<uint4*>(to)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  }
+}
+__device__ __forceinline__ void load_row(const __nv_bfloat16* from, uint32_t (&w)[16], int left, bool wide) {
+  if (wide && left >= 32) {
+    load32(from, w);
+    load32(from + 16, w + 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 v = 8 * j < left ? reinterpret_cast<const uint4*>(from)[j] : make_uint4(0u, 0u, 0u, 0u);
+      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+    }
+  }
+}
+// 32 e4m3 columns
+__device__ __forceinline__ void store_row8(uint8_t* to, const uint32_t (&q)[8], int left, bool wide) {
+  if (wide && left >= 32) {
+    store32(to, q);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (8 * j < left) reinterpret_cast<uint2*>(to)[j] = make_uint2(q[2 * j], q[2 * j + 1]);
+  }
+}
+__device__ __forceinline__ void load_row8(const uint8_t* from, uint32_t (&q)[8], int left, bool wide) {
+  if (wide && left >= 32) {
+    load32(from, q);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint2 v = 8 * j < left ? reinterpret_cast<const uint2*>(from)[j] : make_uint2(0u, 0u);
+      q[2 * j] = v.x; q[2 * j + 1] = v.y;
+    }
+  }
+}
+__device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = attn_util::pack_bf16(__float_as_uint(v[2 * j]), __float_as_uint(v[2 * j + 1]));
 }
 
-// The eight epilogue warps of each CTA: two groups of four take the 64-column slices of a tile in turn, as in gemm_pair.cuh.  The GELU is that of
-// the fp32 sum.  KEEP8: a thread has whole blocks of 32 columns of its row, so the checkpoint of the fp32 sum takes no exchange between threads.
+// The sixteen epilogue warps of each CTA.  A thread has a row of the tile, and its warp works on 32 of its columns at a time, without a word to
+// the others: results go to memory from registers, 32 bytes a store, so that whole and partial tiles take the same path and no barrier or fence stands
+// in it.  The GELU is that of the fp32 sum, and so is the 8-bit checkpoint, whose blocks of 32 columns a thread has to itself.
 template <int MODE>
-__device__ __forceinline__ void finish(Sh* shl, unsigned char* staging, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const CUtensorMap* map_y,
-                                       const CUtensorMap* map_z, uint32_t rank, int group, int quarter, int lane) {
-  Shared* sh = &shl->s;
-  constexpr bool TWO = MODE == WITH_GELU;
-  const int row = quarter * 32 + lane, N = p.N, bn = p.bn;
-  const bool leader = quarter == 0 && lane == 0;
-  unsigned char* stg0 = staging + group * SLICE_BYTES;
-  for_tiles(shl, p, offsets, [&](const Unit& u, int it) -> bool {
-    const int acc = it & 1, rows = u.part_rows(rank);
+__device__ __forceinline__ void finish(Sh* sh, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights, uint32_t rank, int group,
+                                       int quarter, int lane) {
+  constexpr bool GRADIENT = MODE == GRADIENT8 || MODE == GRADIENT16;
+  const int row = quarter * 32 + lane, N = p.N, bn = p.bn, slices = (N + SLICE - 1) / SLICE, blocks = (N + 31) / 32;
+  const bool wide = p.wide != 0;
+  for_tiles(sh, p, offsets, [&](const Unit& u, int it) -> bool {
+    const int acc = it & 1, rows = u.part_rows(rank), c0 = group * SLICE, col0 = u.n_blk * bn + c0;
+    const bool busy = rows > quarter * 32 && c0 < bn && col0 < N;                 // of this warp
+    const bool mine = busy && row < rows;
     const long long row_at = (long long)u.row0 + (int)rank * BM + row;
     const __nv_bfloat16* bias = bias_all ? bias_all + (long long)u.e * N : nullptr;
-    const uint32_t ok = sm100::mbar_wait(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs) && !sh->error;
-    if (!all_of<128>(ok, 1 + group)) { give_up(sh, p.status, 34); return false; }
-    sm100::tc_fence_after();
-    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * BN;
-    if (rows > 0) {
-#pragma unroll 1
-      for (int c0 = group * SLICE; c0 < bn; c0 += GROUPS * SLICE) {
-        const int col0 = u.n_blk * bn + c0;
-        if (col0 >= N) break;
-        uint32_t r[2][32], w[32];
-        sm100::tmem_ld_32x32(t_base + c0, r[0]);
-        sm100::tmem_ld_32x32(t_base + c0 + 32, r[1]);
-        sm100::tmem_ld_wait();
-        if (bias) {
+    float weight = 1.f, dot = 0.f;
+    uint32_t kept[2][GRADIENT ? 8 : 1];
+    uint32_t kept_scale[2] = {1u, 1u};
+    if (GRADIENT && mine) {                              // while the products are under way
+      if (row_weights) weight = __ldg(row_weights + row_at);
+      if (MODE == GRADIENT8) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {                  // N is a multiple of 8
-            if (col0 + 8 * j >= N) break;
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(bias + col0) + j);
-            const uint32_t b[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t* x = &r[j >> 2][(j & 3) * 8 + 2 * q];
-              x[0] = __float_as_uint(__uint_as_float(x[0]) + __uint_as_float(b[q] << 16));
-              x[1] = __float_as_uint(__uint_as_float(x[1]) + __uint_as_float(b[q] & 0xffff0000u));
-            }
+        for (int h = 0; h < 2; ++h)
+          if (col0 + 32 * h < N) {
+            load_row8((const uint8_t*)p.z + row_at * N + col0 + 32 * h, *reinterpret_cast<uint32_t(*)[8]>(&kept[h]), N - col0 - 32 * h, wide);
+            kept_scale[h] = p.scale[row_at * blocks + col0 / 32 + h];
           }
-        }
-        auto put = [&](const CUtensorMap* map, __nv_bfloat16* to, int which) {
-          if (rows == BM) {
-            unsigned char* stg = stg0 + which * GROUPS * SLICE_BYTES;
-            if (leader) {                                // the store that used this staging tile before must have read it
-              if (TWO) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-              else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            }
-            group_sync(group);
-            stage_row(stg + row * 128, row, w);
-            sm100::fence_proxy_async_smem();
-            group_sync(group);
-            if (leader) {
-              sm100::tma_store_2d(map, stg, col0, u.row0 + (int)rank * BM);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
-          } else if (row < rows) {
-            uint4* at = reinterpret_cast<uint4*>(to + row_at * N + col0);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (col0 + 8 * j < N) at[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-          }
-        };
-        if (TWO) {
-          to_bf16(r, w);
-          put(map_z, p.z, 1);
-        }
-        if (MODE == KEEP8) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int col = col0 + 32 * h;
-            uint32_t a = 0;                              // columns behind N: zeros (the weight's rows there read as zero, and have no bias)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) a = max(a, act8::magnitude(__uint_as_float(r[h][j])));
-            const uint32_t byte = act8::scale_byte(a);
-            const float inv = act8::inverse(byte);
-            if (row < rows && col < N) {
-              p.scale[row_at * ((N + 31) / 32) + col / 32] = (uint8_t)byte;
-              uint2* at = reinterpret_cast<uint2*>(p.q + row_at * N + col);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[h][8 * j + i]);
-                if (col + 8 * j < N) at[j] = act8::pack8(x, inv);
-              }
-            }
-          }
-        }
-        if (MODE != PLAIN) {
-#pragma unroll
-          for (int j = 0; j < 64; j += 2) {
-            float y0, y1;
-            uint32_t* x = &r[j >> 5][j & 31];
-            gelu_value2(__uint_as_float(x[0]), __uint_as_float(x[1]), &y0, &y1);
-            x[0] = __float_as_uint(y0);
-            x[1] = __float_as_uint(y1);
-          }
-        }
-        to_bf16(r, w);
-        put(map_y, p.y, 0);
       }
     }
-    sm100::tc_fence_before();
-    __syncwarp();
-    if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&sh->acc_empty[acc], 0));
+    if (!sm100::mbar_wait_warp(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 34); return false; }
+    sm100::tc_fence_after();
+    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * BN + c0;
+    auto release = [&] {                                 // the accumulator has been read
+      sm100::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&sh->acc_empty[acc], 0));
+    };
+    if (!busy) { release(); return true; }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int col = col0 + 32 * half, left = N - col;
+      if (half && left <= 0) { release(); break; }
+      uint32_t r[32], zb[16];
+      if (MODE == GRADIENT16 && mine) load_row((const __nv_bfloat16*)p.z + row_at * N + col, zb, left, wide);
+      sm100::tmem_ld_32x32(t_base + 32 * half, r);
+      uint4 b[4];
+      if (!GRADIENT && bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = 8 * j < left ? __ldg(reinterpret_cast<const uint4*>(bias + col) + j) : make_uint4(0u, 0u, 0u, 0u);
+      }
+      sm100::tmem_ld_wait();
+      if (half) release();
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+      if (!GRADIENT && bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            v[8 * j + 2 * q] += __uint_as_float(x[q] << 16);
+            v[8 * j + 2 * q + 1] += __uint_as_float(x[q] & 0xffff0000u);
+          }
+        }
+      }
+      uint32_t w[16];
+      if (MODE == PLAIN32) {
+        if (mine) {
+          float* to = p.y32 + row_at * N + col;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (8 * j < left) store32(to + 8 * j, reinterpret_cast<const uint32_t*>(v) + 8 * j);
+        }
+        continue;
+      }
+      if (MODE == WITH_GELU) {
+        pack_row(v, w);
+        if (mine) store_row((__nv_bfloat16*)p.z + row_at * N + col, w, left, wide);
+      }
+      if (MODE == KEEP8) {
+        uint32_t q[8];
+        const uint32_t byte = act8::pack_block(v, q);    // columns behind N are zeros: the weight's rows there read as zero, and have no bias
+        if (mine) {
+          store_row8((uint8_t*)p.z + row_at * N + col, q, left, wide);
+          p.scale[row_at * blocks + col / 32] = (uint8_t)byte;
+        }
+      }
+      if (MODE == GELU_ONLY || MODE == WITH_GELU || MODE == KEEP8) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) gelu_value2(v[j], v[j + 1], &v[j], &v[j + 1]);
+      }
+      if (GRADIENT) {
+        float h[32];
+        const float scale = act8::value(kept_scale[half]);
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          float z0, z1, y0, y1, d0, d1;
+          if (MODE == GRADIENT8) {
+            act8::unpack2(kept[half][j >> 2] >> (16 * ((j >> 1) & 1)), scale, &z0, &z1);
+          } else {
+            z0 = __uint_as_float(zb[j >> 1] << 16);
+            z1 = __uint_as_float(zb[j >> 1] & 0xffff0000u);
+          }
+          gelu_both2(z0, z1, &y0, &y1, &d0, &d1);
+          if (j < left) dot += v[j] * y0 + v[j + 1] * y1;
+          v[j] = weight * v[j] * d0;
+          v[j + 1] = weight * v[j + 1] * d1;
+          h[j] = weight * y0;
+          h[j + 1] = weight * y1;
+        }
+        pack_row(h, w);
+        if (mine) store_row(p.h + row_at * N + col, w, left, wide);
+      }
+      pack_row(v, w);
+      if (mine) store_row(p.y + row_at * N + col, w, left, wide);
+    }
+    if (GRADIENT && mine && p.dots) p.dots[row_at * slices + col0 / SLICE] = dot;
     return true;
   });
-  // rows behind the last group
-  const long long used = group_of(offsets, p.rows, p.experts - 1).r1;
-  const long long chunks = (p.rows - used) * (N / 8);
-  uint4* rest = reinterpret_cast<uint4*>(p.y + used * N);
-  for (long long i = (long long)blockIdx.x * EPI_THREADS + (threadIdx.x - 64); i < chunks; i += (long long)gridDim.x * EPI_THREADS) rest[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  if (MODE == PLAIN || MODE == GELU_ONLY || MODE == WITH_GELU) {      // rows behind the last group
+    const long long used = group_of(offsets, p.rows, p.experts - 1).r1;
+    const long long chunks = (p.rows - used) * (N / 8);
+    uint4* rest = reinterpret_cast<uint4*>(p.y + used * N);
+    for (long long i = (long long)blockIdx.x * (ROW_GROUPS * 128) + (threadIdx.x - 64); i < chunks; i += (long long)gridDim.x * (ROW_GROUPS * 128))
+      rest[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
 }
 
 template <int MODE, bool B_MN>
-__global__ void __launch_bounds__(GROUP_THREADS, 1)
+__global__ void __launch_bounds__(ROW_THREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_few, const __grid_constant__ CUtensorMap map_b,
-               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z, const __grid_constant__ Problem p) {
+               const __grid_constant__ Problem p) {
   extern __shared__ unsigned char smem_raw[];
-  unsigned char *tiles, *staging;
-  Shared* sh0;
-  constexpr int NST = MODE == WITH_GELU ? STAGES - 1 : STAGES;
-  carve<NST>(smem_raw, &tiles, &sh0, &staging);
-  Sh* sh = reinterpret_cast<Sh*>(sh0);
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  Sh* sh = reinterpret_cast<Sh*>(tiles + (size_t)NST * STAGE_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = sm100::cluster_ctarank();
-  setup(sh0, warp, &map_a, &map_b, 4 * GROUPS);
+  if (warp == 0 && sm100::elect_one()) {
+    sm100::tma_prefetch_desc(&map_a);
+    sm100::tma_prefetch_desc(&map_b);
+    for (int s = 0; s < NST; ++s) { sm100::mbar_init(&sh->full[s], 1); sm100::mbar_init(&sh->empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { sm100::mbar_init(&sh->acc_full[a], 1); sm100::mbar_init(&sh->acc_empty[a], 8 * ROW_GROUPS); }
+    sh->error = 0;
+    sm100::fence_barrier_init();
+  }
+  if (warp == 1) {
+    sm100::tmem_alloc_pair(&sh->tmem_base, TMEM_COLS);
+    sm100::tmem_relinquish_pair();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::cluster_sync();          // the other CTA's barriers exist before anything signals them
+  sm100::tc_fence_after();
   const int* offsets = p.offsets;
   const __nv_bfloat16* bias = p.bias;
-  wait_previous(offsets, bias);
-  count_tiles(sh, p, p.offsets ? offsets : nullptr);
+  const float* row_weights = p.row_weights;
+  wait_previous(offsets, bias, row_weights);
   if (!p.offsets) offsets = nullptr;
   if (!p.bias) bias = nullptr;
+  if (!p.row_weights) row_weights = nullptr;
+  count_tiles(sh, p, offsets);
   if (warp == 0) {
-    if (sm100::elect_one()) produce<NST, B_MN>(sh, tiles, p, offsets, &map_a, &map_a_few, &map_b, rank);
+    if (sm100::elect_one()) produce<B_MN>(sh, tiles, p, offsets, &map_a, &map_a_few, &map_b, rank);
   } else if (warp == 1) {
-    if (rank == 0 && sm100::elect_one()) issue<NST, B_MN>(sh, tiles, p, offsets);
+    if (rank == 0 && sm100::elect_one()) issue<B_MN>(sh, tiles, p, offsets);
   } else {
-    finish<MODE>(sh, staging, p, offsets, bias, &map_y, &map_z, rank, (warp - 2) >> 2, warp & 3, lane);
+    finish<MODE>(sh, p, offsets, bias, row_weights, rank, (warp - 2) >> 2, warp & 3, lane);
   }
   __syncwarp();
-  teardown(sh0, warp);
+  // neither CTA frees its tensor memory or exits while the other may still signal its barriers or have the pair's MMAs read its shared memory
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (sh->error && warp == 0 && sm100::elect_one()) {
+    const unsigned long long t0 = sm100::now_ns();
+    while (sm100::now_ns() - t0 < 200000000ull) { __nanosleep(1000); }   // copies in flight complete within microseconds
+  }
+  __syncthreads();
+  sm100::cluster_sync();
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc_pair(sh->tmem_base, TMEM_COLS);
+  }
 }
 
 // ---------------------------------------------------------------- the weights' gradient
@@ -381,7 +481,8 @@ struct DwSh {
   uint64_t tail[STAGES];                                // a block with rows of another group: its loads, one barrier per CTA
   uint64_t cleared[STAGES];                             // in the even CTA: the odd one's part of such a block is cleared
 };
-static_assert(sizeof(DwSh) <= 1280, "barriers");
+constexpr size_t DW_SMEM = (size_t)STAGES * STAGE_BYTES + gemm::EPI_STAGING_BYTES + 1024 + sizeof(DwSh);
+static_assert(DW_SMEM <= 232448, "shared memory of one CTA");
 
 struct DwUnit { int e, m_blk, n_blk, r0, r1, k_blocks; };
 
@@ -520,6 +621,16 @@ __device__ __forceinline__ void dw_issue(DwSh* shl, unsigned char* tiles, const 
     sm100::umma_commit_pair(sm100::map_to_cta(&sh->acc_full[acc], 1));
     return true;
   });
+}
+
+// 64 columns of a row as bf16
+__device__ __forceinline__ void to_bf16(const uint32_t (&r)[2][32], uint32_t (&w)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) w[j] = attn_util::pack_bf16(r[j >> 4][2 * (j & 15)], r[j >> 4][2 * (j & 15) + 1]);
+}
+__device__ __forceinline__ void stage_row(unsigned char* stg_row, int row, const uint32_t (&w)[32]) {
+#pragma unroll
+  for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(stg_row + ((u ^ (row & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
 }
 
 __device__ __forceinline__ void all_sync() { asm volatile("bar.sync 3, %0;" ::"n"(EPI_THREADS) : "memory"); }
@@ -666,24 +777,28 @@ grouped_dw_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_const
 }
 
 // ---------------------------------------------------------------- host side
-static void allow(const void* kernel) { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM); }
+static const void* row_kernel(int mode, bool w_is_kn) {
+  if (w_is_kn)
+    return mode == PLAIN32 ? (const void*)grouped_kernel<PLAIN32, true> : mode == GRADIENT8 ? (const void*)grouped_kernel<GRADIENT8, true>
+           : mode == GRADIENT16 ? (const void*)grouped_kernel<GRADIENT16, true> : (const void*)grouped_kernel<PLAIN, true>;
+  return mode == GELU_ONLY ? (const void*)grouped_kernel<GELU_ONLY, false> : mode == WITH_GELU ? (const void*)grouped_kernel<WITH_GELU, false>
+         : mode == KEEP8 ? (const void*)grouped_kernel<KEEP8, false> : mode == PLAIN32 ? (const void*)grouped_kernel<PLAIN32, false>
+                                                                                       : (const void*)grouped_kernel<PLAIN, false>;
+}
 
 static int max_clusters() {
   static int n = 0;
   static std::once_flag once;
   std::call_once(once, [] {
-    allow((const void*)grouped_kernel<PLAIN, false>);
-    allow((const void*)grouped_kernel<GELU_ONLY, false>);
-    allow((const void*)grouped_kernel<WITH_GELU, false>);
-    allow((const void*)grouped_kernel<KEEP8, false>);
-    allow((const void*)grouped_kernel<PLAIN, true>);
-    allow((const void*)grouped_dw_kernel);
+    for (int mode = PLAIN; mode <= GRADIENT16; ++mode)
+      for (int kn = 0; kn < 2; ++kn) cudaFuncSetAttribute(row_kernel(mode, kn != 0), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+    cudaFuncSetAttribute((const void*)grouped_dw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM);
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(2 * (gemm_sm_count() / 2)); cfg.blockDim = dim3(DW_THREADS);
-    cfg.dynamicSmemBytes = SMEM; cfg.attrs = at; cfg.numAttrs = 1;
+    cfg.dynamicSmemBytes = DW_SMEM; cfg.attrs = at; cfg.numAttrs = 1;
     int c = 0;
     if (cudaOccupancyMaxActiveClusters(&c, (void*)grouped_dw_kernel, &cfg) == cudaSuccess && c > 0) n = c;
     else { cudaGetLastError(); n = gemm_sm_count() / 2; }
@@ -699,7 +814,7 @@ static int tile_columns(long long tiles_m, int N, int clusters) {
   return 100 * c192 < 95 * c256 ? 192 : 256;
 }
 
-static cudaError_t launch(const void* kernel, long long clusters, int threads, void** args, cudaStream_t stream) {
+static cudaError_t launch(const void* kernel, long long clusters, int threads, size_t smem, void** args, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -707,7 +822,7 @@ static cudaError_t launch(const void* kernel, long long clusters, int threads, v
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // see pdl.cuh
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)(2 * clusters)); cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = SMEM; cfg.stream = stream; cfg.attrs = at; cfg.numAttrs = 2;
+  cfg.dynamicSmemBytes = smem; cfg.stream = stream; cfg.attrs = at; cfg.numAttrs = 2;
   return cudaLaunchKernelExC(&cfg, kernel, args);
 }
 
@@ -721,6 +836,29 @@ static int checked(const int* offsets, int rows, int nexperts, int K, int N, con
   return TMPI_OK;
 }
 
+static int run(Problem p, const void* x, const void* w, const int* offsets, int rows, int nexperts, int K, int N, bool w_is_kn, int mode, cudaStream_t stream) {
+  int st = checked(offsets, rows, nexperts, K, N, "grouped_gemm");
+  if (st) return st;
+  if (!all_aligned16({x, w, p.bias})) return fail(TMPI_ERR_INVALID, "grouped_gemm: tensors must be 16-byte aligned");
+  if (!rows) return TMPI_OK;
+  const int clusters = max_clusters();
+  const long long tiles_m = rows / (2 * BM) + std::min(nexperts, rows);        // at most
+  p.offsets = offsets; p.rows = rows; p.experts = nexperts; p.K = K; p.N = N;
+  p.bn = tile_columns(tiles_m, N, clusters);
+  p.tiles_n = (N + p.bn - 1) / p.bn;
+  p.k_blocks = (K + BK - 1) / BK;
+  p.status = gemm_status_word();
+  CUtensorMap ma, ma_few, mb;
+  if ((st = make_tmap_bf16(&ma, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, BM))) return st;
+  if ((st = make_tmap_bf16(&ma_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW))) return st;
+  if (w_is_kn) st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, BK);
+  else st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, p.bn / 2);
+  if (st) return st;
+  void* args[] = {&ma, &ma_few, &mb, &p};
+  const cudaError_t e = launch(row_kernel(mode, w_is_kn), std::min<long long>(tiles_m * p.tiles_n, clusters), ROW_THREADS, SMEM, args, stream);
+  return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_gemm launch: %s", cudaGetErrorString(e));
+}
+
 }  // namespace grouped
 }  // namespace tmpi
 
@@ -732,45 +870,39 @@ int tmpi_grouped_max_experts(void) { return grouped::MAX_EXPERTS; }
 
 // y [rows, N] = act(x w_e^T + b_e) for x [rows, K] and w [experts, N, K] (w_is_kn: [experts, K, N], without activation), zeros behind the
 // last group; offsets [experts + 1] on the device, or null for one expert.  mode: 0 none; 1 GELU; 2 GELU, and the pre-activation in z; 3 GELU, and
-// the pre-activation's 8-bit checkpoint in z and scale [rows, ceil(N / 32)].  All bf16 but those, on 16-byte boundaries.
+// the pre-activation's 8-bit checkpoint in z and scale [rows, ceil(N / 32)]; 4 none, y in fp32, and rows behind the last group left alone.  All bf16
+// but those, on 16-byte boundaries (fp32: 32).
 int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,
                       int w_is_kn, int mode, void* stream) {
-  int st = grouped::checked(offsets, rows, nexperts, K, N, "grouped_gemm");
-  if (st) return st;
-  if (mode < grouped::PLAIN || mode > grouped::KEEP8 || (w_is_kn && mode) || (mode >= grouped::WITH_GELU && !z) || (mode == grouped::KEEP8 && !scale))
+  if (mode < grouped::PLAIN || mode > grouped::PLAIN32 || (w_is_kn && mode && mode != grouped::PLAIN32) ||
+      ((mode == grouped::WITH_GELU || mode == grouped::KEEP8) && !z) || (mode == grouped::KEEP8 && !scale))
     return fail(TMPI_ERR_INVALID, "grouped_gemm: mode %d", mode);
-  if (!all_aligned16({x, w, bias, y, z})) return fail(TMPI_ERR_INVALID, "grouped_gemm: tensors must be 16-byte aligned");
-  if (!rows) return TMPI_OK;
-  const int clusters = grouped::max_clusters();
-  const long long tiles_m = rows / (2 * gemm2::BM) + std::min(nexperts, rows);        // at most
+  if (!all_aligned16({y, z}) || (mode == grouped::PLAIN32 && (uintptr_t)y % 32)) return fail(TMPI_ERR_INVALID, "grouped_gemm: tensors must be 16-byte aligned");
   grouped::Problem p{};
-  p.offsets = offsets; p.rows = rows; p.experts = nexperts; p.K = K; p.N = N;
-  p.bn = grouped::tile_columns(tiles_m, N, clusters);
-  p.tiles_n = (N + p.bn - 1) / p.bn;
-  p.k_blocks = (K + gemm2::BK - 1) / gemm2::BK;
   p.bias = (const __nv_bfloat16*)bias;
-  p.y = (__nv_bfloat16*)y;
-  p.z = mode == grouped::WITH_GELU ? (__nv_bfloat16*)z : nullptr;
-  p.q = mode == grouped::KEEP8 ? (uint8_t*)z : nullptr;
+  if (mode == grouped::PLAIN32) p.y32 = (float*)y;
+  else p.y = (__nv_bfloat16*)y;
+  p.z = z;
   p.scale = (uint8_t*)scale;
-  p.status = gemm_status_word();
-  CUtensorMap ma, ma_few, mb, my, mz;
-  if ((st = make_tmap_bf16(&ma, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, gemm2::BM))) return st;
-  if ((st = make_tmap_bf16(&ma_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, grouped::FEW))) return st;
-  if (w_is_kn) st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, gemm2::BK);
-  else st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, p.bn / 2);
-  if (st) return st;
-  if ((st = make_tmap_bf16(&my, y, (uint64_t)rows, (uint64_t)N, (uint64_t)N, gemm2::BM))) return st;
-  mz = my;
-  if (p.z && (st = make_tmap_bf16(&mz, z, (uint64_t)rows, (uint64_t)N, (uint64_t)N, gemm2::BM))) return st;
-  const void* kernel = w_is_kn ? (const void*)grouped::grouped_kernel<grouped::PLAIN, true>
-                       : mode == grouped::PLAIN ? (const void*)grouped::grouped_kernel<grouped::PLAIN, false>
-                       : mode == grouped::GELU_ONLY ? (const void*)grouped::grouped_kernel<grouped::GELU_ONLY, false>
-                       : mode == grouped::WITH_GELU ? (const void*)grouped::grouped_kernel<grouped::WITH_GELU, false>
-                                                    : (const void*)grouped::grouped_kernel<grouped::KEEP8, false>;
-  void* args[] = {&ma, &ma_few, &mb, &my, &mz, &p};
-  const cudaError_t e = grouped::launch(kernel, std::min<long long>(tiles_m * p.tiles_n, clusters), gemm2::GROUP_THREADS, args, (cudaStream_t)stream);
-  return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_gemm launch: %s", cudaGetErrorString(e));
+  p.wide = N % 32 == 0 && ((uintptr_t)y | (uintptr_t)z) % 32 == 0;
+  return grouped::run(p, x, w, offsets, rows, nexperts, K, N, w_is_kn != 0, mode, (cudaStream_t)stream);
+}
+
+// The gradients of gelu(z) h's input and value in one product: with g = dy w_e (dy [rows, K], w [experts, K, N]) in fp32 and the kept z [rows, N] (bf16, or
+// with `scale` its 8-bit checkpoint), dz = weight g gelu'(z) and h = weight gelu(z), both bf16 [rows, N]; row_weights fp32 [rows] or null for
+// ones.  dots [rows, ceil(N / 64)] (or null): the sums of g gelu(z) over 64 columns each.  Rows behind the last group are left alone.
+int tmpi_grouped_gelu_gradient(const void* dy, const void* w, const int* offsets, const void* z, const void* scale, const float* row_weights, void* dz, void* h,
+                               float* dots, int rows, int nexperts, int K, int N, void* stream) {
+  if (!all_aligned16({z, dz, h}) || !z || !h) return fail(TMPI_ERR_INVALID, "grouped_gelu_gradient: tensors must be 16-byte aligned");
+  grouped::Problem p{};
+  p.y = (__nv_bfloat16*)dz;
+  p.h = (__nv_bfloat16*)h;
+  p.z = const_cast<void*>(z);
+  p.scale = (uint8_t*)const_cast<void*>(scale);
+  p.row_weights = row_weights;
+  p.dots = dots;
+  p.wide = N % 32 == 0 && ((uintptr_t)dz | (uintptr_t)h | (uintptr_t)z) % 32 == 0;
+  return grouped::run(p, dy, w, offsets, rows, nexperts, K, N, true, scale ? grouped::GRADIENT8 : grouped::GRADIENT16, (cudaStream_t)stream);
 }
 
 // dw [experts, N, K] = dy_e^T x_e and, where given, db [experts, N] = the column sums of dy_e, each row times row_weights[row] where given
@@ -802,7 +934,7 @@ int tmpi_grouped_weight_gradient(const void* dy, const void* x, const int* offse
   if ((st = make_tmap_bf16_3d(&mdw, dw, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, 64))) return st;
   void* args[] = {&mdy, &mx, &mdw, &p};
   const cudaError_t e = grouped::launch((const void*)grouped::grouped_dw_kernel, std::min<long long>((long long)p.tiles_m * p.tiles_n * nexperts, clusters),
-                                        grouped::DW_THREADS, args, (cudaStream_t)stream);
+                                        grouped::DW_THREADS, grouped::DW_SMEM, args, (cudaStream_t)stream);
   return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_weight_gradient launch: %s", cudaGetErrorString(e));
 }
 
