@@ -367,29 +367,40 @@ __device__ __forceinline__ void finish(Sh* sh, const Problem& p, const int* offs
       }
       if (MODE == GELU_ONLY || MODE == WITH_GELU || MODE == KEEP8) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) gelu_value2(v[j], v[j + 1], &v[j], &v[j + 1]);
+        for (int j = 0; j < 32; j += 2)
+          attn_util::unpack2(quick_gelu2(attn_util::pack2(__float_as_uint(v[j]), __float_as_uint(v[j + 1]))), v[j], v[j + 1]);
       }
       if (GRADIENT) {
-        float h[32];
         const float scale = act8::value(kept_scale[half]);
+        const unsigned long long weight2 = attn_util::pack2(__float_as_uint(weight), __float_as_uint(weight));
+        unsigned long long dot2 = 0ull;
+        uint32_t hw[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-          float z0, z1, y0, y1, d0, d1;
+          float z0, z1, a0, a1;
           if (MODE == GRADIENT8) {
             act8::unpack2(kept[half][j >> 2] >> (16 * ((j >> 1) & 1)), scale, &z0, &z1);
           } else {
             z0 = __uint_as_float(zb[j >> 1] << 16);
             z1 = __uint_as_float(zb[j >> 1] & 0xffff0000u);
           }
-          gelu_both2(z0, z1, &y0, &y1, &d0, &d1);
-          if (j < left) dot += v[j] * y0 + v[j + 1] * y1;
-          v[j] = weight * v[j] * d0;
-          v[j + 1] = weight * v[j + 1] * d1;
-          h[j] = weight * y0;
-          h[j + 1] = weight * y1;
+          unsigned long long y, slope;
+          quick_gelu_both2(attn_util::pack2(__float_as_uint(z0), __float_as_uint(z1)), &y, &slope);
+          const unsigned long long g = attn_util::pack2(__float_as_uint(v[j]), __float_as_uint(v[j + 1]));
+          if (j < left) dot2 = attn_util::fma2(g, y, dot2);
+          attn_util::unpack2(attn_util::mul2(attn_util::mul2(g, slope), weight2), a0, a1);
+          w[j >> 1] = attn_util::pack_bf16(__float_as_uint(a0), __float_as_uint(a1));
+          attn_util::unpack2(attn_util::mul2(y, weight2), a0, a1);
+          hw[j >> 1] = attn_util::pack_bf16(__float_as_uint(a0), __float_as_uint(a1));
         }
-        pack_row(h, w);
-        if (mine) store_row(p.h + row_at * N + col, w, left, wide);
+        float a0, a1;
+        attn_util::unpack2(dot2, a0, a1);
+        dot += a0 + a1;
+        if (mine) {
+          store_row(p.h + row_at * N + col, hw, left, wide);
+          store_row(p.y + row_at * N + col, w, left, wide);
+        }
+        continue;
       }
       pack_row(v, w);
       if (mine) store_row(p.y + row_at * N + col, w, left, wide);
