@@ -124,6 +124,26 @@ int make_tmap_bf16_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)
   return TMPI_OK;
 }
 
+// Dense [rows, cols] matrix of 1-, 2- or 4-byte elements (bytes), boxes of box_rows rows x box_cols columns of 64 or 128 bytes with the swizzle of
+// that width; the row pitch a multiple of 16 bytes.
+int make_tmap_box(CUtensorMap* map, int bytes, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(TMPI_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+  if (((uintptr_t)base & 15) || (cols * bytes) % 16) return fail(TMPI_ERR_INVALID, "TMA operand must be 16-byte aligned with a 16-byte multiple row pitch");
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {cols * bytes};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode_in_context([&] {
+    return fn(map, bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
+              const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              box_cols * bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+  if (r != CUDA_SUCCESS) return fail(TMPI_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+  return TMPI_OK;
+}
+
 // Dense [outer, rows, cols] bf16 tensor, boxes of 64 columns x box_rows rows of one outer index: what lies outside the extents of
 // that index's matrix reads as zero and is not written.
 int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows) {

@@ -27,6 +27,7 @@ namespace tmpi {
 
 int make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows);
 int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows);
+int make_tmap_box(CUtensorMap* map, int bytes, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols);
 int gemm_sm_count();
 int* gemm_status_word();
 
@@ -54,23 +55,27 @@ struct Problem {
   const float* row_weights;  // GRADIENT: [rows] or null (ones)
   float* dots;               // GRADIENT: [rows, slices], the sum over 64 columns of gradient times gelu(z); or null
   int wide;                  // every row of y, z, h starts on a 32-byte boundary
+  int q_rows16;              // KEEP8: every row of z starts on a 16-byte boundary, as TMA tiles need
   int* status;
 };
 
-// Four groups of four epilogue warps: a group takes 64 columns of a tile.  With two groups, whose warps met at barriers around TMA stores, a GELU
-// epilogue ran at 1.1 instructions per cycle and SM and was longer than its tile's MMAs: 16384 x 4096 x 1024 127 us with a GELU, 176 with an
-// 8-bit checkpoint beside it, 103 plain.
+// Four groups of four epilogue warps: a group takes 64 columns of a tile, a warp of it 32 rows, which it stages and stores by itself.  With two groups,
+// whose warps met at barriers around the stores, a GELU epilogue ran at 1.1 instructions per cycle and SM and was longer than its tile's MMAs:
+// 16384 x 4096 x 1024 127 us with a GELU, 176 with an 8-bit checkpoint beside it, 103 plain.
 constexpr int ROW_GROUPS = 4, ROW_THREADS = 64 + ROW_GROUPS * 128;
-constexpr int NST = 7;                                  // stages of the operand ring: no staging for the epilogue beside them
+// Stages of the operand ring: a warp has a staging buffer of 32 rows x 64 bytes, or two (one of 128 bytes) where it has two results or fp32.
+__host__ __device__ constexpr int stages_of(int mode) { return mode == PLAIN || mode == GELU_ONLY ? 6 : 5; }
+__host__ __device__ constexpr int staging_of(int mode) { return mode == PLAIN || mode == GELU_ONLY ? 2048 : 4096; }
 
 struct Sh {
-  uint64_t full[NST], empty[NST], acc_full[2], acc_empty[2];
+  uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int error;
   int warp_sums[8];
   int tile_end[MAX_EXPERTS];                            // tiles of the experts up to and with this one
 };
-constexpr size_t SMEM = (size_t)NST * STAGE_BYTES + 1024 + 1280;
+constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + 32768 + 1024 + 1280;
+static_assert(5 * STAGE_BYTES + 16 * 4096 == 6 * STAGE_BYTES + 16 * 2048 && 6 * STAGE_BYTES + 16 * 2048 == STAGES * STAGE_BYTES + 32768, "staging");
 static_assert(sizeof(Sh) <= 1280 && SMEM <= 232448, "shared memory of one CTA");
 
 // Offsets as given, but inside the tensor and not before the group's start: wrong ones give wrong results, never an access outside.
@@ -150,7 +155,7 @@ template <int N>
 __device__ __forceinline__ void advance(Ring* r) { if (++r->stage == N) { r->stage = 0; r->phase ^= 1; } }
 
 // One thread in each CTA.
-template <bool B_MN>
+template <int NST, bool B_MN>
 __device__ __forceinline__ void produce(Sh* sh, unsigned char* tiles, const Problem& p, const int* offsets, const CUtensorMap* ma, const CUtensorMap* ma_few,
                                         const CUtensorMap* mb, uint32_t rank) {
   const int half = p.bn / 2;
@@ -180,7 +185,7 @@ __device__ __forceinline__ void produce(Sh* sh, unsigned char* tiles, const Prob
 }
 
 // One thread of the even CTA.
-template <bool B_MN>
+template <int NST, bool B_MN>
 __device__ __forceinline__ void issue(Sh* sh, unsigned char* tiles, const Problem& p, const int* offsets) {
   const uint32_t idesc = sm100::make_idesc_f16(2 * BM, p.bn, true, B_MN, false);
   Ring ring{0, 0};
@@ -278,18 +283,42 @@ __device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]
 }
 
 // The sixteen epilogue warps of each CTA.  A thread has a row of the tile, and its warp works on 32 of its columns at a time, without a word to
-// the others: results go to memory from registers, 32 bytes a store, so that whole and partial tiles take the same path and no barrier or fence stands
-// in it.  The GELU is that of the fp32 sum, and so is the 8-bit checkpoint, whose blocks of 32 columns a thread has to itself.
+// the others.  A warp whose 32 rows all belong to the group stores through its own staging and the TMA unit, others from registers, row by row.  (Stores of
+// registers, 32 bytes a lane, for all of them: the shared memory's data path, which the MMAs read their operands through, moved 16 bytes a cycle for
+// them; two results of 8192 x 4096 kept it busy half of the time, and the launch took as much longer.)  The GELU is that of the fp32 sum, and so is the
+// 8-bit checkpoint, whose blocks of 32 columns a thread has to itself.
 template <int MODE>
-__device__ __forceinline__ void finish(Sh* sh, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights, uint32_t rank, int group,
-                                       int quarter, int lane) {
+__device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights,
+                                       const CUtensorMap* map_y, const CUtensorMap* map_z, uint32_t rank, int group, int quarter, int lane) {
   constexpr bool GRADIENT = MODE == GRADIENT8 || MODE == GRADIENT16;
   const int row = quarter * 32 + lane, N = p.N, bn = p.bn, slices = (N + SLICE - 1) / SLICE, blocks = (N + 31) / 32;
   const bool wide = p.wide != 0;
   for_tiles(sh, p, offsets, [&](const Unit& u, int it) -> bool {
     const int acc = it & 1, rows = u.part_rows(rank), c0 = group * SLICE, col0 = u.n_blk * bn + c0;
     const bool busy = rows > quarter * 32 && c0 < bn && col0 < N;                 // of this warp
-    const bool mine = busy && row < rows;
+    const bool mine = busy && row < rows, whole = rows >= quarter * 32 + 32;
+    const int warp_row = u.row0 + (int)rank * BM + quarter * 32;
+    // staged results: rows of 64 bytes (128 in fp32), 16-byte pieces permuted as the tensor maps' swizzle has it
+    auto reuse = [&](int pending) {                      // all but the last `pending` stores have been read out of the staging
+      if (lane == 0) {
+        if (pending) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
+      __syncwarp();
+    };
+    auto stage = [&](int buffer, const uint32_t (&w)[16]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4*>(staging + buffer * 2048 + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    };
+    auto send = [&](const CUtensorMap* map, int buffer, int col) {
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        sm100::tma_store_2d(map, staging + buffer * 2048, col, warp_row);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    };
     const long long row_at = (long long)u.row0 + (int)rank * BM + row;
     const __nv_bfloat16* bias = bias_all ? bias_all + (long long)u.e * N : nullptr;
     float weight = 1.f, dot = 0.f;
@@ -312,7 +341,7 @@ __device__ __forceinline__ void finish(Sh* sh, const Problem& p, const int* offs
     auto release = [&] {                                 // the accumulator has been read
       sm100::tc_fence_before();
       __syncwarp();
-      if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&sh->acc_empty[acc], 0));
+      if (lane == 0) sm100::mbar_arrive_cluster_no_stores(sm100::map_to_cta(&sh->acc_empty[acc], 0));
     };
     if (!busy) { release(); return true; }
 #pragma unroll
@@ -345,7 +374,13 @@ __device__ __forceinline__ void finish(Sh* sh, const Problem& p, const int* offs
       }
       uint32_t w[16];
       if (MODE == PLAIN32) {
-        if (mine) {
+        if (whole) {
+          reuse(0);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          send(map_y, 0, col);
+        } else if (mine) {
           float* to = p.y32 + row_at * N + col;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -355,14 +390,26 @@ __device__ __forceinline__ void finish(Sh* sh, const Problem& p, const int* offs
       }
       if (MODE == WITH_GELU) {
         pack_row(v, w);
-        if (mine) store_row((__nv_bfloat16*)p.z + row_at * N + col, w, left, wide);
+        if (whole) {
+          reuse(1);
+          stage(1, w);
+          send(map_z, 1, col);
+        } else if (mine) {
+          store_row((__nv_bfloat16*)p.z + row_at * N + col, w, left, wide);
+        }
       }
       if (MODE == KEEP8) {
         uint32_t q[8];
         const uint32_t byte = act8::pack_block(v, q);    // columns behind N are zeros: the weight's rows there read as zero, and have no bias
-        if (mine) {
+        if (mine) p.scale[row_at * blocks + col / 32] = (uint8_t)byte;
+        if (whole && p.q_rows16) {                       // rows of 64 bytes from both halves
+          if (!half) reuse(0);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            *reinterpret_cast<uint4*>(staging + 2048 + lane * 64 + (((2 * half + j) ^ (lane >> 1 & 3)) << 4)) = make_uint4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+          if (half || left <= 32) send(map_z, 1, col0);
+        } else if (mine) {
           store_row8((uint8_t*)p.z + row_at * N + col, q, left, wide);
-          p.scale[row_at * blocks + col / 32] = (uint8_t)byte;
         }
       }
       if (MODE == GELU_ONLY || MODE == WITH_GELU || MODE == KEEP8) {
@@ -396,18 +443,32 @@ __device__ __forceinline__ void finish(Sh* sh, const Problem& p, const int* offs
         float a0, a1;
         attn_util::unpack2(dot2, a0, a1);
         dot += a0 + a1;
-        if (mine) {
+        if (whole) {
+          reuse(1);
+          stage(1, hw);
+          send(map_z, 1, col);
+          reuse(1);
+          stage(0, w);
+          send(map_y, 0, col);
+        } else if (mine) {
           store_row(p.h + row_at * N + col, hw, left, wide);
           store_row(p.y + row_at * N + col, w, left, wide);
         }
         continue;
       }
       pack_row(v, w);
-      if (mine) store_row(p.y + row_at * N + col, w, left, wide);
+      if (whole) {
+        reuse(MODE == WITH_GELU || (MODE == KEEP8 && p.q_rows16));      // the one store that may be pending is the other buffer's
+        stage(0, w);
+        send(map_y, 0, col);
+      } else if (mine) {
+        store_row(p.y + row_at * N + col, w, left, wide);
+      }
     }
     if (GRADIENT && mine && p.dots) p.dots[row_at * slices + col0 / SLICE] = dot;
     return true;
   });
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   if (MODE == PLAIN || MODE == GELU_ONLY || MODE == WITH_GELU) {      // rows behind the last group
     const long long used = group_of(offsets, p.rows, p.experts - 1).r1;
     const long long chunks = (p.rows - used) * (N / 8);
@@ -420,10 +481,11 @@ __device__ __forceinline__ void finish(Sh* sh, const Problem& p, const int* offs
 template <int MODE, bool B_MN>
 __global__ void __launch_bounds__(ROW_THREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_few, const __grid_constant__ CUtensorMap map_b,
-               const __grid_constant__ Problem p) {
+               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z, const __grid_constant__ Problem p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  Sh* sh = reinterpret_cast<Sh*>(tiles + (size_t)NST * STAGE_BYTES);
+  constexpr int NST = stages_of(MODE);
+  Sh* sh = reinterpret_cast<Sh*>(tiles + (size_t)STAGES * STAGE_BYTES + 32768);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = sm100::cluster_ctarank();
   if (warp == 0 && sm100::elect_one()) {
@@ -451,11 +513,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   if (!p.row_weights) row_weights = nullptr;
   count_tiles(sh, p, offsets);
   if (warp == 0) {
-    if (sm100::elect_one()) produce<B_MN>(sh, tiles, p, offsets, &map_a, &map_a_few, &map_b, rank);
+    if (sm100::elect_one()) produce<NST, B_MN>(sh, tiles, p, offsets, &map_a, &map_a_few, &map_b, rank);
   } else if (warp == 1) {
-    if (rank == 0 && sm100::elect_one()) issue<B_MN>(sh, tiles, p, offsets);
+    if (rank == 0 && sm100::elect_one()) issue<NST, B_MN>(sh, tiles, p, offsets);
   } else {
-    finish<MODE>(sh, p, offsets, bias, row_weights, rank, (warp - 2) >> 2, warp & 3, lane);
+    finish<MODE>(sh, tiles + (size_t)NST * STAGE_BYTES + (warp - 2) * staging_of(MODE), p, offsets, bias, row_weights, &map_y, &map_z, rank, (warp - 2) >> 2, warp & 3, lane);
   }
   __syncwarp();
   // neither CTA frees its tensor memory or exits while the other may still signal its barriers or have the pair's MMAs read its shared memory
@@ -859,13 +921,21 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   p.tiles_n = (N + p.bn - 1) / p.bn;
   p.k_blocks = (K + BK - 1) / BK;
   p.status = gemm_status_word();
-  CUtensorMap ma, ma_few, mb;
+  CUtensorMap ma, ma_few, mb, my, mz;
   if ((st = make_tmap_bf16(&ma, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, BM))) return st;
   if ((st = make_tmap_bf16(&ma_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW))) return st;
   if (w_is_kn) st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, BK);
   else st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, p.bn / 2);
   if (st) return st;
-  void* args[] = {&ma, &ma_few, &mb, &p};
+  // results go in boxes of 32 rows x 64 bytes (128 in fp32): y, and beside it z, h or the e4m3 numbers
+  const bool fp32 = mode == PLAIN32;
+  if ((st = make_tmap_box(&my, fp32 ? 4 : 2, fp32 ? (const void*)p.y32 : p.y, (uint64_t)rows, (uint64_t)N, 32, 32))) return st;
+  mz = my;
+  p.q_rows16 = N % 16 == 0;
+  if (mode == WITH_GELU || mode == GRADIENT8 || mode == GRADIENT16) st = make_tmap_box(&mz, 2, mode == WITH_GELU ? p.z : p.h, (uint64_t)rows, (uint64_t)N, 32, 32);
+  else if (mode == KEEP8 && p.q_rows16) st = make_tmap_box(&mz, 1, p.z, (uint64_t)rows, (uint64_t)N, 32, 64);
+  if (st) return st;
+  void* args[] = {&ma, &ma_few, &mb, &my, &mz, &p};
   const cudaError_t e = launch(row_kernel(mode, w_is_kn), std::min<long long>(tiles_m * p.tiles_n, clusters), ROW_THREADS, SMEM, args, stream);
   return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_gemm launch: %s", cudaGetErrorString(e));
 }

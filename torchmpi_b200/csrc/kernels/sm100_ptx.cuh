@@ -267,6 +267,10 @@ __device__ __forceinline__ uint32_t map_to_cta(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same without waiting for the thread's stores to be visible to the cluster: for what tensor-memory fences order alone.
+__device__ __forceinline__ void mbar_arrive_cluster_no_stores(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // 2-D tiled load into THIS CTA's shared memory whose completion bytes are counted on an mbarrier
 // that may live in the other CTA of the pair (`bar_cluster_addr` from map_to_cta).  No multicast.
 __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, int c0, int c1, uint32_t bar_cluster_addr) {
