@@ -1,6 +1,9 @@
-// Autograd functions of layers of experts and of 8-bit activation checkpoints (ops/experts.py, ops/act8.py), which make the checks.  Rows
-// are flattened by the callers: x is [rows, width] here.  Scratch memory comes from PyTorch's allocator on the calling stream, per call.
+// Autograd functions of layers of experts and of 8-bit activation checkpoints (ops/experts.py, ops/act8.py).  An entry returns nothing (None) for what
+// the kernels do not take, wrong arguments among it: the Python function then raises, or computes with PyTorch's operations.  So a call
+// that the kernels take is looked at once, here (in Python the checks of a layer of experts took 17 us of a call of 39).  Scratch
+// memory comes from PyTorch's allocator on the calling stream, per call.
 #include "common.h"
+#include <c10/cuda/CUDAFunctions.h>
 #include <initializer_list>
 
 namespace tmpi_bind {
@@ -19,30 +22,58 @@ bool wants_grad(std::initializer_list<Tensor> inputs) {
   return false;
 }
 
-struct Kept { Tensor q, scale; };                                   // an 8-bit checkpoint
-
-Kept empty_kept(const Tensor& like, int64_t rows, int64_t cols) {
-  const auto bytes = like.options().dtype(at::kByte);
-  return {at::empty({rows, cols}, bytes), at::empty({rows, (cols + 31) / 32}, bytes)};
+// all on the current device, which there is one of per process
+bool here(std::initializer_list<const Tensor*> tensors) {
+  const int64_t device = c10::cuda::current_device();
+  for (const Tensor* t : tensors)
+    if (t->defined() && !(t->is_cuda() && t->get_device() == device)) return false;
+  return true;
 }
-Kept quantize(const Tensor& x) {
-  Kept k = empty_kept(x, x.size(0), x.size(1));
-  check(tmpi_act8_quantize(x.data_ptr(), k.q.data_ptr(), k.scale.data_ptr(), x.size(0), (int)x.size(1), dtype_code(x.scalar_type()), stream()));
+bool all_of_type(std::initializer_list<const Tensor*> tensors, at::ScalarType type) {
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->scalar_type() != type) return false;
+  return true;
+}
+bool floating(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat; }
+bool shaped(const Tensor& t, std::initializer_list<int64_t> sizes) { return !t.defined() || t.sizes() == at::IntArrayRef(sizes); }
+// [..., cols] as rows
+Tensor rows_of(const Tensor& x) { return x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}); }
+constexpr int64_t MOST = int64_t(1) << 30;                          // rows, columns and entries that the kernels count in 32 bits
+
+struct Kept { Tensor q, scale; };                                   // an 8-bit checkpoint, [..., cols] and [..., ceil(cols / 32)]
+
+Kept empty_kept(const Tensor& like, at::IntArrayRef sizes) {
+  std::vector<int64_t> blocks = sizes.vec();
+  blocks.back() = (blocks.back() + 31) / 32;
+  return {at::empty(sizes, like.options().dtype(at::kFloat8_e4m3fn)), at::empty(blocks, like.options().dtype(at::kByte))};
+}
+Kept quantize(const Tensor& x) {                                    // packed
+  Kept k = empty_kept(x, x.sizes());
+  const int64_t cols = x.size(-1);
+  check(tmpi_act8_quantize(x.data_ptr(), k.q.data_ptr(), k.scale.data_ptr(), x.numel() / cols, (int)cols, dtype_code(x.scalar_type()), stream()));
   launched(ACT8, 1);
   return k;
 }
 Tensor restore(const Kept& k, at::ScalarType type) {
   Tensor x = at::empty(k.q.sizes(), k.q.options().dtype(type));
-  check(tmpi_act8_restore(k.q.data_ptr(), k.scale.data_ptr(), x.data_ptr(), x.size(0), (int)x.size(1), dtype_code(type), stream()));
+  const int64_t cols = x.size(-1);
+  check(tmpi_act8_restore(k.q.data_ptr(), k.scale.data_ptr(), x.data_ptr(), x.numel() / cols, (int)cols, dtype_code(type), stream()));
   launched(ACT8, 1);
   return x;
 }
 std::pair<Tensor, Tensor> gelu_gradient(const Tensor& dy, const Kept& k) {
   Tensor dz = at::empty_like(dy), h = at::empty_like(dy);
-  check(tmpi_act8_gelu_gradient(dy.data_ptr(), k.q.data_ptr(), k.scale.data_ptr(), dz.data_ptr(), h.data_ptr(), dy.size(0), (int)dy.size(1),
+  const int64_t cols = dy.size(-1);
+  check(tmpi_act8_gelu_gradient(dy.data_ptr(), k.q.data_ptr(), k.scale.data_ptr(), dz.data_ptr(), h.data_ptr(), dy.numel() / cols, (int)cols,
                                 dtype_code(dy.scalar_type()), stream()));
   launched(ACT8, 1);
   return {dz, h};
+}
+bool is_kept(const Tensor& q, const Tensor& scale) {
+  if (!(q.scalar_type() == at::kFloat8_e4m3fn && scale.scalar_type() == at::kByte && q.dim() >= 1 && scale.dim() == q.dim() && q.numel() > 0 && q.size(-1) <= MOST)) return false;
+  for (int64_t i = 0; i + 1 < q.dim(); ++i)
+    if (q.size(i) != scale.size(i)) return false;
+  return scale.size(-1) == (q.size(-1) + 31) / 32 && here({&q, &scale});
 }
 
 // ---------------------------------------------------------------- products grouped by expert
@@ -107,7 +138,7 @@ struct GroupedLinearFn : public torch::autograd::Function<GroupedLinearFn> {
 struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w1_, const OptTensor& b1_, const Tensor& w2_, const OptTensor& b2_) {
     const Tensor x = packed(x_), w1 = packed(w1_), w2 = packed(w2_), b1 = b1_.has_value() ? packed(*b1_) : Tensor(), b2 = b2_.has_value() ? packed(*b2_) : Tensor();
-    const Kept kx = quantize(x), kz = empty_kept(x, x.size(0), w1.size(0));
+    const Kept kx = quantize(x), kz = empty_kept(x, {x.size(0), w1.size(0)});
     const Tensor h = grouped(x, w1, b1, Tensor(), false, GELU_AND_Z8, kz.q, kz.scale);
     const Tensor y = matmul_nt(h, w2, b2);
     ctx->save_for_backward({kx.q, kx.scale, kz.q, kz.scale, w1, w2});
@@ -153,9 +184,11 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     ctx->saved_data["k"] = k;
     ctx->saved_data["renormalize"] = renormalize;
     ctx->mark_non_differentiable({chosen, order, place, offsets});
+    ctx->set_materialize_grads(false);                              // or autograd fills a tensor with zeros for each of them
     return {weights, chosen, order, place, offsets};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
     const Tensor logits = saved[0].stride(1) == 1 && (saved[0].size(0) < 2 || saved[0].stride(0) >= saved[0].size(1)) ? saved[0] : saved[0].contiguous();
     const Tensor weights = as_saved(saved[1]), chosen = as_saved(saved[2]), dw = packed(grads[0].to(at::kFloat));
@@ -168,9 +201,14 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
   }
 };
 
-Tensor dispatch(const Tensor& x, const Tensor& order, int64_t tokens, int64_t k) {
-  Tensor out = at::empty({tokens * k, x.size(1)}, x.options());
-  check(tmpi_expert_dispatch(x.data_ptr(), order.data_ptr<int>(), out.data_ptr(), (int)tokens, (int)k, (int)x.size(1), dtype_code(x.scalar_type()), stream()));
+const int* last(const Tensor& offsets) { return offsets.data_ptr<int>() + offsets.numel() - 1; }      // how many places are used
+
+// offsets undefined: rows behind the last entry are left as they are
+Tensor dispatch(const Tensor& x, const Tensor& place, const Tensor& offsets) {
+  const int64_t T = place.size(0), k = place.size(1);
+  Tensor out = at::empty({T * k, x.size(1)}, x.options());
+  check(tmpi_expert_dispatch(x.data_ptr(), place.data_ptr<int>(), offsets.defined() ? last(offsets) : nullptr, out.data_ptr(), (int)T, (int)k, (int)x.size(1),
+                             dtype_code(x.scalar_type()), stream()));
   launched(EXPERTS, 1);
   return out;
 }
@@ -185,10 +223,10 @@ Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place, a
 }
 
 struct DispatchFn : public torch::autograd::Function<DispatchFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& order_, const Tensor& place_) {
-    const Tensor order = order_.contiguous(), place = place_.contiguous();
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& place_, const Tensor& offsets) {
+    const Tensor place = place_.contiguous();
     ctx->save_for_backward({place});
-    return dispatch(packed(x), order, place.size(0), place.size(1));
+    return dispatch(packed(x), place, offsets.contiguous());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
@@ -197,18 +235,18 @@ struct DispatchFn : public torch::autograd::Function<DispatchFn> {
 };
 
 struct CombineFn : public torch::autograd::Function<CombineFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& rows_, const Tensor& weights_, const Tensor& order_, const Tensor& place_) {
-    const Tensor rows = packed(rows_), weights = weights_.contiguous(), order = order_.contiguous(), place = place_.contiguous();
-    ctx->save_for_backward({rows, weights, order});
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows_, const Tensor& weights_, const Tensor& place_, const Tensor& offsets_) {
+    const Tensor rows = packed(rows_), weights = weights_.contiguous(), place = place_.contiguous();
+    ctx->save_for_backward({rows, weights, place, offsets_.contiguous()});
     return combine(rows, weights, place, rows.scalar_type());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor rows = as_saved(saved[0]), weights = as_saved(saved[1]), order = as_saved(saved[2]), dy = packed(grads[0]);
+    const Tensor rows = as_saved(saved[0]), weights = as_saved(saved[1]), place = as_saved(saved[2]), offsets = as_saved(saved[3]), dy = packed(grads[0]);
     const bool need_w = ctx->needs_input_grad(1);
     Tensor drows = at::empty_like(rows), dw;
-    if (need_w) dw = at::zeros_like(weights);
-    check(tmpi_expert_combine_gradient(dy.data_ptr(), need_w ? rows.data_ptr() : nullptr, weights.data_ptr<float>(), 1, order.data_ptr<int>(), nullptr,
+    if (need_w) dw = at::empty_like(weights);
+    check(tmpi_expert_combine_gradient(dy.data_ptr(), need_w ? rows.data_ptr() : nullptr, weights.data_ptr<float>(), 1, place.data_ptr<int>(), nullptr, last(offsets),
                                        drows.data_ptr(), need_w ? dw.data_ptr<float>() : nullptr, nullptr, (int)weights.size(0), (int)weights.size(1),
                                        (int)rows.size(1), 0, dtype_code(rows.scalar_type()), stream()));
     launched(EXPERTS, 1);
@@ -228,14 +266,20 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
                  offsets = offsets_.contiguous(), w1 = packed(w1_), w2 = packed(w2_), b1 = b1_.has_value() ? packed(*b1_) : Tensor(),
                  b2 = b2_.has_value() ? packed(*b2_) : Tensor();
     const int64_t T = place.size(0), k = place.size(1), H = w1.size(1);
-    const Tensor xs = dispatch(x, order, T, k);
+    Tensor xs;
     Kept kx, kz;
     if (keep && act8) {
-      kx = quantize(x);
-      kz = empty_kept(x, T * k, H);
-    } else if (keep) {
-      kx.q = x;
-      kz.q = at::empty({T * k, H}, x.options());
+      kx = empty_kept(x, x.sizes());
+      kz = empty_kept(x, {T * k, H});
+      xs = at::empty({T * k, x.size(1)}, x.options());
+      check(tmpi_expert_dispatch_keep(x.data_ptr(), place.data_ptr<int>(), xs.data_ptr(), kx.q.data_ptr(), kx.scale.data_ptr(), (int)T, (int)k, (int)x.size(1), stream()));
+      launched(EXPERTS, 1);
+    } else {
+      xs = dispatch(x, place, Tensor());
+      if (keep) {
+        kx.q = x;
+        kz.q = at::empty({T * k, H}, x.options());
+      }
     }
     const Tensor h = grouped(xs, w1, b1, offsets, false, !keep ? GELU : act8 ? GELU_AND_Z8 : GELU_AND_Z, kz.q, kz.scale);
     const Tensor y = combine(grouped(h, w2, b2, offsets, false, FP32, Tensor(), Tensor()), weights, place, x.scalar_type());
@@ -255,9 +299,9 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(6), need_b1 = has_b1 && ctx->needs_input_grad(7),
                need_w2 = ctx->needs_input_grad(7 + has_b1), need_b2 = b2.defined() && ctx->needs_input_grad(8 + has_b1);
     const auto f32 = dy.options().dtype(at::kFloat);
-    Tensor dwt = at::zeros({T, k}, f32), by_place = at::empty({T * k}, f32), g = at::empty({T * k, C}, dy.options());
-    check(tmpi_expert_combine_gradient(dy.data_ptr(), ptr(b2), weights.data_ptr<float>(), 0, order.data_ptr<int>(), b2.defined() ? chosen.data_ptr<int>() : nullptr,
-                                       g.data_ptr(), b2.defined() ? dwt.data_ptr<float>() : nullptr, by_place.data_ptr<float>(), (int)T, (int)k, (int)C, (int)E,
+    Tensor dwt = at::empty({T, k}, f32), by_place = at::empty({T * k}, f32), g = at::empty({T * k, C}, dy.options());
+    check(tmpi_expert_combine_gradient(dy.data_ptr(), ptr(b2), weights.data_ptr<float>(), 0, place.data_ptr<int>(), b2.defined() ? chosen.data_ptr<int>() : nullptr,
+                                       nullptr, g.data_ptr(), dwt.data_ptr<float>(), by_place.data_ptr<float>(), (int)T, (int)k, (int)C, (int)E,
                                        dtype_code(dy.scalar_type()), stream()));
     launched(EXPERTS, 1);
     const bool need_wt = ctx->needs_input_grad(1);
@@ -276,10 +320,10 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
       Tensor xs;
       if (kx.scale.defined()) {
         xs = at::empty({T * k, C}, dy.options());
-        check(tmpi_expert_dispatch8(kx.q.data_ptr(), kx.scale.data_ptr(), order.data_ptr<int>(), xs.data_ptr(), (int)T, (int)k, (int)C, stream()));
+        check(tmpi_expert_dispatch8(kx.q.data_ptr(), kx.scale.data_ptr(), place.data_ptr<int>(), xs.data_ptr(), (int)T, (int)k, (int)C, stream()));
         launched(EXPERTS, 1);
       } else {
-        xs = dispatch(kx.q, order, T, k);
+        xs = dispatch(kx.q, place, Tensor());
       }
       grouped_weight_gradient(dz, xs, offsets, Tensor(), E, &dw1, need_b1 ? &db1 : nullptr);
     }
@@ -292,34 +336,77 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
 }  // namespace
 
 void register_experts(pybind11::module_& m) {
-  m.def("act8_quantize", [](const Tensor& x) {
-    const Kept k = quantize(packed(x));
+  using OptPair = c10::optional<std::pair<Tensor, Tensor>>;
+  m.def("act8_quantize", [](const Tensor& x) -> OptPair {
+    if (!(x.is_cuda() && floating(x) && x.dim() >= 1 && x.numel() > 0 && x.size(-1) <= MOST && here({&x}))) return c10::nullopt;
+    const Kept k = quantize(packed(x.detach()));
     return std::make_pair(k.q, k.scale);
   });
-  m.def("act8_restore", [](const Tensor& q, const Tensor& scale, int code) {
+  m.def("act8_restore", [](const Tensor& q, const Tensor& scale, int code) -> OptTensor {
+    if (!(code == TMPI_F32 || code == TMPI_F16 || code == TMPI_BF16) || !q.is_cuda() || !is_kept(q, scale)) return c10::nullopt;
     return restore({packed(q), packed(scale)}, code == TMPI_F32 ? at::kFloat : code == TMPI_F16 ? at::kHalf : at::kBFloat16);
   });
-  m.def("act8_gelu_gradient", [](const Tensor& dy, const Tensor& q, const Tensor& scale) { return gelu_gradient(packed(dy), {packed(q), packed(scale)}); });
-  m.def("act8_mlp", [](const Tensor& x, const Tensor& w1, const OptTensor& b1, const Tensor& w2, const OptTensor& b2) -> Tensor {
-    if (wants_grad({x, w1, w2, or_none(b1), or_none(b2)})) return Mlp8Fn::apply(x, w1, b1, w2, b2);
-    const Tensor h = grouped(packed(x), packed(w1), b1.has_value() ? packed(*b1) : Tensor(), Tensor(), false, GELU, Tensor(), Tensor());
-    return matmul_nt(h, packed(w2), b2.has_value() ? packed(*b2) : Tensor());
+  m.def("act8_gelu_gradient", [](const Tensor& dy, const Tensor& q, const Tensor& scale) -> OptPair {
+    if (!(dy.is_cuda() && floating(dy) && dy.sizes() == q.sizes() && is_kept(q, scale) && here({&dy}))) return c10::nullopt;
+    return gelu_gradient(packed(dy.detach()), {packed(q), packed(scale)});
   });
-  m.def("grouped_linear", [](const Tensor& x, const Tensor& w, const OptTensor& bias, const Tensor& offsets, bool gelu) -> Tensor {
-    if (wants_grad({x, w, or_none(bias)})) return GroupedLinearFn::apply(x, w, bias, offsets, gelu);
-    return grouped(packed(x), packed(w), bias.has_value() ? packed(*bias) : Tensor(), offsets.contiguous(), false, gelu ? GELU : PLAIN, Tensor(), Tensor());
+  m.def("act8_mlp", [](const Tensor& x, const Tensor& w1, const OptTensor& b1_, const Tensor& w2, const OptTensor& b2_) -> OptTensor {
+    const Tensor b1 = or_none(b1_), b2 = or_none(b2_);
+    if (!(x.is_cuda() && x.dim() >= 1 && w1.dim() == 2 && w2.dim() == 2 && all_of_type({&x, &w1, &b1, &w2, &b2}, at::kBFloat16) && here({&x, &w1, &b1, &w2, &b2}))) return c10::nullopt;
+    const int64_t C = w1.size(1), H = w1.size(0), D = w2.size(0), rows = x.size(-1) ? x.numel() / x.size(-1) : 0;
+    if (!(x.size(-1) == C && w2.size(1) == H && shaped(b1, {H}) && shaped(b2, {D}) && C % 8 == 0 && H % 8 == 0 && D % 8 == 0 && C && H && D && rows && rows <= MOST)) return c10::nullopt;
+    const Tensor x2 = rows_of(x);
+    Tensor y;
+    if (wants_grad({x, w1, w2, b1, b2})) {
+      y = Mlp8Fn::apply(x2, w1, b1_, w2, b2_);
+    } else {
+      const Tensor h = grouped(packed(x2), packed(w1), b1.defined() ? packed(b1) : b1, Tensor(), false, GELU, Tensor(), Tensor());
+      y = matmul_nt(h, packed(w2), b2.defined() ? packed(b2) : b2);
+    }
+    if (x.dim() == 2) return y;
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = D;
+    return y.view(shape);
   });
-  m.def("expert_route", [](const Tensor& logits, int64_t k, bool renormalize) {
+  m.def("grouped_linear", [](const Tensor& x, const Tensor& w, const OptTensor& bias_, const Tensor& offsets, bool gelu) -> OptTensor {
+    const Tensor bias = or_none(bias_);
+    if (!(x.is_cuda() && x.dim() == 2 && w.dim() == 3 && all_of_type({&x, &w, &bias}, at::kBFloat16) && offsets.scalar_type() == at::kInt && here({&x, &w, &bias, &offsets}))) return c10::nullopt;
+    const int64_t E = w.size(0), N = w.size(1), K = w.size(2);
+    if (!(x.size(1) == K && shaped(bias, {E, N}) && shaped(offsets, {E + 1}) && K % 8 == 0 && N % 8 == 0 && w.numel() && E <= tmpi_grouped_max_experts() && x.size(0) && x.size(0) <= MOST)) return c10::nullopt;
+    if (wants_grad({x, w, bias})) return GroupedLinearFn::apply(x, w, bias_, offsets, gelu);
+    return grouped(packed(x), packed(w), bias.defined() ? packed(bias) : bias, offsets.contiguous(), false, gelu ? GELU : PLAIN, Tensor(), Tensor());
+  });
+  m.def("expert_route", [](const Tensor& logits, int64_t k, bool renormalize) -> c10::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>> {
+    if (!(logits.is_cuda() && logits.dim() == 2 && floating(logits) && here({&logits}))) return c10::nullopt;
+    int experts = 0, most = 0;
+    check(tmpi_route_limits(&experts, &most));
+    const int64_t T = logits.size(0), E = logits.size(1);
+    if (!(k >= 1 && k <= E && E <= experts && k <= most && T * k <= MOST)) return c10::nullopt;
     const variable_list r = RouteFn::apply(logits, k, renormalize);
     return std::make_tuple(r[0], r[1], r[2], r[3], r[4]);
   });
-  m.def("expert_dispatch", [](const Tensor& x, const Tensor& order, const Tensor& place) { return DispatchFn::apply(x, order, place); });
-  m.def("expert_combine", [](const Tensor& rows, const Tensor& weights, const Tensor& order, const Tensor& place) {
-    return CombineFn::apply(rows, weights, order, place);
+  m.def("expert_dispatch", [](const Tensor& x, const Tensor& place, const Tensor& offsets) -> OptTensor {
+    if (!(x.is_cuda() && x.dim() == 2 && floating(x) && x.numel() && place.dim() == 2 && offsets.dim() == 1 && offsets.size(0) >= 1 && all_of_type({&place, &offsets}, at::kInt) &&
+          here({&x, &place, &offsets}) && place.size(0) == x.size(0) && place.numel() && place.numel() <= MOST && x.size(1) <= MOST)) return c10::nullopt;
+    return DispatchFn::apply(x, place, offsets);
+  });
+  m.def("expert_combine", [](const Tensor& rows, const Tensor& weights, const Tensor& place, const Tensor& offsets) -> OptTensor {
+    if (!(rows.is_cuda() && rows.dim() == 2 && floating(rows) && rows.numel() && place.dim() == 2 && offsets.dim() == 1 && offsets.size(0) >= 1 && all_of_type({&place, &offsets}, at::kInt) &&
+          weights.scalar_type() == at::kFloat && weights.sizes() == place.sizes() && here({&rows, &weights, &place, &offsets}) && place.numel() == rows.size(0) && place.numel() <= MOST &&
+          rows.size(1) <= MOST)) return c10::nullopt;
+    return CombineFn::apply(rows, weights, place, offsets);
   });
   m.def("expert_mlp", [](const Tensor& x, const Tensor& weights, const Tensor& chosen, const Tensor& order, const Tensor& place, const Tensor& offsets,
-                         const Tensor& w1, const OptTensor& b1, const Tensor& w2, const OptTensor& b2, bool act8) {
-    return ExpertsFn::apply(x, weights, chosen, order, place, offsets, w1, b1, w2, b2, act8, wants_grad({x, weights, w1, w2, or_none(b1), or_none(b2)}));
+                         const Tensor& w1, const OptTensor& b1_, const Tensor& w2, const OptTensor& b2_, bool act8) -> OptTensor {
+    const Tensor b1 = or_none(b1_), b2 = or_none(b2_);
+    if (!(x.is_cuda() && x.dim() >= 1 && w1.dim() == 3 && w2.dim() == 3 && place.dim() == 2 && all_of_type({&x, &w1, &b1, &w2, &b2}, at::kBFloat16) &&
+          all_of_type({&chosen, &order, &place, &offsets}, at::kInt) && weights.scalar_type() == at::kFloat &&
+          here({&x, &weights, &chosen, &order, &place, &offsets, &w1, &b1, &w2, &b2}))) return c10::nullopt;
+    const int64_t E = w1.size(0), H = w1.size(1), C = w1.size(2), T = place.size(0), k = place.size(1);
+    if (!(x.size(-1) == C && x.numel() == T * C && shaped(weights, {T, k}) && shaped(chosen, {T, k}) && shaped(order, {T * k}) && shaped(offsets, {E + 1}) && shaped(w2, {E, C, H}) &&
+          shaped(b1, {E, H}) && shaped(b2, {E, C}) && C % 8 == 0 && H % 8 == 0 && w1.numel() && E <= tmpi_grouped_max_experts() && T && T * k && T * k <= MOST)) return c10::nullopt;
+    const Tensor y = ExpertsFn::apply(rows_of(x), weights, chosen, order, place, offsets, w1, b1_, w2, b2_, act8, wants_grad({x, weights, w1, w2, b1, b2}));
+    return x.dim() == 2 ? y : y.view(x.sizes());
   });
 }
 

@@ -1,10 +1,10 @@
 // Rows on their way to the experts and back: dispatch (a token's row to each of its experts' places), combine (the weighted sum of
 // what the experts made of it) and their gradients.
 //
-// `order` (route.cu) gives the entry token * k + j at each place, `place` the place of each entry.  All passes read and write each element once
-// and are bound by memory.  Passes without a sum over a row give a thread one 16-byte piece of a row, so that one token of a long row is
+// `place` (route.cu) gives the place of each entry token * k + j, `order` the entry at each place.  All passes go by tokens, read and write each
+// element once, and are bound by memory.  Passes without a sum over a row give a thread one 16-byte piece of a row, so that one token of a long row is
 // spread over many blocks; those with one give a warp a row.  Sums are in fp32, in one order whatever the launch: nothing is accumulated
-// by atomics.
+// by atomics.  Places behind the last entry (from *used on) get zeros where the caller asks for it.
 #include "act8.cuh"
 #include "pdl.cuh"
 #include "vec.cuh"
@@ -32,87 +32,114 @@ __device__ __forceinline__ int token_at(const int* __restrict__ order, int s, in
   const int e = order[s];
   return e >= 0 && e / k < tokens ? e / k : -1;
 }
-
-// out[s] = x[token of s], zeros where there is none
+// zeros in the places from *used on; all threads of the grid
 template <typename T, int V>
-__global__ void __launch_bounds__(THREADS) dispatch_kernel(const T* __restrict__ x, const int* __restrict__ order, T* __restrict__ out, int places, int tokens,
-                                                           int k, int cols) {
-  wait_previous(x, order);
+__device__ __forceinline__ void clear_rest(const int* __restrict__ used, T* __restrict__ rows, int places, int cols) {
+  if (!used) return;
+  const int first = min(max(*used, 0), places);
+  Pack<T, V> zero;
+#pragma unroll
+  for (int e = 0; e < V; ++e) zero.v[e] = from_acc<T>(0);
+  const long long n = (long long)(places - first) * (cols / V);
+  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < n; i += (long long)gridDim.x * THREADS) st_pack<T, V>(rows + (long long)first * cols + i * V, zero);
+}
+
+// out[place of each of a token's entries] = x[token]
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS) dispatch_kernel(const T* __restrict__ x, const int* __restrict__ place, const int* __restrict__ used, T* __restrict__ out,
+                                                           int places, int tokens, int k, int cols) {
+  wait_previous(x, place, used);
   const int parts = cols / V;
-  const long long items = (long long)places * parts, stride = (long long)gridDim.x * THREADS;
-  constexpr int U = 4;
+  const long long items = (long long)tokens * parts, stride = (long long)gridDim.x * THREADS;
+  constexpr int U = 2;
   for (long long i0 = (long long)blockIdx.x * THREADS + threadIdx.x; i0 < items; i0 += U * stride) {
     Pack<T, V> v[U];
-    long long row[U];
+    long long t[U];
     int part[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long i = i0 + u * stride;
-      if (i >= items) { row[u] = -1; continue; }
-      split(i, parts, &row[u], &part[u]);
-      const int t = token_at(order, (int)row[u], k, tokens);
-      if (t >= 0) {
-        v[u] = ld_pack<T, V>(x + (long long)t * cols + part[u] * V);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[u].v[e] = from_acc<T>(0);
+      t[u] = -1;
+      if (i0 + u * stride < items) {
+        split(i0 + u * stride, parts, &t[u], &part[u]);
+        v[u] = ld_pack<T, V>(x + t[u] * cols + part[u] * V);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (row[u] >= 0) st_pack<T, V>(out + row[u] * cols + part[u] * V, v[u]);
+      if (t[u] >= 0)
+        for (int j = 0; j < k; ++j) {
+          const int s = place[t[u] * k + j];
+          if (s >= 0 && s < places) st_pack<T, V>(out + (long long)s * cols + part[u] * V, v[u]);
+        }
+  }
+  clear_rest<T, V>(used, out, places, cols);
+}
+
+// The same for bf16 rows of a multiple of 8 columns, with the 8-bit checkpoint of x beside it: four threads hold the 32 elements of a block.
+__global__ void __launch_bounds__(THREADS) dispatch_keep_kernel(const __nv_bfloat16* __restrict__ x, const int* __restrict__ place, __nv_bfloat16* __restrict__ out,
+                                                                uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int places, int tokens, int k, int cols) {
+  wait_previous(x, place);
+  const int blocks = (cols + act8::BLOCK - 1) / act8::BLOCK, parts = blocks * (act8::BLOCK / 8);      // the last block of a row padded
+  const long long items = (long long)tokens * parts, stride = (long long)gridDim.x * THREADS;
+  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; (i & ~31LL) < items; i += stride) {
+    long long t = 0;
+    int part = parts;
+    if (i < items) split(i, parts, &t, &part);
+    const bool in = part * 8 < cols;
+    const uint4 v = in ? *reinterpret_cast<const uint4*>(x + t * cols + part * 8) : make_uint4(0u, 0u, 0u, 0u);
+    if (in)
+      for (int j = 0; j < k; ++j) {
+        const int s = place[t * k + j];
+        if (s >= 0 && s < places) *reinterpret_cast<uint4*>(out + (long long)s * cols + part * 8) = v;
+      }
+    const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+    float f[8];
+    uint32_t a = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[2 * e] = __uint_as_float(b[e] << 16);
+      f[2 * e + 1] = __uint_as_float(b[e] & 0xffff0000u);
+      a = max(a, max(act8::magnitude(f[2 * e]), act8::magnitude(f[2 * e + 1])));
+    }
+    a = max(a, __shfl_xor_sync(~0u, a, 1));
+    a = max(a, __shfl_xor_sync(~0u, a, 2));
+    const uint32_t byte = act8::scale_byte(a);
+    if (in) *reinterpret_cast<uint2*>(q + t * cols + part * 8) = act8::pack8(f, act8::inverse(byte));
+    if (i < items && (part & 3) == 0) scale[t * blocks + part / 4] = (uint8_t)byte;
   }
 }
 
-// The same from the 8-bit checkpoint of x, in bf16.  A thread restores eight elements.
-template <bool VEC>
-__global__ void __launch_bounds__(THREADS) dispatch8_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, const int* __restrict__ order,
+// The dispatch of what an 8-bit checkpoint of x stands for, bf16 rows of a multiple of 8 columns.  A thread restores eight elements.
+__global__ void __launch_bounds__(THREADS) dispatch8_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, const int* __restrict__ place,
                                                             __nv_bfloat16* __restrict__ out, int places, int tokens, int k, int cols) {
-  wait_previous(q, scale, order);
-  const int parts = (cols + 7) / 8, blocks = (cols + act8::BLOCK - 1) / act8::BLOCK;
-  const long long items = (long long)places * parts, stride = (long long)gridDim.x * THREADS;
-  constexpr int U = 4;
+  wait_previous(q, scale, place);
+  const int parts = cols / 8, blocks = (cols + act8::BLOCK - 1) / act8::BLOCK;
+  const long long items = (long long)tokens * parts, stride = (long long)gridDim.x * THREADS;
+  constexpr int U = 2;
   for (long long i0 = (long long)blockIdx.x * THREADS + threadIdx.x; i0 < items; i0 += U * stride) {
     uint2 v[U];
     uint32_t s[U];
-    long long row[U];
+    long long t[U];
     int part[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long i = i0 + u * stride;
-      row[u] = -1;
-      part[u] = 0;
-      v[u] = make_uint2(0u, 0u);
-      s[u] = 1;
-      if (i >= items) continue;
-      split(i, parts, &row[u], &part[u]);
-      const int t = token_at(order, (int)row[u], k, tokens);
-      if (t < 0) continue;
-      s[u] = scale[(long long)t * blocks + (part[u] >> 2)];
-      const uint8_t* from = q + (long long)t * cols + part[u] * 8;
-      if (VEC) {
-        v[u] = *reinterpret_cast<const uint2*>(from);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (part[u] * 8 + e < cols) (e < 4 ? v[u].x : v[u].y) |= (uint32_t)from[e] << (8 * (e & 3));
-      }
+      t[u] = -1;
+      if (i0 + u * stride >= items) continue;
+      split(i0 + u * stride, parts, &t[u], &part[u]);
+      v[u] = *reinterpret_cast<const uint2*>(q + t[u] * cols + part[u] * 8);
+      s[u] = scale[t[u] * blocks + (part[u] >> 2)];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (row[u] < 0) continue;
+      if (t[u] < 0) continue;
       float f[8];
       act8::unpack8(v[u], act8::value(s[u]), f);
-      __nv_bfloat16* to = out + row[u] * cols + part[u] * 8;
-      if (VEC) {
-        Pack<__nv_bfloat16, 8> o;
+      Pack<__nv_bfloat16, 8> o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o.v[e] = __float2bfloat16_rn(f[e]);
-        st_pack<__nv_bfloat16, 8>(to, o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (part[u] * 8 + e < cols) to[e] = __float2bfloat16_rn(f[e]);
+      for (int e = 0; e < 8; ++e) o.v[e] = __float2bfloat16_rn(f[e]);
+      for (int j = 0; j < k; ++j) {
+        const int at = place[t[u] * k + j];
+        if (at >= 0 && at < places) st_pack<__nv_bfloat16, 8>(out + (long long)at * cols + part[u] * 8, o);
       }
     }
   }
@@ -137,21 +164,21 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const R* __restrict__ 
     for (int j0 = 0; j0 < k; j0 += U) {
       Pack<R, V> v[U];
       float w[U];
-      bool there[U];
+      int s[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        there[u] = false;
-        w[u] = 0.f;
-        if (j0 + u >= k) continue;
-        const int s = place[t * k + j0 + u];
-        w[u] = weights ? weights[t * k + j0 + u] : 1.f;
-        there[u] = s >= 0 && s < places;
-        if (there[u]) v[u] = ld_pack<R, V>(rows + (long long)s * cols + part * V);
+        s[u] = j0 + u < k ? place[t * k + j0 + u] : -1;
+        w[u] = j0 + u < k ? weights ? weights[t * k + j0 + u] : 1.f : 0.f;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
+        if ((unsigned)s[u] < (unsigned)places) v[u] = ld_pack<R, V>(rows + (long long)s[u] * cols + part * V);
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum[e] += w[u] * (there[u] ? (float)to_acc<R>(v[u].v[e]) : 0.f);
+      for (int u = 0; u < U; ++u) {
+        const bool there = (unsigned)s[u] < (unsigned)places;
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] += w[u] * (there ? (float)to_acc<R>(v[u].v[e]) : 0.f);
+      }
     }
     Pack<T, V> o;
 #pragma unroll
@@ -160,58 +187,65 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const R* __restrict__ 
   }
 }
 
-// The gradients of combine, a warp to a place: drows[s] = weight dy[token] (without `scaled` dy[token] itself), and
-// dweights[entry] = dy[token] . other, where other is rows[s] or, with `chosen`, the row of the entry's expert (its bias).  Places without an
-// entry get zeros; dweights of entries without a place are left to the caller.  place_weights: the weight of the entry at each place.
+// The gradients of combine, a warp to a token: drows[place] = weight dy[token] (without `scaled` dy[token] itself), and
+// dweights[entry] = dy[token] . other, where other is rows[place] or, with `chosen`, the row of the entry's expert (its bias); 0 for entries without a
+// place, and without `other`.  place_weights: the weight of the entry at each place.
 template <typename T, int V>
-__global__ void __launch_bounds__(THREADS) combine_gradient_kernel(const T* __restrict__ dy, const T* __restrict__ other, const float* __restrict__ weights,
-                                                                   const int* __restrict__ order, const int* __restrict__ chosen, T* __restrict__ drows,
-                                                                   float* __restrict__ dweights, float* __restrict__ place_weights, int scaled,
+__global__ void __launch_bounds__(THREADS, 3) combine_gradient_kernel(const T* __restrict__ dy, const T* __restrict__ other, const float* __restrict__ weights,
+                                                                   const int* __restrict__ place, const int* __restrict__ chosen, const int* __restrict__ used,
+                                                                   T* __restrict__ drows, float* __restrict__ dweights, float* __restrict__ place_weights, int scaled,
                                                                    int places, int tokens, int k, int cols, int nexperts) {
-  wait_previous(dy, other, weights, order, chosen);
+  wait_previous(dy, other, weights, place, chosen, used);
   const int lane = threadIdx.x & 31, parts = cols / V;
-  for (long long s = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); s < places; s += (long long)gridDim.x * WARPS) {
-    const int t = token_at(order, (int)s, k, tokens), entry = t >= 0 ? order[s] : 0;
-    const float w = t >= 0 && weights ? weights[entry] : 1.f;
-    const T* o = other;
-    if (other && t >= 0) {
-      const int e = chosen ? chosen[entry] : 0;
-      o = chosen ? (e >= 0 && e < nexperts ? other + (long long)e * cols : nullptr) : other + s * cols;
-    }
-    float dot = 0.f;
-    for (int c0 = lane; c0 < parts; c0 += 4 * 32) {
-      Pack<T, V> g[4], b[4];
+  for (long long t = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); t < tokens; t += (long long)gridDim.x * WARPS) {
+    constexpr int U = 4;                                  // pieces of dy that a lane holds at a time
+    for (int c0 = lane; c0 - lane < parts; c0 += U * 32) {
+      const bool first = c0 == lane, last = c0 - lane + U * 32 >= parts;
+      Pack<T, V> g[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int c = c0 + 32 * u;
-        if (c < parts && t >= 0) {
-          g[u] = ld_pack<T, V>(dy + (long long)t * cols + c * V);
-          if (o) b[u] = ld_pack<T, V>(o + (long long)c * V);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) g[u].v[e] = b[u].v[e] = from_acc<T>(0);
+      for (int u = 0; u < U; ++u)
+        if (c0 + 32 * u < parts) g[u] = ld_pack<T, V>(dy + t * cols + (long long)(c0 + 32 * u) * V);
+      for (int j = 0; j < k; ++j) {
+        const long long entry = t * k + j;
+        const int s = place[entry];
+        if (s < 0 || s >= places) {
+          if (dweights && first && lane == 0) dweights[entry] = 0.f;
+          continue;
         }
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int c = c0 + 32 * u;
-        if (c >= parts) break;
-        Pack<T, V> out;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float f = (float)to_acc<T>(g[u].v[e]);
-          if (o) dot += f * (float)to_acc<T>(b[u].v[e]);
-          out.v[e] = scaled ? from_acc<T>((typename AccOf<T>::type)(w * f)) : g[u].v[e];
+        const float w = weights ? weights[entry] : 1.f;
+        const T* o = other;
+        if (other) {
+          const int e = chosen ? chosen[entry] : 0;
+          o = chosen ? (e >= 0 && e < nexperts ? other + (long long)e * cols : nullptr) : other + (long long)s * cols;
         }
-        st_pack<T, V>(drows + s * cols + (long long)c * V, out);
+        Pack<T, V> b[U];
+        if (o) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c0 + 32 * u < parts) b[u] = ld_pack<T, V>(o + (long long)(c0 + 32 * u) * V);
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (c0 + 32 * u >= parts) break;
+          Pack<T, V> out;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float f = (float)to_acc<T>(g[u].v[e]);
+            if (o) dot += f * (float)to_acc<T>(b[u].v[e]);
+            out.v[e] = scaled ? from_acc<T>((typename AccOf<T>::type)(w * f)) : g[u].v[e];
+          }
+          st_pack<T, V>(drows + (long long)s * cols + (long long)(c0 + 32 * u) * V, out);
+        }
+        if (dweights) {
+          if (o) dot = warp_sum(dot);
+          if (lane == 0) dweights[entry] = first ? dot : dweights[entry] + dot;      // the parts of a long row, in their order
+        }
+        if (place_weights && last && lane == 0) place_weights[s] = w;
       }
-    }
-    if (place_weights && lane == 0) place_weights[s] = t >= 0 ? w : 0.f;
-    if (dweights) {
-      dot = warp_sum(dot);
-      if (lane == 0 && t >= 0) dweights[entry] = dot;
     }
   }
+  clear_rest<T, V>(used, drows, places, cols);
 }
 
 // dweights[entry] += the sum of the entry's row of `dots` (grouped.cu: a number for 64 columns), a warp to a place
@@ -263,27 +297,36 @@ using namespace tmpi;
 
 extern "C" {
 
-// out [tokens * k, cols] from x [tokens, cols]
-int tmpi_expert_dispatch(const void* x, const int* order, void* out, int tokens, int k, int cols, int dtype, void* stream) {
+// out [tokens * k, cols] from x [tokens, cols]; used (optional): places from *used on get zeros
+int tmpi_expert_dispatch(const void* x, const int* place, const int* used, void* out, int tokens, int k, int cols, int dtype, void* stream) {
   const int st = experts::checked(tokens, k, cols, dtype, "expert_dispatch");
   if (st || !tokens) return st;
-  const int places = tokens * k;
   return experts::finish(experts::by_type(dtype, cols, {x, out}, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
-    return launch_overlapped(experts::dispatch_kernel<T, V>, experts::grid_items((long long)places * (cols / V), 4, 8), experts::THREADS, 0, (cudaStream_t)stream,
-                             (const T*)x, order, (T*)out, places, tokens, k, cols);
+    return launch_overlapped(experts::dispatch_kernel<T, V>, experts::grid_items((long long)tokens * (cols / V), 2, 8), experts::THREADS, 0, (cudaStream_t)stream,
+                             (const T*)x, place, used, (T*)out, tokens * k, tokens, k, cols);
   }), "expert_dispatch");
 }
 
-// The same from an 8-bit checkpoint of x, in bf16
-int tmpi_expert_dispatch8(const void* q, const void* scale, const int* order, void* out, int tokens, int k, int cols, void* stream) {
+// The same for bf16, and x's 8-bit checkpoint in q [tokens, cols], scale [tokens, ceil(cols / 32)]; cols a multiple of 8, 16-byte boundaries
+int tmpi_expert_dispatch_keep(const void* x, const int* place, void* out, void* q, void* scale, int tokens, int k, int cols, void* stream) {
+  const int st = experts::checked(tokens, k, cols, TMPI_BF16, "expert_dispatch_keep");
+  if (st || !tokens) return st;
+  if (cols % 8 || !all_aligned16({x, out}) || ((uintptr_t)q & 7)) return fail(TMPI_ERR_INVALID, "expert_dispatch_keep: rows must be multiples of 16 bytes, on 16-byte boundaries");
+  const long long items = (long long)tokens * ((cols + 31) / 32) * 4;
+  return experts::finish(launch_overlapped(experts::dispatch_keep_kernel, experts::grid_items(items, 1, 8), experts::THREADS, 0, (cudaStream_t)stream,
+                                           (const __nv_bfloat16*)x, place, (__nv_bfloat16*)out, (uint8_t*)q, (uint8_t*)scale, tokens * k, tokens, k, cols),
+                         "expert_dispatch_keep");
+}
+
+// out [tokens * k, cols] bf16 from the 8-bit checkpoint of x; cols a multiple of 8
+int tmpi_expert_dispatch8(const void* q, const void* scale, const int* place, void* out, int tokens, int k, int cols, void* stream) {
   const int st = experts::checked(tokens, k, cols, TMPI_BF16, "expert_dispatch8");
   if (st || !tokens) return st;
-  const int places = tokens * k;
-  const auto kernel = cols % 8 == 0 && !((uintptr_t)q & 7) && all_aligned16({out}) ? experts::dispatch8_kernel<true> : experts::dispatch8_kernel<false>;
-  return experts::finish(launch_overlapped(kernel, experts::grid_items((long long)places * ((cols + 7) / 8), 4, 8), experts::THREADS, 0, (cudaStream_t)stream,
-                                           (const uint8_t*)q, (const uint8_t*)scale, order, (__nv_bfloat16*)out, places, tokens, k, cols), "expert_dispatch8");
+  if (cols % 8 || ((uintptr_t)q & 7) || !all_aligned16({out})) return fail(TMPI_ERR_INVALID, "expert_dispatch8: rows must be multiples of 16 bytes, on 16-byte boundaries");
+  return experts::finish(launch_overlapped(experts::dispatch8_kernel, experts::grid_items((long long)tokens * (cols / 8), 2, 8), experts::THREADS, 0, (cudaStream_t)stream,
+                                           (const uint8_t*)q, (const uint8_t*)scale, place, (__nv_bfloat16*)out, tokens * k, tokens, k, cols), "expert_dispatch8");
 }
 
 // y [tokens, cols] of `dtype` from rows [tokens * k, cols] of `dtype`, or in fp32 (rows_fp32: y bf16); weights [tokens, k] or null
@@ -299,26 +342,25 @@ int tmpi_expert_combine(const void* rows, int rows_fp32, const float* weights, c
                              (const R*)rows, weights, place, (T*)y, tokens, tokens * k, k, cols);
   };
   if (rows_fp32) {
-    const bool wide = cols % 4 == 0 && all_aligned16({rows, y});
-    return experts::finish(wide ? go(float(), __nv_bfloat16(), std::integral_constant<int, 4>()) : go(float(), __nv_bfloat16(), std::integral_constant<int, 1>()),
+    const bool wide = cols % 8 == 0 && (uintptr_t)rows % 32 == 0 && all_aligned16({y});
+    return experts::finish(wide ? go(float(), __nv_bfloat16(), std::integral_constant<int, 8>()) : go(float(), __nv_bfloat16(), std::integral_constant<int, 1>()),
                            "expert_combine");
   }
   return experts::finish(experts::by_type(dtype, cols, {rows, y}, [&](auto t, auto v) { return go(t, t, v); }), "expert_combine");
 }
 
-// drows [tokens * k, cols] and, where given, dweights [tokens * k] (of the entries that have a place) from dy [tokens, cols].  other: rows
-// [tokens * k, cols], or with `chosen` a row for each of nexperts experts; null: no dweights.  scaled: drows holds weight times dy, else
-// dy.  place_weights [tokens * k] (optional): the weights in the order of the places.
-int tmpi_expert_combine_gradient(const void* dy, const void* other, const float* weights, int scaled, const int* order, const int* chosen, void* drows,
+// drows [tokens * k, cols] and, where given, dweights [tokens * k] from dy [tokens, cols].  other: rows [tokens * k, cols], or with `chosen` a row for
+// each of nexperts experts; null: dweights gets zeros.  scaled: drows holds weight times dy, else dy.  place_weights [tokens * k]
+// (optional): the weights in the order of the places.  used (optional): rows of drows from *used on get zeros.
+int tmpi_expert_combine_gradient(const void* dy, const void* other, const float* weights, int scaled, const int* place, const int* chosen, const int* used, void* drows,
                                  float* dweights, float* place_weights, int tokens, int k, int cols, int nexperts, int dtype, void* stream) {
   const int st = experts::checked(tokens, k, cols, dtype, "expert_combine_gradient");
   if (st || !tokens) return st;
-  if (dweights && !other) return fail(TMPI_ERR_INVALID, "expert_combine_gradient: dweights without the rows");
   return experts::finish(experts::by_type(dtype, cols, {dy, other, drows}, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
-    return launch_overlapped(experts::combine_gradient_kernel<T, V>, experts::grid_rows(tokens * k, 8), experts::THREADS, 0, (cudaStream_t)stream, (const T*)dy,
-                             (const T*)other, weights, order, chosen, (T*)drows, dweights, place_weights, scaled, tokens * k, tokens, k, cols, nexperts);
+    return launch_overlapped(experts::combine_gradient_kernel<T, V>, experts::grid_rows(tokens, 8), experts::THREADS, 0, (cudaStream_t)stream, (const T*)dy,
+                             (const T*)other, weights, place, chosen, used, (T*)drows, dweights, place_weights, scaled, tokens * k, tokens, k, cols, nexperts);
   }), "expert_combine_gradient");
 }
 

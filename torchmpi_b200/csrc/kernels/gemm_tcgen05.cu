@@ -144,19 +144,19 @@ int make_tmap_box(CUtensorMap* map, int bytes, const void* base, uint64_t rows, 
   return TMPI_OK;
 }
 
-// Dense [outer, rows, cols] bf16 tensor, boxes of 64 columns x box_rows rows of one outer index: what lies outside the extents of
-// that index's matrix reads as zero and is not written.
-int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+// Dense [outer, rows, cols] bf16 tensor, boxes of box_cols (64, or 32) columns x box_rows rows of one outer index, with the swizzle of their
+// width: what lies outside the extents of that index's matrix reads as zero and is not written.
+int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(TMPI_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
   if (((uintptr_t)base & 15) || (cols * 2) % 16) return fail(TMPI_ERR_INVALID, "TMA operand must be 16-byte aligned with a 16-byte multiple row pitch");
   cuuint64_t d[3] = {cols, rows, outer};
   cuuint64_t strides[2] = {cols * 2, cols * rows * 2};
-  cuuint32_t b[3] = {64, box_rows, 1};
+  cuuint32_t b[3] = {box_cols, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = encode_in_context([&] {
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), d, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+              box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   });
   if (r != CUDA_SUCCESS) return fail(TMPI_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
   return TMPI_OK;

@@ -26,7 +26,7 @@
 namespace tmpi {
 
 int make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows);
-int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows);
+int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols);
 int make_tmap_box(CUtensorMap* map, int bytes, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols);
 int gemm_sm_count();
 int* gemm_status_word();
@@ -36,8 +36,7 @@ namespace grouped {
 using namespace gemm2;
 constexpr int MAX_EXPERTS = 256;
 constexpr int FEW = 32;                                 // rows of the smaller box of x
-constexpr int EPI_THREADS = GROUPS * 128;
-constexpr int SLICE = 64, SLICE_BYTES = BM * SLICE * 2;
+constexpr int SLICE = 64;                               // columns of a tile that an epilogue warp takes
 
 // PLAIN32: the sum in fp32.  GRADIENT8 / 16: the sum is the gradient of a GELU's value, whose input z was kept in 8 bits or in bf16.
 enum { PLAIN = 0, GELU_ONLY = 1, WITH_GELU = 2, KEEP8 = 3, PLAIN32 = 4, GRADIENT8 = 5, GRADIENT16 = 6 };
@@ -213,15 +212,6 @@ __device__ __forceinline__ void issue(Sh* sh, unsigned char* tiles, const Proble
     sm100::umma_commit_pair(sm100::map_to_cta(&sh->acc_full[acc], 1));
     return true;
   });
-}
-
-// Whether the wait succeeded for all `threads` threads that share the named barrier: they go on, or leave, together.
-template <int THREADS_>
-__device__ __forceinline__ bool all_of(uint32_t ok, int barrier) {
-  uint32_t all;
-  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-               : "=r"(all) : "r"(ok), "r"(barrier), "n"(THREADS_) : "memory");
-  return all != 0;
 }
 
 // n 32-bit words to or from consecutive addresses: 32 bytes at once where rows start on such a boundary (a whole sector of L2 per lane), else 16 or 8.
@@ -546,8 +536,10 @@ struct DwProblem {
   int* status;
 };
 
-constexpr int DW_THREADS = GROUP_THREADS + 32;          // and the warp that clears rows of other groups
+constexpr int EPI_THREADS = ROW_GROUPS * 128;
+constexpr int DW_THREADS = ROW_THREADS + 32;            // and the warp that clears rows of other groups
 constexpr int DB_GROUPS = EPI_THREADS / (BM / 8);
+static_assert(EPI_THREADS * 8 * 4 <= 32768, "the sums' exchange in the staging");
 
 struct DwSh {
   Shared s;
@@ -586,7 +578,7 @@ __device__ __forceinline__ void dw_setup(DwSh* sh, int warp, const CUtensorMap* 
       sm100::mbar_init(&sh->tail[s], 1);
       sm100::mbar_init(&sh->cleared[s], 1);
     }
-    for (int a = 0; a < 2; ++a) { sm100::mbar_init(&sh->s.acc_full[a], 1); sm100::mbar_init(&sh->s.acc_empty[a], 8 * GROUPS); }
+    for (int a = 0; a < 2; ++a) { sm100::mbar_init(&sh->s.acc_full[a], 1); sm100::mbar_init(&sh->s.acc_empty[a], 8 * ROW_GROUPS); }
     sh->s.error = 0;
     sm100::fence_barrier_init();
   }
@@ -696,21 +688,18 @@ __device__ __forceinline__ void dw_issue(DwSh* shl, unsigned char* tiles, const 
   });
 }
 
-// 64 columns of a row as bf16
-__device__ __forceinline__ void to_bf16(const uint32_t (&r)[2][32], uint32_t (&w)[32]) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j) w[j] = attn_util::pack_bf16(r[j >> 4][2 * (j & 15)], r[j >> 4][2 * (j & 15) + 1]);
+// whether it holds for all epilogue threads
+__device__ __forceinline__ bool all_of(bool ok) {
+  uint32_t all;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, 3, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(all) : "r"((uint32_t)ok), "n"(EPI_THREADS) : "memory");
+  return all != 0;
 }
-__device__ __forceinline__ void stage_row(unsigned char* stg_row, int row, const uint32_t (&w)[32]) {
-#pragma unroll
-  for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(stg_row + ((u ^ (row & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
-}
-
 __device__ __forceinline__ void all_sync() { asm volatile("bar.sync 3, %0;" ::"n"(EPI_THREADS) : "memory"); }
 
-// The sums of 128 columns of dY from col0 over the rows [r0, r1), by all epilogue threads; thread `row` of group 0 has column col0 + row.  Sixteen threads
-// share eight columns, each with 16-byte loads of every 16th row, eight in flight, which are added as a tree; a value passes 3 additions in its batch, one
-// for every 128 rows and 4 among the threads.  part: 8 KB of group 0's staging, which its last store has read.
+// The sums of 128 columns of dY from col0 over the rows [r0, r1), by all epilogue threads; thread `row` of group 0 has column col0 + row.  Thirty-two
+// threads share eight columns, each with 16-byte loads of every 32nd row, eight in flight, which are added as a tree; a value passes 3 additions in its batch,
+// one for every 256 rows and 5 among the threads.  part: 16 KB of the warps' staging, which their last stores have read.
 template <bool WEIGHTS>
 __device__ __forceinline__ float column_sums(const DwProblem& p, const __nv_bfloat16* dy, const float* weights, float* part, int col0, int r0, int r1, int group, int row) {
   constexpr int U = 8, STEP = DB_GROUPS;
@@ -745,78 +734,85 @@ __device__ __forceinline__ float column_sums(const DwProblem& p, const __nv_bflo
   float s[8];
 #pragma unroll
   for (int w = 0; w < 4; ++w) attn_util::unpack2(acc[w], s[2 * w], s[2 * w + 1]);
-  if (e == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // thread 0 is group 0's leader only where it issued the stores (see finish)
-  all_sync();                          // and the sums of the unit before have been read
+  if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  all_sync();
   float4* to = reinterpret_cast<float4*>(part + e * 8);
   to[0] = make_float4(s[0], s[1], s[2], s[3]);
   to[1] = make_float4(s[4], s[5], s[6], s[7]);
   all_sync();
-  if (group) return 0.f;
   float t[DB_GROUPS];
+  if (group == 0) {
 #pragma unroll
-  for (int g = 0; g < DB_GROUPS; ++g) t[g] = part[g * BM + row];
+    for (int g = 0; g < DB_GROUPS; ++g) t[g] = part[g * BM + row];
 #pragma unroll
-  for (int n = DB_GROUPS / 2; n; n /= 2)
+    for (int n = DB_GROUPS / 2; n; n /= 2)
 #pragma unroll
-    for (int g = 0; g < n; ++g) t[g] += t[g + n];
-  return t[0];
+      for (int g = 0; g < n; ++g) t[g] += t[g + n];
+  }
+  all_sync();                          // the staging is the warps' own again
+  return group ? 0.f : t[0];
 }
 
-__device__ __forceinline__ void dw_finish(DwSh* shl, unsigned char* staging, const DwProblem& p, const int* offsets, const CUtensorMap* mdw, const __nv_bfloat16* dy,
+__device__ __forceinline__ void dw_finish(DwSh* shl, unsigned char* staging_all, const DwProblem& p, const int* offsets, const CUtensorMap* mdw, const __nv_bfloat16* dy,
                                           const float* row_weights, uint32_t rank, int group, int quarter, int lane) {
   Shared* sh = &shl->s;
-  const int row = quarter * 32 + lane, bn = p.bn;
-  const bool leader = (int)threadIdx.x - 64 == group * 128;
-  unsigned char* stg = staging + group * SLICE_BYTES;
+  const int row = quarter * 32 + lane, bn = p.bn, c0 = group * SLICE;
+  unsigned char* staging = staging_all + ((int)(threadIdx.x >> 5) - 2) * 2048;      // 32 rows x 64 bytes of this warp
   int it = 0;
   for_units(p, offsets, rank, [&](const DwUnit& u) -> bool {
-    const int row0 = u.m_blk * BM;
+    const int row0 = u.m_blk * BM, col0 = u.n_blk * bn + c0, warp_row = row0 + quarter * 32;
     if (p.db && u.n_blk == 0) {
-      const float sum = row_weights ? column_sums<true>(p, dy, row_weights, reinterpret_cast<float*>(staging), row0, u.r0, u.r1, group, row)
-                                    : column_sums<false>(p, dy, row_weights, reinterpret_cast<float*>(staging), row0, u.r0, u.r1, group, row);
+      const float sum = row_weights ? column_sums<true>(p, dy, row_weights, reinterpret_cast<float*>(staging_all), row0, u.r0, u.r1, group, row)
+                                    : column_sums<false>(p, dy, row_weights, reinterpret_cast<float*>(staging_all), row0, u.r0, u.r1, group, row);
       if (group == 0 && row0 + row < p.N) p.db[(long long)u.e * p.N + row0 + row] = __float2bfloat16_rn(sum);
     }
     const int acc = it & 1;
     if (u.k_blocks) {
-      const uint32_t ok = sm100::mbar_wait(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs) && !sh->error;
-      if (!all_of<EPI_THREADS>(ok, 3)) { give_up(sh, p.status, 44); return false; }
+      bool ok = sm100::mbar_wait_warp(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs, &sh->error);
+      if (p.db) ok = all_of(ok);                         // where the warps meet for the sums, they go on, or leave, together
+      if (!ok) { give_up(sh, p.status, 44); return false; }
       ++it;
       sm100::tc_fence_after();
     }
-    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * BN;
-#pragma unroll 1
-    for (int c0 = group * SLICE; c0 < bn && u.n_blk * bn + c0 < p.K; c0 += GROUPS * SLICE) {
-      uint32_t w[32];
+    const bool busy = c0 < bn && col0 < p.K && warp_row < p.N;
+    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * BN + c0;
+    auto release = [&] {
+      if (!u.k_blocks) return;
+      sm100::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive_cluster_no_stores(sm100::map_to_cta(&sh->acc_empty[acc], 0));
+    };
+    if (!busy) { release(); return true; }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half && col0 + 32 >= p.K) { release(); break; }
+      uint32_t w[16];
       if (u.k_blocks) {
-        uint32_t r[2][32];
-        sm100::tmem_ld_32x32(t_base + c0, r[0]);
-        sm100::tmem_ld_32x32(t_base + c0 + 32, r[1]);
+        uint32_t r[32];
+        sm100::tmem_ld_32x32(t_base + 32 * half, r);
         sm100::tmem_ld_wait();
-        to_bf16(r, w);
+        if (half) release();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = attn_util::pack_bf16(r[2 * j], r[2 * j + 1]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) w[j] = 0u;
+        for (int j = 0; j < 16; ++j) w[j] = 0u;
       }
-      if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      group_sync(group);
-      stage_row(stg + row * 128, row, w);
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4*>(staging + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
       sm100::fence_proxy_async_smem();
-      group_sync(group);
-      if (leader) {
-        const int col0 = u.n_blk * bn + c0;
-        if (row0 < p.N) sm100::tma_store_3d(mdw, stg, col0, row0, u.e);
-        if (row0 + 64 < p.N) sm100::tma_store_3d(mdw, stg + SLICE_BYTES / 2, col0, row0 + 64, u.e);
+      __syncwarp();
+      if (lane == 0) {
+        sm100::tma_store_3d(mdw, staging, col0 + 32 * half, warp_row, u.e);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
-    if (u.k_blocks) {
-      sm100::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&sh->acc_empty[acc], 0));
-    }
     return true;
   });
-  if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(DW_THREADS, 1)
@@ -840,7 +836,7 @@ grouped_dw_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_const
     if (sm100::elect_one()) dw_produce(sh, tiles, p, offsets, &map_dy, &map_x, rank);
   } else if (warp == 1) {
     if (rank == 0 && sm100::elect_one()) dw_issue(sh, tiles, p, offsets);
-  } else if (warp < 2 + 4 * GROUPS) {
+  } else if (warp < 2 + 4 * ROW_GROUPS) {
     dw_finish(sh, staging, p, offsets, &map_dw, dy, row_weights, rank, (warp - 2) >> 2, warp & 3, lane);
   } else {
     dw_clear(sh, tiles, p, offsets, rank, lane);
@@ -924,8 +920,8 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   CUtensorMap ma, ma_few, mb, my, mz;
   if ((st = make_tmap_bf16(&ma, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, BM))) return st;
   if ((st = make_tmap_bf16(&ma_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW))) return st;
-  if (w_is_kn) st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, BK);
-  else st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, p.bn / 2);
+  if (w_is_kn) st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, BK, 64);
+  else st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, p.bn / 2, 64);
   if (st) return st;
   // results go in boxes of 32 rows x 64 bytes (128 in fp32): y, and beside it z, h or the e4m3 numbers
   const bool fp32 = mode == PLAIN32;
@@ -1012,7 +1008,7 @@ int tmpi_grouped_weight_gradient(const void* dy, const void* x, const int* offse
   CUtensorMap mdy, mx, mdw;
   if ((st = make_tmap_bf16(&mdy, dy, (uint64_t)rows, (uint64_t)N, (uint64_t)N, gemm2::BK))) return st;
   if ((st = make_tmap_bf16(&mx, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, gemm2::BK))) return st;
-  if ((st = make_tmap_bf16_3d(&mdw, dw, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, 64))) return st;
+  if ((st = make_tmap_bf16_3d(&mdw, dw, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, 32, 32))) return st;
   void* args[] = {&mdy, &mx, &mdw, &p};
   const cudaError_t e = grouped::launch((const void*)grouped::grouped_dw_kernel, std::min<long long>((long long)p.tiles_m * p.tiles_n * nexperts, clusters),
                                         grouped::DW_THREADS, grouped::DW_SMEM, args, (cudaStream_t)stream);

@@ -20,10 +20,9 @@ import torch
 import torch.nn.functional as F
 
 from .. import _native
-from .._lib import dtype_code, has_symbol
+from .._lib import DTYPES
 
 BLOCK = 32          # elements that share a scale
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
 class Act8(NamedTuple):
@@ -46,10 +45,6 @@ def same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     d = devices.pop()
     if d.type == "cuda" and d.index != torch.cuda.current_device():
         raise ValueError(f"{what}: tensors on {d}, but the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _takes(x: torch.Tensor) -> bool:
-    return x.is_cuda and x.dtype in _FLOATS and x.numel() > 0 and has_symbol("tmpi_act8_quantize")
 
 
 def _two_to(e: torch.Tensor) -> torch.Tensor:
@@ -86,26 +81,27 @@ def _checked(what: str, a: Act8) -> None:
 
 def quantize(x: torch.Tensor) -> Act8:
     """The checkpoint of ``x [..., C]``; not differentiable."""
+    if x.is_cuda:
+        kept = _native.ext().act8_quantize(x)          # None: nothing for the kernel
+        if kept is not None:
+            return Act8(*kept)
     if x.dim() < 1 or not x.dtype.is_floating_point:
         raise ValueError(f"quantize expects a floating tensor with at least one dimension, got {x.dtype} {tuple(x.shape)}")
     same_device("quantize", x)
-    x = x.detach()
-    if not _takes(x):
-        return _quantize(x)
-    q, scale = _native.ext().act8_quantize(x.reshape(-1, x.shape[-1]))
-    return Act8(q.view(torch.float8_e4m3fn).view(x.shape), scale.view(x.shape[:-1] + (-1,)))
+    return _quantize(x.detach())
 
 
 def dequantize(a: Act8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """What the checkpoint stands for, rounded to ``dtype`` (exact in bf16 and fp32 within their range)."""
+    if a[0].is_cuda:
+        x = _native.ext().act8_restore(a[0], a[1], DTYPES.get(dtype, -1))
+        if x is not None:
+            return x
     _checked("dequantize", a)
     same_device("dequantize", *a)
     if not dtype.is_floating_point:
         raise ValueError(f"dequantize: {dtype} is not a floating type")
-    if not (a.q.is_cuda and dtype in _FLOATS and a.q.numel() and has_symbol("tmpi_act8_restore")):
-        return _dequantize(a, dtype)
-    C = a.q.shape[-1]
-    return _native.ext().act8_restore(a.q.reshape(-1, C), a.scale.reshape(-1, a.scale.shape[-1]), dtype_code(dtype)).view(a.q.shape)
+    return _dequantize(a, dtype)
 
 
 def _gelu_parts(z: torch.Tensor):
@@ -115,17 +111,16 @@ def _gelu_parts(z: torch.Tensor):
 
 def gelu_gradient(dy: torch.Tensor, a: Act8) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(dy * gelu'(z), gelu(z))`` (erf form) for the values ``z`` of the checkpoint ``a``, both of ``dy``'s dtype."""
+    if dy.is_cuda:
+        both = _native.ext().act8_gelu_gradient(dy, a[0], a[1])
+        if both is not None:
+            return both
     _checked("gelu_gradient", a)
     if dy.shape != a.q.shape or not dy.dtype.is_floating_point:
         raise ValueError(f"gelu_gradient: a gradient of {dy.dtype} {tuple(dy.shape)} for a checkpoint of {tuple(a.q.shape)}")
     same_device("gelu_gradient", dy, *a)
-    dy = dy.detach()
-    if not _takes(dy):
-        h, slope = _gelu_parts(_dequantize(a, torch.float32))
-        return (dy.float() * slope).to(dy.dtype), h.to(dy.dtype)
-    C = dy.shape[-1]
-    dz, h = _native.ext().act8_gelu_gradient(dy.reshape(-1, C), a.q.reshape(-1, C), a.scale.reshape(-1, a.scale.shape[-1]))
-    return dz.view(dy.shape), h.view(dy.shape)
+    h, slope = _gelu_parts(_dequantize(a, torch.float32))
+    return (dy.detach().float() * slope).to(dy.dtype), h.to(dy.dtype)
 
 
 class _Mlp(torch.autograd.Function):
@@ -148,17 +143,16 @@ class _Mlp(torch.autograd.Function):
 def mlp(x: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor], w2: torch.Tensor, b2: Optional[torch.Tensor]) -> torch.Tensor:
     """``gelu(x @ w1.T + b1) @ w2.T + b2`` for ``x [..., C]``, ``w1 [H, C]``, ``w2 [D, H]``; where gradients are wanted, ``x`` and the
     pre-activation are kept in 8 bits.  The checkpoint is that of the fp32 sums, and the GELU is formed from them too."""
+    if x.is_cuda:
+        y = _native.ext().act8_mlp(x, w1, b1, w2, b2)
+        if y is not None:
+            return y
     if not (w1.dim() == 2 and w2.dim() == 2 and x.dim() >= 1 and x.shape[-1] == w1.shape[1] and w2.shape[1] == w1.shape[0]
             and (b1 is None or b1.shape == w1.shape[:1]) and (b2 is None or b2.shape == w2.shape[:1])):
         raise ValueError("mlp expects x [..., C], w1 [H, C], b1 [H], w2 [D, H] and b2 [D]")
     tensors = [t for t in (x, w1, b1, w2, b2) if t is not None]
     same_device("mlp", *tensors)
-    x2 = x.reshape(-1, x.shape[-1])
-    if all(t.is_cuda and t.dtype == torch.bfloat16 for t in tensors) and x2.numel() > 0 and not any(n % 8 for n in w1.shape + w2.shape) \
-            and all(w1.shape) and all(w2.shape) and has_symbol("tmpi_grouped_gemm"):
-        y = _native.ext().act8_mlp(x2, w1, b1, w2, b2)
-    else:
-        if len({t.dtype for t in tensors}) > 1 or not x.dtype.is_floating_point:
-            raise ValueError(f"mlp: tensors of one floating dtype are expected, got {sorted({str(t.dtype) for t in tensors})}")
-        y = _Mlp.apply(x2, w1, b1, w2, b2)
+    if len({t.dtype for t in tensors}) > 1 or not x.dtype.is_floating_point:
+        raise ValueError(f"mlp: tensors of one floating dtype are expected, got {sorted({str(t.dtype) for t in tensors})}")
+    y = _Mlp.apply(x.reshape(-1, x.shape[-1]), w1, b1, w2, b2)
     return y.view(x.shape[:-1] + w2.shape[:1])

@@ -20,12 +20,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import _native
-from .._lib import has_symbol, lib, TorchMPIError
+from .._lib import lib, TorchMPIError
 from . import act8 as _act8
 from .act8 import same_device
-
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
-MAX_EXPERTS, MAX_K = 256, 32          # of the kernels
 
 
 class Routing(NamedTuple):
@@ -147,12 +144,13 @@ def route(logits: torch.Tensor, k: int, renormalize: bool = True) -> Routing:
     """The ``k`` largest of each token's ``logits [T, E]``, largest first, of equal ones that with the lowest index.  The weights are the softmax over
     the chosen logits, or (``renormalize=False``) over all of the token's.  An expert whose logit is -inf is never used, so a
     token may get fewer than ``k``, and one without any gets none (a padded position).  NaN is not chosen either, and makes the token's weights NaN."""
+    if logits.is_cuda:
+        r = _native.ext().expert_route(logits, k, renormalize)          # None: nothing for the kernel
+        if r is not None:
+            return Routing(*r)
     if logits.dim() != 2 or not logits.dtype.is_floating_point or not 1 <= k <= logits.shape[1]:
         raise ValueError(f"route expects floating logits [T, E] and 1 <= k <= E, got {logits.dtype} {tuple(logits.shape)} and k = {k}")
     same_device("route", logits)
-    T, E = logits.shape
-    if logits.is_cuda and logits.dtype in _FLOATS and E <= MAX_EXPERTS and k <= MAX_K and T * k <= 1 << 30 and has_symbol("tmpi_route"):
-        return Routing(*_native.ext().expert_route(logits, k, renormalize))
     return _route(logits, k, renormalize)
 
 
@@ -167,43 +165,44 @@ def _check_routing(what: str, r: Routing, tokens: Optional[int] = None) -> None:
 
 def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """``x [T, C]`` -> ``[T * k, C]``: the token's row at each place, zeros behind the last."""
+    if x.is_cuda:
+        rows = _native.ext().expert_dispatch(x, routing.place, routing.offsets)
+        if rows is not None:
+            return rows
     if x.dim() != 2 or not x.dtype.is_floating_point:
         raise ValueError(f"dispatch expects floating rows [T, C], got {x.dtype} {tuple(x.shape)}")
     _check_routing("dispatch", routing, x.shape[0])
-    same_device("dispatch", x, routing.order, routing.place)
-    if x.is_cuda and x.dtype in _FLOATS and x.numel() and has_symbol("tmpi_expert_dispatch"):
-        return _native.ext().expert_dispatch(x, routing.order, routing.place)
+    same_device("dispatch", x, routing.order, routing.place, routing.offsets)
     return _dispatch(x, routing.order, routing.place.shape[1])
 
 
 def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
     """``rows [T * k, C]`` -> ``[T, C]``: each token's rows times their weights, added in fp32 and rounded once."""
+    if rows.is_cuda:
+        y = _native.ext().expert_combine(rows, routing.weights, routing.place, routing.offsets)
+        if y is not None:
+            return y
     if rows.dim() != 2 or not rows.dtype.is_floating_point or rows.shape[0] != routing.order.shape[0]:
         raise ValueError(f"combine expects floating rows [T * k, C], got {rows.dtype} {tuple(rows.shape)}")
     _check_routing("combine", routing)
     same_device("combine", rows, *routing)
-    if rows.is_cuda and rows.dtype in _FLOATS and rows.numel() and has_symbol("tmpi_expert_combine"):
-        return _native.ext().expert_combine(rows, routing.weights, routing.order, routing.place)
     return _combine(rows, routing.weights, routing.place)
-
-
-def _product_takes(experts: int, *tensors: Optional[torch.Tensor]) -> bool:
-    return (experts <= MAX_EXPERTS and has_symbol("tmpi_grouped_gemm")
-            and all(t is None or (t.is_cuda and t.dtype == torch.bfloat16) for t in tensors))
 
 
 def grouped_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], offsets: torch.Tensor, gelu: bool = False) -> torch.Tensor:
     """``y[r] = gelu?(x[r] @ w[e].T + bias[e])`` for ``offsets[e] <= r < offsets[e + 1]``: ``x [R, K]``, ``w [E, N, K]``, ``bias [E, N]`` or None,
     ``offsets [E + 1]`` int32, ascending, with 0 first.  Groups may be empty; rows of ``x`` behind the last group give zeros and get no gradient.
     The kernel cannot refuse offsets that do not ascend (that would wait for the GPU): it stays inside the tensors, and its results mean nothing."""
+    if x.is_cuda:
+        y = _native.ext().grouped_linear(x, w, bias, offsets, gelu)
+        if y is not None:
+            return y
     if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2] or (bias is not None and bias.shape != w.shape[:2]) \
             or offsets.shape != (w.shape[0] + 1,) or offsets.dtype != torch.int32 or w.shape[0] < 1:
         raise ValueError("grouped_linear expects x [R, K], w [E, N, K], bias [E, N] and int32 offsets [E + 1]")
     if not x.dtype.is_floating_point or w.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise ValueError(f"grouped_linear: tensors of one floating dtype are expected, got {x.dtype}, {w.dtype}")
     same_device("grouped_linear", x, w, bias, offsets)
-    if _product_takes(w.shape[0], x, w, bias) and x.shape[1] % 8 == 0 and w.shape[1] % 8 == 0 and w.numel() and x.shape[0]:
-        return _native.ext().grouped_linear(x, w, bias, offsets, gelu)
     return _grouped(x, w, bias, offsets, gelu)
 
 
@@ -212,6 +211,10 @@ def mlp(x: torch.Tensor, routing: Routing, w1: torch.Tensor, b1: Optional[torch.
     """The weighted sum over a token's experts of ``gelu(x @ w1[e].T + b1[e]) @ w2[e].T + b2[e]``: ``x [..., C]`` with the routing of its ``T`` rows,
     ``w1 [E, H, C]``, ``b1 [E, H]``, ``w2 [E, C, H]``, ``b2 [E, C]``.  Kept for backward are ``x`` and the pre-activations, with ``act8`` in 8 bits
     (``ops.act8``), and no dispatched rows; the backward pass forms everything else from those."""
+    if x.is_cuda:
+        y = _native.ext().expert_mlp(x, *routing, w1, b1, w2, b2, act8)
+        if y is not None:
+            return y
     if not (w1.dim() == 3 and w2.dim() == 3 and x.dim() >= 1 and x.shape[-1] == w1.shape[2] and w2.shape == (w1.shape[0], w1.shape[2], w1.shape[1])
             and (b1 is None or b1.shape == w1.shape[:2]) and (b2 is None or b2.shape == w2.shape[:2])):
         raise ValueError("mlp expects x [..., C], w1 [E, H, C], b1 [E, H], w2 [E, C, H] and b2 [E, C]")
@@ -223,9 +226,7 @@ def mlp(x: torch.Tensor, routing: Routing, w1: torch.Tensor, b1: Optional[torch.
     if routing.offsets.shape[0] != w1.shape[0] + 1:
         raise ValueError(f"mlp: weights of {w1.shape[0]} experts for a routing to {routing.offsets.shape[0] - 1}")
     same_device("mlp", *tensors, *routing)
-    if _product_takes(w1.shape[0], *tensors) and w1.shape[1] % 8 == 0 and w1.shape[2] % 8 == 0 and w1.numel() and x2.shape[0]:
-        y = _native.ext().expert_mlp(x2, *routing, w1, b1, w2, b2, act8)
-    elif act8:
+    if act8:
         y = _Mlp8.apply(x2, routing.weights, w1, b1, w2, b2, *routing[2:])
     else:
         h = grouped_linear(dispatch(x2, routing), w1, b1, routing.offsets, gelu=True)
