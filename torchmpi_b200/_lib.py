@@ -221,12 +221,12 @@ _CUDA_PROTOS = {
     "tmpi_route_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmpi_route": (_i, [_vp, _i64, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "tmpi_route_gradient": (_i, [_vp, _i64, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
-    "tmpi_expert_dispatch": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "tmpi_expert_dispatch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "tmpi_expert_dispatch_keep": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "tmpi_expert_dispatch8": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "tmpi_expert_combine": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
-    "tmpi_expert_combine_gradient": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
-    "tmpi_expert_dots": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
+    "tmpi_expert_combine_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "tmpi_expert_weight_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "tmpi_grouped_max_experts": (_i, []),
     "tmpi_grouped_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "tmpi_grouped_gelu_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),

@@ -203,11 +203,12 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
 
 const int* last(const Tensor& offsets) { return offsets.data_ptr<int>() + offsets.numel() - 1; }      // how many places are used
 
-// offsets undefined: rows behind the last entry are left as they are
-Tensor dispatch(const Tensor& x, const Tensor& place, const Tensor& offsets) {
+// offsets undefined: rows behind the last entry are left as they are; by_place: receives the weights in the order of the places
+Tensor dispatch(const Tensor& x, const Tensor& place, const Tensor& offsets, const Tensor& weights = Tensor(), const Tensor& by_place = Tensor()) {
   const int64_t T = place.size(0), k = place.size(1);
   Tensor out = at::empty({T * k, x.size(1)}, x.options());
-  check(tmpi_expert_dispatch(x.data_ptr(), place.data_ptr<int>(), offsets.defined() ? last(offsets) : nullptr, out.data_ptr(), (int)T, (int)k, (int)x.size(1),
+  check(tmpi_expert_dispatch(x.data_ptr(), place.data_ptr<int>(), offsets.defined() ? last(offsets) : nullptr, weights.defined() ? weights.data_ptr<float>() : nullptr, out.data_ptr(),
+                             by_place.defined() ? by_place.data_ptr<float>() : nullptr, (int)T, (int)k, (int)x.size(1),
                              dtype_code(x.scalar_type()), stream()));
   launched(EXPERTS, 1);
   return out;
@@ -246,9 +247,9 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
     const bool need_w = ctx->needs_input_grad(1);
     Tensor drows = at::empty_like(rows), dw;
     if (need_w) dw = at::empty_like(weights);
-    check(tmpi_expert_combine_gradient(dy.data_ptr(), need_w ? rows.data_ptr() : nullptr, weights.data_ptr<float>(), 1, place.data_ptr<int>(), nullptr, last(offsets),
-                                       drows.data_ptr(), need_w ? dw.data_ptr<float>() : nullptr, nullptr, (int)weights.size(0), (int)weights.size(1),
-                                       (int)rows.size(1), 0, dtype_code(rows.scalar_type()), stream()));
+    check(tmpi_expert_combine_gradient(dy.data_ptr(), need_w ? rows.data_ptr() : nullptr, weights.data_ptr<float>(), place.data_ptr<int>(), last(offsets),
+                                       drows.data_ptr(), need_w ? dw.data_ptr<float>() : nullptr, (int)weights.size(0), (int)weights.size(1), (int)rows.size(1),
+                                       dtype_code(rows.scalar_type()), stream()));
     launched(EXPERTS, 1);
     return {drows, dw, Tensor(), Tensor()};
   }
@@ -260,9 +261,9 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
 // dy . (w2 h + b2) is (w2^T dy) . h + dy . b2, of which the first product is there anyway.  What a token's experts return, and the gradients
 // that they return to it, are handed over in fp32 and rounded once, as their sum.
 struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weights_, const Tensor& chosen_, const Tensor& order_, const Tensor& place_,
-                        const Tensor& offsets_, const Tensor& w1_, const OptTensor& b1_, const Tensor& w2_, const OptTensor& b2_, bool act8, bool keep) {
-    const Tensor x = packed(x_), weights = weights_.contiguous(), chosen = chosen_.contiguous(), order = order_.contiguous(), place = place_.contiguous(),
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weights_, const Tensor& chosen_, const Tensor& place_, const Tensor& offsets_,
+                        const Tensor& w1_, const OptTensor& b1_, const Tensor& w2_, const OptTensor& b2_, bool act8, bool keep) {
+    const Tensor x = packed(x_), weights = weights_.contiguous(), chosen = chosen_.contiguous(), place = place_.contiguous(),
                  offsets = offsets_.contiguous(), w1 = packed(w1_), w2 = packed(w2_), b1 = b1_.has_value() ? packed(*b1_) : Tensor(),
                  b2 = b2_.has_value() ? packed(*b2_) : Tensor();
     const int64_t T = place.size(0), k = place.size(1), H = w1.size(1);
@@ -284,7 +285,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     const Tensor h = grouped(xs, w1, b1, offsets, false, !keep ? GELU : act8 ? GELU_AND_Z8 : GELU_AND_Z, kz.q, kz.scale);
     const Tensor y = combine(grouped(h, w2, b2, offsets, false, FP32, Tensor(), Tensor()), weights, place, x.scalar_type());
     if (keep) {
-      ctx->save_for_backward({kx.q, kx.scale, kz.q, kz.scale, weights, chosen, order, place, offsets, w1, w2, b2});
+      ctx->save_for_backward({kx.q, kx.scale, kz.q, kz.scale, weights, chosen, place, offsets, w1, w2, b2});
       ctx->saved_data["b1"] = b1.defined();
     }
     return y;
@@ -292,26 +293,24 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Kept kx{as_saved(saved[0]), as_saved(saved[1])}, kz{as_saved(saved[2]), as_saved(saved[3])};
-    const Tensor weights = as_saved(saved[4]), chosen = as_saved(saved[5]), order = as_saved(saved[6]), place = as_saved(saved[7]), offsets = as_saved(saved[8]),
-                 w1 = as_saved(saved[9]), w2 = as_saved(saved[10]), b2 = as_saved(saved[11]), dy = packed(grads[0]);
+    const Tensor weights = as_saved(saved[4]), chosen = as_saved(saved[5]), place = as_saved(saved[6]), offsets = as_saved(saved[7]), w1 = as_saved(saved[8]),
+                 w2 = as_saved(saved[9]), b2 = as_saved(saved[10]), dy = packed(grads[0]);
     const int64_t T = place.size(0), k = place.size(1), C = dy.size(1), H = w1.size(1), E = w1.size(0);
     const bool has_b1 = ctx->saved_data["b1"].toBool();                 // an absent bias has no number among the inputs
-    const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(6), need_b1 = has_b1 && ctx->needs_input_grad(7),
-               need_w2 = ctx->needs_input_grad(7 + has_b1), need_b2 = b2.defined() && ctx->needs_input_grad(8 + has_b1);
+    const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(5), need_b1 = has_b1 && ctx->needs_input_grad(6),
+               need_w2 = ctx->needs_input_grad(6 + has_b1), need_b2 = b2.defined() && ctx->needs_input_grad(7 + has_b1);
     const auto f32 = dy.options().dtype(at::kFloat);
-    Tensor dwt = at::empty({T, k}, f32), by_place = at::empty({T * k}, f32), g = at::empty({T * k, C}, dy.options());
-    check(tmpi_expert_combine_gradient(dy.data_ptr(), ptr(b2), weights.data_ptr<float>(), 0, place.data_ptr<int>(), b2.defined() ? chosen.data_ptr<int>() : nullptr,
-                                       nullptr, g.data_ptr(), dwt.data_ptr<float>(), by_place.data_ptr<float>(), (int)T, (int)k, (int)C, (int)E,
-                                       dtype_code(dy.scalar_type()), stream()));
-    launched(EXPERTS, 1);
     const bool need_wt = ctx->needs_input_grad(1);
-    const int64_t slices = (H + 63) / 64;
-    Tensor dots;
+    const Tensor by_place = at::empty({T * k}, f32), g = dispatch(dy, place, Tensor(), weights, by_place);
+    const int64_t slices = (H + 31) / 32;
+    Tensor dots, dwt;
     if (need_wt) dots = at::empty({T * k, slices}, f32);
     const auto both = grouped_gelu_gradient(g, w2, offsets, kz, by_place, dots);
     const Tensor dz = both.first, hw = both.second;
     if (need_wt) {
-      check(tmpi_expert_dots(dots.data_ptr<float>(), order.data_ptr<int>(), dwt.data_ptr<float>(), (int)T, (int)k, (int)slices, stream()));
+      dwt = at::empty({T, k}, f32);
+      check(tmpi_expert_weight_gradient(dots.data_ptr<float>(), dy.data_ptr(), ptr(b2), place.data_ptr<int>(), chosen.data_ptr<int>(), dwt.data_ptr<float>(), (int)T, (int)k,
+                                        (int)slices, (int)C, (int)E, stream()));
       launched(EXPERTS, 1);
     }
     Tensor dx, dw1, db1, dw2, db2;
@@ -329,7 +328,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     }
     if (need_x) dx = combine(grouped(dz, w1, Tensor(), offsets, true, FP32, Tensor(), Tensor()), Tensor(), place, dy.scalar_type());
     const Tensor none;
-    return {dx, need_wt ? dwt : none, none, none, none, none, need_w1 ? dw1 : none, db1, need_w2 ? dw2 : none, db2, none, none};
+    return {dx, dwt, none, none, none, need_w1 ? dw1 : none, db1, need_w2 ? dw2 : none, db2, none, none};
   }
 };
 
@@ -405,7 +404,7 @@ void register_experts(pybind11::module_& m) {
     const int64_t E = w1.size(0), H = w1.size(1), C = w1.size(2), T = place.size(0), k = place.size(1);
     if (!(x.size(-1) == C && x.numel() == T * C && shaped(weights, {T, k}) && shaped(chosen, {T, k}) && shaped(order, {T * k}) && shaped(offsets, {E + 1}) && shaped(w2, {E, C, H}) &&
           shaped(b1, {E, H}) && shaped(b2, {E, C}) && C % 8 == 0 && H % 8 == 0 && w1.numel() && E <= tmpi_grouped_max_experts() && T && T * k && T * k <= MOST)) return c10::nullopt;
-    const Tensor y = ExpertsFn::apply(rows_of(x), weights, chosen, order, place, offsets, w1, b1_, w2, b2_, act8, wants_grad({x, weights, w1, w2, b1, b2}));
+    const Tensor y = ExpertsFn::apply(rows_of(x), weights, chosen, place, offsets, w1, b1_, w2, b2_, act8, wants_grad({x, weights, w1, w2, b1, b2}));
     return x.dim() == 2 ? y : y.view(x.sizes());
   });
 }

@@ -390,13 +390,15 @@ int tmpi_route(const void* logits, int64_t ld, int tokens, int experts, int k, i
                int* place, int* offsets, void* workspace, size_t workspace_bytes, void* stream);
 int tmpi_route_gradient(const void* logits, int64_t ld, int tokens, int experts, int k, int renormalize, int dtype, const float* weights, const int* chosen,
                         const float* dweights, void* dlogits, void* stream);
-int tmpi_expert_dispatch(const void* x, const int* place, const int* used, void* out, int tokens, int k, int cols, int dtype, void* stream);
+int tmpi_expert_dispatch(const void* x, const int* place, const int* used, const float* weights, void* out, float* place_weights, int tokens, int k, int cols,
+                         int dtype, void* stream);
 int tmpi_expert_dispatch_keep(const void* x, const int* place, void* out, void* q, void* scale, int tokens, int k, int cols, void* stream);
 int tmpi_expert_dispatch8(const void* q, const void* scale, const int* place, void* out, int tokens, int k, int cols, void* stream);
 int tmpi_expert_combine(const void* rows, int rows_fp32, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream);
-int tmpi_expert_combine_gradient(const void* dy, const void* other, const float* weights, int scaled, const int* place, const int* chosen, const int* used, void* drows,
-                                 float* dweights, float* place_weights, int tokens, int k, int cols, int nexperts, int dtype, void* stream);
-int tmpi_expert_dots(const float* dots, const int* order, float* dweights, int tokens, int k, int slices, void* stream);
+int tmpi_expert_combine_gradient(const void* dy, const void* rows, const float* weights, const int* place, const int* used, void* drows, float* dweights, int tokens,
+                                 int k, int cols, int dtype, void* stream);
+int tmpi_expert_weight_gradient(const float* dots, const void* dy, const void* bias, const int* place, const int* chosen, float* dweights, int tokens, int k, int slices,
+                                int cols, int nexperts, void* stream);
 // Products grouped by expert: rows offsets[e] <= r < offsets[e + 1] (on the device) of x belong to expert e
 int tmpi_grouped_max_experts(void);
 int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,

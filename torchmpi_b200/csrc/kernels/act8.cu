@@ -101,7 +101,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS) quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, const Layout l) {
   wait_previous(x);
   const long long items = l.items(), stride = (long long)gridDim.x * THREADS;
-  constexpr int U = 2;
+  constexpr int U = 16 / sizeof(T) / 2;                 // 64 bytes of a thread
   for (long long i0 = (long long)blockIdx.x * THREADS + threadIdx.x; (i0 & ~31LL) < items; i0 += U * stride) {
     float v[U][PER];
     int n[U];
@@ -119,14 +119,20 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(const T* __restrict__
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      uint32_t a = 0;
+      uint32_t a = 0;                                   // largest magnitude, infinities and NaN among them: they are looked at where a warp has one
 #pragma unroll
-      for (int k = 0; k < PER; ++k) a = max(a, magnitude(v[u][k]));
+      for (int k = 0; k < PER; ++k) a = max(a, __float_as_uint(v[u][k]) & 0x7fffffffu);
+      const bool finite = __all_sync(~0u, a < 0x7f800000u);
+      if (!finite) {
+        a = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) a = max(a, magnitude(v[u][k]));
+      }
       a = max(a, __shfl_xor_sync(~0u, a, 1));
       a = max(a, __shfl_xor_sync(~0u, a, 2));
       const uint32_t byte = scale_byte(a);
       const long long i = i0 + u * stride;
-      store_q<VEC>(q + at[u], n[u], pack8(v[u], inverse(byte)));
+      store_q<VEC>(q + at[u], n[u], finite ? pack8_finite(v[u], inverse(byte)) : pack8(v[u], inverse(byte)));
       if ((threadIdx.x & 3) == 0 && i < items) scale[i >> 2] = (uint8_t)byte;
     }
   }
@@ -198,7 +204,14 @@ __global__ void __launch_bounds__(THREADS, 4) gelu_gradient_kernel(const T* __re
 #pragma unroll
       for (int k = 0; k < PER; k += 2) {
         float d0, d1;
-        gelu_both2(z[k], z[k + 1], &y[k], &y[k + 1], &d0, &d1);
+        if (sizeof(T) == 2) {                           // results of 8 or 11 bits: the quicker form (gelu.cuh)
+          unsigned long long value2, slope2;
+          quick_gelu_both2(attn_util::pack2(__float_as_uint(z[k]), __float_as_uint(z[k + 1])), &value2, &slope2);
+          attn_util::unpack2(value2, y[k], y[k + 1]);
+          attn_util::unpack2(slope2, d0, d1);
+        } else {
+          gelu_both2(z[k], z[k + 1], &y[k], &y[k + 1], &d0, &d1);
+        }
         g[u][k] *= d0;
         g[u][k + 1] *= d1;
       }
@@ -228,7 +241,7 @@ static bool vectors(int cols, std::initializer_list<const void*> wide, const voi
 template <typename T>
 static cudaError_t quantize_t(const void* x, void* q, void* scale, const Layout& l, cudaStream_t s) {
   const auto kernel = vectors(l.cols, {x}, q) ? quantize_kernel<T, true> : quantize_kernel<T, false>;
-  return launch_overlapped(kernel, grid(l, 2, 8), THREADS, 0, s, (const T*)x, (uint8_t*)q, (uint8_t*)scale, l);
+  return launch_overlapped(kernel, grid(l, 16 / sizeof(T) / 2, 8), THREADS, 0, s, (const T*)x, (uint8_t*)q, (uint8_t*)scale, l);
 }
 template <typename T>
 static cudaError_t restore_t(const void* q, const void* scale, void* x, const Layout& l, cudaStream_t s) {

@@ -95,5 +95,18 @@ __device__ __forceinline__ uint2 pack8(const float (&x)[8], float inv) {
   return make_uint2(pack2(x[0], x[1], inv) | pack2(x[2], x[3], inv) << 16, pack2(x[4], x[5], inv) | pack2(x[6], x[7], inv) << 16);
 }
 
+// the same where all are finite
+__device__ __forceinline__ uint2 pack8_finite(const float (&x)[8], float inv) {
+  const unsigned long long inv2 = attn_util::pack2(__float_as_uint(inv), __float_as_uint(inv));
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 v;
+    attn_util::unpack2(attn_util::mul2(attn_util::pack2(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1])), inv2), v.x, v.y);
+    h[i] = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+}
+
 }  // namespace act8
 }  // namespace tmpi

@@ -27,13 +27,8 @@ __device__ __forceinline__ float warp_sum(float x) {
   for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
   return x;
 }
-// the token of the entry at place `s`, -1 for places that hold none; entries that no token has (a caller's own order) count as none
-__device__ __forceinline__ int token_at(const int* __restrict__ order, int s, int k, int tokens) {
-  const int e = order[s];
-  return e >= 0 && e / k < tokens ? e / k : -1;
-}
 // zeros in the places from *used on; all threads of the grid
-template <typename T, int V>
+template <typename T, int V, int BLOCK_THREADS = THREADS>
 __device__ __forceinline__ void clear_rest(const int* __restrict__ used, T* __restrict__ rows, int places, int cols) {
   if (!used) return;
   const int first = min(max(*used, 0), places);
@@ -41,14 +36,15 @@ __device__ __forceinline__ void clear_rest(const int* __restrict__ used, T* __re
 #pragma unroll
   for (int e = 0; e < V; ++e) zero.v[e] = from_acc<T>(0);
   const long long n = (long long)(places - first) * (cols / V);
-  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < n; i += (long long)gridDim.x * THREADS) st_pack<T, V>(rows + (long long)first * cols + i * V, zero);
+  for (long long i = (long long)blockIdx.x * BLOCK_THREADS + threadIdx.x; i < n; i += (long long)gridDim.x * BLOCK_THREADS) st_pack<T, V>(rows + (long long)first * cols + i * V, zero);
 }
 
-// out[place of each of a token's entries] = x[token]
+// out[place of each of a token's entries] = x[token]; place_weights: the weight of the entry at each place
 template <typename T, int V>
-__global__ void __launch_bounds__(THREADS) dispatch_kernel(const T* __restrict__ x, const int* __restrict__ place, const int* __restrict__ used, T* __restrict__ out,
-                                                           int places, int tokens, int k, int cols) {
-  wait_previous(x, place, used);
+__global__ void __launch_bounds__(THREADS) dispatch_kernel(const T* __restrict__ x, const int* __restrict__ place, const int* __restrict__ used,
+                                                           const float* __restrict__ weights, T* __restrict__ out, float* __restrict__ place_weights, int places,
+                                                           int tokens, int k, int cols) {
+  wait_previous(x, place, used, weights);
   const int parts = cols / V;
   const long long items = (long long)tokens * parts, stride = (long long)gridDim.x * THREADS;
   constexpr int U = 2;
@@ -69,7 +65,9 @@ __global__ void __launch_bounds__(THREADS) dispatch_kernel(const T* __restrict__
       if (t[u] >= 0)
         for (int j = 0; j < k; ++j) {
           const int s = place[t[u] * k + j];
-          if (s >= 0 && s < places) st_pack<T, V>(out + (long long)s * cols + part[u] * V, v[u]);
+          if (s < 0 || s >= places) continue;
+          st_pack<T, V>(out + (long long)s * cols + part[u] * V, v[u]);
+          if (place_weights && part[u] == 0) place_weights[s] = weights[t[u] * k + j];
         }
   }
   clear_rest<T, V>(used, out, places, cols);
@@ -187,78 +185,130 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const R* __restrict__ 
   }
 }
 
-// The gradients of combine, a warp to a token: drows[place] = weight dy[token] (without `scaled` dy[token] itself), and
-// dweights[entry] = dy[token] . other, where other is rows[place] or, with `chosen`, the row of the entry's expert (its bias); 0 for entries without a
-// place, and without `other`.  place_weights: the weight of the entry at each place.
+// The gradients of combine: drows[place] = weight dy[token], and dweights[entry] = dy[token] . rows[place] (0 for entries without a place).
+// `group` threads (a power of two) share a token, a piece of its row each where there are enough of them, so that all that a token needs is under way
+// at once.
+constexpr int GRAD_THREADS = 128;
 template <typename T, int V>
-__global__ void __launch_bounds__(THREADS, 3) combine_gradient_kernel(const T* __restrict__ dy, const T* __restrict__ other, const float* __restrict__ weights,
-                                                                   const int* __restrict__ place, const int* __restrict__ chosen, const int* __restrict__ used,
-                                                                   T* __restrict__ drows, float* __restrict__ dweights, float* __restrict__ place_weights, int scaled,
-                                                                   int places, int tokens, int k, int cols, int nexperts) {
-  wait_previous(dy, other, weights, place, chosen, used);
-  const int lane = threadIdx.x & 31, parts = cols / V;
-  for (long long t = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); t < tokens; t += (long long)gridDim.x * WARPS) {
-    constexpr int U = 4;                                  // pieces of dy that a lane holds at a time
-    for (int c0 = lane; c0 - lane < parts; c0 += U * 32) {
-      const bool first = c0 == lane, last = c0 - lane + U * 32 >= parts;
-      Pack<T, V> g[U];
+__global__ void __launch_bounds__(GRAD_THREADS) combine_gradient_kernel(const T* __restrict__ dy, const T* __restrict__ rows, const float* __restrict__ weights,
+                                                                        const int* __restrict__ place, const int* __restrict__ used, T* __restrict__ drows,
+                                                                        float* __restrict__ dweights, int places, int tokens, int k, int cols, int group) {
+  wait_previous(dy, rows, weights, place, used);
+  constexpr int J = 2;                                    // entries at a time
+  __shared__ float sums[GRAD_THREADS / 32][J];
+  const int lane = threadIdx.x % group, mine = threadIdx.x / group, per_block = GRAD_THREADS / group, parts = cols / V;
+  const bool across = group > 32;                         // a token's sums cross warps
+  for (long long t0 = (long long)blockIdx.x * per_block; t0 < tokens; t0 += (long long)gridDim.x * per_block) {      // the same for the whole block
+    const long long t = t0 + mine;
+    const bool in = t < tokens;
+    for (int j0 = 0; j0 < k; j0 += J) {
+      int s[J];
+      float w[J], dot[J];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (c0 + 32 * u < parts) g[u] = ld_pack<T, V>(dy + t * cols + (long long)(c0 + 32 * u) * V);
-      for (int j = 0; j < k; ++j) {
-        const long long entry = t * k + j;
-        const int s = place[entry];
-        if (s < 0 || s >= places) {
-          if (dweights && first && lane == 0) dweights[entry] = 0.f;
-          continue;
-        }
-        const float w = weights ? weights[entry] : 1.f;
-        const T* o = other;
-        if (other) {
-          const int e = chosen ? chosen[entry] : 0;
-          o = chosen ? (e >= 0 && e < nexperts ? other + (long long)e * cols : nullptr) : other + (long long)s * cols;
-        }
-        Pack<T, V> b[U];
-        if (o) {
+      for (int j = 0; j < J; ++j) {
+        const bool there = in && j0 + j < k;
+        s[j] = there ? place[t * k + j0 + j] : -1;
+        w[j] = there ? weights[t * k + j0 + j] : 0.f;
+        dot[j] = 0.f;
+      }
+      if (in)
+        for (int c = lane; c < parts; c += group) {
+          const Pack<T, V> g = ld_pack<T, V>(dy + t * cols + (long long)c * V);
+          Pack<T, V> b[J];
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-            if (c0 + 32 * u < parts) b[u] = ld_pack<T, V>(o + (long long)(c0 + 32 * u) * V);
-        }
-        float dot = 0.f;
+          for (int j = 0; j < J; ++j)
+            if (rows && (unsigned)s[j] < (unsigned)places) b[j] = ld_pack<T, V>(rows + (long long)s[j] * cols + (long long)c * V);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (c0 + 32 * u >= parts) break;
-          Pack<T, V> out;
+          for (int j = 0; j < J; ++j) {
+            if ((unsigned)s[j] >= (unsigned)places) continue;
+            Pack<T, V> out;
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float f = (float)to_acc<T>(g[u].v[e]);
-            if (o) dot += f * (float)to_acc<T>(b[u].v[e]);
-            out.v[e] = scaled ? from_acc<T>((typename AccOf<T>::type)(w * f)) : g[u].v[e];
+            for (int i = 0; i < V; ++i) {
+              const float f = (float)to_acc<T>(g.v[i]);
+              if (rows) dot[j] += f * (float)to_acc<T>(b[j].v[i]);
+              out.v[i] = from_acc<T>((typename AccOf<T>::type)(w[j] * f));
+            }
+            st_pack<T, V>(drows + (long long)s[j] * cols + (long long)c * V, out);
           }
-          st_pack<T, V>(drows + (long long)s * cols + (long long)(c0 + 32 * u) * V, out);
         }
-        if (dweights) {
-          if (o) dot = warp_sum(dot);
-          if (lane == 0) dweights[entry] = first ? dot : dweights[entry] + dot;      // the parts of a long row, in their order
+      if (rows) {
+        for (int d = min(group, 32) / 2; d; d /= 2)
+#pragma unroll
+          for (int j = 0; j < J; ++j) dot[j] += __shfl_xor_sync(~0u, dot[j], d);
+        if (across) {
+          if ((threadIdx.x & 31) == 0)
+#pragma unroll
+            for (int j = 0; j < J; ++j) sums[threadIdx.x / 32][j] = dot[j];
+          __syncthreads();
+          if (lane == 0)
+            for (int i = 1; i < group / 32; ++i)
+#pragma unroll
+              for (int j = 0; j < J; ++j) dot[j] += sums[threadIdx.x / 32 + i][j];
+          __syncthreads();
         }
-        if (place_weights && last && lane == 0) place_weights[s] = w;
+        if (lane == 0 && in)
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            if (j0 + j < k) dweights[t * k + j0 + j] = (unsigned)s[j] < (unsigned)places ? dot[j] : 0.f;
       }
     }
   }
-  clear_rest<T, V>(used, drows, places, cols);
+  clear_rest<T, V, GRAD_THREADS>(used, drows, places, cols);
 }
 
-// dweights[entry] += the sum of the entry's row of `dots` (grouped.cu: a number for 64 columns), a warp to a place
-__global__ void __launch_bounds__(THREADS) dots_kernel(const float* __restrict__ dots, const int* __restrict__ order, float* __restrict__ dweights, int places, int tokens,
-                                                       int k, int slices) {
-  wait_previous(dots, order);
-  const int lane = threadIdx.x & 31;
-  for (long long s = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); s < places; s += (long long)gridDim.x * WARPS) {
-    if (token_at(order, (int)s, k, tokens) < 0) continue;
-    float sum = 0.f;
-    for (int i = lane; i < slices; i += 32) sum += dots[s * slices + i];
-    sum = warp_sum(sum);
-    if (lane == 0) dweights[order[s]] += sum;
+// The weights' gradient in a layer of experts, a warp to a token: dweights[entry] = the sum of the entry's row of `dots` (grouped.cu: a number for
+// 32 columns) + dy[token] . bias[expert].  0 for entries without a place.
+template <int V>
+__global__ void __launch_bounds__(THREADS) weight_gradient_kernel(const float* __restrict__ dots, const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ bias,
+                                                                  const int* __restrict__ place, const int* __restrict__ chosen, float* __restrict__ dweights,
+                                                                  int places, int tokens, int k, int slices, int cols, int nexperts) {
+  wait_previous(dots, dy, bias, place, chosen);
+  const int lane = threadIdx.x & 31, parts = cols / V;
+  for (long long t = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); t < tokens; t += (long long)gridDim.x * WARPS) {
+    constexpr int J = 2, U = 4;
+    for (int j0 = 0; j0 < k; j0 += J) {
+      int s[J], e[J];
+      float sum[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        s[j] = j0 + j < k ? place[t * k + j0 + j] : -1;
+        e[j] = j0 + j < k && bias ? chosen[t * k + j0 + j] : -1;
+        sum[j] = 0.f;
+      }
+      if (bias)
+        for (int c0 = lane; c0 < parts; c0 += 32 * U) {
+          Pack<__nv_bfloat16, V> g[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c0 + 32 * u < parts) g[u] = ld_pack<__nv_bfloat16, V>(dy + t * cols + (long long)(c0 + 32 * u) * V);
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            if ((unsigned)e[j] >= (unsigned)nexperts) continue;
+            Pack<__nv_bfloat16, V> b[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              if (c0 + 32 * u < parts) b[u] = ld_pack<__nv_bfloat16, V>(bias + (long long)e[j] * cols + (long long)(c0 + 32 * u) * V);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              if (c0 + 32 * u < parts)
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[j] += __bfloat162float(g[u].v[i]) * __bfloat162float(b[u].v[i]);
+          }
+        }
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if ((unsigned)s[j] < (unsigned)places) {
+          float more = 0.f;
+#pragma unroll 4
+          for (int i = lane; i < slices; i += 32) more += dots[(long long)s[j] * slices + i];
+          sum[j] += more;
+        }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const float total = warp_sum(sum[j]);
+        if (lane == 0 && j0 + j < k) dweights[t * k + j0 + j] = (unsigned)s[j] < (unsigned)places ? total : 0.f;
+      }
+    }
   }
 }
 
@@ -297,15 +347,16 @@ using namespace tmpi;
 
 extern "C" {
 
-// out [tokens * k, cols] from x [tokens, cols]; used (optional): places from *used on get zeros
-int tmpi_expert_dispatch(const void* x, const int* place, const int* used, void* out, int tokens, int k, int cols, int dtype, void* stream) {
+// out [tokens * k, cols] from x [tokens, cols]; used (optional): places from *used on get zeros; place_weights [tokens * k] (optional): the
+// weights [tokens, k] in the order of the places
+int tmpi_expert_dispatch(const void* x, const int* place, const int* used, const float* weights, void* out, float* place_weights, int tokens, int k, int cols, int dtype, void* stream) {
   const int st = experts::checked(tokens, k, cols, dtype, "expert_dispatch");
   if (st || !tokens) return st;
   return experts::finish(experts::by_type(dtype, cols, {x, out}, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
     return launch_overlapped(experts::dispatch_kernel<T, V>, experts::grid_items((long long)tokens * (cols / V), 2, 8), experts::THREADS, 0, (cudaStream_t)stream,
-                             (const T*)x, place, used, (T*)out, tokens * k, tokens, k, cols);
+                             (const T*)x, place, used, weights, (T*)out, place_weights, tokens * k, tokens, k, cols);
   }), "expert_dispatch");
 }
 
@@ -349,27 +400,31 @@ int tmpi_expert_combine(const void* rows, int rows_fp32, const float* weights, c
   return experts::finish(experts::by_type(dtype, cols, {rows, y}, [&](auto t, auto v) { return go(t, t, v); }), "expert_combine");
 }
 
-// drows [tokens * k, cols] and, where given, dweights [tokens * k] from dy [tokens, cols].  other: rows [tokens * k, cols], or with `chosen` a row for
-// each of nexperts experts; null: dweights gets zeros.  scaled: drows holds weight times dy, else dy.  place_weights [tokens * k]
-// (optional): the weights in the order of the places.  used (optional): rows of drows from *used on get zeros.
-int tmpi_expert_combine_gradient(const void* dy, const void* other, const float* weights, int scaled, const int* place, const int* chosen, const int* used, void* drows,
-                                 float* dweights, float* place_weights, int tokens, int k, int cols, int nexperts, int dtype, void* stream) {
+// drows [tokens * k, cols] = weight times dy [tokens, cols], zeros from *used on, and, where rows [tokens * k, cols] is given, dweights [tokens * k]
+int tmpi_expert_combine_gradient(const void* dy, const void* rows, const float* weights, const int* place, const int* used, void* drows, float* dweights, int tokens,
+                                 int k, int cols, int dtype, void* stream) {
   const int st = experts::checked(tokens, k, cols, dtype, "expert_combine_gradient");
   if (st || !tokens) return st;
-  return experts::finish(experts::by_type(dtype, cols, {dy, other, drows}, [&](auto t, auto v) {
+  if (rows && !dweights) return fail(TMPI_ERR_INVALID, "expert_combine_gradient: rows without dweights");
+  return experts::finish(experts::by_type(dtype, cols, {dy, rows, drows}, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
-    return launch_overlapped(experts::combine_gradient_kernel<T, V>, experts::grid_rows(tokens, 8), experts::THREADS, 0, (cudaStream_t)stream, (const T*)dy,
-                             (const T*)other, weights, place, chosen, used, (T*)drows, dweights, place_weights, scaled, tokens * k, tokens, k, cols, nexperts);
+    int group = 1;
+    while (group < experts::GRAD_THREADS && group < cols / V) group *= 2;
+    const int per_block = experts::GRAD_THREADS / group, blocks = std::min((tokens + per_block - 1) / per_block, 148 * 16);
+    return launch_overlapped(experts::combine_gradient_kernel<T, V>, blocks, experts::GRAD_THREADS, 0, (cudaStream_t)stream, (const T*)dy, (const T*)rows, weights,
+                             place, used, (T*)drows, dweights, tokens * k, tokens, k, cols, group);
   }), "expert_combine_gradient");
 }
 
-// dweights [tokens * k] += the sums of the rows of dots [tokens * k, slices], for the entries that have a place
-int tmpi_expert_dots(const float* dots, const int* order, float* dweights, int tokens, int k, int slices, void* stream) {
-  const int st = experts::checked(tokens, k, slices, TMPI_F32, "expert_dots");
+// dweights [tokens, k] = the sums of the rows of dots [tokens * k, slices] + dy [tokens, cols] . bias [nexperts, cols] (bf16, or null) of the chosen expert
+int tmpi_expert_weight_gradient(const float* dots, const void* dy, const void* bias, const int* place, const int* chosen, float* dweights, int tokens, int k, int slices,
+                                int cols, int nexperts, void* stream) {
+  const int st = experts::checked(tokens, k, cols, TMPI_BF16, "expert_weight_gradient");
   if (st || !tokens) return st;
-  return experts::finish(launch_overlapped(experts::dots_kernel, experts::grid_rows(tokens * k, 8), experts::THREADS, 0, (cudaStream_t)stream, dots, order, dweights,
-                                           tokens * k, tokens, k, slices), "expert_dots");
+  const auto kernel = cols % 8 == 0 && all_aligned16({dy, bias}) ? experts::weight_gradient_kernel<8> : experts::weight_gradient_kernel<1>;
+  return experts::finish(launch_overlapped(kernel, experts::grid_rows(tokens, 8), experts::THREADS, 0, (cudaStream_t)stream, dots, (const __nv_bfloat16*)dy,
+                                           (const __nv_bfloat16*)bias, place, chosen, dweights, tokens * k, tokens, k, slices, cols, nexperts), "expert_weight_gradient");
 }
 
 }  // extern "C"

@@ -52,7 +52,7 @@ struct Problem {
   uint8_t* scale;            // and their scales
   __nv_bfloat16* h;          // GRADIENT: weight times gelu(z)
   const float* row_weights;  // GRADIENT: [rows] or null (ones)
-  float* dots;               // GRADIENT: [rows, slices], the sum over 64 columns of gradient times gelu(z); or null
+  float* dots;               // GRADIENT: [rows, ceil(N / 32)], the sum over 32 columns of gradient times gelu(z); or null
   int wide;                  // every row of y, z, h starts on a 32-byte boundary
   int q_rows16;              // KEEP8: every row of z starts on a 16-byte boundary, as TMA tiles need
   int* status;
@@ -97,13 +97,13 @@ __device__ __forceinline__ void give_up(S* sh, int* status, int where) {
   if (status) atomicCAS(status, 0, 1000 + where);
 }
 
-// All threads of the CTA; ends with a barrier.
-__device__ __forceinline__ void count_tiles(Sh* sh, const Problem& p, const int* offsets) {
+// Tiles of `rows` rows.  All threads of the CTA; ends with a barrier.
+__device__ __forceinline__ void count_tiles(Sh* sh, const Problem& p, const int* offsets, int rows) {
   const int e = threadIdx.x, lane = e & 31, warp = e >> 5;
   int tiles = 0;
   if (e < p.experts) {
     const Group g = group_of(offsets, p.rows, e);
-    tiles = (g.r1 - g.r0 + 2 * BM - 1) / (2 * BM) * p.tiles_n;
+    tiles = (g.r1 - g.r0 + rows - 1) / rows * p.tiles_n;
   }
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -281,7 +281,7 @@ template <int MODE>
 __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights,
                                        const CUtensorMap* map_y, const CUtensorMap* map_z, uint32_t rank, int group, int quarter, int lane) {
   constexpr bool GRADIENT = MODE == GRADIENT8 || MODE == GRADIENT16;
-  const int row = quarter * 32 + lane, N = p.N, bn = p.bn, slices = (N + SLICE - 1) / SLICE, blocks = (N + 31) / 32;
+  const int row = quarter * 32 + lane, N = p.N, bn = p.bn, blocks = (N + 31) / 32;
   const bool wide = p.wide != 0;
   for_tiles(sh, p, offsets, [&](const Unit& u, int it) -> bool {
     const int acc = it & 1, rows = u.part_rows(rank), c0 = group * SLICE, col0 = u.n_blk * bn + c0;
@@ -311,7 +311,7 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
     };
     const long long row_at = (long long)u.row0 + (int)rank * BM + row;
     const __nv_bfloat16* bias = bias_all ? bias_all + (long long)u.e * N : nullptr;
-    float weight = 1.f, dot = 0.f;
+    float weight = 1.f;
     uint32_t kept[2][GRADIENT ? 8 : 1];
     uint32_t kept_scale[2] = {1u, 1u};
     if (GRADIENT && mine) {                              // while the products are under way
@@ -432,7 +432,7 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
         }
         float a0, a1;
         attn_util::unpack2(dot2, a0, a1);
-        dot += a0 + a1;
+        if (mine && p.dots) p.dots[row_at * blocks + col / 32] = a0 + a1;
         if (whole) {
           reuse(1);
           stage(1, hw);
@@ -455,7 +455,6 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
         store_row(p.y + row_at * N + col, w, left, wide);
       }
     }
-    if (GRADIENT && mine && p.dots) p.dots[row_at * slices + col0 / SLICE] = dot;
     return true;
   });
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -501,7 +500,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   if (!p.offsets) offsets = nullptr;
   if (!p.bias) bias = nullptr;
   if (!p.row_weights) row_weights = nullptr;
-  count_tiles(sh, p, offsets);
+  count_tiles(sh, p, offsets, 2 * BM);
   if (warp == 0) {
     if (sm100::elect_one()) produce<NST, B_MN>(sh, tiles, p, offsets, &map_a, &map_a_few, &map_b, rank);
   } else if (warp == 1) {
@@ -525,6 +524,233 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   }
 }
 
+// ---------------------------------------------------------------- few rows to an expert
+// The product the other way round, y^T = w_e x^T, on one CTA per tile: 128 rows of the weight are the M of the MMAs, up to 128 rows of x
+// (as many as there are, in steps of 16) their N.  A tile of the kernel above multiplies 256 rows of x whether there are two or 200: with 2
+// rows to each of 8 experts, 1024 -> 4096, MMAs were under way for 10 of its 20 us, where the weights need 10.  What bounds this one is the
+// weights' way from memory: 96 KB of them are under way per SM.
+// A thread has a column of y and walks the rows, so a warp's stores are 64 bytes of a row each, the 32 columns of an 8-bit block are its lanes', and a row
+// behind the group's end is not touched.
+constexpr int FEW_BM = 128, FEW_BN = 128, FEW_STAGES = 6, FEW_EPI_WARPS = 8, FEW_THREADS = 64 + FEW_EPI_WARPS * 32;
+constexpr int FEW_A_BYTES = FEW_BM * BK * 2, FEW_STAGE_BYTES = FEW_A_BYTES + FEW_BN * BK * 2;
+constexpr size_t FEW_SMEM = (size_t)FEW_STAGES * FEW_STAGE_BYTES + 1024 + 1280;
+static_assert(FEW_STAGES == STAGES && FEW_SMEM <= 232448, "shared memory of one CTA");
+
+// f(expert, first row, rows, row of the weight, number in this CTA's list) for each tile of this CTA until it returns false; the tiles that share a part of the
+// weight follow each other
+template <typename F>
+__device__ __forceinline__ void for_few(const Sh* sh, const Problem& p, const int* offsets, F f) {
+  const int total = sh->tile_end[p.experts - 1], step = (int)gridDim.x;
+  int e = 0, it = 0;
+  for (int t = (int)blockIdx.x; t < total; t += step, ++it) {
+    if (sh->tile_end[e] <= t) {
+      int hi = p.experts - 1;
+      ++e;
+      while (e < hi) {
+        const int mid = (e + hi) >> 1;
+        if (sh->tile_end[mid] > t) hi = mid;
+        else e = mid + 1;
+      }
+    }
+    const int at = t - (e ? sh->tile_end[e - 1] : 0);
+    const Group g = group_of(offsets, p.rows, e);
+    const int across = (g.r1 - g.r0 + FEW_BN - 1) / FEW_BN, row0 = g.r0 + at % across * FEW_BN;
+    if (!f(e, row0, min(g.r1 - row0, FEW_BN), at / across * FEW_BM, it)) return;
+  }
+}
+
+__device__ __forceinline__ float one_gelu(float z) {
+  float y, none;
+  attn_util::unpack2(quick_gelu2(attn_util::pack2(__float_as_uint(z), __float_as_uint(z))), y, none);
+  return y;
+}
+
+template <int MODE>
+__device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights, int half, int quarter, int lane) {
+  constexpr bool GRADIENT = MODE == GRADIENT8 || MODE == GRADIENT16;
+  const int N = p.N, blocks = (N + 31) / 32;
+  for_few(sh, p, offsets, [&](int e, int row0, int rows, int col0, int it) -> bool {
+    const int acc = it & 1, col = col0 + quarter * 32 + lane;
+    const bool in = col < N;
+    const float bias = bias_all && in ? __bfloat162float(bias_all[(long long)e * N + col]) : 0.f;
+    if (!sm100::mbar_wait_warp(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 54); return false; }
+    sm100::tc_fence_after();
+    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * FEW_BN;
+    // the two groups of warps take 16 rows in turn
+    for (int c = half * 16; c < rows && col0 + quarter * 32 < N; c += 32) {
+      uint32_t r[16];
+      float z_of[GRADIENT ? 16 : 1], weight_of[GRADIENT ? 16 : 1];
+      if (GRADIENT) {                                    // all that these rows need, at once
+        uint32_t kept[16], scales[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const bool there = in && c + j < rows;
+          const long long row = row0 + c + j, at = row * N + col;
+          if (MODE == GRADIENT8) {
+            kept[j] = there ? ((const uint8_t*)p.z)[at] : 0u;
+            scales[j] = there ? p.scale[row * blocks + col / 32] : 1u;
+          } else {
+            z_of[j] = there ? __bfloat162float(((const __nv_bfloat16*)p.z)[at]) : 0.f;
+          }
+          weight_of[j] = row_weights && c + j < rows ? __ldg(row_weights + row) : 1.f;
+        }
+        if (MODE == GRADIENT8) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float none;
+            act8::unpack2(kept[j], act8::value(scales[j]), &z_of[j], &none);
+          }
+        }
+      }
+      sm100::tmem_ld_32x16(t_base + c, r);
+      sm100::tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (c + j >= rows) break;
+        const long long row = row0 + c + j, at = row * N + col;
+        float v = __uint_as_float(r[j]);
+        if (!GRADIENT) v += bias;
+        if (MODE == PLAIN32) {
+          if (in) p.y32[at] = v;
+        } else if (GRADIENT) {
+          const float z = z_of[GRADIENT ? j : 0], weight = weight_of[GRADIENT ? j : 0];
+          float y0, y1, d0, d1;
+          unsigned long long y, slope;
+          quick_gelu_both2(attn_util::pack2(__float_as_uint(z), __float_as_uint(z)), &y, &slope);
+          attn_util::unpack2(y, y0, y1);
+          attn_util::unpack2(slope, d0, d1);
+          if (p.dots) {
+            float dot = in ? v * y0 : 0.f;
+#pragma unroll
+            for (int d = 16; d; d /= 2) dot += __shfl_xor_sync(~0u, dot, d);
+            if (lane == 0) p.dots[row * blocks + col / 32] = dot;
+          }
+          if (in) {
+            p.h[at] = __float2bfloat16_rn(weight * y0);
+            p.y[at] = __float2bfloat16_rn(v * d0 * weight);
+          }
+        } else {
+          if (MODE == WITH_GELU && in) ((__nv_bfloat16*)p.z)[at] = __float2bfloat16_rn(v);
+          if (MODE == KEEP8) {
+            const uint32_t byte = act8::scale_byte(__reduce_max_sync(~0u, in ? act8::magnitude(v) : 0u));
+            if (in) ((uint8_t*)p.z)[at] = (uint8_t)act8::pack2(v, 0.f, act8::inverse(byte));
+            if (lane == 0) p.scale[row * blocks + col / 32] = (uint8_t)byte;
+          }
+          if (MODE != PLAIN) v = one_gelu(v);
+          if (in) p.y[at] = __float2bfloat16_rn(v);
+        }
+      }
+    }
+    sm100::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) sm100::mbar_arrive(&sh->acc_empty[acc]);
+    return true;
+  });
+  if (MODE == PLAIN || MODE == GELU_ONLY || MODE == WITH_GELU) {      // rows behind the last group
+    const long long used = group_of(offsets, p.rows, p.experts - 1).r1;
+    const long long chunks = (p.rows - used) * (N / 8);
+    uint4* rest = reinterpret_cast<uint4*>(p.y + used * N);
+    for (long long i = (long long)blockIdx.x * (FEW_EPI_WARPS * 32) + (threadIdx.x - 64); i < chunks; i += (long long)gridDim.x * (FEW_EPI_WARPS * 32))
+      rest[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+template <int MODE, bool W_MN>
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x_few,
+                   const __grid_constant__ Problem p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  Sh* sh = reinterpret_cast<Sh*>(tiles + (size_t)FEW_STAGES * FEW_STAGE_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0 && sm100::elect_one()) {
+    sm100::tma_prefetch_desc(&map_w);
+    sm100::tma_prefetch_desc(&map_x);
+    for (int s = 0; s < FEW_STAGES; ++s) { sm100::mbar_init(&sh->full[s], 1); sm100::mbar_init(&sh->empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { sm100::mbar_init(&sh->acc_full[a], 1); sm100::mbar_init(&sh->acc_empty[a], FEW_EPI_WARPS); }
+    sh->error = 0;
+    sm100::fence_barrier_init();
+  }
+  if (warp == 1) {
+    sm100::tmem_alloc(&sh->tmem_base, 2 * FEW_BN);
+    sm100::tmem_relinquish();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const int* offsets = p.offsets;
+  const __nv_bfloat16* bias = p.bias;
+  const float* row_weights = p.row_weights;
+  wait_previous(offsets, bias, row_weights);
+  if (!p.offsets) offsets = nullptr;
+  if (!p.bias) bias = nullptr;
+  if (!p.row_weights) row_weights = nullptr;
+  count_tiles(sh, p, offsets, FEW_BN);
+  if (warp == 0) {
+    if (sm100::elect_one()) {
+      Ring ring{0, 0};
+      for_few(sh, p, offsets, [&](int e, int row0, int rows, int col0, int) -> bool {
+        const uint32_t tx = FEW_A_BYTES + (rows > FEW ? FEW_BN : FEW) * BK * 2;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          const int stage = ring.stage;
+          if (!sm100::mbar_wait(&sh->empty[stage], ring.phase ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 51); return false; }
+          unsigned char* dst = tiles + (size_t)stage * FEW_STAGE_BYTES;
+          sm100::mbar_expect_tx(&sh->full[stage], tx);
+          if (!W_MN) {
+            sm100::tma_load_3d(dst, &map_w, kb * BK, col0, e, &sh->full[stage]);
+          } else {
+            sm100::tma_load_3d(dst, &map_w, col0, kb * BK, e, &sh->full[stage]);
+            sm100::tma_load_3d(dst + FEW_A_BYTES / 2, &map_w, col0 + 64, kb * BK, e, &sh->full[stage]);
+          }
+          sm100::tma_load_2d(dst + FEW_A_BYTES, rows > FEW ? &map_x : &map_x_few, kb * BK, row0, &sh->full[stage]);
+          advance<FEW_STAGES>(&ring);
+        }
+        return true;
+      });
+    }
+  } else if (warp == 1) {
+    if (sm100::elect_one()) {
+      Ring ring{0, 0};
+      for_few(sh, p, offsets, [&](int, int, int rows, int, int it) -> bool {
+        const int acc = it & 1;
+        if (!sm100::mbar_wait(&sh->acc_empty[acc], ((it >> 1) & 1) ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 52); return false; }
+        sm100::tc_fence_after();
+        const uint32_t idesc = sm100::make_idesc_f16(FEW_BM, (rows + 15) / 16 * 16, true, false, W_MN);
+        const uint32_t d = sh->tmem_base + (uint32_t)acc * FEW_BN;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          const int stage = ring.stage;
+          if (!sm100::mbar_wait(&sh->full[stage], ring.phase, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 53); return false; }
+          sm100::tc_fence_after();
+          const uint32_t a = sm100::smem_u32(tiles + (size_t)stage * FEW_STAGE_BYTES), b = a + FEW_A_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k) {
+            const uint64_t da = W_MN ? sm100::make_desc_sw128_mn(a + k * UMMA_K * 128, FEW_A_BYTES / 2, 1024) : sm100::make_desc_sw128(a + k * UMMA_K * 2);
+            sm100::umma_f16(d, da, sm100::make_desc_sw128(b + k * UMMA_K * 2), idesc, (uint32_t)kb | (uint32_t)k);
+          }
+          sm100::umma_commit(&sh->empty[stage]);
+          advance<FEW_STAGES>(&ring);
+        }
+        sm100::umma_commit(&sh->acc_full[acc]);
+        return true;
+      });
+    }
+  } else {
+    few_finish<MODE>(sh, p, offsets, bias, row_weights, (warp - 2) >> 2, warp & 3, lane);
+  }
+  __syncwarp();
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (sh->error && warp == 0 && sm100::elect_one()) {
+    const unsigned long long t0 = sm100::now_ns();
+    while (sm100::now_ns() - t0 < 200000000ull) { __nanosleep(1000); }   // copies in flight complete within microseconds
+  }
+  __syncthreads();
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(sh->tmem_base, 2 * FEW_BN);
+  }
+}
+
 // ---------------------------------------------------------------- the weights' gradient
 struct DwProblem {
   const int* offsets;
@@ -539,15 +765,15 @@ struct DwProblem {
 constexpr int EPI_THREADS = ROW_GROUPS * 128;
 constexpr int DW_THREADS = ROW_THREADS + 32;            // and the warp that clears rows of other groups
 constexpr int DB_GROUPS = EPI_THREADS / (BM / 8);
-static_assert(EPI_THREADS * 8 * 4 <= 32768, "the sums' exchange in the staging");
 
 struct DwSh {
   Shared s;
   uint64_t tail[STAGES];                                // a block with rows of another group: its loads, one barrier per CTA
   uint64_t cleared[STAGES];                             // in the even CTA: the odd one's part of such a block is cleared
 };
-constexpr size_t DW_SMEM = (size_t)STAGES * STAGE_BYTES + gemm::EPI_STAGING_BYTES + 1024 + sizeof(DwSh);
-static_assert(DW_SMEM <= 232448, "shared memory of one CTA");
+constexpr int DW_STAGES = 5, DW_STAGING = 4096;           // a warp's 32 rows x 64 columns; the sixth stage's room with the staging
+constexpr size_t DW_SMEM = (size_t)DW_STAGES * STAGE_BYTES + 16 * DW_STAGING + 1024 + sizeof(DwSh);
+static_assert(DW_SMEM <= 232448 && EPI_THREADS * 8 * 4 <= 16 * DW_STAGING, "shared memory of one CTA");
 
 struct DwUnit { int e, m_blk, n_blk, r0, r1, k_blocks; };
 
@@ -572,7 +798,7 @@ __device__ __forceinline__ void dw_setup(DwSh* sh, int warp, const CUtensorMap* 
   if (warp == 0 && sm100::elect_one()) {
     sm100::tma_prefetch_desc(ma);
     sm100::tma_prefetch_desc(mb);
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < DW_STAGES; ++s) {
       sm100::mbar_init(&sh->s.full[s], 1);
       sm100::mbar_init(&sh->s.empty[s], 1);
       sm100::mbar_init(&sh->tail[s], 1);
@@ -617,7 +843,7 @@ __device__ __forceinline__ void dw_produce(DwSh* shl, unsigned char* tiles, cons
       sm100::tma_load_2d_pair(dst + A_BYTES / 2, ma, m0 + 64, k0, bar);
       sm100::tma_load_2d_pair(dst + A_BYTES, mb, n0, k0, bar);
       if (two) sm100::tma_load_2d_pair(dst + A_BYTES + B_BYTES / 2, mb, n0 + 64, k0, bar);
-      advance<STAGES>(&ring);
+      advance<DW_STAGES>(&ring);
     }
     return true;
   });
@@ -633,7 +859,7 @@ __device__ __forceinline__ void dw_clear(DwSh* shl, unsigned char* tiles, const 
   for_units(p, offsets, rank, [&](const DwUnit& u) -> bool {
     const int rem = (u.r1 - u.r0) % BK;
     if (rem) {
-      const int at = (stage + u.k_blocks - 1) % STAGES;
+      const int at = (stage + u.k_blocks - 1) % DW_STAGES;
       const uint32_t phase = phases >> at & 1;
       if (!sm100::mbar_wait_warp(&shl->tail[at], phase, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 45); return false; }
       phases ^= 1u << at;
@@ -649,7 +875,7 @@ __device__ __forceinline__ void dw_clear(DwSh* shl, unsigned char* tiles, const 
         if (lane == 0) sm100::mbar_arrive(&sh->full[at]);
       }
     }
-    stage = (stage + u.k_blocks) % STAGES;
+    stage = (stage + u.k_blocks) % DW_STAGES;
     return true;
   });
 }
@@ -680,7 +906,7 @@ __device__ __forceinline__ void dw_issue(DwSh* shl, unsigned char* tiles, const 
       }
       sm100::umma_commit_pair(sm100::map_to_cta(&sh->empty[stage], 0));
       sm100::umma_commit_pair(sm100::map_to_cta(&sh->empty[stage], 1));
-      advance<STAGES>(&ring);
+      advance<DW_STAGES>(&ring);
     }
     sm100::umma_commit_pair(sm100::map_to_cta(&sh->acc_full[acc], 0));
     sm100::umma_commit_pair(sm100::map_to_cta(&sh->acc_full[acc], 1));
@@ -757,7 +983,7 @@ __device__ __forceinline__ void dw_finish(DwSh* shl, unsigned char* staging_all,
                                           const float* row_weights, uint32_t rank, int group, int quarter, int lane) {
   Shared* sh = &shl->s;
   const int row = quarter * 32 + lane, bn = p.bn, c0 = group * SLICE;
-  unsigned char* staging = staging_all + ((int)(threadIdx.x >> 5) - 2) * 2048;      // 32 rows x 64 bytes of this warp
+  unsigned char* staging = staging_all + ((int)(threadIdx.x >> 5) - 2) * DW_STAGING;
   int it = 0;
   for_units(p, offsets, rank, [&](const DwUnit& u) -> bool {
     const int row0 = u.m_blk * BM, col0 = u.n_blk * bn + c0, warp_row = row0 + quarter * 32;
@@ -783,9 +1009,10 @@ __device__ __forceinline__ void dw_finish(DwSh* shl, unsigned char* staging_all,
       if (lane == 0) sm100::mbar_arrive_cluster_no_stores(sm100::map_to_cta(&sh->acc_empty[acc], 0));
     };
     if (!busy) { release(); return true; }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      if (half && col0 + 32 >= p.K) { release(); break; }
       uint32_t w[16];
       if (u.k_blocks) {
         uint32_t r[32];
@@ -798,17 +1025,15 @@ __device__ __forceinline__ void dw_finish(DwSh* shl, unsigned char* staging_all,
 #pragma unroll
         for (int j = 0; j < 16; ++j) w[j] = 0u;
       }
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      __syncwarp();
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint4*>(staging + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-      sm100::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        sm100::tma_store_3d(mdw, staging, col0 + 32 * half, warp_row, u.e);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      }
+        *reinterpret_cast<uint4*>(staging + lane * 128 + (((4 * half + j) ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    }
+    sm100::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      sm100::tma_store_3d(mdw, staging, col0, warp_row, u.e);
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
     return true;
   });
@@ -819,10 +1044,9 @@ __global__ void __launch_bounds__(DW_THREADS, 1)
 grouped_dw_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dw,
                   const __grid_constant__ DwProblem p) {
   extern __shared__ unsigned char smem_raw[];
-  unsigned char *tiles, *staging;
-  Shared* sh0;
-  carve(smem_raw, &tiles, &sh0, &staging);
-  DwSh* sh = reinterpret_cast<DwSh*>(sh0);
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* staging = tiles + (size_t)DW_STAGES * STAGE_BYTES;
+  DwSh* sh = reinterpret_cast<DwSh*>(staging + 16 * DW_STAGING);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = sm100::cluster_ctarank();
   dw_setup(sh, warp, &map_dy, &map_x);
@@ -842,17 +1066,19 @@ grouped_dw_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_const
     dw_clear(sh, tiles, p, offsets, rank, lane);
   }
   __syncwarp();
-  teardown(sh0, warp);
+  teardown(&sh->s, warp);
 }
 
 // ---------------------------------------------------------------- host side
-static const void* row_kernel(int mode, bool w_is_kn) {
+// few: grouped_few_kernel
+template <int MODE, bool KN>
+static const void* kernel_of(bool few) { return few ? (const void*)grouped_few_kernel<MODE, KN> : (const void*)grouped_kernel<MODE, KN>; }
+static const void* row_kernel(int mode, bool w_is_kn, bool few) {
   if (w_is_kn)
-    return mode == PLAIN32 ? (const void*)grouped_kernel<PLAIN32, true> : mode == GRADIENT8 ? (const void*)grouped_kernel<GRADIENT8, true>
-           : mode == GRADIENT16 ? (const void*)grouped_kernel<GRADIENT16, true> : (const void*)grouped_kernel<PLAIN, true>;
-  return mode == GELU_ONLY ? (const void*)grouped_kernel<GELU_ONLY, false> : mode == WITH_GELU ? (const void*)grouped_kernel<WITH_GELU, false>
-         : mode == KEEP8 ? (const void*)grouped_kernel<KEEP8, false> : mode == PLAIN32 ? (const void*)grouped_kernel<PLAIN32, false>
-                                                                                       : (const void*)grouped_kernel<PLAIN, false>;
+    return mode == PLAIN32 ? kernel_of<PLAIN32, true>(few) : mode == GRADIENT8 ? kernel_of<GRADIENT8, true>(few)
+           : mode == GRADIENT16 ? kernel_of<GRADIENT16, true>(few) : kernel_of<PLAIN, true>(few);
+  return mode == GELU_ONLY ? kernel_of<GELU_ONLY, false>(few) : mode == WITH_GELU ? kernel_of<WITH_GELU, false>(few)
+         : mode == KEEP8 ? kernel_of<KEEP8, false>(few) : mode == PLAIN32 ? kernel_of<PLAIN32, false>(few) : kernel_of<PLAIN, false>(few);
 }
 
 static int max_clusters() {
@@ -860,7 +1086,9 @@ static int max_clusters() {
   static std::once_flag once;
   std::call_once(once, [] {
     for (int mode = PLAIN; mode <= GRADIENT16; ++mode)
-      for (int kn = 0; kn < 2; ++kn) cudaFuncSetAttribute(row_kernel(mode, kn != 0), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+      for (int kn = 0; kn < 2; ++kn)
+        for (int few = 0; few < 2; ++few)
+          cudaFuncSetAttribute(row_kernel(mode, kn != 0, few != 0), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(few ? FEW_SMEM : SMEM));
     cudaFuncSetAttribute((const void*)grouped_dw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DW_SMEM);
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
@@ -883,14 +1111,15 @@ static int tile_columns(long long tiles_m, int N, int clusters) {
   return 100 * c192 < 95 * c256 ? 192 : 256;
 }
 
-static cudaError_t launch(const void* kernel, long long clusters, int threads, size_t smem, void** args, cudaStream_t stream) {
+// `clusters` clusters of `size` CTAs
+static cudaError_t launch(const void* kernel, long long clusters, int size, int threads, size_t smem, void** args, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.x = size; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // see pdl.cuh
   at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(2 * clusters)); cfg.blockDim = dim3(threads);
+  cfg.gridDim = dim3((unsigned)(size * clusters)); cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem; cfg.stream = stream; cfg.attrs = at; cfg.numAttrs = 2;
   return cudaLaunchKernelExC(&cfg, kernel, args);
 }
@@ -905,18 +1134,34 @@ static int checked(const int* offsets, int rows, int nexperts, int K, int N, con
   return TMPI_OK;
 }
 
+// Rows to an expert, on average, up to which the product is formed the other way round.  Its epilogue takes a row at a time, and longer the more it does.
+// us of this form and the other, 8 experts, 1024 -> 4096: GELU with 2 rows each 12.7 and 18.2, 64 13.3 and 19.7, 128 17.0 and 19.0, 192 27.5 and 19.7;
+// with a checkpoint, 64 17.2 and 22.7, 96 21.7 and 21.4; the GELU's gradient, 2 14.1 and 21.7, 16 20.2 and 22.7, 64 39.6 and 28.0; 4096 -> 1024
+// in fp32, 2 14.9 and 18.7, 128 19.6 and 24.3.  64 ragged groups of 0 to 200 rows, 520 -> 1000: 26.7 and 24.6.
+static int few_mean(int mode) { return mode == GRADIENT8 || mode == GRADIENT16 ? 16 : mode == KEEP8 ? 64 : 96; }
 static int run(Problem p, const void* x, const void* w, const int* offsets, int rows, int nexperts, int K, int N, bool w_is_kn, int mode, cudaStream_t stream) {
   int st = checked(offsets, rows, nexperts, K, N, "grouped_gemm");
   if (st) return st;
   if (!all_aligned16({x, w, p.bias})) return fail(TMPI_ERR_INVALID, "grouped_gemm: tensors must be 16-byte aligned");
   if (!rows) return TMPI_OK;
   const int clusters = max_clusters();
-  const long long tiles_m = rows / (2 * BM) + std::min(nexperts, rows);        // at most
   p.offsets = offsets; p.rows = rows; p.experts = nexperts; p.K = K; p.N = N;
-  p.bn = tile_columns(tiles_m, N, clusters);
-  p.tiles_n = (N + p.bn - 1) / p.bn;
   p.k_blocks = (K + BK - 1) / BK;
   p.status = gemm_status_word();
+  if (rows <= (long long)few_mean(mode) * nexperts) {
+    p.tiles_n = (N + FEW_BM - 1) / FEW_BM;
+    CUtensorMap mw, mx, mx_few;
+    if (w_is_kn) st = make_tmap_bf16_3d(&mw, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, BK, 64);
+    else st = make_tmap_bf16_3d(&mw, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, FEW_BM, 64);
+    if (st || (st = make_tmap_bf16(&mx, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW_BN)) || (st = make_tmap_bf16(&mx_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW))) return st;
+    const long long tiles = ((long long)rows / FEW_BN + std::min(nexperts, rows)) * p.tiles_n;      // at most
+    void* args[] = {&mw, &mx, &mx_few, &p};
+    const cudaError_t e = launch(row_kernel(mode, w_is_kn, true), std::min<long long>(tiles, gemm_sm_count()), 1, FEW_THREADS, FEW_SMEM, args, stream);
+    return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_gemm launch: %s", cudaGetErrorString(e));
+  }
+  const long long tiles_m = rows / (2 * BM) + std::min(nexperts, rows);        // at most
+  p.bn = tile_columns(tiles_m, N, clusters);
+  p.tiles_n = (N + p.bn - 1) / p.bn;
   CUtensorMap ma, ma_few, mb, my, mz;
   if ((st = make_tmap_bf16(&ma, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, BM))) return st;
   if ((st = make_tmap_bf16(&ma_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW))) return st;
@@ -932,7 +1177,7 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   else if (mode == KEEP8 && p.q_rows16) st = make_tmap_box(&mz, 1, p.z, (uint64_t)rows, (uint64_t)N, 32, 64);
   if (st) return st;
   void* args[] = {&ma, &ma_few, &mb, &my, &mz, &p};
-  const cudaError_t e = launch(row_kernel(mode, w_is_kn), std::min<long long>(tiles_m * p.tiles_n, clusters), ROW_THREADS, SMEM, args, stream);
+  const cudaError_t e = launch(row_kernel(mode, w_is_kn, false), std::min<long long>(tiles_m * p.tiles_n, clusters), 2, ROW_THREADS, SMEM, args, stream);
   return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_gemm launch: %s", cudaGetErrorString(e));
 }
 
@@ -967,7 +1212,7 @@ int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int*
 
 // The gradients of gelu(z) h's input and value in one product: with g = dy w_e (dy [rows, K], w [experts, K, N]) in fp32 and the kept z [rows, N] (bf16, or
 // with `scale` its 8-bit checkpoint), dz = weight g gelu'(z) and h = weight gelu(z), both bf16 [rows, N]; row_weights fp32 [rows] or null for
-// ones.  dots [rows, ceil(N / 64)] (or null): the sums of g gelu(z) over 64 columns each.  Rows behind the last group are left alone.
+// ones.  dots [rows, ceil(N / 32)] (or null): the sums of g gelu(z) over 32 columns each.  Rows behind the last group are left alone.
 int tmpi_grouped_gelu_gradient(const void* dy, const void* w, const int* offsets, const void* z, const void* scale, const float* row_weights, void* dz, void* h,
                                float* dots, int rows, int nexperts, int K, int N, void* stream) {
   if (!all_aligned16({z, dz, h}) || !z || !h) return fail(TMPI_ERR_INVALID, "grouped_gelu_gradient: tensors must be 16-byte aligned");
@@ -1008,10 +1253,10 @@ int tmpi_grouped_weight_gradient(const void* dy, const void* x, const int* offse
   CUtensorMap mdy, mx, mdw;
   if ((st = make_tmap_bf16(&mdy, dy, (uint64_t)rows, (uint64_t)N, (uint64_t)N, gemm2::BK))) return st;
   if ((st = make_tmap_bf16(&mx, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, gemm2::BK))) return st;
-  if ((st = make_tmap_bf16_3d(&mdw, dw, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, 32, 32))) return st;
+  if ((st = make_tmap_bf16_3d(&mdw, dw, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, 32, 64))) return st;
   void* args[] = {&mdy, &mx, &mdw, &p};
   const cudaError_t e = grouped::launch((const void*)grouped::grouped_dw_kernel, std::min<long long>((long long)p.tiles_m * p.tiles_n * nexperts, clusters),
-                                        grouped::DW_THREADS, grouped::DW_SMEM, args, (cudaStream_t)stream);
+                                        2, grouped::DW_THREADS, grouped::DW_SMEM, args, (cudaStream_t)stream);
   return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_weight_gradient launch: %s", cudaGetErrorString(e));
 }
 

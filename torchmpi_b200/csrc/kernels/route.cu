@@ -54,6 +54,7 @@ __device__ __forceinline__ float warp_sum(float x) {
 // One token by one warp: chosen and weights of lane j < k.
 template <typename T, int NREG>
 __device__ __forceinline__ void choose(const Problem& p, const T* logits, int token, int lane, int* chosen, float* weight) {
+  static_assert(WARPS == 32, "a lane per warp in place_block");
   float l[NREG];
   uint32_t key[NREG];
   bool nan = false;
@@ -76,7 +77,7 @@ __device__ __forceinline__ void choose(const Problem& p, const T* logits, int to
     const uint32_t m = __reduce_max_sync(~0u, best);
     if (m <= KEY_NONE) break;                                      // nothing left that may be used
     if (!j) top_key = m;
-    const int i = (int)__reduce_min_sync(~0u, (unsigned)(best == m ? at : 0x7fffffff));
+    const int i = NREG == 1 ? __ffs(__ballot_sync(~0u, best == m)) - 1 : (int)__reduce_min_sync(~0u, (unsigned)(best == m ? at : 0x7fffffff));
     if (lane == j) { mine = i; my_key = m; }
 #pragma unroll
     for (int r = 0; r < NREG; ++r)
@@ -117,7 +118,8 @@ __device__ __forceinline__ void choose_block(const Problem& p, const T* logits, 
 }
 
 struct Place {
-  int base[WARPS][MAX_EXPERTS];            // a warp's choices of an expert, then the place of the next of them
+  int base[WARPS][MAX_EXPERTS + 1];        // a warp's choices of an expert, then the place of the next of them; padded, for a warp reads a column
+  int start[MAX_EXPERTS];                  // the place of the block's first choice of an expert
   int warp_sums[WARPS];
 };
 
@@ -140,24 +142,26 @@ __device__ __forceinline__ void for_choices(const Problem& p, F f) {
 // Places of this block's choices.  All threads; `s.base` is cleared here.  counts [blocks, experts] (or the block's own), of `blocks` blocks.
 __device__ __forceinline__ void place_block(const Problem& p, Place& s, const int* counts, int blocks) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < WARPS * MAX_EXPERTS; i += THREADS) (&s.base[0][0])[i] = 0;
-  // an expert's choices in all blocks and in those in front: THREADS / MAX_EXPERTS threads share an expert
-  constexpr int SHARE = THREADS / MAX_EXPERTS;
+  for (int e = lane; e < p.experts; e += 32) s.base[warp][e] = 0;
+  // an expert's choices in all blocks and in those in front: up to 32 threads share an expert
+  int share = 32;
+  while (share * p.experts > THREADS) share /= 2;
+  const int expert = tid / share;
   int before = 0, total = 0;
-  if (tid / SHARE < p.experts) {
+  if (expert < p.experts) {
 #pragma unroll 8
-    for (int b = tid % SHARE; b < blocks; b += SHARE) {
-      const int c = counts[(long long)b * p.experts + tid / SHARE];
+    for (int b = tid % share; b < blocks; b += share) {
+      const int c = counts[(long long)b * p.experts + expert];
       if (b < (int)blockIdx.x) before += c;
       total += c;
     }
   }
-#pragma unroll
-  for (int d = 1; d < SHARE; d *= 2) {
+  for (int d = 1; d < share; d *= 2) {
     before += __shfl_xor_sync(~0u, before, d);
     total += __shfl_xor_sync(~0u, total, d);
   }
-  int sum = tid % SHARE ? 0 : total;                               // inclusive prefix over the experts
+  const bool first = tid % share == 0;
+  int sum = first ? total : 0;                                     // inclusive prefix over the experts
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
     const int v = __shfl_up_sync(~0u, sum, d);
@@ -165,15 +169,21 @@ __device__ __forceinline__ void place_block(const Problem& p, Place& s, const in
   }
   if (lane == 31) s.warp_sums[warp] = sum;
   __syncthreads();                                                 // and base is clear
-  int used = 0, front = 0;
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) front += s.warp_sums[w];
-    used += s.warp_sums[w];
+  int front = s.warp_sums[lane];                                   // every warp scans the warps' sums
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int v = __shfl_up_sync(~0u, front, d);
+    if (lane >= d) front += v;
   }
-  const int begin = front + sum - total;                           // in the first thread of an expert
-  if (blockIdx.x == 0 && tid % SHARE == 0 && tid / SHARE < p.experts) {
-    p.offsets[tid / SHARE] = begin;
-    if (tid / SHARE == p.experts - 1) p.offsets[p.experts] = used;
+  const int used = __shfl_sync(~0u, front, 31);
+  front = __shfl_sync(~0u, front, (warp + 31) & 31);
+  const int begin = (warp ? front : 0) + sum - total;              // in the first thread of an expert
+  if (first && expert < p.experts) {
+    s.start[expert] = begin + before;
+    if (blockIdx.x == 0) {
+      p.offsets[expert] = begin;
+      if (expert == p.experts - 1) p.offsets[p.experts] = used;
+    }
   }
   int* mine = s.base[warp];
   for_choices(p, [&](int c, long long) {
@@ -182,13 +192,15 @@ __device__ __forceinline__ void place_block(const Problem& p, Place& s, const in
     __syncwarp();
   });
   __syncthreads();
-  if (tid % SHARE == 0 && tid / SHARE < p.experts) {
-    int next = begin + before;
-    for (int w = 0; w < WARPS; ++w) {
-      const int n = s.base[w][tid / SHARE];
-      s.base[w][tid / SHARE] = next;
-      next += n;
+  for (int e = warp; e < p.experts; e += WARPS) {                  // a warp to an expert: the counts of the block's warps, each behind those in front
+    const int n = s.base[lane][e];
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int v = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += v;
     }
+    s.base[lane][e] = s.start[e] + upto - n;
   }
   __syncthreads();
   for_choices(p, [&](int c, long long entry) {
@@ -285,16 +297,11 @@ __global__ void __launch_bounds__(GRADIENT_THREADS) gradient_kernel(const Proble
         for (int r = 0; r < NREG; ++r) d[r] = __uint_as_float(0x7fffffffu);
       }
     }
-    for (int j = 0; j < p.k; ++j) {
-      const int i = __shfl_sync(~0u, c, j);
-      const float g = __shfl_sync(~0u, p.renormalize ? wd - w * inner : wd, j);
-#pragma unroll
-      for (int r = 0; r < NREG; ++r)
-        if (i == lane + 32 * r) d[r] += g;
-    }
 #pragma unroll
     for (int r = 0; r < NREG; ++r)
       if (lane + 32 * r < p.experts) dlogits[t * p.experts + lane + 32 * r] = from_acc<T>((typename AccOf<T>::type)d[r]);
+    __syncwarp();                                                  // the chosen ones' are written over it: their p is their weight either way
+    if (c >= 0) dlogits[t * p.experts + c] = from_acc<T>((typename AccOf<T>::type)(wd - w * inner));
   }
 }
 
