@@ -6,7 +6,11 @@ The reference stops at MNIST networks; this example shows the same engine and gr
 model.  On CUDA (``EXAMPLE_DEVICE=cuda``) the model runs with ``tc_linear=True``: its matrix products, attention, layer
 norm and loss are the package's own kernels (sequence length 128 so that the attention kernel applies) and the
 optimizer is the fused allreduce + SGD; on CPU everything falls back to PyTorch and the gradients travel over gloo.
+``EXAMPLE_EXPERTS=8`` puts layers of eight experts, two for each token, in the place of the MLPs, ``EXAMPLE_ACT8=1`` keeps the
+MLPs' activations in 8 bits for the backward pass.
 """
+import os
+
 from common import device_from_env
 import torch
 import torchmpi_b200 as mpi
@@ -19,7 +23,8 @@ cuda = dev == "cuda"
 mpi.start(with_cuda=cuda)
 torch.manual_seed(0)
 T, V = (128, 64) if cuda else (32, 32)
-net = gpt2.gpt2_tiny(n_layer=2, n_head=2, n_embd=128, block_size=T, vocab_size=V, tc_linear=cuda).to(mpi.device)
+net = gpt2.gpt2_tiny(n_layer=2, n_head=2, n_embd=128, block_size=T, vocab_size=V, tc_linear=cuda,
+                     n_expert=int(os.environ.get("EXAMPLE_EXPERTS", 0)), act8=bool(int(os.environ.get("EXAMPLE_ACT8", 0)))).to(mpi.device)
 if cuda:
     net = net.to(torch.bfloat16)
 

@@ -126,8 +126,9 @@ def mlp8(x, w1, b1, w2, b2, dy):
             matmul(V(dy).t(), h.rounded()).rounded(), total(V(dy), 0).rounded())
 
 
-def experts(x, weights, chosen, w1, b1, w2, b2, dy, act8, parts=False):
-    """(y, dx, dweights, dw1, db1, dw2, db2) of experts.mlp in bf16, where x w1^T + b1 is exact in fp32.  parts: of combine, two
+def experts(x, weights, chosen, w1, b1, w2, b2, dy, act8, parts=False, exact_z=True):
+    """(y, dx, dweights, dw1, db1, dw2, db2) of experts.mlp in bf16, where x w1^T + b1 is exact in fp32 (or, without
+    act8, carries its bound: exact_z=False).  parts: of combine, two
     grouped_linear and dispatch one by one, which round the weighted rows of dy, and take the weights' gradient from what the experts returned."""
     T, k = chosen.shape
     E, (H, C) = w1.shape[0], w1.shape[1:]
@@ -146,7 +147,7 @@ def experts(x, weights, chosen, w1, b1, w2, b2, dy, act8, parts=False):
         if not len(t):
             continue
         wt = V(weights[t, j].double().unsqueeze(1))
-        z = V(x[t].double() @ w1[e].double().t() + zero_b(b1, e, H).v)
+        z = V(x[t].double() @ w1[e].double().t() + zero_b(b1, e, H).v) if exact_z else add(matmul(V(x[t]), V(w1[e]).t()), zero_b(b1, e, H))
         ys = add(matmul(gelu(z)[0].rounded(), V(w2[e]).t()), zero_b(b2, e, C)).rounded()
         into(y, t, mul(wt, ys))
         zk = V(kept(z.v)) if act8 else z.rounded()

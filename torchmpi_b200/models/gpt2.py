@@ -6,7 +6,9 @@ GPU-resident parameter server across groups.  The reference has no sequence mode
 products of the MLP and projections go through ``ops.gemm.linear`` (the tcgen05 kernel), attention through
 ``ops.attention`` (its own tcgen05 forward kernel on the packed QKV projection; PyTorch's scaled-dot-product
 attention otherwise, and for shapes that kernel does not take), layer norm through the one-pass ``ops.layernorm``
-and the LM head through the pitched ``ops.gemm.wide_head``; the loss is ``ops.xent``.
+and the LM head through the pitched ``ops.gemm.wide_head``; the loss is ``ops.xent``.  ``n_expert`` puts a layer of experts
+(``ops.experts.Experts``, ``expert_k`` of them for each token) in the place of each block's MLP; ``act8`` keeps the MLPs'
+activations in 8 bits for the backward pass (``ops.act8``).
 """
 from __future__ import annotations
 
@@ -26,6 +28,9 @@ class GPT2Config:
     block_size: int = 1024
     vocab_size: int = 50257
     tc_linear: bool = False
+    n_expert: int = 0
+    expert_k: int = 2
+    act8: bool = False
 
 
 def gpt2_medium(**kw) -> "GPT2":
@@ -67,12 +72,29 @@ class Block(nn.Module):
         self.qkv = _Linear(c.n_embd, 3 * c.n_embd, c.tc_linear)
         self.proj = _Linear(c.n_embd, c.n_embd, c.tc_linear)
         self.ln2 = _layer_norm(c)
-        self.fc = _Linear(c.n_embd, 4 * c.n_embd, c.tc_linear, gelu=True)
-        self.out = _Linear(4 * c.n_embd, c.n_embd, c.tc_linear)
+        self.act8 = c.act8
+        if c.n_expert:
+            from ..ops.experts import Experts
+            self.experts = Experts(c.n_embd, 4 * c.n_embd, c.n_expert, c.expert_k, act8=c.act8)
+        else:
+            self.fc = _Linear(c.n_embd, 4 * c.n_embd, c.tc_linear, gelu=True)
+            self.out = _Linear(4 * c.n_embd, c.n_embd, c.tc_linear)
 
     def _attention(self, qkv):
         from ..ops import attention
         return attention.causal_attention(qkv, self.n_head)
+
+    def _mlp_apart(self, h):
+        """The MLP's output where it is no pair of linear layers, else None: a layer of experts, or one function with 8-bit checkpoints
+        (not where a layer is replaced or hooked, which would see neither input nor output)."""
+        if "experts" in self._modules:
+            return self.experts(h)
+        if self.act8:
+            from ..ops import act8
+            from ..ops.conv import bare
+            if all(type(self._modules[n]) is _Linear and bare(self._modules[n]) for n in ("fc", "out")):
+                return act8.mlp(h, self.fc.weight, self.fc.bias, self.out.weight, self.out.bias)
+        return None
 
     def _sums_in_kernels(self, x) -> bool:
         """Whether the residual sums can be formed inside the projections (forward) and the layer norms (backward): the kernels'
@@ -85,7 +107,8 @@ class Block(nn.Module):
         if not all(type(mods[n]) is layernorm.LayerNorm and bare(mods[n]) and mods[n].normalized_shape == x.shape[-1:]
                    and layernorm.supported(x, mods[n].weight, mods[n].bias) for n in ("ln1", "ln2")):
             return False
-        return all(type(mods[n]) is _Linear and mods[n].tc and not mods[n].gelu and bare(mods[n]) for n in ("proj", "out"))
+        return all(type(mods[n]) is _Linear and mods[n].tc and not mods[n].gelu and bare(mods[n])
+                   for n in ("proj", "out") if n in mods)
 
     def forward(self, x):
         if self._sums_in_kernels(x):
@@ -93,6 +116,9 @@ class Block(nn.Module):
             h, x = layernorm.layer_norm_fork(x, self.ln1.weight, self.ln1.bias, self.ln1.eps)
             x = gemm.linear_add(self._attention(self.qkv(h)), self.proj.weight, self.proj.bias, x)
             h, x = layernorm.layer_norm_fork(x, self.ln2.weight, self.ln2.bias, self.ln2.eps)
+            y = self._mlp_apart(h)
+            if y is not None:
+                return x + y
             return gemm.linear_add(self.fc(h), self.out.weight, self.out.bias, x)
         B, T, C = x.shape
         qkv = self.qkv(self.ln1(x).to(x.dtype))
@@ -102,7 +128,9 @@ class Block(nn.Module):
             q, k, v = (t.view(B, T, self.n_head, C // self.n_head).transpose(1, 2) for t in qkv.split(C, dim=2))
             a = F.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2).reshape(B, T, C)
         x = x + self.proj(a)
-        return x + self.out(self.fc(self.ln2(x).to(x.dtype)))
+        h = self.ln2(x).to(x.dtype)
+        y = self._mlp_apart(h)
+        return x + (self.out(self.fc(h)) if y is None else y)
 
 
 class GPT2(nn.Module):
@@ -115,8 +143,8 @@ class GPT2(nn.Module):
         self.ln_f = _layer_norm(c)
         self.apply(self._init)
         for b in self.blocks:   # scaled init of the residual projections
-            for lin in (b.proj, b.out):
-                nn.init.normal_(lin.weight, std=0.02 / math.sqrt(2 * c.n_layer))
+            for w in (b.proj.weight, b.experts.w2 if c.n_expert else b.out.weight):
+                nn.init.normal_(w, std=0.02 / math.sqrt(2 * c.n_layer))
 
     @staticmethod
     def _init(m):

@@ -31,6 +31,8 @@ def main():
     ap.add_argument("--warmup", type=int, default=4)
     ap.add_argument("--update-frequency", type=int, default=4)
     ap.add_argument("--tc-linear", type=int, default=1)
+    ap.add_argument("--n-expert", type=int, default=0, help="layers of so many experts, two for each token, in the place of the MLPs")
+    ap.add_argument("--act8", type=int, default=0, help="keep the MLPs' activations in 8 bits for the backward pass")
     ap.add_argument("--profile-one-step", action="store_true",
                     help="after the warm-up run one step between cudaProfilerStart/Stop and exit (no timing)")
     args = ap.parse_args()
@@ -49,8 +51,8 @@ def main():
     mpi.set_communicator(0)
     rank, world, dev = mpi.world_rank(), mpi.world_size(), mpi.device
     torch.manual_seed(1)
-    model = (gpt2.gpt2_medium(tc_linear=bool(args.tc_linear)) if args.model == "gpt2_medium"
-             else gpt2.gpt2_tiny(tc_linear=bool(args.tc_linear), block_size=args.seq))
+    form = dict(tc_linear=bool(args.tc_linear), n_expert=args.n_expert, act8=bool(args.act8))
+    model = gpt2.gpt2_medium(**form) if args.model == "gpt2_medium" else gpt2.gpt2_tiny(block_size=args.seq, **form)
     model = model.to(dev).to(torch.bfloat16)
     seq = min(args.seq, model.config.block_size)
     vocab = model.config.vocab_size

@@ -225,6 +225,41 @@ def lazy_cases(small: bool) -> dict:
     out["layernorm_fwd"] = ln_case(False)
     out["layernorm_bwd"] = ln_case(True)
 
+    def grouped_case(which):
+        def build():
+            from torchmpi_b200.ops import experts
+            R, E, C, H = (8192 if small else 16384), 8, 1024, 4096           # 8 x 1024 tokens, two experts each
+            x = torch.randn(R, C, device=dev).to(torch.bfloat16)
+            w = (torch.randn(E, H, C, device=dev) * C ** -0.5).to(torch.bfloat16)
+            b = torch.zeros(E, H, device=dev, dtype=torch.bfloat16)
+            offsets = torch.arange(0, R + 1, R // E, device=dev, dtype=torch.int32)
+            flops, nbytes = 2.0 * R * C * H, 2 * (R * (C + H) + E * C * H)
+            if which == "up":
+                return (lambda: experts.grouped_linear(x, w, b, offsets, gelu=True)), nbytes, flops
+            dy = torch.randn(R, H, device=dev).to(torch.bfloat16)
+            leaf = (x if which == "dx" else w).requires_grad_(True)
+            y = experts.grouped_linear(x, w, b, offsets)
+            return (lambda: torch.autograd.grad(y, leaf, dy, retain_graph=True)), nbytes, flops
+        return build
+    for which in ("up", "dx", "dw"):
+        out[f"grouped_{which}"] = grouped_case(which)
+
+    def act8_case(which):
+        def build():
+            from torchmpi_b200.ops import act8
+            rows, C = (16384 if small else 65536), 4096
+            x = torch.randn(rows, C, device=dev).to(torch.bfloat16)
+            kept = act8.quantize(x)
+            n = x.numel()
+            if which == "quantize":
+                return (lambda: act8.quantize(x)), n * 3 + n // 32
+            if which == "dequantize":
+                return (lambda: act8.dequantize(kept)), n * 3 + n // 32
+            return (lambda: act8.gelu_gradient(x, kept)), n * 7 + n // 32
+        return build
+    for which in ("quantize", "dequantize", "gelu_gradient"):
+        out[f"act8_{which}"] = act8_case(which)
+
     def pool_case():
         N, C, H = (B, 64, 112)
         x = torch.randn(N, C, H, H, device=dev).to(torch.bfloat16).contiguous(memory_format=torch.channels_last).requires_grad_(True)
