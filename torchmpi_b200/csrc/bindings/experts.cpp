@@ -168,29 +168,37 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
 };
 
 // ---------------------------------------------------------------- routing
+Tensor dense_columns(const Tensor& l) { return l.stride(1) == 1 && (l.size(0) < 2 || l.stride(0) >= l.size(1)) ? l : l.contiguous(); }
+
+// weights, chosen, order, place, offsets
+variable_list route(const Tensor& logits, int64_t k, bool renormalize) {
+  const int T = (int)logits.size(0), E = (int)logits.size(1);
+  const auto i32 = logits.options().dtype(at::kInt);
+  Tensor weights = at::empty({T, k}, logits.options().dtype(at::kFloat)), chosen = at::empty({T, k}, i32), order = at::empty({T * k}, i32),
+         place = at::empty({T, k}, i32), offsets = at::empty({E + 1}, i32), ws;
+  const size_t need = tmpi_route_workspace_bytes(T, E, (int)k);
+  if (need) ws = at::empty({(int64_t)need}, logits.options().dtype(at::kByte));
+  check(tmpi_route(logits.data_ptr(), T > 1 ? logits.stride(0) : E, T, E, (int)k, renormalize, dtype_code(logits.scalar_type()), weights.data_ptr<float>(),
+                   chosen.data_ptr<int>(), order.data_ptr<int>(), place.data_ptr<int>(), offsets.data_ptr<int>(), need ? ws.data_ptr() : nullptr, need, stream()));
+  launched(EXPERTS, need ? 2 : 1);
+  return {weights, chosen, order, place, offsets};
+}
+
 struct RouteFn : public torch::autograd::Function<RouteFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits_, int64_t k, bool renormalize) {
-    const Tensor logits = logits_.stride(1) == 1 && (logits_.size(0) < 2 || logits_.stride(0) >= logits_.size(1)) ? logits_ : logits_.contiguous();
-    const int T = (int)logits.size(0), E = (int)logits.size(1);
-    const auto i32 = logits.options().dtype(at::kInt);
-    Tensor weights = at::empty({T, k}, logits.options().dtype(at::kFloat)), chosen = at::empty({T, k}, i32), order = at::empty({T * k}, i32),
-           place = at::empty({T, k}, i32), offsets = at::empty({E + 1}, i32), ws;
-    const size_t need = tmpi_route_workspace_bytes(T, E, (int)k);
-    if (need) ws = at::empty({(int64_t)need}, logits.options().dtype(at::kByte));
-    check(tmpi_route(logits.data_ptr(), T > 1 ? logits.stride(0) : E, T, E, (int)k, renormalize, dtype_code(logits.scalar_type()), weights.data_ptr<float>(),
-                     chosen.data_ptr<int>(), order.data_ptr<int>(), place.data_ptr<int>(), offsets.data_ptr<int>(), need ? ws.data_ptr() : nullptr, need, stream()));
-    launched(EXPERTS, need ? 2 : 1);
-    ctx->save_for_backward({logits, weights, chosen});
+    const Tensor logits = dense_columns(logits_);
+    variable_list r = route(logits, k, renormalize);
+    ctx->save_for_backward({logits, r[0], r[1]});
     ctx->saved_data["k"] = k;
     ctx->saved_data["renormalize"] = renormalize;
-    ctx->mark_non_differentiable({chosen, order, place, offsets});
+    ctx->mark_non_differentiable({r[1], r[2], r[3], r[4]});
     ctx->set_materialize_grads(false);                              // or autograd fills a tensor with zeros for each of them
-    return {weights, chosen, order, place, offsets};
+    return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const Tensor logits = saved[0].stride(1) == 1 && (saved[0].size(0) < 2 || saved[0].stride(0) >= saved[0].size(1)) ? saved[0] : saved[0].contiguous();
+    const Tensor logits = dense_columns(saved[0]);
     const Tensor weights = as_saved(saved[1]), chosen = as_saved(saved[2]), dw = packed(grads[0].to(at::kFloat));
     const int T = (int)logits.size(0), E = (int)logits.size(1);
     Tensor dl = at::empty({T, E}, logits.options());
@@ -260,34 +268,37 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
 // in bf16 or (act8) in 8 bits, and neither the dispatched rows nor what the experts returned: the rows are gathered again, and the weight's gradient
 // dy . (w2 h + b2) is (w2^T dy) . h + dy . b2, of which the first product is there anyway.  What a token's experts return, and the gradients
 // that they return to it, are handed over in fp32 and rounded once, as their sum.
-struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weights_, const Tensor& chosen_, const Tensor& place_, const Tensor& offsets_,
-                        const Tensor& w1_, const OptTensor& b1_, const Tensor& w2_, const OptTensor& b2_, bool act8, bool keep) {
-    const Tensor x = packed(x_), weights = weights_.contiguous(), chosen = chosen_.contiguous(), place = place_.contiguous(),
-                 offsets = offsets_.contiguous(), w1 = packed(w1_), w2 = packed(w2_), b1 = b1_.has_value() ? packed(*b1_) : Tensor(),
-                 b2 = b2_.has_value() ? packed(*b2_) : Tensor();
-    const int64_t T = place.size(0), k = place.size(1), H = w1.size(1);
-    Tensor xs;
-    Kept kx, kz;
-    if (keep && act8) {
-      kx = empty_kept(x, x.sizes());
-      kz = empty_kept(x, {T * k, H});
-      xs = at::empty({T * k, x.size(1)}, x.options());
-      check(tmpi_expert_dispatch_keep(x.data_ptr(), place.data_ptr<int>(), xs.data_ptr(), kx.q.data_ptr(), kx.scale.data_ptr(), (int)T, (int)k, (int)x.size(1), stream()));
-      launched(EXPERTS, 1);
-    } else {
-      xs = dispatch(x, place, Tensor());
-      if (keep) {
-        kx.q = x;
-        kz.q = at::empty({T * k, H}, x.options());
-      }
-    }
-    const Tensor h = grouped(xs, w1, b1, offsets, false, !keep ? GELU : act8 ? GELU_AND_Z8 : GELU_AND_Z, kz.q, kz.scale);
-    const Tensor y = combine(grouped(h, w2, b2, offsets, false, FP32, Tensor(), Tensor()), weights, place, x.scalar_type());
+struct Layer { Tensor x, weights, chosen, place, offsets, w1, b1, w2, b2; };
+
+// keep: the checkpoints go to kx and kz
+Tensor expert_forward(const Layer& l, bool act8, bool keep, Kept* kx, Kept* kz) {
+  const int64_t T = l.place.size(0), k = l.place.size(1), H = l.w1.size(1);
+  Tensor xs;
+  if (keep && act8) {
+    *kx = empty_kept(l.x, l.x.sizes());
+    *kz = empty_kept(l.x, {T * k, H});
+    xs = at::empty({T * k, l.x.size(1)}, l.x.options());
+    check(tmpi_expert_dispatch_keep(l.x.data_ptr(), l.place.data_ptr<int>(), xs.data_ptr(), kx->q.data_ptr(), kx->scale.data_ptr(), (int)T, (int)k, (int)l.x.size(1), stream()));
+    launched(EXPERTS, 1);
+  } else {
+    xs = dispatch(l.x, l.place, Tensor());
     if (keep) {
-      ctx->save_for_backward({kx.q, kx.scale, kz.q, kz.scale, weights, chosen, place, offsets, w1, w2, b2});
-      ctx->saved_data["b1"] = b1.defined();
+      kx->q = l.x;
+      kz->q = at::empty({T * k, H}, l.x.options());
     }
+  }
+  const Tensor h = grouped(xs, l.w1, l.b1, l.offsets, false, !keep ? GELU : act8 ? GELU_AND_Z8 : GELU_AND_Z, kz->q, kz->scale);
+  return combine(grouped(h, l.w2, l.b2, l.offsets, false, FP32, Tensor(), Tensor()), l.weights, l.place, l.x.scalar_type());
+}
+
+struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weights, const Tensor& chosen, const Tensor& place, const Tensor& offsets, const Tensor& w1,
+                        const OptTensor& b1, const Tensor& w2, const OptTensor& b2, bool act8) {
+    const Layer l{x, weights, chosen, place, offsets, w1, or_none(b1), w2, or_none(b2)};
+    Kept kx, kz;
+    const Tensor y = expert_forward(l, act8, true, &kx, &kz);
+    ctx->save_for_backward({kx.q, kx.scale, kz.q, kz.scale, weights, chosen, place, offsets, w1, w2, l.b2});
+    ctx->saved_data["b1"] = l.b1.defined();
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -328,7 +339,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     }
     if (need_x) dx = combine(grouped(dz, w1, Tensor(), offsets, true, FP32, Tensor(), Tensor()), Tensor(), place, dy.scalar_type());
     const Tensor none;
-    return {dx, dwt, none, none, none, need_w1 ? dw1 : none, db1, need_w2 ? dw2 : none, db2, none, none};
+    return {dx, dwt, none, none, none, need_w1 ? dw1 : none, db1, need_w2 ? dw2 : none, db2, none};
   }
 };
 
@@ -381,18 +392,20 @@ void register_experts(pybind11::module_& m) {
     check(tmpi_route_limits(&experts, &most));
     const int64_t T = logits.size(0), E = logits.size(1);
     if (!(k >= 1 && k <= E && E <= experts && k <= most && T * k <= MOST)) return c10::nullopt;
-    const variable_list r = RouteFn::apply(logits, k, renormalize);
+    const variable_list r = wants_grad({logits}) ? RouteFn::apply(logits, k, renormalize) : route(dense_columns(logits), k, renormalize);
     return std::make_tuple(r[0], r[1], r[2], r[3], r[4]);
   });
   m.def("expert_dispatch", [](const Tensor& x, const Tensor& place, const Tensor& offsets) -> OptTensor {
     if (!(x.is_cuda() && x.dim() == 2 && floating(x) && x.numel() && place.dim() == 2 && offsets.dim() == 1 && offsets.size(0) >= 1 && all_of_type({&place, &offsets}, at::kInt) &&
           here({&x, &place, &offsets}) && place.size(0) == x.size(0) && place.numel() && place.numel() <= MOST && x.size(1) <= MOST)) return c10::nullopt;
+    if (!wants_grad({x})) return dispatch(packed(x), place.contiguous(), offsets.contiguous());
     return DispatchFn::apply(x, place, offsets);
   });
   m.def("expert_combine", [](const Tensor& rows, const Tensor& weights, const Tensor& place, const Tensor& offsets) -> OptTensor {
     if (!(rows.is_cuda() && rows.dim() == 2 && floating(rows) && rows.numel() && place.dim() == 2 && offsets.dim() == 1 && offsets.size(0) >= 1 && all_of_type({&place, &offsets}, at::kInt) &&
           weights.scalar_type() == at::kFloat && weights.sizes() == place.sizes() && here({&rows, &weights, &place, &offsets}) && place.numel() == rows.size(0) && place.numel() <= MOST &&
           rows.size(1) <= MOST)) return c10::nullopt;
+    if (!wants_grad({rows, weights})) return combine(packed(rows), weights.contiguous(), place.contiguous(), rows.scalar_type());
     return CombineFn::apply(rows, weights, place, offsets);
   });
   m.def("expert_mlp", [](const Tensor& x, const Tensor& weights, const Tensor& chosen, const Tensor& order, const Tensor& place, const Tensor& offsets,
@@ -404,7 +417,15 @@ void register_experts(pybind11::module_& m) {
     const int64_t E = w1.size(0), H = w1.size(1), C = w1.size(2), T = place.size(0), k = place.size(1);
     if (!(x.size(-1) == C && x.numel() == T * C && shaped(weights, {T, k}) && shaped(chosen, {T, k}) && shaped(order, {T * k}) && shaped(offsets, {E + 1}) && shaped(w2, {E, C, H}) &&
           shaped(b1, {E, H}) && shaped(b2, {E, C}) && C % 8 == 0 && H % 8 == 0 && w1.numel() && E <= tmpi_grouped_max_experts() && T && T * k && T * k <= MOST)) return c10::nullopt;
-    const Tensor y = ExpertsFn::apply(rows_of(x), weights, chosen, place, offsets, w1, b1_, w2, b2_, act8, wants_grad({x, weights, w1, w2, b1, b2}));
+    const Layer l{packed(rows_of(x)), weights.contiguous(), chosen.contiguous(), place.contiguous(), offsets.contiguous(), packed(w1), b1.defined() ? packed(b1) : b1,
+                  packed(w2), b2.defined() ? packed(b2) : b2};
+    Tensor y;
+    if (wants_grad({x, weights, w1, w2, b1, b2})) {
+      y = ExpertsFn::apply(l.x, l.weights, l.chosen, l.place, l.offsets, l.w1, b1.defined() ? OptTensor(l.b1) : OptTensor(), l.w2, b2.defined() ? OptTensor(l.b2) : OptTensor(), act8);
+    } else {
+      Kept none;
+      y = expert_forward(l, act8, false, &none, &none);
+    }
     return x.dim() == 2 ? y : y.view(x.sizes());
   });
 }

@@ -11,8 +11,8 @@
 // expert's, whose infinities would come back as NaN.
 //
 // The weights' gradient has the rows as its K.  The last 64 rows of a group may hold rows of the next one: a warp of each CTA waits
-// for that block's loads and overwrites those rows with zeros in both operands (zero times infinity is not zero); the even CTA's, once both are done,
-// lets the MMAs read the block.  db is
+// for that block's loads and overwrites those rows with zeros in both operands (zero times infinity is not zero), as far as the
+// MMAs read; the issuer waits for both CTAs' warps there.  db is
 // summed by the epilogue warps under the tile's MMAs, in fp32 and in short chains, as in linear_bwd.cu.  Experts without rows get zeros.
 #include "act8.cuh"
 #include "attn_util.cuh"
@@ -531,7 +531,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 // weights' way from memory: 96 KB of them are under way per SM.
 // A thread has a column of y and walks the rows, so a warp's stores are 64 bytes of a row each, the 32 columns of an 8-bit block are its lanes', and a row
 // behind the group's end is not touched.
-constexpr int FEW_BM = 128, FEW_BN = 128, FEW_STAGES = 6, FEW_EPI_WARPS = 8, FEW_THREADS = 64 + FEW_EPI_WARPS * 32;
+constexpr int FEW_BM = 128, FEW_BN = 128, FEW_STAGES = 6, FEW_EPI_WARPS = 16, FEW_THREADS = 64 + FEW_EPI_WARPS * 32;
 constexpr int FEW_A_BYTES = FEW_BM * BK * 2, FEW_STAGE_BYTES = FEW_A_BYTES + FEW_BN * BK * 2;
 constexpr size_t FEW_SMEM = (size_t)FEW_STAGES * FEW_STAGE_BYTES + 1024 + 1280;
 static_assert(FEW_STAGES == STAGES && FEW_SMEM <= 232448, "shared memory of one CTA");
@@ -566,7 +566,7 @@ __device__ __forceinline__ float one_gelu(float z) {
 }
 
 template <int MODE>
-__device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights, int half, int quarter, int lane) {
+__device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights, int group, int quarter, int lane) {
   constexpr bool GRADIENT = MODE == GRADIENT8 || MODE == GRADIENT16;
   const int N = p.N, blocks = (N + 31) / 32;
   for_few(sh, p, offsets, [&](int e, int row0, int rows, int col0, int it) -> bool {
@@ -576,23 +576,25 @@ __device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* 
     if (!sm100::mbar_wait_warp(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 54); return false; }
     sm100::tc_fence_after();
     const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * FEW_BN;
-    // the two groups of warps take 16 rows in turn
-    for (int c = half * 16; c < rows && col0 + quarter * 32 < N; c += 32) {
+    // the four groups of warps take 16 rows in turn
+    for (int c = group * 16; c < rows && col0 + quarter * 32 < N; c += FEW_EPI_WARPS * 4) {
+      const int left = rows - c;
+      const long long at0 = (long long)(row0 + c) * N + col;
       uint32_t r[16];
       float z_of[GRADIENT ? 16 : 1], weight_of[GRADIENT ? 16 : 1];
       if (GRADIENT) {                                    // all that these rows need, at once
         uint32_t kept[16], scales[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const bool there = in && c + j < rows;
-          const long long row = row0 + c + j, at = row * N + col;
+          const bool there = in && j < left;
+          const long long row = row0 + c + j, at = at0 + (long long)j * N;
           if (MODE == GRADIENT8) {
             kept[j] = there ? ((const uint8_t*)p.z)[at] : 0u;
             scales[j] = there ? p.scale[row * blocks + col / 32] : 1u;
           } else {
             z_of[j] = there ? __bfloat162float(((const __nv_bfloat16*)p.z)[at]) : 0.f;
           }
-          weight_of[j] = row_weights && c + j < rows ? __ldg(row_weights + row) : 1.f;
+          weight_of[j] = row_weights && j < left ? __ldg(row_weights + row) : 1.f;
         }
         if (MODE == GRADIENT8) {
 #pragma unroll
@@ -606,12 +608,12 @@ __device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* 
       sm100::tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        if (c + j >= rows) break;
-        const long long row = row0 + c + j, at = row * N + col;
+        if (MODE != PLAIN32 && MODE != PLAIN && j >= left) break;
+        const long long row = row0 + c + j, at = at0 + (long long)j * N;
         float v = __uint_as_float(r[j]);
         if (!GRADIENT) v += bias;
         if (MODE == PLAIN32) {
-          if (in) p.y32[at] = v;
+          if (in && j < left) p.y32[at] = v;
         } else if (GRADIENT) {
           const float z = z_of[GRADIENT ? j : 0], weight = weight_of[GRADIENT ? j : 0];
           float y0, y1, d0, d1;
@@ -637,7 +639,7 @@ __device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* 
             if (lane == 0) p.scale[row * blocks + col / 32] = (uint8_t)byte;
           }
           if (MODE != PLAIN) v = one_gelu(v);
-          if (in) p.y[at] = __float2bfloat16_rn(v);
+          if (in && j < left) p.y[at] = __float2bfloat16_rn(v);
         }
       }
     }
@@ -657,8 +659,8 @@ __device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* 
 
 template <int MODE, bool W_MN>
 __global__ void __launch_bounds__(FEW_THREADS, 1)
-grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x_few,
-                   const __grid_constant__ Problem p) {
+grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x_half,
+                   const __grid_constant__ CUtensorMap map_x_few, const __grid_constant__ Problem p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   Sh* sh = reinterpret_cast<Sh*>(tiles + (size_t)FEW_STAGES * FEW_STAGE_BYTES);
@@ -690,7 +692,8 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (sm100::elect_one()) {
       Ring ring{0, 0};
       for_few(sh, p, offsets, [&](int e, int row0, int rows, int col0, int) -> bool {
-        const uint32_t tx = FEW_A_BYTES + (rows > FEW ? FEW_BN : FEW) * BK * 2;
+        const CUtensorMap* map = rows > FEW_BN / 2 ? &map_x : rows > FEW ? &map_x_half : &map_x_few;
+        const uint32_t tx = FEW_A_BYTES + (rows > FEW_BN / 2 ? FEW_BN : rows > FEW ? FEW_BN / 2 : FEW) * BK * 2;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           const int stage = ring.stage;
           if (!sm100::mbar_wait(&sh->empty[stage], ring.phase ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 51); return false; }
@@ -702,7 +705,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             sm100::tma_load_3d(dst, &map_w, col0, kb * BK, e, &sh->full[stage]);
             sm100::tma_load_3d(dst + FEW_A_BYTES / 2, &map_w, col0 + 64, kb * BK, e, &sh->full[stage]);
           }
-          sm100::tma_load_2d(dst + FEW_A_BYTES, rows > FEW ? &map_x : &map_x_few, kb * BK, row0, &sh->full[stage]);
+          sm100::tma_load_2d(dst + FEW_A_BYTES, map, kb * BK, row0, &sh->full[stage]);
           advance<FEW_STAGES>(&ring);
         }
         return true;
@@ -864,15 +867,14 @@ __device__ __forceinline__ void dw_clear(DwSh* shl, unsigned char* tiles, const 
       if (!sm100::mbar_wait_warp(&shl->tail[at], phase, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 45); return false; }
       phases ^= 1u << at;
       unsigned char* box = tiles + (size_t)at * STAGE_BYTES;
+      const int upto = (rem + UMMA_K - 1) / UMMA_K * UMMA_K;         // the MMAs read no further
       for (int b = 0; b < boxes; ++b)
-        for (int c = rem * 8 + lane; c < BK * 8; c += 32) *reinterpret_cast<uint4*>(box + b * (BK * 128) + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = rem * 8 + lane; c < upto * 8; c += 32) *reinterpret_cast<uint4*>(box + b * (BK * 128) + c * 16) = make_uint4(0u, 0u, 0u, 0u);
       sm100::fence_proxy_async_smem();
       __syncwarp();
-      if (rank) {
-        if (lane == 0) sm100::mbar_arrive_cluster(sm100::map_to_cta(&shl->cleared[at], 0));
-      } else {
-        if (!sm100::mbar_wait_warp(&shl->cleared[at], phase, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 46); return false; }
-        if (lane == 0) sm100::mbar_arrive(&sh->full[at]);
+      if (lane == 0) {                                   // the issuer waits for both
+        if (rank) sm100::mbar_arrive_cluster(sm100::map_to_cta(&shl->cleared[at], 0));
+        else sm100::mbar_arrive(&sh->full[at]);
       }
     }
     stage = (stage + u.k_blocks) % DW_STAGES;
@@ -886,6 +888,7 @@ __device__ __forceinline__ void dw_issue(DwSh* shl, unsigned char* tiles, const 
   const uint32_t idesc = sm100::make_idesc_f16(2 * BM, p.bn, true, true, true);
   Ring ring{0, 0};
   int it = 0;
+  uint32_t cleared = 0;                                  // phases of the barriers of the odd CTA's clearing
   for_units(p, offsets, 0, [&](const DwUnit& u) -> bool {
     if (!u.k_blocks) return true;
     const int acc = it & 1;
@@ -896,10 +899,16 @@ __device__ __forceinline__ void dw_issue(DwSh* shl, unsigned char* tiles, const 
     for (int kb = 0; kb < u.k_blocks; ++kb) {
       const int stage = ring.stage;
       if (!sm100::mbar_wait(&sh->full[stage], ring.phase, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 43); return false; }
+      const int left = u.r1 - u.r0 - kb * BK;
+      if (left < BK) {
+        if (!sm100::mbar_wait(&shl->cleared[stage], cleared >> stage & 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 46); return false; }
+        cleared ^= 1u << stage;
+      }
       sm100::tc_fence_after();
       const uint32_t a = sm100::smem_u32(tiles + (size_t)stage * STAGE_BYTES), b = a + A_BYTES;
 #pragma unroll
       for (int k = 0; k < BK / UMMA_K; ++k) {
+        if (k * UMMA_K >= left) break;
         const uint64_t da = sm100::make_desc_sw128_mn(a + k * UMMA_K * 128, A_BYTES / 2, 1024);
         const uint64_t db = sm100::make_desc_sw128_mn(b + k * UMMA_K * 128, B_BYTES / 2, 1024);
         sm100::umma_f16_pair(d, da, db, idesc, (uint32_t)kb | (uint32_t)k);
@@ -1135,10 +1144,11 @@ static int checked(const int* offsets, int rows, int nexperts, int K, int N, con
 }
 
 // Rows to an expert, on average, up to which the product is formed the other way round.  Its epilogue takes a row at a time, and longer the more it does.
-// us of this form and the other, 8 experts, 1024 -> 4096: GELU with 2 rows each 12.7 and 18.2, 64 13.3 and 19.7, 128 17.0 and 19.0, 192 27.5 and 19.7;
-// with a checkpoint, 64 17.2 and 22.7, 96 21.7 and 21.4; the GELU's gradient, 2 14.1 and 21.7, 16 20.2 and 22.7, 64 39.6 and 28.0; 4096 -> 1024
-// in fp32, 2 14.9 and 18.7, 128 19.6 and 24.3.  64 ragged groups of 0 to 200 rows, 520 -> 1000: 26.7 and 24.6.
-static int few_mean(int mode) { return mode == GRADIENT8 || mode == GRADIENT16 ? 16 : mode == KEEP8 ? 64 : 96; }
+// us of this form and the other, 8 experts, 1024 -> 4096: GELU with 2 rows each 12.7 and 19.2, 64 12.8 and 20.1, 128 15.7 and 19.5, 160 24.0 and 19.8;
+// with a checkpoint, 64 14.6 and 22.9, 160 33.3 and 23.2; the GELU's gradient, 2 13.3 and 21.5, 64 20.6 and 27.3, 96 31.1 and 25.1; 4096 -> 1024
+// in fp32, 2 15.2 and 18.7, 128 18.2 and 23.8.  64 ragged groups of 0 to 200 rows, 80 on average, 520 -> 1000: 25.0 and 24.9, with a checkpoint 36.8 and
+// 33.5; of half as many, 16.9 and 21.4, with a checkpoint 21.9 and 28.9, the gradient 36.0 and 34.7.
+static int few_mean(int mode) { return mode == GRADIENT8 || mode == GRADIENT16 ? 32 : mode == KEEP8 ? 64 : 96; }
 static int run(Problem p, const void* x, const void* w, const int* offsets, int rows, int nexperts, int K, int N, bool w_is_kn, int mode, cudaStream_t stream) {
   int st = checked(offsets, rows, nexperts, K, N, "grouped_gemm");
   if (st) return st;
@@ -1150,12 +1160,14 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   p.status = gemm_status_word();
   if (rows <= (long long)few_mean(mode) * nexperts) {
     p.tiles_n = (N + FEW_BM - 1) / FEW_BM;
-    CUtensorMap mw, mx, mx_few;
+    CUtensorMap mw, mx, mx_half, mx_few;
     if (w_is_kn) st = make_tmap_bf16_3d(&mw, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, BK, 64);
     else st = make_tmap_bf16_3d(&mw, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, FEW_BM, 64);
-    if (st || (st = make_tmap_bf16(&mx, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW_BN)) || (st = make_tmap_bf16(&mx_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW))) return st;
+    if (st || (st = make_tmap_bf16(&mx, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW_BN)) ||
+        (st = make_tmap_bf16(&mx_half, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW_BN / 2)) ||
+        (st = make_tmap_bf16(&mx_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW))) return st;
     const long long tiles = ((long long)rows / FEW_BN + std::min(nexperts, rows)) * p.tiles_n;      // at most
-    void* args[] = {&mw, &mx, &mx_few, &p};
+    void* args[] = {&mw, &mx, &mx_half, &mx_few, &p};
     const cudaError_t e = launch(row_kernel(mode, w_is_kn, true), std::min<long long>(tiles, gemm_sm_count()), 1, FEW_THREADS, FEW_SMEM, args, stream);
     return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_gemm launch: %s", cudaGetErrorString(e));
   }
