@@ -81,7 +81,7 @@ bool is_kept(const Tensor& q, const Tensor& scale) {
 Tensor grouped(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& offsets, bool w_is_kn, int mode, const Tensor& z, const Tensor& scale) {
   const int experts = offsets.defined() ? (int)w.size(0) : 1, d = (int)w.dim();
   const int N = (int)w.size(w_is_kn ? d - 1 : d - 2), K = (int)x.size(1);
-  Tensor y = at::empty({x.size(0), N}, mode == FP32 ? x.options().dtype(at::kFloat) : x.options());
+  Tensor y = mode == FP32 ? at::empty({tmpi_grouped_slices((int)x.size(0), experts, K, N) * x.size(0), N}, x.options().dtype(at::kFloat)) : at::empty({x.size(0), N}, x.options());
   check(tmpi_grouped_gemm(x.data_ptr(), w.data_ptr(), ptr(bias), ints(offsets), y.data_ptr(), z.defined() ? z.data_ptr() : nullptr,
                           scale.defined() ? scale.data_ptr() : nullptr, (int)x.size(0), experts, K, N, w_is_kn ? 1 : 0, mode, stream()));
   launched(EXPERTS, 1);
@@ -221,11 +221,11 @@ Tensor dispatch(const Tensor& x, const Tensor& place, const Tensor& offsets, con
   launched(EXPERTS, 1);
   return out;
 }
-// rows of `type`, or in fp32 for bf16
+// rows of `type`, or for bf16 in fp32, as many results as grouped() has left there
 Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place, at::ScalarType type) {
-  const bool fp32 = type == at::kBFloat16 && rows.scalar_type() == at::kFloat;
+  const int slices = type == at::kBFloat16 && rows.scalar_type() == at::kFloat ? (int)(rows.size(0) / place.numel()) : 0;
   Tensor y = at::empty({place.size(0), rows.size(1)}, rows.options().dtype(type));
-  check(tmpi_expert_combine(rows.data_ptr(), fp32, weights.defined() ? weights.data_ptr<float>() : nullptr, place.data_ptr<int>(), y.data_ptr(), (int)place.size(0),
+  check(tmpi_expert_combine(rows.data_ptr(), slices, weights.defined() ? weights.data_ptr<float>() : nullptr, place.data_ptr<int>(), y.data_ptr(), (int)place.size(0),
                             (int)place.size(1), (int)rows.size(1), dtype_code(type), stream()));
   launched(EXPERTS, 1);
   return y;

@@ -394,13 +394,14 @@ int tmpi_expert_dispatch(const void* x, const int* place, const int* used, const
                          int dtype, void* stream);
 int tmpi_expert_dispatch_keep(const void* x, const int* place, void* out, void* q, void* scale, int tokens, int k, int cols, void* stream);
 int tmpi_expert_dispatch8(const void* q, const void* scale, const int* place, void* out, int tokens, int k, int cols, void* stream);
-int tmpi_expert_combine(const void* rows, int rows_fp32, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream);
+int tmpi_expert_combine(const void* rows, int fp32_slices, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream);
 int tmpi_expert_combine_gradient(const void* dy, const void* rows, const float* weights, const int* place, const int* used, void* drows, float* dweights, int tokens,
                                  int k, int cols, int dtype, void* stream);
 int tmpi_expert_weight_gradient(const float* dots, const void* dy, const void* bias, const int* place, const int* chosen, float* dweights, int tokens, int k, int slices,
                                 int cols, int nexperts, void* stream);
 // Products grouped by expert: rows offsets[e] <= r < offsets[e + 1] (on the device) of x belong to expert e
 int tmpi_grouped_max_experts(void);
+int tmpi_grouped_slices(int rows, int nexperts, int K, int N);   // fp32 results of mode 4
 int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,
                       int w_is_kn, int mode, void* stream);
 int tmpi_grouped_gelu_gradient(const void* dy, const void* w, const int* offsets, const void* z, const void* scale, const float* row_weights, void* dz, void* h,

@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(THREADS) dispatch8_kernel(const uint8_t* __res
 // place adds its weight times zero: nothing, or NaN where the weight is.
 template <typename R, typename T, int V>
 __global__ void __launch_bounds__(THREADS) combine_kernel(const R* __restrict__ rows, const float* __restrict__ weights, const int* __restrict__ place,
-                                                          T* __restrict__ y, int tokens, int places, int k, int cols) {
+                                                          T* __restrict__ y, int tokens, int places, int k, int cols, int slices) {
   wait_previous(rows, weights, place);
   const int parts = cols / V;
   const long long items = (long long)tokens * parts, stride = (long long)gridDim.x * THREADS;
@@ -174,6 +174,12 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const R* __restrict__ 
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const bool there = (unsigned)s[u] < (unsigned)places;
+        if (slices > 1 && there)                          // in their order
+          for (int i = 1; i < slices; ++i) {
+            const Pack<R, V> more = ld_pack<R, V>(rows + ((long long)i * places + s[u]) * cols + part * V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[u].v[e] = from_acc<R>(to_acc<R>(v[u].v[e]) + to_acc<R>(more.v[e]));
+          }
 #pragma unroll
         for (int e = 0; e < V; ++e) sum[e] += w[u] * (there ? (float)to_acc<R>(v[u].v[e]) : 0.f);
       }
@@ -380,19 +386,21 @@ int tmpi_expert_dispatch8(const void* q, const void* scale, const int* place, vo
                                            (const uint8_t*)q, (const uint8_t*)scale, place, (__nv_bfloat16*)out, tokens * k, tokens, k, cols), "expert_dispatch8");
 }
 
-// y [tokens, cols] of `dtype` from rows [tokens * k, cols] of `dtype`, or in fp32 (rows_fp32: y bf16); weights [tokens, k] or null
-int tmpi_expert_combine(const void* rows, int rows_fp32, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream) {
+// y [tokens, cols] of `dtype` from rows [tokens * k, cols] of `dtype`, or (fp32_slices > 0, y bf16) from the sum of fp32 rows [slices, tokens * k, cols];
+// weights [tokens, k] or null
+int tmpi_expert_combine(const void* rows, int fp32_slices, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream) {
   const int st = experts::checked(tokens, k, cols, dtype, "expert_combine");
   if (st || !tokens) return st;
-  if (rows_fp32 && dtype != TMPI_BF16) return fail(TMPI_ERR_UNSUPPORTED, "expert_combine: fp32 rows to dtype %d", dtype);
+  if (fp32_slices < 0) return fail(TMPI_ERR_INVALID, "expert_combine: %d slices", fp32_slices);
+  if (fp32_slices && dtype != TMPI_BF16) return fail(TMPI_ERR_UNSUPPORTED, "expert_combine: fp32 rows to dtype %d", dtype);
   auto go = [&](auto r, auto t, auto v) {
     using R = decltype(r);
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
     return launch_overlapped(experts::combine_kernel<R, T, V>, experts::grid_items((long long)tokens * (cols / V), 1, 8), experts::THREADS, 0, (cudaStream_t)stream,
-                             (const R*)rows, weights, place, (T*)y, tokens, tokens * k, k, cols);
+                             (const R*)rows, weights, place, (T*)y, tokens, tokens * k, k, cols, std::max(1, fp32_slices));
   };
-  if (rows_fp32) {
+  if (fp32_slices) {
     const bool wide = cols % 8 == 0 && (uintptr_t)rows % 32 == 0 && all_aligned16({y});
     return experts::finish(wide ? go(float(), __nv_bfloat16(), std::integral_constant<int, 8>()) : go(float(), __nv_bfloat16(), std::integral_constant<int, 1>()),
                            "expert_combine");

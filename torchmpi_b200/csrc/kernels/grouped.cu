@@ -45,6 +45,7 @@ struct Problem {
   const int* offsets;        // [experts + 1]; null: one expert with all rows
   int rows, experts, K, N;   // of x; N: columns of the result
   int bn, tiles_n, k_blocks;
+  int slices, per;           // PLAIN32 with few rows: parts of K, of `per` blocks, each with a result of its own [slices, rows, N]
   const __nv_bfloat16* bias; // [experts, N] or null
   __nv_bfloat16* y;          // [rows, N]; GRADIENT: dz
   float* y32;                // PLAIN32
@@ -536,8 +537,9 @@ constexpr int FEW_A_BYTES = FEW_BM * BK * 2, FEW_STAGE_BYTES = FEW_A_BYTES + FEW
 constexpr size_t FEW_SMEM = (size_t)FEW_STAGES * FEW_STAGE_BYTES + 1024 + 1280;
 static_assert(FEW_STAGES == STAGES && FEW_SMEM <= 232448, "shared memory of one CTA");
 
-// f(expert, first row, rows, row of the weight, number in this CTA's list) for each tile of this CTA until it returns false; the tiles that share a part of the
-// weight follow each other
+struct FewUnit { int e, row0, rows, col0, kb0, kb1, slice; };      // first row and rows of x, row of the weight, blocks of K
+
+// f(unit, its number in this CTA's list) for each tile of this CTA until it returns false; the tiles that share a part of the weight follow each other
 template <typename F>
 __device__ __forceinline__ void for_few(const Sh* sh, const Problem& p, const int* offsets, F f) {
   const int total = sh->tile_end[p.experts - 1], step = (int)gridDim.x;
@@ -554,8 +556,16 @@ __device__ __forceinline__ void for_few(const Sh* sh, const Problem& p, const in
     }
     const int at = t - (e ? sh->tile_end[e - 1] : 0);
     const Group g = group_of(offsets, p.rows, e);
-    const int across = (g.r1 - g.r0 + FEW_BN - 1) / FEW_BN, row0 = g.r0 + at % across * FEW_BN;
-    if (!f(e, row0, min(g.r1 - row0, FEW_BN), at / across * FEW_BM, it)) return;
+    const int across = (g.r1 - g.r0 + FEW_BN - 1) / FEW_BN, part = at / across;
+    FewUnit u;
+    u.e = e;
+    u.row0 = g.r0 + at % across * FEW_BN;
+    u.rows = min(g.r1 - u.row0, FEW_BN);
+    u.slice = part % p.slices;
+    u.col0 = part / p.slices * FEW_BM;
+    u.kb0 = u.slice * p.per;
+    u.kb1 = min(p.k_blocks, u.kb0 + p.per);
+    if (!f(u, it)) return;
   }
 }
 
@@ -569,10 +579,11 @@ template <int MODE>
 __device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights, int group, int quarter, int lane) {
   constexpr bool GRADIENT = MODE == GRADIENT8 || MODE == GRADIENT16;
   const int N = p.N, blocks = (N + 31) / 32;
-  for_few(sh, p, offsets, [&](int e, int row0, int rows, int col0, int it) -> bool {
-    const int acc = it & 1, col = col0 + quarter * 32 + lane;
+  for_few(sh, p, offsets, [&](const FewUnit& u, int it) -> bool {
+    const int e = u.e, row0 = u.row0, rows = u.rows, col0 = u.col0, acc = it & 1, col = col0 + quarter * 32 + lane;
     const bool in = col < N;
-    const float bias = bias_all && in ? __bfloat162float(bias_all[(long long)e * N + col]) : 0.f;
+    float* y32 = MODE == PLAIN32 ? p.y32 + (long long)u.slice * p.rows * N : nullptr;
+    const float bias = bias_all && in && u.slice == 0 ? __bfloat162float(bias_all[(long long)e * N + col]) : 0.f;
     if (!sm100::mbar_wait_warp(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 54); return false; }
     sm100::tc_fence_after();
     const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)acc * FEW_BN;
@@ -613,7 +624,7 @@ __device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* 
         float v = __uint_as_float(r[j]);
         if (!GRADIENT) v += bias;
         if (MODE == PLAIN32) {
-          if (in && j < left) p.y32[at] = v;
+          if (in && j < left) y32[at] = v;
         } else if (GRADIENT) {
           const float z = z_of[GRADIENT ? j : 0], weight = weight_of[GRADIENT ? j : 0];
           float y0, y1, d0, d1;
@@ -691,10 +702,11 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   if (warp == 0) {
     if (sm100::elect_one()) {
       Ring ring{0, 0};
-      for_few(sh, p, offsets, [&](int e, int row0, int rows, int col0, int) -> bool {
+      for_few(sh, p, offsets, [&](const FewUnit& u, int) -> bool {
+        const int e = u.e, row0 = u.row0, rows = u.rows, col0 = u.col0;
         const CUtensorMap* map = rows > FEW_BN / 2 ? &map_x : rows > FEW ? &map_x_half : &map_x_few;
         const uint32_t tx = FEW_A_BYTES + (rows > FEW_BN / 2 ? FEW_BN : rows > FEW ? FEW_BN / 2 : FEW) * BK * 2;
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
           const int stage = ring.stage;
           if (!sm100::mbar_wait(&sh->empty[stage], ring.phase ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 51); return false; }
           unsigned char* dst = tiles + (size_t)stage * FEW_STAGE_BYTES;
@@ -714,13 +726,13 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   } else if (warp == 1) {
     if (sm100::elect_one()) {
       Ring ring{0, 0};
-      for_few(sh, p, offsets, [&](int, int, int rows, int, int it) -> bool {
+      for_few(sh, p, offsets, [&](const FewUnit& u, int it) -> bool {
         const int acc = it & 1;
         if (!sm100::mbar_wait(&sh->acc_empty[acc], ((it >> 1) & 1) ^ 1, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 52); return false; }
         sm100::tc_fence_after();
-        const uint32_t idesc = sm100::make_idesc_f16(FEW_BM, (rows + 15) / 16 * 16, true, false, W_MN);
+        const uint32_t idesc = sm100::make_idesc_f16(FEW_BM, (u.rows + 15) / 16 * 16, true, false, W_MN);
         const uint32_t d = sh->tmem_base + (uint32_t)acc * FEW_BN;
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
           const int stage = ring.stage;
           if (!sm100::mbar_wait(&sh->full[stage], ring.phase, kWaitBudgetNs) || sh->error) { give_up(sh, p.status, 53); return false; }
           sm100::tc_fence_after();
@@ -728,7 +740,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
           for (int k = 0; k < BK / UMMA_K; ++k) {
             const uint64_t da = W_MN ? sm100::make_desc_sw128_mn(a + k * UMMA_K * 128, FEW_A_BYTES / 2, 1024) : sm100::make_desc_sw128(a + k * UMMA_K * 2);
-            sm100::umma_f16(d, da, sm100::make_desc_sw128(b + k * UMMA_K * 2), idesc, (uint32_t)kb | (uint32_t)k);
+            sm100::umma_f16(d, da, sm100::make_desc_sw128(b + k * UMMA_K * 2), idesc, (uint32_t)(kb > u.kb0) | (uint32_t)k);
           }
           sm100::umma_commit(&sh->empty[stage]);
           advance<FEW_STAGES>(&ring);
@@ -1149,6 +1161,16 @@ static int checked(const int* offsets, int rows, int nexperts, int K, int N, con
 // in fp32, 2 15.2 and 18.7, 128 18.2 and 23.8.  64 ragged groups of 0 to 200 rows, 80 on average, 520 -> 1000: 25.0 and 24.9, with a checkpoint 36.8 and
 // 33.5; of half as many, 16.9 and 21.4, with a checkpoint 21.9 and 28.9, the gradient 36.0 and 34.7.
 static int few_mean(int mode) { return mode == GRADIENT8 || mode == GRADIENT16 ? 32 : mode == KEEP8 ? 64 : 96; }
+// Parts of K of a product with few rows and an fp32 result, whose reader adds them: as many as leave eight blocks of K each and about a tile for every SM,
+// if half of the experts have rows.  4 tokens with two of 8 experts each, 4096 -> 1024: 14.6 us whole, 9.9 in three parts.
+static int few_slices(int rows, int nexperts, int K, int N) {
+  if (rows > (long long)few_mean(PLAIN32) * nexperts) return 1;
+  const int tiles = std::max(1, std::min(nexperts, rows) / 2 + 1) * ((N + FEW_BM - 1) / FEW_BM), k_blocks = (K + BK - 1) / BK;
+  const int most = std::max(1, std::min({4, k_blocks / 8, gemm_sm_count() / tiles}));
+  const int per = (k_blocks + most - 1) / most;
+  return (k_blocks + per - 1) / per;                    // none is empty
+}
+
 static int run(Problem p, const void* x, const void* w, const int* offsets, int rows, int nexperts, int K, int N, bool w_is_kn, int mode, cudaStream_t stream) {
   int st = checked(offsets, rows, nexperts, K, N, "grouped_gemm");
   if (st) return st;
@@ -1159,7 +1181,9 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   p.k_blocks = (K + BK - 1) / BK;
   p.status = gemm_status_word();
   if (rows <= (long long)few_mean(mode) * nexperts) {
-    p.tiles_n = (N + FEW_BM - 1) / FEW_BM;
+    p.slices = mode == PLAIN32 ? few_slices(rows, nexperts, K, N) : 1;
+    p.per = (p.k_blocks + p.slices - 1) / p.slices;
+    p.tiles_n = (N + FEW_BM - 1) / FEW_BM * p.slices;
     CUtensorMap mw, mx, mx_half, mx_few;
     if (w_is_kn) st = make_tmap_bf16_3d(&mw, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, BK, 64);
     else st = make_tmap_bf16_3d(&mw, w, (uint64_t)nexperts, (uint64_t)N, (uint64_t)K, FEW_BM, 64);
@@ -1201,10 +1225,13 @@ using namespace tmpi;
 extern "C" {
 
 int tmpi_grouped_max_experts(void) { return grouped::MAX_EXPERTS; }
+// the results that tmpi_grouped_gemm leaves in mode 4, [slices, rows, N], whose sum is the product
+int tmpi_grouped_slices(int rows, int nexperts, int K, int N) { return rows < 1 || nexperts < 1 || K < 1 || N < 1 ? 1 : grouped::few_slices(rows, nexperts, K, N); }
 
 // y [rows, N] = act(x w_e^T + b_e) for x [rows, K] and w [experts, N, K] (w_is_kn: [experts, K, N], without activation), zeros behind the
 // last group; offsets [experts + 1] on the device, or null for one expert.  mode: 0 none; 1 GELU; 2 GELU, and the pre-activation in z; 3 GELU, and
-// the pre-activation's 8-bit checkpoint in z and scale [rows, ceil(N / 32)]; 4 none, y in fp32, and rows behind the last group left alone.  All bf16
+// the pre-activation's 8-bit checkpoint in z and scale [rows, ceil(N / 32)]; 4 none, y in fp32 [tmpi_grouped_slices, rows, N], of which the sum is the
+// product, and rows behind the last group left alone.  All bf16
 // but those, on 16-byte boundaries (fp32: 32).
 int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,
                       int w_is_kn, int mode, void* stream) {

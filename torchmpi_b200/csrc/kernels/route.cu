@@ -1,14 +1,15 @@
 // Routing of tokens to experts: the choice of k experts by a token's logits, its weights, the order of all choices by expert, and the
 // weights' gradient.
 //
-// A warp takes a token; a lane holds the logits of experts lane, lane + 32, ... as integers that compare like the values, so that a round of the
-// choice is a maximum over the lane's own, and two warp-wide reductions (largest value, then the lowest index that has it).  The order by expert is a
-// counting sort in two launches: the first counts the choices of a block of tokens per expert; the second adds the counts of the blocks in front, and
-// each warp places a contiguous part of the block's choices, 32 at a time, equal ones ranked by their lane.  So entries of an expert keep their
-// order, and no atomic decides about a place.  Up to SMALL choices one block does both.
+// G lanes take a token; a lane holds the logits of experts lane, lane + G, ... as integers that compare like the values, and the best of them apart, so that a
+// round of the choice is a maximum over G lanes (log G exchanges of value and index, the lower index of equals) and a new best of the lane that lost its
+// own.  The order by expert is a counting sort in two launches: the first counts the choices of a block of tokens per expert; the second adds the counts of
+// the blocks in front, and each warp places a contiguous part of the block's choices, 32 at a time, equal ones ranked by their lane.  So entries of an expert
+// keep their order, and no atomic decides about a place.  Up to SMALL choices one block does both.
 //
-// Both launches are bound by latency, a few dependent passes over little data, hence as many warps as an SM takes.  65536 tokens of 64 experts, 8
-// each, forward: 200 us with 8 warps and a thread per expert that walked all choices of its block, 34 so.
+// The choice is bound by instructions, the rest by latency, a few dependent passes over little data, hence as many warps as an SM takes.  65536 tokens of 64
+// experts, 8 each, forward: 200 us with 8 warps a block, a warp to a token and a thread per expert that walked all choices of its block; 50 with 32
+// warps and a warp to a token; 46 with eight lanes to a token, and the gradient 10 where it took 20.
 #include "pdl.cuh"
 #include "vec.cuh"
 #include "../include/tmpi_c_api.h"
@@ -45,76 +46,119 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
-__device__ __forceinline__ float warp_sum(float x) {
+template <int G>
+__device__ __forceinline__ float group_sum(float x) {
 #pragma unroll
-  for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
+  for (int d = G / 2; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
   return x;
 }
+template <int G>
+__device__ __forceinline__ bool group_any(bool x) {
+  const unsigned all = __ballot_sync(~0u, x);
+  return G == 32 ? all != 0 : (all >> ((threadIdx.x & 31) & ~(G - 1)) & ((1u << (G & 31)) - 1)) != 0;
+}
 
-// One token by one warp: chosen and weights of lane j < k.
-template <typename T, int NREG>
-__device__ __forceinline__ void choose(const Problem& p, const T* logits, int token, int lane, int* chosen, float* weight) {
-  static_assert(WARPS == 32, "a lane per warp in place_block");
-  float l[NREG];
-  uint32_t key[NREG];
+// One token by G lanes, of which this is lane g with the logits of experts g + G r: chosen and weights of the choices g + G q.  All lanes of the warp;
+// `in`: the group has a token.
+template <typename T, int G, int R>
+__device__ __forceinline__ void choose(const Problem& p, const T* logits, long long token, bool in, int g, int (&chosen)[MAX_K / G], float (&weight)[MAX_K / G]) {
+  constexpr int Q = MAX_K / G;
+  uint32_t key[R];
   bool nan = false;
 #pragma unroll
-  for (int r = 0; r < NREG; ++r) {
-    const int e = lane + 32 * r;
-    l[r] = e < p.experts ? (float)to_acc<T>(logits[(long long)token * p.ld + e]) : 0.f;
-    key[r] = e < p.experts ? key_of(l[r]) : 0u;
-    nan |= l[r] != l[r];
+  for (int r = 0; r < R; ++r) {
+    const int e = g + G * r;
+    const float l = in && e < p.experts ? (float)to_acc<T>(logits[token * p.ld + e]) : 0.f;
+    nan |= l != l;
+    key[r] = in && e < p.experts ? key_of(l) : 0u;
   }
-  nan = __any_sync(~0u, nan);
-  int mine = -1;
-  uint32_t my_key = KEY_NONE, top_key = KEY_NONE;
-  for (int j = 0; j < p.k; ++j) {
-    uint32_t best = 0;
-    int at = 0x7fffffff;
+  nan = group_any<G>(nan);
+  uint32_t best = 0;
+  int at = g;
+  auto renew = [&] {                                               // the lane's best, the lowest index of equals
+    best = key[0];
+    at = g;
 #pragma unroll
-    for (int r = 0; r < NREG; ++r)
-      if (key[r] > best) { best = key[r]; at = lane + 32 * r; }
-    const uint32_t m = __reduce_max_sync(~0u, best);
-    if (m <= KEY_NONE) break;                                      // nothing left that may be used
-    if (!j) top_key = m;
-    const int i = NREG == 1 ? __ffs(__ballot_sync(~0u, best == m)) - 1 : (int)__reduce_min_sync(~0u, (unsigned)(best == m ? at : 0x7fffffff));
-    if (lane == j) { mine = i; my_key = m; }
+    for (int r = 1; r < R; ++r)
+      if (key[r] > best) { best = key[r]; at = g + G * r; }
+  };
+  renew();
+  uint32_t top_key = best;
 #pragma unroll
-    for (int r = 0; r < NREG; ++r)
-      if (i == lane + 32 * r) key[r] = 0;
-  }
-  const float top = of_key(top_key);
+  for (int d = G / 2; d; d /= 2) top_key = max(top_key, __shfl_xor_sync(~0u, top_key, d));
   const bool any = top_key > KEY_NONE;
-  const float e_mine = mine >= 0 ? expf(of_key(my_key) - top) : 0.f;
+  const float top = of_key(any ? top_key : KEY_NONE + 1);
   float sum = 0.f;
-  if (p.renormalize) {
-    sum = e_mine;
-  } else if (any) {
+  if (!p.renormalize) {                                            // over all experts
 #pragma unroll
-    for (int r = 0; r < NREG; ++r)
-      if (lane + 32 * r < p.experts) sum += expf(l[r] - top);
+    for (int r = 0; r < R; ++r)
+      if (any && g + G * r < p.experts) sum += expf(of_key(key[r]) - top);
   }
-  sum = warp_sum(sum);
-  *chosen = mine;
-  *weight = nan ? __uint_as_float(0x7fffffffu) : mine >= 0 ? e_mine / sum : 0.f;
+  float mine[Q];
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    chosen[q] = -1;
+    mine[q] = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < G && q * G + j < p.k; ++j) {
+      uint32_t m = best;
+      int i = at;
+#pragma unroll
+      for (int d = G / 2; d; d /= 2) {
+        const uint32_t m2 = __shfl_xor_sync(~0u, m, d);
+        const int i2 = __shfl_xor_sync(~0u, i, d);
+        if (m2 > m || (m2 == m && i2 < i)) { m = m2; i = i2; }
+      }
+      if (m <= KEY_NONE) i = -1;                                   // nothing left that may be used
+      if (g == j) {
+        chosen[q] = i;
+        mine[q] = __uint_as_float(m);
+      }
+      if (i >= 0 && i % G == g) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (i == g + G * r) key[r] = 0;
+        renew();
+      }
+    }
+    mine[q] = chosen[q] >= 0 ? expf(of_key(__float_as_uint(mine[q])) - top) : 0.f;
+    if (p.renormalize) sum += mine[q];
+  }
+  sum = group_sum<G>(sum);
+#pragma unroll
+  for (int q = 0; q < Q; ++q) weight[q] = nan ? __uint_as_float(0x7fffffffu) : chosen[q] >= 0 ? mine[q] / sum : 0.f;
 }
 
 // The tokens of this block: choices and weights to memory, counts per expert to shared memory (cleared by the caller).
-template <typename T, int NREG>
+template <typename T, int G, int R>
 __device__ __forceinline__ void choose_block(const Problem& p, const T* logits, int* counts) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long t0 = (long long)blockIdx.x * p.per_block;
-  const int t1 = (int)min((long long)p.tokens, t0 + p.per_block);
-  for (int t = (int)t0 + warp; t < t1; t += WARPS) {
-    int c;
-    float w;
-    choose<T, NREG>(p, logits, t, lane, &c, &w);
-    if (lane < p.k) {
-      p.chosen[(long long)t * p.k + lane] = c;
-      p.weights[(long long)t * p.k + lane] = w;
-      if (c >= 0) atomicAdd(&counts[c], 1);                        // a count: the order of the additions does not matter
-    }
+  const int g = threadIdx.x % G, group = threadIdx.x / G;
+  const long long t0 = (long long)blockIdx.x * p.per_block, t1 = min((long long)p.tokens, t0 + p.per_block);
+  for (long long tw = t0 + (group & ~(32 / G - 1)); tw < t1; tw += THREADS / G) {      // the same for a warp
+    const long long t = tw + (group & (32 / G - 1));
+    const bool in = t < t1;
+    int c[MAX_K / G];
+    float w[MAX_K / G];
+    choose<T, G, R>(p, logits, t, in, g, c, w);
+#pragma unroll
+    for (int q = 0; q < MAX_K / G; ++q)
+      if (in && g + G * q < p.k) {
+        p.chosen[t * p.k + g + G * q] = c[q];
+        p.weights[t * p.k + g + G * q] = w[q];
+        if (c[q] >= 0) atomicAdd(&counts[c[q]], 1);                // a count: the order of the additions does not matter
+      }
   }
+}
+
+// The lanes whose choice is the same, by one vote for each bit of an expert's number (a warp-wide match goes through the different values one by one:
+// 65536 tokens of 64 experts, 8 each, took 18.8 us to place out of a cold cache, 14.6 so).  c < 0: no choice, nothing that counts.
+__device__ __forceinline__ unsigned same_choice(int c, int bits) {
+  unsigned same = __ballot_sync(~0u, c >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned set = __ballot_sync(~0u, c >> b & 1);
+    same &= c >> b & 1 ? set : ~set;
+  }
+  return same;
 }
 
 struct Place {
@@ -135,7 +179,10 @@ __device__ __forceinline__ void for_choices(const Problem& p, F f) {
 #pragma unroll
     for (int u = 0; u < U; ++u) c[u] = i0 + 32 * u + lane < w1 ? p.chosen[i0 + 32 * u + lane] : -2;
 #pragma unroll
-    for (int u = 0; u < U; ++u) f(c[u], i0 + 32 * u + lane);
+    for (int u = 0; u < U; ++u) {
+      if (i0 + 32 * u >= w1) break;
+      f(c[u], i0 + 32 * u + lane);
+    }
   }
 }
 
@@ -186,8 +233,9 @@ __device__ __forceinline__ void place_block(const Problem& p, Place& s, const in
     }
   }
   int* mine = s.base[warp];
+  const int bits = 32 - __clz(p.experts - 1);                      // none for one expert
   for_choices(p, [&](int c, long long) {
-    const unsigned same = __match_any_sync(~0u, c);
+    const unsigned same = same_choice(c, bits);
     if (c >= 0 && lane == __ffs(same) - 1) mine[c] += __popc(same);
     __syncwarp();
   });
@@ -204,7 +252,7 @@ __device__ __forceinline__ void place_block(const Problem& p, Place& s, const in
   }
   __syncthreads();
   for_choices(p, [&](int c, long long entry) {
-    const unsigned same = __match_any_sync(~0u, c);
+    const unsigned same = same_choice(c, bits);
     int at = -1;
     if (c >= 0) at = mine[c] + __popc(same & ((1u << lane) - 1));
     __syncwarp();
@@ -216,14 +264,14 @@ __device__ __forceinline__ void place_block(const Problem& p, Place& s, const in
   for (long long i = used + (long long)blockIdx.x * THREADS + tid; i < (long long)p.tokens * p.k; i += (long long)gridDim.x * THREADS) p.order[i] = -1;
 }
 
-template <typename T, int NREG>
+template <typename T, int G, int R>
 __global__ void __launch_bounds__(THREADS) choose_kernel(const Problem p) {
   __shared__ int counts[MAX_EXPERTS];
   const T* logits = (const T*)p.logits;
   wait_previous(logits);
   for (int e = threadIdx.x; e < p.experts; e += THREADS) counts[e] = 0;
   __syncthreads();
-  choose_block<T, NREG>(p, logits, counts);
+  choose_block<T, G, R>(p, logits, counts);
   __syncthreads();
   for (int e = threadIdx.x; e < p.experts; e += THREADS) p.counts[(long long)blockIdx.x * p.experts + e] = counts[e];
 }
@@ -235,7 +283,7 @@ __global__ void __launch_bounds__(THREADS) place_kernel(const Problem p) {
   place_block(p, s, counts, (int)gridDim.x);
 }
 
-template <typename T, int NREG>
+template <typename T, int G, int R>
 __global__ void __launch_bounds__(THREADS) small_kernel(const Problem p) {
   __shared__ Place s;
   __shared__ int counts[MAX_EXPERTS];
@@ -243,65 +291,70 @@ __global__ void __launch_bounds__(THREADS) small_kernel(const Problem p) {
   wait_previous(logits);
   if (threadIdx.x < MAX_EXPERTS) counts[threadIdx.x] = 0;
   __syncthreads();
-  choose_block<T, NREG>(p, logits, counts);
+  choose_block<T, G, R>(p, logits, counts);
   __syncthreads();                                                 // the choices, which this block has written, are read again
   place_block(p, s, counts, 1);
 }
 
-// dl of one token: over the chosen, w_j (dw_j - sum w dw); with weights over all experts, the others get -p_e sum w dw.
-template <typename T, int NREG>
+// dl of one token by G lanes: of the chosen, w_j (dw_j - sum w dw); with weights over all experts, the others get -p_e sum w dw.
+template <typename T, int G, int R>
 __global__ void __launch_bounds__(GRADIENT_THREADS) gradient_kernel(const Problem p, const float* dweights, T* dlogits) {
   const T* logits = (const T*)p.logits;
   wait_previous(logits, dweights);
-  const int lane = threadIdx.x & 31;
-  constexpr int W = GRADIENT_THREADS / 32;
-  for (long long t = (long long)blockIdx.x * W + (threadIdx.x >> 5); t < p.tokens; t += (long long)gridDim.x * W) {
-    int c = -1;
-    float w = 0.f, wd = 0.f;
-    if (lane < p.k) {
-      c = p.chosen[t * p.k + lane];
-      w = p.weights[t * p.k + lane];                               // NaN in a row with a NaN among its logits, whether used or not
-      if (c >= 0) wd = w * dweights[t * p.k + lane];
-    }
-    const float inner = warp_sum(wd);
-    float l[NREG], d[NREG];
-    bool nan = false;
-    float top = __uint_as_float(0xff800000u), sum = 0.f;
+  constexpr int Q = MAX_K / G, PER = GRADIENT_THREADS / G;
+  const int g = threadIdx.x % G, group = threadIdx.x / G;
+  for (long long tw = (long long)blockIdx.x * PER + (group & ~(32 / G - 1)); tw < p.tokens; tw += (long long)gridDim.x * PER) {      // the same for a warp
+    const long long t = tw + (group & (32 / G - 1));
+    const bool in = t < p.tokens;
+    int c[Q];
+    float w[Q], wd[Q], inner = 0.f;
 #pragma unroll
-    for (int r = 0; r < NREG; ++r) {
-      const int e = lane + 32 * r;
-      d[r] = 0.f;
-      l[r] = __uint_as_float(0xff800000u);
-      if (!p.renormalize && e < p.experts) {
-        l[r] = (float)to_acc<T>(logits[t * p.ld + e]);
-        nan |= l[r] != l[r];
-        top = fmaxf(top, l[r]);
+    for (int q = 0; q < Q; ++q) {
+      c[q] = -1;
+      w[q] = wd[q] = 0.f;
+      if (in && g + G * q < p.k) {
+        c[q] = p.chosen[t * p.k + g + G * q];
+        w[q] = p.weights[t * p.k + g + G * q];                     // NaN in a row with a NaN among its logits, whether used or not
+        if (c[q] >= 0) wd[q] = w[q] * dweights[t * p.k + g + G * q];
       }
+      inner += wd[q];
     }
+    float d[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) d[r] = 0.f;
     if (!p.renormalize) {
+      bool nan = false;
+      float top = __uint_as_float(0xff800000u), sum = 0.f;
 #pragma unroll
-      for (int k = 16; k; k /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
-      nan = __any_sync(~0u, nan);
-      if (top > __uint_as_float(0xff800000u)) {                    // warp-uniform
-#pragma unroll
-        for (int r = 0; r < NREG; ++r) {
-          d[r] = expf(l[r] - top);
-          if (lane + 32 * r < p.experts) sum += d[r];
-        }
-        sum = warp_sum(sum);
-        const float scale = nan ? __uint_as_float(0x7fffffffu) : -inner / sum;
-#pragma unroll
-        for (int r = 0; r < NREG; ++r) d[r] *= scale;
-      } else if (nan) {
-#pragma unroll
-        for (int r = 0; r < NREG; ++r) d[r] = __uint_as_float(0x7fffffffu);
+      for (int r = 0; r < R; ++r) {
+        d[r] = in && g + G * r < p.experts ? (float)to_acc<T>(logits[t * p.ld + g + G * r]) : __uint_as_float(0xff800000u);
+        nan |= d[r] != d[r];
+        top = fmaxf(top, d[r]);
       }
+#pragma unroll
+      for (int k = G / 2; k; k /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
+      nan = group_any<G>(nan);
+      const bool any = top > __uint_as_float(0xff800000u);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        d[r] = any ? expf(d[r] - top) : 0.f;
+        sum += d[r];
+      }
+      sum = group_sum<G>(sum);
+      inner = group_sum<G>(inner);
+      const float scale = nan ? __uint_as_float(0x7fffffffu) : any ? -inner / sum : 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) d[r] = nan ? scale : d[r] * scale;
+    } else {
+      inner = group_sum<G>(inner);
     }
 #pragma unroll
-    for (int r = 0; r < NREG; ++r)
-      if (lane + 32 * r < p.experts) dlogits[t * p.experts + lane + 32 * r] = from_acc<T>((typename AccOf<T>::type)d[r]);
+    for (int r = 0; r < R; ++r)
+      if (in && g + G * r < p.experts) dlogits[t * p.experts + g + G * r] = from_acc<T>((typename AccOf<T>::type)d[r]);
     __syncwarp();                                                  // the chosen ones' are written over it: their p is their weight either way
-    if (c >= 0) dlogits[t * p.experts + c] = from_acc<T>((typename AccOf<T>::type)(wd - w * inner));
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (c[q] >= 0) dlogits[t * p.experts + c[q]] = from_acc<T>((typename AccOf<T>::type)(wd[q] - w[q] * inner));
   }
 }
 
@@ -310,13 +363,16 @@ static int blocks_of(int tokens, int k) {
   return (int)std::min<long long>(MAX_BLOCKS, ((long long)tokens + 31) / 32);
 }
 
-// f(template arguments) for the smallest number of registers that holds the experts
+template <int G_, int R_> struct Form { static constexpr int G = G_, R = R_; };
+// f(lanes to a token and logits to a lane)
 template <typename F>
 static cudaError_t by_experts(int experts, F f) {
-  if (experts <= 32) return f(std::integral_constant<int, 1>());
-  if (experts <= 64) return f(std::integral_constant<int, 2>());
-  if (experts <= 128) return f(std::integral_constant<int, 4>());
-  return f(std::integral_constant<int, 8>());
+  if (experts <= 8) return f(Form<8, 1>());
+  if (experts <= 16) return f(Form<8, 2>());
+  if (experts <= 32) return f(Form<8, 4>());
+  if (experts <= 64) return f(Form<8, 8>());
+  if (experts <= 128) return f(Form<16, 8>());
+  return f(Form<32, 8>());
 }
 
 template <typename T>
@@ -324,17 +380,20 @@ static cudaError_t forward_t(Problem p, cudaStream_t s) {
   const int blocks = blocks_of(p.tokens, p.k);
   p.per_block = (p.tokens + blocks - 1) / blocks;
   return by_experts(p.experts, [&](auto n) {
-    if (blocks == 1) return launch_overlapped(small_kernel<T, decltype(n)::value>, 1, THREADS, 0, s, p);
-    const cudaError_t e = launch_overlapped(choose_kernel<T, decltype(n)::value>, blocks, THREADS, 0, s, p);
+    using N = decltype(n);
+    if (blocks == 1) return launch_overlapped(small_kernel<T, N::G, N::R>, 1, THREADS, 0, s, p);
+    const cudaError_t e = launch_overlapped(choose_kernel<T, N::G, N::R>, blocks, THREADS, 0, s, p);
     return e == cudaSuccess ? launch_overlapped(place_kernel, blocks, THREADS, 0, s, p) : e;
   });
 }
 
 template <typename T>
 static cudaError_t gradient_t(const Problem& p, const float* dweights, void* dlogits, cudaStream_t s) {
-  const int blocks = (int)std::min<long long>(148 * 8, ((long long)p.tokens + GRADIENT_THREADS / 32 - 1) / (GRADIENT_THREADS / 32));
   return by_experts(p.experts, [&](auto n) {
-    return launch_overlapped(gradient_kernel<T, decltype(n)::value>, blocks, GRADIENT_THREADS, 0, s, p, dweights, (T*)dlogits);
+    using N = decltype(n);
+    constexpr int per = GRADIENT_THREADS / N::G;
+    const int blocks = (int)std::min<long long>(148 * 8, ((long long)p.tokens + per - 1) / per);
+    return launch_overlapped(gradient_kernel<T, N::G, N::R>, blocks, GRADIENT_THREADS, 0, s, p, dweights, (T*)dlogits);
   });
 }
 
