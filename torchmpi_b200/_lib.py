@@ -230,6 +230,7 @@ _CUDA_PROTOS = {
     "tmpi_grouped_max_experts": (_i, []),
     "tmpi_grouped_slices": (_i, [_i, _i, _i, _i]),
     "tmpi_grouped_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "tmpi_grouped_dots": (_i, [_i, _i, _i, _i]),
     "tmpi_grouped_gelu_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "tmpi_grouped_weight_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "tmpi_gemm_status": (_i, []),

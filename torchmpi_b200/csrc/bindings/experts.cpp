@@ -313,9 +313,9 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     const auto f32 = dy.options().dtype(at::kFloat);
     const bool need_wt = ctx->needs_input_grad(1);
     const Tensor by_place = at::empty({T * k}, f32), g = dispatch(dy, place, Tensor(), weights, by_place);
-    const int64_t slices = (H + 31) / 32;
+    const int64_t slices = tmpi_grouped_dots((int)(T * k), (int)E, (int)H, kz.scale.defined());
     Tensor dots, dwt;
-    if (need_wt) dots = at::empty({T * k, slices}, f32);
+    if (need_wt) dots = at::empty({slices, T * k}, f32);
     const auto both = grouped_gelu_gradient(g, w2, offsets, kz, by_place, dots);
     const Tensor dz = both.first, hw = both.second;
     if (need_wt) {

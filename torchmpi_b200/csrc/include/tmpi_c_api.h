@@ -397,13 +397,14 @@ int tmpi_expert_dispatch8(const void* q, const void* scale, const int* place, vo
 int tmpi_expert_combine(const void* rows, int fp32_slices, const float* weights, const int* place, void* y, int tokens, int k, int cols, int dtype, void* stream);
 int tmpi_expert_combine_gradient(const void* dy, const void* rows, const float* weights, const int* place, const int* used, void* drows, float* dweights, int tokens,
                                  int k, int cols, int dtype, void* stream);
-int tmpi_expert_weight_gradient(const float* dots, const void* dy, const void* bias, const int* place, const int* chosen, float* dweights, int tokens, int k, int slices,
-                                int cols, int nexperts, void* stream);
+int tmpi_expert_weight_gradient(const float* dots, const void* dy, const void* bias, const int* place, const int* chosen, float* dweights, int tokens, int k,
+                                int slices, int cols, int nexperts, void* stream);
 // Products grouped by expert: rows offsets[e] <= r < offsets[e + 1] (on the device) of x belong to expert e
 int tmpi_grouped_max_experts(void);
 int tmpi_grouped_slices(int rows, int nexperts, int K, int N);   // fp32 results of mode 4
 int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,
                       int w_is_kn, int mode, void* stream);
+int tmpi_grouped_dots(int rows, int nexperts, int N, int kept8);   // the first extent of dots
 int tmpi_grouped_gelu_gradient(const void* dy, const void* w, const int* offsets, const void* z, const void* scale, const float* row_weights, void* dz, void* h,
                                float* dots, int rows, int nexperts, int K, int N, void* stream);
 int tmpi_grouped_weight_gradient(const void* dy, const void* x, const int* offsets, const float* row_weights, void* dw, void* db, int rows, int nexperts, int K,

@@ -46,16 +46,18 @@ __device__ __forceinline__ void unpack2(uint32_t q, float scale, float* x0, floa
   *x1 = f.y * scale;
 }
 
-// A whole block by one thread; returns its scale byte.  Where all are finite, which the maximum tells, the elements need no look of their own.
+// A whole block by one thread; returns its scale byte.  Where none is infinite, which the maximum tells, the elements need no look of their own (a NaN
+// converts to NaN; a maximum leaves it out as long as there is a number).
 __device__ __forceinline__ uint32_t pack_block(const float (&x)[32], uint32_t (&q)[8]) {
-  float a = fabsf(x[0]), b = fabsf(x[1]);
+  float m[4];
 #pragma unroll
-  for (int j = 2; j < 32; j += 4) {
-    a = attn_util::max3_nan(a, fabsf(x[j]), fabsf(x[j + 1]));
-    if (j + 3 < 32) b = attn_util::max3_nan(b, fabsf(x[j + 2]), fabsf(x[j + 3]));
+  for (int j = 0; j < 4; ++j) {
+    m[j] = fmaxf(fmaxf(fabsf(x[8 * j]), fabsf(x[8 * j + 1])), fabsf(x[8 * j + 2]));
+    m[j] = fmaxf(fmaxf(m[j], fabsf(x[8 * j + 3])), fabsf(x[8 * j + 4]));
+    m[j] = fmaxf(fmaxf(m[j], fabsf(x[8 * j + 5])), fabsf(x[8 * j + 6]));
+    m[j] = fmaxf(m[j], fabsf(x[8 * j + 7]));
   }
-  a = attn_util::max_nan(a, b);
-  uint32_t top = __float_as_uint(a);
+  uint32_t top = __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
   const bool finite = top < 0x7f800000u;
   if (!finite) {
     top = 0;

@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(THREADS) dispatch8_kernel(const uint8_t* __res
 
 // y[t] = sum over j of weights[t, j] rows[place[t, j]], added in the order of j and rounded once; weights null: ones.  An entry without a
 // place adds its weight times zero: nothing, or NaN where the weight is.
-template <typename R, typename T, int V>
+template <typename R, typename T, int V, bool SLICES>
 __global__ void __launch_bounds__(THREADS) combine_kernel(const R* __restrict__ rows, const float* __restrict__ weights, const int* __restrict__ place,
                                                           T* __restrict__ y, int tokens, int places, int k, int cols, int slices) {
   wait_previous(rows, weights, place);
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const R* __restrict__ 
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const bool there = (unsigned)s[u] < (unsigned)places;
-        if (slices > 1 && there)                          // in their order
+        if (SLICES && there)                              // in their order
           for (int i = 1; i < slices; ++i) {
             const Pack<R, V> more = ld_pack<R, V>(rows + ((long long)i * places + s[u]) * cols + part * V);
 #pragma unroll
@@ -262,8 +262,9 @@ __global__ void __launch_bounds__(GRAD_THREADS) combine_gradient_kernel(const T*
   clear_rest<T, V, GRAD_THREADS>(used, drows, places, cols);
 }
 
-// The weights' gradient in a layer of experts, a warp to a token: dweights[entry] = the sum of the entry's row of `dots` (grouped.cu: a number for
-// 32 columns) + dy[token] . bias[expert].  0 for entries without a place.
+// The weights' gradient in a layer of experts, a warp to a token: dweights[entry] = the sum of the entry's place over `dots` [slices, places]
+// (grouped.cu) + dy[token] . bias[expert]; 0 for entries without a place.  By tokens, what belongs to the entries and the row of dy are one step of
+// loads, and the row is read once: 13 us for 8192 x 1024 and two experts of eight; by places, which come in the order of the experts, 20.
 template <int V>
 __global__ void __launch_bounds__(THREADS) weight_gradient_kernel(const float* __restrict__ dots, const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ bias,
                                                                   const int* __restrict__ place, const int* __restrict__ chosen, float* __restrict__ dweights,
@@ -281,6 +282,11 @@ __global__ void __launch_bounds__(THREADS) weight_gradient_kernel(const float* _
         e[j] = j0 + j < k && bias ? chosen[t * k + j0 + j] : -1;
         sum[j] = 0.f;
       }
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if ((unsigned)s[j] < (unsigned)places)
+#pragma unroll 2
+          for (int i = lane; i < slices; i += 32) sum[j] += dots[(long long)i * places + s[j]];
       if (bias)
         for (int c0 = lane; c0 < parts; c0 += 32 * U) {
           Pack<__nv_bfloat16, V> g[U];
@@ -300,14 +306,6 @@ __global__ void __launch_bounds__(THREADS) weight_gradient_kernel(const float* _
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[j] += __bfloat162float(g[u].v[i]) * __bfloat162float(b[u].v[i]);
           }
-        }
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-        if ((unsigned)s[j] < (unsigned)places) {
-          float more = 0.f;
-#pragma unroll 4
-          for (int i = lane; i < slices; i += 32) more += dots[(long long)s[j] * slices + i];
-          sum[j] += more;
         }
 #pragma unroll
       for (int j = 0; j < J; ++j) {
@@ -397,8 +395,9 @@ int tmpi_expert_combine(const void* rows, int fp32_slices, const float* weights,
     using R = decltype(r);
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
-    return launch_overlapped(experts::combine_kernel<R, T, V>, experts::grid_items((long long)tokens * (cols / V), 1, 8), experts::THREADS, 0, (cudaStream_t)stream,
-                             (const R*)rows, weights, place, (T*)y, tokens, tokens * k, k, cols, std::max(1, fp32_slices));
+    const auto kernel = fp32_slices > 1 ? experts::combine_kernel<R, T, V, sizeof(R) == 4> : experts::combine_kernel<R, T, V, false>;
+    return launch_overlapped(kernel, experts::grid_items((long long)tokens * (cols / V), 1, 8), experts::THREADS, 0, (cudaStream_t)stream, (const R*)rows, weights,
+                             place, (T*)y, tokens, tokens * k, k, cols, std::max(1, fp32_slices));
   };
   if (fp32_slices) {
     const bool wide = cols % 8 == 0 && (uintptr_t)rows % 32 == 0 && all_aligned16({y});
@@ -425,9 +424,10 @@ int tmpi_expert_combine_gradient(const void* dy, const void* rows, const float* 
   }), "expert_combine_gradient");
 }
 
-// dweights [tokens, k] = the sums of the rows of dots [tokens * k, slices] + dy [tokens, cols] . bias [nexperts, cols] (bf16, or null) of the chosen expert
-int tmpi_expert_weight_gradient(const float* dots, const void* dy, const void* bias, const int* place, const int* chosen, float* dweights, int tokens, int k, int slices,
-                                int cols, int nexperts, void* stream) {
+// dweights [tokens, k] = the sums over dots [slices, tokens * k] of the entries' places + dy [tokens, cols] . bias [nexperts, cols] (bf16, or null) of
+// the chosen expert
+int tmpi_expert_weight_gradient(const float* dots, const void* dy, const void* bias, const int* place, const int* chosen, float* dweights, int tokens, int k,
+                                int slices, int cols, int nexperts, void* stream) {
   const int st = experts::checked(tokens, k, cols, TMPI_BF16, "expert_weight_gradient");
   if (st || !tokens) return st;
   const auto kernel = cols % 8 == 0 && all_aligned16({dy, bias}) ? experts::weight_gradient_kernel<8> : experts::weight_gradient_kernel<1>;

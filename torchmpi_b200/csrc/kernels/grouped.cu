@@ -53,9 +53,10 @@ struct Problem {
   uint8_t* scale;            // and their scales
   __nv_bfloat16* h;          // GRADIENT: weight times gelu(z)
   const float* row_weights;  // GRADIENT: [rows] or null (ones)
-  float* dots;               // GRADIENT: [rows, ceil(N / 32)], the sum over 32 columns of gradient times gelu(z); or null
+  float* dots;               // GRADIENT: [columns' groups, rows], the sum over 64 (few rows: 32) columns of gradient times gelu(z); or null
   int wide;                  // every row of y, z, h starts on a 32-byte boundary
-  int q_rows16;              // KEEP8: every row of z starts on a 16-byte boundary, as TMA tiles need
+  int q_rows16;              // 8 bits: every row of z starts on a 16-byte boundary, as TMA tiles and 16-byte loads need
+  int scale_pairs;           // 8 bits: two scales of a row that belong to 64 columns lie in one aligned 16-bit word
   int* status;
 };
 
@@ -235,18 +236,6 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* to, const uint32_t (&w)
       if (8 * j < left) reinterpret_cast<uint4*>(to)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
   }
 }
-__device__ __forceinline__ void load_row(const __nv_bfloat16* from, uint32_t (&w)[16], int left, bool wide) {
-  if (wide && left >= 32) {
-    load32(from, w);
-    load32(from + 16, w + 8);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint4 v = 8 * j < left ? reinterpret_cast<const uint4*>(from)[j] : make_uint4(0u, 0u, 0u, 0u);
-      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
-    }
-  }
-}
 // 32 e4m3 columns
 __device__ __forceinline__ void store_row8(uint8_t* to, const uint32_t (&q)[8], int left, bool wide) {
   if (wide && left >= 32) {
@@ -312,18 +301,49 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
     };
     const long long row_at = (long long)u.row0 + (int)rank * BM + row;
     const __nv_bfloat16* bias = bias_all ? bias_all + (long long)u.e * N : nullptr;
-    float weight = 1.f;
-    uint32_t kept[2][GRADIENT ? 8 : 1];
-    uint32_t kept_scale[2] = {1u, 1u};
-    if (GRADIENT && mine) {                              // while the products are under way
-      if (row_weights) weight = __ldg(row_weights + row_at);
-      if (MODE == GRADIENT8) {
+    // GRADIENT: what was kept of z, 64 bytes of each of the warp's rows (8 bits: of both halves), comes in 16-byte pieces, four lanes to a row, and is
+    // handed to the rows' lanes through the staging.  (A lane with the 64 bytes of its own row: every load touched 32 lines, and moved 16 bytes a cycle
+    // of the data path that the MMAs read through; 16384 x 4096 x 1024 took 16 us longer than without them.)
+    float weight = 1.f, dot = 0.f;
+    uint4 piece[GRADIENT ? 4 : 1];
+    uint32_t kept[GRADIENT ? 16 : 1], scales = 0x0101u;
+    auto fetch = [&](int byte0) {                        // from this byte of the warp's columns
+      const long long pitch = MODE == GRADIENT8 ? N : 2LL * N, first = (MODE == GRADIENT8 ? col0 : 2LL * col0) + byte0 + (lane & 3) * 16;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (col0 + 32 * h < N) {
-            load_row8((const uint8_t*)p.z + row_at * N + col0 + 32 * h, *reinterpret_cast<uint32_t(*)[8]>(&kept[h]), N - col0 - 32 * h, wide);
-            kept_scale[h] = p.scale[row_at * blocks + col0 / 32 + h];
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        piece[i] = busy && quarter * 32 + r < rows && first < pitch ? *reinterpret_cast<const uint4*>((const uint8_t*)p.z + (warp_row + (long long)r) * pitch + first)
+                                                                     : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    auto hand_over = [&] {                               // pieces -> this lane's row; the staging is free
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        *reinterpret_cast<uint4*>(staging + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4)) = piece[i];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 v = *reinterpret_cast<const uint4*>(staging + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4));
+        kept[4 * j] = v.x; kept[4 * j + 1] = v.y; kept[4 * j + 2] = v.z; kept[4 * j + 3] = v.w;
+      }
+      __syncwarp();
+    };
+    const bool by_pieces = MODE == GRADIENT16 || p.q_rows16;
+    if (GRADIENT) {                                      // while the products are under way
+      if (by_pieces) fetch(0);
+      if (mine) {
+        if (row_weights) weight = __ldg(row_weights + row_at);
+        if (MODE == GRADIENT8) {
+          const uint8_t* at = p.scale + row_at * blocks + col0 / 32;
+          if (p.scale_pairs) scales = *reinterpret_cast<const uint16_t*>(at);
+          else scales = at[0] | (col0 + 32 < N ? (uint32_t)at[1] << 8 : 0x0100u);
+          if (!by_pieces) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) load_row8((const uint8_t*)p.z + row_at * N + col0 + 32 * h, *reinterpret_cast<uint32_t(*)[8]>(&kept[8 * h]), N - col0 - 32 * h, wide);
           }
+        }
       }
     }
     if (!sm100::mbar_wait_warp(&sh->acc_full[acc], (it >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 34); return false; }
@@ -339,29 +359,33 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
     for (int half = 0; half < 2; ++half) {
       const int col = col0 + 32 * half, left = N - col;
       if (half && left <= 0) { release(); break; }
-      uint32_t r[32], zb[16];
-      if (MODE == GRADIENT16 && mine) load_row((const __nv_bfloat16*)p.z + row_at * N + col, zb, left, wide);
+      uint32_t r[32];
+      if (GRADIENT && by_pieces && (MODE == GRADIENT16 || !half)) {
+        reuse(0);
+        hand_over();
+        if (MODE == GRADIENT16 && !half) fetch(64);
+      }
       sm100::tmem_ld_32x32(t_base + 32 * half, r);
       uint4 b[4];
       if (!GRADIENT && bias) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = 8 * j < left ? __ldg(reinterpret_cast<const uint4*>(bias + col) + j) : make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < 4; ++j) b[j] = __ldg(reinterpret_cast<const uint4*>(bias + (8 * j < left ? col + 8 * j : 0)));      // what lies behind N is never read
       }
       sm100::tmem_ld_wait();
       if (half) release();
       float v[32];
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
       if (!GRADIENT && bias) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t x[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            v[8 * j + 2 * q] += __uint_as_float(x[q] << 16);
-            v[8 * j + 2 * q + 1] += __uint_as_float(x[q] & 0xffff0000u);
-          }
+          for (int q = 0; q < 4; ++q)
+            attn_util::unpack2(attn_util::add2(attn_util::pack2(r[8 * j + 2 * q], r[8 * j + 2 * q + 1]), attn_util::pack2(x[q] << 16, x[q] & 0xffff0000u)), v[8 * j + 2 * q],
+                               v[8 * j + 2 * q + 1]);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
       }
       uint32_t w[16];
       if (MODE == PLAIN32) {
@@ -391,8 +415,18 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
       }
       if (MODE == KEEP8) {
         uint32_t q[8];
-        const uint32_t byte = act8::pack_block(v, q);    // columns behind N are zeros: the weight's rows there read as zero, and have no bias
-        if (mine) p.scale[row_at * blocks + col / 32] = (uint8_t)byte;
+        if (left < 32) {                                 // columns behind N do not count
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j >= left) v[j] = 0.f;
+        }
+        const uint32_t byte = act8::pack_block(v, q);
+        scales = half ? scales | byte << 8 : byte;
+        if (mine) {
+          uint8_t* at = p.scale + row_at * blocks + col0 / 32;
+          if (!p.scale_pairs) at[half] = (uint8_t)byte;
+          else if (half) *reinterpret_cast<uint16_t*>(at) = (uint16_t)scales;
+        }
         if (whole && p.q_rows16) {                       // rows of 64 bytes from both halves
           if (!half) reuse(0);
 #pragma unroll
@@ -409,7 +443,7 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
           attn_util::unpack2(quick_gelu2(attn_util::pack2(__float_as_uint(v[j]), __float_as_uint(v[j + 1]))), v[j], v[j + 1]);
       }
       if (GRADIENT) {
-        const float scale = act8::value(kept_scale[half]);
+        const float scale = act8::value(half ? scales >> 8 : scales & 0xffu);
         const unsigned long long weight2 = attn_util::pack2(__float_as_uint(weight), __float_as_uint(weight));
         unsigned long long dot2 = 0ull;
         uint32_t hw[16];
@@ -417,15 +451,15 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
         for (int j = 0; j < 32; j += 2) {
           float z0, z1, a0, a1;
           if (MODE == GRADIENT8) {
-            act8::unpack2(kept[half][j >> 2] >> (16 * ((j >> 1) & 1)), scale, &z0, &z1);
+            act8::unpack2(kept[8 * half + (j >> 2)] >> (16 * ((j >> 1) & 1)), scale, &z0, &z1);
           } else {
-            z0 = __uint_as_float(zb[j >> 1] << 16);
-            z1 = __uint_as_float(zb[j >> 1] & 0xffff0000u);
+            z0 = __uint_as_float(kept[j >> 1] << 16);
+            z1 = __uint_as_float(kept[j >> 1] & 0xffff0000u);
           }
           unsigned long long y, slope;
           quick_gelu_both2(attn_util::pack2(__float_as_uint(z0), __float_as_uint(z1)), &y, &slope);
           const unsigned long long g = attn_util::pack2(__float_as_uint(v[j]), __float_as_uint(v[j + 1]));
-          if (j < left) dot2 = attn_util::fma2(g, y, dot2);
+          dot2 = attn_util::fma2(g, y, dot2);            // columns behind N: the weight reads as zero there, and so does z
           attn_util::unpack2(attn_util::mul2(attn_util::mul2(g, slope), weight2), a0, a1);
           w[j >> 1] = attn_util::pack_bf16(__float_as_uint(a0), __float_as_uint(a1));
           attn_util::unpack2(attn_util::mul2(y, weight2), a0, a1);
@@ -433,7 +467,7 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
         }
         float a0, a1;
         attn_util::unpack2(dot2, a0, a1);
-        if (mine && p.dots) p.dots[row_at * blocks + col / 32] = a0 + a1;
+        dot += a0 + a1;
         if (whole) {
           reuse(1);
           stage(1, hw);
@@ -445,6 +479,7 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
           store_row(p.h + row_at * N + col, hw, left, wide);
           store_row(p.y + row_at * N + col, w, left, wide);
         }
+        if (mine && p.dots && (half || left <= 32)) p.dots[(long long)(col0 / SLICE) * p.rows + row_at] = dot;      // rows side by side
         continue;
       }
       pack_row(v, w);
@@ -636,7 +671,7 @@ __device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* 
             float dot = in ? v * y0 : 0.f;
 #pragma unroll
             for (int d = 16; d; d /= 2) dot += __shfl_xor_sync(~0u, dot, d);
-            if (lane == 0) p.dots[row * blocks + col / 32] = dot;
+            if (lane == 0) p.dots[(long long)(col / 32) * p.rows + row] = dot;
           }
           if (in) {
             p.h[at] = __float2bfloat16_rn(weight * y0);
@@ -1179,6 +1214,8 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   const int clusters = max_clusters();
   p.offsets = offsets; p.rows = rows; p.experts = nexperts; p.K = K; p.N = N;
   p.k_blocks = (K + BK - 1) / BK;
+  p.q_rows16 = N % 16 == 0;                              // z itself is on a 16-byte boundary
+  p.scale_pairs = N % 64 == 0 && !((uintptr_t)p.scale & 1);
   p.status = gemm_status_word();
   if (rows <= (long long)few_mean(mode) * nexperts) {
     p.slices = mode == PLAIN32 ? few_slices(rows, nexperts, K, N) : 1;
@@ -1208,7 +1245,6 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   const bool fp32 = mode == PLAIN32;
   if ((st = make_tmap_box(&my, fp32 ? 4 : 2, fp32 ? (const void*)p.y32 : p.y, (uint64_t)rows, (uint64_t)N, 32, 32))) return st;
   mz = my;
-  p.q_rows16 = N % 16 == 0;
   if (mode == WITH_GELU || mode == GRADIENT8 || mode == GRADIENT16) st = make_tmap_box(&mz, 2, mode == WITH_GELU ? p.z : p.h, (uint64_t)rows, (uint64_t)N, 32, 32);
   else if (mode == KEEP8 && p.q_rows16) st = make_tmap_box(&mz, 1, p.z, (uint64_t)rows, (uint64_t)N, 32, 64);
   if (st) return st;
@@ -1249,9 +1285,15 @@ int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int*
   return grouped::run(p, x, w, offsets, rows, nexperts, K, N, w_is_kn != 0, mode, (cudaStream_t)stream);
 }
 
+// the sums of a row that tmpi_grouped_gelu_gradient leaves in dots
+int tmpi_grouped_dots(int rows, int nexperts, int N, int kept8) {
+  const bool few = rows <= (long long)grouped::few_mean(kept8 ? grouped::GRADIENT8 : grouped::GRADIENT16) * nexperts;
+  return few ? (N + 31) / 32 : (N + grouped::SLICE - 1) / grouped::SLICE;
+}
+
 // The gradients of gelu(z) h's input and value in one product: with g = dy w_e (dy [rows, K], w [experts, K, N]) in fp32 and the kept z [rows, N] (bf16, or
 // with `scale` its 8-bit checkpoint), dz = weight g gelu'(z) and h = weight gelu(z), both bf16 [rows, N]; row_weights fp32 [rows] or null for
-// ones.  dots [rows, ceil(N / 32)] (or null): the sums of g gelu(z) over 32 columns each.  Rows behind the last group are left alone.
+// ones.  dots [tmpi_grouped_dots, rows] (or null): the sums of g gelu(z) over 32 or 64 columns each.  Rows behind the last group are left alone.
 int tmpi_grouped_gelu_gradient(const void* dy, const void* w, const int* offsets, const void* z, const void* scale, const float* row_weights, void* dz, void* h,
                                float* dots, int rows, int nexperts, int K, int N, void* stream) {
   if (!all_aligned16({z, dz, h}) || !z || !h) return fail(TMPI_ERR_INVALID, "grouped_gelu_gradient: tensors must be 16-byte aligned");
