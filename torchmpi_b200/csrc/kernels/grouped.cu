@@ -236,6 +236,18 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* to, const uint32_t (&w)
       if (8 * j < left) reinterpret_cast<uint4*>(to)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
   }
 }
+__device__ __forceinline__ void load_row(const __nv_bfloat16* from, uint32_t (&w)[16], int left, bool wide) {
+  if (wide && left >= 32) {
+    load32(from, w);
+    load32(from + 16, w + 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 v = 8 * j < left ? reinterpret_cast<const uint4*>(from)[j] : make_uint4(0u, 0u, 0u, 0u);
+      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+    }
+  }
+}
 // 32 e4m3 columns
 __device__ __forceinline__ void store_row8(uint8_t* to, const uint32_t (&q)[8], int left, bool wide) {
   if (wide && left >= 32) {
@@ -301,18 +313,19 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
     };
     const long long row_at = (long long)u.row0 + (int)rank * BM + row;
     const __nv_bfloat16* bias = bias_all ? bias_all + (long long)u.e * N : nullptr;
-    // GRADIENT: what was kept of z, 64 bytes of each of the warp's rows (8 bits: of both halves), comes in 16-byte pieces, four lanes to a row, and is
-    // handed to the rows' lanes through the staging.  (A lane with the 64 bytes of its own row: every load touched 32 lines, and moved 16 bytes a cycle
-    // of the data path that the MMAs read through; 16384 x 4096 x 1024 took 16 us longer than without them.)
+    // GRADIENT: what was kept of z.  8 bits: the 64 bytes of both halves come in 16-byte pieces, four lanes to a row, and are handed to the rows' lanes
+    // through the staging, once a tile (a lane with its own row's 64 bytes, every load over 32 lines: 147 us against 141 at 16384 x 4096 x 1024).  16 bits:
+    // a lane loads its own row, the first half before the products are there (through the staging, which then waits for the stores' reads twice a tile:
+    // 158 us against 154; both halves after the products: 159).
     float weight = 1.f, dot = 0.f;
-    uint4 piece[GRADIENT ? 4 : 1];
+    uint4 piece[MODE == GRADIENT8 ? 4 : 1];
     uint32_t kept[GRADIENT ? 16 : 1], scales = 0x0101u;
-    auto fetch = [&](int byte0) {                        // from this byte of the warp's columns
-      const long long pitch = MODE == GRADIENT8 ? N : 2LL * N, first = (MODE == GRADIENT8 ? col0 : 2LL * col0) + byte0 + (lane & 3) * 16;
+    auto fetch = [&] {
+      const long long first = col0 + (lane & 3) * 16;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = i * 8 + (lane >> 2);
-        piece[i] = busy && quarter * 32 + r < rows && first < pitch ? *reinterpret_cast<const uint4*>((const uint8_t*)p.z + (warp_row + (long long)r) * pitch + first)
+        piece[i] = busy && quarter * 32 + r < rows && first < N ? *reinterpret_cast<const uint4*>((const uint8_t*)p.z + (warp_row + (long long)r) * N + first)
                                                                      : make_uint4(0u, 0u, 0u, 0u);
       }
     };
@@ -330,10 +343,11 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
       }
       __syncwarp();
     };
-    const bool by_pieces = MODE == GRADIENT16 || p.q_rows16;
+    const bool by_pieces = MODE == GRADIENT8 && p.q_rows16;
     if (GRADIENT) {                                      // while the products are under way
-      if (by_pieces) fetch(0);
+      if (by_pieces) fetch();
       if (mine) {
+        if (MODE == GRADIENT16) load_row((const __nv_bfloat16*)p.z + row_at * N + col0, *reinterpret_cast<uint32_t(*)[16]>(kept), N - col0, wide);
         if (row_weights) weight = __ldg(row_weights + row_at);
         if (MODE == GRADIENT8) {
           const uint8_t* at = p.scale + row_at * blocks + col0 / 32;
@@ -360,11 +374,11 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
       const int col = col0 + 32 * half, left = N - col;
       if (half && left <= 0) { release(); break; }
       uint32_t r[32];
-      if (GRADIENT && by_pieces && (MODE == GRADIENT16 || !half)) {
+      if (MODE == GRADIENT8 && by_pieces && !half) {
         reuse(0);
         hand_over();
-        if (MODE == GRADIENT16 && !half) fetch(64);
       }
+      if (MODE == GRADIENT16 && half && mine) load_row((const __nv_bfloat16*)p.z + row_at * N + col, *reinterpret_cast<uint32_t(*)[16]>(kept), left, wide);
       sm100::tmem_ld_32x32(t_base + 32 * half, r);
       uint4 b[4];
       if (!GRADIENT && bias) {
