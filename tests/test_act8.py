@@ -234,3 +234,36 @@ def test_refuses_tensors_of_two_devices():
                  lambda: act8.mlp(x, torch.zeros(8, 32, device="cuda"), None, torch.zeros(8, 8), None)):
         with pytest.raises(ValueError):
             call()
+
+
+# ---------------------------------------------------------------- what a training program meets
+@gpu
+def test_saved_tensors_on_the_host_and_an_expanded_input():
+    x, w1, b1, w2, b2 = (t.requires_grad_() for t in _mlp_inputs(1, 40, 64, 24, "cuda")[:5])
+    leaves = (x, w1, b1, w2, b2)
+    dy = torch.randn(6, 24, device="cuda").bfloat16()
+    grads = lambda y: torch.autograd.grad(y, leaves, dy)
+    want = grads(act8.mlp(x.expand(6, 40).contiguous(), w1, b1, w2, b2))
+    with torch.autograd.graph.save_on_cpu():
+        y = act8.mlp(x.expand(6, 40), w1, b1, w2, b2)
+    for a, b, c in zip(want, grads(y), grads(act8.mlp(x.expand(6, 40), w1, b1, w2, b2))):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@gpu
+def test_more_elements_than_32_bits_count():
+    """The rows around and behind element 2^31 are those of small tensors (70000 x 32768, 4.6 GB)."""
+    n, C = 70000, 32768
+    x = torch.randn(n, C, device="cuda", dtype=torch.bfloat16)
+    a = act8.quantize(x)
+    y = act8.dequantize(a)
+    rows = [0, 65535, 65536, n - 1]
+    assert n * C > 2 ** 31
+    for i in rows:
+        assert _same(y[i].float().cpu(), ref.kept(x[i].cpu()).bfloat16().float())
+    del y
+    dz, h = act8.gelu_gradient(x, a)
+    for i in rows:
+        value, slope = ref.gelu(ref.V(ref.kept(x[i].cpu())))
+        ref.close(h[i], value.rounded(), f"value of row {i}")
+        ref.close(dz[i], ref.mul(ref.V(x[i].cpu()), slope).rounded(), f"gradient of row {i}")

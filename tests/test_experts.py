@@ -1,5 +1,8 @@
 """Layers of experts: routing, rows to the experts and back, products grouped by expert, and the whole layer."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -486,4 +489,105 @@ def test_wrong_offsets_stay_inside():
         y = experts.grouped_linear(*leaves, torch.tensor(bad, dtype=torch.int32, device="cuda"), True)
         torch.autograd.grad(y, leaves, torch.ones_like(y))
     torch.cuda.synchronize()
+    experts.check_status()
+
+
+# ---------------------------------------------------------------- what a training program meets
+@gpu
+@pytest.mark.parametrize("kept8", [False, True])
+def test_no_tokens(kept8):
+    x, w1, b1, w2, b2 = (t.requires_grad_() for t in (torch.empty(0, 8, device="cuda", dtype=BF), *(torch.randn(s, device="cuda").to(BF) for s in ((4, 16, 8), (4, 16), (4, 8, 16), (4, 8)))))
+    y = experts.mlp(x, experts.route(torch.empty(0, 4, device="cuda"), 2), w1, b1, w2, b2, kept8)
+    assert y.shape == (0, 8)
+    for g, t in zip(torch.autograd.grad(y.sum(), (x, w1, b1, w2, b2)), (x, w1, b1, w2, b2)):
+        assert g.shape == t.shape and bool((g == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("kept8", [False, True])
+def test_saved_tensors_on_the_host_and_an_expanded_input(kept8):
+    x, w1, b1, w2, b2 = leaves = [t.requires_grad_() for t in (torch.randn(1, 8, device="cuda").to(BF), *(torch.randn(s, device="cuda").to(BF) for s in ((4, 16, 8), (4, 16), (4, 8, 16), (4, 8))))]
+    r = experts.route(torch.randn(6, 4, device="cuda"), 2)
+    dy = torch.randn(6, 8, device="cuda").to(BF)
+    grads = lambda y: torch.autograd.grad(y, leaves, dy)
+    want = grads(experts.mlp(x.expand(6, 8).contiguous(), r, w1, b1, w2, b2, kept8))
+    with torch.autograd.graph.save_on_cpu():
+        y = experts.mlp(x.expand(6, 8), r, w1, b1, w2, b2, kept8)
+    for a, b, c in zip(want, grads(y), grads(experts.mlp(x.expand(6, 8), r, w1, b1, w2, b2, kept8))):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+CAPTURE = '''
+import sys, torch
+from torchmpi_b200.ops import act8, experts
+torch.manual_seed(0)
+new = lambda *s: torch.randn(s, device="cuda").bfloat16().requires_grad_()
+x, u1, u2, w1, w2 = new(64, 128), new(256, 128), new(128, 256), new(4, 256, 128), new(4, 128, 256)
+logits, dy = torch.randn(64, 4, device="cuda", requires_grad=True), torch.randn(64, 128, device="cuda").bfloat16()
+leaves = [x, u1, u2] if sys.argv[1] == "act8" else [x, logits, w1, w2]
+forward = (lambda: act8.mlp(x, u1, None, u2, None)) if sys.argv[1] == "act8" else (lambda: experts.mlp(x, experts.route(logits, 2), w1, None, w2, None, act8=True))
+def step():
+    y = forward()
+    if sys.argv[2] == "grad":
+        return torch.autograd.grad(y, leaves, dy)
+    y.backward(dy)
+    return [t.grad for t in leaves]
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(side):
+    step()
+    alive = forward() if sys.argv[3] == "side" else None           # an eager graph of the same leaves
+torch.cuda.current_stream().wait_stream(side)
+alive = alive if alive is not None else forward()
+for t in leaves:
+    t.grad = None
+with torch.cuda.stream(side):
+    want = [g.clone() for g in torch.autograd.grad(forward(), leaves, dy)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(graph):
+        got = step()
+except RuntimeError:
+    print("refused")
+    sys.exit(0)
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("as the eager step")
+'''
+
+
+@gpu
+@pytest.mark.parametrize("where", ["side", "default"])
+@pytest.mark.parametrize("how", ["grad", "backward"])
+@pytest.mark.parametrize("what", ["act8", "experts"])
+def test_captured_backward_while_an_eager_graph_lives(what, how, where):
+    """In a process of its own, which has to survive.  Where the eager graph was made on the default stream, autograd refuses the capture with an
+    exception for PyTorch's own operations as for these: a leaf's gradient belongs to the stream of the graph that met it first."""
+    out = subprocess.run([sys.executable, "-c", CAPTURE, what, how, where], capture_output=True, text=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert out.returncode == 0 and ("as the eager step" in out.stdout or where == "default" and "refused" in out.stdout), out.stderr[-2000:]
+
+
+@gpu
+def test_more_elements_than_32_bits_count():
+    """Both forms of the products, with results of more than 2^31 elements, against 64 bits at rows before and behind that border."""
+    R, K, N = 600000, 64, 4096
+    assert R * N > 2 ** 31
+    x, w, off = torch.randn(R, K, device="cuda").to(BF), torch.randn(3, N, K, device="cuda").to(BF), torch.tensor([0, 10, R - 70, R - 5], dtype=torch.int32, device="cuda")
+    groups = ((0, 3, 0), (10, 12, 1), (524286, 524290, 1), (R - 75, R - 70, 1), (R - 70, R - 5, 2))
+    y = experts.grouped_linear(x, w, None, off)
+    for a, b, e in groups:
+        ref.close(y[a:b], ref.matmul(ref.V(x[a:b].cpu()), ref.V(w[e].cpu()).t()).rounded(), f"rows {a} to {b}")
+    assert bool((y[R - 5:] == 0).all())
+    dw, = torch.autograd.grad(experts.grouped_linear(x, w.requires_grad_(), None, off), w, y)
+    ref.close(dw[2], ref.matmul(ref.V(y[R - 70:R - 5].cpu()).t(), ref.V(x[R - 70:R - 5].cpu())).rounded(), "dw of the last group")
+    del x, y, dw
+    R, N, E = 24000, 131072, 256
+    assert R * N > 2 ** 31
+    x, w, off = torch.randn(R, K, device="cuda").to(BF), torch.randn(E, N, K, device="cuda", dtype=BF), (torch.arange(E + 1, device="cuda") * R // E).int()
+    y = experts.grouped_linear(x, w, None, off)
+    for r in (0, 16383, 16384, R - 1):
+        e = int((off <= r).sum()) - 1
+        ref.close(y[r:r + 1], ref.matmul(ref.V(x[r:r + 1].cpu()), ref.V(w[e].cpu()).t()).rounded(), f"row {r}")
     experts.check_status()
