@@ -591,3 +591,20 @@ def test_more_elements_than_32_bits_count():
         e = int((off <= r).sum()) - 1
         ref.close(y[r:r + 1], ref.matmul(ref.V(x[r:r + 1].cpu()), ref.V(w[e].cpu()).t()).rounded(), f"row {r}")
     experts.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("kept8", [False, True])
+@pytest.mark.parametrize("T,H", [(200, 40), (200, 72), (200, 128), (6, 40)])
+def test_an_infinite_gradient_stays_infinite(T, H, kept8):
+    """Positive weights, activations and a gradient with one infinity: the routing weight's gradient is infinite, not NaN, whatever lies behind the columns."""
+    E, k, C = 2, 2, 16
+    x, w1, w2 = (torch.rand(s, device="cuda").add(0.5).to(BF) for s in ((T, C), (E, H, C), (E, C, H)))
+    r = experts.route(torch.zeros(T, E, device="cuda"), k)
+    weights = r.weights.clone().requires_grad_()
+    dy = torch.rand(T, C, device="cuda").add(0.5).to(BF)
+    dy[T // 2, 3] = math.inf
+    g, = torch.autograd.grad(experts.mlp(x, r._replace(weights=weights), w1, None, w2, None, kept8), weights, dy)
+    inf = torch.zeros_like(g, dtype=torch.bool)
+    inf[T // 2] = True
+    assert torch.equal(torch.isinf(g) & (g > 0), inf) and not bool(torch.isnan(g).any())

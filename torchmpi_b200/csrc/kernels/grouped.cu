@@ -427,13 +427,13 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
           store_row((__nv_bfloat16*)p.z + row_at * N + col, w, left, wide);
         }
       }
+      if ((MODE == KEEP8 || GRADIENT) && left < 32) {    // columns behind N do not count: an infinity times the weight's zeros there is NaN
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j >= left) v[j] = 0.f;
+      }
       if (MODE == KEEP8) {
         uint32_t q[8];
-        if (left < 32) {                                 // columns behind N do not count
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j >= left) v[j] = 0.f;
-        }
         const uint32_t byte = act8::pack_block(v, q);
         scales = half ? scales | byte << 8 : byte;
         if (mine) {
@@ -473,7 +473,7 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
           unsigned long long y, slope;
           quick_gelu_both2(attn_util::pack2(__float_as_uint(z0), __float_as_uint(z1)), &y, &slope);
           const unsigned long long g = attn_util::pack2(__float_as_uint(v[j]), __float_as_uint(v[j + 1]));
-          dot2 = attn_util::fma2(g, y, dot2);            // columns behind N: the weight reads as zero there, and so does z
+          dot2 = attn_util::fma2(g, y, dot2);            // columns behind N: z reads as zero there
           attn_util::unpack2(attn_util::mul2(attn_util::mul2(g, slope), weight2), a0, a1);
           w[j >> 1] = attn_util::pack_bf16(__float_as_uint(a0), __float_as_uint(a1));
           attn_util::unpack2(attn_util::mul2(y, weight2), a0, a1);
