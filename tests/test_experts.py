@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import expert_reference as ref
+from torchmpi_b200 import _native
 from torchmpi_b200.ops import act8, experts
 
 gpu = pytest.mark.gpu
@@ -608,3 +609,16 @@ def test_an_infinite_gradient_stays_infinite(T, H, kept8):
     inf = torch.zeros_like(g, dtype=torch.bool)
     inf[T // 2] = True
     assert torch.equal(torch.isinf(g) & (g > 0), inf) and not bool(torch.isnan(g).any())
+
+
+@gpu
+def test_widths_that_32_bits_do_not_count_are_left_to_pytorch():
+    """A width of 2^32 + 8 is not one of 8: the kernels' entries take none of these (views of one element, nothing is allocated)."""
+    ext, wide = _native.ext(), 2 ** 32 + 8
+    new = lambda *s: torch.zeros(1, device="cuda", dtype=BF).expand(s)
+    x, r = torch.zeros(4, 8, device="cuda", dtype=BF), experts.route(torch.zeros(4, 2, device="cuda"), 1)
+    assert ext.grouped_linear(x, new(2, wide, 8), None, r.offsets, False) is None
+    assert ext.grouped_linear(new(4, wide), new(2, 8, wide), None, r.offsets, False) is None
+    assert ext.expert_mlp(x, *r, new(2, wide, 8), None, new(2, 8, wide), None, False) is None
+    assert ext.act8_mlp(x, new(wide, 8), None, new(8, wide), None) is None
+    assert ext.act8_mlp(x, new(8, 8), None, new(wide, 8), None) is None

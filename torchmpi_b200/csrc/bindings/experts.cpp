@@ -4,6 +4,7 @@
 // memory comes from PyTorch's allocator on the calling stream, per call.
 #include "common.h"
 #include <c10/cuda/CUDAFunctions.h>
+#include <algorithm>
 #include <initializer_list>
 
 namespace tmpi_bind {
@@ -364,7 +365,7 @@ void register_experts(pybind11::module_& m) {
     const Tensor b1 = or_none(b1_), b2 = or_none(b2_);
     if (!(x.is_cuda() && x.dim() >= 1 && w1.dim() == 2 && w2.dim() == 2 && all_of_type({&x, &w1, &b1, &w2, &b2}, at::kBFloat16) && here({&x, &w1, &b1, &w2, &b2}))) return c10::nullopt;
     const int64_t C = w1.size(1), H = w1.size(0), D = w2.size(0), rows = x.size(-1) ? x.numel() / x.size(-1) : 0;
-    if (!(x.size(-1) == C && w2.size(1) == H && shaped(b1, {H}) && shaped(b2, {D}) && C % 8 == 0 && H % 8 == 0 && D % 8 == 0 && C && H && D && rows && rows <= MOST)) return c10::nullopt;
+    if (!(x.size(-1) == C && w2.size(1) == H && shaped(b1, {H}) && shaped(b2, {D}) && C % 8 == 0 && H % 8 == 0 && D % 8 == 0 && C && H && D && rows && std::max({rows, C, H, D}) <= MOST)) return c10::nullopt;
     const Tensor x2 = rows_of(x);
     Tensor y;
     if (wants_grad({x, w1, w2, b1, b2})) {
@@ -382,7 +383,7 @@ void register_experts(pybind11::module_& m) {
     const Tensor bias = or_none(bias_);
     if (!(x.is_cuda() && x.dim() == 2 && w.dim() == 3 && all_of_type({&x, &w, &bias}, at::kBFloat16) && offsets.scalar_type() == at::kInt && here({&x, &w, &bias, &offsets}))) return c10::nullopt;
     const int64_t E = w.size(0), N = w.size(1), K = w.size(2);
-    if (!(x.size(1) == K && shaped(bias, {E, N}) && shaped(offsets, {E + 1}) && K % 8 == 0 && N % 8 == 0 && w.numel() && E <= tmpi_grouped_max_experts() && x.size(0) && x.size(0) <= MOST)) return c10::nullopt;
+    if (!(x.size(1) == K && shaped(bias, {E, N}) && shaped(offsets, {E + 1}) && K % 8 == 0 && N % 8 == 0 && w.numel() && E <= tmpi_grouped_max_experts() && x.size(0) && std::max({x.size(0), N, K}) <= MOST)) return c10::nullopt;
     if (wants_grad({x, w, bias})) return GroupedLinearFn::apply(x, w, bias_, offsets, gelu);
     return grouped(packed(x), packed(w), bias.defined() ? packed(bias) : bias, offsets.contiguous(), false, gelu ? GELU : PLAIN, Tensor(), Tensor());
   });
@@ -416,7 +417,7 @@ void register_experts(pybind11::module_& m) {
           here({&x, &weights, &chosen, &order, &place, &offsets, &w1, &b1, &w2, &b2}))) return c10::nullopt;
     const int64_t E = w1.size(0), H = w1.size(1), C = w1.size(2), T = place.size(0), k = place.size(1);
     if (!(x.size(-1) == C && x.numel() == T * C && shaped(weights, {T, k}) && shaped(chosen, {T, k}) && shaped(order, {T * k}) && shaped(offsets, {E + 1}) && shaped(w2, {E, C, H}) &&
-          shaped(b1, {E, H}) && shaped(b2, {E, C}) && C % 8 == 0 && H % 8 == 0 && w1.numel() && E <= tmpi_grouped_max_experts() && T && T * k && T * k <= MOST)) return c10::nullopt;
+          shaped(b1, {E, H}) && shaped(b2, {E, C}) && C % 8 == 0 && H % 8 == 0 && w1.numel() && E <= tmpi_grouped_max_experts() && T && T * k && std::max({T * k, C, H}) <= MOST)) return c10::nullopt;
     const Layer l{packed(rows_of(x)), weights.contiguous(), chosen.contiguous(), place.contiguous(), offsets.contiguous(), packed(w1), b1.defined() ? packed(b1) : b1,
                   packed(w2), b2.defined() ? packed(b2) : b2};
     Tensor y;
