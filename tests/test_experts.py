@@ -622,3 +622,21 @@ def test_widths_that_32_bits_do_not_count_are_left_to_pytorch():
     assert ext.expert_mlp(x, *r, new(2, wide, 8), None, new(2, 8, wide), None, False) is None
     assert ext.act8_mlp(x, new(wide, 8), None, new(8, wide), None) is None
     assert ext.act8_mlp(x, new(8, 8), None, new(wide, 8), None) is None
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_second_derivatives_are_refused(device):
+    """A gradient asked for with a graph, which would be a constant in it, is refused."""
+    new = lambda *s: torch.randn(s, device=device).to(BF).requires_grad_()
+    x, w1, w2, u1, u2, logits = new(6, 16), new(4, 24, 16), new(4, 16, 24), new(24, 16), new(16, 24), torch.randn(6, 4, device=device, requires_grad=True)
+    r = experts.route(logits.detach(), 2)
+    calls = [(lambda: act8.mlp(x, u1, None, u2, None), (x, u1, u2)),
+             (lambda: experts.mlp(x, experts.route(logits, 2), w1, None, w2, None, act8=True), (x, logits, w1, w2))]
+    if device == "cuda":                      # elsewhere these are PyTorch's operations, which can be differentiated again
+        calls += [(lambda: experts.mlp(x, r, w1, None, w2, None), (x, w1, w2)), (lambda: experts.route(logits, 2).weights, (logits,)),
+                  (lambda: experts.dispatch(x, r), (x,)), (lambda: experts.combine(x.repeat(2, 1), r), (x,)),
+                  (lambda: experts.grouped_linear(x, w1, None, torch.tensor([0, 2, 2, 5, 6], dtype=torch.int32, device=device)), (x, w1))]
+    for call, leaves in calls:
+        torch.autograd.grad(call().sum(), leaves)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(call().sum(), leaves, create_graph=True)

@@ -23,6 +23,9 @@ bool wants_grad(std::initializer_list<Tensor> inputs) {
   return false;
 }
 
+// The kernels' gradients are constants to autograd: one asked for with a graph (create_graph) would lose its part of what it enters in silence.
+void refuse_graph() { TORCH_CHECK(!at::GradMode::is_enabled(), "layers of experts and 8-bit checkpoints can be differentiated once (no create_graph)"); }
+
 // all on the current device, which there is one of per process
 bool here(std::initializer_list<const Tensor*> tensors) {
   const int64_t device = c10::cuda::current_device();
@@ -118,6 +121,7 @@ struct GroupedLinearFn : public torch::autograd::Function<GroupedLinearFn> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_graph();
     const auto saved = ctx->get_saved_variables();
     const Tensor x = as_saved(saved[0]), w = as_saved(saved[1]), offsets = as_saved(saved[2]), z = as_saved(saved[3]);
     Tensor dy = packed(grads[0]), dx, dw, db;
@@ -148,6 +152,7 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_graph();
     const auto saved = ctx->get_saved_variables();
     const Kept kx{as_saved(saved[0]), as_saved(saved[1])}, kz{as_saved(saved[2]), as_saved(saved[3])};
     const Tensor w1 = as_saved(saved[4]), w2 = as_saved(saved[5]), dy = packed(grads[0]);
@@ -197,6 +202,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_graph();
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
     const Tensor logits = dense_columns(saved[0]);
@@ -239,6 +245,7 @@ struct DispatchFn : public torch::autograd::Function<DispatchFn> {
     return dispatch(packed(x), place, offsets.contiguous());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_graph();
     const auto saved = ctx->get_saved_variables();
     return {combine(packed(grads[0]), Tensor(), as_saved(saved[0]), grads[0].scalar_type()), Tensor(), Tensor()};
   }
@@ -251,6 +258,7 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
     return combine(rows, weights, place, rows.scalar_type());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_graph();
     const auto saved = ctx->get_saved_variables();
     const Tensor rows = as_saved(saved[0]), weights = as_saved(saved[1]), place = as_saved(saved[2]), offsets = as_saved(saved[3]), dy = packed(grads[0]);
     const bool need_w = ctx->needs_input_grad(1);
@@ -303,6 +311,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_graph();
     const auto saved = ctx->get_saved_variables();
     const Kept kx{as_saved(saved[0]), as_saved(saved[1])}, kz{as_saved(saved[2]), as_saved(saved[3])};
     const Tensor weights = as_saved(saved[4]), chosen = as_saved(saved[5]), place = as_saved(saved[6]), offsets = as_saved(saved[7]), w1 = as_saved(saved[8]),

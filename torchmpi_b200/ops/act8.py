@@ -123,6 +123,12 @@ def gelu_gradient(dy: torch.Tensor, a: Act8) -> Tuple[torch.Tensor, torch.Tensor
     return (dy.detach().float() * slope).to(dy.dtype), h.to(dy.dtype)
 
 
+def refuse_graph() -> None:
+    """Called by backward functions whose gradients are constants to autograd: one asked for with a graph would lose its part of what it enters in silence."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("layers of experts and 8-bit checkpoints can be differentiated once (no create_graph)")
+
+
 class _Mlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, b1, w2, b2):
@@ -132,6 +138,7 @@ class _Mlp(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        refuse_graph()
         xq, xs, zq, zs, w1, b1, w2, b2 = ctx.saved_tensors
         x, z, dy = _dequantize(Act8(xq, xs), torch.float32), _dequantize(Act8(zq, zs), torch.float32), dy.float()
         h, slope = _gelu_parts(z)

@@ -115,6 +115,7 @@ class _Mlp8(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _act8.refuse_graph()
         xq, xs, zq, zs, weights, w1, b1, w2, b2, order, place, offsets = ctx.saved_tensors
         k, n = place.shape[1], order.shape[0]
         x, z = _act8._dequantize(_act8.Act8(xq, xs), torch.float32), _act8._dequantize(_act8.Act8(zq, zs), torch.float32)
