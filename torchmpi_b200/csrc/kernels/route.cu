@@ -2,14 +2,15 @@
 // weights' gradient.
 //
 // G lanes take a token; a lane holds the logits of experts lane, lane + G, ... as integers that compare like the values, and the best of them apart, so that a
-// round of the choice is a maximum over G lanes (log G exchanges of value and index, the lower index of equals) and a new best of the lane that lost its
-// own.  The order by expert is a counting sort in two launches: the first counts the choices of a block of tokens per expert; the second adds the counts of
-// the blocks in front, and each warp places a contiguous part of the block's choices, 32 at a time, equal ones ranked by their lane.  So entries of an expert
+// round of the choice is a maximum over G lanes, a vote for its owner (of equals, which are rare, the lowest index by a second minimum) and a new best of
+// the lane that lost its own.  The order by expert is a counting sort in two launches: the first counts the choices of a block of tokens per expert; the second adds the counts of
+// the blocks in front, and each warp ranks a contiguous part of the block's choices, 32 at a time, equal ones by their lane, and places them when all ranks are known.  So entries of an expert
 // keep their order, and no atomic decides about a place.  Up to SMALL choices one block does both.
 //
 // The choice is bound by instructions, the rest by latency, a few dependent passes over little data, hence as many warps as an SM takes.  65536 tokens of 64
 // experts, 8 each, forward: 200 us with 8 warps a block, a warp to a token and a thread per expert that walked all choices of its block; 50 with 32
-// warps and a warp to a token; 46 with eight lanes to a token, and the gradient 10 where it took 20.
+// warps and a warp to a token; 45 with eight lanes to a token, and the gradient 10 where it took 20.  The owner by a vote, where index and value
+// were exchanged together, and ranks formed once in place of twice: 8192 tokens of 256 experts 42 -> 36, of 128 21 -> 20, the 65536 of 64 by 1 %.
 #include "pdl.cuh"
 #include "vec.cuh"
 #include "../include/tmpi_c_api.h"
@@ -94,6 +95,8 @@ __device__ __forceinline__ void choose(const Problem& p, const T* logits, long l
     for (int r = 0; r < R; ++r)
       if (any && g + G * r < p.experts) sum += expf(of_key(key[r]) - top);
   }
+  constexpr unsigned ALL = G == 32 ? ~0u : (1u << (G & 31)) - 1;
+  const int base = (int)(threadIdx.x & 31) & ~(G - 1);             // the group's first lane
   float mine[Q];
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
@@ -102,19 +105,22 @@ __device__ __forceinline__ void choose(const Problem& p, const T* logits, long l
 #pragma unroll 1
     for (int j = 0; j < G && q * G + j < p.k; ++j) {
       uint32_t m = best;
-      int i = at;
 #pragma unroll
-      for (int d = G / 2; d; d /= 2) {
-        const uint32_t m2 = __shfl_xor_sync(~0u, m, d);
-        const int i2 = __shfl_xor_sync(~0u, i, d);
-        if (m2 > m || (m2 == m && i2 < i)) { m = m2; i = i2; }
+      for (int d = G / 2; d; d /= 2) m = max(m, __shfl_xor_sync(~0u, m, d));
+      const bool there = m > KEY_NONE;                             // else nothing is left that may be used
+      const unsigned have = __ballot_sync(~0u, there && best == m) >> base & ALL;
+      int i = __shfl_sync(~0u, at, base + __ffs(have) - 1);        // none: any lane's
+      if (__any_sync(~0u, (have & (have - 1)) != 0)) {             // equal ones: the lowest index
+        i = best == m ? at : p.experts;
+#pragma unroll
+        for (int d = G / 2; d; d /= 2) i = min(i, __shfl_xor_sync(~0u, i, d));
       }
-      if (m <= KEY_NONE) i = -1;                                   // nothing left that may be used
+      if (!there) i = -1;
       if (g == j) {
         chosen[q] = i;
         mine[q] = __uint_as_float(m);
       }
-      if (i >= 0 && i % G == g) {
+      if (i == at) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
           if (i == g + G * r) key[r] = 0;
@@ -234,10 +240,14 @@ __device__ __forceinline__ void place_block(const Problem& p, Place& s, const in
   }
   int* mine = s.base[warp];
   const int bits = 32 - __clz(p.experts - 1);                      // none for one expert
-  for_choices(p, [&](int c, long long) {
+  for_choices(p, [&](int c, long long entry) {                     // a choice's rank among those of this warp; kept where its place will be
     const unsigned same = same_choice(c, bits);
+    int rank = -1;
+    if (c >= 0) rank = mine[c] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
     if (c >= 0 && lane == __ffs(same) - 1) mine[c] += __popc(same);
     __syncwarp();
+    if (c >= -1) p.place[entry] = rank;
   });
   __syncthreads();
   for (int e = warp; e < p.experts; e += WARPS) {                  // a warp to an expert: the counts of the block's warps, each behind those in front
@@ -251,15 +261,11 @@ __device__ __forceinline__ void place_block(const Problem& p, Place& s, const in
     s.base[lane][e] = s.start[e] + upto - n;
   }
   __syncthreads();
-  for_choices(p, [&](int c, long long entry) {
-    const unsigned same = same_choice(c, bits);
-    int at = -1;
-    if (c >= 0) at = mine[c] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (c >= 0 && lane == __ffs(same) - 1) mine[c] += __popc(same);
-    __syncwarp();
-    if (c >= 0) p.order[at] = (int)entry;
-    if (c >= -1) p.place[entry] = at;
+  for_choices(p, [&](int c, long long entry) {                     // the same thread has the same choices
+    if (c < 0) return;
+    const int at = mine[c] + p.place[entry];
+    p.order[at] = (int)entry;
+    p.place[entry] = at;
   });
   for (long long i = used + (long long)blockIdx.x * THREADS + tid; i < (long long)p.tokens * p.k; i += (long long)gridDim.x * THREADS) p.order[i] = -1;
 }
