@@ -70,14 +70,15 @@ __host__ __device__ constexpr int staging_of(int mode) { return mode == PLAIN ||
 
 struct Sh {
   uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  uint64_t kept[4 * ROW_GROUPS];                        // GRADIENT8: what was kept of z for a warp's part of the tile
   uint32_t tmem_base;
   int error;
   int warp_sums[8];
   int tile_end[MAX_EXPERTS];                            // tiles of the experts up to and with this one
 };
-constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + 32768 + 1024 + 1280;
+constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + 32768 + 1024 + 1408;
 static_assert(5 * STAGE_BYTES + 16 * 4096 == 6 * STAGE_BYTES + 16 * 2048 && 6 * STAGE_BYTES + 16 * 2048 == STAGES * STAGE_BYTES + 32768, "staging");
-static_assert(sizeof(Sh) <= 1280 && SMEM <= 232448, "shared memory of one CTA");
+static_assert(sizeof(Sh) <= 1408 && SMEM <= 232448, "shared memory of one CTA");
 
 // Offsets as given, but inside the tensor and not before the group's start: wrong ones give wrong results, never an access outside.
 struct Group { int r0, r1; };
@@ -236,18 +237,6 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* to, const uint32_t (&w)
       if (8 * j < left) reinterpret_cast<uint4*>(to)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
   }
 }
-__device__ __forceinline__ void load_row(const __nv_bfloat16* from, uint32_t (&w)[16], int left, bool wide) {
-  if (wide && left >= 32) {
-    load32(from, w);
-    load32(from + 16, w + 8);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint4 v = 8 * j < left ? reinterpret_cast<const uint4*>(from)[j] : make_uint4(0u, 0u, 0u, 0u);
-      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
-    }
-  }
-}
 // 32 e4m3 columns
 __device__ __forceinline__ void store_row8(uint8_t* to, const uint32_t (&q)[8], int left, bool wide) {
   if (wide && left >= 32) {
@@ -281,9 +270,11 @@ __device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]
 // 8-bit checkpoint, whose blocks of 32 columns a thread has to itself.
 template <int MODE>
 __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Problem& p, const int* offsets, const __nv_bfloat16* bias_all, const float* row_weights,
-                                       const CUtensorMap* map_y, const CUtensorMap* map_z, uint32_t rank, int group, int quarter, int lane) {
+                                       const CUtensorMap* map_y, const CUtensorMap* map_z, const CUtensorMap* map_kept, uint32_t rank, int group, int quarter, int lane) {
   constexpr bool GRADIENT = MODE == GRADIENT8 || MODE == GRADIENT16;
   const int row = quarter * 32 + lane, N = p.N, bn = p.bn, blocks = (N + 31) / 32;
+  uint64_t* kept_bar = &sh->kept[group * 4 + quarter];
+  uint32_t kept_phase = 0;
   const bool wide = p.wide != 0;
   for_tiles(sh, p, offsets, [&](const Unit& u, int it) -> bool {
     const int acc = it & 1, rows = u.part_rows(rank), c0 = group * SLICE, col0 = u.n_blk * bn + c0;
@@ -313,47 +304,26 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
     };
     const long long row_at = (long long)u.row0 + (int)rank * BM + row;
     const __nv_bfloat16* bias = bias_all ? bias_all + (long long)u.e * N : nullptr;
-    // GRADIENT: what was kept of z.  8 bits: the 64 bytes of both halves come in 16-byte pieces, four lanes to a row, and are handed to the rows' lanes
-    // through the staging, once a tile (a lane with its own row's 64 bytes, every load over 32 lines: 147 us against 141 at 16384 x 4096 x 1024).  16 bits:
-    // a lane loads its own row, the first half before the products are there (through the staging, which then waits for the stores' reads twice a tile:
-    // 158 us against 154; both halves after the products: 159).
+    // GRADIENT: what was kept of z comes through the TMA unit into the warp's staging while the products are under way, and is in registers before
+    // results are staged there.  16384 x 4096 x 1024, each pair measured in turn: 8 bits 136.0 us (139.7 with 16-byte loads, four lanes to a row, handed over
+    // through the staging; 147 against 141 with a lane's own row), 16 bits 140.6 (147.0 with a lane's own row).
     float weight = 1.f, dot = 0.f;
-    uint4 piece[MODE == GRADIENT8 ? 4 : 1];
-    uint32_t kept[GRADIENT ? 16 : 1], scales = 0x0101u;
-    auto fetch = [&] {
-      const long long first = col0 + (lane & 3) * 16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
-        piece[i] = busy && quarter * 32 + r < rows && first < N ? *reinterpret_cast<const uint4*>((const uint8_t*)p.z + (warp_row + (long long)r) * N + first)
-                                                                     : make_uint4(0u, 0u, 0u, 0u);
-      }
-    };
-    auto hand_over = [&] {                               // pieces -> this lane's row; the staging is free
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
-        *reinterpret_cast<uint4*>(staging + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4)) = piece[i];
-      }
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint4 v = *reinterpret_cast<const uint4*>(staging + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4));
-        kept[4 * j] = v.x; kept[4 * j + 1] = v.y; kept[4 * j + 2] = v.z; kept[4 * j + 3] = v.w;
-      }
-      __syncwarp();
-    };
-    const bool by_pieces = MODE == GRADIENT8 && p.q_rows16;
+    uint32_t kept[MODE == GRADIENT8 ? 16 : GRADIENT ? 32 : 1], scales = 0x0101u;
+    const bool by_tma = MODE == GRADIENT16 || (MODE == GRADIENT8 && p.q_rows16);
     if (GRADIENT) {                                      // while the products are under way
-      if (by_pieces) fetch();
+      if (by_tma && busy && lane == 0) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        sm100::mbar_expect_tx(kept_bar, MODE == GRADIENT8 ? 2048 : 4096);
+        sm100::tma_load_2d(staging, map_kept, col0, warp_row, kept_bar);
+        if (MODE == GRADIENT16) sm100::tma_load_2d(staging + 2048, map_kept, col0 + 32, warp_row, kept_bar);
+      }
       if (mine) {
-        if (MODE == GRADIENT16) load_row((const __nv_bfloat16*)p.z + row_at * N + col0, *reinterpret_cast<uint32_t(*)[16]>(kept), N - col0, wide);
         if (row_weights) weight = __ldg(row_weights + row_at);
         if (MODE == GRADIENT8) {
           const uint8_t* at = p.scale + row_at * blocks + col0 / 32;
           if (p.scale_pairs) scales = *reinterpret_cast<const uint16_t*>(at);
           else scales = at[0] | (col0 + 32 < N ? (uint32_t)at[1] << 8 : 0x0100u);
-          if (!by_pieces) {
+          if (!by_tma) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) load_row8((const uint8_t*)p.z + row_at * N + col0 + 32 * h, *reinterpret_cast<uint32_t(*)[8]>(&kept[8 * h]), N - col0 - 32 * h, wide);
           }
@@ -374,11 +344,16 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
       const int col = col0 + 32 * half, left = N - col;
       if (half && left <= 0) { release(); break; }
       uint32_t r[32];
-      if (MODE == GRADIENT8 && by_pieces && !half) {
-        reuse(0);
-        hand_over();
+      if (GRADIENT && by_tma && !half) {
+        if (!sm100::mbar_wait_warp(kept_bar, kept_phase, kWaitBudgetNs, &sh->error)) { give_up(sh, p.status, 35); return false; }
+        kept_phase ^= 1;
+#pragma unroll
+        for (int j = 0; j < (MODE == GRADIENT8 ? 4 : 8); ++j) {
+          const uint4 v = *reinterpret_cast<const uint4*>(staging + (j >> 2) * 2048 + lane * 64 + (((j & 3) ^ (lane >> 1 & 3)) << 4));
+          kept[4 * j] = v.x; kept[4 * j + 1] = v.y; kept[4 * j + 2] = v.z; kept[4 * j + 3] = v.w;
+        }
+        __syncwarp();
       }
-      if (MODE == GRADIENT16 && half && mine) load_row((const __nv_bfloat16*)p.z + row_at * N + col, *reinterpret_cast<uint32_t(*)[16]>(kept), left, wide);
       sm100::tmem_ld_32x32(t_base + 32 * half, r);
       uint4 b[4];
       if (!GRADIENT && bias) {
@@ -467,8 +442,8 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
           if (MODE == GRADIENT8) {
             act8::unpack2(kept[8 * half + (j >> 2)] >> (16 * ((j >> 1) & 1)), scale, &z0, &z1);
           } else {
-            z0 = __uint_as_float(kept[j >> 1] << 16);
-            z1 = __uint_as_float(kept[j >> 1] & 0xffff0000u);
+            z0 = __uint_as_float(kept[16 * half + (j >> 1)] << 16);
+            z1 = __uint_as_float(kept[16 * half + (j >> 1)] & 0xffff0000u);
           }
           unsigned long long y, slope;
           quick_gelu_both2(attn_util::pack2(__float_as_uint(z0), __float_as_uint(z1)), &y, &slope);
@@ -520,7 +495,8 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
 template <int MODE, bool B_MN>
 __global__ void __launch_bounds__(ROW_THREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_few, const __grid_constant__ CUtensorMap map_b,
-               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z, const __grid_constant__ Problem p) {
+               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z, const __grid_constant__ CUtensorMap map_kept,
+               const __grid_constant__ Problem p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   constexpr int NST = stages_of(MODE);
@@ -532,6 +508,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     sm100::tma_prefetch_desc(&map_b);
     for (int s = 0; s < NST; ++s) { sm100::mbar_init(&sh->full[s], 1); sm100::mbar_init(&sh->empty[s], 1); }
     for (int a = 0; a < 2; ++a) { sm100::mbar_init(&sh->acc_full[a], 1); sm100::mbar_init(&sh->acc_empty[a], 8 * ROW_GROUPS); }
+    if (MODE == GRADIENT8 || MODE == GRADIENT16)
+      for (int w = 0; w < 4 * ROW_GROUPS; ++w) sm100::mbar_init(&sh->kept[w], 1);
     sh->error = 0;
     sm100::fence_barrier_init();
   }
@@ -556,7 +534,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   } else if (warp == 1) {
     if (rank == 0 && sm100::elect_one()) issue<NST, B_MN>(sh, tiles, p, offsets);
   } else {
-    finish<MODE>(sh, tiles + (size_t)NST * STAGE_BYTES + (warp - 2) * staging_of(MODE), p, offsets, bias, row_weights, &map_y, &map_z, rank, (warp - 2) >> 2, warp & 3, lane);
+    finish<MODE>(sh, tiles + (size_t)NST * STAGE_BYTES + (warp - 2) * staging_of(MODE), p, offsets, bias, row_weights, &map_y, &map_z, &map_kept, rank, (warp - 2) >> 2, warp & 3, lane);
   }
   __syncwarp();
   // neither CTA frees its tensor memory or exits while the other may still signal its barriers or have the pair's MMAs read its shared memory
@@ -583,7 +561,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 // behind the group's end is not touched.
 constexpr int FEW_BM = 128, FEW_BN = 128, FEW_STAGES = 6, FEW_EPI_WARPS = 16, FEW_THREADS = 64 + FEW_EPI_WARPS * 32;
 constexpr int FEW_A_BYTES = FEW_BM * BK * 2, FEW_STAGE_BYTES = FEW_A_BYTES + FEW_BN * BK * 2;
-constexpr size_t FEW_SMEM = (size_t)FEW_STAGES * FEW_STAGE_BYTES + 1024 + 1280;
+constexpr size_t FEW_SMEM = (size_t)FEW_STAGES * FEW_STAGE_BYTES + 1024 + 1408;
 static_assert(FEW_STAGES == STAGES && FEW_SMEM <= 232448, "shared memory of one CTA");
 
 struct FewUnit { int e, row0, rows, col0, kb0, kb1, slice; };      // first row and rows of x, row of the weight, blocks of K
@@ -1249,7 +1227,7 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   const long long tiles_m = rows / (2 * BM) + std::min(nexperts, rows);        // at most
   p.bn = tile_columns(tiles_m, N, clusters);
   p.tiles_n = (N + p.bn - 1) / p.bn;
-  CUtensorMap ma, ma_few, mb, my, mz;
+  CUtensorMap ma, ma_few, mb, my, mz, mkept;
   if ((st = make_tmap_bf16(&ma, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, BM))) return st;
   if ((st = make_tmap_bf16(&ma_few, x, (uint64_t)rows, (uint64_t)K, (uint64_t)K, FEW))) return st;
   if (w_is_kn) st = make_tmap_bf16_3d(&mb, w, (uint64_t)nexperts, (uint64_t)K, (uint64_t)N, BK, 64);
@@ -1258,11 +1236,14 @@ static int run(Problem p, const void* x, const void* w, const int* offsets, int 
   // results go in boxes of 32 rows x 64 bytes (128 in fp32): y, and beside it z, h or the e4m3 numbers
   const bool fp32 = mode == PLAIN32;
   if ((st = make_tmap_box(&my, fp32 ? 4 : 2, fp32 ? (const void*)p.y32 : p.y, (uint64_t)rows, (uint64_t)N, 32, 32))) return st;
-  mz = my;
+  mz = mkept = my;
+  if (mode == GRADIENT8 && p.q_rows16) st = make_tmap_box(&mkept, 1, p.z, (uint64_t)rows, (uint64_t)N, 32, 64);
+  else if (mode == GRADIENT16) st = make_tmap_box(&mkept, 2, p.z, (uint64_t)rows, (uint64_t)N, 32, 32);
+  if (st) return st;
   if (mode == WITH_GELU || mode == GRADIENT8 || mode == GRADIENT16) st = make_tmap_box(&mz, 2, mode == WITH_GELU ? p.z : p.h, (uint64_t)rows, (uint64_t)N, 32, 32);
   else if (mode == KEEP8 && p.q_rows16) st = make_tmap_box(&mz, 1, p.z, (uint64_t)rows, (uint64_t)N, 32, 64);
   if (st) return st;
-  void* args[] = {&ma, &ma_few, &mb, &my, &mz, &p};
+  void* args[] = {&ma, &ma_few, &mb, &my, &mz, &mkept, &p};
   const cudaError_t e = launch(row_kernel(mode, w_is_kn, false), std::min<long long>(tiles_m * p.tiles_n, clusters), 2, ROW_THREADS, SMEM, args, stream);
   return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "grouped_gemm launch: %s", cudaGetErrorString(e));
 }
