@@ -277,6 +277,9 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
 // in bf16 or (act8) in 8 bits, and neither the dispatched rows nor what the experts returned: the rows are gathered again, and the weight's gradient
 // dy . (w2 h + b2) is (w2^T dy) . h + dy . b2, of which the first product is there anyway.  What a token's experts return, and the gradients
 // that they return to it, are handed over in fp32 and rounded once, as their sum.
+// Roundings that are choices: weight gelu(z) and dz to bf16, as operands of the MMAs, and without act8 the pre-activation to bf16, as a layer of bf16
+// tensors has it (fp32 would double what is kept).  15 tokens, 4 of 10 experts, 520 -> 512, errors relative to the norms: dw2 0.0017 from the rounding of the
+// result alone, 0.0024 with that of weight gelu(z), 0.0030 with that of z; the weights' gradient has the last alone, 0.0020 where the result's is 0.0016.
 struct Layer { Tensor x, weights, chosen, place, offsets, w1, b1, w2, b2; };
 
 // keep: the checkpoints go to kx and kz
