@@ -328,7 +328,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     const Tensor by_place = at::empty({T * k}, f32), g = dispatch(dy, place, Tensor(), weights, by_place);
     const int64_t slices = tmpi_grouped_dots((int)(T * k), (int)E, (int)H, kz.scale.defined());
     Tensor dots, dwt;
-    if (need_wt) dots = at::empty({slices, T * k}, f32);
+    if (need_wt) dots = at::empty({(slices + 3) / 4, T * k, 4}, f32);
     const auto both = grouped_gelu_gradient(g, w2, offsets, kz, by_place, dots);
     const Tensor dz = both.first, hw = both.second;
     if (need_wt) {

@@ -404,7 +404,7 @@ int tmpi_grouped_max_experts(void);
 int tmpi_grouped_slices(int rows, int nexperts, int K, int N);   // fp32 results of mode 4
 int tmpi_grouped_gemm(const void* x, const void* w, const void* bias, const int* offsets, void* y, void* z, void* scale, int rows, int nexperts, int K, int N,
                       int w_is_kn, int mode, void* stream);
-int tmpi_grouped_dots(int rows, int nexperts, int N, int kept8);   // the first extent of dots
+int tmpi_grouped_dots(int rows, int nexperts, int N, int kept8);   // slices of dots
 int tmpi_grouped_gelu_gradient(const void* dy, const void* w, const int* offsets, const void* z, const void* scale, const float* row_weights, void* dz, void* h,
                                float* dots, int rows, int nexperts, int K, int N, void* stream);
 int tmpi_grouped_weight_gradient(const void* dy, const void* x, const int* offsets, const float* row_weights, void* dw, void* db, int rows, int nexperts, int K,

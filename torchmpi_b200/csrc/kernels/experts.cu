@@ -262,10 +262,10 @@ __global__ void __launch_bounds__(GRAD_THREADS) combine_gradient_kernel(const T*
   clear_rest<T, V, GRAD_THREADS>(used, drows, places, cols);
 }
 
-// The weights' gradient in a layer of experts, a warp to a token: dweights[entry] = the sum of the entry's place over `dots` [slices, places]
-// (grouped.cu) + dy[token] . bias[expert]; 0 for entries without a place.  By tokens, what belongs to the entries and the row of dy are one step of
-// loads, and the row is read once: 12.8 us for 8192 x 1024 and two experts of eight; by places, which come in the order of the experts, 20.  (With the
-// slices of eight or sixteen tokens shared by a block's threads, in lines, 11.1 and 15.0, but 36.1 and 46.2 in place of 34.1 for eight of 64.)
+// The weights' gradient in a layer of experts, a warp to a token: dweights[entry] = the sum of the entry's place over `dots` (four slices side by side,
+// grouped.cu) + dy[token] . bias[expert]; 0 for entries without a place.  By tokens, what belongs to the entries and the row of dy are one step of
+// loads, and the row is read once; two entries at a time, the slices of each by half a warp.  8192 x 1024 and two
+// experts of eight 9.8 us, eight of 64 27.5; 12.8 and 34.2 where each slice lay apart (a lane to a slice: a load touched 32 lines).
 template <int V>
 __global__ void __launch_bounds__(THREADS) weight_gradient_kernel(const float* __restrict__ dots, const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ bias,
                                                                   const int* __restrict__ place, const int* __restrict__ chosen, float* __restrict__ dweights,
@@ -275,19 +275,23 @@ __global__ void __launch_bounds__(THREADS) weight_gradient_kernel(const float* _
   for (long long t = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); t < tokens; t += (long long)gridDim.x * WARPS) {
     constexpr int J = 2, U = 4;
     for (int j0 = 0; j0 < k; j0 += J) {
-      int s[J], e[J];
+      const int js = j0 + (lane >> 4);                    // the entry whose slices this lane adds
+      const int s = js < k ? place[t * k + js] : -1;
+      int e[J];
       float sum[J];
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        s[j] = j0 + j < k ? place[t * k + j0 + j] : -1;
         e[j] = j0 + j < k && bias ? chosen[t * k + j0 + j] : -1;
         sum[j] = 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-        if ((unsigned)s[j] < (unsigned)places)
+      const bool there = (unsigned)s < (unsigned)places;
+      float of_slices = 0.f;
+      if (there)
 #pragma unroll 2
-          for (int i = lane; i < slices; i += 32) sum[j] += dots[(long long)i * places + s[j]];
+        for (int i = lane & 15; 4 * i < slices; i += 16) {
+          const float4 v = *reinterpret_cast<const float4*>(dots + ((long long)i * places + s) * 4);
+          of_slices += v.x + (4 * i + 1 < slices ? v.y : 0.f) + (4 * i + 2 < slices ? v.z : 0.f) + (4 * i + 3 < slices ? v.w : 0.f);
+        }
       if (bias)
         for (int c0 = lane; c0 < parts; c0 += 32 * U) {
           Pack<__nv_bfloat16, V> g[U];
@@ -309,10 +313,10 @@ __global__ void __launch_bounds__(THREADS) weight_gradient_kernel(const float* _
           }
         }
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const float total = warp_sum(sum[j]);
-        if (lane == 0 && j0 + j < k) dweights[t * k + j0 + j] = (unsigned)s[j] < (unsigned)places ? total : 0.f;
-      }
+      for (int d = 8; d; d /= 2) of_slices += __shfl_xor_sync(~0u, of_slices, d);
+#pragma unroll
+      for (int j = 0; j < J; ++j) sum[j] = warp_sum(sum[j]);
+      if ((lane & 15) == 0 && js < k) dweights[t * k + js] = there ? of_slices + (lane ? sum[1] : sum[0]) : 0.f;
     }
   }
 }
@@ -425,12 +429,13 @@ int tmpi_expert_combine_gradient(const void* dy, const void* rows, const float* 
   }), "expert_combine_gradient");
 }
 
-// dweights [tokens, k] = the sums over dots [slices, tokens * k] of the entries' places + dy [tokens, cols] . bias [nexperts, cols] (bf16, or null) of
+// dweights [tokens, k] = the sums over dots [ceil(slices / 4), tokens * k, 4] of the entries' places + dy [tokens, cols] . bias [nexperts, cols] (bf16, or null) of
 // the chosen expert
 int tmpi_expert_weight_gradient(const float* dots, const void* dy, const void* bias, const int* place, const int* chosen, float* dweights, int tokens, int k,
                                 int slices, int cols, int nexperts, void* stream) {
   const int st = experts::checked(tokens, k, cols, TMPI_BF16, "expert_weight_gradient");
   if (st || !tokens) return st;
+  if ((uintptr_t)dots & 15) return fail(TMPI_ERR_INVALID, "expert_weight_gradient: dots must be 16-byte aligned");
   const auto kernel = cols % 8 == 0 && all_aligned16({dy, bias}) ? experts::weight_gradient_kernel<8> : experts::weight_gradient_kernel<1>;
   return experts::finish(launch_overlapped(kernel, experts::grid_rows(tokens, 8), experts::THREADS, 0, (cudaStream_t)stream, dots, (const __nv_bfloat16*)dy,
                                            (const __nv_bfloat16*)bias, place, chosen, dweights, tokens * k, tokens, k, slices, cols, nexperts), "expert_weight_gradient");

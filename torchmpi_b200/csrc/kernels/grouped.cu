@@ -53,7 +53,7 @@ struct Problem {
   uint8_t* scale;            // and their scales
   __nv_bfloat16* h;          // GRADIENT: weight times gelu(z)
   const float* row_weights;  // GRADIENT: [rows] or null (ones)
-  float* dots;               // GRADIENT: [columns' groups, rows], the sum over 64 (few rows: 32) columns of gradient times gelu(z); or null
+  float* dots;               // GRADIENT: sums over 64 (few rows: 32) columns of gradient times gelu(z), where dots_at says; or null
   int wide;                  // every row of y, z, h starts on a 32-byte boundary
   int q_rows16;              // 8 bits: every row of z starts on a 16-byte boundary, as TMA tiles and 16-byte loads need
   int scale_pairs;           // 8 bits: two scales of a row that belong to 64 columns lie in one aligned 16-bit word
@@ -93,6 +93,10 @@ struct Unit {
   int row0, end;             // of the pair's tile: first row, end of the group
   __device__ __forceinline__ int part_rows(uint32_t rank) const { return min(max(end - row0 - (int)rank * BM, 0), BM); }
 };
+
+// Four slices of a row lie side by side, [slices / 4, rows, 4]: a warp, with a slice of 32 rows, writes to 16 sectors, and whoever adds a row's slices reads
+// 16 bytes of each.
+__device__ __forceinline__ long long dots_at(int slice, int rows, long long row) { return ((long long)(slice >> 2) * rows + row) * 4 + (slice & 3); }
 
 template <typename S>
 __device__ __forceinline__ void give_up(S* sh, int* status, int where) {
@@ -468,7 +472,7 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
           store_row(p.h + row_at * N + col, hw, left, wide);
           store_row(p.y + row_at * N + col, w, left, wide);
         }
-        if (mine && p.dots && (half || left <= 32)) p.dots[(long long)(col0 / SLICE) * p.rows + row_at] = dot;      // rows side by side
+        if (mine && p.dots && (half || left <= 32)) p.dots[dots_at(col0 / SLICE, p.rows, row_at)] = dot;
         continue;
       }
       pack_row(v, w);
@@ -663,7 +667,7 @@ __device__ __forceinline__ void few_finish(Sh* sh, const Problem& p, const int* 
             float dot = in ? v * y0 : 0.f;
 #pragma unroll
             for (int d = 16; d; d /= 2) dot += __shfl_xor_sync(~0u, dot, d);
-            if (lane == 0) p.dots[(long long)(col / 32) * p.rows + row] = dot;
+            if (lane == 0) p.dots[dots_at(col / 32, p.rows, row)] = dot;
           }
           if (in) {
             p.h[at] = __float2bfloat16_rn(weight * y0);
@@ -1288,7 +1292,7 @@ int tmpi_grouped_dots(int rows, int nexperts, int N, int kept8) {
 
 // The gradients of gelu(z) h's input and value in one product: with g = dy w_e (dy [rows, K], w [experts, K, N]) in fp32 and the kept z [rows, N] (bf16, or
 // with `scale` its 8-bit checkpoint), dz = weight g gelu'(z) and h = weight gelu(z), both bf16 [rows, N]; row_weights fp32 [rows] or null for
-// ones.  dots [tmpi_grouped_dots, rows] (or null): the sums of g gelu(z) over 32 or 64 columns each.  Rows behind the last group are left alone.
+// ones.  dots [ceil(tmpi_grouped_dots / 4), rows, 4] (or null): the sums of g gelu(z) over 32 or 64 columns each.  Rows behind the last group are left alone.
 int tmpi_grouped_gelu_gradient(const void* dy, const void* w, const int* offsets, const void* z, const void* scale, const float* row_weights, void* dz, void* h,
                                float* dots, int rows, int nexperts, int K, int N, void* stream) {
   if (!all_aligned16({z, dz, h}) || !z || !h) return fail(TMPI_ERR_INVALID, "grouped_gelu_gradient: tensors must be 16-byte aligned");
