@@ -1,0 +1,62 @@
+"""Derivatives of layers of experts and 8-bit checkpoints that are asked for in other ways than by one backward pass."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from torchmpi_b200.ops import act8, experts
+
+gpu = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+BF = torch.bfloat16
+
+
+def _calls(device):
+    """name -> (function of the tensors, the tensors)"""
+    g = torch.Generator().manual_seed(0)
+    new = lambda *s: torch.randn(s, generator=g).to(BF).to(device)
+    logits = torch.randn(6, 4, generator=g).to(device)
+    r = experts.route(logits, 2)
+    off = torch.tensor([0, 2, 2, 5, 6], dtype=torch.int32, device=device)
+    return {
+        "grouped_linear": (lambda x, w, b: experts.grouped_linear(x, w, b, off), (new(6, 16), new(4, 24, 16), new(4, 24))),
+        "grouped_linear with GELU": (lambda x, w, b: experts.grouped_linear(x, w, b, off, gelu=True), (new(6, 16), new(4, 24, 16), new(4, 24))),
+        "route": (lambda l: experts.route(l, 2).weights, (logits,)),
+        "route over all": (lambda l: experts.route(l, 2, renormalize=False).weights, (logits,)),
+        "dispatch": (lambda x: experts.dispatch(x, r), (new(6, 16),)),
+        "combine": (lambda rows, w: experts.combine(rows, r._replace(weights=w)), (new(12, 16), r.weights)),
+        "experts.mlp": (lambda x, w, *p: experts.mlp(x, r._replace(weights=w), *p), (new(6, 16), r.weights, new(4, 24, 16), new(4, 24), new(4, 16, 24), new(4, 16))),
+        "experts.mlp in 8 bits": (lambda x, w, *p: experts.mlp(x, r._replace(weights=w), *p, act8=True),
+                                  (new(6, 16), r.weights, new(4, 24, 16), new(4, 24), new(4, 16, 24), new(4, 16))),
+        "act8.mlp": (lambda *p: act8.mlp(*p), (new(6, 16), new(24, 16), new(24), new(16, 24), new(16))),
+    }
+
+
+NAMES = ("grouped_linear", "grouped_linear with GELU", "route", "route over all", "dispatch", "combine", "experts.mlp", "experts.mlp in 8 bits", "act8.mlp")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_a_forward_tangent_is_refused_or_carried_on(name, graph, device):
+    """An input with a forward-mode tangent, each in turn, with and without the grad mode: PyTorch's operations carry it on, the kernels' functions refuse it.  A
+    result without a tangent would stand for a derivative of zero."""
+    call, tensors = _calls(device)[name]
+    for i, t in enumerate(tensors):
+        with torch.set_grad_enabled(graph), fwd.dual_level():
+            given = list(tensors)
+            given[i] = fwd.make_dual(t, torch.ones_like(t))
+            try:
+                out = call(*given)
+            except RuntimeError as e:
+                assert "jvp" in str(e) and (device == "cuda" or "8" in name), e
+            else:
+                assert device == "cpu" and fwd.unpack_dual(out).tangent is not None, i
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", NAMES)
+def test_without_a_tangent_results_are_the_same_inside_a_dual_level(name, device):
+    call, tensors = _calls(device)[name]
+    want = call(*tensors)
+    with fwd.dual_level():
+        assert torch.equal(call(*tensors), want)

@@ -16,10 +16,12 @@ using OptTensor = c10::optional<Tensor>;
 Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 const int* ints(const Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
+// Whether a call goes by its autograd function: a gradient may be asked for, or an input has a forward-mode tangent (whatever the grad mode), which the
+// function refuses; a result without one would stand for a derivative of zero.
 bool wants_grad(std::initializer_list<Tensor> inputs) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool backward = at::GradMode::is_enabled();
   for (const Tensor& t : inputs)
-    if (t.defined() && t.requires_grad()) return true;
+    if (t.defined() && ((backward && t.requires_grad()) || t._fw_grad(/*level=*/0).defined())) return true;
   return false;
 }
 
