@@ -60,3 +60,33 @@ def test_without_a_tangent_results_are_the_same_inside_a_dual_level(name, device
     want = call(*tensors)
     with fwd.dual_level():
         assert torch.equal(call(*tensors), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("E,k", [(4, 2), (5, 5), (40, 3), (200, 8)])
+def test_the_gradient_of_a_token_with_a_nan(E, k, renormalize, device):
+    """NaN at the logits that enter the token's weights (those of the chosen experts, or all), and nothing of it elsewhere, whoever computes it."""
+    nan, inf = float("nan"), float("inf")
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn(9, E, generator=g)
+    logits[1, 1] = nan                                     # one NaN among others
+    logits[2] = nan                                        # nothing else
+    logits[3], logits[3, 0], logits[3, 1] = -inf, 1.0, nan # fewer than k to choose, and a NaN
+    logits[4], logits[4, 2] = -inf, nan                    # nothing to choose, and a NaN
+    logits[5] = -inf                                       # padding
+    logits[6, 3], logits[6, 0] = nan, -inf
+    dw = torch.randn(9, k, generator=g)
+    bad = torch.tensor([False, True, True, True, True, False, True, False, False])
+    leaf = logits.to(device).requires_grad_(True)
+    r = experts.route(leaf, k, renormalize)
+    (got,) = torch.autograd.grad(r.weights, leaf, dw.to(device))
+    got, weights, chosen = got.cpu(), r.weights.detach().cpu(), r.chosen.cpu().long()
+    assert torch.equal(torch.isnan(weights), bad.unsqueeze(1).expand(9, k))
+    mine = torch.zeros(9, E + 1, dtype=torch.bool).scatter_(1, torch.where(chosen >= 0, chosen, E), True)[:, :E]
+    entered = mine if renormalize else torch.ones(9, E, dtype=torch.bool)
+    assert torch.equal(torch.isnan(got), bad.unsqueeze(1) & entered)
+    assert not got[bad][~torch.isnan(got[bad])].any() and not got[5].any()
+    ordinary = logits[~bad].to(device).requires_grad_(True)          # the others are what they are without it
+    (want,) = torch.autograd.grad(experts.route(ordinary, k, renormalize).weights, ordinary, dw[~bad].to(device))
+    assert torch.equal(got[~bad], want.cpu())

@@ -54,14 +54,19 @@ def _route(logits: torch.Tensor, k: int, renormalize: bool) -> Routing:
     l = logits.float()
     T, E = l.shape
     nan = torch.isnan(l)
-    key, index = torch.sort(torch.where(nan, -math.inf, l), dim=1, descending=True, stable=True)
+    bad = nan.any(1, keepdim=True)
+    usable = torch.where(nan, -math.inf, l)
+    key, index = torch.sort(usable, dim=1, descending=True, stable=True)
     key, index = key[:, :k], index[:, :k]
     used = key > -math.inf
     top = torch.where(used[:, :1], key[:, :1], 0).detach()
-    scores = torch.where(used, torch.exp(torch.gather(l, 1, index) - top), 0)
-    total = scores.sum(1, keepdim=True) if renormalize else torch.exp(l - top).sum(1, keepdim=True)
+    scores = torch.where(used, torch.exp(torch.gather(usable, 1, index) - top), 0)
+    total = scores.sum(1, keepdim=True) if renormalize else torch.exp(usable - top).sum(1, keepdim=True)
     weights = torch.where(used, scores / torch.where(used[:, :1], total, 1), 0)
-    weights = torch.where(nan.any(1, keepdim=True), math.nan, weights)
+    # a token with a NaN: its weights are NaN, and so are the gradients of the logits that enter them, the chosen ones or all
+    one, zero = torch.ones_like(l[:, :1]), torch.zeros_like(l[:, :1])
+    poison = torch.where(bad, math.nan, one) if renormalize else torch.where(bad, (l * torch.where(bad, math.nan, zero)).sum(1, keepdim=True), one)
+    weights = weights * poison
     expert, order = torch.sort(torch.where(used, index, E).reshape(-1), stable=True)
     slot = torch.arange(T * k, device=l.device)
     place = torch.empty_like(slot)
@@ -144,7 +149,8 @@ class _Mlp8(torch.autograd.Function):
 def route(logits: torch.Tensor, k: int, renormalize: bool = True) -> Routing:
     """The ``k`` largest of each token's ``logits [T, E]``, largest first, of equal ones that with the lowest index.  The weights are the softmax over
     the chosen logits, or (``renormalize=False``) over all of the token's.  An expert whose logit is -inf is never used, so a
-    token may get fewer than ``k``, and one without any gets none (a padded position).  NaN is not chosen either, and makes the token's weights NaN."""
+    token may get fewer than ``k``, and one without any gets none (a padded position).  NaN is not chosen either, and makes the token's weights NaN,
+    and in backward the gradients of the logits that the weights are formed from."""
     if logits.is_cuda:
         r = _native.ext().expert_route(logits, k, renormalize)          # None: nothing for the kernel
         if r is not None:
