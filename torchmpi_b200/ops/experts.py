@@ -50,8 +50,13 @@ def check_status() -> None:
 
 
 # ---------------------------------------------------------------- PyTorch forms
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    """32 bits, or 64 where the tensor has them."""
+    return t.to(torch.promote_types(t.dtype, torch.float32))
+
+
 def _route(logits: torch.Tensor, k: int, renormalize: bool) -> Routing:
-    l = logits.float()
+    l = _wide(logits)
     T, E = l.shape
     nan = torch.isnan(l)
     bad = nan.any(1, keepdim=True)
@@ -66,7 +71,7 @@ def _route(logits: torch.Tensor, k: int, renormalize: bool) -> Routing:
     # a token with a NaN: its weights are NaN, and so are the gradients of the logits that enter them, the chosen ones or all
     one, zero = torch.ones_like(l[:, :1]), torch.zeros_like(l[:, :1])
     poison = torch.where(bad, math.nan, one) if renormalize else torch.where(bad, (l * torch.where(bad, math.nan, zero)).sum(1, keepdim=True), one)
-    weights = weights * poison
+    weights = (weights * poison).float()
     expert, order = torch.sort(torch.where(used, index, E).reshape(-1), stable=True)
     slot = torch.arange(T * k, device=l.device)
     place = torch.empty_like(slot)
@@ -83,7 +88,7 @@ def _combine(rows, weights, place):
 
 def _dispatch(x, order, k):
     token = torch.div(order.long(), k, rounding_mode="floor")
-    wide = x.to(torch.promote_types(x.dtype, torch.float32))          # so that the gradients of a token's rows are added in fp32
+    wide = _wide(x)          # so that the gradients of a token's rows are added in fp32
     return torch.where((token >= 0).unsqueeze(1), wide[token.clamp_min(0)], 0).to(x.dtype)
 
 
