@@ -47,6 +47,11 @@ def same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
         raise ValueError(f"{what}: tensors on {d}, but the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    """32 bits, or 64 where the tensor has them."""
+    return t.to(torch.promote_types(t.dtype, torch.float32))
+
+
 def _two_to(e: torch.Tensor) -> torch.Tensor:
     return ((e.int() + 127) << 23).view(torch.float32)            # exact, unlike a power function
 
@@ -80,7 +85,7 @@ def _checked(what: str, a: Act8) -> None:
 
 
 def quantize(x: torch.Tensor) -> Act8:
-    """The checkpoint of ``x [..., C]``; not differentiable."""
+    """The checkpoint of ``x [..., C]`` (of 64 bits: of their values in 32); not differentiable."""
     if x.is_cuda:
         kept = _native.ext().act8_quantize(x)          # None: nothing for the kernel
         if kept is not None:
@@ -119,8 +124,9 @@ def gelu_gradient(dy: torch.Tensor, a: Act8) -> Tuple[torch.Tensor, torch.Tensor
     if dy.shape != a.q.shape or not dy.dtype.is_floating_point:
         raise ValueError(f"gelu_gradient: a gradient of {dy.dtype} {tuple(dy.shape)} for a checkpoint of {tuple(a.q.shape)}")
     same_device("gelu_gradient", dy, *a)
-    h, slope = _gelu_parts(_dequantize(a, torch.float32))
-    return (dy.detach().float() * slope).to(dy.dtype), h.to(dy.dtype)
+    g = _wide(dy.detach())
+    h, slope = _gelu_parts(_dequantize(a, g.dtype))
+    return (g * slope).to(dy.dtype), h.to(dy.dtype)
 
 
 def refuse_graph() -> None:
@@ -132,18 +138,19 @@ def refuse_graph() -> None:
 class _Mlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, b1, w2, b2):
-        z = F.linear(x.float(), w1.float(), None if b1 is None else b1.float())
+        z = F.linear(_wide(x), _wide(w1), None if b1 is None else _wide(b1))
         ctx.save_for_backward(*_quantize(x), *_quantize(z), w1, b1, w2, b2)
-        return F.linear(_gelu_parts(z)[0], w2.float(), None if b2 is None else b2.float()).to(x.dtype)
+        return F.linear(_gelu_parts(z)[0], _wide(w2), None if b2 is None else _wide(b2)).to(x.dtype)
 
     @staticmethod
     def backward(ctx, dy):
         refuse_graph()
         xq, xs, zq, zs, w1, b1, w2, b2 = ctx.saved_tensors
-        x, z, dy = _dequantize(Act8(xq, xs), torch.float32), _dequantize(Act8(zq, zs), torch.float32), dy.float()
+        dy = _wide(dy)
+        x, z = _dequantize(Act8(xq, xs), dy.dtype), _dequantize(Act8(zq, zs), dy.dtype)
         h, slope = _gelu_parts(z)
-        dz = dy @ w2.float() * slope
-        grads = (dz @ w1.float(), dz.t() @ x, None if b1 is None else dz.sum(0), dy.t() @ h, None if b2 is None else dy.sum(0))
+        dz = dy @ _wide(w2) * slope
+        grads = (dz @ _wide(w1), dz.t() @ x, None if b1 is None else dz.sum(0), dy.t() @ h, None if b2 is None else dy.sum(0))
         return tuple(g if g is None else g.to(t.dtype) for g, t in zip(grads, (w1, w1, b1, w2, b2)))
 
 

@@ -22,7 +22,7 @@ import torch.nn.functional as F
 from .. import _native
 from .._lib import lib, TorchMPIError
 from . import act8 as _act8
-from .act8 import same_device
+from .act8 import _wide, same_device
 
 
 class Routing(NamedTuple):
@@ -50,11 +50,6 @@ def check_status() -> None:
 
 
 # ---------------------------------------------------------------- PyTorch forms
-def _wide(t: torch.Tensor) -> torch.Tensor:
-    """32 bits, or 64 where the tensor has them."""
-    return t.to(torch.promote_types(t.dtype, torch.float32))
-
-
 def _route(logits: torch.Tensor, k: int, renormalize: bool) -> Routing:
     l = _wide(logits)
     T, E = l.shape
@@ -82,7 +77,7 @@ def _route(logits: torch.Tensor, k: int, renormalize: bool) -> Routing:
 
 def _combine(rows, weights, place):
     at = place.long()
-    picked = torch.where((at >= 0).unsqueeze(2), rows.float()[at.clamp_min(0)], 0)
+    picked = torch.where((at >= 0).unsqueeze(2), _wide(rows)[at.clamp_min(0)], 0)
     return (picked * weights.unsqueeze(2)).sum(1).to(rows.dtype)
 
 
@@ -102,7 +97,7 @@ def _groups(offsets, rows):
 def _grouped(x, w, bias, offsets, gelu):
     parts, at = [F.linear(x[:0], w[0], None if bias is None else bias[0])], 0      # no row, but gradients where there are no groups
     for e, a, b in _groups(offsets, x.shape[0]):
-        y = F.linear(x[a:b].float(), w[e].float(), None if bias is None else bias[e].float())
+        y = F.linear(_wide(x[a:b]), _wide(w[e]), None if bias is None else _wide(bias[e]))
         parts.append((F.gelu(y) if gelu else y).to(x.dtype))
         at = b
     if at < x.shape[0]:
@@ -115,11 +110,11 @@ class _Mlp8(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weights, w1, b1, w2, b2, order, place, offsets):
-        k, xs = place.shape[1], _dispatch(x.float(), order, place.shape[1])
+        k, xs = place.shape[1], _dispatch(_wide(x), order, place.shape[1])
         z, ys = xs.new_zeros(xs.shape[0], w1.shape[1]), torch.zeros_like(xs)
         for e, a, b in _groups(offsets, xs.shape[0]):
-            z[a:b] = F.linear(xs[a:b], w1[e].float(), None if b1 is None else b1[e].float())
-            ys[a:b] = F.linear(_act8._gelu_parts(z[a:b])[0], w2[e].float(), None if b2 is None else b2[e].float())
+            z[a:b] = F.linear(xs[a:b], _wide(w1[e]), None if b1 is None else _wide(b1[e]))
+            ys[a:b] = F.linear(_act8._gelu_parts(z[a:b])[0], _wide(w2[e]), None if b2 is None else _wide(b2[e]))
         ctx.save_for_backward(*_act8._quantize(x), *_act8._quantize(z), weights, w1, b1, w2, b2, order, place, offsets)
         return _combine(ys, weights, place).to(x.dtype)
 
@@ -128,19 +123,20 @@ class _Mlp8(torch.autograd.Function):
         _act8.refuse_graph()
         xq, xs, zq, zs, weights, w1, b1, w2, b2, order, place, offsets = ctx.saved_tensors
         k, n = place.shape[1], order.shape[0]
-        x, z = _act8._dequantize(_act8.Act8(xq, xs), torch.float32), _act8._dequantize(_act8.Act8(zq, zs), torch.float32)
-        g, x = _dispatch(dy.float(), order, k), _dispatch(x, order, k)
+        g = _dispatch(_wide(dy), order, k)
+        x, z = _act8._dequantize(_act8.Act8(xq, xs), g.dtype), _act8._dequantize(_act8.Act8(zq, zs), g.dtype)
+        x = _dispatch(x, order, k)
         wt = weights.reshape(-1)[order.long().clamp_min(0)].unsqueeze(1)
         h, slope = _act8._gelu_parts(z)
         dxs, dwe = torch.zeros_like(g), g.new_zeros(n)
-        dw1, db1, dw2, db2 = (None if t is None else torch.zeros_like(t, dtype=torch.float32) for t in (w1, b1, w2, b2))
+        dw1, db1, dw2, db2 = (None if t is None else torch.zeros_like(t, dtype=g.dtype) for t in (w1, b1, w2, b2))
         for e, a, b in _groups(offsets, n):
-            dh = g[a:b] @ w2[e].float()
+            dh = g[a:b] @ _wide(w2[e])
             dwe[a:b] = (dh * h[a:b]).sum(1)
             dz, gw = wt[a:b] * dh * slope[a:b], wt[a:b] * g[a:b]
-            dw2[e], dw1[e], dxs[a:b] = gw.t() @ h[a:b], dz.t() @ x[a:b], dz @ w1[e].float()
+            dw2[e], dw1[e], dxs[a:b] = gw.t() @ h[a:b], dz.t() @ x[a:b], dz @ _wide(w1[e])
             if b2 is not None:
-                dwe[a:b] += (g[a:b] * b2[e].float()).sum(1)
+                dwe[a:b] += (g[a:b] * _wide(b2[e])).sum(1)
                 db2[e] = gw.sum(0)
             if b1 is not None:
                 db1[e] = dz.sum(0)
@@ -189,7 +185,7 @@ def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
 
 
 def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
-    """``rows [T * k, C]`` -> ``[T, C]``: each token's rows times their weights, added in fp32 and rounded once."""
+    """``rows [T * k, C]`` -> ``[T, C]``: each token's rows times their weights, added in fp32 (of 64 bits: in those) and rounded once."""
     if rows.is_cuda:
         y = _native.ext().expert_combine(rows, routing.weights, routing.place, routing.offsets)
         if y is not None:
