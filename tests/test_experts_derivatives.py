@@ -90,3 +90,33 @@ def test_the_gradient_of_a_token_with_a_nan(E, k, renormalize, device):
     ordinary = logits[~bad].to(device).requires_grad_(True)          # the others are what they are without it
     (want,) = torch.autograd.grad(experts.route(ordinary, k, renormalize).weights, ordinary, dw[~bad].to(device))
     assert torch.equal(got[~bad], want.cpu())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (5, 33), (4, 64), (2, 3, 40)], ids=str)
+def test_the_gelu_gradient_is_linear_in_its_gradient(shape, dtype, device):
+    """dz = dy gelu'(z): its derivative takes a gradient g to g gelu'(z), which is the function's own result for g; gelu(z) does not depend on dy."""
+    g = torch.Generator().manual_seed(2)
+    z, dy, gz = (torch.randn(shape, generator=g).to(dtype).to(device) for _ in range(3))
+    a = act8.quantize(z)
+    leaf = dy.clone().requires_grad_(True)
+    dz, h = act8.gelu_gradient(leaf, a)
+    want = act8.gelu_gradient(dy, a)
+    assert dz.requires_grad and not h.requires_grad and torch.equal(dz, want[0]) and torch.equal(h, want[1])
+    (got,) = torch.autograd.grad(dz, leaf, gz)
+    assert got.dtype == dtype and torch.equal(got, act8.gelu_gradient(gz, a)[0])
+    with torch.no_grad():
+        assert not act8.gelu_gradient(leaf, a)[0].requires_grad
+    for graph in (False, True):
+        with torch.set_grad_enabled(graph), fwd.dual_level():
+            dual = fwd.make_dual(dy, gz)
+            if device == "cuda":
+                with pytest.raises(RuntimeError, match="jvp"):
+                    act8.gelu_gradient(dual, a)
+            else:
+                dz, h = act8.gelu_gradient(dual, a)
+                assert torch.equal(fwd.unpack_dual(dz).tangent, act8.gelu_gradient(gz, a)[0]) and fwd.unpack_dual(h).tangent is None
+    if device == "cuda":
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(act8.gelu_gradient(leaf, a)[0], leaf, gz, create_graph=True)

@@ -67,14 +67,33 @@ Tensor restore(const Kept& k, at::ScalarType type) {
   launched(ACT8, 1);
   return x;
 }
-std::pair<Tensor, Tensor> gelu_gradient(const Tensor& dy, const Kept& k) {
-  Tensor dz = at::empty_like(dy), h = at::empty_like(dy);
+// (dz, h) of tmpi_act8_gelu_gradient; h only where it is asked for
+std::pair<Tensor, Tensor> gelu_gradient(const Tensor& dy, const Kept& k, bool with_h = true) {
+  Tensor dz = at::empty_like(dy), h;
+  if (with_h) h = at::empty_like(dy);
   const int64_t cols = dy.size(-1);
-  check(tmpi_act8_gelu_gradient(dy.data_ptr(), k.q.data_ptr(), k.scale.data_ptr(), dz.data_ptr(), h.data_ptr(), dy.numel() / cols, (int)cols,
+  check(tmpi_act8_gelu_gradient(dy.data_ptr(), k.q.data_ptr(), k.scale.data_ptr(), dz.data_ptr(), with_h ? h.data_ptr() : nullptr, dy.numel() / cols, (int)cols,
                                 dtype_code(dy.scalar_type()), stream()));
   launched(ACT8, 1);
   return {dz, h};
 }
+// dz is linear in dy, with the slope at what the checkpoint stands for; h and the slope do not depend on it.
+struct GeluGradientFn : public torch::autograd::Function<GeluGradientFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& dy, const Tensor& q, const Tensor& scale) {
+    const Kept k{packed(q), packed(scale)};
+    const auto both = gelu_gradient(packed(dy), k);
+    ctx->save_for_backward({k.q, k.scale});
+    ctx->mark_non_differentiable({both.second});
+    ctx->set_materialize_grads(false);
+    return {both.first, both.second};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_graph();
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    return {gelu_gradient(packed(grads[0]), {as_saved(saved[0]), as_saved(saved[1])}, false).first, Tensor(), Tensor()};
+  }
+};
 bool is_kept(const Tensor& q, const Tensor& scale) {
   if (!(q.scalar_type() == at::kFloat8_e4m3fn && scale.scalar_type() == at::kByte && q.dim() >= 1 && scale.dim() == q.dim() && q.numel() > 0 && q.size(-1) <= MOST)) return false;
   for (int64_t i = 0; i + 1 < q.dim(); ++i)
@@ -373,7 +392,9 @@ void register_experts(pybind11::module_& m) {
   });
   m.def("act8_gelu_gradient", [](const Tensor& dy, const Tensor& q, const Tensor& scale) -> OptPair {
     if (!(dy.is_cuda() && floating(dy) && dy.sizes() == q.sizes() && is_kept(q, scale) && here({&dy}))) return c10::nullopt;
-    return gelu_gradient(packed(dy.detach()), {packed(q), packed(scale)});
+    if (!wants_grad({dy})) return gelu_gradient(packed(dy), {packed(q), packed(scale)});
+    const variable_list both = GeluGradientFn::apply(dy, q, scale);
+    return std::make_pair(both[0], both[1]);
   });
   m.def("act8_mlp", [](const Tensor& x, const Tensor& w1, const OptTensor& b1_, const Tensor& w2, const OptTensor& b2_) -> OptTensor {
     const Tensor b1 = or_none(b1_), b2 = or_none(b2_);

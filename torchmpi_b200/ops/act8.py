@@ -115,7 +115,7 @@ def _gelu_parts(z: torch.Tensor):
 
 
 def gelu_gradient(dy: torch.Tensor, a: Act8) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``(dy * gelu'(z), gelu(z))`` (erf form) for the values ``z`` of the checkpoint ``a``, both of ``dy``'s dtype."""
+    """``(dy * gelu'(z), gelu(z))`` (erf form) for the values ``z`` of the checkpoint ``a``, both of ``dy``'s dtype; the first is differentiable in ``dy``."""
     if dy.is_cuda:
         both = _native.ext().act8_gelu_gradient(dy, a[0], a[1])
         if both is not None:
@@ -124,7 +124,7 @@ def gelu_gradient(dy: torch.Tensor, a: Act8) -> Tuple[torch.Tensor, torch.Tensor
     if dy.shape != a.q.shape or not dy.dtype.is_floating_point:
         raise ValueError(f"gelu_gradient: a gradient of {dy.dtype} {tuple(dy.shape)} for a checkpoint of {tuple(a.q.shape)}")
     same_device("gelu_gradient", dy, *a)
-    g = _wide(dy.detach())
+    g = _wide(dy)
     h, slope = _gelu_parts(_dequantize(a, g.dtype))
     return (g * slope).to(dy.dtype), h.to(dy.dtype)
 
