@@ -221,14 +221,10 @@ __device__ __forceinline__ void issue(Sh* sh, unsigned char* tiles, const Proble
   });
 }
 
-// n 32-bit words to or from consecutive addresses: 32 bytes at once where rows start on such a boundary (a whole sector of L2 per lane), else 16 or 8.
+// 32-bit words to consecutive addresses: 32 bytes at once where rows start on such a boundary (a whole sector of L2 per lane), else 16 or 8.
 __device__ __forceinline__ void store32(void* to, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-}
-__device__ __forceinline__ void load32(const void* from, uint32_t* w) {
-  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(from));
 }
 // 32 bf16 columns of a row, `left` of them inside it (a multiple of 8)
 __device__ __forceinline__ void store_row(__nv_bfloat16* to, const uint32_t (&w)[16], int left, bool wide) {
@@ -251,15 +247,12 @@ __device__ __forceinline__ void store_row8(uint8_t* to, const uint32_t (&q)[8], 
       if (8 * j < left) reinterpret_cast<uint2*>(to)[j] = make_uint2(q[2 * j], q[2 * j + 1]);
   }
 }
-__device__ __forceinline__ void load_row8(const uint8_t* from, uint32_t (&q)[8], int left, bool wide) {
-  if (wide && left >= 32) {
-    load32(from, q);
-  } else {
+// the same read, where rows start on 8-byte boundaries alone (others come through the TMA unit)
+__device__ __forceinline__ void load_row8(const uint8_t* from, uint32_t (&q)[8], int left) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint2 v = 8 * j < left ? reinterpret_cast<const uint2*>(from)[j] : make_uint2(0u, 0u);
-      q[2 * j] = v.x; q[2 * j + 1] = v.y;
-    }
+  for (int j = 0; j < 4; ++j) {
+    const uint2 v = 8 * j < left ? reinterpret_cast<const uint2*>(from)[j] : make_uint2(0u, 0u);
+    q[2 * j] = v.x; q[2 * j + 1] = v.y;
   }
 }
 __device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]) {
@@ -329,7 +322,7 @@ __device__ __forceinline__ void finish(Sh* sh, unsigned char* staging, const Pro
           else scales = at[0] | (col0 + 32 < N ? (uint32_t)at[1] << 8 : 0x0100u);
           if (!by_tma) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) load_row8((const uint8_t*)p.z + row_at * N + col0 + 32 * h, *reinterpret_cast<uint32_t(*)[8]>(&kept[8 * h]), N - col0 - 32 * h, wide);
+            for (int h = 0; h < 2; ++h) load_row8((const uint8_t*)p.z + row_at * N + col0 + 32 * h, *reinterpret_cast<uint32_t(*)[8]>(&kept[8 * h]), N - col0 - 32 * h);
           }
         }
       }
