@@ -1,10 +1,12 @@
 // 8-bit activation checkpoints (act8.cuh has the format): quantize, restore, and the GELU backward that reads one.
 //
-// All are bound by memory: every element is read and written once.  Four threads hold the 32 elements of a block, eight each, so a block's
+// Every element is read and written once.  Four threads hold the 32 elements of a block, eight each, so a block's
 // largest magnitude takes two shuffles, loads are 16 bytes and more per thread and a warp's loads are consecutive.  Rows whose length
 // is no multiple of 8 elements, or that do not start on a 16-byte boundary, take the same kernels with single elements (VEC = false).
-// Measured, bf16, us and share of the copy rate: 65536 x 4096 quantize 145 (0.86), restore 137 (0.91), GELU backward 317 (0.91) after a flush of the L2;
+// With whole pieces they are bound by memory.  Measured, bf16, us and share of the copy rate: 65536 x 4096 quantize 145 (0.86), restore 137 (0.91), GELU backward 317 (0.91) after a flush of the L2;
 // 32768 x 1024 back to back 19.5 and 15.9, in one wave of blocks that loop (two waves: 21.4 and 17.3; 65536 x 4096 is the same either way).
+// Single elements are bound by their loads and stores, a byte or two of each: 32768 x 1001, after a flush, quantize 51, restore 98, GELU backward 169, where 1000
+// columns take 38, 24 and 57.
 #include "act8.cuh"
 #include "gelu.cuh"
 #include "pdl.cuh"

@@ -1,8 +1,9 @@
 // Rows on their way to the experts and back: dispatch (a token's row to each of its experts' places), combine (the weighted sum of
 // what the experts made of it) and their gradients.
 //
-// `place` (route.cu) gives the place of each entry token * k + j, `order` the entry at each place.  All passes go by tokens, read and write each
-// element once, and are bound by memory.  Passes without a sum over a row give a thread one 16-byte piece of a row, so that one token of a long row is
+// `place` (route.cu) gives the place of each entry token * k + j, `order` the entry at each place.  All passes go by tokens and read and write each
+// element once.  Back to back, out of memory, bf16, 8192 x 1024: dispatch to two experts 8.5 us, 0.91 of the copy rate, to eight 26.4, 0.87; combine 12.0, 0.64, and 26.5, 0.87 (a
+// thread has one piece of a row, whose loads wait for those of its places: with two experts not enough is under way).  Passes without a sum over a row give a thread one 16-byte piece of a row, so that one token of a long row is
 // spread over many blocks; those with one give a warp a row.  Sums are in fp32, in one order whatever the launch: nothing is accumulated
 // by atomics.  Places behind the last entry (from *used on) get zeros where the caller asks for it.
 #include "act8.cuh"

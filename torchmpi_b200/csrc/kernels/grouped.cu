@@ -552,8 +552,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 // ---------------------------------------------------------------- few rows to an expert
 // The product the other way round, y^T = w_e x^T, on one CTA per tile: 128 rows of the weight are the M of the MMAs, up to 128 rows of x
 // (as many as there are, in steps of 16) their N.  A tile of the kernel above multiplies 256 rows of x whether there are two or 200: with 2
-// rows to each of 8 experts, 1024 -> 4096, MMAs were under way for 10 of its 20 us, where the weights need 10.  What bounds this one is the
-// weights' way from memory: 96 KB of them are under way per SM.
+// rows to each of 8 experts, 1024 -> 4096, MMAs were under way for 10 of its 20 us, where the weights need 10.  96 KB of the weights are under way
+// per SM.  What bounds this one is the launch with one tile's chain, and then whole rounds of tiles, more than the weights' way from memory: 16 rows, 1024 -> 4096 with a GELU, weights out
+// of memory (out of the L2), one expert with rows 7.6 us (6.7), four, 128 tiles, 9.3 (7.6), five, 160 tiles and so a second round, 12.8 (10.3), eight 14.3 (12.0); the bytes
+// take 1.3, 5.1, 6.4 and 10.3.
 // A thread has a column of y and walks the rows, so a warp's stores are 64 bytes of a row each, the 32 columns of an 8-bit block are its lanes', and a row
 // behind the group's end is not touched.
 constexpr int FEW_BM = 128, FEW_BN = 128, FEW_STAGES = 6, FEW_EPI_WARPS = 16, FEW_THREADS = 64 + FEW_EPI_WARPS * 32;
@@ -1184,6 +1186,8 @@ static int checked(const int* offsets, int rows, int nexperts, int K, int N, con
 // with a checkpoint, 64 14.6 and 22.9, 160 33.3 and 23.2; the GELU's gradient, 2 13.3 and 21.5, 64 20.6 and 27.3, 96 31.1 and 25.1; 4096 -> 1024
 // in fp32, 2 15.2 and 18.7, 128 18.2 and 23.8.  64 ragged groups of 0 to 200 rows, 80 on average, 520 -> 1000: 25.0 and 24.9, with a checkpoint 36.8 and
 // 33.5; of half as many, 16.9 and 21.4, with a checkpoint 21.9 and 28.9, the gradient 36.0 and 34.7.
+// The host knows the mean alone.  Where few experts have all rows this form is the slower one: 5000 rows of 64 experts, all of one, with a GELU, 520 -> 1000 18.8 and
+// 13.5, 1024 -> 4096 44.5 and 33.6; 2048 rows, 2048 <- 512, the GELU's gradient 25 and 15.
 static int few_mean(int mode) { return mode == GRADIENT8 || mode == GRADIENT16 ? 32 : mode == KEEP8 ? 64 : 96; }
 // Parts of K of a product with few rows and an fp32 result, whose reader adds them: as many as leave eight blocks of K each and about a tile for every SM,
 // if half of the experts have rows.  4 tokens with two of 8 experts each, 4096 -> 1024: 14.6 us whole, 9.9 in three parts.
