@@ -63,8 +63,8 @@ __device__ __forceinline__ void gelu_both2(float z0, float z1, float* y0, float*
 // of z, as z times a polynomial of degree 6 in z^2 (least squares made equal-ripple on |z| <= 5; beyond it grows like z^13, so that Phi goes to 0 or
 // 1).  No absolute value, no choice between two tails, one exponential: 10 packed operations and 4 of the special-function unit for two elements,
 // where the rational form above takes 12, 6 and 4.  Absolute errors in fp32: Phi and slope 1.4e-6, gelu 1.1e-6.
-// A result in bf16 shows them below z = -5 alone, where gelu is under 2e-6 in magnitude, and at the slope's root, -0.75; one in fp16 by up to 2.3 half steps (gelu at -3.6), and
-// slopes next to the root more.
+// That is at most a third of a half step of bf16 for gelu down to z = -5 (below it, where gelu is under 2e-6 in magnitude, more), and up to 2.3 half steps of fp16 (at
+// -3.6); of the slope, more next to its root at -0.75 alone.
 __device__ __forceinline__ unsigned long long quick_cdf2(unsigned long long z, unsigned long long t) {      // t = z^2
   using namespace attn_util;
   auto both = [](float v) { return attn_util::pack2(__float_as_uint(v), __float_as_uint(v)); };
