@@ -217,6 +217,15 @@ _CUDA_PROTOS = {
     "tmpi_act8_quantize": (_i, [_vp, _vp, _vp, _i64, _i, _i, _vp]),
     "tmpi_act8_restore": (_i, [_vp, _vp, _vp, _i64, _i, _i, _vp]),
     "tmpi_act8_gelu_gradient": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _vp]),
+    "tmpi_fp8_pitch": (_i64, [_i64]),
+    "tmpi_fp8_scale_bytes": (_sz, [_i64, _i64]),
+    "tmpi_fp8_quantize": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _vp]),
+    "tmpi_fp8_column_sums": (_i, [_vp, _i, _i, _vp, _i, _vp]),
+    "tmpi_fp8_restore": (_i, [_vp, _vp, _vp, _i64, _i64, _i, _vp]),
+    "tmpi_fp8_few_tokens": (_i, []),
+    "tmpi_fp8_few": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "tmpi_fp8_product_workspace_bytes": (_sz, [_i, _i, _i]),
+    "tmpi_fp8_product": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "tmpi_route_limits": (_i, [_ip, _ip]),
     "tmpi_route_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmpi_route": (_i, [_vp, _i64, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

@@ -10,7 +10,7 @@ import importlib.util
 
 from . import _lib, build  # noqa: F401  (_lib loads the native library first)
 
-LINEAR, LAYERNORM, ATTENTION, XENT, ATTENTION_BACKWARD, BATCHNORM, CONV, STEM, ACT8, EXPERTS = range(10)      # counters of ``launches``; attention counts calls
+LINEAR, LAYERNORM, ATTENTION, XENT, ATTENTION_BACKWARD, BATCHNORM, CONV, STEM, ACT8, EXPERTS, FP8, ADAMW = range(12)      # counters of ``launches``; attention counts calls
 _ext = None
 
 

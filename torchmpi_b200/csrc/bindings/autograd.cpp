@@ -389,7 +389,6 @@ Tensor channels_last(const Tensor& t) { return packed(t, at::MemoryFormat::Chann
 Tensor empty_channels_last(at::IntArrayRef sizes, const Tensor& like) {
   return at::empty(sizes, like.options(), at::MemoryFormat::ChannelsLast);
 }
-const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 
 // the gradient where its mask bit is set
@@ -593,5 +592,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cross_entropy_scratch", xent_scratch);
   m.def("arrival_counters", arrival_counters);
   register_experts(m);
+  register_fp8(m);
   m.def("launches", [](int what) { return g_launches[what].load(std::memory_order_relaxed); });
 }

@@ -3,7 +3,6 @@
 // that the kernels take is looked at once, here (in Python the checks of a layer of experts took 17 us of a call of 39).  Scratch
 // memory comes from PyTorch's allocator on the calling stream, per call.
 #include "common.h"
-#include <c10/cuda/CUDAFunctions.h>
 #include <algorithm>
 #include <initializer_list>
 
@@ -12,39 +11,8 @@ namespace {
 
 enum { PLAIN = 0, GELU = 1, GELU_AND_Z = 2, GELU_AND_Z8 = 3, FP32 = 4 };      // tmpi_grouped_gemm's modes
 
-using OptTensor = c10::optional<Tensor>;
-Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-const int* ints(const Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
-// Whether a call goes by its autograd function: a gradient may be asked for, or an input has a forward-mode tangent (whatever the grad mode), which the
-// function refuses; a result without one would stand for a derivative of zero.
-bool wants_grad(std::initializer_list<Tensor> inputs) {
-  const bool backward = at::GradMode::is_enabled();
-  for (const Tensor& t : inputs)
-    if (t.defined() && ((backward && t.requires_grad()) || t._fw_grad(/*level=*/0).defined())) return true;
-  return false;
-}
-
 // The kernels' gradients are constants to autograd: one asked for with a graph (create_graph) would lose its part of what it enters in silence.
 void refuse_graph() { TORCH_CHECK(!at::GradMode::is_enabled(), "layers of experts and 8-bit checkpoints can be differentiated once (no create_graph)"); }
-
-// all on the current device, which there is one of per process
-bool here(std::initializer_list<const Tensor*> tensors) {
-  const int64_t device = c10::cuda::current_device();
-  for (const Tensor* t : tensors)
-    if (t->defined() && !(t->is_cuda() && t->get_device() == device)) return false;
-  return true;
-}
-bool all_of_type(std::initializer_list<const Tensor*> tensors, at::ScalarType type) {
-  for (const Tensor* t : tensors)
-    if (t->defined() && t->scalar_type() != type) return false;
-  return true;
-}
-bool floating(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat; }
-bool shaped(const Tensor& t, std::initializer_list<int64_t> sizes) { return !t.defined() || t.sizes() == at::IntArrayRef(sizes); }
-// [..., cols] as rows
-Tensor rows_of(const Tensor& x) { return x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}); }
-constexpr int64_t MOST = int64_t(1) << 30;                          // rows, columns and entries that the kernels count in 32 bits
 
 struct Kept { Tensor q, scale; };                                   // an 8-bit checkpoint, [..., cols] and [..., ceil(cols / 32)]
 

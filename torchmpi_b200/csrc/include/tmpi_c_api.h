@@ -381,6 +381,24 @@ int tmpi_act8_restore(const void* q, const void* scale, void* x, int64_t rows, i
 // dz = dy gelu'(z~) and, where h is given, h = gelu(z~) for the checkpoint z~ of z
 int tmpi_act8_gelu_gradient(const void* dy, const void* q, const void* scale, void* dz, void* h, int64_t rows, int cols, int dtype, void* stream);
 
+// ---------------------------------------------------------------- 8 bits with a scale for each block of 128 (fp8.cu, gemm_fp8.cu)
+// A matrix of `cols` columns in rows of tmpi_fp8_pitch(cols) e4m3 numbers (zeros behind the last column) and tmpi_fp8_scale_bytes bytes of scales, e + 127 for 2^e:
+// row r, block b at ((r / 128) * ceil(blocks / 4) + b / 4) * 512 + (r % 32) * 16 + r % 128 / 32 * 4 + b % 4.  All pointers on 16-byte boundaries but x.
+int64_t tmpi_fp8_pitch(int64_t cols);
+size_t tmpi_fp8_scale_bytes(int64_t rows, int64_t cols);
+// q, scale: along the rows; qt, scalet: of the transpose; either may be null.  z: x is the gradient behind a GELU of z (dense), and x gelu'(z), rounded to the type, is
+// what is kept; sums [ceil(rows / 128), cols]: the columns' sums of that over 128 rows each.  Both need qt.
+int tmpi_fp8_quantize(const void* x, int64_t ld, const void* z, void* q, void* scale, void* qt, void* scalet, float* sums, int64_t rows, int64_t cols, int dtype, void* stream);
+int tmpi_fp8_column_sums(const float* sums, int tiles, int cols, void* db, int dtype, void* stream);
+int tmpi_fp8_restore(const void* q, const void* scale, void* x, int64_t rows, int64_t cols, int dtype, void* stream);
+// y [tokens, N] = x w^T (+ bias), then the GELU of what is rounded: few tokens that the kernel quantizes itself, weights in 8 bits
+int tmpi_fp8_few_tokens(void);
+int tmpi_fp8_few(const void* x, int64_t ld, const void* q, const void* scale, const void* bias, void* y, int tokens, int N, int K, int gelu, int dtype, void* stream);
+// c [M, N] = a b^T (+ bias), both in 8 bits, K columns; gelu: the GELU of the rounded sums, which go to z where it is given
+size_t tmpi_fp8_product_workspace_bytes(int M, int N, int K);
+int tmpi_fp8_product(const void* qa, const void* sa, const void* qb, const void* sb, const void* bias, void* c, void* z, int M, int N, int K, int gelu, int dtype,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 // ---------------------------------------------------------------- layers of experts (route.cu, experts.cu, grouped.cu)
 // The k largest logits of each token (ties: the lowest index; -inf and NaN never), their weights, and all entries token * k + j in the order of the
 // experts: entry order[s] is at place s, place[entry] = s (-1: not used), the places of expert e from offsets[e] to offsets[e + 1].

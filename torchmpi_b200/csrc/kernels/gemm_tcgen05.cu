@@ -144,6 +144,23 @@ int make_tmap_box(CUtensorMap* map, int bytes, const void* base, uint64_t rows, 
   return TMPI_OK;
 }
 
+// Rows of 512 bytes, one row to a box, as they lie.
+int make_tmap_words(CUtensorMap* map, const void* base, uint64_t rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(TMPI_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+  if ((uintptr_t)base & 15) return fail(TMPI_ERR_INVALID, "TMA operand must be 16-byte aligned");
+  cuuint64_t dims[2] = {128, rows};
+  cuuint64_t strides[1] = {512};
+  cuuint32_t box[2] = {128, 1};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode_in_context([&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+  if (r != CUDA_SUCCESS) return fail(TMPI_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+  return TMPI_OK;
+}
+
 // Dense [outer, rows, cols] bf16 tensor, boxes of box_cols (64, or 32) columns x box_rows rows of one outer index, with the swizzle of their
 // width: what lies outside the extents of that index's matrix reads as zero and is not written.
 int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols) {
