@@ -226,6 +226,12 @@ _CUDA_PROTOS = {
     "tmpi_fp8_few": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "tmpi_fp8_product_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmpi_fp8_product": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "tmpi_adamw_max_groups": (_i, []),
+    "tmpi_adamw_step": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _vp]),
+    "tmpi_adamw_values": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp]),
+    "tmpi_norm_sums": (_i, [_i]),
+    "tmpi_norm_squares": (_i, [_vp, _i, _i, _vp, _ip, _vp]),
+    "tmpi_norm_finish": (_i, [_vp, _i, _f, _f, _vp, _vp, _vp]),
     "tmpi_route_limits": (_i, [_ip, _ip]),
     "tmpi_route_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmpi_route": (_i, [_vp, _i64, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

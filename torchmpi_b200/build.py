@@ -64,7 +64,7 @@ def is_current() -> bool:
 
 
 # ---- C++ autograd functions: compiled against PyTorch's headers, resolved against the native library at load time
-BINDINGS_SRC = [CSRC / "bindings" / "autograd.cpp", CSRC / "bindings" / "experts.cpp", CSRC / "bindings" / "fp8.cpp"]
+BINDINGS_SRC = [CSRC / "bindings" / "autograd.cpp", CSRC / "bindings" / "experts.cpp", CSRC / "bindings" / "fp8.cpp", CSRC / "bindings" / "adamw.cpp"]
 BINDINGS = PKG / "lib" / "_autograd.so"
 BINDINGS_STAMP = PKG / "lib" / "bindings.stamp"
 

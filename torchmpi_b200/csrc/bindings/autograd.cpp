@@ -593,5 +593,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("arrival_counters", arrival_counters);
   register_experts(m);
   register_fp8(m);
+  register_adamw(m);
   m.def("launches", [](int what) { return g_launches[what].load(std::memory_order_relaxed); });
 }

@@ -89,5 +89,6 @@ Tensor matmul_nt(const Tensor& a, const Tensor& b, const Tensor& bias);
 void linear_gradients(const Tensor& dy, const Tensor& x, const Tensor& w, Tensor* dx, Tensor* dw, Tensor* db);
 void register_experts(pybind11::module_& m);      // experts.cpp
 void register_fp8(pybind11::module_& m);          // fp8.cpp
+void register_adamw(pybind11::module_& m);        // adamw.cpp
 
 }  // namespace tmpi_bind

@@ -399,6 +399,37 @@ size_t tmpi_fp8_product_workspace_bytes(int M, int N, int K);
 int tmpi_fp8_product(const void* qa, const void* sa, const void* qb, const void* sb, const void* bias, void* c, void* z, int M, int N, int K, int gelu, int dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+// ---------------------------------------------------------------- AdamW over many tensors (adamw.cu)
+typedef struct {
+  void* param;
+  const void* grad;        // of param's type and extent, in the order of its storage
+  int64_t offset;          // of its states, in elements: a multiple of 128; they go on to the next multiple
+  int64_t n;
+  int element_bytes, group, step;      // step: the number of its step count
+} tmpi_adamw_tensor_t;
+typedef struct {
+  float lr, beta1, beta2, rest1, rest2, log_beta1, log_beta2, eps, weight_decay;      // rest: 1 - beta
+  const float* device_lr;              // in the place of lr, or null
+} tmpi_adamw_group_t;
+typedef struct {
+  void *m, *v;                         // fp32, or codes of a byte
+  float *m_top, *v_top;                // of codes: the largest magnitude of 128 elements
+  float* master;                       // of 16-bit parameters, or null
+  int* steps;                          // steps taken by each tensor: one more after the call
+  const float* coefficient;            // the gradients are multiplied by it and by scale; null: by scale alone
+  unsigned* counter;                   // zero, and left zero
+  float scale;
+} tmpi_adamw_states_t;
+int tmpi_adamw_max_groups(void);
+int tmpi_adamw_step(const tmpi_adamw_tensor_t* tensors, int count, const tmpi_adamw_group_t* groups, int ngroups, const tmpi_adamw_states_t* states, int bits, int dtype, void* stream);
+// 8-bit states of `blocks` times 128 elements as numbers
+int tmpi_adamw_values(const void* m, const float* m_top, const void* v, const float* v_top, void* m_values, void* v_values, int64_t blocks, int dtype, void* stream);
+// The norm of many tensors (grad and n of the table): sums of squares, *used of them (at most tmpi_norm_sums(count)), then scale times the root of all sums'
+// sum and, where asked for, min(1, most / (norm + 1e-6)).
+int tmpi_norm_sums(int count);
+int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, double* sums, int* used, void* stream);
+int tmpi_norm_finish(const double* sums, int n, float scale, float most, float* norm, float* coefficient, void* stream);
+
 // ---------------------------------------------------------------- layers of experts (route.cu, experts.cu, grouped.cu)
 // The k largest logits of each token (ties: the lowest index; -inf and NaN never), their weights, and all entries token * k + j in the order of the
 // experts: entry order[s] is at place s, place[entry] = s (-1: not used), the places of expert e from offsets[e] to offsets[e + 1].

@@ -1,0 +1,447 @@
+// AdamW over many tensors at once, with states in 32 or in 8 bits, and the norm of many gradients.
+//
+//   g = coefficient * gradient;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+//   w = (1 - lr decay) w - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// All of it in fp32, w being the fp32 master where there is one (its rounding is then stored as the weight).  t counts a tensor's steps and lies on the
+// device, like the clipping coefficient: a captured step can be replayed.
+//
+// The states of all tensors lie in one buffer each, a tensor's from a multiple of 128 elements on; the tensors' own addresses and extents come as a
+// table among the kernel's parameters (32 bytes a tensor), so that a step is one launch without a copy to the device.  A block takes 2048 consecutive
+// elements of one tensor, a thread eight of them, and finds its tensor by bisection.  Bound by memory.
+//
+// In 8 bits, 128 elements share the largest magnitude among them (fp32), and an element is kept as the root of its share of that, in multiples of 1/127 with
+// its sign for m, and of 1/255 for the root of v: m = +-c^2 top / 127^2, sqrt(v) = c^2 top / 255^2.  The root spends the codes evenly over ratios: the
+// largest are kept within 0.4 % (m: 0.8 %), what is 1/100 of it within 4 % (8 %), and the least number that is not zero is 1/65025 (1/16129) of it.  Of v it is the root
+// that divides the update, and an element whose root is not zero never becomes zero: m / sqrt(v) stays bounded, by a divisor that is then too
+// large, not too small.  The scale of a block is not rounded: where all of its averages shrink alike, as without gradients, the codes stay and
+// the scale follows (with a scale rounded to a power of two an average would stand still, its step of 1 % being less than half a code).
+// A block with an element that is not finite becomes NaN.
+#include "pdl.cuh"
+#include "vec.cuh"
+#include "../include/tmpi_c_api.h"
+#include "../runtime/common.h"
+#include <algorithm>
+#include <vector>
+
+namespace tmpi {
+namespace adamw {
+
+constexpr int THREADS = 256, PER = 8, CHUNK = THREADS * PER, BLOCK = 128;
+
+struct Entry {
+  void* param;
+  const void* grad;
+  uint32_t chunk;        // the first of its chunks
+  uint32_t n;            // elements
+  uint32_t place;        // of its states, in blocks of 128
+  uint32_t which;        // the number of its step count, << 8 | its group | PART | COUNTED
+};
+static_assert(sizeof(Entry) == 32, "the table's size");
+constexpr uint32_t PART = 0x80000000u;        // a further part of a tensor, whose first part counts the step
+constexpr uint32_t COUNTED = 0x40000000u;     // that part was in a launch before this one
+constexpr int MAX_STEPS = 1 << 22;            // step counts that an entry can name
+struct Group { float decay, lr, beta1, beta2, rest1, rest2, log_beta1, log_beta2, eps; const float* device_lr; };      // rest: 1 - beta
+constexpr int MAX_GROUPS = 8;
+
+// SMALL fits the 4 KB of parameters that cost least to launch with
+constexpr int SMALL = 100, LARGE = 980;
+template <int CAP> struct Table {
+  Group group[MAX_GROUPS];
+  Entry entry[CAP];
+};
+
+struct States {
+  void *m, *v;                   // fp32, or codes
+  float *m_top, *v_top;          // of 8 bits
+  float* master;
+  int* steps;
+  const float* coefficient;      // of the gradients, on the device, or null
+  unsigned* counter;             // zero between launches
+  float scale;                   // of the gradients
+  int entries;
+};
+
+__device__ __forceinline__ float root(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// the entry that a chunk belongs to
+template <int CAP>
+__device__ __forceinline__ int entry_of(const Table<CAP>& t, int entries, uint32_t chunk) {
+  int lo = 0, hi = entries - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.entry[mid].chunk <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void load(const T* __restrict__ p, int n, bool vec, float (&x)[PER]) {
+  if (vec && n >= PER) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < PER / V; ++j) {
+      const Pack<T, V> a = ld_pack<T, V>(p + j * V);
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[j * V + k] = (float)to_acc<T>(a.v[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) x[k] = k < n ? (float)to_acc<T>(p[k]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store(T* __restrict__ p, int n, bool vec, const float (&x)[PER]) {
+  if (vec && n >= PER) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < PER / V; ++j) {
+      Pack<T, V> a;
+#pragma unroll
+      for (int k = 0; k < V; ++k) a.v[k] = from_acc<T>((typename AccOf<T>::type)x[j * V + k]);
+      st_pack<T, V>(p + j * V, a);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (k < n) p[k] = from_acc<T>((typename AccOf<T>::type)x[k]);
+  }
+}
+
+// a byte as a float through the mantissa of 2^23, and back: rounded to the nearest integer, of which the low byte counts
+__device__ __forceinline__ float of_byte(uint32_t w, int k) { return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540u + k)); }
+__device__ __forceinline__ uint32_t bytes(const float (&r)[PER], int k) {
+  const uint32_t lo = __byte_perm(__float_as_uint(r[k]), __float_as_uint(r[k + 1]), 0x0040), hi = __byte_perm(__float_as_uint(r[k + 2]), __float_as_uint(r[k + 3]), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+constexpr float LEAST = 7.888609052210118e-31f;          // 2^-100: what a share is divided by at least
+
+// the largest of 128 elements, of which 16 lanes have eight each; magnitudes as integers, so that NaN is the largest
+__device__ __forceinline__ float block_top(const float (&x)[PER]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) a = max(a, __float_as_uint(x[k]) & 0x7fffffffu);
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) a = max(a, __shfl_xor_sync(~0u, a, d));
+  return a < 0x7f800000u ? __uint_as_float(a) : __uint_as_float(0x7fffffffu);
+}
+__device__ __forceinline__ float share(float top) { return __fdividef(1.f, fmaxf(top, LEAST)); }
+
+template <typename T, int BITS, bool MASTER, int CAP>
+__global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ Table<CAP> table, const States s) {
+  __shared__ float rate[2];                              // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  __shared__ unsigned ticket;
+  wait_previous();
+  const uint32_t chunk = blockIdx.x;
+  const int at = entry_of(table, s.entries, chunk);
+  const Entry& e = table.entry[at];
+  const Group& g = table.group[e.which & 0xff];
+  const uint32_t first = (chunk - e.chunk) * CHUNK + threadIdx.x * PER;      // of the tensor
+  const int n = first < e.n ? (int)min((uint32_t)PER, e.n - first) : 0;
+  const bool padded = first < (e.n + BLOCK - 1) / BLOCK * BLOCK;             // the states go on to the end of the block
+  const bool vec = (((uintptr_t)e.param | (uintptr_t)e.grad) & 15) == 0;
+  const size_t p = (size_t)e.place * BLOCK + first;
+  float grad[PER], w[PER], m[PER], v[PER];
+  load<T>((const T*)e.grad + first, n, vec, grad);
+  if (MASTER) load<float>(s.master + p, padded ? PER : 0, true, w);
+  else load<T>((const T*)e.param + first, n, vec, w);
+  if constexpr (BITS == 32) {
+    load<float>((const float*)s.m + p, padded ? PER : 0, true, m);
+    load<float>((const float*)s.v + p, padded ? PER : 0, true, v);
+  } else {
+    uint2 cm = make_uint2(0u, 0u), cv = make_uint2(0u, 0u);
+    float um = 0.f, uv = 0.f;
+    if (padded) {
+      cm = *reinterpret_cast<const uint2*>((const uint8_t*)s.m + p);
+      cv = *reinterpret_cast<const uint2*>((const uint8_t*)s.v + p);
+      um = s.m_top[p / BLOCK] * (1.f / 16129.f);
+      uv = s.v_top[p / BLOCK] * (1.f / 65025.f);
+    }
+    cm.x ^= 0x80808080u, cm.y ^= 0x80808080u;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const float c = of_byte(k < 4 ? cm.x : cm.y, k & 3) - 8388736.f, d = of_byte(k < 4 ? cv.x : cv.y, k & 3) - 8388608.f;
+      m[k] = c * fabsf(c) * um;
+      const float r = d * d * uv;
+      v[k] = r * r;
+    }
+  }
+  if (threadIdx.x == 0) {
+    const float t = (float)(s.steps[(e.which & (COUNTED - 1)) >> 8] + (e.which & COUNTED ? 0 : 1));
+    const float lr = g.device_lr ? *g.device_lr : g.lr;
+    rate[0] = lr / -expm1f(t * g.log_beta1);
+    rate[1] = rsqrtf(-expm1f(t * g.log_beta2));
+  }
+  __syncthreads();
+  const float step = rate[0], unbias = rate[1], coefficient = s.scale * (s.coefficient ? *s.coefficient : 1.f);
+  const float keep = 1.f - (g.device_lr ? *g.device_lr : g.lr) * g.decay, b1 = g.beta1, b2 = g.beta2, eps = g.eps, a1 = g.rest1, a2 = g.rest2;
+  float r[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const float x = grad[k] * coefficient;
+    m[k] = k < n ? b1 * m[k] + a1 * x : 0.f;             // what lies behind the tensor stays zero
+    v[k] = k < n ? b2 * v[k] + a2 * x * x : 0.f;
+    r[k] = root(v[k]);
+    w[k] = k < n ? keep * w[k] - step * __fdividef(m[k], r[k] * unbias + eps) : 0.f;
+  }
+  store<T>((T*)e.param + first, n, vec, w);
+  if (MASTER && padded) store<float>(s.master + p, PER, true, w);
+  if constexpr (BITS == 32) {
+    if (padded) {
+      store<float>((float*)s.m + p, PER, true, m);
+      store<float>((float*)s.v + p, PER, true, v);
+    }
+  } else {
+    const float mt = block_top(m), vt = block_top(r), sm = share(mt), sv = share(vt);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      m[k] = copysignf(127.f * root(fabsf(m[k]) * sm), m[k]) + 12582912.f;
+      const float c = 255.f * root(r[k] * sv) + 8388608.f;
+      r[k] = r[k] > 0.f ? fmaxf(c, 8388609.f) : 8388608.f;
+    }
+    if (padded) {
+      *reinterpret_cast<uint2*>((uint8_t*)s.m + p) = make_uint2(bytes(m, 0), bytes(m, 4));
+      *reinterpret_cast<uint2*>((uint8_t*)s.v + p) = make_uint2(bytes(r, 0), bytes(r, 4));
+      if ((threadIdx.x & 15) == 0) {
+        s.m_top[p / BLOCK] = mt;
+        s.v_top[p / BLOCK] = vt;
+      }
+    }
+  }
+  // The last block to come counts the step: all others have read the counts.
+  if (threadIdx.x == 0) {
+    __threadfence();
+    ticket = atomicAdd(s.counter, 1u);
+  }
+  __syncthreads();
+  if (ticket == gridDim.x - 1) {
+    for (int i = threadIdx.x; i < s.entries; i += THREADS)
+      if (!(table.entry[i].which & PART)) s.steps[table.entry[i].which >> 8] += 1;
+    if (threadIdx.x == 0) *s.counter = 0;
+  }
+}
+
+// ---------------------------------------------------------------- the norm of many tensors
+// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.
+constexpr int NORM_BLOCKS = 148 * 4;
+
+template <typename T, int CAP>
+__global__ void __launch_bounds__(THREADS) squares_kernel(const __grid_constant__ Table<CAP> table, const int entries, const uint32_t chunks, double* __restrict__ sums) {
+  wait_previous(sums);
+  const uint32_t per = (chunks + gridDim.x - 1) / gridDim.x, c0 = blockIdx.x * per, c1 = min(chunks, c0 + per);
+  float a[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) a[k] = 0.f;
+  if (c0 < c1) {
+    int at = entry_of(table, entries, c0);
+    uint32_t next = at + 1 < entries ? table.entry[at + 1].chunk : 0xffffffffu;
+    for (uint32_t c = c0; c < c1; c += 4) {
+      float x[4][PER];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool any = c + u < c1;
+        if (any && c + u >= next) {
+          ++at;
+          next = at + 1 < entries ? table.entry[at + 1].chunk : 0xffffffffu;
+        }
+        const Entry& e = table.entry[at];
+        const uint32_t first = (c + u - e.chunk) * CHUNK + threadIdx.x * PER;
+        load<T>((const T*)e.grad + first, any && first < e.n ? (int)min((uint32_t)PER, e.n - first) : 0, ((uintptr_t)e.grad & 15) == 0, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) a[k] = fmaf(x[u][k], x[u][k], a[k]);
+    }
+  }
+  double d = 0.;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) d += (double)a[k];
+  __shared__ double part[THREADS / 32];
+#pragma unroll
+  for (int i = 16; i; i >>= 1) d += __shfl_xor_sync(~0u, d, i);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = d;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) d += part[i];
+    sums[blockIdx.x] = d;
+  }
+}
+
+// norm = scale sqrt(sum of the sums); coefficient = min(1, most / (norm + 1e-6))
+__global__ void __launch_bounds__(THREADS) norm_kernel(const double* __restrict__ sums, const int n, const float scale, const float most, float* __restrict__ norm,
+                                                       float* __restrict__ coefficient) {
+  wait_previous(sums);
+  double d = 0.;
+  for (int i = threadIdx.x; i < n; i += THREADS) d += sums[i];
+  __shared__ double part[THREADS / 32];
+#pragma unroll
+  for (int i = 16; i; i >>= 1) d += __shfl_xor_sync(~0u, d, i);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = d;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) d += part[i];
+    const float r = (float)(fabs((double)scale) * sqrt(d));
+    *norm = r;
+    if (coefficient) *coefficient = most / (r + 1e-6f) > 1.f ? 1.f : most / (r + 1e-6f);      // NaN stays
+  }
+}
+
+// ---------------------------------------------------------------- what 8-bit states stand for
+template <typename T>
+__global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* __restrict__ m, const float* __restrict__ m_top, const uint8_t* __restrict__ v, const float* __restrict__ v_top,
+                                                         T* __restrict__ mo, T* __restrict__ vo, const long long items) {
+  wait_previous(m, m_top, v, v_top);
+  const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
+  if (i >= items) return;
+  const uint2 cm = *reinterpret_cast<const uint2*>(m + i * PER), cv = *reinterpret_cast<const uint2*>(v + i * PER);
+  const float um = m_top[i * PER / BLOCK] * (1.f / 16129.f), uv = v_top[i * PER / BLOCK] * (1.f / 65025.f);
+  float a[PER], b[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const float c = of_byte((k < 4 ? cm.x : cm.y) ^ 0x80808080u, k & 3) - 8388736.f, d = of_byte(k < 4 ? cv.x : cv.y, k & 3) - 8388608.f, r = d * d * uv;
+    a[k] = c * fabsf(c) * um;
+    b[k] = r * r;
+  }
+  store<T>(mo + i * PER, PER, true, a);
+  store<T>(vo + i * PER, PER, true, b);
+}
+
+// ---------------------------------------------------------------- host side
+// Tables for the tensors [i, ...) until one is full; returns the next tensor and how much of it is in the table.
+struct Filled { int entries; uint32_t chunks; };
+constexpr int64_t MOST = int64_t(1) << 30;               // elements of an entry
+
+template <int CAP>
+static Filled fill(Table<CAP>* t, const tmpi_adamw_tensor_t* tensors, int count, int* i, int64_t* done, bool groups) {
+  Filled f{0, 0};
+  uint32_t counted = *done ? COUNTED : 0u;
+  while (*i < count && f.entries < CAP) {
+    const tmpi_adamw_tensor_t& x = tensors[*i];
+    if (x.n <= 0) { ++*i; continue; }                    // counted by the caller's steps as soon as it has elements
+    const int64_t n = std::min(x.n - *done, MOST);
+    if (f.chunks + (uint64_t)(n + CHUNK - 1) / CHUNK > 0x7fffffffull) break;
+    const int64_t bytes = *done * x.element_bytes;
+    Entry& e = t->entry[f.entries++];
+    e.param = x.param ? (char*)x.param + bytes : nullptr;
+    e.grad = (const char*)x.grad + bytes;
+    e.chunk = f.chunks;
+    e.n = (uint32_t)n;
+    e.place = (uint32_t)((x.offset + *done) / BLOCK);
+    e.which = groups ? (uint32_t)x.step << 8 | (uint32_t)x.group | (*done ? PART : 0u) | counted : 0u;
+    f.chunks += (uint32_t)((n + CHUNK - 1) / CHUNK);
+    *done += n;
+    if (*done >= x.n) { ++*i; *done = 0; counted = 0u; }
+  }
+  return f;
+}
+
+template <typename T, int CAP>
+static cudaError_t launch_step(const Table<CAP>& t, const States& s, int bits, uint32_t chunks, cudaStream_t stream) {
+  const bool master = s.master != nullptr;
+  const auto kernel = bits == 8 ? (master ? step_kernel<T, 8, true, CAP> : step_kernel<T, 8, false, CAP>) : (master ? step_kernel<T, 32, true, CAP> : step_kernel<T, 32, false, CAP>);
+  return launch_overlapped(kernel, chunks, THREADS, 0, stream, t, s);
+}
+
+template <typename F>
+static int by_type(int dtype, const char* what, F f) {
+  cudaError_t e;
+  switch (dtype) {
+    case TMPI_BF16: e = f((__nv_bfloat16*)nullptr); break;
+    case TMPI_F16: e = f((__half*)nullptr); break;
+    case TMPI_F32: e = f((float*)nullptr); break;
+    default: return fail(TMPI_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+  }
+  return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+}
+
+template <int CAP, typename F>
+static cudaError_t each_table(const tmpi_adamw_tensor_t* tensors, int count, const tmpi_adamw_group_t* groups, int ngroups, F f) {
+  Table<CAP> t;
+  for (int g = 0; g < ngroups; ++g) {
+    const tmpi_adamw_group_t& x = groups[g];
+    t.group[g] = {x.weight_decay, x.lr, x.beta1, x.beta2, x.rest1, x.rest2, x.log_beta1, x.log_beta2, x.eps, x.device_lr};
+  }
+  int i = 0;
+  int64_t done = 0;
+  while (i < count) {
+    const Filled filled = fill<CAP>(&t, tensors, count, &i, &done, ngroups > 0);
+    if (!filled.entries) continue;
+    const cudaError_t e = f(t, filled);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace adamw
+}  // namespace tmpi
+
+using namespace tmpi;
+
+extern "C" {
+
+int tmpi_adamw_max_groups(void) { return adamw::MAX_GROUPS; }
+
+int tmpi_adamw_step(const tmpi_adamw_tensor_t* tensors, int count, const tmpi_adamw_group_t* groups, int ngroups, const tmpi_adamw_states_t* states, int bits, int dtype, void* stream) {
+  if (count < 0 || ngroups < 1 || ngroups > adamw::MAX_GROUPS || (bits != 8 && bits != 32)) return fail(TMPI_ERR_INVALID, "adamw: %d groups, %d bits", ngroups, bits);
+  if (!all_aligned16({states->m, states->v, states->master})) return fail(TMPI_ERR_INVALID, "adamw: states must be 16-byte aligned");
+  for (int i = 0; i < count; ++i)
+    if (tensors[i].offset % adamw::BLOCK || tensors[i].offset / adamw::BLOCK + (tensors[i].n + 127) / 128 > 0xffffffffLL || tensors[i].group < 0 || tensors[i].group >= ngroups || tensors[i].step < 0 ||
+        tensors[i].step >= adamw::MAX_STEPS)
+      return fail(TMPI_ERR_INVALID, "adamw: tensor %d has no place among the states", i);
+  adamw::States s{states->m, states->v, states->m_top, states->v_top, states->master, states->steps, states->coefficient, states->counter, states->scale, 0};
+  return adamw::by_type(dtype, "adamw", [&](auto* type) -> cudaError_t {
+    using T = std::remove_pointer_t<decltype(type)>;
+    if (sizeof(T) == 4 && s.master) return cudaErrorInvalidValue;
+    auto run = [&](const auto& table, const adamw::Filled& f) {
+      s.entries = f.entries;
+      return adamw::launch_step<T>(table, s, bits, f.chunks, (cudaStream_t)stream);
+    };
+    return count <= adamw::SMALL ? adamw::each_table<adamw::SMALL>(tensors, count, groups, ngroups, run) : adamw::each_table<adamw::LARGE>(tensors, count, groups, ngroups, run);
+  });
+}
+
+// Sums of squares of `count` tensors into sums [tmpi_norm_sums(count)], of which *used were written.  A launch takes SMALL entries at least, and the tensors of a GPU (less than
+// 2^38 bytes) have not more than 256 entries beside their first ones.
+int tmpi_norm_sums(int count) { return (count / adamw::SMALL + 5) * adamw::NORM_BLOCKS; }
+int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, double* sums, int* used, void* stream) {
+  *used = 0;
+  if (count < 0) return fail(TMPI_ERR_INVALID, "norm: %d tensors", count);
+  return adamw::by_type(dtype, "norm", [&](auto* type) -> cudaError_t {
+    using T = std::remove_pointer_t<decltype(type)>;
+    auto run = [&](const auto& table, const adamw::Filled& f) {
+      constexpr int CAP = sizeof(table.entry) / sizeof(adamw::Entry);
+      const int blocks = (int)std::min<uint32_t>(adamw::NORM_BLOCKS, f.chunks);
+      const cudaError_t e = launch_overlapped(adamw::squares_kernel<T, CAP>, blocks, adamw::THREADS, 0, (cudaStream_t)stream, table, f.entries, f.chunks, sums + *used);
+      *used += blocks;
+      return e;
+    };
+    return count <= adamw::SMALL ? adamw::each_table<adamw::SMALL>(tensors, count, nullptr, 0, run) : adamw::each_table<adamw::LARGE>(tensors, count, nullptr, 0, run);
+  });
+}
+int tmpi_norm_finish(const double* sums, int n, float scale, float most, float* norm, float* coefficient, void* stream) {
+  const cudaError_t e = launch_overlapped(adamw::norm_kernel, 1, adamw::THREADS, 0, (cudaStream_t)stream, sums, n, scale, most, norm, coefficient);
+  return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "norm launch: %s", cudaGetErrorString(e));
+}
+
+// blocks of 128 elements -> m and v in `dtype`
+int tmpi_adamw_values(const void* m, const float* m_top, const void* v, const float* v_top, void* mo, void* vo, int64_t blocks, int dtype, void* stream) {
+  if (blocks < 0 || blocks > (int64_t)1 << 31) return fail(TMPI_ERR_INVALID, "adamw_values: %lld blocks", (long long)blocks);
+  if (!blocks) return TMPI_OK;
+  if (!all_aligned16({m, v, mo, vo})) return fail(TMPI_ERR_INVALID, "adamw_values: tensors must be 16-byte aligned");
+  return adamw::by_type(dtype, "adamw_values", [&](auto* type) -> cudaError_t {
+    using T = std::remove_pointer_t<decltype(type)>;
+    const long long items = blocks * (adamw::BLOCK / adamw::PER);
+    return launch_overlapped(adamw::values_kernel<T>, (unsigned)((items + adamw::THREADS - 1) / adamw::THREADS), adamw::THREADS, 0, (cudaStream_t)stream, (const uint8_t*)m, m_top,
+                             (const uint8_t*)v, v_top, (T*)mo, (T*)vo, items);
+  });
+}
+
+}  // extern "C"
