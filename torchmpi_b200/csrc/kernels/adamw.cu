@@ -7,8 +7,9 @@
 // device, like the clipping coefficient: a captured step can be replayed.
 //
 // The states of all tensors lie in one buffer each, a tensor's from a multiple of 128 elements on; the tensors' own addresses and extents come as a
-// table among the kernel's parameters (32 bytes a tensor), so that a step is one launch without a copy to the device.  A block takes 2048 consecutive
-// elements of one tensor, a thread eight of them, and finds its tensor by bisection.  Bound by memory.
+// table among the kernel's parameters (32 bytes a tensor), so that a step is one launch without a copy to the device.  Tensors are cut into chunks of 2048 elements,
+// a thread eight of them; a block takes chunk after chunk, as many apart as there are blocks, finds the first one's tensor by bisection and forms a
+// tensor's rates when it comes to it.  Bound by memory.
 //
 // In 8 bits, 128 elements share the largest magnitude among them (fp32), and an element is kept as the root of its share of that, in multiples of 1/127 with
 // its sign for m, and of 1/255 for the root of v: m = +-c^2 top / 127^2, sqrt(v) = c^2 top / 255^2.  The root spends the codes evenly over ratios: the
@@ -17,6 +18,7 @@
 // large, not too small.  The scale of a block is not rounded: where all of its averages shrink alike, as without gradients, the codes stay and
 // the scale follows (with a scale rounded to a power of two an average would stand still, its step of 1 % being less than half a code).
 // A block with an element that is not finite becomes NaN.
+#include "attn_util.cuh"
 #include "pdl.cuh"
 #include "vec.cuh"
 #include "../include/tmpi_c_api.h"
@@ -27,7 +29,8 @@
 namespace tmpi {
 namespace adamw {
 
-constexpr int THREADS = 256, PER = 8, CHUNK = THREADS * PER, BLOCK = 128;
+constexpr int THREADS = 256, BLOCK = 128;
+constexpr int CHUNK = THREADS * 8;
 
 struct Entry {
   void* param;
@@ -62,9 +65,15 @@ struct States {
   int entries;
 };
 
+// sqrt to within two units in the last place, of subnormals too; `quick_root` takes those for zero
 __device__ __forceinline__ float root(float x) {
   float y;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float quick_root(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -80,10 +89,11 @@ __device__ __forceinline__ int entry_of(const Table<CAP>& t, int entries, uint32
   return lo;
 }
 
-template <typename T>
-__device__ __forceinline__ void load(const T* __restrict__ p, int n, bool vec, float (&x)[PER]) {
+// PER consecutive elements, in pieces of 16 bytes at most
+template <typename T, int PER>
+__device__ __forceinline__ void load(const T* __restrict__ p, int n, bool vec, float* x) {
   if (vec && n >= PER) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = PER * sizeof(T) <= 16 ? PER : 16 / sizeof(T);
 #pragma unroll
     for (int j = 0; j < PER / V; ++j) {
       const Pack<T, V> a = ld_pack<T, V>(p + j * V);
@@ -95,10 +105,10 @@ __device__ __forceinline__ void load(const T* __restrict__ p, int n, bool vec, f
     for (int k = 0; k < PER; ++k) x[k] = k < n ? (float)to_acc<T>(p[k]) : 0.f;
   }
 }
-template <typename T>
-__device__ __forceinline__ void store(T* __restrict__ p, int n, bool vec, const float (&x)[PER]) {
+template <typename T, int PER>
+__device__ __forceinline__ void store(T* __restrict__ p, int n, bool vec, const float* x) {
   if (vec && n >= PER) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = PER * sizeof(T) <= 16 ? PER : 16 / sizeof(T);
 #pragma unroll
     for (int j = 0; j < PER / V; ++j) {
       Pack<T, V> a;
@@ -115,109 +125,140 @@ __device__ __forceinline__ void store(T* __restrict__ p, int n, bool vec, const 
 
 // a byte as a float through the mantissa of 2^23, and back: rounded to the nearest integer, of which the low byte counts
 __device__ __forceinline__ float of_byte(uint32_t w, int k) { return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540u + k)); }
-__device__ __forceinline__ uint32_t bytes(const float (&r)[PER], int k) {
-  const uint32_t lo = __byte_perm(__float_as_uint(r[k]), __float_as_uint(r[k + 1]), 0x0040), hi = __byte_perm(__float_as_uint(r[k + 2]), __float_as_uint(r[k + 3]), 0x0040);
+__device__ __forceinline__ uint32_t bytes(const float* r) {
+  const uint32_t lo = __byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040), hi = __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
 }
 constexpr float LEAST = 7.888609052210118e-31f;          // 2^-100: what a share is divided by at least
+constexpr float LEAST_EPS = 1e-37f;                      // an element without any gradient is 0 / (0 + eps): stays, also with eps = 0
+constexpr float LEAST_EPS8 = 1e-18f;                     // of 8-bit states, which know no root below 1e-19
 
-// the largest of 128 elements, of which 16 lanes have eight each; magnitudes as integers, so that NaN is the largest
+// the largest magnitude of 128 elements, of which 128 / PER lanes have PER each; NaN if one is not finite
+template <int PER>
 __device__ __forceinline__ float block_top(const float (&x)[PER]) {
-  uint32_t a = 0;
+  float a = attn_util::max_nan(fabsf(x[0]), fabsf(x[1]));
 #pragma unroll
-  for (int k = 0; k < PER; ++k) a = max(a, __float_as_uint(x[k]) & 0x7fffffffu);
+  for (int k = 2; k < PER; k += 2) a = attn_util::max3_nan(a, fabsf(x[k]), fabsf(x[k + 1]));
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) a = max(a, __shfl_xor_sync(~0u, a, d));
-  return a < 0x7f800000u ? __uint_as_float(a) : __uint_as_float(0x7fffffffu);
+  for (int d = 1; d < BLOCK / PER; d *= 2) a = attn_util::max_nan(a, __shfl_xor_sync(~0u, a, d));
+  return a < __uint_as_float(0x7f800000u) ? a : __uint_as_float(0x7fffffffu);
 }
-__device__ __forceinline__ float share(float top) { return __fdividef(1.f, fmaxf(top, LEAST)); }
+
+// four codes of the first moment, and of the second's root
+__device__ __forceinline__ void decode_m(uint32_t w, float unit, float* m) {
+  w ^= 0x80808080u;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float c = of_byte(w, k) - 8388736.f;
+    m[k] = c * fabsf(c) * unit;
+  }
+}
+__device__ __forceinline__ void decode_v(uint32_t w, float unit, float* v) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float c = of_byte(w, k) - 8388608.f, r = c * c * unit;
+    v[k] = r * r;
+  }
+}
 
 template <typename T, int BITS, bool MASTER, int CAP>
-__global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ Table<CAP> table, const States s) {
-  __shared__ float rate[2];                              // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+__global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant__ Table<CAP> table, const States s, const uint32_t chunks) {
+  constexpr int PER = CHUNK / THREADS;
+  // Elements of a thread that lie beside each other; its next ones are APART further.  Four, where most bytes are those of fp32, so that a warp's accesses are whole
+  // lines (two 16-byte stores beside each other are half sectors for each of the warp's instructions); else all, whose 16-bit loads are then 16 bytes.
+  constexpr int RUN = BITS == 32 && (MASTER || sizeof(T) == 4) ? 4 : PER;
+  constexpr uint32_t APART = RUN * THREADS;
   __shared__ unsigned ticket;
   wait_previous();
-  const uint32_t chunk = blockIdx.x;
-  const int at = entry_of(table, s.entries, chunk);
-  const Entry& e = table.entry[at];
-  const Group& g = table.group[e.which & 0xff];
-  const uint32_t first = (chunk - e.chunk) * CHUNK + threadIdx.x * PER;      // of the tensor
-  const int n = first < e.n ? (int)min((uint32_t)PER, e.n - first) : 0;
-  const bool padded = first < (e.n + BLOCK - 1) / BLOCK * BLOCK;             // the states go on to the end of the block
-  const bool vec = (((uintptr_t)e.param | (uintptr_t)e.grad) & 15) == 0;
-  const size_t p = (size_t)e.place * BLOCK + first;
-  float grad[PER], w[PER], m[PER], v[PER];
-  load<T>((const T*)e.grad + first, n, vec, grad);
-  if (MASTER) load<float>(s.master + p, padded ? PER : 0, true, w);
-  else load<T>((const T*)e.param + first, n, vec, w);
-  if constexpr (BITS == 32) {
-    load<float>((const float*)s.m + p, padded ? PER : 0, true, m);
-    load<float>((const float*)s.v + p, padded ? PER : 0, true, v);
-  } else {
-    uint2 cm = make_uint2(0u, 0u), cv = make_uint2(0u, 0u);
-    float um = 0.f, uv = 0.f;
-    if (padded) {
-      cm = *reinterpret_cast<const uint2*>((const uint8_t*)s.m + p);
-      cv = *reinterpret_cast<const uint2*>((const uint8_t*)s.v + p);
-      um = s.m_top[p / BLOCK] * (1.f / 16129.f);
-      uv = s.v_top[p / BLOCK] * (1.f / 65025.f);
-    }
-    cm.x ^= 0x80808080u, cm.y ^= 0x80808080u;
+  const float coefficient = s.scale * (s.coefficient ? *s.coefficient : 1.f);
+  int at = entry_of(table, s.entries, blockIdx.x);
+  for (uint32_t c = blockIdx.x; c < chunks; ++at) {        // one tensor after another
+    while (at + 1 < s.entries && table.entry[at + 1].chunk <= c) ++at;
+    const Entry& e = table.entry[at];
+    const Group& g = table.group[e.which & 0xff];
+    const float t = (float)(s.steps[(e.which & (COUNTED - 1)) >> 8] + (e.which & COUNTED ? 0 : 1)), lr = g.device_lr ? *g.device_lr : g.lr;
+    // The update is m / (sqrt(v) unbias + eps) with the rate lr / (1 - b1^t) in the divisor (as 1e-30 at least: its inverse is a number), and a root of what a
+    // square takes on its way into v in front of the square.
+    const float step = fmaxf(lr / -expm1f(t * g.log_beta1), 1e-30f), unbias = rsqrtf(-expm1f(t * g.log_beta2)) / step, keep = 1.f - lr * g.decay;
+    const float b1 = g.beta1, b2 = g.beta2, a1 = g.rest1 * coefficient, a2 = sqrtf(g.rest2) * coefficient, eps = fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step;
+    const float unit_m = b1 * (1.f / 16129.f), unit_v = sqrtf(b2) * (1.f / 65025.f);
+    const uint32_t e0 = e.chunk, end = at + 1 < s.entries ? table.entry[at + 1].chunk : chunks, extent = e.n, whole = (extent + BLOCK - 1) / BLOCK * BLOCK;
+    T* const param = (T*)e.param;
+    const T* const grads = (const T*)e.grad;
+    const bool vec = (((uintptr_t)param | (uintptr_t)grads) & 15) == 0;
+    const size_t place = (size_t)e.place * BLOCK;
+    for (; c < end; c += gridDim.x) {
+      const uint32_t first = (c - e0) * CHUNK + threadIdx.x * RUN;             // of the tensor
+      float grad[PER], w[PER], m[PER], v[PER];
+      auto left = [&](int j) { const uint32_t f = first + j * APART; return f < extent ? (int)min((uint32_t)RUN, extent - f) : 0; };
+      auto padded = [&](int j) { return first + j * APART < whole ? RUN : 0; };      // the states go on, as zeros, to the end of a block
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const float c = of_byte(k < 4 ? cm.x : cm.y, k & 3) - 8388736.f, d = of_byte(k < 4 ? cv.x : cv.y, k & 3) - 8388608.f;
-      m[k] = c * fabsf(c) * um;
-      const float r = d * d * uv;
-      v[k] = r * r;
-    }
-  }
-  if (threadIdx.x == 0) {
-    const float t = (float)(s.steps[(e.which & (COUNTED - 1)) >> 8] + (e.which & COUNTED ? 0 : 1));
-    const float lr = g.device_lr ? *g.device_lr : g.lr;
-    rate[0] = lr / -expm1f(t * g.log_beta1);
-    rate[1] = rsqrtf(-expm1f(t * g.log_beta2));
-  }
-  __syncthreads();
-  const float step = rate[0], unbias = rate[1], coefficient = s.scale * (s.coefficient ? *s.coefficient : 1.f);
-  const float keep = 1.f - (g.device_lr ? *g.device_lr : g.lr) * g.decay, b1 = g.beta1, b2 = g.beta2, eps = g.eps, a1 = g.rest1, a2 = g.rest2;
-  float r[PER];
+      for (int j = 0; j < PER / RUN; ++j) {
+        const size_t p = place + first + j * APART;
+        load<T, RUN>(grads + first + j * APART, left(j), vec, grad + RUN * j);
+        if (MASTER) load<float, RUN>(s.master + p, padded(j), true, w + RUN * j);
+        else load<T, RUN>(param + first + j * APART, left(j), vec, w + RUN * j);
+        if constexpr (BITS == 32) {
+          load<float, RUN>((const float*)s.m + p, padded(j), true, m + RUN * j);
+          load<float, RUN>((const float*)s.v + p, padded(j), true, v + RUN * j);
+        }
+      }
+      const size_t p0 = place + first;
+      if constexpr (BITS == 8) {                       // times the decay of the averages, which enters the units
+        uint2 cm = make_uint2(0u, 0u), cv = cm;
+        float um = 0.f, uv = 0.f;
+        if (padded(0)) {
+          cm = *reinterpret_cast<const uint2*>((const uint8_t*)s.m + p0);
+          cv = *reinterpret_cast<const uint2*>((const uint8_t*)s.v + p0);
+          um = s.m_top[p0 / BLOCK] * unit_m;
+          uv = s.v_top[p0 / BLOCK] * unit_v;
+        }
+        decode_m(cm.x, um, m), decode_m(cm.y, um, m + 4);
+        decode_v(cv.x, uv, v), decode_v(cv.y, uv, v + 4);
+      }
+      float r[PER];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const float x = grad[k] * coefficient;
-    m[k] = k < n ? b1 * m[k] + a1 * x : 0.f;             // what lies behind the tensor stays zero
-    v[k] = k < n ? b2 * v[k] + a2 * x * x : 0.f;
-    r[k] = root(v[k]);
-    w[k] = k < n ? keep * w[k] - step * __fdividef(m[k], r[k] * unbias + eps) : 0.f;
-  }
-  store<T>((T*)e.param + first, n, vec, w);
-  if (MASTER && padded) store<float>(s.master + p, PER, true, w);
-  if constexpr (BITS == 32) {
-    if (padded) {
-      store<float>((float*)s.m + p, PER, true, m);
-      store<float>((float*)s.v + p, PER, true, v);
-    }
-  } else {
-    const float mt = block_top(m), vt = block_top(r), sm = share(mt), sv = share(vt);
+      for (int k = 0; k < PER; ++k) {
+        const float x = grad[k] * a2;
+        m[k] = fmaf(a1, grad[k], BITS == 8 ? m[k] : b1 * m[k]);
+        v[k] = fmaf(x, x, BITS == 8 ? v[k] : b2 * v[k]);
+        r[k] = BITS == 8 ? quick_root(v[k]) : root(v[k]);
+        w[k] = fmaf(-m[k], attn_util::rcp(fmaf(r[k], unbias, eps)), keep * w[k]);
+      }
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      m[k] = copysignf(127.f * root(fabsf(m[k]) * sm), m[k]) + 12582912.f;
-      const float c = 255.f * root(r[k] * sv) + 8388608.f;
-      r[k] = r[k] > 0.f ? fmaxf(c, 8388609.f) : 8388608.f;
-    }
-    if (padded) {
-      *reinterpret_cast<uint2*>((uint8_t*)s.m + p) = make_uint2(bytes(m, 0), bytes(m, 4));
-      *reinterpret_cast<uint2*>((uint8_t*)s.v + p) = make_uint2(bytes(r, 0), bytes(r, 4));
-      if ((threadIdx.x & 15) == 0) {
-        s.m_top[p / BLOCK] = mt;
-        s.v_top[p / BLOCK] = vt;
+      for (int j = 0; j < PER / RUN; ++j) {
+        const size_t p = place + first + j * APART;
+        store<T, RUN>(param + first + j * APART, left(j), vec, w + RUN * j);
+        if (padded(j)) {
+          if (MASTER) store<float, RUN>(s.master + p, RUN, true, w + RUN * j);
+          if constexpr (BITS == 32) {
+            store<float, RUN>((float*)s.m + p, RUN, true, m + RUN * j);
+            store<float, RUN>((float*)s.v + p, RUN, true, v + RUN * j);
+          }
+        }
+      }
+      if constexpr (BITS == 8) {
+        const float mt = block_top<PER>(m), vt = block_top<PER>(r), sm = 16129.f * attn_util::rcp(fmaxf(mt, LEAST)), sv = 65025.f * attn_util::rcp(fmaxf(vt, LEAST));
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          m[k] = copysignf(quick_root(fabsf(m[k]) * sm), m[k]) + 12582912.f;
+          r[k] = quick_root(fmaxf(r[k] * sv, __saturatef(r[k] * 3e38f))) + 8388608.f;      // at least 1 for what is not zero
+        }
+        if (padded(0)) {
+          *reinterpret_cast<uint2*>((uint8_t*)s.m + p0) = make_uint2(bytes(m), bytes(m + 4));
+          *reinterpret_cast<uint2*>((uint8_t*)s.v + p0) = make_uint2(bytes(r), bytes(r + 4));
+          if ((threadIdx.x & (BLOCK / PER - 1)) == 0) {
+            s.m_top[p0 / BLOCK] = mt;
+            s.v_top[p0 / BLOCK] = vt;
+          }
+        }
       }
     }
   }
   // The last block to come counts the step: all others have read the counts.
-  if (threadIdx.x == 0) {
-    __threadfence();
-    ticket = atomicAdd(s.counter, 1u);
-  }
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) ticket = atomicAdd(s.counter, 1u);
   __syncthreads();
   if (ticket == gridDim.x - 1) {
     for (int i = threadIdx.x; i < s.entries; i += THREADS)
@@ -227,36 +268,57 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ T
 }
 
 // ---------------------------------------------------------------- the norm of many tensors
-// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.
+// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.  Eight chunks are under way at a time.
 constexpr int NORM_BLOCKS = 148 * 4;
 
+// not moved behind what is done with the loads before it
+__device__ __forceinline__ uint4 load_in_order(const void* p) {
+  uint4 u;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
+}
+
 template <typename T, int CAP>
-__global__ void __launch_bounds__(THREADS) squares_kernel(const __grid_constant__ Table<CAP> table, const int entries, const uint32_t chunks, double* __restrict__ sums) {
+__global__ void __launch_bounds__(THREADS) squares_kernel(const __grid_constant__ Table<CAP> table, const int entries, const uint32_t chunks, const uint32_t per_block, double* __restrict__ sums) {
+  constexpr int PER = CHUNK / THREADS, AHEAD = sizeof(T) == 2 ? 8 : 4;
   wait_previous(sums);
-  const uint32_t per = (chunks + gridDim.x - 1) / gridDim.x, c0 = blockIdx.x * per, c1 = min(chunks, c0 + per);
+  const uint32_t c0 = blockIdx.x * per_block, c1 = min(chunks, c0 + per_block);
   float a[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) a[k] = 0.f;
-  if (c0 < c1) {
-    int at = entry_of(table, entries, c0);
-    uint32_t next = at + 1 < entries ? table.entry[at + 1].chunk : 0xffffffffu;
-    for (uint32_t c = c0; c < c1; c += 4) {
-      float x[4][PER];
+  int at = entry_of(table, entries, c0);
+  for (uint32_t c = c0; c < c1; ++at) {
+    const Entry& e = table.entry[at];
+    const uint32_t e0 = e.chunk, end = min(c1, at + 1 < entries ? table.entry[at + 1].chunk : chunks), extent = e.n;
+    const T* const grads = (const T*)e.grad;
+    const bool vec = ((uintptr_t)grads & 15) == 0;
+    const uint32_t whole = min(end, e0 + extent / CHUNK);       // chunks without an end of the tensor
+    if (vec) {
+      constexpr int V = 16 / sizeof(T), PACKS = PER / V;
+      for (; c + AHEAD <= whole; c += AHEAD) {
+        uint4 x[AHEAD][PACKS];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool any = c + u < c1;
-        if (any && c + u >= next) {
-          ++at;
-          next = at + 1 < entries ? table.entry[at + 1].chunk : 0xffffffffu;
-        }
-        const Entry& e = table.entry[at];
-        const uint32_t first = (c + u - e.chunk) * CHUNK + threadIdx.x * PER;
-        load<T>((const T*)e.grad + first, any && first < e.n ? (int)min((uint32_t)PER, e.n - first) : 0, ((uintptr_t)e.grad & 15) == 0, x[u]);
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+          for (int j = 0; j < PACKS; ++j) x[u][j] = load_in_order(grads + (size_t)(c + u - e0) * CHUNK + j * (V * THREADS) + threadIdx.x * V);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            const float f = (float)to_acc<T>(reinterpret_cast<const T*>(&x[u][k / V])[k % V]);
+            a[k] = fmaf(f, f, a[k]);
+          }
+      }
+    }
+    for (; c < end; ++c) {
+      float x[PER];
+#pragma unroll
+      for (int j = 0; j < PER; j += 4) {
+        const uint32_t first = (c - e0) * CHUNK + j * THREADS + threadIdx.x * 4;
+        load<T, 4>(grads + first, first < extent ? (int)min(4u, extent - first) : 0, vec, x + j);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int k = 0; k < PER; ++k) a[k] = fmaf(x[u][k], x[u][k], a[k]);
+      for (int k = 0; k < PER; ++k) a[k] = fmaf(x[k], x[k], a[k]);
     }
   }
   double d = 0.;
@@ -301,17 +363,13 @@ __global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* __restri
   wait_previous(m, m_top, v, v_top);
   const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
   if (i >= items) return;
-  const uint2 cm = *reinterpret_cast<const uint2*>(m + i * PER), cv = *reinterpret_cast<const uint2*>(v + i * PER);
-  const float um = m_top[i * PER / BLOCK] * (1.f / 16129.f), uv = v_top[i * PER / BLOCK] * (1.f / 65025.f);
-  float a[PER], b[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const float c = of_byte((k < 4 ? cm.x : cm.y) ^ 0x80808080u, k & 3) - 8388736.f, d = of_byte(k < 4 ? cv.x : cv.y, k & 3) - 8388608.f, r = d * d * uv;
-    a[k] = c * fabsf(c) * um;
-    b[k] = r * r;
-  }
-  store<T>(mo + i * PER, PER, true, a);
-  store<T>(vo + i * PER, PER, true, b);
+  const uint2 cm = reinterpret_cast<const uint2*>(m)[i], cv = reinterpret_cast<const uint2*>(v)[i];
+  const float um = m_top[i / 16] * (1.f / 16129.f), uv = v_top[i / 16] * (1.f / 65025.f);
+  float a[8], b[8];
+  decode_m(cm.x, um, a), decode_m(cm.y, um, a + 4);
+  decode_v(cv.x, uv, b), decode_v(cv.y, uv, b + 4);
+  store<T, 8>(mo + i * 8, 8, true, a);
+  store<T, 8>(vo + i * 8, 8, true, b);
 }
 
 // ---------------------------------------------------------------- host side
@@ -343,11 +401,14 @@ static Filled fill(Table<CAP>* t, const tmpi_adamw_tensor_t* tensors, int count,
   return f;
 }
 
+// chunks of a block, for at most `most` blocks
+static uint32_t per_block(uint32_t chunks, uint32_t most) { return (chunks + most - 1) / most; }
+
 template <typename T, int CAP>
 static cudaError_t launch_step(const Table<CAP>& t, const States& s, int bits, uint32_t chunks, cudaStream_t stream) {
   const bool master = s.master != nullptr;
   const auto kernel = bits == 8 ? (master ? step_kernel<T, 8, true, CAP> : step_kernel<T, 8, false, CAP>) : (master ? step_kernel<T, 32, true, CAP> : step_kernel<T, 32, false, CAP>);
-  return launch_overlapped(kernel, chunks, THREADS, 0, stream, t, s);
+  return launch_overlapped(kernel, std::min<uint32_t>(chunks, 148 * 5), THREADS, 0, stream, t, s, chunks);
 }
 
 template <typename F>
@@ -418,9 +479,9 @@ int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, 
     using T = std::remove_pointer_t<decltype(type)>;
     auto run = [&](const auto& table, const adamw::Filled& f) {
       constexpr int CAP = sizeof(table.entry) / sizeof(adamw::Entry);
-      const int blocks = (int)std::min<uint32_t>(adamw::NORM_BLOCKS, f.chunks);
-      const cudaError_t e = launch_overlapped(adamw::squares_kernel<T, CAP>, blocks, adamw::THREADS, 0, (cudaStream_t)stream, table, f.entries, f.chunks, sums + *used);
-      *used += blocks;
+      const uint32_t per = adamw::per_block(f.chunks, adamw::NORM_BLOCKS), blocks = (f.chunks + per - 1) / per;
+      const cudaError_t e = launch_overlapped(adamw::squares_kernel<T, CAP>, blocks, adamw::THREADS, 0, (cudaStream_t)stream, table, f.entries, f.chunks, per, sums + *used);
+      *used += (int)blocks;
       return e;
     };
     return count <= adamw::SMALL ? adamw::each_table<adamw::SMALL>(tensors, count, nullptr, 0, run) : adamw::each_table<adamw::LARGE>(tensors, count, nullptr, 0, run);
@@ -438,7 +499,7 @@ int tmpi_adamw_values(const void* m, const float* m_top, const void* v, const fl
   if (!all_aligned16({m, v, mo, vo})) return fail(TMPI_ERR_INVALID, "adamw_values: tensors must be 16-byte aligned");
   return adamw::by_type(dtype, "adamw_values", [&](auto* type) -> cudaError_t {
     using T = std::remove_pointer_t<decltype(type)>;
-    const long long items = blocks * (adamw::BLOCK / adamw::PER);
+    const long long items = blocks * (adamw::BLOCK / 8);
     return launch_overlapped(adamw::values_kernel<T>, (unsigned)((items + adamw::THREADS - 1) / adamw::THREADS), adamw::THREADS, 0, (cudaStream_t)stream, (const uint8_t*)m, m_top,
                              (const uint8_t*)v, v_top, (T*)mo, (T*)vo, items);
   });

@@ -12,29 +12,38 @@
 #include "../include/tmpi_c_api.h"
 #include "../runtime/common.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace tmpi {
 namespace fp8 {
 
 using act8::inverse;
-using act8::magnitude;
 using act8::pack2;
 using act8::scale_byte;
 using act8::value;
 
-// Eight elements as words: magnitudes of 16-bit types are compared two at a time, as integers (which order like the values).
+// Eight elements as words: magnitudes of 16-bit types are compared two at a time.  `largest` gives the larger magnitude, with a sign that means nothing, and NaN if
+// either is.
 template <typename T> struct Eight;
 template <> struct Eight<__nv_bfloat16> {
   static constexpr int WORDS = 4;
   static constexpr uint32_t ABS = 0x7fff7fffu, INF = 0x7f80u;
-  static __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  static __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
   static __device__ __forceinline__ float get(const uint32_t* w, int k) { return __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return attn_util::pack_bf16(__float_as_uint(lo), __float_as_uint(hi)); }
 };
 template <> struct Eight<__half> {
   static constexpr int WORDS = 4;
   static constexpr uint32_t ABS = 0x7fff7fffu, INF = 0x7c00u;
-  static __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  static __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
   static __device__ __forceinline__ float get(const uint32_t* w, int k) { return __half2float(__ushort_as_half((unsigned short)(w[k >> 1] >> (16 * (k & 1))))); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -44,15 +53,28 @@ template <> struct Eight<__half> {
 template <> struct Eight<float> {
   static constexpr int WORDS = 8;
   static constexpr uint32_t ABS = 0x7fffffffu, INF = 0x7f800000u;
-  static __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) { return max(a, b); }
+  static __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
+    float r;
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+    return __float_as_uint(r);
+  }
   static __device__ __forceinline__ float get(const uint32_t* w, int k) { return __uint_as_float(w[k]); }
 };
 // the largest magnitude in a word, as the type's bits, and the bits of the fp32 number that it is
-template <typename T> __device__ __forceinline__ uint32_t of_word(uint32_t w) { return sizeof(T) == 2 ? max(w & 0xffffu, w >> 16) : w; }
+template <typename T> __device__ __forceinline__ uint32_t of_word(uint32_t w) {
+  w &= Eight<T>::ABS;
+  return sizeof(T) == 2 ? max(w & 0xffffu, w >> 16) : w;
+}
 template <typename T> __device__ __forceinline__ uint32_t as_fp32(uint32_t bits);
 template <> __device__ __forceinline__ uint32_t as_fp32<__nv_bfloat16>(uint32_t b) { return b << 16; }
 template <> __device__ __forceinline__ uint32_t as_fp32<__half>(uint32_t b) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)b))); }
 template <> __device__ __forceinline__ uint32_t as_fp32<float>(uint32_t b) { return b; }
+// the same word with zeros for what is not finite
+template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
+  const uint32_t m = w & Eight<T>::ABS;
+  if (sizeof(T) == 2) return ((m & 0xffffu) < Eight<T>::INF ? m & 0xffffu : 0u) | ((m >> 16) < Eight<T>::INF ? m & 0xffff0000u : 0u);
+  return m < Eight<T>::INF ? m : 0u;
+}
 
 // n elements (up to 8) at p; vec: whole, and on 16-byte boundaries
 template <typename T>
@@ -76,9 +98,19 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int n, bool vec, 
   }
 }
 
-// four values in a word; `finite`: none is infinite
-__device__ __forceinline__ uint32_t four(float a, float b, float c, float d, float inv, bool finite) {
-  if (finite) {
+template <typename T>
+__device__ __forceinline__ void load_whole(const T* __restrict__ p, uint32_t (&w)[Eight<T>::WORDS]) {
+#pragma unroll
+  for (int j = 0; j < Eight<T>::WORDS; j += 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + j);
+    w[j] = u.x, w[j + 1] = u.y, w[j + 2] = u.z, w[j + 3] = u.w;
+  }
+}
+
+// four values in a word; FINITE: none is infinite
+template <bool FINITE>
+__device__ __forceinline__ uint32_t four(float a, float b, float c, float d, float inv) {
+  if (FINITE) {
     const unsigned long long inv2 = attn_util::pack2(__float_as_uint(inv), __float_as_uint(inv));
     float2 v, u;
     attn_util::unpack2(attn_util::mul2(attn_util::pack2(__float_as_uint(a), __float_as_uint(b)), inv2), v.x, v.y);
@@ -87,119 +119,157 @@ __device__ __forceinline__ uint32_t four(float a, float b, float c, float d, flo
   }
   return pack2(a, b, inv) | pack2(c, d, inv) << 16;
 }
+template <typename T, bool FINITE>
+__device__ __forceinline__ uint2 eight(const uint32_t* w, float inv) {
+  using E = Eight<T>;
+  return make_uint2(four<FINITE>(E::get(w, 0), E::get(w, 1), E::get(w, 2), E::get(w, 3), inv), four<FINITE>(E::get(w, 4), E::get(w, 5), E::get(w, 6), E::get(w, 7), inv));
+}
 
 // ---------------------------------------------------------------- along rows
-// Eight threads to a block of 128, sixteen elements each.
+// Eight threads to a block of 128, sixteen elements each, two of a thread's pieces under way at a time (16 bytes by each thread, so that a warp's loads
+// are whole lines, took more instructions for an element and 25.7 us in place of ROWS_US at 8192 x 4096).
 constexpr int ROW_THREADS = 256;
+struct Stride { int rows, pieces; };          // a launch's threads, as rows of pieces: what a thread's next piece lies further
 
 template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __restrict__ x, const long long ld, uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
-                                                                    const long long rows, const int cols, const bool vec) {
-  wait_previous(x);
-  const int blocks = blocks_of(cols), groups = groups_of(cols);
-  const long long pitch = pitch_of(cols), items = rows * blocks * 8, stride = (long long)gridDim.x * ROW_THREADS;
+                                                                    const long long rows, const int cols, const bool vec, const Stride step) {
+  constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
   using E = Eight<T>;
-  for (long long i = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; (i & ~31LL) < items; i += stride) {
-    const long long per_row = blocks * 8, row = i < items ? i / per_row : 0;
-    const int col = (int)(i - row * per_row) * 16, n = i < items ? cols - col : 0;
-    uint32_t w[2][E::WORDS];
-    load8<T>(x + row * ld + col, min(8, max(0, n)), vec, w[0]);
-    load8<T>(x + row * ld + col + 8, min(8, max(0, n - 8)), vec, w[1]);
-    uint32_t a = 0;
+  wait_previous(x);
+  const int groups = groups_of(cols), per_row = blocks_of(cols) * 8;
+  const long long pitch = pitch_of(cols), items = rows * per_row, stride = (long long)gridDim.x * ROW_THREADS;
+  long long at = ((long long)blockIdx.x * ROW_THREADS + threadIdx.x) / per_row;
+  int piece = (int)((long long)blockIdx.x * ROW_THREADS + threadIdx.x - at * per_row);
+  for (long long i0 = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; (i0 & ~31LL) < items; i0 += AHEAD * stride) {
+    uint32_t w[AHEAD][2][E::WORDS];
+    long long row[AHEAD];
+    int col[AHEAD];
 #pragma unroll
-    for (int j = 0; j < E::WORDS; ++j) a = E::largest(a, E::largest(w[0][j] & E::ABS, w[1][j] & E::ABS));
-    a = of_word<T>(a);
-    const bool finite = __all_sync(~0u, a < E::INF);
-    a = as_fp32<T>(a);
-    if (!finite) {
-      a = 0;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) a = max(a, magnitude(E::get(w[k >> 3], k & 7)));
+    for (int u = 0; u < AHEAD; ++u) {
+      row[u] = at;
+      col[u] = piece * 16;
+      const int n = at < rows ? cols - col[u] : 0;
+      load8<T>(x + row[u] * ld + col[u], min(8, max(0, n)), vec, w[u][0]);
+      load8<T>(x + row[u] * ld + col[u] + 8, min(8, max(0, n - 8)), vec, w[u][1]);
+      at += step.rows;
+      piece += step.pieces;
+      if (piece >= per_row) { piece -= per_row; ++at; }
     }
-    a = max(a, __shfl_xor_sync(~0u, a, 1));
-    a = max(a, __shfl_xor_sync(~0u, a, 2));
-    a = max(a, __shfl_xor_sync(~0u, a, 4));
-    if (i >= items) continue;
-    const uint32_t byte = scale_byte(a);
-    const float inv = inverse(byte);
-    uint32_t o[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t* v = w[j >> 1];
-      const int k = 4 * (j & 1);
-      o[j] = four(E::get(v, k), E::get(v, k + 1), E::get(v, k + 2), E::get(v, k + 3), inv, finite);
+    for (int u = 0; u < AHEAD; ++u) {
+      uint32_t a = 0;
+#pragma unroll
+      for (int j = 0; j < E::WORDS; ++j) a = E::largest(a, E::largest(w[u][0][j], w[u][1][j]));
+      a = of_word<T>(a);
+      const bool finite = __all_sync(~0u, a < E::INF);
+      if (!finite) {
+        a = 0;
+#pragma unroll
+        for (int j = 0; j < E::WORDS; ++j) a = max(a, max(of_word<T>(finite_part<T>(w[u][0][j])), of_word<T>(finite_part<T>(w[u][1][j]))));
+      }
+      a = max(a, __shfl_xor_sync(~0u, a, 1));
+      a = max(a, __shfl_xor_sync(~0u, a, 2));
+      a = max(a, __shfl_xor_sync(~0u, a, 4));
+      if (row[u] >= rows) continue;
+      const uint32_t byte = scale_byte(as_fp32<T>(a));
+      const float inv = inverse(byte);
+      uint2 lo, hi;
+      if (finite) lo = eight<T, true>(w[u][0], inv), hi = eight<T, true>(w[u][1], inv);
+      else lo = eight<T, false>(w[u][0], inv), hi = eight<T, false>(w[u][1], inv);
+      *reinterpret_cast<uint4*>(q + row[u] * pitch + col[u]) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      if ((threadIdx.x & 7) == 0) scale[scale_at(row[u], col[u] / BLOCK, groups)] = (uint8_t)byte;
     }
-    *reinterpret_cast<uint4*>(q + row * pitch + col) = make_uint4(o[0], o[1], o[2], o[3]);
-    if ((threadIdx.x & 7) == 0) scale[scale_at(row, col / BLOCK, groups)] = (uint8_t)byte;
   }
 }
 
 // ---------------------------------------------------------------- along columns, or both
-constexpr int TILE = 128, TILE_THREADS = 256;
+constexpr int TILE = 128, TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32, ROWS = 8;
 
 // GELU: x is the gradient behind a GELU of z; what is kept is x gelu'(z), rounded to T.  q, scale: along the rows, or null.  sums: the columns'
 // sums over this tile's rows, [row tiles, cols], or null.
 template <typename T, bool GELU>
-__global__ void __launch_bounds__(TILE_THREADS, sizeof(T) == 2 ? 3 : 2)
+__global__ void __launch_bounds__(TILE_THREADS, sizeof(T) == 4 || GELU ? 2 : 3)
 quantize_tiles_kernel(const T* __restrict__ x, const long long ld, const T* __restrict__ z, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, uint8_t* __restrict__ qt,
                       uint8_t* __restrict__ scalet, float* __restrict__ sums, const int rows, const int cols, const bool vec) {
   using E = Eight<T>;
   constexpr int W = E::WORDS;
-  __shared__ __align__(16) uint32_t tops[8][16 * W];
-  __shared__ __align__(16) float part[8][TILE];
+  __shared__ __align__(16) uint32_t tops[TILE_WARPS][16 * W];
+  __shared__ __align__(16) float part[TILE_WARPS][TILE];
+  __shared__ __align__(16) float column_inv[TILE];
   __shared__ __align__(16) uint8_t turned[TILE * TILE];
   wait_previous(x, z);
   const int t = threadIdx.x, cg = t & 15, rg = t >> 4, warp = t >> 5;
   const int col_tiles = blocks_of(cols), cb = (int)(blockIdx.x % col_tiles), rb = (int)(blockIdx.x / col_tiles);
-  const int row0 = rb * TILE + rg * 8, col0 = cb * TILE + cg * 8, n = max(0, min(8, cols - col0));
-  uint32_t w[8][W];
+  const int row0 = rb * TILE + rg * ROWS, col0 = cb * TILE + cg * 8, n = max(0, min(8, cols - col0));
+  const bool whole = vec && (cb + 1) * TILE <= cols && (rb + 1) * TILE <= rows;      // no edge, no odd address
+  uint32_t w[ROWS][W];
+  const T* from = x + (long long)row0 * ld + col0;
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load8<T>(x + (long long)(row0 + i) * ld + col0, row0 + i < rows ? n : 0, vec, w[i]);
+    for (int i = 0; i < ROWS; ++i) load_whole<T>(from + i * ld, w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) load8<T>(from + i * ld, row0 + i < rows ? n : 0, vec, w[i]);
+  }
   if constexpr (GELU) {
+    const T* z0 = z + (long long)row0 * cols + col0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t u[W];
-      load8<T>(z + (long long)(row0 + i) * cols + col0, row0 + i < rows ? n : 0, vec, u);
+    for (int h = 0; h < ROWS; h += 4) {                   // z four rows at a time
+      uint32_t zs[4][W];
+      if (whole) {
 #pragma unroll
-      for (int k = 0; k < 8; k += 2) {
-        float d0, d1;
-        gelu_grad2(E::get(u, k), E::get(u, k + 1), &d0, &d1);
-        d0 *= E::get(w[i], k);
-        d1 *= E::get(w[i], k + 1);
-        if constexpr (sizeof(T) == 2) w[i][k >> 1] = E::pack(d0, d1);
-        else w[i][k] = __float_as_uint(d0), w[i][k + 1] = __float_as_uint(d1);
+        for (int i = 0; i < 4; ++i) load_whole<T>(z0 + (long long)(h + i) * cols, zs[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load8<T>(z0 + (long long)(h + i) * cols, row0 + h + i < rows ? n : 0, vec, zs[i]);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          uint32_t* v = w[h + i];
+          unsigned long long slope;
+          if constexpr (std::is_same_v<T, __nv_bfloat16>) {          // results of 8 bits: the quicker form (gelu.cuh)
+            slope = quick_gelu_slope2(attn_util::pack2(__float_as_uint(E::get(zs[i], k)), __float_as_uint(E::get(zs[i], k + 1))));
+          } else {
+            float s0, s1;
+            gelu_grad2(E::get(zs[i], k), E::get(zs[i], k + 1), &s0, &s1);
+            slope = attn_util::pack2(__float_as_uint(s0), __float_as_uint(s1));
+          }
+          float d0, d1;
+          attn_util::unpack2(attn_util::mul2(slope, attn_util::pack2(__float_as_uint(E::get(v, k)), __float_as_uint(E::get(v, k + 1)))), d0, d1);
+          if constexpr (sizeof(T) == 2) v[k >> 1] = E::pack(d0, d1);
+          else v[k] = __float_as_uint(d0), v[k + 1] = __float_as_uint(d1);
+        }
     }
   }
-  uint32_t top_row[8], top_col[W], all = 0;
+  uint32_t top_row[ROWS], top_col[W];
 #pragma unroll
   for (int j = 0; j < W; ++j) top_col[j] = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t a = 0;
+  for (int i = 0; i < ROWS; ++i) {
+    top_row[i] = 0;
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      const uint32_t m = w[i][j] & E::ABS;
-      a = E::largest(a, m);
-      top_col[j] = E::largest(top_col[j], m);
+      top_row[i] = E::largest(top_row[i], w[i][j]);
+      top_col[j] = E::largest(top_col[j], w[i][j]);
     }
-    top_row[i] = of_word<T>(a);
-    all = max(all, top_row[i]);
   }
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) all = max(all, top_row[i] = of_word<T>(top_row[i]));
   const bool finite = __syncthreads_and(all < E::INF);      // of the whole tile: both directions take the same elements
   if (!finite) {                                            // what is not finite has no say about the scales
 #pragma unroll
     for (int j = 0; j < W; ++j) top_col[j] = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       top_row[i] = 0;
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        uint32_t m = w[i][j] & E::ABS;
-        if (sizeof(T) == 2) m = ((m & 0xffffu) < E::INF ? m & 0xffffu : 0u) | ((m >> 16) < E::INF ? m & 0xffff0000u : 0u);
-        else m = m < E::INF ? m : 0u;
-        top_col[j] = E::largest(top_col[j], m);
-        top_row[i] = max(top_row[i], of_word<T>(m));
+        top_row[i] = max(top_row[i], of_word<T>(finite_part<T>(w[i][j])));
+        top_col[j] = E::largest(top_col[j], finite_part<T>(w[i][j]));
       }
     }
   }
@@ -209,7 +279,7 @@ quantize_tiles_kernel(const T* __restrict__ x, const long long ld, const T* __re
     for (int k = 0; k < 8; ++k) {
       s[k] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[k] += E::get(w[i], k);
+      for (int i = 0; i < ROWS; ++i) s[k] += E::get(w[i], k);
       s[k] += __shfl_xor_sync(~0u, s[k], 16);
     }
     if (!(t & 16)) {
@@ -224,57 +294,86 @@ quantize_tiles_kernel(const T* __restrict__ x, const long long ld, const T* __re
     for (int j = 0; j < W; j += 4) *reinterpret_cast<uint4*>(&tops[warp][cg * W + j]) = make_uint4(top_col[j], top_col[j + 1], top_col[j + 2], top_col[j + 3]);
   }
   if (q) {
-    const int groups = groups_of(cols);
+    // The 16 threads of a row exchange halves of their rows' maxima: lane cg is left with that of row cg / 2, whose scale it forms, and all take the
+    // eight scales from there.
+    uint32_t a[4];
+    const bool up8 = cg & 8, up4 = cg & 4, up2 = cg & 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = max(up8 ? top_row[4 + i] : top_row[i], __shfl_xor_sync(~0u, up8 ? top_row[i] : top_row[4 + i], 8));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) a[i] = max(up4 ? a[2 + i] : a[i], __shfl_xor_sync(~0u, up4 ? a[i] : a[2 + i], 4));
+    a[0] = max(up2 ? a[1] : a[0], __shfl_xor_sync(~0u, up2 ? a[0] : a[1], 2));
+    a[0] = max(a[0], __shfl_xor_sync(~0u, a[0], 1));
+    const uint32_t byte = scale_byte(as_fp32<T>(a[0]));
+    if (!(cg & 1)) scale[scale_at(row0 + (cg >> 1), cb, groups_of(cols))] = (uint8_t)byte;
     const long long pitch = pitch_of(cols);
+    uint8_t* to = q + row0 * pitch + col0;
+    float inv[ROWS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t a = top_row[i];
+    for (int i = 0; i < ROWS; ++i) inv[i] = inverse(__shfl_sync(~0u, byte, (t & 16) + 2 * i));
+    if (finite && whole) {
 #pragma unroll
-      for (int d = 1; d < 16; d *= 2) a = max(a, __shfl_xor_sync(~0u, a, d));
-      const uint32_t byte = scale_byte(as_fp32<T>(a));
-      const float inv = inverse(byte);
-      if (cg == 0) scale[scale_at(row0 + i, cb, groups)] = (uint8_t)byte;
-      if (row0 + i < rows)
-        *reinterpret_cast<uint2*>(q + (row0 + i) * pitch + col0) =
-            make_uint2(four(E::get(w[i], 0), E::get(w[i], 1), E::get(w[i], 2), E::get(w[i], 3), inv, finite),
-                       four(E::get(w[i], 4), E::get(w[i], 5), E::get(w[i], 6), E::get(w[i], 7), inv, finite));
+      for (int i = 0; i < ROWS; ++i) *reinterpret_cast<uint2*>(to + i * pitch) = eight<T, true>(w[i], inv[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (row0 + i < rows) *reinterpret_cast<uint2*>(to + i * pitch) = finite ? eight<T, true>(w[i], inv[i]) : eight<T, false>(w[i], inv[i]);
     }
   }
   __syncthreads();
+  // the columns' maxima over the warps, a word by each of the first threads, and their scales
+  if (t < 16 * W) {
+    uint32_t m = tops[0][t];
 #pragma unroll
-  for (int j = 0; j < W; j += 4) {
-    uint4 m = *reinterpret_cast<const uint4*>(&tops[0][cg * W + j]);
-#pragma unroll
-    for (int v = 1; v < 8; ++v) {
-      const uint4 u = *reinterpret_cast<const uint4*>(&tops[v][cg * W + j]);
-      m.x = E::largest(m.x, u.x), m.y = E::largest(m.y, u.y), m.z = E::largest(m.z, u.z), m.w = E::largest(m.w, u.w);
+    for (int v = 1; v < TILE_WARPS; ++v) m = E::largest(m, tops[v][t]);
+    m &= E::ABS;
+    const int c = sizeof(T) == 2 ? 2 * t : t;
+    uint8_t* to = scalet + scale_at(cb * TILE + c, rb, groups_of(rows));          // a column further: 16 bytes (an even column never ends a group of 32)
+    const uint32_t byte = scale_byte(as_fp32<T>(sizeof(T) == 2 ? m & 0xffffu : m));
+    to[0] = (uint8_t)byte;
+    column_inv[c] = inverse(byte);
+    if (sizeof(T) == 2) {
+      const uint32_t odd = scale_byte(as_fp32<T>(m >> 16));
+      to[16] = (uint8_t)odd;
+      column_inv[c + 1] = inverse(odd);
     }
-    top_col[j] = m.x, top_col[j + 1] = m.y, top_col[j + 2] = m.z, top_col[j + 3] = m.w;
   }
-  const int groups_t = groups_of(rows);
+  __syncthreads();
+  float inv[8];
+  *reinterpret_cast<float4*>(&inv[0]) = *reinterpret_cast<const float4*>(&column_inv[cg * 8]);
+  *reinterpret_cast<float4*>(&inv[4]) = *reinterpret_cast<const float4*>(&column_inv[cg * 8 + 4]);
+  // eight rows of column col0 + k; pieces of 8 bytes change places by the column's group, so that the 16 threads that store together hit all banks
+  uint8_t* to = &turned[cg * 8 * TILE + ((rg ^ cg) << 3)];
+  if (finite) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t a = sizeof(T) == 2 ? (top_col[k >> 1] >> (16 * (k & 1))) & 0xffffu : top_col[k & (W - 1)];
-    const uint32_t byte = scale_byte(as_fp32<T>(a));
-    const float inv = inverse(byte);
-    if (rg == 0) scalet[scale_at(col0 + k, rb, groups_t)] = (uint8_t)byte;
-    // eight rows of column col0 + k; pieces of 8 bytes change places by the column's group, so that the 16 threads that store together hit all banks
-    *reinterpret_cast<uint2*>(&turned[(cg * 8 + k) * TILE + ((rg ^ cg) << 3)]) =
-        make_uint2(four(E::get(w[0], k), E::get(w[1], k), E::get(w[2], k), E::get(w[3], k), inv, finite),
-                   four(E::get(w[4], k), E::get(w[5], k), E::get(w[6], k), E::get(w[7], k), inv, finite));
+    for (int k = 0; k < 8; ++k)
+      *reinterpret_cast<uint2*>(to + k * TILE) = make_uint2(four<true>(E::get(w[0], k), E::get(w[1], k), E::get(w[2], k), E::get(w[3], k), inv[k]),
+                                                            four<true>(E::get(w[4], k), E::get(w[5], k), E::get(w[6], k), E::get(w[7], k), inv[k]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      *reinterpret_cast<uint2*>(to + k * TILE) = make_uint2(four<false>(E::get(w[0], k), E::get(w[1], k), E::get(w[2], k), E::get(w[3], k), inv[k]),
+                                                            four<false>(E::get(w[4], k), E::get(w[5], k), E::get(w[6], k), E::get(w[7], k), inv[k]));
   }
   __syncthreads();
   const long long pitch_t = pitch_of(rows);
+  uint8_t* out = qt + (cb * TILE + (t >> 4)) * pitch_t + rb * TILE + (t & 15) * 8;
+  // column (t >> 4) + 16 j: its group is (t >> 7) + 2 j
+  const uint8_t* piece = &turned[(t >> 4) * TILE];
+  if (whole) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = (t >> 4) + 16 * j, ch = t & 15;
-    if (cb * TILE + c < cols)
-      *reinterpret_cast<uint2*>(qt + (cb * TILE + c) * pitch_t + rb * TILE + ch * 8) = *reinterpret_cast<const uint2*>(&turned[c * TILE + ((ch ^ (c >> 3)) << 3)]);
+    for (int j = 0; j < TILE / 16; ++j)
+      *reinterpret_cast<uint2*>(out + 16 * j * pitch_t) = *reinterpret_cast<const uint2*>(piece + 16 * j * TILE + (((t & 15) ^ ((t >> 7) + 2 * j)) << 3));
+  } else {
+#pragma unroll
+    for (int j = 0; j < TILE / 16; ++j)
+      if (cb * TILE + (t >> 4) + 16 * j < cols)
+        *reinterpret_cast<uint2*>(out + 16 * j * pitch_t) = *reinterpret_cast<const uint2*>(piece + 16 * j * TILE + (((t & 15) ^ ((t >> 7) + 2 * j)) << 3));
   }
   if (sums && t < TILE && cb * TILE + t < cols) {
     float s = 0.f;
 #pragma unroll
-    for (int v = 0; v < 8; ++v) s += part[v][t];
+    for (int v = 0; v < TILE_WARPS; ++v) s += part[v][t];
     sums[(size_t)rb * cols + cb * TILE + t] = s;
   }
 }
@@ -299,46 +398,61 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const float* __restric
 }
 
 // ---------------------------------------------------------------- back
+// 16 bytes of the result by each thread
 template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS) restore_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, T* __restrict__ x, const long long rows, const int cols,
-                                                              const bool vec) {
+                                                              const bool vec, const Stride step) {
+  constexpr int PER = 16 / sizeof(T), AHEAD = 4;
   wait_previous(q, scale);
-  const int blocks = blocks_of(cols), groups = groups_of(cols);
-  const long long pitch = pitch_of(cols), items = rows * blocks * 8, stride = (long long)gridDim.x * ROW_THREADS;
-  for (long long i = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; i < items; i += stride) {
-    const long long row = i / (blocks * 8);
-    const int col = (int)(i - row * (blocks * 8)) * 16, n = cols - col;
-    if (n <= 0) continue;
-    const uint4 u = *reinterpret_cast<const uint4*>(q + row * pitch + col);
-    const float s = value(scale[scale_at(row, col / BLOCK, groups)]);
-    float f[2][8];
-    act8::unpack8(make_uint2(u.x, u.y), s, f[0]);
-    act8::unpack8(make_uint2(u.z, u.w), s, f[1]);
-    T* p = x + row * cols + col;
-    if (vec && n >= 16) {
-      constexpr int V = 16 / sizeof(T);
+  const int groups = groups_of(cols), per_row = (cols + PER - 1) / PER;
+  const long long pitch = pitch_of(cols), items = rows * per_row, stride = (long long)gridDim.x * ROW_THREADS;
+  long long at = ((long long)blockIdx.x * ROW_THREADS + threadIdx.x) / per_row;
+  int piece = (int)((long long)blockIdx.x * ROW_THREADS + threadIdx.x - at * per_row);
+  for (long long i0 = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; i0 < items; i0 += AHEAD * stride) {
+    uint2 u[AHEAD];
+    uint32_t s[AHEAD];
+    long long row[AHEAD];
+    int col[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 16 / V; ++j) {
-        Pack<T, V> a;
+    for (int a = 0; a < AHEAD; ++a) {
+      const long long i = i0 + a * stride;
+      row[a] = i < items ? at : 0;
+      col[a] = i < items ? piece * PER : 0;
+      at += step.rows;
+      piece += step.pieces;
+      if (piece >= per_row) { piece -= per_row; ++at; }
+      const uint8_t* p = q + row[a] * pitch + col[a];
+      u[a] = PER == 8 ? *reinterpret_cast<const uint2*>(p) : make_uint2(*reinterpret_cast<const uint32_t*>(p), 0u);
+      s[a] = scale[scale_at(row[a], col[a] / BLOCK, groups)];
+    }
 #pragma unroll
-        for (int k = 0; k < V; ++k) a.v[k] = from_acc<T>((typename AccOf<T>::type)f[(j * V + k) >> 3][(j * V + k) & 7]);
-        st_pack<T, V>(p + j * V, a);
+    for (int a = 0; a < AHEAD; ++a) {
+      if (i0 + a * stride >= items) break;
+      float f[8];
+      act8::unpack8(u[a], value(s[a]), f);
+      T* p = x + row[a] * cols + col[a];
+      const int n = cols - col[a];
+      if (vec && n >= PER) {
+        Pack<T, PER> o;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) o.v[k] = from_acc<T>((typename AccOf<T>::type)f[k]);
+        st_pack<T, PER>(p, o);
+      } else {
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+          if (k < n) p[k] = from_acc<T>((typename AccOf<T>::type)f[k]);
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (k < n) p[k] = from_acc<T>((typename AccOf<T>::type)f[k >> 3][k & 7]);
     }
   }
 }
 
 // ---------------------------------------------------------------- a few tokens
 // y = x w^T (+ bias, GELU) for up to 32 rows of x and weights in 8 bits, in one launch: bound by reading the weights and by latency.  A block takes
-// 16 weight rows, its eight warps the blocks of K in turn, so that no warp waits for another before the last sum.  A warp
+// 16 weight rows, its warps (up to 16) the blocks of K in turn, so that no warp waits for another before the last sum.  A warp
 // quantizes the tokens' blocks itself, straight into the operand registers of mma.sync (16 weight rows x 8 tokens x 32 of K): which K
 // index stands where is free as long as both operands agree, so a thread's 32 bytes of a weight row are the 32 consecutive ones of its quarter of the
-// block, and so are the tokens'.  The sums of a block are scaled into fp32 sums.
-constexpr int FEW_ROWS = 16, FEW_WARPS = 8, FEW_AHEAD = 4;
+// block, and so are the tokens'.  The sums of a block are scaled into fp32 sums.  The next block's weights are under way meanwhile.
+constexpr int FEW_ROWS = 16, FEW_WARPS = 16;
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -356,73 +470,71 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict
   using E = Eight<T>;
   __shared__ float part[FEW_WARPS][FEW_ROWS][NT * 8 + 1];
   wait_previous(x, q, scale, bias);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
   const int blocks = blocks_of(K), groups = groups_of(K), n0 = blockIdx.x * FEW_ROWS;
   const long long pitch = pitch_of(K);
   const int r0 = min(n0 + g, N - 1), r1 = min(n0 + g + 8, N - 1);
   const uint8_t *w0 = q + r0 * pitch + t * 32, *w1 = q + r1 * pitch + t * 32;
+  uint4 next[4];
+  uint32_t next_scale[2];
+  auto fetch = [&](int b) {
+    next[0] = __ldg(reinterpret_cast<const uint4*>(w0 + b * BLOCK));
+    next[1] = __ldg(reinterpret_cast<const uint4*>(w0 + b * BLOCK + 16));
+    next[2] = __ldg(reinterpret_cast<const uint4*>(w1 + b * BLOCK));
+    next[3] = __ldg(reinterpret_cast<const uint4*>(w1 + b * BLOCK + 16));
+    next_scale[0] = scale[scale_at(r0, b, groups)];
+    next_scale[1] = scale[scale_at(r1, b, groups)];
+  };
+  if (warp < blocks) fetch(warp);
   float acc[NT][4];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[i][k] = 0.f;
-  for (int b0 = warp; b0 < blocks; b0 += FEW_WARPS * FEW_AHEAD) {
-    uint4 a[FEW_AHEAD][4];
-    uint32_t sw[FEW_AHEAD][2];
+#pragma unroll 1
+  for (int b = warp; b < blocks; b += warps) {
+    const int col = b * BLOCK + t * 32;
+    uint32_t v[NT][4][E::WORDS];
 #pragma unroll
-    for (int u = 0; u < FEW_AHEAD; ++u) {
-      const int b = b0 + u * FEW_WARPS;
-      if (b < blocks) {
-        a[u][0] = __ldg(reinterpret_cast<const uint4*>(w0 + b * BLOCK));
-        a[u][1] = __ldg(reinterpret_cast<const uint4*>(w0 + b * BLOCK + 16));
-        a[u][2] = __ldg(reinterpret_cast<const uint4*>(w1 + b * BLOCK));
-        a[u][3] = __ldg(reinterpret_cast<const uint4*>(w1 + b * BLOCK + 16));
-        sw[u][0] = scale[scale_at(r0, b, groups)];
-        sw[u][1] = scale[scale_at(r1, b, groups)];
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        load8<T>(x + (long long)(i * 8 + g) * ld + col + 8 * j, i * 8 + g < tokens ? min(8, max(0, K - col - 8 * j)) : 0, vec, v[i][j]);
+    const uint4 a[4] = {next[0], next[1], next[2], next[3]};
+    const uint32_t sw[2] = {next_scale[0], next_scale[1]};
+    if (b + warps < blocks) fetch(b + warps);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (i * 8 >= tokens) break;
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < E::WORDS; ++k) top = E::largest(top, v[i][j][k]);
+      top = of_word<T>(top);
+      const bool finite = __all_sync(~0u, top < E::INF);
+      if (!finite) {
+        top = 0;
+#pragma unroll
+        for (int k = 0; k < 4 * E::WORDS; ++k) top = max(top, of_word<T>(finite_part<T>(v[i][k / E::WORDS][k % E::WORDS])));
       }
-    }
+      top = max(top, __shfl_xor_sync(~0u, top, 1));
+      top = max(top, __shfl_xor_sync(~0u, top, 2));
+      const uint32_t sx = scale_byte(as_fp32<T>(top));
+      const float inv = inverse(sx);
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < FEW_AHEAD; ++u) {
-      const int b = b0 + u * FEW_WARPS;
-      if (b >= blocks) break;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        if (i * 8 >= tokens) break;
-        const int token = i * 8 + g, col = b * BLOCK + t * 32;
-        uint32_t v[4][E::WORDS], top = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          load8<T>(x + (long long)token * ld + col + 8 * j, token < tokens ? min(8, max(0, K - col - 8 * j)) : 0, vec, v[j]);
-#pragma unroll
-          for (int k = 0; k < E::WORDS; ++k) top = E::largest(top, v[j][k] & E::ABS);
-        }
-        top = of_word<T>(top);
-        const bool finite = __all_sync(~0u, top < E::INF);
-        top = as_fp32<T>(top);
-        if (!finite) {
-          top = 0;
-#pragma unroll
-          for (int k = 0; k < 32; ++k) top = max(top, magnitude(E::get(v[k >> 3], k & 7)));
-        }
-        top = max(top, __shfl_xor_sync(~0u, top, 1));
-        top = max(top, __shfl_xor_sync(~0u, top, 2));
-        const uint32_t sx = scale_byte(top);
-        const float inv = inverse(sx);
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {                    // 8 of the thread's 32 bytes for each of the four instructions
-          const uint32_t x0 = four(E::get(v[j], 0), E::get(v[j], 1), E::get(v[j], 2), E::get(v[j], 3), inv, finite);
-          const uint32_t x1 = four(E::get(v[j], 4), E::get(v[j], 5), E::get(v[j], 6), E::get(v[j], 7), inv, finite);
-          const uint4 p = a[u][j >> 1], r = a[u][2 + (j >> 1)];
-          if (j & 1) mma_e4m3(c, p.z, r.z, p.w, r.w, x0, x1);
-          else mma_e4m3(c, p.x, r.x, p.y, r.y, x0, x1);
-        }
-        const uint32_t s0 = __shfl_sync(~0u, sx, 8 * t), s1 = __shfl_sync(~0u, sx, 8 * t + 4);      // of the tokens 2 t and 2 t + 1
-        acc[i][0] += scaled(c[0], sw[u][0], s0);
-        acc[i][1] += scaled(c[1], sw[u][0], s1);
-        acc[i][2] += scaled(c[2], sw[u][1], s0);
-        acc[i][3] += scaled(c[3], sw[u][1], s1);
+      for (int j = 0; j < 4; ++j) {                    // 8 of the thread's 32 bytes for each of the four instructions
+        const uint2 xq = finite ? eight<T, true>(v[i][j], inv) : eight<T, false>(v[i][j], inv);
+        const uint4 p = a[j >> 1], r = a[2 + (j >> 1)];
+        if (j & 1) mma_e4m3(c, p.z, r.z, p.w, r.w, xq.x, xq.y);
+        else mma_e4m3(c, p.x, r.x, p.y, r.y, xq.x, xq.y);
       }
+      const uint32_t s0 = __shfl_sync(~0u, sx, 8 * t), s1 = __shfl_sync(~0u, sx, 8 * t + 4);      // of the tokens 2 t and 2 t + 1
+      acc[i][0] += scaled(c[0], sw[0], s0);
+      acc[i][1] += scaled(c[1], sw[0], s1);
+      acc[i][2] += scaled(c[2], sw[1], s0);
+      acc[i][3] += scaled(c[3], sw[1], s1);
     }
   }
 #pragma unroll
@@ -433,12 +545,11 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict
     part[warp][g + 8][i * 8 + 2 * t + 1] = acc[i][3];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < FEW_ROWS * NT * 8; i += FEW_WARPS * 32) {
+  for (int i = threadIdx.x; i < FEW_ROWS * tokens; i += blockDim.x) {
     const int r = i & (FEW_ROWS - 1), token = i / FEW_ROWS;
-    if (token >= tokens || n0 + r >= N) continue;
+    if (n0 + r >= N) continue;
     float s = 0.f;
-#pragma unroll
-    for (int v = 0; v < FEW_WARPS; ++v) s += part[v][r][token];
+    for (int v = 0; v < warps; ++v) s += part[v][r][token];
     if (bias) s += (float)to_acc<T>(bias[n0 + r]);
     T out = from_acc<T>((typename AccOf<T>::type)s);
     if (gelu) {
@@ -462,8 +573,11 @@ static int by_type(int dtype, const char* what, F f) {
   return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
 }
 static bool whole_pieces(std::initializer_list<const void*> p, int64_t ld, int es) { return all_aligned16(p) && ld * es % 16 == 0; }
-static int row_grid(int64_t rows, int cols) {
-  return (int)std::min<int64_t>((rows * blocks_of(cols) * 8 + ROW_THREADS - 1) / ROW_THREADS, 148 * 8);
+// A launch for rows of `per_row` pieces, `ahead` of them by each thread at a time, in at most `most` blocks.
+struct RowLaunch { int blocks; Stride step; };
+static RowLaunch row_launch(int64_t rows, int per_row, int ahead, int most) {
+  const int blocks = (int)std::min<int64_t>((rows * per_row + ahead * ROW_THREADS - 1) / (ahead * ROW_THREADS), most);
+  return {blocks, {(int)((int64_t)blocks * ROW_THREADS / per_row), (int)((int64_t)blocks * ROW_THREADS % per_row)}};
 }
 static int checked(int64_t rows, int64_t cols, const char* what) {
   if (rows < 0 || cols < 1 || rows > (int64_t)1 << 30 || cols > (int64_t)1 << 30) return fail(TMPI_ERR_INVALID, "%s: %lld rows of %lld", what, (long long)rows, (long long)cols);
@@ -494,9 +608,11 @@ int tmpi_fp8_quantize(const void* x, int64_t ld, const void* z, void* q, void* s
   return fp8::by_type(dtype, "fp8_quantize", [&](auto* type) -> cudaError_t {
     using T = std::remove_pointer_t<decltype(type)>;
     const bool vec = fp8::whole_pieces({x, z}, ld, sizeof(T)) && (!z || cols * sizeof(T) % 16 == 0);
-    if (!qt)
-      return launch_overlapped(fp8::quantize_rows_kernel<T>, fp8::row_grid(rows, (int)cols), fp8::ROW_THREADS, 0, s, (const T*)x, (long long)ld, (uint8_t*)q, (uint8_t*)scale,
-                               (long long)rows, (int)cols, vec);
+    if (!qt) {
+      const fp8::RowLaunch l = fp8::row_launch(rows, fp8::blocks_of(cols) * 8, sizeof(T) == 2 ? 2 : 1, 148 * 8);
+      return launch_overlapped(fp8::quantize_rows_kernel<T>, l.blocks, fp8::ROW_THREADS, 0, s, (const T*)x, (long long)ld, (uint8_t*)q, (uint8_t*)scale, (long long)rows, (int)cols, vec,
+                               l.step);
+    }
     const long long tiles = (long long)fp8::blocks_of(rows) * fp8::blocks_of(cols);
     if (tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_overlapped(z ? fp8::quantize_tiles_kernel<T, true> : fp8::quantize_tiles_kernel<T, false>, (unsigned)tiles, fp8::TILE_THREADS, 0, s, (const T*)x, (long long)ld,
@@ -519,8 +635,9 @@ int tmpi_fp8_restore(const void* q, const void* scale, void* x, int64_t rows, in
   if (!all_aligned16({q})) return fail(TMPI_ERR_INVALID, "fp8_restore: the 8-bit numbers must be 16-byte aligned");
   return fp8::by_type(dtype, "fp8_restore", [&](auto* type) -> cudaError_t {
     using T = std::remove_pointer_t<decltype(type)>;
-    return launch_overlapped(fp8::restore_kernel<T>, fp8::row_grid(rows, (int)cols), fp8::ROW_THREADS, 0, (cudaStream_t)stream, (const uint8_t*)q, (const uint8_t*)scale, (T*)x,
-                             (long long)rows, (int)cols, fp8::whole_pieces({x}, cols, sizeof(T)));
+    const fp8::RowLaunch l = fp8::row_launch(rows, (int)((cols * sizeof(T) + 15) / 16), 4, 1 << 20);
+    return launch_overlapped(fp8::restore_kernel<T>, l.blocks, fp8::ROW_THREADS, 0, (cudaStream_t)stream, (const uint8_t*)q, (const uint8_t*)scale, (T*)x, (long long)rows, (int)cols,
+                             fp8::whole_pieces({x}, cols, sizeof(T)), l.step);
   });
 }
 
@@ -532,7 +649,7 @@ int tmpi_fp8_few(const void* x, int64_t ld, const void* q, const void* scale, co
   return fp8::by_type(dtype, "fp8_few", [&](auto* type) -> cudaError_t {
     using T = std::remove_pointer_t<decltype(type)>;
     const auto kernel = tokens <= 8 ? fp8::few_kernel<T, 1> : tokens <= 16 ? fp8::few_kernel<T, 2> : fp8::few_kernel<T, 4>;
-    return launch_overlapped(kernel, (N + fp8::FEW_ROWS - 1) / fp8::FEW_ROWS, fp8::FEW_WARPS * 32, 0, (cudaStream_t)stream, (const T*)x, (long long)ld, (const uint8_t*)q,
+    return launch_overlapped(kernel, (N + fp8::FEW_ROWS - 1) / fp8::FEW_ROWS, 32 * std::min(fp8::FEW_WARPS, fp8::blocks_of(K)), 0, (cudaStream_t)stream, (const T*)x, (long long)ld, (const uint8_t*)q,
                              (const uint8_t*)scale, (const T*)bias, (T*)y, tokens, N, K, gelu, fp8::whole_pieces({x}, ld, sizeof(T)));
   });
 }

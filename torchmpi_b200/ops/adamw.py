@@ -5,7 +5,7 @@
     g = gradient * grad_scale * min(1, max_norm / (norm + 1e-6));   m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2
     w = (1 - lr * weight_decay) w - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
-in fp32.  Parameters of 16 bits have fp32 masters (``master_weights=True``) that the step goes by and whose rounding the parameter becomes; without, the
+in fp32 (an element that never had a gradient stays, also with ``eps = 0``; with 8 bits ``eps`` counts as 1e-18 at least).  Parameters of 16 bits have fp32 masters (``master_weights=True``) that the step goes by and whose rounding the parameter becomes; without, the
 parameter itself is updated and rounded.  ``bits=8`` keeps ``m`` and the root of ``v`` as a byte an element with an fp32 scale for 128 (4.1 bytes an element
 less to read and to write than the 8 of 32 bits, each way): ``m = sign(c) c^2 top / 127^2``, ``sqrt(v) = c^2 top / 255^2``, where ``top`` is the block's
 largest magnitude; a root that is not zero never becomes zero.  An average that changes by less than half a code in a step, its block's largest
@@ -211,7 +211,7 @@ class AdamW:
             m, v = self.moments(p)
             g = p.grad.float() * scale
             m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
-            w = (1 - rate * decay) * w - rate / (1 - b1 ** t) * m / (torch.sqrt(v) / math.sqrt(1 - b2 ** t) + eps)
+            w = (1 - rate * decay) * w - rate / (1 - b1 ** t) * m / (torch.sqrt(v) / math.sqrt(1 - b2 ** t) + max(eps, 1e-37 if self.bits == 32 else 1e-18))
             if "master" in st:
                 st["master"].copy_(w)
             p.copy_(w)
