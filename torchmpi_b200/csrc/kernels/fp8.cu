@@ -231,7 +231,7 @@ quantize_tiles_kernel(const T* __restrict__ x, const long long ld, const T* __re
           uint32_t* v = w[h + i];
           unsigned long long slope;
           if constexpr (std::is_same_v<T, __nv_bfloat16>) {          // results of 8 bits: the quicker form (gelu.cuh)
-            slope = quick_gelu_slope2(attn_util::pack2(__float_as_uint(E::get(zs[i], k)), __float_as_uint(E::get(zs[i], k + 1))));
+            slope = shared_gelu_slope2(attn_util::pack2(__float_as_uint(E::get(zs[i], k)), __float_as_uint(E::get(zs[i], k + 1))));
           } else {
             float s0, s1;
             gelu_grad2(E::get(zs[i], k), E::get(zs[i], k + 1), &s0, &s1);

@@ -79,23 +79,30 @@ __device__ __forceinline__ unsigned long long quick_cdf2(unsigned long long z, u
   unpack2(add2(pack2(__float_as_uint(ex2(x0)), __float_as_uint(ex2(x1))), both(1.f)), x0, x1);
   return pack2(__float_as_uint(rcp(x0)), __float_as_uint(rcp(x1)));
 }
-// The slope alone, and with one reciprocal for two elements: 1 / a = b / (a b), 1 / b = a / (a b).  The exponents stop at 60 for that (Phi below 2^-60 is as good as 0).
-__device__ __forceinline__ unsigned long long quick_gelu_slope2(unsigned long long z) {
+// The same with one reciprocal for two elements: 1 / a = b / (a b), 1 / b = a / (a b).  The exponents stop at 60 for that (Phi below 2^-60 is as good as 0).
+// For kernels that the special-function unit bounds.
+__device__ __forceinline__ unsigned long long shared_cdf2(unsigned long long z, unsigned long long t) {      // t = z^2
   using namespace attn_util;
   auto both = [](float v) { return attn_util::pack2(__float_as_uint(v), __float_as_uint(v)); };
-  const unsigned long long t = mul2(z, z);
   unsigned long long p = fma2(both(-3.29422556e-09f), t, both(2.84630659e-07f));
   p = fma2(p, t, both(-9.59334011e-06f));
   p = fma2(p, t, both(0.00014446408f));
   p = fma2(p, t, both(0.000148453692f));
   p = fma2(p, t, both(-0.104912885f));
   p = mul2(fma2(p, t, both(-2.30217791f)), z);
-  float x0, x1, g0, g1;
+  float x0, x1;
   unpack2(p, x0, x1);
   unpack2(add2(pack2(__float_as_uint(ex2(fminf(x0, 60.f))), __float_as_uint(ex2(fminf(x1, 60.f)))), both(1.f)), x0, x1);
-  const float r = rcp(x0 * x1);
-  unpack2(mul2(t, both(-0.5f * 1.4426950408889634f)), g0, g1);
-  return fma2(mul2(z, both(0.3989422804014327f)), pack2(__float_as_uint(ex2(g0)), __float_as_uint(ex2(g1))), mul2(both(r), pack2(__float_as_uint(x1), __float_as_uint(x0))));
+  return mul2(both(rcp(x0 * x1)), pack2(__float_as_uint(x1), __float_as_uint(x0)));
+}
+__device__ __forceinline__ unsigned long long shared_gelu2(unsigned long long z) { return attn_util::mul2(z, shared_cdf2(z, attn_util::mul2(z, z))); }
+__device__ __forceinline__ unsigned long long shared_gelu_slope2(unsigned long long z) {
+  using namespace attn_util;
+  auto both = [](float v) { return attn_util::pack2(__float_as_uint(v), __float_as_uint(v)); };
+  const unsigned long long t = mul2(z, z);
+  float x0, x1;
+  unpack2(fma2(t, both(-0.5f * 1.4426950408889634f), both(-1.3257480647361593f)), x0, x1);          // log2 of the density: log2(0.39894228) = -1.32574806
+  return fma2(z, pack2(__float_as_uint(ex2(x0)), __float_as_uint(ex2(x1))), shared_cdf2(z, t));
 }
 __device__ __forceinline__ unsigned long long quick_gelu2(unsigned long long z) { return attn_util::mul2(z, quick_cdf2(z, attn_util::mul2(z, z))); }
 __device__ __forceinline__ void quick_gelu_both2(unsigned long long z, unsigned long long* y, unsigned long long* slope) {

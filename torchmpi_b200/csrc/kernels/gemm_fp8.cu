@@ -23,6 +23,7 @@
 #include "../runtime/common.h"
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 namespace tmpi {
 
@@ -36,18 +37,22 @@ namespace gemm8 {
 constexpr int BM = 128, BN = 256, BK = 128, UMMA_K = 32;
 constexpr int A_BYTES = BM * BK, B_BYTES = BN / 2 * BK, STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int SF_BYTES = fp8::TILE_BYTES, SF_STAGE = 3 * SF_BYTES;          // 128 rows of A, up to 256 of B
-constexpr int STAGING_TILE = BM * 128;                                      // 128 rows of 128 bytes
-constexpr int GROUPS = 2, THREADS = 64 + GROUPS * 128;
+constexpr int COLS = 32;                                                    // of a slice of the epilogue
 constexpr int TMEM_COLS = 512, SHARED_COLS = 64, ACC1 = BN - SHARED_COLS, SF_COL = ACC1 + BN, SF_SET = 12;
+constexpr int FIRST = SHARED_COLS / COLS;                                   // slices in the columns that the accumulators share
 constexpr unsigned long long kWaitBudgetNs = 4000000000ull;
 
 enum { PLAIN = 0, WITH_GELU = 1, GELU_AND_Z = 2 };
 
-template <int MODE> struct Layout {
+template <typename T, int MODE> struct Layout {
   static constexpr int OUTPUTS = MODE == GELU_AND_Z ? 2 : 1;
-  static constexpr int STAGES = MODE == GELU_AND_Z ? 4 : 5;
-  static constexpr size_t SF_AT = (size_t)STAGES * STAGE_BYTES, STAGING_AT = SF_AT + (size_t)STAGES * SF_STAGE + (STAGES * SF_STAGE % 1024 ? 1024 - STAGES * SF_STAGE % 1024 : 0);
-  static constexpr size_t SHARED_AT = STAGING_AT + (size_t)OUTPUTS * GROUPS * STAGING_TILE;
+  static constexpr int GROUPS = sizeof(T) == 4 && MODE == GELU_AND_Z ? 2 : 4;      // of four epilogue warps
+  static constexpr int THREADS = 64 + GROUPS * 128;
+  static constexpr int TILE = 32 * COLS * sizeof(T);                               // staging of a warp and output
+  static constexpr size_t STAGING = (size_t)OUTPUTS * GROUPS * 4 * TILE;
+  static constexpr int STAGES = STAGING > 32768 ? 4 : 5;
+  static constexpr size_t SF_AT = (size_t)STAGES * STAGE_BYTES, STAGING_AT = (SF_AT + (size_t)STAGES * SF_STAGE + 1023) / 1024 * 1024;
+  static constexpr size_t SHARED_AT = STAGING_AT + STAGING;
   static constexpr size_t BYTES = SHARED_AT + 256 + 1024;
   static_assert(BYTES <= 232448, "shared memory of one CTA");
 };
@@ -178,8 +183,6 @@ __device__ __forceinline__ void issuer(Shared* sh, unsigned char* tiles, unsigne
   }
 }
 
-__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
-
 template <typename T> __device__ __forceinline__ uint32_t two(float a, float b);
 template <> __device__ __forceinline__ uint32_t two<__nv_bfloat16>(float a, float b) { return attn_util::pack_bf16(__float_as_uint(a), __float_as_uint(b)); }
 template <> __device__ __forceinline__ uint32_t two<__half>(float a, float b) {
@@ -190,40 +193,45 @@ template <typename T> __device__ __forceinline__ float2 untwo(uint32_t w);
 template <> __device__ __forceinline__ float2 untwo<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 untwo<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// Two groups of four warps in each CTA take the tile's slices of 128 bytes of a row in turn, each through a staging tile of its own.
+// gelu of two rounded values, in a word of them
+template <typename T>
+__device__ __forceinline__ uint32_t gelu_word(uint32_t w) {
+  const float2 f = untwo<T>(w);
+  float y0, y1;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {          // results of 8 bits: the quicker form (gelu.cuh)
+    attn_util::unpack2(shared_gelu2(attn_util::pack2(__float_as_uint(f.x), __float_as_uint(f.y))), y0, y1);
+  } else {
+    gelu_value2(f.x, f.y, &y0, &y1);
+  }
+  return two<T>(y0, y1);
+}
+
+// Four (two) groups of four warps in each CTA take the tile's slices of 32 columns in turn.  A warp has 32 rows of a slice: it stages them in shared memory and
+// stores them through the TMA unit by itself, so that the warps meet nowhere.
 template <typename T, int MODE>
 __device__ __forceinline__ void epilogue(Shared* sh, unsigned char* staging, const Problem& p, const T* bias, int group, int quarter, int lane, uint32_t rank, int cluster, int clusters,
                                          const CUtensorMap* map_c, const CUtensorMap* map_z) {
-  constexpr int COLS = 128 / sizeof(T), WORDS = 32;
-  constexpr int FIRST = COLS == SHARED_COLS ? 1 : GROUPS;          // groups whose first slice lies in the shared columns
-  const int row = quarter * 32 + lane;
-  const bool leader = quarter == 0 && lane == 0, overlap = p.bn == BN;
+  using L = Layout<T, MODE>;
+  constexpr int WORDS = COLS * sizeof(T) / 4, ROW = COLS * sizeof(T), PIECES = ROW / 16;
+  const bool overlap = p.bn == BN;
   const int parts = p.bn / COLS;
-  T *c_out = (T*)p.c, *z_out = (T*)p.z;
+  unsigned char* stg = staging + (size_t)(group * 4 + quarter) * L::OUTPUTS * L::TILE;
+  const int swizzle = ROW == 128 ? lane & 7 : (lane >> 1) & 3;
   Item it;
   int n = 0;
   for (int t = cluster; item_of(p, t, &it); t += clusters, ++n) {
     const int acc = n & 1;
-    const uint32_t ok = sm100::mbar_wait(&sh->acc_full[acc], (n >> 1) & 1, kWaitBudgetNs, &sh->error);
-    uint32_t all_ok;                    // the group meets at named barriers below: it goes on, or leaves, together
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-                 : "=r"(all_ok) : "r"(ok), "r"(1 + group) : "memory");
-    if (!all_ok) { give_up(sh, p, 5); break; }
+    if (!sm100::mbar_wait_warp(&sh->acc_full[acc], (n >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p, 5); break; }
     sm100::tc_fence_after();
-    const int row0 = (it.m_tile * 2 + (int)rank) * BM, out0 = row0 + it.slice * p.slice_rows;
+    const int row0 = (it.m_tile * 2 + (int)rank) * BM + quarter * 32, out0 = row0 + it.slice * p.slice_rows;
     const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (acc ? (overlap ? ACC1 : BN / 2) : 0);
 #pragma unroll 1
-    for (int i = group; i < parts; i += GROUPS) {
+    for (int i = group; i < parts; i += L::GROUPS) {
       const int c0 = (overlap && !acc ? parts - 1 - i : i) * COLS, col0 = it.n_tile * p.bn + c0;
+      const bool inside = col0 < p.N && row0 < p.M;              // the same in all lanes
       uint32_t r[COLS], w[WORDS];
-      const bool inside = col0 < p.N;   // the same in all threads of the group
       if (inside) {
-        if constexpr (COLS == 64) {
-          sm100::tmem_ld_32x32(t_base + c0, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-          sm100::tmem_ld_32x32(t_base + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-        } else {
-          sm100::tmem_ld_32x32(t_base + c0, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-        }
+        sm100::tmem_ld_32x32(t_base + c0, r);
         sm100::tmem_ld_wait();
       }
       if (overlap && i < FIRST) {       // the columns that the next tile shares have been read
@@ -236,7 +244,7 @@ __device__ __forceinline__ void epilogue(Shared* sh, unsigned char* staging, con
       if (bias) {
         if (col0 + COLS <= p.N && ((uintptr_t)bias & 15) == 0) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < PIECES; ++j) {
             const uint4 u = __ldg(reinterpret_cast<const uint4*>(bias + col0) + j);
             const uint32_t b[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -256,75 +264,68 @@ __device__ __forceinline__ void epilogue(Shared* sh, unsigned char* staging, con
             if (col0 + j < p.N) v[j] += (float)to_acc<T>(bias[col0 + j]);
         }
       }
-      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int j = 0; j < WORDS; ++j) w[j] = two<T>(v[2 * j], v[2 * j + 1]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < WORDS; ++j) w[j] = r[j];
+      for (int j = 0; j < WORDS; ++j) {
+        if constexpr (sizeof(T) == 2) w[j] = two<T>(v[2 * j], v[2 * j + 1]);
+        else w[j] = r[j];
       }
-      auto put = [&](const CUtensorMap* map, T* out, int which) {
-        unsigned char* stg = staging + (which * GROUPS + group) * STAGING_TILE;
-        if (leader) {                   // the store that used this staging tile before must have read it
-          if (MODE == GELU_AND_Z) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        }
-        group_sync(group);
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the stores before have read the staging
+      __syncwarp();
+      auto put = [&](int which) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          *reinterpret_cast<uint4*>(stg + row * 128 + ((u ^ (row & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
-        if (p.by_tma) {
-          sm100::fence_proxy_async_smem();
-          group_sync(group);
-          if (leader && row0 < p.M) sm100::tma_store_2d(map, stg, col0, out0);
-          if (leader) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        } else {                        // rows that start anywhere: a warp writes its 32 rows, consecutive elements by consecutive lanes
-          __syncwarp();
-#pragma unroll 1
-          for (int j = 0; j < 32; ++j) {
-            const int rr = quarter * 32 + j;
-            if (row0 + rr >= p.M) break;
-#pragma unroll
-            for (int e = lane; e < COLS; e += 32)
-              if (col0 + e < p.N) {
-                const int at = e * (int)sizeof(T);
-                out[(long long)(row0 + rr) * p.N + col0 + e] = *reinterpret_cast<const T*>(stg + rr * 128 + (((at >> 4) ^ (rr & 7)) << 4) + (at & 15));
-              }
-          }
-          __syncwarp();
-        }
+        for (int u = 0; u < PIECES; ++u)
+          *reinterpret_cast<uint4*>(stg + which * L::TILE + lane * ROW + ((u ^ swizzle) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
       };
-      if (MODE == PLAIN || MODE == GELU_AND_Z) put(MODE == PLAIN ? map_c : map_z, MODE == PLAIN ? c_out : z_out, 0);
+      if (MODE != WITH_GELU) put(0);
       if (MODE != PLAIN) {              // the GELU of what is rounded
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int j = 0; j < WORDS; ++j) {
-          if constexpr (sizeof(T) == 2) {
-            const float2 f = untwo<T>(w[j]);
-            float y0, y1;
-            gelu_value2(f.x, f.y, &y0, &y1);
-            w[j] = two<T>(y0, y1);
-          } else if (j % 2 == 0) {
+          for (int j = 0; j < WORDS; ++j) w[j] = gelu_word<T>(w[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < WORDS; j += 2) {
             float y0, y1;
             gelu_value2(__uint_as_float(w[j]), __uint_as_float(w[j + 1]), &y0, &y1);
             w[j] = __float_as_uint(y0);
             w[j + 1] = __float_as_uint(y1);
           }
         }
-        put(map_c, c_out, MODE == GELU_AND_Z ? 1 : 0);
+        put(MODE == GELU_AND_Z ? 1 : 0);
+      }
+      if (p.by_tma) {
+        sm100::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          sm100::tma_store_2d(MODE == GELU_AND_Z ? map_z : map_c, stg, col0, out0);
+          if (MODE == GELU_AND_Z) sm100::tma_store_2d(map_c, stg + L::TILE, col0, out0);
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      } else {                          // rows that start anywhere: consecutive elements by consecutive lanes
+        __syncwarp();
+#pragma unroll 1
+        for (int o = 0; o < L::OUTPUTS; ++o) {
+          T* out = (T*)(L::OUTPUTS == 2 && o == 0 ? p.z : p.c) + col0 + lane;
+          if (col0 + lane < p.N)
+            for (int j = 0; j < 32 && row0 + j < p.M; ++j) {
+              const int at = lane * (int)sizeof(T), sw = ROW == 128 ? j & 7 : (j >> 1) & 3;
+              out[(long long)(row0 + j) * p.N] = *reinterpret_cast<const T*>(stg + o * L::TILE + j * ROW + (((at >> 4) ^ sw) << 4) + (at & 15));
+            }
+        }
+        __syncwarp();
       }
     }
     sm100::tc_fence_before();
     __syncwarp();
     if (lane == 0) sm100::mbar_arrive_cluster_no_stores(sm100::map_to_cta(&sh->acc_empty[acc], 0));
   }
-  if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // read before the CTA gives its shared memory back
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // read before the CTA gives its shared memory back
 }
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Layout<T, MODE>::THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
                const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_z, const Problem p) {
-  using L = Layout<MODE>;
+  using L = Layout<T, MODE>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);      // the same offset in both CTAs
   Shared* sh = (Shared*)(base + L::SHARED_AT);
@@ -334,10 +335,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     sm100::tma_prefetch_desc(&map_a);
     sm100::tma_prefetch_desc(&map_b);
     for (int s = 0; s < L::STAGES; ++s) { sm100::mbar_init(&sh->full[s], 1); sm100::mbar_init(&sh->empty[s], 1); }
-    constexpr int FIRST = sizeof(T) == 2 ? 1 : GROUPS;
     for (int a = 0; a < 2; ++a) {
       sm100::mbar_init(&sh->acc_full[a], 1);
-      sm100::mbar_init(&sh->acc_empty[a], 2 * 4 * GROUPS);
+      sm100::mbar_init(&sh->acc_empty[a], 2 * 4 * L::GROUPS);
       sm100::mbar_init(&sh->shared_free[a], 2 * 4 * FIRST);
     }
     sh->error = 0;
@@ -452,7 +452,7 @@ static Plan plan_of(int M, int N, int k_blocks) {
 template <typename T, int MODE>
 static cudaError_t launch(const CUtensorMap* m, const Problem& p, cudaStream_t stream) {
   static std::once_flag once;
-  std::call_once(once, [] { cudaFuncSetAttribute(product_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<MODE>::BYTES); });
+  std::call_once(once, [] { cudaFuncSetAttribute(product_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<T, MODE>::BYTES); });
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -461,8 +461,8 @@ static cudaError_t launch(const CUtensorMap* m, const Problem& p, cudaStream_t s
   at[1].val.programmaticStreamSerializationAllowed = 1;
   const long long items = (long long)p.tiles_m * p.tiles_n * p.slices;
   cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(items, max_clusters()));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = Layout<MODE>::BYTES; cfg.stream = stream; cfg.attrs = at; cfg.numAttrs = 2;
+  cfg.blockDim = dim3(Layout<T, MODE>::THREADS);
+  cfg.dynamicSmemBytes = Layout<T, MODE>::BYTES; cfg.stream = stream; cfg.attrs = at; cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, product_kernel<T, MODE>, m[0], m[1], m[2], m[3], m[4], m[5], p);
 }
 
@@ -493,7 +493,7 @@ static int run(const void* qa, const void* sa, const void* qb, const void* sb, c
     const int ld = ld_of(N);
     if (!ws || ws_bytes < (size_t)pl.slices * slice_rows(pl) * ld * 4) return fail(TMPI_ERR_INVALID, "fp8_product: a workspace of %zu bytes is too small", ws_bytes);
     if ((int64_t)pl.slices * slice_rows(pl) > 0x7fffffff) return fail(TMPI_ERR_UNSUPPORTED, "fp8_product: %d x %d is too large", M, N);
-    if ((st = make_tmap_box(&m[4], 4, ws, (uint64_t)pl.slices * slice_rows(pl), (uint64_t)ld, BM, 32))) return st;
+    if ((st = make_tmap_box(&m[4], 4, ws, (uint64_t)pl.slices * slice_rows(pl), (uint64_t)ld, 32, gemm8::COLS))) return st;
     m[5] = m[4];
     p.slice_rows = (int)slice_rows(pl);
     p.by_tma = 1;
@@ -507,8 +507,8 @@ static int run(const void* qa, const void* sa, const void* qb, const void* sb, c
   } else {
     p.by_tma = (size_t)N * es % 16 == 0 && all_aligned16({c, z});
     m[4] = m[5] = m[0];                 // not used without by_tma
-    if (p.by_tma && (st = make_tmap_box(&m[4], es, c, (uint64_t)M, (uint64_t)N, BM, 128 / es))) return st;
-    if (p.by_tma && z && (st = make_tmap_box(&m[5], es, z, (uint64_t)M, (uint64_t)N, BM, 128 / es))) return st;
+    if (p.by_tma && (st = make_tmap_box(&m[4], es, c, (uint64_t)M, (uint64_t)N, 32, gemm8::COLS))) return st;
+    if (p.by_tma && z && (st = make_tmap_box(&m[5], es, z, (uint64_t)M, (uint64_t)N, 32, gemm8::COLS))) return st;
     e = z ? launch<T, GELU_AND_Z>(m, p, stream) : gelu ? launch<T, WITH_GELU>(m, p, stream) : launch<T, PLAIN>(m, p, stream);
   }
   return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "fp8_product launch: %s", cudaGetErrorString(e));
