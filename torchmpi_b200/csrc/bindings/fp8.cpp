@@ -18,76 +18,90 @@ Mat8 empty_mat(const Tensor& like, int64_t rows, int64_t cols) {
 Tensor dense_rows(const Tensor& x) { return x.stride(1) == 1 && (x.size(0) < 2 || x.stride(0) >= x.size(1)) ? x : x.contiguous(); }
 int64_t pitch(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
 
+// The same inside a larger buffer.
+struct Place8 {
+  char *q = nullptr, *scale = nullptr;
+  static int64_t bytes(int64_t rows, int64_t cols) { return aligned(rows * tmpi_fp8_pitch(cols)) + aligned((int64_t)tmpi_fp8_scale_bytes(rows, cols)); }
+  static int64_t aligned(int64_t n) { return (n + 255) / 256 * 256; }
+  Place8() = default;
+  Place8(char* at, int64_t rows, int64_t cols) : q(at), scale(at + aligned(rows * tmpi_fp8_pitch(cols))) {}
+  Place8(const Mat8& m) : q((char*)m.q.data_ptr()), scale((char*)m.scale.data_ptr()) {}
+};
+Tensor bytes_like(const Tensor& like, int64_t n) { return at::empty({n}, like.options().dtype(at::kByte)); }
+
 // a, t: along the rows and the columns, each where it is given; z, sums: see tmpi_fp8_quantize
-void quantize(const Tensor& x, const Tensor& z, Mat8* a, Mat8* t, const Tensor& sums) {
-  const int64_t rows = x.size(0), cols = x.size(1);
-  if (a) *a = empty_mat(x, rows, cols);
-  if (t) *t = empty_mat(x, cols, rows);
-  check(tmpi_fp8_quantize(x.data_ptr(), pitch(x), ptr(z), a ? a->q.data_ptr() : nullptr, a ? a->scale.data_ptr() : nullptr, t ? t->q.data_ptr() : nullptr,
-                          t ? t->scale.data_ptr() : nullptr, sums.defined() ? sums.data_ptr<float>() : nullptr, rows, cols, dtype_code(x.scalar_type()), stream()));
+void quantize(const Tensor& x, const Tensor& z, const Place8& a, const Place8& t, float* sums) {
+  check(tmpi_fp8_quantize(x.data_ptr(), pitch(x), ptr(z), a.q, a.scale, t.q, t.scale, sums, x.size(0), x.size(1), dtype_code(x.scalar_type()), stream()));
   launched(FP8, 1);
 }
 
-// a b^T (+ bias) with `cols` columns of K; with gelu the GELU of it, and the rounded sums in z where it is given
-Tensor product(const Mat8& a, const Mat8& b, int64_t cols, const Tensor& bias, bool gelu, Tensor* z, at::ScalarType type) {
-  const int M = (int)a.q.size(0), N = (int)b.q.size(0), K = (int)cols;
-  Tensor c = at::empty({M, N}, a.q.options().dtype(type)), ws;
-  if (z) *z = at::empty_like(c);
-  const size_t need = tmpi_fp8_product_workspace_bytes(M, N, K);
-  if (need) ws = at::empty({(int64_t)need}, a.q.options().dtype(at::kByte));
-  check(tmpi_fp8_product(a.q.data_ptr(), a.scale.data_ptr(), b.q.data_ptr(), b.scale.data_ptr(), ptr(bias), c.data_ptr(), z ? z->data_ptr() : nullptr, M, N, K, gelu, dtype_code(type),
+// a b^T (+ bias) of [M, K] and [N, K]; with gelu the GELU of it, and the rounded sums in z where it is given
+Tensor product(const Place8& a, const Place8& b, int64_t M, int64_t N, int64_t K, const Tensor& bias, bool gelu, Tensor* z, const at::TensorOptions& options) {
+  Tensor c = at::empty({M, N}, options), ws;
+  if (z) *z = at::empty({M, N}, options);
+  const size_t need = tmpi_fp8_product_workspace_bytes((int)M, (int)N, (int)K);
+  if (need) ws = bytes_like(c, (int64_t)need);
+  check(tmpi_fp8_product(a.q, a.scale, b.q, b.scale, ptr(bias), c.data_ptr(), z ? z->data_ptr() : nullptr, (int)M, (int)N, (int)K, gelu, dtype_code(c.scalar_type()),
                          need ? ws.data_ptr() : nullptr, need, stream()));
   launched(FP8, need ? 2 : 1);
   return c;
 }
 
 // x w^T (+ bias, GELU) without gradients
-Tensor linear_kept(const Tensor& x, const Mat8& w, const Tensor& bias, bool gelu) {
+Tensor linear_kept(const Tensor& x, const Place8& w, int64_t rows, const Tensor& bias, bool gelu) {
   if (x.size(0) <= tmpi_fp8_few_tokens()) {
-    Tensor y = at::empty({x.size(0), w.q.size(0)}, x.options());
-    check(tmpi_fp8_few(x.data_ptr(), pitch(x), w.q.data_ptr(), w.scale.data_ptr(), ptr(bias), y.data_ptr(), (int)x.size(0), (int)w.q.size(0), (int)x.size(1), gelu,
+    Tensor y = at::empty({x.size(0), rows}, x.options());
+    check(tmpi_fp8_few(x.data_ptr(), pitch(x), w.q, w.scale, ptr(bias), y.data_ptr(), (int)x.size(0), (int)rows, (int)x.size(1), gelu,
                        dtype_code(x.scalar_type()), stream()));
     launched(FP8, 1);
     return y;
   }
-  Mat8 a;
-  quantize(x, Tensor(), &a, nullptr, Tensor());
-  return product(a, w, x.size(1), bias, gelu, nullptr, x.scalar_type());
+  const Tensor room = bytes_like(x, Place8::bytes(x.size(0), x.size(1)));
+  const Place8 a((char*)room.data_ptr(), x.size(0), x.size(1));
+  quantize(x, Tensor(), a, Place8(), nullptr);
+  return product(a, w, x.size(0), rows, x.size(1), bias, gelu, nullptr, x.options());
 }
 
-// Kept for backward: x and w along their columns, in 8 bits, and with a GELU the rounded pre-activation; each where a gradient needs it.
+// Kept for backward: x and w along their columns, in 8 bits, in one buffer, and with a GELU the rounded pre-activation; each where a gradient needs it.
 struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const OptTensor& bias_, bool gelu, bool need_x, bool need_w) {
     const Tensor x = dense_rows(x_), w = dense_rows(w_), bias = bias_.has_value() ? packed(*bias_) : Tensor();
-    Mat8 xr, xc, wr, wc;
-    Tensor z;
-    quantize(x, Tensor(), &xr, need_w ? &xc : nullptr, Tensor());
-    quantize(w, Tensor(), &wr, need_x ? &wc : nullptr, Tensor());
-    Tensor y = product(xr, wr, x.size(1), bias, gelu, gelu ? &z : nullptr, x.scalar_type());
-    ctx->save_for_backward({xc.q, xc.scale, wc.q, wc.scale, z});
-    ctx->saved_data["bias"] = bias.defined();
-    ctx->saved_data["inputs"] = x.size(1);
+    const int64_t T = x.size(0), K = x.size(1), N = w.size(0), xs = Place8::bytes(T, K), xt = need_w ? Place8::bytes(K, T) : 0, wt = need_x ? Place8::bytes(K, N) : 0;
+    const Tensor room = bytes_like(x, xs + Place8::bytes(N, K));
+    Tensor kept, z;
+    if (xt + wt) kept = bytes_like(x, xt + wt);
+    char *at = (char*)room.data_ptr(), *to = xt + wt ? (char*)kept.data_ptr() : nullptr;
+    const Place8 xr(at, T, K), wr(at + xs, N, K);
+    quantize(x, Tensor(), xr, need_w ? Place8(to, K, T) : Place8(), nullptr);
+    quantize(w, Tensor(), wr, need_x ? Place8(to + xt, K, N) : Place8(), nullptr);
+    Tensor y = product(xr, wr, T, N, K, bias, gelu, gelu ? &z : nullptr, x.options());
+    ctx->save_for_backward({kept, z});
+    ctx->saved_data["inputs"] = K;
+    ctx->saved_data["kept"] = (need_x ? 1 : 0) | (need_w ? 2 : 0) | (bias.defined() ? 4 : 0);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_graph();
     const auto saved = ctx->get_saved_variables();
-    const Mat8 xc{as_saved(saved[0]), as_saved(saved[1])}, wc{as_saved(saved[2]), as_saved(saved[3])};
-    const Tensor z = as_saved(saved[4]), dy = z.defined() ? packed(grads[0]) : dense_rows(grads[0]);
-    const bool need_x = wc.q.defined() && ctx->needs_input_grad(0), need_w = xc.q.defined() && ctx->needs_input_grad(1),
-               need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);      // an absent bias has no number among the inputs
+    const int64_t flags = ctx->saved_data["kept"].toInt();
+    const Tensor kept = as_saved(saved[0]), z = as_saved(saved[1]), dy = z.defined() ? packed(grads[0]) : dense_rows(grads[0]);
+    const bool need_x = (flags & 1) && ctx->needs_input_grad(0), need_w = (flags & 2) && ctx->needs_input_grad(1),
+               need_b = (flags & 4) && ctx->needs_input_grad(2);      // an absent bias has no number among the inputs
     const int64_t T = dy.size(0), N = dy.size(1), K = ctx->saved_data["inputs"].toInt();
-    const auto type = dy.scalar_type();
-    Tensor dx, dw, db, sums;
+    Tensor dx, dw, db;
     if (need_x || need_w || need_b) {
-      Mat8 rows, columns;
-      if (need_b) sums = at::empty({(T + 127) / 128, N}, dy.options().dtype(at::kFloat));
-      quantize(dy, z, need_x ? &rows : nullptr, need_w || need_b || z.defined() ? &columns : nullptr, sums);
-      if (need_x) dx = product(rows, wc, N, Tensor(), false, nullptr, type);
-      if (need_w) dw = product(columns, xc, T, Tensor(), false, nullptr, type);
+      const bool columns = need_w || need_b || z.defined();
+      const int64_t tiles = (T + 127) / 128, rb = need_x ? Place8::bytes(T, N) : 0, cb = columns ? Place8::bytes(N, T) : 0;
+      const Tensor room = bytes_like(dy, rb + cb + (need_b ? tiles * N * 4 : 0));
+      char *at = (char*)room.data_ptr(), *from = kept.defined() ? (char*)kept.data_ptr() : nullptr;
+      const Place8 r = need_x ? Place8(at, T, N) : Place8(), c = columns ? Place8(at + rb, N, T) : Place8();
+      float* sums = need_b ? (float*)(at + rb + cb) : nullptr;
+      quantize(dy, z, r, c, sums);
+      if (need_x) dx = product(r, Place8(from + (flags & 2 ? Place8::bytes(K, T) : 0), K, N), T, K, N, Tensor(), false, nullptr, dy.options());
+      if (need_w) dw = product(c, Place8(from, K, T), N, K, T, Tensor(), false, nullptr, dy.options());
       if (need_b) {
         db = at::empty({N}, dy.options());
-        check(tmpi_fp8_column_sums(sums.data_ptr<float>(), (int)sums.size(0), (int)N, db.data_ptr(), dtype_code(type), stream()));
+        check(tmpi_fp8_column_sums(sums, (int)tiles, (int)N, db.data_ptr(), dtype_code(dy.scalar_type()), stream()));
         launched(FP8, 1);
       }
     }
@@ -114,10 +128,13 @@ Tensor shaped_as(const Tensor& y, const Tensor& x) {
 void register_fp8(pybind11::module_& m) {
   // (q, scale) along the rows, and of the transpose, each where it is asked for
   m.def("fp8_quantize", [](const Tensor& x_, bool rows, bool columns) -> c10::optional<std::vector<Tensor>> {
-    if (!(x_.is_cuda() && floating(x_) && x_.dim() == 2 && extents(x_.size(0), x_.size(1), 1) && here({&x_}))) return c10::nullopt;
-    const Tensor x = dense_rows(x_.detach());
+    if (!(x_.is_cuda() && floating(x_) && x_.dim() >= 1 && x_.size(-1) >= 1 && extents(x_.numel() / x_.size(-1), x_.size(-1), 1) && here({&x_}))) return c10::nullopt;
+    at::AutoDispatchBelowAutograd no_graph;
+    const Tensor x = dense_rows(rows_of(x_));
     Mat8 a, t;
-    quantize(x, Tensor(), rows ? &a : nullptr, columns ? &t : nullptr, Tensor());
+    if (rows) a = empty_mat(x, x.size(0), x.size(1));
+    if (columns) t = empty_mat(x, x.size(1), x.size(0));
+    quantize(x, Tensor(), rows ? Place8(a) : Place8(), columns ? Place8(t) : Place8(), nullptr);
     std::vector<Tensor> out;
     if (rows) out.insert(out.end(), {a.q, a.scale});
     if (columns) out.insert(out.end(), {t.q, t.scale});
@@ -136,13 +153,15 @@ void register_fp8(pybind11::module_& m) {
     if (!(code == TMPI_F32 || code == TMPI_F16 || code == TMPI_BF16) || !qa.is_cuda() || !is_mat(qa, sa, cols) || !is_mat(qb, sb, cols)) return c10::nullopt;
     const auto type = code == TMPI_F32 ? at::kFloat : code == TMPI_F16 ? at::kHalf : at::kBFloat16;
     if (!(shaped(bias, {qb.size(0)}) && all_of_type({&bias}, type) && here({&bias}))) return c10::nullopt;
-    return product(packed_mat(qa, sa), packed_mat(qb, sb), cols, bias.defined() ? packed(bias.detach()) : bias, false, nullptr, type);
+    const Mat8 a = packed_mat(qa, sa), b = packed_mat(qb, sb);
+    return product(a, b, qa.size(0), qb.size(0), cols, bias.defined() ? packed(bias.detach()) : bias, false, nullptr, qa.options().dtype(type));
   });
   m.def("fp8_linear_kept", [](const Tensor& x, const Tensor& q, const Tensor& scale, int64_t cols, const OptTensor& bias_, bool gelu) -> OptTensor {
     const Tensor bias = or_none(bias_);
     if (!(x.is_cuda() && floating(x) && x.dim() >= 1 && x.size(-1) == cols && is_mat(q, scale, cols) && shaped(bias, {q.size(0)}) && all_of_type({&bias}, x.scalar_type()) &&
           here({&x, &bias}) && extents(x.numel() / cols, 1, 1) && !wants_grad({x, bias}))) return c10::nullopt;
-    return shaped_as(linear_kept(dense_rows(rows_of(x)), packed_mat(q, scale), bias.defined() ? packed(bias) : bias, gelu), x);
+    const Mat8 w = packed_mat(q, scale);
+    return shaped_as(linear_kept(dense_rows(rows_of(x)), w, q.size(0), bias.defined() ? packed(bias) : bias, gelu), x);
   });
   m.def("fp8_linear", [](const Tensor& x, const Tensor& w, const OptTensor& bias_, bool gelu) -> OptTensor {
     const Tensor bias = or_none(bias_);
@@ -151,9 +170,10 @@ void register_fp8(pybind11::module_& m) {
     if (!(K >= 1 && x.size(-1) == K && shaped(bias, {N}) && extents(x.numel() / K, N, K))) return c10::nullopt;
     const Tensor x2 = rows_of(x);
     if (wants_grad({x, w, bias})) return shaped_as(Linear8Fn::apply(x2, w, bias_, gelu, x.requires_grad(), w.requires_grad()), x);
-    Mat8 kept;
-    quantize(dense_rows(w), Tensor(), &kept, nullptr, Tensor());
-    return shaped_as(linear_kept(dense_rows(x2), kept, bias.defined() ? packed(bias) : bias, gelu), x);
+    const Tensor room = bytes_like(x, Place8::bytes(N, K));
+    const Place8 kept((char*)room.data_ptr(), N, K);
+    quantize(dense_rows(w), Tensor(), kept, Place8(), nullptr);
+    return shaped_as(linear_kept(dense_rows(x2), kept, N, bias.defined() ? packed(bias) : bias, gelu), x);
   });
 }
 

@@ -67,7 +67,7 @@ static_assert(sizeof(Shared) <= 256, "the barriers' place");
 struct Problem {
   int M, N, k_blocks;
   int tiles_m, tiles_n;        // of 256 rows, of bn columns
-  int bn;                      // columns of a tile: 256 or 128
+  int bn;                      // columns of a tile: 256, 192 or 128
   int slices, slice_blocks;    // K blocks of a slice, a multiple of four
   int slice_rows;              // rows between the slices' results
   int by_tma;                  // the results' rows are 16-byte multiples
@@ -116,7 +116,7 @@ __device__ __forceinline__ uint32_t instruction(int M, int N) { return (uint32_t
 template <int STAGES>
 __device__ __forceinline__ void producer(Shared* sh, unsigned char* tiles, unsigned char* sf, const Problem& p, const CUtensorMap* ma, const CUtensorMap* mb, const CUtensorMap* msa,
                                          const CUtensorMap* msb, uint32_t rank, int cluster, int clusters) {
-  const int groups = (p.k_blocks + fp8::GROUP - 1) / fp8::GROUP, half = p.bn / 2, b_tiles = p.bn / 128;
+  const int groups = (p.k_blocks + fp8::GROUP - 1) / fp8::GROUP, half = p.bn / 2, b_tiles = (p.bn + 127) / 128;      // 192 columns from a multiple of 64 on: two
   const uint32_t tx = 2 * (A_BYTES + half * BK), tx_scales = 2 * (1 + b_tiles) * SF_BYTES;
   int stage = 0;
   uint32_t phase = 0;
@@ -136,7 +136,7 @@ __device__ __forceinline__ void producer(Shared* sh, unsigned char* tiles, unsig
         unsigned char* s = sf + (size_t)stage * SF_STAGE;
         const int g = kb / fp8::GROUP;
         sm100::tma_load_2d_pair(s, msa, 0, (it.m_tile * 2 + (int)rank) * groups + g, full0);
-        for (int j = 0; j < b_tiles; ++j) sm100::tma_load_2d_pair(s + (1 + j) * SF_BYTES, msb, 0, (it.n_tile * b_tiles + j) * groups + g, full0);
+        for (int j = 0; j < b_tiles; ++j) sm100::tma_load_2d_pair(s + (1 + j) * SF_BYTES, msb, 0, (it.n_tile * p.bn / 128 + j) * groups + g, full0);
       }
       if (++stage == STAGES) { stage = 0; phase ^= 1; }
     }
@@ -156,7 +156,7 @@ __device__ __forceinline__ void issuer(Shared* sh, unsigned char* tiles, unsigne
     if (!sm100::mbar_wait(&sh->acc_empty[acc], ((n >> 1) & 1) ^ 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p, 2); return; }
     if (overlap && n && !sm100::mbar_wait(&sh->shared_free[acc ^ 1], ((n - 1) >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p, 3); return; }
     sm100::tc_fence_after();
-    const uint32_t d = sh->tmem_base + (acc ? (overlap ? ACC1 : BN / 2) : 0);
+    const uint32_t d = sh->tmem_base + (acc ? (overlap ? ACC1 : p.bn) : 0);
     const int kb0 = it.slice * p.slice_blocks, kb1 = min(p.k_blocks, kb0 + p.slice_blocks);
     for (int kb = kb0; kb < kb1; ++kb) {
       if (!sm100::mbar_wait(&sh->full[stage], phase, kWaitBudgetNs, &sh->error)) { give_up(sh, p, 4); return; }
@@ -167,13 +167,14 @@ __device__ __forceinline__ void issuer(Shared* sh, unsigned char* tiles, unsigne
         const uint32_t s = sm100::smem_u32(sf + (size_t)stage * SF_STAGE), to = sh->tmem_base + SF_COL + set * SF_SET;
         copy_scales_pair(to, scales_desc(s));
         copy_scales_pair(to + 4, scales_desc(s + SF_BYTES));
-        if (p.bn == BN) copy_scales_pair(to + 8, scales_desc(s + 2 * SF_BYTES));
+        if (p.bn > 128) copy_scales_pair(to + 8, scales_desc(s + 2 * SF_BYTES));
       }
-      const uint32_t sfa = sh->tmem_base + SF_COL + set * SF_SET, a = sm100::smem_u32(tiles + (size_t)stage * STAGE_BYTES), b = a + A_BYTES;
+      // 192 columns may start at the third of a tile's four groups of 32 rows
+      const uint32_t sfa = sh->tmem_base + SF_COL + set * SF_SET, sfb = sfa + 4 + (it.n_tile * p.bn % 128) / 32, a = sm100::smem_u32(tiles + (size_t)stage * STAGE_BYTES), b = a + A_BYTES;
       const uint32_t desc = idesc | (uint32_t)part << 29 | (uint32_t)part << 4;
 #pragma unroll
       for (int k = 0; k < BK / UMMA_K; ++k)
-        mma_scaled_pair(d, sm100::make_desc_sw128(a + k * UMMA_K), sm100::make_desc_sw128(b + k * UMMA_K), desc, sfa, sfa + 4, (kb - kb0) | k);
+        mma_scaled_pair(d, sm100::make_desc_sw128(a + k * UMMA_K), sm100::make_desc_sw128(b + k * UMMA_K), desc, sfa, sfb, (kb - kb0) | k);
       sm100::umma_commit_pair(sm100::map_to_cta(&sh->empty[stage], 0));
       sm100::umma_commit_pair(sm100::map_to_cta(&sh->empty[stage], 1));
       if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -224,7 +225,7 @@ __device__ __forceinline__ void epilogue(Shared* sh, unsigned char* staging, con
     if (!sm100::mbar_wait_warp(&sh->acc_full[acc], (n >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p, 5); break; }
     sm100::tc_fence_after();
     const int row0 = (it.m_tile * 2 + (int)rank) * BM + quarter * 32, out0 = row0 + it.slice * p.slice_rows;
-    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (acc ? (overlap ? ACC1 : BN / 2) : 0);
+    const uint32_t t_base = sh->tmem_base + ((uint32_t)(quarter * 32) << 16) + (acc ? (overlap ? ACC1 : p.bn) : 0);
 #pragma unroll 1
     for (int i = group; i < parts; i += L::GROUPS) {
       const int c0 = (overlap && !acc ? parts - 1 - i : i) * COLS, col0 = it.n_tile * p.bn + c0;
@@ -426,23 +427,27 @@ struct Plan { int bn, slices, slice_blocks, tiles_m, tiles_n; };
 
 static int max_clusters() { return gemm_sm_count() / 2; }
 
-// Columns of a tile, and slices of K.  The time of a launch is its rounds of tiles: a block of 128 of K takes 512 cycles of MMAs at 256 columns, and
-// at 128 the operands' way out of L2 (48 KB for a pair at about 128 bytes a cycle), with an epilogue once a round; slices cost their sums' way to memory and back.
+// Columns of a tile, and slices of K, by the time that they take, in us: 3 for the launch and its first loads, and for each round of tiles that for a block of 128 of K
+// and that for what the next tile's MMAs do not hide of the epilogue.  Measured: 256 columns 0.371 and 1.25, 192 0.285 and 1.0, 128 0.222 and 1.05 (8192 x 4096 x 1024 in
+// 33.1, 36.0, 42.6 us; 8192 x 1024 x 4096 29.3, 33.5, 35.6; 4096 x 1024 x 8192, one round of 64 tiles of 256, 28.0, 39.9, 36.5).  Slices cost a launch and their
+// sums' way to memory and back (1024 x 1024 x 8192: 17.4 in four slices, 20.0 in tiles of 128 without).
 static Plan plan_of(int M, int N, int k_blocks) {
-  const int clusters = max_clusters();
+  struct Width { int columns; double block, tile; };
+  constexpr Width widths[] = {{256, 0.371, 1.25}, {192, 0.285, 1.0}, {128, 0.222, 1.05}};
+  const int clusters = max_clusters(), tm = (M + 2 * BM - 1) / (2 * BM);
   Plan best{};
   double least = 1e30;
-  for (int bn : {256, 128}) {
-    const int tm = (M + 2 * BM - 1) / (2 * BM), tn = (N + bn - 1) / bn;
+  for (const Width& w : widths) {
+    const int tn = (N + w.columns - 1) / w.columns;
     for (int s = 1; s <= 16; ++s) {
       const int per = ((k_blocks + s - 1) / s + 3) / 4 * 4, slices = (k_blocks + per - 1) / per;
       if (slices != s) continue;
       const long long rounds = ((long long)tm * tn * s + clusters - 1) / clusters;
-      double cycles = rounds * (std::min(per, k_blocks) * (bn == 256 ? 600. : 400.) + (bn == 256 ? 1200. : 700.)) + 3000.;
-      if (s > 1) cycles += 6000. + (double)M * N * 4. * (s + 1) / 2000.;
-      if (cycles < least) {
-        least = cycles;
-        best = {bn, s, per, tm, tn};
+      double us = 3. + rounds * (std::min(per, k_blocks) * w.block + w.tile);
+      if (s > 1) us += 2.5 + (double)M * N * 4. * (s + 1) / 4.5e6;
+      if (us < least) {
+        least = us;
+        best = {w.columns, s, per, tm, tn};
       }
     }
   }

@@ -107,37 +107,37 @@ def _matrix(what: str, x: torch.Tensor) -> torch.Tensor:
 # ---------------------------------------------------------------- entry points
 def quantize(x: torch.Tensor) -> Block8:
     """The rows of ``x [..., C]`` in 8 bits (of 64 bits: of their values in 32); not differentiable."""
-    x2 = _matrix("quantize", x)
-    if x2.is_cuda:
-        kept = _native.ext().fp8_quantize(x2, True, False)          # None: nothing for the kernel
+    if x.is_cuda:
+        kept = _native.ext().fp8_quantize(x, True, False)          # None: nothing for the kernel
         if kept is not None:
-            return Block8(*kept, x2.shape[1])
+            return Block8(*kept, x.shape[-1])
+    x2 = _matrix("quantize", x)
     same_device("quantize", x2)
     return _quantize(x2)
 
 
 def quantize_columns(x: torch.Tensor) -> Block8:
     """The columns of ``x [..., C]``: ``quantize(x.reshape(-1, C).T)``."""
+    if x.is_cuda:
+        kept = _native.ext().fp8_quantize(x, False, True)
+        if kept is not None:
+            return Block8(*kept, x.numel() // x.shape[-1])
     x2 = _matrix("quantize_columns", x)
     if not x2.shape[0]:
         raise ValueError("quantize_columns: there are no rows")
-    if x2.is_cuda:
-        kept = _native.ext().fp8_quantize(x2, False, True)
-        if kept is not None:
-            return Block8(*kept, x2.shape[0])
     same_device("quantize_columns", x2)
     return _quantize(x2.t())
 
 
 def quantize_both(x: torch.Tensor) -> Tuple[Block8, Block8]:
     """``(quantize(x), quantize_columns(x))``, reading ``x`` once."""
+    if x.is_cuda:
+        kept = _native.ext().fp8_quantize(x, True, True)
+        if kept is not None:
+            return Block8(kept[0], kept[1], x.shape[-1]), Block8(kept[2], kept[3], x.numel() // x.shape[-1])
     x2 = _matrix("quantize_both", x)
     if not x2.shape[0]:
         raise ValueError("quantize_both: there are no rows")
-    if x2.is_cuda:
-        kept = _native.ext().fp8_quantize(x2, True, True)
-        if kept is not None:
-            return Block8(*kept[:2], x2.shape[1]), Block8(*kept[2:], x2.shape[0])
     same_device("quantize_both", x2)
     return _quantize(x2), _quantize(x2.t())
 
