@@ -9,7 +9,8 @@ flat buckets inside the symmetric heap, and as soon as backward has produced a
 bucket one kernel sums it over the peers' memory, applies scaling, momentum and
 the weight update, and writes the new weights to every peer - no NCCL call and
 no separate optimizer kernel.  ``fused=False`` (and every CPU run) takes the
-reference's shape: ``synchronize_gradients`` then a per-tensor update.
+reference's shape: ``synchronize_gradients`` then a per-tensor update.  With ``optimizer`` (a function that makes one of the network's
+parameters, ``lambda params: ops.adamw.AdamW(params, bits=8)`` say) its ``step(lr)`` takes the place of that update, after the same synchronisation.
 
 Per sample:  onSample -> forward -> onForward -> criterion -> onForwardCriterion
 -> zero grads -> criterion backward -> onBackwardCriterion -> network backward
@@ -34,14 +35,18 @@ class AllReduceSGDEngine:
                  dynamicnetwork: bool = True, debug: bool = False, *, fused: Optional[bool] = None,
                  momentum: float = 0.0, dampening: float = 0.0, weight_decay: float = 0.0,
                  nesterov: bool = False, gradient_scale: float = 1.0, master_weights: bool = True,
-                 bucket_bytes: Optional[int] = None, **kw):
+                 bucket_bytes: Optional[int] = None, optimizer: Optional[Callable] = None, **kw):
         if "async" in kw:  # the reference's option name is a Python keyword
             async_ = kw.pop("async")
         if kw:
             raise TypeError(f"unknown options {sorted(kw)}")
         self.usegpu, self.async_, self.devicesync = usegpu, async_, devicesync
         self.dynamicnetwork, self.debug = dynamicnetwork, debug
-        self.fused = (usegpu and S.with_cuda) if fused is None else fused
+        if optimizer is not None and (fused or momentum or dampening or weight_decay or nesterov):
+            raise ValueError("an optimizer takes the place of SGD, fused or not, and has options of its own")
+        self.fused = (usegpu and S.with_cuda and optimizer is None) if fused is None else fused
+        self.optimizer = optimizer
+        self.own_optimizer = None  # what it made, for the network of the last train()
         self.momentum, self.dampening, self.weight_decay, self.nesterov = momentum, dampening, weight_decay, nesterov
         self.gradient_scale = gradient_scale
         self.master_weights = master_weights
@@ -113,6 +118,8 @@ class AllReduceSGDEngine:
                 mpinn.synchronize_parameters(criterion)
         if self._opt is not None:
             self._opt.refresh_master()
+        if self.optimizer is not None:           # after the synchronisation: masters are copies of the parameters
+            self.own_optimizer = self.optimizer([p for p in network.parameters() if p.requires_grad])
 
     def _plain_update(self, params: Iterable[torch.nn.Parameter], lr: float) -> None:
         """w += -lr * g per tensor (torchnet's SGD step), with optional momentum / weight decay."""
@@ -165,7 +172,10 @@ class AllReduceSGDEngine:
                     if p.grad is not None:
                         p.grad.mul_(self.gradient_scale)
             self.hook("onBackward", state)
-            self._plain_update(network.parameters(), state["lr"])
+            if self.own_optimizer is not None:
+                self.own_optimizer.step(state["lr"])
+            else:
+                self._plain_update(network.parameters(), state["lr"])
             if isinstance(criterion, torch.nn.Module) and any(True for _ in criterion.parameters()):
                 self._plain_update(criterion.parameters(), state["lrcriterion"])
         state["t"] += 1

@@ -8,7 +8,8 @@ products of the MLP and projections go through ``ops.gemm.linear`` (the tcgen05 
 attention otherwise, and for shapes that kernel does not take), layer norm through the one-pass ``ops.layernorm``
 and the LM head through the pitched ``ops.gemm.wide_head``; the loss is ``ops.xent``.  ``n_expert`` puts a layer of experts
 (``ops.experts.Experts``, ``expert_k`` of them for each token) in the place of each block's MLP; ``act8`` keeps the MLPs'
-activations in 8 bits for the backward pass (``ops.act8``).
+activations in 8 bits for the backward pass (``ops.act8``); ``fp8`` forms the products of the blocks' linear layers in 8 bits (``ops.fp8``; not those of an MLP with
+``act8`` or of experts).
 """
 from __future__ import annotations
 
@@ -31,6 +32,7 @@ class GPT2Config:
     n_expert: int = 0
     expert_k: int = 2
     act8: bool = False
+    fp8: bool = False
 
 
 def gpt2_medium(**kw) -> "GPT2":
@@ -44,11 +46,14 @@ def gpt2_tiny(**kw) -> "GPT2":
 
 
 class _Linear(nn.Linear):
-    def __init__(self, i, o, tc, gelu=False):
+    def __init__(self, i, o, tc, gelu=False, fp8=False):
         super().__init__(i, o)
-        self.tc, self.gelu = tc, gelu
+        self.tc, self.gelu, self.fp8 = tc, gelu, fp8
 
     def forward(self, x):
+        if self.fp8:
+            from ..ops import fp8
+            return fp8.linear(x, self.weight, self.bias, self.gelu)
         if self.tc:
             from ..ops import gemm
             return gemm.linear(x, self.weight, self.bias, self.gelu)
@@ -69,16 +74,16 @@ class Block(nn.Module):
         self.n_head = c.n_head
         self.own_attention = c.tc_linear
         self.ln1 = _layer_norm(c)
-        self.qkv = _Linear(c.n_embd, 3 * c.n_embd, c.tc_linear)
-        self.proj = _Linear(c.n_embd, c.n_embd, c.tc_linear)
+        self.qkv = _Linear(c.n_embd, 3 * c.n_embd, c.tc_linear, fp8=c.fp8)
+        self.proj = _Linear(c.n_embd, c.n_embd, c.tc_linear, fp8=c.fp8)
         self.ln2 = _layer_norm(c)
         self.act8 = c.act8
         if c.n_expert:
             from ..ops.experts import Experts
             self.experts = Experts(c.n_embd, 4 * c.n_embd, c.n_expert, c.expert_k, act8=c.act8)
         else:
-            self.fc = _Linear(c.n_embd, 4 * c.n_embd, c.tc_linear, gelu=True)
-            self.out = _Linear(4 * c.n_embd, c.n_embd, c.tc_linear)
+            self.fc = _Linear(c.n_embd, 4 * c.n_embd, c.tc_linear, gelu=True, fp8=c.fp8)
+            self.out = _Linear(4 * c.n_embd, c.n_embd, c.tc_linear, fp8=c.fp8)
 
     def _attention(self, qkv):
         from ..ops import attention
@@ -107,7 +112,7 @@ class Block(nn.Module):
         if not all(type(mods[n]) is layernorm.LayerNorm and bare(mods[n]) and mods[n].normalized_shape == x.shape[-1:]
                    and layernorm.supported(x, mods[n].weight, mods[n].bias) for n in ("ln1", "ln2")):
             return False
-        return all(type(mods[n]) is _Linear and mods[n].tc and not mods[n].gelu and bare(mods[n])
+        return all(type(mods[n]) is _Linear and mods[n].tc and not mods[n].fp8 and not mods[n].gelu and bare(mods[n])
                    for n in ("proj", "out") if n in mods)
 
     def forward(self, x):

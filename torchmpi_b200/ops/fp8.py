@@ -80,7 +80,7 @@ def _quantize(x: torch.Tensor) -> Block8:
     e = torch.where(a > 0, torch.where(m > 0.875, e - 8, e - 9), -126).clamp_min(-126)
     half = torch.div(-e, 2, rounding_mode="floor")                 # 2^126 * 2^-e in two exact steps
     q = torch.where(finite, b * _two_to(half) * _two_to(-e - half), float("nan")).to(torch.float8_e4m3fn)
-    return Block8(q.view(rows, -1), _tiled((e + 127).to(torch.uint8).view(rows, -1)), cols)
+    return Block8(q.view(rows, b.shape[1] * BLOCK), _tiled((e + 127).to(torch.uint8).view(rows, b.shape[1])), cols)
 
 
 def _dequantize(a: Block8, dtype: torch.dtype) -> torch.Tensor:

@@ -33,6 +33,7 @@ def main():
     ap.add_argument("--tc-linear", type=int, default=1)
     ap.add_argument("--n-expert", type=int, default=0, help="layers of so many experts, two for each token, in the place of the MLPs")
     ap.add_argument("--act8", type=int, default=0, help="keep the MLPs' activations in 8 bits for the backward pass")
+    ap.add_argument("--fp8", type=int, default=0, help="form the products of the blocks' linear layers in 8 bits")
     ap.add_argument("--profile-one-step", action="store_true",
                     help="after the warm-up run one step between cudaProfilerStart/Stop and exit (no timing)")
     args = ap.parse_args()
@@ -51,7 +52,7 @@ def main():
     mpi.set_communicator(0)
     rank, world, dev = mpi.world_rank(), mpi.world_size(), mpi.device
     torch.manual_seed(1)
-    form = dict(tc_linear=bool(args.tc_linear), n_expert=args.n_expert, act8=bool(args.act8))
+    form = dict(tc_linear=bool(args.tc_linear), n_expert=args.n_expert, act8=bool(args.act8), fp8=bool(args.fp8))
     model = gpt2.gpt2_medium(**form) if args.model == "gpt2_medium" else gpt2.gpt2_tiny(block_size=args.seq, **form)
     model = model.to(dev).to(torch.bfloat16)
     seq = min(args.seq, model.config.block_size)
