@@ -177,10 +177,12 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
     const Entry& e = table.entry[at];
     const Group& g = table.group[e.which & 0xff];
     const float t = (float)(s.steps[(e.which & (COUNTED - 1)) >> 8] + (e.which & COUNTED ? 0 : 1)), lr = g.device_lr ? *g.device_lr : g.lr;
-    // The update is m / (sqrt(v) unbias + eps) with the rate lr / (1 - b1^t) in the divisor (as 1e-30 at least: its inverse is a number), and a root of what a
-    // square takes on its way into v in front of the square.
-    const float step = fmaxf(lr / -expm1f(t * g.log_beta1), 1e-30f), unbias = rsqrtf(-expm1f(t * g.log_beta2)) / step, keep = 1.f - lr * g.decay;
-    const float b1 = g.beta1, b2 = g.beta2, a1 = g.rest1 * coefficient, a2 = sqrtf(g.rest2) * coefficient, eps = fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step;
+    // The update is m / (sqrt(v) unbias + eps) with the rate lr / (1 - b1^t) in the divisor (a rate below 1e-30, whose inverse may be no number, counts as 0: an infinite
+    // divisor), and of what is squared on its way into v the root is taken here.
+    const float step = lr / -expm1f(t * g.log_beta1), keep = 1.f - lr * g.decay;
+    const bool moves = step >= 1e-30f;
+    const float unbias = moves ? rsqrtf(-expm1f(t * g.log_beta2)) / step : 0.f, eps = moves ? fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step : __uint_as_float(0x7f800000u);
+    const float b1 = g.beta1, b2 = g.beta2, a1 = g.rest1 * coefficient, a2 = sqrtf(g.rest2) * coefficient;
     const float unit_m = b1 * (1.f / 16129.f), unit_v = sqrtf(b2) * (1.f / 65025.f);
     const uint32_t e0 = e.chunk, end = at + 1 < s.entries ? table.entry[at + 1].chunk : chunks, extent = e.n, whole = (extent + BLOCK - 1) / BLOCK * BLOCK;
     T* const param = (T*)e.param;
