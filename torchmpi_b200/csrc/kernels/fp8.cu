@@ -231,7 +231,7 @@ quantize_tiles_kernel(const T* __restrict__ x, const long long ld, const T* __re
           uint32_t* v = w[h + i];
           unsigned long long slope;
           if constexpr (std::is_same_v<T, __nv_bfloat16>) {          // results of 8 bits: the quicker form (gelu.cuh)
-            slope = shared_gelu_slope2(attn_util::pack2(__float_as_uint(E::get(zs[i], k)), __float_as_uint(E::get(zs[i], k + 1))));
+            slope = quick_gelu_slope2(attn_util::pack2(__float_as_uint(E::get(zs[i], k)), __float_as_uint(E::get(zs[i], k + 1))));
           } else {
             float s0, s1;
             gelu_grad2(E::get(zs[i], k), E::get(zs[i], k + 1), &s0, &s1);
@@ -276,11 +276,13 @@ quantize_tiles_kernel(const T* __restrict__ x, const long long ld, const T* __re
   if (sums) {
     float s[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      s[k] = 0.f;
+    for (int k = 0; k < 8; k += 2) {
+      unsigned long long a = attn_util::pack2(0u, 0u);
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) s[k] += E::get(w[i], k);
+      for (int i = 0; i < ROWS; ++i) a = attn_util::add2(a, attn_util::pack2(__float_as_uint(E::get(w[i], k)), __float_as_uint(E::get(w[i], k + 1))));
+      attn_util::unpack2(a, s[k], s[k + 1]);
       s[k] += __shfl_xor_sync(~0u, s[k], 16);
+      s[k + 1] += __shfl_xor_sync(~0u, s[k + 1], 16);
     }
     if (!(t & 16)) {
       *reinterpret_cast<float4*>(&part[warp][cg * 8]) = make_float4(s[0], s[1], s[2], s[3]);

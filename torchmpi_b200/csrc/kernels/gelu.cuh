@@ -96,15 +96,16 @@ __device__ __forceinline__ unsigned long long shared_cdf2(unsigned long long z, 
   return mul2(both(rcp(x0 * x1)), pack2(__float_as_uint(x1), __float_as_uint(x0)));
 }
 __device__ __forceinline__ unsigned long long shared_gelu2(unsigned long long z) { return attn_util::mul2(z, shared_cdf2(z, attn_util::mul2(z, z))); }
-__device__ __forceinline__ unsigned long long shared_gelu_slope2(unsigned long long z) {
+__device__ __forceinline__ unsigned long long quick_gelu2(unsigned long long z) { return attn_util::mul2(z, quick_cdf2(z, attn_util::mul2(z, z))); }
+// the slope alone, with the density's factor in its exponent: log2(0.39894228) = -1.32574806
+__device__ __forceinline__ unsigned long long quick_gelu_slope2(unsigned long long z) {
   using namespace attn_util;
   auto both = [](float v) { return attn_util::pack2(__float_as_uint(v), __float_as_uint(v)); };
   const unsigned long long t = mul2(z, z);
   float x0, x1;
-  unpack2(fma2(t, both(-0.5f * 1.4426950408889634f), both(-1.3257480647361593f)), x0, x1);          // log2 of the density: log2(0.39894228) = -1.32574806
-  return fma2(z, pack2(__float_as_uint(ex2(x0)), __float_as_uint(ex2(x1))), shared_cdf2(z, t));
+  unpack2(fma2(t, both(-0.5f * 1.4426950408889634f), both(-1.3257480647361593f)), x0, x1);
+  return fma2(z, pack2(__float_as_uint(ex2(x0)), __float_as_uint(ex2(x1))), quick_cdf2(z, t));
 }
-__device__ __forceinline__ unsigned long long quick_gelu2(unsigned long long z) { return attn_util::mul2(z, quick_cdf2(z, attn_util::mul2(z, z))); }
 __device__ __forceinline__ void quick_gelu_both2(unsigned long long z, unsigned long long* y, unsigned long long* slope) {
   using namespace attn_util;
   auto both = [](float v) { return attn_util::pack2(__float_as_uint(v), __float_as_uint(v)); };
