@@ -172,18 +172,27 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
   wait_previous();
   const float coefficient = s.scale * (s.coefficient ? *s.coefficient : 1.f);
   int at = entry_of(table, s.entries, blockIdx.x);
-  for (uint32_t c = blockIdx.x; c < chunks; ++at) {        // one tensor after another
-    while (at + 1 < s.entries && table.entry[at + 1].chunk <= c) ++at;
+  // Rates of a group's tensors with the same step count, which most have: formed anew where that changes (for each tensor they took 4 % of a step).
+  float seen = -1.f, unbias = 0.f, eps = 0.f, keep = 0.f, b1 = 0.f, b2 = 0.f, a1 = 0.f, a2 = 0.f, unit_m = 0.f, unit_v = 0.f;
+  uint32_t seen_group = ~0u;
+  for (uint32_t c = blockIdx.x; c < chunks; at = entry_of(table, s.entries, c)) {      // one tensor after another
     const Entry& e = table.entry[at];
-    const Group& g = table.group[e.which & 0xff];
-    const float t = (float)(s.steps[(e.which & (COUNTED - 1)) >> 8] + (e.which & COUNTED ? 0 : 1)), lr = g.device_lr ? *g.device_lr : g.lr;
-    // The update is m / (sqrt(v) unbias + eps) with the rate lr / (1 - b1^t) in the divisor (a rate below 1e-30, whose inverse may be no number, counts as 0: an infinite
-    // divisor), and of what is squared on its way into v the root is taken here.
-    const float step = lr / -expm1f(t * g.log_beta1), keep = 1.f - lr * g.decay;
-    const bool moves = step >= 1e-30f;
-    const float unbias = moves ? rsqrtf(-expm1f(t * g.log_beta2)) / step : 0.f, eps = moves ? fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step : __uint_as_float(0x7f800000u);
-    const float b1 = g.beta1, b2 = g.beta2, a1 = g.rest1 * coefficient, a2 = sqrtf(g.rest2) * coefficient;
-    const float unit_m = b1 * (1.f / 16129.f), unit_v = sqrtf(b2) * (1.f / 65025.f);
+    const float t = (float)(s.steps[(e.which & (COUNTED - 1)) >> 8] + (e.which & COUNTED ? 0 : 1));
+    if (t != seen || (e.which & 0xff) != seen_group) {
+      seen = t;
+      seen_group = e.which & 0xff;
+      const Group& g = table.group[seen_group];
+      const float lr = g.device_lr ? *g.device_lr : g.lr;
+      // The update is m / (sqrt(v) unbias + eps) with the rate lr / (1 - b1^t) in the divisor (a rate below 1e-30, whose inverse may be no number, counts as 0: an
+      // infinite divisor), and of what is squared on its way into v the root is taken here.
+      const float step = lr / -expm1f(t * g.log_beta1);
+      const bool moves = step >= 1e-30f;
+      unbias = moves ? rsqrtf(-expm1f(t * g.log_beta2)) / step : 0.f;
+      eps = moves ? fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step : __uint_as_float(0x7f800000u);
+      keep = 1.f - lr * g.decay;
+      b1 = g.beta1, b2 = g.beta2, a1 = g.rest1 * coefficient, a2 = sqrtf(g.rest2) * coefficient;
+      unit_m = b1 * (1.f / 16129.f), unit_v = sqrtf(b2) * (1.f / 65025.f);
+    }
     const uint32_t e0 = e.chunk, end = at + 1 < s.entries ? table.entry[at + 1].chunk : chunks, extent = e.n, whole = (extent + BLOCK - 1) / BLOCK * BLOCK;
     T* const param = (T*)e.param;
     const T* const grads = (const T*)e.grad;
@@ -270,57 +279,60 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
 }
 
 // ---------------------------------------------------------------- the norm of many tensors
-// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.  Eight chunks are under way at a time.
+// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.
 constexpr int NORM_BLOCKS = 148 * 4;
+__host__ __device__ constexpr uint32_t unit_chunks(int element_bytes) { return 32768 / (CHUNK * element_bytes); }
 
-// not moved behind what is done with the loads before it
-__device__ __forceinline__ uint4 load_in_order(const void* p) {
-  uint4 u;
-  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
-  return u;
+// Eight loads of 16 bytes, 4096 apart, that the compiler does not take apart (it waits for the first before it sends the last otherwise).
+__device__ __forceinline__ void load_eight(const void* p, uint32_t (&u)[32]) {
+  asm volatile(
+      "ld.global.v4.u32 {%0, %1, %2, %3}, [%32];\n\tld.global.v4.u32 {%4, %5, %6, %7}, [%32+4096];\n\t"
+      "ld.global.v4.u32 {%8, %9, %10, %11}, [%32+8192];\n\tld.global.v4.u32 {%12, %13, %14, %15}, [%32+12288];\n\t"
+      "ld.global.v4.u32 {%16, %17, %18, %19}, [%32+16384];\n\tld.global.v4.u32 {%20, %21, %22, %23}, [%32+20480];\n\t"
+      "ld.global.v4.u32 {%24, %25, %26, %27}, [%32+24576];\n\tld.global.v4.u32 {%28, %29, %30, %31}, [%32+28672];"
+      : "=&r"(u[0]), "=&r"(u[1]), "=&r"(u[2]), "=&r"(u[3]), "=&r"(u[4]), "=&r"(u[5]), "=&r"(u[6]), "=&r"(u[7]), "=&r"(u[8]), "=&r"(u[9]), "=&r"(u[10]), "=&r"(u[11]), "=&r"(u[12]),
+        "=&r"(u[13]), "=&r"(u[14]), "=&r"(u[15]), "=&r"(u[16]), "=&r"(u[17]), "=&r"(u[18]), "=&r"(u[19]), "=&r"(u[20]), "=&r"(u[21]), "=&r"(u[22]), "=&r"(u[23]), "=&r"(u[24]),
+        "=&r"(u[25]), "=&r"(u[26]), "=&r"(u[27]), "=&r"(u[28]), "=&r"(u[29]), "=&r"(u[30]), "=&r"(u[31])
+      : "l"(p));
 }
 
+// A block takes units of 32 KB (a few chunks in a row), as many apart as there are blocks, so that many small tensors are shared among all.
 template <typename T, int CAP>
-__global__ void __launch_bounds__(THREADS) squares_kernel(const __grid_constant__ Table<CAP> table, const int entries, const uint32_t chunks, const uint32_t per_block, double* __restrict__ sums) {
-  constexpr int PER = CHUNK / THREADS, AHEAD = sizeof(T) == 2 ? 8 : 4;
+__global__ void __launch_bounds__(THREADS, 4) squares_kernel(const __grid_constant__ Table<CAP> table, const int entries, const uint32_t chunks, double* __restrict__ sums) {
+  constexpr int PER = CHUNK / THREADS;
   wait_previous(sums);
-  const uint32_t c0 = blockIdx.x * per_block, c1 = min(chunks, c0 + per_block);
   float a[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) a[k] = 0.f;
-  int at = entry_of(table, entries, c0);
-  for (uint32_t c = c0; c < c1; ++at) {
-    const Entry& e = table.entry[at];
-    const uint32_t e0 = e.chunk, end = min(c1, at + 1 < entries ? table.entry[at + 1].chunk : chunks), extent = e.n;
-    const T* const grads = (const T*)e.grad;
-    const bool vec = ((uintptr_t)grads & 15) == 0;
-    const uint32_t whole = min(end, e0 + extent / CHUNK);       // chunks without an end of the tensor
-    if (vec) {
-      constexpr int V = 16 / sizeof(T), PACKS = PER / V;
-      for (; c + AHEAD <= whole; c += AHEAD) {
-        uint4 x[AHEAD][PACKS];
+  for (uint32_t c0 = blockIdx.x * unit_chunks(sizeof(T)); c0 < chunks; c0 += gridDim.x * unit_chunks(sizeof(T))) {
+    const uint32_t c1 = min(chunks, c0 + unit_chunks(sizeof(T)));
+    int at = entry_of(table, entries, c0);
+    for (uint32_t c = c0; c < c1; ++at) {
+      const Entry& e = table.entry[at];
+      const uint32_t e0 = e.chunk, end = min(c1, at + 1 < entries ? table.entry[at + 1].chunk : chunks), extent = e.n;
+      const T* const grads = (const T*)e.grad;
+      const bool vec = ((uintptr_t)grads & 15) == 0;
+      if (vec && end - c == unit_chunks(sizeof(T)) && (end - e0) * CHUNK <= extent) {          // the whole unit
+        constexpr int V = 16 / sizeof(T);
+        uint32_t x[32];
+        load_eight(grads + (size_t)(c - e0) * CHUNK + threadIdx.x * V, x);
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-          for (int j = 0; j < PACKS; ++j) x[u][j] = load_in_order(grads + (size_t)(c + u - e0) * CHUNK + j * (V * THREADS) + threadIdx.x * V);
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-          for (int k = 0; k < PER; ++k) {
-            const float f = (float)to_acc<T>(reinterpret_cast<const T*>(&x[u][k / V])[k % V]);
-            a[k] = fmaf(f, f, a[k]);
-          }
+        for (int j = 0; j < 8 * V; ++j) {
+          const float f = (float)to_acc<T>(reinterpret_cast<const T*>(x)[j]);
+          a[j % PER] = fmaf(f, f, a[j % PER]);
+        }
+        c = end;
       }
-    }
-    for (; c < end; ++c) {
-      float x[PER];
+      for (; c < end; ++c) {
+        float x[PER];
 #pragma unroll
-      for (int j = 0; j < PER; j += 4) {
-        const uint32_t first = (c - e0) * CHUNK + j * THREADS + threadIdx.x * 4;
-        load<T, 4>(grads + first, first < extent ? (int)min(4u, extent - first) : 0, vec, x + j);
+        for (int j = 0; j < PER; j += 4) {
+          const uint32_t first = (c - e0) * CHUNK + j * THREADS + threadIdx.x * 4;
+          load<T, 4>(grads + first, first < extent ? (int)min(4u, extent - first) : 0, vec, x + j);
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) a[k] = fmaf(x[k], x[k], a[k]);
       }
-#pragma unroll
-      for (int k = 0; k < PER; ++k) a[k] = fmaf(x[k], x[k], a[k]);
     }
   }
   double d = 0.;
@@ -403,9 +415,6 @@ static Filled fill(Table<CAP>* t, const tmpi_adamw_tensor_t* tensors, int count,
   return f;
 }
 
-// chunks of a block, for at most `most` blocks
-static uint32_t per_block(uint32_t chunks, uint32_t most) { return (chunks + most - 1) / most; }
-
 template <typename T, int CAP>
 static cudaError_t launch_step(const Table<CAP>& t, const States& s, int bits, uint32_t chunks, cudaStream_t stream) {
   const bool master = s.master != nullptr;
@@ -481,8 +490,8 @@ int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, 
     using T = std::remove_pointer_t<decltype(type)>;
     auto run = [&](const auto& table, const adamw::Filled& f) {
       constexpr int CAP = sizeof(table.entry) / sizeof(adamw::Entry);
-      const uint32_t per = adamw::per_block(f.chunks, adamw::NORM_BLOCKS), blocks = (f.chunks + per - 1) / per;
-      const cudaError_t e = launch_overlapped(adamw::squares_kernel<T, CAP>, blocks, adamw::THREADS, 0, (cudaStream_t)stream, table, f.entries, f.chunks, per, sums + *used);
+      const uint32_t unit = adamw::unit_chunks(sizeof(T)), blocks = std::min<uint32_t>((f.chunks + unit - 1) / unit, adamw::NORM_BLOCKS);
+      const cudaError_t e = launch_overlapped(adamw::squares_kernel<T, CAP>, blocks, adamw::THREADS, 0, (cudaStream_t)stream, table, f.entries, f.chunks, sums + *used);
       *used += (int)blocks;
       return e;
     };
