@@ -346,6 +346,7 @@ def test_the_entry_points_refuse():
     assert lib.tmpi_fp8_product(16, 16, 16, 16, None, 16, 16, 4, 4, 8, 0, 7, None, 0, None) != 0         # a pre-activation without a GELU
     assert lib.tmpi_fp8_restore(8, 16, 16, 4, 8, 7, None) != 0 and lib.tmpi_fp8_restore(16, 16, 16, -1, 8, 7, None) != 0
     assert lib.tmpi_fp8_product_workspace_bytes(0, 4, 8) == 0
+    assert lib.tmpi_fp8_product_sums(16, 16, 16, 16, 16, None, 1, 16, 4, 4, 8, 7, None, 0, None) != 0 and lib.tmpi_fp8_product_sums(16, 16, 16, 16, 16, 16, 0, 16, 4, 4, 8, 7, None, 0, None) != 0
 
 
 @gpu

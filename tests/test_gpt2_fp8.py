@@ -34,8 +34,8 @@ def test_trains(form, device):
     net, idx, target = _net(device, **form)
     before = fp8.launch_count
     loss, grads = _step(net, idx, target)
-    # a layer: two launches of quantization and one product forward; one, two, and one for the bias backward
-    assert device == "cpu" or fp8.launch_count - before >= 2 * 7 * (2 if form else 4)
+    # a layer: one launch of quantization and one product forward; one and two backward
+    assert device == "cpu" or fp8.launch_count - before >= 2 * 5 * (2 if form else 4)
     assert torch.isfinite(loss) and all(g.isfinite().all() and g.any() for g in grads if not form)
     again = _step(net, idx, target)
     assert torch.equal(loss, again[0])

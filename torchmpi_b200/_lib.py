@@ -220,6 +220,8 @@ _CUDA_PROTOS = {
     "tmpi_fp8_pitch": (_i64, [_i64]),
     "tmpi_fp8_scale_bytes": (_sz, [_i64, _i64]),
     "tmpi_fp8_quantize": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _vp]),
+    "tmpi_fp8_quantize_two": (_i, [_vp, _i, _vp]),
+    "tmpi_fp8_product_sums": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
     "tmpi_fp8_column_sums": (_i, [_vp, _i, _i, _vp, _i, _vp]),
     "tmpi_fp8_restore": (_i, [_vp, _vp, _vp, _i64, _i64, _i, _vp]),
     "tmpi_fp8_few_tokens": (_i, []),

@@ -47,6 +47,13 @@ Tensor product(const Place8& a, const Place8& b, int64_t M, int64_t N, int64_t K
   return c;
 }
 
+// x and w both ways
+void quantize_two(const Tensor& x, const Place8& xr, const Place8& xc, const Tensor& w, const Place8& wr, const Place8& wc) {
+  const tmpi_fp8_matrix_t two[2] = {{x.data_ptr(), pitch(x), xr.q, xr.scale, xc.q, xc.scale, x.size(0), x.size(1)}, {w.data_ptr(), pitch(w), wr.q, wr.scale, wc.q, wc.scale, w.size(0), w.size(1)}};
+  check(tmpi_fp8_quantize_two(two, dtype_code(x.scalar_type()), stream()));
+  launched(FP8, 1);
+}
+
 // x w^T (+ bias, GELU) without gradients
 Tensor linear_kept(const Tensor& x, const Place8& w, int64_t rows, const Tensor& bias, bool gelu) {
   if (x.size(0) <= tmpi_fp8_few_tokens()) {
@@ -72,8 +79,13 @@ struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
     if (xt + wt) kept = bytes_like(x, xt + wt);
     char *at = (char*)room.data_ptr(), *to = xt + wt ? (char*)kept.data_ptr() : nullptr;
     const Place8 xr(at, T, K), wr(at + xs, N, K);
-    quantize(x, Tensor(), xr, need_w ? Place8(to, K, T) : Place8(), nullptr);
-    quantize(w, Tensor(), wr, need_x ? Place8(to + xt, K, N) : Place8(), nullptr);
+    const Place8 xc = need_w ? Place8(to, K, T) : Place8(), wc = need_x ? Place8(to + xt, K, N) : Place8();
+    if (need_x && need_w) {
+      quantize_two(x, xr, xc, w, wr, wc);
+    } else {
+      quantize(x, Tensor(), xr, xc, nullptr);
+      quantize(w, Tensor(), wr, wc, nullptr);
+    }
     Tensor y = product(xr, wr, T, N, K, bias, gelu, gelu ? &z : nullptr, x.options());
     ctx->save_for_backward({kept, z});
     ctx->saved_data["inputs"] = K;
@@ -98,9 +110,18 @@ struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
       float* sums = need_b ? (float*)(at + rb + cb) : nullptr;
       quantize(dy, z, r, c, sums);
       if (need_x) dx = product(r, Place8(from + (flags & 2 ? Place8::bytes(K, T) : 0), K, N), T, K, N, Tensor(), false, nullptr, dy.options());
-      if (need_w) dw = product(c, Place8(from, K, T), N, K, T, Tensor(), false, nullptr, dy.options());
-      if (need_b) {
-        db = at::empty({N}, dy.options());
+      if (need_b) db = at::empty({N}, dy.options());
+      if (need_w && !need_b) dw = product(c, Place8(from, K, T), N, K, T, Tensor(), false, nullptr, dy.options());
+      if (need_w && need_b) {                          // the bias sums ride along
+        const Place8 xc(from, K, T);
+        dw = at::empty({N, K}, dy.options());
+        const size_t need = tmpi_fp8_product_workspace_bytes((int)N, (int)K, (int)T);
+        Tensor ws;
+        if (need) ws = bytes_like(dy, (int64_t)need);
+        check(tmpi_fp8_product_sums(c.q, c.scale, xc.q, xc.scale, dw.data_ptr(), sums, (int)tiles, db.data_ptr(), (int)N, (int)K, (int)T, dtype_code(dy.scalar_type()), need ? ws.data_ptr() : nullptr,
+                                    need, stream()));
+        launched(FP8, need ? 2 : 1);
+      } else if (need_b) {
         check(tmpi_fp8_column_sums(sums, (int)tiles, (int)N, db.data_ptr(), dtype_code(dy.scalar_type()), stream()));
         launched(FP8, 1);
       }

@@ -389,15 +389,25 @@ size_t tmpi_fp8_scale_bytes(int64_t rows, int64_t cols);
 // q, scale: along the rows; qt, scalet: of the transpose; either may be null.  z: x is the gradient behind a GELU of z (dense), and x gelu'(z), rounded to the type, is
 // what is kept; sums [ceil(rows / 128), cols]: the columns' sums of that over 128 rows each.  Both need qt.
 int tmpi_fp8_quantize(const void* x, int64_t ld, const void* z, void* q, void* scale, void* qt, void* scalet, float* sums, int64_t rows, int64_t cols, int dtype, void* stream);
+typedef struct {
+  const void* x;
+  int64_t ld;
+  void *q, *scale, *qt, *scalet;
+  int64_t rows, cols;
+} tmpi_fp8_matrix_t;
+int tmpi_fp8_quantize_two(const tmpi_fp8_matrix_t* two, int dtype, void* stream);      // two matrices, both ways, in one launch
 int tmpi_fp8_column_sums(const float* sums, int tiles, int cols, void* db, int dtype, void* stream);
 int tmpi_fp8_restore(const void* q, const void* scale, void* x, int64_t rows, int64_t cols, int dtype, void* stream);
 // y [tokens, N] = x w^T (+ bias), then the GELU of what is rounded: few tokens that the kernel quantizes itself, weights in 8 bits
 int tmpi_fp8_few_tokens(void);
 int tmpi_fp8_few(const void* x, int64_t ld, const void* q, const void* scale, const void* bias, void* y, int tokens, int N, int K, int gelu, int dtype, void* stream);
-// c [M, N] = a b^T (+ bias), both in 8 bits, K columns; gelu: the GELU of the rounded sums, which go to z where it is given
+// c [M, N] = a b^T (+ bias), both in 8 bits, K columns; gelu: the GELU of the rounded sums, which go to z where it is given.  tmpi_fp8_product_sums: the same without
+// either, and db [M] = the columns' sums of `tiles` rows of sums [tiles, M] beside it.
 size_t tmpi_fp8_product_workspace_bytes(int M, int N, int K);
 int tmpi_fp8_product(const void* qa, const void* sa, const void* qb, const void* sb, const void* bias, void* c, void* z, int M, int N, int K, int gelu, int dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
+int tmpi_fp8_product_sums(const void* qa, const void* sa, const void* qb, const void* sb, void* c, const float* sums, int tiles, void* db, int M, int N, int K, int dtype,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 // ---------------------------------------------------------------- AdamW over many tensors (adamw.cu)
 typedef struct {

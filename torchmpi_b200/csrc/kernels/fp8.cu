@@ -186,21 +186,35 @@ __global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __r
 // ---------------------------------------------------------------- along columns, or both
 constexpr int TILE = 128, TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32, ROWS = 8;
 
+// One matrix, or two in one launch (the input and the weight of a layer): the blocks from a's tiles on take b's.
 // GELU: x is the gradient behind a GELU of z; what is kept is x gelu'(z), rounded to T.  q, scale: along the rows, or null.  sums: the columns'
-// sums over this tile's rows, [row tiles, cols], or null.
+// sums over this tile's rows, [row tiles, cols], or null; both are of a alone.
+template <typename T> struct Matrix {
+  const T* x;
+  long long ld;
+  uint8_t *q, *scale, *qt, *scalet;
+  int rows, cols, vec;
+};
 template <typename T, bool GELU>
 __global__ void __launch_bounds__(TILE_THREADS, sizeof(T) == 4 || GELU ? 2 : 3)
-quantize_tiles_kernel(const T* __restrict__ x, const long long ld, const T* __restrict__ z, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, uint8_t* __restrict__ qt,
-                      uint8_t* __restrict__ scalet, float* __restrict__ sums, const int rows, const int cols, const bool vec) {
+quantize_tiles_kernel(const Matrix<T> a, const Matrix<T> b, const T* __restrict__ z, float* __restrict__ sums_of_a) {
   using E = Eight<T>;
   constexpr int W = E::WORDS;
   __shared__ __align__(16) uint32_t tops[TILE_WARPS][16 * W];
   __shared__ __align__(16) float part[TILE_WARPS][TILE];
   __shared__ __align__(16) float column_inv[TILE];
   __shared__ __align__(16) uint8_t turned[TILE * TILE];
+  const int tiles_of_a = blocks_of(a.cols) * blocks_of(a.rows);
+  const bool second = (int)blockIdx.x >= tiles_of_a;
+  const T* x = second ? b.x : a.x;
   wait_previous(x, z);
-  const int t = threadIdx.x, cg = t & 15, rg = t >> 4, warp = t >> 5;
-  const int col_tiles = blocks_of(cols), cb = (int)(blockIdx.x % col_tiles), rb = (int)(blockIdx.x / col_tiles);
+  const long long ld = second ? b.ld : a.ld;
+  uint8_t *const q = second ? b.q : a.q, *const scale = second ? b.scale : a.scale, *const qt = second ? b.qt : a.qt, *const scalet = second ? b.scalet : a.scalet;
+  float* const sums = second ? nullptr : sums_of_a;
+  const int rows = second ? b.rows : a.rows, cols = second ? b.cols : a.cols;
+  const bool vec = second ? b.vec : a.vec;
+  const int t = threadIdx.x, cg = t & 15, rg = t >> 4, warp = t >> 5, tile = (int)blockIdx.x - (second ? tiles_of_a : 0);
+  const int col_tiles = blocks_of(cols), cb = tile % col_tiles, rb = tile / col_tiles;
   const int row0 = rb * TILE + rg * ROWS, col0 = cb * TILE + cg * 8, n = max(0, min(8, cols - col0));
   const bool whole = vec && (cb + 1) * TILE <= cols && (rb + 1) * TILE <= rows;      // no edge, no odd address
   uint32_t w[ROWS][W];
@@ -298,15 +312,15 @@ quantize_tiles_kernel(const T* __restrict__ x, const long long ld, const T* __re
   if (q) {
     // The 16 threads of a row exchange halves of their rows' maxima: lane cg is left with that of row cg / 2, whose scale it forms, and all take the
     // eight scales from there.
-    uint32_t a[4];
+    uint32_t m[4];
     const bool up8 = cg & 8, up4 = cg & 4, up2 = cg & 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = max(up8 ? top_row[4 + i] : top_row[i], __shfl_xor_sync(~0u, up8 ? top_row[i] : top_row[4 + i], 8));
+    for (int i = 0; i < 4; ++i) m[i] = max(up8 ? top_row[4 + i] : top_row[i], __shfl_xor_sync(~0u, up8 ? top_row[i] : top_row[4 + i], 8));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) a[i] = max(up4 ? a[2 + i] : a[i], __shfl_xor_sync(~0u, up4 ? a[i] : a[2 + i], 4));
-    a[0] = max(up2 ? a[1] : a[0], __shfl_xor_sync(~0u, up2 ? a[0] : a[1], 2));
-    a[0] = max(a[0], __shfl_xor_sync(~0u, a[0], 1));
-    const uint32_t byte = scale_byte(as_fp32<T>(a[0]));
+    for (int i = 0; i < 2; ++i) m[i] = max(up4 ? m[2 + i] : m[i], __shfl_xor_sync(~0u, up4 ? m[i] : m[2 + i], 4));
+    m[0] = max(up2 ? m[1] : m[0], __shfl_xor_sync(~0u, up2 ? m[0] : m[1], 2));
+    m[0] = max(m[0], __shfl_xor_sync(~0u, m[0], 1));
+    const uint32_t byte = scale_byte(as_fp32<T>(m[0]));
     if (!(cg & 1)) scale[scale_at(row0 + (cg >> 1), cb, groups_of(cols))] = (uint8_t)byte;
     const long long pitch = pitch_of(cols);
     uint8_t* to = q + row0 * pitch + col0;
@@ -617,8 +631,30 @@ int tmpi_fp8_quantize(const void* x, int64_t ld, const void* z, void* q, void* s
     }
     const long long tiles = (long long)fp8::blocks_of(rows) * fp8::blocks_of(cols);
     if (tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
-    return launch_overlapped(z ? fp8::quantize_tiles_kernel<T, true> : fp8::quantize_tiles_kernel<T, false>, (unsigned)tiles, fp8::TILE_THREADS, 0, s, (const T*)x, (long long)ld,
-                             (const T*)z, (uint8_t*)q, (uint8_t*)scale, (uint8_t*)qt, (uint8_t*)scalet, sums, (int)rows, (int)cols, vec);
+    const fp8::Matrix<T> a{(const T*)x, ld, (uint8_t*)q, (uint8_t*)scale, (uint8_t*)qt, (uint8_t*)scalet, (int)rows, (int)cols, vec};
+    return launch_overlapped(z ? fp8::quantize_tiles_kernel<T, true> : fp8::quantize_tiles_kernel<T, false>, (unsigned)tiles, fp8::TILE_THREADS, 0, s, a, a, (const T*)z, sums);
+  });
+}
+
+// Two matrices both ways in one launch.
+int tmpi_fp8_quantize_two(const tmpi_fp8_matrix_t* two, int dtype, void* stream) {
+  long long tiles = 0;
+  for (int i = 0; i < 2; ++i) {
+    const tmpi_fp8_matrix_t& m = two[i];
+    const int st = fp8::checked(m.rows, m.cols, "fp8_quantize_two");
+    if (st) return st;
+    if (!m.q || !m.qt || m.ld < m.cols || !m.rows) return fail(TMPI_ERR_INVALID, "fp8_quantize_two: nothing to write, or row pitch %lld for %lld columns", (long long)m.ld, (long long)m.cols);
+    if (!all_aligned16({m.q, m.scale, m.qt, m.scalet})) return fail(TMPI_ERR_INVALID, "fp8_quantize_two: results must be 16-byte aligned");
+    tiles += (long long)fp8::blocks_of(m.rows) * fp8::blocks_of(m.cols);
+  }
+  if (tiles > 0x7fffffffLL) return fail(TMPI_ERR_UNSUPPORTED, "fp8_quantize_two: %lld tiles", tiles);
+  return fp8::by_type(dtype, "fp8_quantize_two", [&](auto* type) -> cudaError_t {
+    using T = std::remove_pointer_t<decltype(type)>;
+    fp8::Matrix<T> m[2];
+    for (int i = 0; i < 2; ++i)
+      m[i] = {(const T*)two[i].x, two[i].ld, (uint8_t*)two[i].q, (uint8_t*)two[i].scale, (uint8_t*)two[i].qt, (uint8_t*)two[i].scalet, (int)two[i].rows, (int)two[i].cols,
+              fp8::whole_pieces({two[i].x}, two[i].ld, sizeof(T))};
+    return launch_overlapped(fp8::quantize_tiles_kernel<T, false>, (unsigned)tiles, fp8::TILE_THREADS, 0, (cudaStream_t)stream, m[0], m[1], (const T*)nullptr, (float*)nullptr);
   });
 }
 

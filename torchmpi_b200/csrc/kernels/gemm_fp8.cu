@@ -73,6 +73,9 @@ struct Problem {
   int by_tma;                  // the results' rows are 16-byte multiples
   const void* bias;
   void *c, *z;
+  const float* sums;           // [sum_tiles, M]: their sums over the first go to db, of the type db_type, while the first K blocks are under way; or null
+  void* db;
+  int sum_tiles, db_type;
   int* status;
 };
 
@@ -210,7 +213,7 @@ __device__ __forceinline__ uint32_t gelu_word(uint32_t w) {
 // Four (two) groups of four warps in each CTA take the tile's slices of 32 columns in turn.  A warp has 32 rows of a slice: it stages them in shared memory and
 // stores them through the TMA unit by itself, so that the warps meet nowhere.
 template <typename T, int MODE>
-__device__ __forceinline__ void epilogue(Shared* sh, unsigned char* staging, const Problem& p, const T* bias, int group, int quarter, int lane, uint32_t rank, int cluster, int clusters,
+__device__ __forceinline__ void epilogue(Shared* sh, unsigned char* staging, const Problem& p, const T* bias, const float* sums, int group, int quarter, int lane, uint32_t rank, int cluster, int clusters,
                                          const CUtensorMap* map_c, const CUtensorMap* map_z) {
   using L = Layout<T, MODE>;
   constexpr int WORDS = COLS * sizeof(T) / 4, ROW = COLS * sizeof(T), PIECES = ROW / 16;
@@ -222,6 +225,18 @@ __device__ __forceinline__ void epilogue(Shared* sh, unsigned char* staging, con
   int n = 0;
   for (int t = cluster; item_of(p, t, &it); t += clusters, ++n) {
     const int acc = n & 1;
+    if (MODE == PLAIN && sums && group == 0 && it.n_tile == 0 && it.slice == 0) {
+      const int row = (it.m_tile * 2 + (int)rank) * BM + quarter * 32 + lane;
+      if (row < p.M) {
+        float s = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < p.sum_tiles; ++i) s += sums[(size_t)i * p.M + row];
+        if (p.db_type == TMPI_BF16) ((__nv_bfloat16*)p.db)[row] = __float2bfloat16_rn(s);
+        else if (p.db_type == TMPI_F16) ((__half*)p.db)[row] = __float2half_rn(s);
+        else ((float*)p.db)[row] = s;
+      }
+      __syncwarp();
+    }
     if (!sm100::mbar_wait_warp(&sh->acc_full[acc], (n >> 1) & 1, kWaitBudgetNs, &sh->error)) { give_up(sh, p, 5); break; }
     sm100::tc_fence_after();
     const int row0 = (it.m_tile * 2 + (int)rank) * BM + quarter * 32, out0 = row0 + it.slice * p.slice_rows;
@@ -353,14 +368,15 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   sm100::cluster_sync();
   sm100::tc_fence_after();
   const T* bias = (const T*)p.bias;
-  wait_previous(bias);
+  const float* sums = p.sums;
+  wait_previous(bias, sums);
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
   if (warp == 0) {
     if (sm100::elect_one()) producer<L::STAGES>(sh, base, base + L::SF_AT, p, &map_a, &map_b, &map_sa, &map_sb, rank, cluster, clusters);
   } else if (warp == 1) {
     if (rank == 0 && sm100::elect_one()) issuer<L::STAGES>(sh, base, base + L::SF_AT, p, cluster, clusters);
   } else {
-    epilogue<T, MODE>(sh, base + L::STAGING_AT, p, bias, (warp - 2) >> 2, warp & 3, lane, rank, cluster, clusters, &map_c, &map_z);
+    epilogue<T, MODE>(sh, base + L::STAGING_AT, p, bias, sums, (warp - 2) >> 2, warp & 3, lane, rank, cluster, clusters, &map_c, &map_z);
   }
   __syncwarp();
   sm100::tc_fence_before();
@@ -479,13 +495,14 @@ static bool too_large(int64_t M, int64_t N, int64_t K) {
 
 template <typename T>
 static int run(const void* qa, const void* sa, const void* qb, const void* sb, const void* bias, void* c, void* z, int M, int N, int K, int gelu, void* ws, size_t ws_bytes,
-               cudaStream_t stream) {
+               cudaStream_t stream, const float* sums = nullptr, int sum_tiles = 0, void* db = nullptr, int db_type = 0) {
   const Plan pl = plan_of(M, N, fp8::blocks_of(K));
   const int groups = fp8::groups_of(K), es = sizeof(T);
   Problem p{};
   p.M = M; p.N = N; p.k_blocks = fp8::blocks_of(K);
   p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.bn = pl.bn; p.slices = pl.slices; p.slice_blocks = pl.slice_blocks;
   p.bias = bias; p.c = c; p.z = z;
+  p.sums = sums; p.sum_tiles = sum_tiles; p.db = db; p.db_type = db_type;
   p.status = gemm_status_word();
   CUtensorMap m[6];
   int st;
@@ -545,6 +562,19 @@ int tmpi_fp8_product(const void* qa, const void* sa, const void* qb, const void*
     case TMPI_F32: return gemm8::run<float>(qa, sa, qb, sb, bias, c, z, M, N, K, gelu, ws, ws_bytes, s);
   }
   return fail(TMPI_ERR_UNSUPPORTED, "fp8_product: dtype %d", dtype);
+}
+
+int tmpi_fp8_product_sums(const void* qa, const void* sa, const void* qb, const void* sb, void* c, const float* sums, int tiles, void* db, int M, int N, int K, int dtype, void* ws,
+                          size_t ws_bytes, void* stream) {
+  if (gemm8::too_large(M, N, K) || !sums || !db || tiles < 1) return fail(TMPI_ERR_INVALID, "fp8_product_sums: %d x %d x %d, %d rows of sums", M, N, K, tiles);
+  if (!all_aligned16({qa, sa, qb, sb, ws})) return fail(TMPI_ERR_INVALID, "fp8_product_sums: operands must be 16-byte aligned");
+  cudaStream_t s = (cudaStream_t)stream;
+  switch (dtype) {
+    case TMPI_BF16: return gemm8::run<__nv_bfloat16>(qa, sa, qb, sb, nullptr, c, nullptr, M, N, K, 0, ws, ws_bytes, s, sums, tiles, db, dtype);
+    case TMPI_F16: return gemm8::run<__half>(qa, sa, qb, sb, nullptr, c, nullptr, M, N, K, 0, ws, ws_bytes, s, sums, tiles, db, dtype);
+    case TMPI_F32: return gemm8::run<float>(qa, sa, qb, sb, nullptr, c, nullptr, M, N, K, 0, ws, ws_bytes, s, sums, tiles, db, dtype);
+  }
+  return fail(TMPI_ERR_UNSUPPORTED, "fp8_product_sums: dtype %d", dtype);
 }
 
 }  // extern "C"
