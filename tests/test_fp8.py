@@ -130,6 +130,23 @@ def test_the_forms_of_the_products_are_met():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HALF, FP32])
+@pytest.mark.parametrize("T", [1, 8, 9, 16, 17, 32])
+@pytest.mark.parametrize("K,N", [(4096, 1000), (8192, 24), (2100, 590), (3000, 2368), (127, 5000)])
+def test_few_tokens(T, K, N, dtype):
+    """One block, or two or four of them, to the blocks of K; odd numbers of weight rows."""
+    g = torch.Generator().manual_seed(T + K + N)
+    x, w, b = torch.randn(T, K, generator=g).to(dtype), (torch.randn(N, K, generator=g) * K ** -0.5).to(dtype), torch.randn(N, generator=g).to(dtype)
+    for bias in (None, b):
+        y = fp8.linear(x.cuda(), fp8.quantize(w.cuda()), None if bias is None else bias.cuda())
+        want, bound = ref.product(ref.kept(x), ref.kept(w), bias)
+        ref.close(y, want, bound + ref.half_step(want.abs() + bound, dtype), "y")
+        assert torch.equal(y, fp8.linear(x.cuda(), fp8.quantize(w.cuda()), None if bias is None else bias.cuda()))
+        one = fp8.linear(x[-1:].cuda(), fp8.quantize(w.cuda()), None if bias is None else bias.cuda())
+        assert torch.equal(one[0], y[-1])                    # a token's results do not depend on the others
+
+
+@gpu
 def test_rows_and_columns_are_independent():
     """A row's results do not depend on the others, and NaN stays with its row or column."""
     g = torch.Generator().manual_seed(3)

@@ -178,21 +178,6 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
   for (uint32_t c = blockIdx.x; c < chunks; at = entry_of(table, s.entries, c)) {      // one tensor after another
     const Entry& e = table.entry[at];
     const float t = (float)(s.steps[(e.which & (COUNTED - 1)) >> 8] + (e.which & COUNTED ? 0 : 1));
-    if (t != seen || (e.which & 0xff) != seen_group) {
-      seen = t;
-      seen_group = e.which & 0xff;
-      const Group& g = table.group[seen_group];
-      const float lr = g.device_lr ? *g.device_lr : g.lr;
-      // The update is m / (sqrt(v) unbias + eps) with the rate lr / (1 - b1^t) in the divisor (a rate below 1e-30, whose inverse may be no number, counts as 0: an
-      // infinite divisor), and of what is squared on its way into v the root is taken here.
-      const float step = lr / -expm1f(t * g.log_beta1);
-      const bool moves = step >= 1e-30f;
-      unbias = moves ? rsqrtf(-expm1f(t * g.log_beta2)) / step : 0.f;
-      eps = moves ? fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step : __uint_as_float(0x7f800000u);
-      keep = 1.f - lr * g.decay;
-      b1 = g.beta1, b2 = g.beta2, a1 = g.rest1 * coefficient, a2 = sqrtf(g.rest2) * coefficient;
-      unit_m = b1 * (1.f / 16129.f), unit_v = sqrtf(b2) * (1.f / 65025.f);
-    }
     const uint32_t e0 = e.chunk, end = at + 1 < s.entries ? table.entry[at + 1].chunk : chunks, extent = e.n, whole = (extent + BLOCK - 1) / BLOCK * BLOCK;
     T* const param = (T*)e.param;
     const T* const grads = (const T*)e.grad;
@@ -215,17 +200,33 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
         }
       }
       const size_t p0 = place + first;
+      uint2 cm = make_uint2(0u, 0u), cv = cm;
+      float um = 0.f, uv = 0.f;
+      if (BITS == 8 && padded(0)) {
+        cm = *reinterpret_cast<const uint2*>((const uint8_t*)s.m + p0);
+        cv = *reinterpret_cast<const uint2*>((const uint8_t*)s.v + p0);
+        um = s.m_top[p0 / BLOCK];
+        uv = s.v_top[p0 / BLOCK];
+      }
+      // behind the loads: a small step is as long as its chain of latencies
+      if (t != seen || (e.which & 0xff) != seen_group) {
+        seen = t;
+        seen_group = e.which & 0xff;
+        const Group& g = table.group[seen_group];
+        const float lr = g.device_lr ? *g.device_lr : g.lr;
+        // The update is m / (sqrt(v) unbias + eps) with the rate lr / (1 - b1^t) in the divisor (a rate below 1e-30, whose inverse may be no number, counts as 0: an
+        // infinite divisor), and of what is squared on its way into v the root is taken here.
+        const float step = lr / -expm1f(t * g.log_beta1);
+        const bool moves = step >= 1e-30f;
+        unbias = moves ? rsqrtf(-expm1f(t * g.log_beta2)) / step : 0.f;
+        eps = moves ? fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step : __uint_as_float(0x7f800000u);
+        keep = 1.f - lr * g.decay;
+        b1 = g.beta1, b2 = g.beta2, a1 = g.rest1 * coefficient, a2 = sqrtf(g.rest2) * coefficient;
+        unit_m = b1 * (1.f / 16129.f), unit_v = sqrtf(b2) * (1.f / 65025.f);
+      }
       if constexpr (BITS == 8) {                       // times the decay of the averages, which enters the units
-        uint2 cm = make_uint2(0u, 0u), cv = cm;
-        float um = 0.f, uv = 0.f;
-        if (padded(0)) {
-          cm = *reinterpret_cast<const uint2*>((const uint8_t*)s.m + p0);
-          cv = *reinterpret_cast<const uint2*>((const uint8_t*)s.v + p0);
-          um = s.m_top[p0 / BLOCK] * unit_m;
-          uv = s.v_top[p0 / BLOCK] * unit_v;
-        }
-        decode_m(cm.x, um, m), decode_m(cm.y, um, m + 4);
-        decode_v(cv.x, uv, v), decode_v(cv.y, uv, v + 4);
+        decode_m(cm.x, um * unit_m, m), decode_m(cm.y, um * unit_m, m + 4);
+        decode_v(cv.x, uv * unit_v, v), decode_v(cv.y, uv * unit_v, v + 4);
       }
       float r[PER];
 #pragma unroll
@@ -266,8 +267,7 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
       }
     }
   }
-  // The last block to come counts the step: all others have read the counts.
-  __threadfence();
+  // The last block to come counts the step.  All others have read the counts then, and need no fence for it: what they read has decided about their branches.
   __syncthreads();
   if (threadIdx.x == 0) ticket = atomicAdd(s.counter, 1u);
   __syncthreads();

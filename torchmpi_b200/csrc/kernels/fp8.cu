@@ -8,6 +8,7 @@
 #include "fp8.cuh"
 #include "gelu.cuh"
 #include "pdl.cuh"
+#include "sm100_ptx.cuh"
 #include "vec.cuh"
 #include "../include/tmpi_c_api.h"
 #include "../runtime/common.h"
@@ -468,6 +469,8 @@ __global__ void __launch_bounds__(ROW_THREADS) restore_kernel(const uint8_t* __r
 // quantizes the tokens' blocks itself, straight into the operand registers of mma.sync (16 weight rows x 8 tokens x 32 of K): which K
 // index stands where is free as long as both operands agree, so a thread's 32 bytes of a weight row are the 32 consecutive ones of its quarter of the
 // block, and so are the tokens'.  The sums of a block are scaled into fp32 sums.  The next block's weights are under way meanwhile.
+// Few weight rows leave SMs idle: then two or four blocks, a cluster, share the blocks of K, and the first adds what the others leave in its shared memory, in order
+// (13 tokens, 4096 -> 1024: BATCH_US us).
 constexpr int FEW_ROWS = 16, FEW_WARPS = 16;
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -485,8 +488,11 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict
                                                              const T* __restrict__ bias, T* __restrict__ y, const int tokens, const int N, const int K, const int gelu, const bool vec) {
   using E = Eight<T>;
   __shared__ float part[FEW_WARPS][FEW_ROWS][NT * 8 + 1];
+  __shared__ float others[3][FEW_ROWS * NT * 8];
   wait_previous(x, q, scale, bias);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
+  const int share = blockIdx.y, shares = gridDim.y;          // of the blocks of K; the rank in the cluster
+  if (shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // started: waited for before its shared memory is written to
+  const int lane = threadIdx.x & 31, in_block = threadIdx.x >> 5, warp = in_block * shares + share, warps = (blockDim.x >> 5) * shares, g = lane >> 2, t = lane & 3;
   const int blocks = blocks_of(K), groups = groups_of(K), n0 = blockIdx.x * FEW_ROWS;
   const long long pitch = pitch_of(K);
   const int r0 = min(n0 + g, N - 1), r1 = min(n0 + g + 8, N - 1);
@@ -555,17 +561,29 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    part[warp][g][i * 8 + 2 * t] = acc[i][0];
-    part[warp][g][i * 8 + 2 * t + 1] = acc[i][1];
-    part[warp][g + 8][i * 8 + 2 * t] = acc[i][2];
-    part[warp][g + 8][i * 8 + 2 * t + 1] = acc[i][3];
+    part[in_block][g][i * 8 + 2 * t] = acc[i][0];
+    part[in_block][g][i * 8 + 2 * t + 1] = acc[i][1];
+    part[in_block][g + 8][i * 8 + 2 * t] = acc[i][2];
+    part[in_block][g + 8][i * 8 + 2 * t + 1] = acc[i][3];
   }
   __syncthreads();
+  if (shares > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (share)
+      for (int i = threadIdx.x; i < FEW_ROWS * tokens; i += blockDim.x) {
+        float s = 0.f;
+        for (int v = 0; v < (int)(blockDim.x >> 5); ++v) s += part[v][i & (FEW_ROWS - 1)][i / FEW_ROWS];
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(sm100::map_to_cta(&others[share - 1][i], 0)), "f"(s) : "memory");
+      }
+    sm100::cluster_sync();
+    if (share) return;
+  }
   for (int i = threadIdx.x; i < FEW_ROWS * tokens; i += blockDim.x) {
     const int r = i & (FEW_ROWS - 1), token = i / FEW_ROWS;
     if (n0 + r >= N) continue;
     float s = 0.f;
-    for (int v = 0; v < warps; ++v) s += part[v][r][token];
+    for (int v = 0; v < (int)(blockDim.x >> 5); ++v) s += part[v][r][token];
+    for (int v = 1; v < shares; ++v) s += others[v - 1][i];
     if (bias) s += (float)to_acc<T>(bias[n0 + r]);
     T out = from_acc<T>((typename AccOf<T>::type)s);
     if (gelu) {
@@ -687,8 +705,22 @@ int tmpi_fp8_few(const void* x, int64_t ld, const void* q, const void* scale, co
   return fp8::by_type(dtype, "fp8_few", [&](auto* type) -> cudaError_t {
     using T = std::remove_pointer_t<decltype(type)>;
     const auto kernel = tokens <= 8 ? fp8::few_kernel<T, 1> : tokens <= 16 ? fp8::few_kernel<T, 2> : fp8::few_kernel<T, 4>;
-    return launch_overlapped(kernel, (N + fp8::FEW_ROWS - 1) / fp8::FEW_ROWS, 32 * std::min(fp8::FEW_WARPS, fp8::blocks_of(K)), 0, (cudaStream_t)stream, (const T*)x, (long long)ld, (const uint8_t*)q,
-                             (const uint8_t*)scale, (const T*)bias, (T*)y, tokens, N, K, gelu, fp8::whole_pieces({x}, ld, sizeof(T)));
+    // Shares of K as long as the blocks fit the SMs and each has blocks of K for half its warps.  More blocks than SMs have eight warps, so that two fit an SM (4 tokens, 4096 -> 4096:
+    // 12.3 -> WIDE_US us).
+    const int groups = (N + fp8::FEW_ROWS - 1) / fp8::FEW_ROWS, blocks = fp8::blocks_of(K);
+    int shares = 1;
+    while (shares < 4 && groups * shares * 2 <= 148 && blocks >= shares * fp8::FEW_WARPS) shares *= 2;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = 1; at[1].val.clusterDim.y = (unsigned)shares; at[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)groups, (unsigned)shares);
+    cfg.blockDim = dim3(32 * std::min(groups > 148 ? fp8::FEW_WARPS / 2 : fp8::FEW_WARPS, (blocks + shares - 1) / shares));
+    cfg.stream = (cudaStream_t)stream; cfg.attrs = at; cfg.numAttrs = shares > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, (const T*)x, (long long)ld, (const uint8_t*)q, (const uint8_t*)scale, (const T*)bias, (T*)y, tokens, N, K, gelu,
+                              fp8::whole_pieces({x}, ld, sizeof(T)));
   });
 }
 
