@@ -343,6 +343,28 @@ def test_state_dict(bits, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_checkpoint(bits, device, tmp_path):
+    """A checkpoint file holds it beside the model; a resumed run takes the same steps."""
+    from torchmpi_b200.utils import checkpoint
+
+    def run(net, opt, steps):
+        for i in steps:
+            for p, g in zip(net.parameters(), _grads([q.shape for q in net.parameters()], BF, i)):
+                p.grad = g.to(device)
+            opt.step(1e-2)
+    torch.manual_seed(0)
+    a, b = (torch.nn.Linear(40, 30).to(BF).to(device) for _ in range(2))
+    one, two = (adamw.AdamW(m.parameters(), bits=bits) for m in (a, b))
+    run(a, one, range(2))
+    checkpoint.save(str(tmp_path / "state.pt"), a, one)
+    run(a, one, range(2, 4))
+    checkpoint.load(str(tmp_path / "state.pt"), b, two)
+    run(b, two, range(2, 4))
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters())) and torch.equal(one.masters(), two.masters())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_options_between_steps_and_refreshed_masters(device):
     p = torch.zeros(4, device=device, dtype=BF).requires_grad_(True)
     opt = adamw.AdamW([p], lr=1.0, weight_decay=0.0, eps=1e-6)

@@ -203,6 +203,8 @@ class AdamW:
         for p, i in zip(self._params, which):
             if p.grad is None or not p.numel():
                 continue
+            if p.grad.is_sparse or p.grad.shape != p.shape:
+                raise ValueError(f"AdamW: a gradient that is not its parameter's: {tuple(p.grad.shape)}")
             st, (rate, b1, b2, eps, decay) = self.state[p], options[i]
             rate = float(rate if rates[i] is None else rates[i])
             st["step"] += 1

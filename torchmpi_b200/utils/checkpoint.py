@@ -3,7 +3,7 @@
 The reference has no save / load at all (parameter-server shards live in host memory and vanish at
 ``free``, lib/parameterserver.cpp:277-280).  Here a checkpoint is a plain PyTorch file written by
 rank 0: the model's ``state_dict`` (parameters are replicated, so rank 0's copy is the model), and,
-when the fused optimizer is in use, its gathered fp32 master weights and momentum, and, when parameter
+when an optimizer is given, its state (of the fused one the gathered fp32 master weights and momentum, of AdamW averages, step counts and masters), and, when parameter
 servers are passed, the tensors they hold (pulled from their shards before the file is written).  ``load``
 restores them on every rank, re-synchronises the parameters from rank 0 and writes the saved tensors
 back into the parameter servers.
@@ -54,8 +54,8 @@ def load(path: str, model: torch.nn.Module, optimizer=None, synchronize: bool = 
         mpinn.synchronize_parameters(model)
     if optimizer is not None and "optimizer" in state and hasattr(optimizer, "load_state_dict"):
         optimizer.load_state_dict(state["optimizer"])
-        if hasattr(optimizer, "refresh_master") and state["optimizer"]["buckets"] and \
-                state["optimizer"]["buckets"][0].get("master") is None:
+        buckets = state["optimizer"].get("buckets")                # of the fused optimizer
+        if hasattr(optimizer, "refresh_master") and buckets and buckets[0].get("master") is None:
             optimizer.refresh_master()
     if parameter_servers and "parameter_servers" in state:
         if len(parameter_servers) != len(state["parameter_servers"]):
