@@ -478,6 +478,26 @@ def test_refuses_what_has_moved():
     assert int(opt.state[q]["step"]) == 0
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_refuses_another_order_or_type_of_a_parameter(device):
+    """The states lie in the order that the parameter had: in another they would be those of other elements."""
+    for change in (lambda q: q.data.t().contiguous().t(), lambda q: q.data.bfloat16(), lambda q: q.data.reshape(6, 4)):
+        q = torch.randn(4, 6, device=device).requires_grad_(True)
+        before = torch.randn(3, device=device).requires_grad_(True)
+        opt = adamw.AdamW([q, before])
+        q.data = change(q)
+        q.grad = torch.zeros_like(q)
+        with pytest.raises(ValueError):
+            opt.step()
+        assert int(opt.state[q]["step"]) == 0
+    q = torch.randn(1, 6, device=device).requires_grad_(True)          # a dimension of one element has no order
+    opt = adamw.AdamW([q])
+    q.data = torch.randn(6, 1, device=device).t()
+    q.grad = torch.ones_like(q)
+    opt.step()
+    assert int(opt.state[q]["step"]) == 1
+
+
 def test_the_entry_points_refuse():
     """What no Python caller passes on: no launch comes of it."""
     assert lib.tmpi_adamw_max_groups() == 8

@@ -5,6 +5,7 @@ import sys
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 import torch.nn.functional as F
 
 import fp8_reference as ref
@@ -349,6 +350,21 @@ def test_second_derivatives_are_refused(device):
     y = fp8.linear(x, w)
     with pytest.raises(RuntimeError, match="once"):
         torch.autograd.grad(y.sum(), (x, w), create_graph=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_tangents_are_refused(device):
+    """A result without a tangent would stand for a derivative of zero, and one through the rounding to 8 bits for a rounded derivative."""
+    x, w, b = torch.randn(4, 200, device=device), torch.randn(16, 200, device=device), torch.randn(16, device=device)
+    m = fp8.quantize(w)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))      # noqa: E731
+        for args in ((dual(x), w, b), (x, dual(w), b), (x, w, dual(b)), (dual(x), m, b), (x, m, dual(b))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises((NotImplementedError, RuntimeError, ValueError)):
+                    fp8.linear(*args)
+        assert fwd.unpack_dual(fp8.dequantize(fp8.quantize(dual(x)))).tangent is None
+        assert torch.equal(fp8.linear(x, m, b), fp8.linear(x, w, b))
 
 
 def test_the_entry_points_refuse():

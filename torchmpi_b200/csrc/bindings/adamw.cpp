@@ -16,12 +16,20 @@ Tensor in_order(const Tensor& g, const Tensor& p) {
   c.copy_(g);
   return c;
 }
+bool in_same_order(const Tensor& p, const std::vector<int64_t>& strides) {
+  if (p.dim() != (int64_t)strides.size()) return false;
+  for (int64_t d = 0; d < p.dim(); ++d)
+    if (p.size(d) != 1 && p.stride(d) != strides[d]) return false;
+  return true;
+}
 bool taken(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf || t == at::kFloat; }
 constexpr at::ScalarType TYPES[] = {at::kBFloat16, at::kHalf, at::kFloat};
 
 struct AdamW {
   std::vector<Tensor> params;
   std::vector<int64_t> places, sizes;
+  std::vector<std::vector<int64_t>> strides;                        // the order of the states
+  std::vector<at::ScalarType> types;
   std::vector<int> group;
   Tensor m, v, m_top, v_top, master, steps, counter, norm;
   int bits;
@@ -47,7 +55,8 @@ struct AdamW {
       const Tensor& grad = p.grad();
       if (!grad.defined() || !sizes[i]) continue;
       TORCH_CHECK_VALUE(p.is_cuda() && p.get_device() == device, "AdamW: a parameter on ", p.device(), ", but the current device is cuda:", device);
-      TORCH_CHECK_VALUE(p.numel() == sizes[i] && p.is_non_overlapping_and_dense() && taken(p.scalar_type()), "AdamW: a parameter has changed: ", p.scalar_type(), " ", p.sizes());
+      TORCH_CHECK_VALUE(p.numel() == sizes[i] && p.scalar_type() == types[i] && in_same_order(p, strides[i]) && p.is_non_overlapping_and_dense(), "AdamW: a parameter has changed: ", p.scalar_type(), " ", p.sizes(),
+                        " with strides ", p.strides());
       TORCH_CHECK_VALUE(!grad.is_sparse() && grad.layout() == at::kStrided && grad.device() == p.device() && grad.sizes() == p.sizes(), "AdamW: a gradient that is not its parameter's: ", grad.sizes());
       const Tensor ordered = in_order(grad, p);
       if (!ordered.is_same(grad)) kept.push_back(ordered);
@@ -94,7 +103,11 @@ void register_adamw(pybind11::module_& m) {
       .def(pybind11::init([](std::vector<Tensor> params, std::vector<int64_t> places, std::vector<int> group, Tensor m_, Tensor v, const OptTensor& m_top, const OptTensor& v_top, const OptTensor& master,
                              Tensor steps, Tensor counter, Tensor norm, int bits) {
         AdamW a;
-        for (const Tensor& p : params) a.sizes.push_back(p.numel());
+        for (const Tensor& p : params) {
+          a.sizes.push_back(p.numel());
+          a.strides.push_back(p.strides().vec());
+          a.types.push_back(p.scalar_type());
+        }
         a.params = std::move(params); a.places = std::move(places); a.group = std::move(group);
         a.m = m_; a.v = v; a.m_top = or_none(m_top); a.v_top = or_none(v_top); a.master = or_none(master);
         a.steps = steps; a.counter = counter; a.norm = norm; a.bits = bits;

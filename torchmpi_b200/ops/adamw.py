@@ -119,6 +119,7 @@ class AdamW:
             raise ValueError(f"AdamW: {len(self.param_groups)} groups of parameters, up to 8 are taken")
         self._options()
         self._params: List[torch.Tensor] = [p for g in self.param_groups for p in g["params"]]
+        self._made = [(p.dtype, p.shape, self._order(p)) for p in self._params]          # the states' order
         group = [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
         if not self._params or len({id(p) for p in self._params}) < len(self._params):
             raise ValueError("AdamW: no parameters, or one of them twice")
@@ -158,6 +159,10 @@ class AdamW:
         self._native = None
         if device.type == "cuda":
             self._native = _native.ext().AdamW(self._params, self._places[:-1], group, self._m, self._v, self._m_top, self._v_top, self._master, self._steps, self._counter, self._norm, bits)
+
+    @staticmethod
+    def _order(p: torch.Tensor) -> List[int]:
+        return [t for s, t in zip(p.shape, p.stride()) if s != 1]
 
     def _has_master(self, p: torch.Tensor) -> bool:
         return self._master is not None and p.dtype != torch.float32
@@ -200,9 +205,11 @@ class AdamW:
             self._norm.copy_(abs(scale) * grad_norm(grads) if grads else torch.zeros(()))
             scale = scale * torch.clamp_max(self.max_norm / (self._norm + 1e-6), 1)
         which = [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
-        for p, i in zip(self._params, which):
+        for p, i, made in zip(self._params, which, self._made):
             if p.grad is None or not p.numel():
                 continue
+            if (p.dtype, p.shape, self._order(p)) != made:
+                raise ValueError(f"AdamW: a parameter has changed: {p.dtype} {tuple(p.shape)} with strides {p.stride()}")
             if p.grad.is_sparse or p.grad.shape != p.shape:
                 raise ValueError(f"AdamW: a gradient that is not its parameter's: {tuple(p.grad.shape)}")
             st, (rate, b1, b2, eps, decay) = self.state[p], options[i]

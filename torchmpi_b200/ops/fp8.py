@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as fwd
 import torch.nn.functional as F
 
 from .. import _native
@@ -212,6 +213,8 @@ def linear(x: torch.Tensor, w: Union[torch.Tensor, Block8], bias: Optional[torch
             raise ValueError(f"linear expects x [..., {w.cols}] and a bias [{w.q.shape[0]}] of its type, got {x.dtype} {tuple(x.shape)}")
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise ValueError("linear: weights kept in 8 bits have no backward pass (use the tensor, or torch.no_grad())")
+        if any(t is not None and fwd.unpack_dual(t).tangent is not None for t in (x, bias)):
+            raise ValueError("linear: the derivative of products in 8 bits is formed backward, not forward")
         same_device("linear", x, w.q, w.scale, bias)
         wide = torch.promote_types(x.dtype, torch.float32)
         z = F.linear(_dequantize(_quantize(x.reshape(-1, w.cols)), wide), _dequantize(w, wide), None if bias is None else bias.to(wide)).to(x.dtype)
