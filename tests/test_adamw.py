@@ -479,6 +479,24 @@ def test_refuses_what_has_moved():
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_a_loaded_learning_rate_lies_where_it_lay(device):
+    """On the parameters' device, and in the tensor that a captured step reads, wherever the saved one lies."""
+    made = lambda lr: adamw.AdamW([torch.zeros(5, device=device).requires_grad_(True)], lr=lr)      # noqa: E731
+    saved = made(torch.tensor(0.25, device=device)).state_dict()
+    saved["param_groups"][0]["lr"] = saved["param_groups"][0]["lr"].cpu()
+    rate = torch.tensor(0.5, device=device)
+    for opt in (made(rate), made(0.5)):
+        opt.load_state_dict(saved)
+        lr = opt.param_groups[0]["lr"]
+        assert lr.device == rate.device and float(lr) == 0.25 and lr is not saved["param_groups"][0]["lr"]
+        p = next(iter(opt.state))
+        p.grad = torch.ones_like(p)
+        opt.step()
+        assert torch.allclose(p.detach(), torch.full_like(p, -0.25), rtol=1e-6)          # the first step has the rate's length
+    assert float(rate) == 0.25
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_refuses_another_order_or_type_of_a_parameter(device):
     """The states lie in the order that the parameter had: in another they would be those of other elements."""
     for change in (lambda q: q.data.t().contiguous().t(), lambda q: q.data.bfloat16(), lambda q: q.data.reshape(6, 4)):

@@ -113,7 +113,7 @@ def build_bindings(force: bool = False) -> Path:
         with cf.ThreadPoolExecutor(max_workers=len(objs)) as ex:
             list(ex.map(lambda so: run([cxx, *flags, "-c", str(so[0]), "-o", str(so[1])], so[0].name), zip(BINDINGS_SRC, objs)))
         run([cxx, "-shared", *map(str, objs), "-o", str(tmp), "-L", str(root / "lib"),
-             "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root / 'lib'}"], BINDINGS.name)
+             "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root / 'lib'}"], BINDINGS.name)
         tmp.replace(BINDINGS)
         BINDINGS_STAMP.write_text(bindings_hash())
     return BINDINGS

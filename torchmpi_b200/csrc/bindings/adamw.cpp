@@ -74,8 +74,8 @@ struct AdamW {
     if (max_norm.has_value()) {
       int total = 0, used = 0;
       for (const auto& t : tables) total += tmpi_norm_sums((int)t.size());
-      sums = at::empty({total}, steps.options().dtype(at::kDouble));
-      coefficient = at::empty({1}, steps.options().dtype(at::kFloat));
+      sums = fresh({total}, at::kDouble);
+      coefficient = fresh({1}, at::kFloat);
       for (int c = 0; c < 3; ++c) {
         int n = 0;
         if (!tables[c].empty()) check(tmpi_norm_squares(tables[c].data(), (int)tables[c].size(), dtype_code(TYPES[c]), sums.data_ptr<double>() + used, &n, stream()));
@@ -116,7 +116,7 @@ void register_adamw(pybind11::module_& m) {
       .def("step", &AdamW::step);
   m.def("adamw_values", [](const Tensor& mq, const Tensor& m_top, const Tensor& vq, const Tensor& v_top, int code) {
     const auto type = code == TMPI_F32 ? at::kFloat : code == TMPI_F16 ? at::kHalf : at::kBFloat16;
-    Tensor a = at::empty({mq.numel()}, m_top.options().dtype(type)), b = at::empty_like(a);
+    Tensor a = fresh({mq.numel()}, type), b = fresh({mq.numel()}, type);
     check(tmpi_adamw_values(mq.data_ptr(), m_top.data_ptr<float>(), vq.data_ptr(), v_top.data_ptr<float>(), a.data_ptr(), b.data_ptr(), mq.numel() / 128, code, stream()));
     launched(ADAMW, 1);
     return std::make_pair(a, b);
@@ -136,7 +136,7 @@ void register_adamw(pybind11::module_& m) {
     }
     if (kept.empty()) return c10::nullopt;
     for (const auto& t : tables) total += tmpi_norm_sums((int)t.size());
-    const Tensor sums = at::empty({total}, kept[0].options().dtype(at::kDouble)), norm = at::empty({}, kept[0].options().dtype(at::kFloat));
+    const Tensor sums = fresh({total}, at::kDouble), norm = fresh({}, at::kFloat);
     for (int c = 0; c < 3; ++c) {
       int n = 0;
       if (!tables[c].empty()) check(tmpi_norm_squares(tables[c].data(), (int)tables[c].size(), dtype_code(TYPES[c]), sums.data_ptr<double>() + used, &n, stream()));

@@ -1,6 +1,7 @@
 // What the autograd functions of autograd.cpp and experts.cpp share.
 #pragma once
 #include <torch/extension.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <atomic>
@@ -53,6 +54,9 @@ inline Tensor packed(const Tensor& t, at::MemoryFormat format = at::MemoryFormat
 
 // A saved tensor as it was saved: hooks (torch.autograd.graph.save_on_cpu, say) may hand it back in another layout.
 inline Tensor as_saved(const Tensor& t, at::MemoryFormat format = at::MemoryFormat::Contiguous) { return t.defined() ? packed(t, format) : t; }
+
+// An uninitialized tensor on the current device, past the dispatcher (half a microsecond for each of a small call's).
+inline Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) { return Tensor(at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, c10::cuda::current_device()), c10::nullopt)); }
 
 using OptTensor = c10::optional<Tensor>;
 inline Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }

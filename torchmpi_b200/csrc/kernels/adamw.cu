@@ -417,8 +417,9 @@ static Filled fill(Table<CAP>* t, const tmpi_adamw_tensor_t* tensors, int count,
 
 template <typename T, int CAP>
 static cudaError_t launch_step(const Table<CAP>& t, const States& s, int bits, uint32_t chunks, cudaStream_t stream) {
-  const bool master = s.master != nullptr;
-  const auto kernel = bits == 8 ? (master ? step_kernel<T, 8, true, CAP> : step_kernel<T, 8, false, CAP>) : (master ? step_kernel<T, 32, true, CAP> : step_kernel<T, 32, false, CAP>);
+  constexpr bool MASTERS = sizeof(T) == 2;               // fp32 has none
+  const bool master = MASTERS && s.master;
+  const auto kernel = bits == 8 ? (master ? step_kernel<T, 8, MASTERS, CAP> : step_kernel<T, 8, false, CAP>) : (master ? step_kernel<T, 32, MASTERS, CAP> : step_kernel<T, 32, false, CAP>);
   return launch_overlapped(kernel, std::min<uint32_t>(chunks, 148 * 5), THREADS, 0, stream, t, s, chunks);
 }
 

@@ -128,7 +128,7 @@ __device__ __forceinline__ uint2 eight(const uint32_t* w, float inv) {
 
 // ---------------------------------------------------------------- along rows
 // Eight threads to a block of 128, sixteen elements each, two of a thread's pieces under way at a time (16 bytes by each thread, so that a warp's loads
-// are whole lines, took more instructions for an element and 25.7 us in place of ROWS_US at 8192 x 4096).
+// are whole lines, took more instructions for an element and 25.7 us in place of 18.1 at 8192 x 4096).
 constexpr int ROW_THREADS = 256;
 struct Stride { int rows, pieces; };          // a launch's threads, as rows of pieces: what a thread's next piece lies further
 
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(ROW_THREADS) restore_kernel(const uint8_t* __r
 // index stands where is free as long as both operands agree, so a thread's 32 bytes of a weight row are the 32 consecutive ones of its quarter of the
 // block, and so are the tokens'.  The sums of a block are scaled into fp32 sums.  The next block's weights are under way meanwhile.
 // Few weight rows leave SMs idle: then two or four blocks, a cluster, share the blocks of K, and the first adds what the others leave in its shared memory, in order
-// (13 tokens, 4096 -> 1024: BATCH_US us).
+// (13 tokens, 4096 -> 1024: 6.5 us, 8.1 without the sharing).
 constexpr int FEW_ROWS = 16, FEW_WARPS = 16;
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -487,6 +487,7 @@ template <typename T, int NT>
 __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict__ x, const long long ld, const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale,
                                                              const T* __restrict__ bias, T* __restrict__ y, const int tokens, const int N, const int K, const int gelu, const bool vec) {
   using E = Eight<T>;
+  constexpr int AT_ONCE = NT == 4 ? (sizeof(T) == 2 ? 2 : 1) : NT;          // groups of eight tokens whose loads are under way together: all of four spilled registers
   __shared__ float part[FEW_WARPS][FEW_ROWS][NT * 8 + 1];
   __shared__ float others[3][FEW_ROWS * NT * 8];
   wait_previous(x, q, scale, bias);
@@ -516,29 +517,33 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict
 #pragma unroll 1
   for (int b = warp; b < blocks; b += warps) {
     const int col = b * BLOCK + t * 32;
-    uint32_t v[NT][4][E::WORDS];
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        load8<T>(x + (long long)(i * 8 + g) * ld + col + 8 * j, i * 8 + g < tokens ? min(8, max(0, K - col - 8 * j)) : 0, vec, v[i][j]);
     const uint4 a[4] = {next[0], next[1], next[2], next[3]};
     const uint32_t sw[2] = {next_scale[0], next_scale[1]};
     if (b + warps < blocks) fetch(b + warps);
+    uint32_t v[AT_ONCE][4][E::WORDS];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       if (i * 8 >= tokens) break;
+      if (i % AT_ONCE == 0) {
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int token = (i + u) * 8 + g;
+            load8<T>(x + (long long)token * ld + col + 8 * j, token < tokens ? min(8, max(0, K - col - 8 * j)) : 0, vec, v[u][j]);
+          }
+      }
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int k = 0; k < E::WORDS; ++k) top = E::largest(top, v[i][j][k]);
+        for (int k = 0; k < E::WORDS; ++k) top = E::largest(top, v[i % AT_ONCE][j][k]);
       top = of_word<T>(top);
       const bool finite = __all_sync(~0u, top < E::INF);
       if (!finite) {
         top = 0;
 #pragma unroll
-        for (int k = 0; k < 4 * E::WORDS; ++k) top = max(top, of_word<T>(finite_part<T>(v[i][k / E::WORDS][k % E::WORDS])));
+        for (int k = 0; k < 4 * E::WORDS; ++k) top = max(top, of_word<T>(finite_part<T>(v[i % AT_ONCE][k / E::WORDS][k % E::WORDS])));
       }
       top = max(top, __shfl_xor_sync(~0u, top, 1));
       top = max(top, __shfl_xor_sync(~0u, top, 2));
@@ -547,7 +552,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict
       float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {                    // 8 of the thread's 32 bytes for each of the four instructions
-        const uint2 xq = finite ? eight<T, true>(v[i][j], inv) : eight<T, false>(v[i][j], inv);
+        const uint2 xq = finite ? eight<T, true>(v[i % AT_ONCE][j], inv) : eight<T, false>(v[i % AT_ONCE][j], inv);
         const uint4 p = a[j >> 1], r = a[2 + (j >> 1)];
         if (j & 1) mma_e4m3(c, p.z, r.z, p.w, r.w, xq.x, xq.y);
         else mma_e4m3(c, p.x, r.x, p.y, r.y, xq.x, xq.y);
@@ -706,7 +711,7 @@ int tmpi_fp8_few(const void* x, int64_t ld, const void* q, const void* scale, co
     using T = std::remove_pointer_t<decltype(type)>;
     const auto kernel = tokens <= 8 ? fp8::few_kernel<T, 1> : tokens <= 16 ? fp8::few_kernel<T, 2> : fp8::few_kernel<T, 4>;
     // Shares of K as long as the blocks fit the SMs and each has blocks of K for half its warps.  More blocks than SMs have eight warps, so that two fit an SM (4 tokens, 4096 -> 4096:
-    // 12.3 -> WIDE_US us).
+    // 12.3 -> 10.9 us).
     const int groups = (N + fp8::FEW_ROWS - 1) / fp8::FEW_ROWS, blocks = fp8::blocks_of(K);
     int shares = 1;
     while (shares < 4 && groups * shares * 2 <= 148 && blocks >= shares * fp8::FEW_WARPS) shares *= 2;

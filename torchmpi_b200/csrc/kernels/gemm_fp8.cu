@@ -455,7 +455,7 @@ static Plan plan_of(int M, int N, int k_blocks) {
   double least = 1e30;
   for (const Width& w : widths) {
     const int tn = (N + w.columns - 1) / w.columns;
-    for (int s = 1; s <= 16; ++s) {
+    for (int s = 1; s <= 16 && 4 * (s - 1) < k_blocks; ++s) {
       const int per = ((k_blocks + s - 1) / s + 3) / 4 * 4, slices = (k_blocks + per - 1) / per;
       if (slices != s) continue;
       const long long rounds = ((long long)tm * tn * s + clusters - 1) / clusters;

@@ -283,9 +283,13 @@ class AdamW:
             mine = self.state[p]
             if set(st) != set(mine) or any(st[k].shape != mine[k].shape or st[k].dtype != mine[k].dtype for k in mine):
                 raise ValueError("AdamW: a parameter's states are not those of this optimizer's")
-        for g, options in zip(self.param_groups, state["param_groups"]):
-            g.update(options)
         with torch.no_grad():
+            for g, options in zip(self.param_groups, state["param_groups"]):
+                for k, v in options.items():
+                    if isinstance(v, torch.Tensor) and isinstance(g[k], torch.Tensor):
+                        g[k].copy_(v)                # where a captured step reads it
+                    else:
+                        g[k] = v.to(self._steps.device, copy=True) if isinstance(v, torch.Tensor) else v
             for p, st in zip(self._params, saved):
                 for k, v in self.state[p].items():
                     v.copy_(st[k])

@@ -260,6 +260,42 @@ def lazy_cases(small: bool) -> dict:
     for which in ("quantize", "dequantize", "gelu_gradient"):
         out[f"act8_{which}"] = act8_case(which)
 
+    def fp8_case(which):
+        def build():
+            from torchmpi_b200.ops import fp8
+            M, N, K = ((4096 if small else 16384), 4096, 1024)
+            if which in ("quantize", "quantize_both", "dequantize"):
+                x = torch.randn(4 * M, K, device=dev).to(torch.bfloat16)
+                kept, n = fp8.quantize(x), x.numel()
+                if which == "dequantize":
+                    return (lambda: fp8.dequantize(kept)), n * 3 + n // 128
+                return (lambda: getattr(fp8, which)(x)), (n * 3 + n // 128 if which == "quantize" else n * 4 + n // 64)
+            w = fp8.quantize((torch.randn(N, K, device=dev) * K ** -0.5).to(torch.bfloat16))
+            if which == "few_tokens":
+                x = torch.randn(4, K, device=dev).to(torch.bfloat16)
+                return (lambda: fp8.linear(x, w)), N * K + N * K // 128
+            a = fp8.quantize(torch.randn(M, K, device=dev).to(torch.bfloat16))
+            return (lambda: fp8.matmul(a, w)), M * K + N * K + 2 * M * N, 2.0 * M * N * K
+        return build
+    for which in ("quantize", "quantize_both", "dequantize", "matmul", "few_tokens"):
+        out[f"fp8_{which}"] = fp8_case(which)
+
+    def adamw_case(which):
+        def build():
+            from torchmpi_b200.ops import adamw
+            n, count = ((1 << 22) if small else (1 << 24)), 8
+            params = [torch.randn(n, device=dev).to(torch.bfloat16).requires_grad_(True) for _ in range(count)]
+            for p in params:
+                p.grad = torch.randn(n, device=dev).to(torch.bfloat16)
+            if which == "norm":
+                grads = [p.grad for p in params]
+                return (lambda: adamw.grad_norm(grads)), 2 * n * count
+            opt = adamw.AdamW(params, bits=int(which))
+            return opt.step, n * count * (28 if which == "32" else 16) + (0 if which == "32" else n * count // 8)
+        return build
+    for which in ("32", "8", "norm"):
+        out[f"adamw_{which}"] = adamw_case(which)
+
     def pool_case():
         N, C, H = (B, 64, 112)
         x = torch.randn(N, C, H, H, device=dev).to(torch.bfloat16).contiguous(memory_format=torch.channels_last).requires_grad_(True)
