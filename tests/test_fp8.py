@@ -72,6 +72,29 @@ def test_read_back_in_each_type(device):
         assert torch.equal(fp8.dequantize(m, dtype).cpu(), ref.kept(x).to(dtype))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows,cols", [(5, 1), (1, 3), (40, 5), (9, 7), (33, 9), (20, 127), (21, 129), (3, 255), (130, 257), (700, 1001)])
+def test_read_back_over_the_ends_of_rows(rows, cols, device):
+    """Rows that are no multiple of 16 bytes: pieces of the result go on over their ends and over those of blocks."""
+    x = _values(torch.Generator().manual_seed(cols), rows, cols, FP32, wild=False)
+    m = fp8.quantize(x.to(device))
+    for dtype in (BF, HALF, FP32):
+        assert torch.equal(fp8.dequantize(m, dtype).cpu(), ref.kept(x).to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HALF, FP32])
+def test_elements_from_any_address(dtype):
+    buf = _values(torch.Generator().manual_seed(3), 1, 40 * 301 + 16, dtype).cuda().view(-1)
+    for first in range(9):
+        for cols, ld in ((301, 301), (128, 301), (136, 136), (5, 8), (264, 299)):
+            x = buf[first:].as_strided((40, cols), (ld, 1))
+            _same(fp8.quantize(x), fp8._quantize(x.cpu()))
+            a, b = fp8.quantize_both(x)
+            _same(a, fp8._quantize(x.cpu()))
+            _same(b, fp8._quantize(x.cpu().t()))
+
+
 def test_scales_are_where_the_documentation_says():
     x = torch.exp2(torch.randint(-9, 9, (300, 5), generator=torch.Generator().manual_seed(1)).float()).repeat_interleave(128, 1)
     m = fp8.quantize(x)

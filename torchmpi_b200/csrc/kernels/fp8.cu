@@ -77,11 +77,50 @@ template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w
   return m < Eight<T>::INF ? m : 0u;
 }
 
-// n elements (up to 8) at p; vec: whole, and on 16-byte boundaries
+// Up to N elements from anywhere, in two steps, so that the loads of several are under way together: the pieces of 16 bytes that hold them (each holds at least one,
+// so that it lies in memory that is there; without any, that of `some` element), then shifted by words and by a half, with zeros behind the n-th.
+template <typename T, int N> struct Raw {
+  static constexpr int WORDS = N * sizeof(T) / 4, PIECES = WORDS / 4 + 1;
+  uint4 u[PIECES];
+  uint32_t off;
+};
+template <int N, typename T>
+__device__ __forceinline__ Raw<T, N> issue(const T* __restrict__ p, int n, const T* __restrict__ some) {
+  Raw<T, N> r;
+  const uintptr_t at = (uintptr_t)(n > 0 ? p : some);
+  r.off = (uint32_t)at & 15;
+  const int last = n > 0 ? (int)(r.off + n * sizeof(T) - 1) >> 4 : 0;
+  const uint4* from = reinterpret_cast<const uint4*>(at & ~(uintptr_t)15);
+#pragma unroll
+  for (int j = 0; j < Raw<T, N>::PIECES; ++j) r.u[j] = from[min(j, last)];
+  return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void settle(const Raw<T, N>& r, int n, uint32_t (&w)[Raw<T, N>::WORDS]) {
+  constexpr int W = Raw<T, N>::WORDS;
+  uint32_t c[W + 4];
+#pragma unroll
+  for (int j = 0; j < Raw<T, N>::PIECES; ++j) c[4 * j] = r.u[j].x, c[4 * j + 1] = r.u[j].y, c[4 * j + 2] = r.u[j].z, c[4 * j + 3] = r.u[j].w;
+#pragma unroll
+  for (int j = 0; j < W + 2; ++j) c[j] = r.off & 8 ? c[j + 2] : c[j];
+#pragma unroll
+  for (int j = 0; j < W + 1; ++j) c[j] = r.off & 4 ? c[j + 1] : c[j];
+#pragma unroll
+  for (int j = 0; j < W; ++j) w[j] = sizeof(T) == 2 ? __funnelshift_r(c[j], c[j + 1], (r.off & 2) * 8) : c[j];
+  if (n < N) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      if (sizeof(T) == 2 && 2 * j + 1 == n) w[j] &= 0xffffu;
+      else if (j * 4 >= n * (int)sizeof(T)) w[j] = 0u;
+    }
+  }
+}
+
+// n elements (up to 8) at p, on a 16-byte boundary
 template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int n, bool vec, uint32_t (&w)[Eight<T>::WORDS]) {
+__device__ __forceinline__ void load8(const T* __restrict__ p, int n, uint32_t* w) {
   constexpr int W = Eight<T>::WORDS;
-  if (vec && n == 8) {
+  if (n == 8) {
 #pragma unroll
     for (int j = 0; j < W; j += 4) {
       const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + j);
@@ -98,9 +137,8 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int n, bool vec, 
       }
   }
 }
-
 template <typename T>
-__device__ __forceinline__ void load_whole(const T* __restrict__ p, uint32_t (&w)[Eight<T>::WORDS]) {
+__device__ __forceinline__ void load_whole(const T* __restrict__ p, uint32_t* w) {
 #pragma unroll
   for (int j = 0; j < Eight<T>::WORDS; j += 4) {
     const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + j);
@@ -130,12 +168,12 @@ __device__ __forceinline__ uint2 eight(const uint32_t* w, float inv) {
 // Eight threads to a block of 128, sixteen elements each, two of a thread's pieces under way at a time (16 bytes by each thread, so that a warp's loads
 // are whole lines, took more instructions for an element and 25.7 us in place of 18.1 at 8192 x 4096).
 constexpr int ROW_THREADS = 256;
-struct Stride { int rows, pieces; };          // a launch's threads, as rows of pieces: what a thread's next piece lies further
+struct Stride { int rows, pieces; };          // a launch's threads, as rows of pieces (or elements): what a thread's next piece lies further
 
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __restrict__ x, const long long ld, uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
-                                                                    const long long rows, const int cols, const bool vec, const Stride step) {
-  constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
+                                                                    const long long rows, const int cols, const Stride step) {
+  constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1, W = Eight<T>::WORDS;
   using E = Eight<T>;
   wait_previous(x);
   const int groups = groups_of(cols), per_row = blocks_of(cols) * 8;
@@ -143,7 +181,8 @@ __global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __r
   long long at = ((long long)blockIdx.x * ROW_THREADS + threadIdx.x) / per_row;
   int piece = (int)((long long)blockIdx.x * ROW_THREADS + threadIdx.x - at * per_row);
   for (long long i0 = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; (i0 & ~31LL) < items; i0 += AHEAD * stride) {
-    uint32_t w[AHEAD][2][E::WORDS];
+    uint32_t w[AHEAD][2 * W];
+    Raw<T, 16> raw[AHEAD];
     long long row[AHEAD];
     int col[AHEAD];
 #pragma unroll
@@ -151,23 +190,29 @@ __global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __r
       row[u] = at;
       col[u] = piece * 16;
       const int n = at < rows ? cols - col[u] : 0;
-      load8<T>(x + row[u] * ld + col[u], min(8, max(0, n)), vec, w[u][0]);
-      load8<T>(x + row[u] * ld + col[u] + 8, min(8, max(0, n - 8)), vec, w[u][1]);
+      const T* from = x + row[u] * ld + col[u];
+      if (VEC) {
+        load8<T>(from, min(8, max(0, n)), w[u]);
+        load8<T>(from + 8, min(8, max(0, n - 8)), w[u] + W);
+      } else {
+        raw[u] = issue<16>(from, min(16, n), x);
+      }
       at += step.rows;
       piece += step.pieces;
       if (piece >= per_row) { piece -= per_row; ++at; }
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
+      if (!VEC) settle(raw[u], row[u] < rows ? cols - col[u] : 0, w[u]);
       uint32_t a = 0;
 #pragma unroll
-      for (int j = 0; j < E::WORDS; ++j) a = E::largest(a, E::largest(w[u][0][j], w[u][1][j]));
+      for (int j = 0; j < 2 * W; ++j) a = E::largest(a, w[u][j]);
       a = of_word<T>(a);
       const bool finite = __all_sync(~0u, a < E::INF);
       if (!finite) {
         a = 0;
 #pragma unroll
-        for (int j = 0; j < E::WORDS; ++j) a = max(a, max(of_word<T>(finite_part<T>(w[u][0][j])), of_word<T>(finite_part<T>(w[u][1][j]))));
+        for (int j = 0; j < 2 * W; ++j) a = max(a, of_word<T>(finite_part<T>(w[u][j])));
       }
       a = max(a, __shfl_xor_sync(~0u, a, 1));
       a = max(a, __shfl_xor_sync(~0u, a, 2));
@@ -176,8 +221,8 @@ __global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __r
       const uint32_t byte = scale_byte(as_fp32<T>(a));
       const float inv = inverse(byte);
       uint2 lo, hi;
-      if (finite) lo = eight<T, true>(w[u][0], inv), hi = eight<T, true>(w[u][1], inv);
-      else lo = eight<T, false>(w[u][0], inv), hi = eight<T, false>(w[u][1], inv);
+      if (finite) lo = eight<T, true>(w[u], inv), hi = eight<T, true>(w[u] + W, inv);
+      else lo = eight<T, false>(w[u], inv), hi = eight<T, false>(w[u] + W, inv);
       *reinterpret_cast<uint4*>(q + row[u] * pitch + col[u]) = make_uint4(lo.x, lo.y, hi.x, hi.y);
       if ((threadIdx.x & 7) == 0) scale[scale_at(row[u], col[u] / BLOCK, groups)] = (uint8_t)byte;
     }
@@ -189,18 +234,18 @@ constexpr int TILE = 128, TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32, RO
 
 // One matrix, or two in one launch (the input and the weight of a layer): the blocks from a's tiles on take b's.
 // GELU: x is the gradient behind a GELU of z; what is kept is x gelu'(z), rounded to T.  q, scale: along the rows, or null.  sums: the columns'
-// sums over this tile's rows, [row tiles, cols], or null; both are of a alone.
+// sums over this tile's rows, [row tiles, cols], or null; both are of a alone.  VEC: rows start on 16-byte boundaries.
 template <typename T> struct Matrix {
   const T* x;
   long long ld;
   uint8_t *q, *scale, *qt, *scalet;
-  int rows, cols, vec;
+  int rows, cols;
 };
-template <typename T, bool GELU>
-__global__ void __launch_bounds__(TILE_THREADS, sizeof(T) == 4 || GELU ? 2 : 3)
+template <typename T, bool GELU, bool VEC>
+__global__ void __launch_bounds__(TILE_THREADS, sizeof(T) == 4 || GELU || !VEC ? 2 : 3)
 quantize_tiles_kernel(const Matrix<T> a, const Matrix<T> b, const T* __restrict__ z, float* __restrict__ sums_of_a) {
   using E = Eight<T>;
-  constexpr int W = E::WORDS;
+  constexpr int W = E::WORDS, R = sizeof(T) == 2 ? 4 : 2;          // rows of a thread whose pieces are under way together
   __shared__ __align__(16) uint32_t tops[TILE_WARPS][16 * W];
   __shared__ __align__(16) float part[TILE_WARPS][TILE];
   __shared__ __align__(16) float column_inv[TILE];
@@ -213,31 +258,48 @@ quantize_tiles_kernel(const Matrix<T> a, const Matrix<T> b, const T* __restrict_
   uint8_t *const q = second ? b.q : a.q, *const scale = second ? b.scale : a.scale, *const qt = second ? b.qt : a.qt, *const scalet = second ? b.scalet : a.scalet;
   float* const sums = second ? nullptr : sums_of_a;
   const int rows = second ? b.rows : a.rows, cols = second ? b.cols : a.cols;
-  const bool vec = second ? b.vec : a.vec;
   const int t = threadIdx.x, cg = t & 15, rg = t >> 4, warp = t >> 5, tile = (int)blockIdx.x - (second ? tiles_of_a : 0);
   const int col_tiles = blocks_of(cols), cb = tile % col_tiles, rb = tile / col_tiles;
   const int row0 = rb * TILE + rg * ROWS, col0 = cb * TILE + cg * 8, n = max(0, min(8, cols - col0));
-  const bool whole = vec && (cb + 1) * TILE <= cols && (rb + 1) * TILE <= rows;      // no edge, no odd address
+  const bool whole = (cb + 1) * TILE <= cols && (rb + 1) * TILE <= rows;
   uint32_t w[ROWS][W];
   const T* from = x + (long long)row0 * ld + col0;
-  if (whole) {
+  if (VEC && whole) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) load_whole<T>(from + i * ld, w[i]);
+  } else if (VEC) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) load8<T>(from + i * ld, row0 + i < rows ? n : 0, w[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) load8<T>(from + i * ld, row0 + i < rows ? n : 0, vec, w[i]);
+    for (int h = 0; h < ROWS; h += R) {
+      Raw<T, 8> raw[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) raw[i] = issue<8>(from + (h + i) * ld, row0 + h + i < rows ? n : 0, x);
+#pragma unroll
+      for (int i = 0; i < R; ++i) settle(raw[i], row0 + h + i < rows ? n : 0, w[h + i]);
+    }
   }
   if constexpr (GELU) {
     const T* z0 = z + (long long)row0 * cols + col0;
 #pragma unroll
     for (int h = 0; h < ROWS; h += 4) {                   // z four rows at a time
       uint32_t zs[4][W];
-      if (whole) {
+      if (VEC && whole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_whole<T>(z0 + (long long)(h + i) * cols, zs[i]);
+      } else if (VEC) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load8<T>(z0 + (long long)(h + i) * cols, row0 + h + i < rows ? n : 0, zs[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load8<T>(z0 + (long long)(h + i) * cols, row0 + h + i < rows ? n : 0, vec, zs[i]);
+        for (int g = 0; g < 4; g += R) {
+          Raw<T, 8> raw[R];
+#pragma unroll
+          for (int i = 0; i < R; ++i) raw[i] = issue<8>(z0 + (long long)(h + g + i) * cols, row0 + h + g + i < rows ? n : 0, z);
+#pragma unroll
+          for (int i = 0; i < R; ++i) settle(raw[i], row0 + h + g + i < rows ? n : 0, zs[g + i]);
+        }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -415,41 +477,95 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const float* __restric
 }
 
 // ---------------------------------------------------------------- back
-// 16 bytes of the result by each thread
+// 16 bytes of the result by each thread, rows being so many whole pieces.  vec: they are on 16-byte boundaries; the branch also keeps the four loads together (without it 21 us at
+// 8192 x 4096 bf16, with it 17).
 template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS) restore_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, T* __restrict__ x, const long long rows, const int cols,
                                                               const bool vec, const Stride step) {
   constexpr int PER = 16 / sizeof(T), AHEAD = 4;
   wait_previous(q, scale);
-  const int groups = groups_of(cols), per_row = (cols + PER - 1) / PER;
-  const long long pitch = pitch_of(cols), items = rows * per_row, stride = (long long)gridDim.x * ROW_THREADS;
-  long long at = ((long long)blockIdx.x * ROW_THREADS + threadIdx.x) / per_row;
-  int piece = (int)((long long)blockIdx.x * ROW_THREADS + threadIdx.x - at * per_row);
-  for (long long i0 = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; i0 < items; i0 += AHEAD * stride) {
+  const int groups = groups_of(cols);
+  const long long pitch = pitch_of(cols), total = rows * cols, stride = (long long)gridDim.x * ROW_THREADS * PER;
+  long long first = ((long long)blockIdx.x * ROW_THREADS + threadIdx.x) * PER, at = first / cols;
+  int in_row = (int)(first - at * cols);
+  for (; first < total; first += AHEAD * stride) {
     uint2 u[AHEAD];
     uint32_t s[AHEAD];
-    long long row[AHEAD];
-    int col[AHEAD];
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const long long i = i0 + a * stride;
-      row[a] = i < items ? at : 0;
-      col[a] = i < items ? piece * PER : 0;
+      const bool there = first + a * stride < total;
+      const long long row = there ? at : 0;
+      const int col = there ? in_row : 0;
+      at += step.rows;
+      in_row += step.pieces;
+      if (in_row >= cols) { in_row -= cols; ++at; }
+      const uint8_t* p = q + row * pitch + col;
+      u[a] = PER == 8 ? *reinterpret_cast<const uint2*>(p) : make_uint2(*reinterpret_cast<const uint32_t*>(p), 0u);
+      s[a] = scale[scale_at(row, col / BLOCK, groups)];
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const long long e = first + a * stride;
+      if (e >= total) break;
+      float f[8];
+      act8::unpack8(u[a], value(s[a]), f);
+      if (vec) {
+        Pack<T, PER> o;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) o.v[k] = from_acc<T>((typename AccOf<T>::type)f[k]);
+        st_pack<T, PER>(x + e, o);
+      } else {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) x[e + k] = from_acc<T>((typename AccOf<T>::type)f[k]);
+      }
+    }
+  }
+}
+
+// Rows that are not: their first and last pieces are shared with their neighbours' (stored by elements), and a piece's bytes lie anywhere in theirs: whole words, shifted
+// (8192 x 4001 bf16 in 31 us, where pieces of rows that were stored by elements took 96; 4096 columns take 17).
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS) restore_any_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, T* __restrict__ x, const long long rows, const int cols,
+                                                                  const Stride step) {
+  constexpr int PER = 16 / sizeof(T), AHEAD = 4;
+  wait_previous(q, scale);
+  const int groups = groups_of(cols), per_row = (cols + PER - 1) / PER + 1;
+  const long long pitch = pitch_of(cols), items = rows * per_row, stride = (long long)gridDim.x * ROW_THREADS;
+  long long i0 = (long long)blockIdx.x * ROW_THREADS + threadIdx.x, at = i0 / per_row;
+  int piece = (int)(i0 - at * per_row);
+  for (; i0 < items; i0 += AHEAD * stride) {
+    uint2 u[AHEAD];
+    uint32_t s[AHEAD], s_next[AHEAD];
+    long long row[AHEAD];
+    int col[AHEAD];                    // of the piece's first element: in front of the row's where that is inside a piece
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const bool there = i0 + a * stride < items;
+      row[a] = there ? at : 0;
+      col[a] = (there ? piece * PER : 0) - (int)((uintptr_t)(x + row[a] * cols) & 15) / (int)sizeof(T);
       at += step.rows;
       piece += step.pieces;
       if (piece >= per_row) { piece -= per_row; ++at; }
-      const uint8_t* p = q + row[a] * pitch + col[a];
-      u[a] = PER == 8 ? *reinterpret_cast<const uint2*>(p) : make_uint2(*reinterpret_cast<const uint32_t*>(p), 0u);
-      s[a] = scale[scale_at(row[a], col[a] / BLOCK, groups)];
+      const int from = col[a] & ~3, by = (col[a] & 3) * 8;
+      uint32_t w[3];
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        w[j] = from + 4 * j >= 0 && from + 4 * j < pitch && (j < 2 || PER == 8) ? *reinterpret_cast<const uint32_t*>(q + row[a] * pitch + from + 4 * j) : 0u;
+      u[a] = make_uint2(__funnelshift_r(w[0], w[1], by), __funnelshift_r(w[1], w[2], by));
+      s[a] = scale[scale_at(row[a], min(max(col[a], 0), cols - 1) / BLOCK, groups)];
+      s_next[a] = scale[scale_at(row[a], min(max(col[a] + PER - 1, 0), cols - 1) / BLOCK, groups)];
     }
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
       if (i0 + a * stride >= items) break;
       float f[8];
-      act8::unpack8(u[a], value(s[a]), f);
+      act8::unpack8(u[a], 1.f, f);
+      const float here = value(s[a]), next = value(s_next[a]);
+      const int last = (max(col[a], 0) | (BLOCK - 1)) - col[a];          // of the first block
+#pragma unroll
+      for (int k = 0; k < PER; ++k) f[k] *= k <= last ? here : next;
       T* p = x + row[a] * cols + col[a];
-      const int n = cols - col[a];
-      if (vec && n >= PER) {
+      if (col[a] >= 0 && col[a] + PER <= cols) {
         Pack<T, PER> o;
 #pragma unroll
         for (int k = 0; k < PER; ++k) o.v[k] = from_acc<T>((typename AccOf<T>::type)f[k]);
@@ -457,7 +573,7 @@ __global__ void __launch_bounds__(ROW_THREADS) restore_kernel(const uint8_t* __r
       } else {
 #pragma unroll
         for (int k = 0; k < PER; ++k)
-          if (k < n) p[k] = from_acc<T>((typename AccOf<T>::type)f[k]);
+          if (col[a] + k >= 0 && col[a] + k < cols) p[k] = from_acc<T>((typename AccOf<T>::type)f[k]);
       }
     }
   }
@@ -520,30 +636,37 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict
     const uint4 a[4] = {next[0], next[1], next[2], next[3]};
     const uint32_t sw[2] = {next_scale[0], next_scale[1]};
     if (b + warps < blocks) fetch(b + warps);
-    uint32_t v[AT_ONCE][4][E::WORDS];
+    uint32_t v[AT_ONCE][4 * E::WORDS];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       if (i * 8 >= tokens) break;
       if (i % AT_ONCE == 0) {
+        const bool whole = vec && col + 32 <= K;
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
+          for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int token = (i + u) * 8 + g;
-            load8<T>(x + (long long)token * ld + col + 8 * j, token < tokens ? min(8, max(0, K - col - 8 * j)) : 0, vec, v[u][j]);
+            for (int j = 0; j < 4 * E::WORDS; j += E::WORDS) {
+              const int token = min((i + u) * 8 + g, tokens - 1);
+              load_whole<T>(x + (long long)token * ld + col + j / E::WORDS * 8, v[u] + j);
+            }
+        } else {
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; ++u) {
+            const int token = min((i + u) * 8 + g, tokens - 1), n = min(32, K - col);
+            settle(issue<32>(x + (long long)token * ld + col, n, x), n, v[u]);
           }
+        }
       }
       uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int k = 0; k < E::WORDS; ++k) top = E::largest(top, v[i % AT_ONCE][j][k]);
+      for (int k = 0; k < 4 * E::WORDS; ++k) top = E::largest(top, v[i % AT_ONCE][k]);
       top = of_word<T>(top);
       const bool finite = __all_sync(~0u, top < E::INF);
       if (!finite) {
         top = 0;
 #pragma unroll
-        for (int k = 0; k < 4 * E::WORDS; ++k) top = max(top, of_word<T>(finite_part<T>(v[i % AT_ONCE][k / E::WORDS][k % E::WORDS])));
+        for (int k = 0; k < 4 * E::WORDS; ++k) top = max(top, of_word<T>(finite_part<T>(v[i % AT_ONCE][k])));
       }
       top = max(top, __shfl_xor_sync(~0u, top, 1));
       top = max(top, __shfl_xor_sync(~0u, top, 2));
@@ -552,7 +675,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) few_kernel(const T* __restrict
       float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {                    // 8 of the thread's 32 bytes for each of the four instructions
-        const uint2 xq = finite ? eight<T, true>(v[i % AT_ONCE][j], inv) : eight<T, false>(v[i % AT_ONCE][j], inv);
+        const uint2 xq = finite ? eight<T, true>(v[i % AT_ONCE] + j * E::WORDS, inv) : eight<T, false>(v[i % AT_ONCE] + j * E::WORDS, inv);
         const uint4 p = a[j >> 1], r = a[2 + (j >> 1)];
         if (j & 1) mma_e4m3(c, p.z, r.z, p.w, r.w, xq.x, xq.y);
         else mma_e4m3(c, p.x, r.x, p.y, r.y, xq.x, xq.y);
@@ -649,13 +772,15 @@ int tmpi_fp8_quantize(const void* x, int64_t ld, const void* z, void* q, void* s
     const bool vec = fp8::whole_pieces({x, z}, ld, sizeof(T)) && (!z || cols * sizeof(T) % 16 == 0);
     if (!qt) {
       const fp8::RowLaunch l = fp8::row_launch(rows, fp8::blocks_of(cols) * 8, sizeof(T) == 2 ? 2 : 1, 148 * 8);
-      return launch_overlapped(fp8::quantize_rows_kernel<T>, l.blocks, fp8::ROW_THREADS, 0, s, (const T*)x, (long long)ld, (uint8_t*)q, (uint8_t*)scale, (long long)rows, (int)cols, vec,
-                               l.step);
+      return launch_overlapped(vec ? fp8::quantize_rows_kernel<T, true> : fp8::quantize_rows_kernel<T, false>, l.blocks, fp8::ROW_THREADS, 0, s, (const T*)x, (long long)ld, (uint8_t*)q,
+                               (uint8_t*)scale, (long long)rows, (int)cols, l.step);
     }
     const long long tiles = (long long)fp8::blocks_of(rows) * fp8::blocks_of(cols);
     if (tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
-    const fp8::Matrix<T> a{(const T*)x, ld, (uint8_t*)q, (uint8_t*)scale, (uint8_t*)qt, (uint8_t*)scalet, (int)rows, (int)cols, vec};
-    return launch_overlapped(z ? fp8::quantize_tiles_kernel<T, true> : fp8::quantize_tiles_kernel<T, false>, (unsigned)tiles, fp8::TILE_THREADS, 0, s, a, a, (const T*)z, sums);
+    const fp8::Matrix<T> a{(const T*)x, ld, (uint8_t*)q, (uint8_t*)scale, (uint8_t*)qt, (uint8_t*)scalet, (int)rows, (int)cols};
+    const auto kernel = z ? (vec ? fp8::quantize_tiles_kernel<T, true, true> : fp8::quantize_tiles_kernel<T, true, false>)
+                          : (vec ? fp8::quantize_tiles_kernel<T, false, true> : fp8::quantize_tiles_kernel<T, false, false>);
+    return launch_overlapped(kernel, (unsigned)tiles, fp8::TILE_THREADS, 0, s, a, a, (const T*)z, sums);
   });
 }
 
@@ -674,10 +799,12 @@ int tmpi_fp8_quantize_two(const tmpi_fp8_matrix_t* two, int dtype, void* stream)
   return fp8::by_type(dtype, "fp8_quantize_two", [&](auto* type) -> cudaError_t {
     using T = std::remove_pointer_t<decltype(type)>;
     fp8::Matrix<T> m[2];
-    for (int i = 0; i < 2; ++i)
-      m[i] = {(const T*)two[i].x, two[i].ld, (uint8_t*)two[i].q, (uint8_t*)two[i].scale, (uint8_t*)two[i].qt, (uint8_t*)two[i].scalet, (int)two[i].rows, (int)two[i].cols,
-              fp8::whole_pieces({two[i].x}, two[i].ld, sizeof(T))};
-    return launch_overlapped(fp8::quantize_tiles_kernel<T, false>, (unsigned)tiles, fp8::TILE_THREADS, 0, (cudaStream_t)stream, m[0], m[1], (const T*)nullptr, (float*)nullptr);
+    bool vec = true;
+    for (int i = 0; i < 2; ++i) {
+      m[i] = {(const T*)two[i].x, two[i].ld, (uint8_t*)two[i].q, (uint8_t*)two[i].scale, (uint8_t*)two[i].qt, (uint8_t*)two[i].scalet, (int)two[i].rows, (int)two[i].cols};
+      vec = vec && fp8::whole_pieces({two[i].x}, two[i].ld, sizeof(T));
+    }
+    return launch_overlapped(vec ? fp8::quantize_tiles_kernel<T, false, true> : fp8::quantize_tiles_kernel<T, false, false>, (unsigned)tiles, fp8::TILE_THREADS, 0, (cudaStream_t)stream, m[0], m[1], (const T*)nullptr, (float*)nullptr);
   });
 }
 
@@ -696,9 +823,16 @@ int tmpi_fp8_restore(const void* q, const void* scale, void* x, int64_t rows, in
   if (!all_aligned16({q})) return fail(TMPI_ERR_INVALID, "fp8_restore: the 8-bit numbers must be 16-byte aligned");
   return fp8::by_type(dtype, "fp8_restore", [&](auto* type) -> cudaError_t {
     using T = std::remove_pointer_t<decltype(type)>;
-    const fp8::RowLaunch l = fp8::row_launch(rows, (int)((cols * sizeof(T) + 15) / 16), 4, 1 << 20);
-    return launch_overlapped(fp8::restore_kernel<T>, l.blocks, fp8::ROW_THREADS, 0, (cudaStream_t)stream, (const uint8_t*)q, (const uint8_t*)scale, (T*)x, (long long)rows, (int)cols,
-                             fp8::whole_pieces({x}, cols, sizeof(T)), l.step);
+    constexpr int PER = 16 / sizeof(T);
+    if (cols % PER == 0) {
+      const int blocks = (int)std::min<int64_t>((rows * cols / PER + 4 * fp8::ROW_THREADS - 1) / (4 * fp8::ROW_THREADS), 1 << 19);
+      const int64_t apart = (int64_t)blocks * fp8::ROW_THREADS * PER;          // elements between a thread's pieces
+      return launch_overlapped(fp8::restore_kernel<T>, blocks, fp8::ROW_THREADS, 0, (cudaStream_t)stream, (const uint8_t*)q, (const uint8_t*)scale, (T*)x, (long long)rows, (int)cols,
+                               all_aligned16({x}), fp8::Stride{(int)(apart / cols), (int)(apart % cols)});
+    }
+    const fp8::RowLaunch l = fp8::row_launch(rows, (int)((cols + PER - 1) / PER) + 1, 4, 1 << 20);
+    return launch_overlapped(fp8::restore_any_kernel<T>, l.blocks, fp8::ROW_THREADS, 0, (cudaStream_t)stream, (const uint8_t*)q, (const uint8_t*)scale, (T*)x, (long long)rows, (int)cols,
+                             l.step);
   });
 }
 
