@@ -9,7 +9,8 @@
 // The states of all tensors lie in one buffer each, a tensor's from a multiple of 128 elements on; the tensors' own addresses and extents come as a
 // table among the kernel's parameters (32 bytes a tensor), so that a step is one launch without a copy to the device.  Tensors are cut into chunks of 2048 elements,
 // a thread eight of them; a block takes chunk after chunk, as many apart as there are blocks, finds the first one's tensor by bisection and forms a
-// tensor's rates when it comes to it.  Bound by memory.
+// tensor's rates when it comes to it.  Bound by memory: 354 M elements of bf16 with masters take 1640 us in 32 bits (28 bytes an element, 6.0 TB/s, 0.92 of the copy rate), 1010 in 8
+// (16.1, 5.6), where half of the issue slots are taken too; without masters 1230 and 890.
 //
 // In 8 bits, 128 elements share the largest magnitude among them (fp32), and an element is kept as the root of its share of that, in multiples of 1/127 with
 // its sign for m, and of 1/255 for the root of v: m = +-c^2 top / 127^2, sqrt(v) = c^2 top / 255^2.  The root spends the codes evenly over ratios: the
@@ -279,7 +280,8 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
 }
 
 // ---------------------------------------------------------------- the norm of many tensors
-// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.
+// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.  Bound by memory: 354 M elements in 387 bf16 tensors 156 - 180 us, in fp32
+// 209 (1.03 of the copy rate, which writes too).
 constexpr int NORM_BLOCKS = 148 * 4;
 __host__ __device__ constexpr uint32_t unit_chunks(int element_bytes) { return 32768 / (CHUNK * element_bytes); }
 

@@ -166,7 +166,8 @@ __device__ __forceinline__ uint2 eight(const uint32_t* w, float inv) {
 
 // ---------------------------------------------------------------- along rows
 // Eight threads to a block of 128, sixteen elements each, two of a thread's pieces under way at a time (16 bytes by each thread, so that a warp's loads
-// are whole lines, took more instructions for an element and 25.7 us in place of 18.1 at 8192 x 4096).
+// are whole lines, took more instructions for an element and 25.7 us in place of 18.1 at 8192 x 4096; now 16.7).  Bound by memory and instructions alike (66 % of
+// the issue slots, 0.92 of the copy rate).  VEC: rows start on 16-byte boundaries (else 8192 x 4001 takes 21.9, by elements it took 42).
 constexpr int ROW_THREADS = 256;
 struct Stride { int rows, pieces; };          // a launch's threads, as rows of pieces (or elements): what a thread's next piece lies further
 
@@ -235,6 +236,8 @@ constexpr int TILE = 128, TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32, RO
 // One matrix, or two in one launch (the input and the weight of a layer): the blocks from a's tiles on take b's.
 // GELU: x is the gradient behind a GELU of z; what is kept is x gelu'(z), rounded to T.  q, scale: along the rows, or null.  sums: the columns'
 // sums over this tile's rows, [row tiles, cols], or null; both are of a alone.  VEC: rows start on 16-byte boundaries.
+// 8192 x 4096 bf16: 24.9 us both ways (0.82 of the copy rate; 57 % of the issue slots, of a warp's time two fifths waiting for its loads), with the sums 26.8, with the GELU's
+// gradient and the sums 53 (0.58; 28 million warp instructions, by four warps to a scheduler).  40 us both ways where rows start anywhere (8192 x 4001).
 template <typename T> struct Matrix {
   const T* x;
   long long ld;
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(ROW_THREADS) restore_any_kernel(const uint8_t*
 // index stands where is free as long as both operands agree, so a thread's 32 bytes of a weight row are the 32 consecutive ones of its quarter of the
 // block, and so are the tokens'.  The sums of a block are scaled into fp32 sums.  The next block's weights are under way meanwhile.
 // Few weight rows leave SMs idle: then two or four blocks, a cluster, share the blocks of K, and the first adds what the others leave in its shared memory, in order
-// (13 tokens, 4096 -> 1024: 6.5 us, 8.1 without the sharing).
+// (13 tokens, 4096 -> 1024: 6.5 us, 8.1 without the sharing; 5.7 since a row's pieces are sent for together).  1024 -> 4096: 3.4 us for one token, 7.0 for 32.
 constexpr int FEW_ROWS = 16, FEW_WARPS = 16;
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -845,7 +848,7 @@ int tmpi_fp8_few(const void* x, int64_t ld, const void* q, const void* scale, co
     using T = std::remove_pointer_t<decltype(type)>;
     const auto kernel = tokens <= 8 ? fp8::few_kernel<T, 1> : tokens <= 16 ? fp8::few_kernel<T, 2> : fp8::few_kernel<T, 4>;
     // Shares of K as long as the blocks fit the SMs and each has blocks of K for half its warps.  More blocks than SMs have eight warps, so that two fit an SM (4 tokens, 4096 -> 4096:
-    // 12.3 -> 10.9 us).
+    // 12.3 -> 10.9 us when it was introduced, 7.3 now).
     const int groups = (N + fp8::FEW_ROWS - 1) / fp8::FEW_ROWS, blocks = fp8::blocks_of(K);
     int shares = 1;
     while (shares < 4 && groups * shares * 2 <= 148 && blocks >= shares * fp8::FEW_WARPS) shares *= 2;
