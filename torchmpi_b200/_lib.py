@@ -232,7 +232,7 @@ _CUDA_PROTOS = {
     "tmpi_adamw_step": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _vp]),
     "tmpi_adamw_values": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp]),
     "tmpi_norm_sums": (_i, [_i]),
-    "tmpi_norm_squares": (_i, [_vp, _i, _i, _vp, _ip, _vp]),
+    "tmpi_norm_squares": (_i, [_vp, _i, _i, _vp, _ip, _vp, _vp]),
     "tmpi_norm_finish": (_i, [_vp, _i, _f, _f, _vp, _vp, _vp]),
     "tmpi_route_limits": (_i, [_ip, _ip]),
     "tmpi_route_workspace_bytes": (_sz, [_i, _i, _i]),

@@ -32,6 +32,7 @@ struct AdamW {
   std::vector<at::ScalarType> types;
   std::vector<int> group;
   Tensor m, v, m_top, v_top, master, steps, counter, norm;
+  Tensor sums, coefficient;                                         // of a clipped step
   int bits;
 
   // groups: lr, beta1, beta2, eps, weight decay; rates: learning rates on the device, or None
@@ -70,20 +71,20 @@ struct AdamW {
     s.steps = steps.data_ptr<int>();
     s.counter = (unsigned*)counter.data_ptr<int>();
     s.scale = (float)scale;
-    Tensor sums, coefficient;
     if (max_norm.has_value()) {
-      int total = 0, used = 0;
-      for (const auto& t : tables) total += tmpi_norm_sums((int)t.size());
-      sums = fresh({total}, at::kDouble);
-      coefficient = fresh({1}, at::kFloat);
+      const tmpi_norm_finish_t finish{norm.data_ptr<float>(), coefficient.data_ptr<float>(), s.counter, (float)scale, (float)*max_norm};
+      int used = 0;
       for (int c = 0; c < 3; ++c) {
-        int n = 0;
-        if (!tables[c].empty()) check(tmpi_norm_squares(tables[c].data(), (int)tables[c].size(), dtype_code(TYPES[c]), sums.data_ptr<double>() + used, &n, stream()));
-        used += n;
+        if (tables[c].empty()) continue;
+        const bool last = (c > 1 || tables[2].empty()) && (c > 0 || tables[1].empty());          // of the types
+        check(tmpi_norm_squares(tables[c].data(), (int)tables[c].size(), dtype_code(TYPES[c]), sums.data_ptr<double>(), &used, last ? &finish : nullptr, stream()));
+        launched(ADAMW, 1);
       }
-      check(tmpi_norm_finish(sums.data_ptr<double>(), used, (float)scale, (float)*max_norm, norm.data_ptr<float>(), coefficient.data_ptr<float>(), stream()));
+      if (!used) {                                                   // no gradient at all
+        check(tmpi_norm_finish(sums.data_ptr<double>(), 0, (float)scale, (float)*max_norm, norm.data_ptr<float>(), coefficient.data_ptr<float>(), stream()));
+        launched(ADAMW, 1);
+      }
       s.coefficient = coefficient.data_ptr<float>();
-      launched(ADAMW, 2);
     }
     for (int c = 0; c < 3; ++c) {
       if (tables[c].empty()) continue;
@@ -111,6 +112,8 @@ void register_adamw(pybind11::module_& m) {
         a.params = std::move(params); a.places = std::move(places); a.group = std::move(group);
         a.m = m_; a.v = v; a.m_top = or_none(m_top); a.v_top = or_none(v_top); a.master = or_none(master);
         a.steps = steps; a.counter = counter; a.norm = norm; a.bits = bits;
+        a.sums = fresh({tmpi_norm_sums((int)a.params.size()) + 2 * tmpi_norm_sums(0)}, at::kDouble);          // of three types' launches
+        a.coefficient = fresh({1}, at::kFloat);
         return a;
       }))
       .def("step", &AdamW::step);
@@ -137,11 +140,8 @@ void register_adamw(pybind11::module_& m) {
     if (kept.empty()) return c10::nullopt;
     for (const auto& t : tables) total += tmpi_norm_sums((int)t.size());
     const Tensor sums = fresh({total}, at::kDouble), norm = fresh({}, at::kFloat);
-    for (int c = 0; c < 3; ++c) {
-      int n = 0;
-      if (!tables[c].empty()) check(tmpi_norm_squares(tables[c].data(), (int)tables[c].size(), dtype_code(TYPES[c]), sums.data_ptr<double>() + used, &n, stream()));
-      used += n;
-    }
+    for (int c = 0; c < 3; ++c)
+      if (!tables[c].empty()) check(tmpi_norm_squares(tables[c].data(), (int)tables[c].size(), dtype_code(TYPES[c]), sums.data_ptr<double>(), &used, nullptr, stream()));
     check(tmpi_norm_finish(sums.data_ptr<double>(), used, 1.f, 1.f, norm.data_ptr<float>(), nullptr, stream()));
     launched(ADAMW, 2);
     return norm;

@@ -434,10 +434,17 @@ int tmpi_adamw_max_groups(void);
 int tmpi_adamw_step(const tmpi_adamw_tensor_t* tensors, int count, const tmpi_adamw_group_t* groups, int ngroups, const tmpi_adamw_states_t* states, int bits, int dtype, void* stream);
 // 8-bit states of `blocks` times 128 elements as numbers
 int tmpi_adamw_values(const void* m, const float* m_top, const void* v, const float* v_top, void* m_values, void* v_values, int64_t blocks, int dtype, void* stream);
-// The norm of many tensors (grad and n of the table): sums of squares, *used of them (at most tmpi_norm_sums(count)), then scale times the root of all sums'
-// sum and, where asked for, min(1, most / (norm + 1e-6)).
+// The norm of many tensors (grad and n of the table): sums of squares behind the first *used, which counts them then (at most tmpi_norm_sums(count) more), and of all scale times
+// their root, with the coefficient min(1, most / (norm + 1e-6)) where it has a place: by the last of those launches, where `finish` is given (its counter is zero between
+// launches), or by tmpi_norm_finish.
 int tmpi_norm_sums(int count);
-int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, double* sums, int* used, void* stream);
+typedef struct {
+  float* norm;
+  float* coefficient;
+  unsigned* counter;
+  float scale, most;
+} tmpi_norm_finish_t;
+int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, double* sums, int* used, const tmpi_norm_finish_t* finish, void* stream);
 int tmpi_norm_finish(const double* sums, int n, float scale, float most, float* norm, float* coefficient, void* stream);
 
 // ---------------------------------------------------------------- layers of experts (route.cu, experts.cu, grouped.cu)

@@ -280,8 +280,8 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
 }
 
 // ---------------------------------------------------------------- the norm of many tensors
-// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.  Bound by memory: 354 M elements in 387 bf16 tensors 156 - 180 us, in fp32
-// 209 (1.03 of the copy rate, which writes too).
+// Sums of squares: a thread's in fp32 (a few thousand of them), all others in fp64, in a fixed order.  Bound by memory: 354 M elements in 387 bf16 tensors 152 us, in 20 109
+// (0.99 of the copy rate), in fp32 205 and 188 (1.06 and 1.15: the copy writes too).
 constexpr int NORM_BLOCKS = 148 * 4;
 __host__ __device__ constexpr uint32_t unit_chunks(int element_bytes) { return 32768 / (CHUNK * element_bytes); }
 
@@ -298,10 +298,36 @@ __device__ __forceinline__ void load_eight(const void* p, uint32_t (&u)[32]) {
       : "l"(p));
 }
 
-// A block takes units of 32 KB (a few chunks in a row), as many apart as there are blocks, so that many small tensors are shared among all.
+// What becomes of the sums: norm = scale sqrt(their sum), coefficient = min(1, most / (norm + 1e-6)), NaN staying.
+struct Finish {
+  float *norm, *coefficient;     // coefficient may be null
+  unsigned* counter;             // zero between launches
+  float scale, most;
+};
+// of the first n sums, by all threads of a block
+__device__ __forceinline__ void finish_norm(const double* sums, int n, const Finish& f) {
+  double d = 0.;
+  for (int i = threadIdx.x; i < n; i += THREADS) d += __ldcg(sums + i);
+  __shared__ double part[THREADS / 32];
+#pragma unroll
+  for (int i = 16; i; i >>= 1) d += __shfl_xor_sync(~0u, d, i);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = d;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) d += part[i];
+    const float r = (float)(fabs((double)f.scale) * sqrt(d));
+    *f.norm = r;
+    if (f.coefficient) *f.coefficient = f.most / (r + 1e-6f) > 1.f ? 1.f : f.most / (r + 1e-6f);
+  }
+}
+
+// A block takes units of 32 KB (a few chunks in a row), as many apart as there are blocks, so that many small tensors are shared among all.  Of a unit that is
+// not whole, or of several tensors, four chunks at a time are under way (7 M fp32 elements of 67 tensors, with what is made of the sums: 14.3 -> 10.6 us).  Its sum goes to sums[before + block]; with a counter the last block to come takes those of all launches for the norm.
 template <typename T, int CAP>
-__global__ void __launch_bounds__(THREADS, 4) squares_kernel(const __grid_constant__ Table<CAP> table, const int entries, const uint32_t chunks, double* __restrict__ sums) {
-  constexpr int PER = CHUNK / THREADS;
+__global__ void __launch_bounds__(THREADS, 4) squares_kernel(const __grid_constant__ Table<CAP> table, const int entries, const uint32_t chunks, double* __restrict__ sums, const int before,
+                                                             const Finish finish) {
+  constexpr int PER = CHUNK / THREADS, AHEAD = 4;
   wait_previous(sums);
   float a[PER];
 #pragma unroll
@@ -309,38 +335,42 @@ __global__ void __launch_bounds__(THREADS, 4) squares_kernel(const __grid_consta
   for (uint32_t c0 = blockIdx.x * unit_chunks(sizeof(T)); c0 < chunks; c0 += gridDim.x * unit_chunks(sizeof(T))) {
     const uint32_t c1 = min(chunks, c0 + unit_chunks(sizeof(T)));
     int at = entry_of(table, entries, c0);
-    for (uint32_t c = c0; c < c1; ++at) {
-      const Entry& e = table.entry[at];
-      const uint32_t e0 = e.chunk, end = min(c1, at + 1 < entries ? table.entry[at + 1].chunk : chunks), extent = e.n;
-      const T* const grads = (const T*)e.grad;
-      const bool vec = ((uintptr_t)grads & 15) == 0;
-      if (vec && end - c == unit_chunks(sizeof(T)) && (end - e0) * CHUNK <= extent) {          // the whole unit
-        constexpr int V = 16 / sizeof(T);
-        uint32_t x[32];
-        load_eight(grads + (size_t)(c - e0) * CHUNK + threadIdx.x * V, x);
+    const Entry& e = table.entry[at];
+    if (c1 - c0 == unit_chunks(sizeof(T)) && (c1 - e.chunk) * (uint64_t)CHUNK <= e.n && ((uintptr_t)e.grad & 15) == 0) {          // whole, and of one tensor
+      constexpr int V = 16 / sizeof(T);
+      uint32_t x[32];
+      load_eight((const T*)e.grad + (size_t)(c0 - e.chunk) * CHUNK + threadIdx.x * V, x);
 #pragma unroll
-        for (int j = 0; j < 8 * V; ++j) {
-          const float f = (float)to_acc<T>(reinterpret_cast<const T*>(x)[j]);
-          a[j % PER] = fmaf(f, f, a[j % PER]);
-        }
-        c = end;
+      for (int j = 0; j < 8 * V; ++j) {
+        const float f = (float)to_acc<T>(reinterpret_cast<const T*>(x)[j]);
+        a[j % PER] = fmaf(f, f, a[j % PER]);
       }
-      for (; c < end; ++c) {
-        float x[PER];
+      continue;
+    }
+    for (uint32_t c = c0; c < c1; c += AHEAD) {
+      float x[AHEAD][PER];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        while (at + 1 < entries && table.entry[at + 1].chunk <= c + u) ++at;
+        const Entry& e = table.entry[at];
+        const T* const grads = (const T*)e.grad;
 #pragma unroll
         for (int j = 0; j < PER; j += 4) {
-          const uint32_t first = (c - e0) * CHUNK + j * THREADS + threadIdx.x * 4;
-          load<T, 4>(grads + first, first < extent ? (int)min(4u, extent - first) : 0, vec, x + j);
+          const uint32_t first = (c + u - e.chunk) * CHUNK + j * THREADS + threadIdx.x * 4;
+          load<T, 4>(grads + first, c + u < c1 && first < e.n ? (int)min(4u, e.n - first) : 0, ((uintptr_t)grads & 15) == 0, x[u] + j);
         }
-#pragma unroll
-        for (int k = 0; k < PER; ++k) a[k] = fmaf(x[k], x[k], a[k]);
       }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) a[k] = fmaf(x[u][k], x[u][k], a[k]);
     }
   }
   double d = 0.;
 #pragma unroll
   for (int k = 0; k < PER; ++k) d += (double)a[k];
   __shared__ double part[THREADS / 32];
+  __shared__ bool last;
 #pragma unroll
   for (int i = 16; i; i >>= 1) d += __shfl_xor_sync(~0u, d, i);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = d;
@@ -348,28 +378,21 @@ __global__ void __launch_bounds__(THREADS, 4) squares_kernel(const __grid_consta
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 1; i < THREADS / 32; ++i) d += part[i];
-    sums[blockIdx.x] = d;
+    __stcg(sums + before + blockIdx.x, d);
+    __threadfence();
+    last = finish.counter && atomicAdd(finish.counter, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (last) {
+    finish_norm(sums, before + (int)gridDim.x, finish);
+    if (threadIdx.x == 0) *finish.counter = 0;
   }
 }
 
-// norm = scale sqrt(sum of the sums); coefficient = min(1, most / (norm + 1e-6))
-__global__ void __launch_bounds__(THREADS) norm_kernel(const double* __restrict__ sums, const int n, const float scale, const float most, float* __restrict__ norm,
-                                                       float* __restrict__ coefficient) {
+__global__ void __launch_bounds__(THREADS) norm_kernel(const double* __restrict__ sums, const int n, const Finish finish) {
   wait_previous(sums);
-  double d = 0.;
-  for (int i = threadIdx.x; i < n; i += THREADS) d += sums[i];
-  __shared__ double part[THREADS / 32];
-#pragma unroll
-  for (int i = 16; i; i >>= 1) d += __shfl_xor_sync(~0u, d, i);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = d;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int i = 1; i < THREADS / 32; ++i) d += part[i];
-    const float r = (float)(fabs((double)scale) * sqrt(d));
-    *norm = r;
-    if (coefficient) *coefficient = most / (r + 1e-6f) > 1.f ? 1.f : most / (r + 1e-6f);      // NaN stays
-  }
+  finish_norm(sums, n, finish);
 }
 
 // ---------------------------------------------------------------- what 8-bit states stand for
@@ -390,12 +413,12 @@ __global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* __restri
 
 // ---------------------------------------------------------------- host side
 // Tables for the tensors [i, ...) until one is full; returns the next tensor and how much of it is in the table.
-struct Filled { int entries; uint32_t chunks; };
+struct Filled { int entries; uint32_t chunks; int finished; };          // finished: tensors whose last element is in the table or before
 constexpr int64_t MOST = int64_t(1) << 30;               // elements of an entry
 
 template <int CAP>
 static Filled fill(Table<CAP>* t, const tmpi_adamw_tensor_t* tensors, int count, int* i, int64_t* done, bool groups) {
-  Filled f{0, 0};
+  Filled f{0, 0, 0};
   uint32_t counted = *done ? COUNTED : 0u;
   while (*i < count && f.entries < CAP) {
     const tmpi_adamw_tensor_t& x = tensors[*i];
@@ -412,7 +435,7 @@ static Filled fill(Table<CAP>* t, const tmpi_adamw_tensor_t* tensors, int count,
     e.which = groups ? (uint32_t)x.step << 8 | (uint32_t)x.group | (*done ? PART : 0u) | counted : 0u;
     f.chunks += (uint32_t)((n + CHUNK - 1) / CHUNK);
     *done += n;
-    if (*done >= x.n) { ++*i; *done = 0; counted = 0u; }
+    if (*done >= x.n) { ++*i; ++f.finished; *done = 0; counted = 0u; }
   }
   return f;
 }
@@ -486,15 +509,21 @@ int tmpi_adamw_step(const tmpi_adamw_tensor_t* tensors, int count, const tmpi_ad
 // Sums of squares of `count` tensors into sums [tmpi_norm_sums(count)], of which *used were written.  A launch takes SMALL entries at least, and the tensors of a GPU (less than
 // 2^38 bytes) have not more than 256 entries beside their first ones.
 int tmpi_norm_sums(int count) { return (count / adamw::SMALL + 5) * adamw::NORM_BLOCKS; }
-int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, double* sums, int* used, void* stream) {
-  *used = 0;
-  if (count < 0) return fail(TMPI_ERR_INVALID, "norm: %d tensors", count);
+// The norm of `used` sums, and a clipping coefficient where it has a place.  With a counter (a word that is zero between launches, of one stream's launches) the last launch of
+// tmpi_norm_squares does that too, of `used` sums before and its own.
+int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, double* sums, int* used, const tmpi_norm_finish_t* finish, void* stream) {
+  if (count < 0 || *used < 0) return fail(TMPI_ERR_INVALID, "norm: %d tensors", count);
+  int rest = 0;
+  for (int i = 0; i < count; ++i) rest += tensors[i].n > 0;
   return adamw::by_type(dtype, "norm", [&](auto* type) -> cudaError_t {
     using T = std::remove_pointer_t<decltype(type)>;
     auto run = [&](const auto& table, const adamw::Filled& f) {
       constexpr int CAP = sizeof(table.entry) / sizeof(adamw::Entry);
       const uint32_t unit = adamw::unit_chunks(sizeof(T)), blocks = std::min<uint32_t>((f.chunks + unit - 1) / unit, adamw::NORM_BLOCKS);
-      const cudaError_t e = launch_overlapped(adamw::squares_kernel<T, CAP>, blocks, adamw::THREADS, 0, (cudaStream_t)stream, table, f.entries, f.chunks, sums + *used);
+      adamw::Finish last{};
+      rest -= f.finished;
+      if (finish && !rest) last = {finish->norm, finish->coefficient, finish->counter, finish->scale, finish->most};
+      const cudaError_t e = launch_overlapped(adamw::squares_kernel<T, CAP>, blocks, adamw::THREADS, 0, (cudaStream_t)stream, table, f.entries, f.chunks, sums, *used, last);
       *used += (int)blocks;
       return e;
     };
@@ -502,7 +531,7 @@ int tmpi_norm_squares(const tmpi_adamw_tensor_t* tensors, int count, int dtype, 
   });
 }
 int tmpi_norm_finish(const double* sums, int n, float scale, float most, float* norm, float* coefficient, void* stream) {
-  const cudaError_t e = launch_overlapped(adamw::norm_kernel, 1, adamw::THREADS, 0, (cudaStream_t)stream, sums, n, scale, most, norm, coefficient);
+  const cudaError_t e = launch_overlapped(adamw::norm_kernel, 1, adamw::THREADS, 0, (cudaStream_t)stream, sums, n, adamw::Finish{norm, coefficient, nullptr, scale, most});
   return e == cudaSuccess ? TMPI_OK : fail(TMPI_ERR_CUDA, "norm launch: %s", cudaGetErrorString(e));
 }
 
