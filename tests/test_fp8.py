@@ -125,7 +125,7 @@ def _matrices(g, M, N, K, device):
 
 
 # tiles of 256, 192 and 128 columns, slices of K, rows that are no 16-byte multiples, ends inside tiles and groups of blocks
-PRODUCTS = [(1, 1, 1), (40, 24, 128), (129, 257, 130), (256, 256, 1024), (300, 523, 640), (256, 192, 2048), (70, 8, 4096), (1000, 1016, 384), (2500, 2304, 520), (130, 4096, 264)]
+PRODUCTS = [(1, 1, 1), (40, 24, 128), (129, 257, 130), (256, 256, 1024), (300, 523, 640), (256, 192, 2048), (70, 8, 4096), (1000, 1016, 384), (2500, 2304, 520), (130, 4096, 264), (2300, 4001, 300)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -258,6 +258,22 @@ def test_layer_with_gelu(T, K, N, dtype, device):
     ref.close(kept, want, 3e-6 + 2.0 ** -22 * want.abs() + ref.half_step(want, dtype), "kept")
     if device == "cuda":
         fp8.check_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, FP32])
+@pytest.mark.parametrize("T", [3, 40])
+def test_gelu_of_any_magnitude(T, dtype, device):
+    """Far from zero nothing, or z itself, is left; NaN stays."""
+    b = torch.tensor([-3e38, -1e30, -1e20, -1e12, -5000.0, -1000.0, -60.0, -9.0, 0.0, 9.0, 60.0, 1e12, 3e38, float("inf"), float("nan")]).to(dtype)
+    x, w = torch.zeros(T, 64, dtype=dtype, device=device), torch.zeros(b.numel(), 64, dtype=dtype, device=device)
+    want = torch.where(b < 0, 0, b).double().expand(T, -1)
+    for weight in (w, fp8.quantize(w)):
+        with torch.no_grad():
+            y = fp8.linear(x, weight, b.to(device), gelu=True).double().cpu()
+        assert torch.isnan(y[:, -1]).all() and torch.equal(y[:, 9:-1], want[:, 9:-1]) and (y[:, :9].abs() <= 3e-6).all(), y[0]
+    y = fp8.linear(x.requires_grad_(), w, b.to(device), gelu=True).detach().double().cpu()
+    assert torch.isnan(y[:, -1]).all() and torch.equal(y[:, 9:-1], want[:, 9:-1]) and (y[:, :9].abs() <= 3e-6).all(), y[0]
 
 
 @pytest.mark.parametrize("device", DEVICES)

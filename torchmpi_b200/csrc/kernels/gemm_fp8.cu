@@ -203,11 +203,13 @@ template <> __device__ __forceinline__ float2 untwo<__half>(uint32_t w) { return
 // gelu of two rounded values, in a word of them
 template <typename T>
 __device__ __forceinline__ uint32_t gelu_word(uint32_t w) {
-  const float2 f = untwo<T>(w);
   float y0, y1;
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) {          // results of 8 bits: the quicker form (gelu.cuh)
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {          // results of 8 bits: the quicker form (gelu.cuh), whose Phi stops at 2^-60: from -1024 on (-inf too) nothing is left of z
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(w), "r"(0xc480c480u));
+    const float2 f = untwo<T>(w);
     attn_util::unpack2(shared_gelu2(attn_util::pack2(__float_as_uint(f.x), __float_as_uint(f.y))), y0, y1);
   } else {
+    const float2 f = untwo<T>(w);
     gelu_value2(f.x, f.y, &y0, &y1);
   }
   return two<T>(y0, y1);
