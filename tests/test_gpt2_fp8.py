@@ -127,7 +127,7 @@ def _example(launcher, **env):
 @pytest.mark.parametrize("bits", ["0", "8", "32"])
 def test_two_ranks_train_it_data_parallel(bits):
     """The example over gloo: the replicas stay equal, which it checks itself."""
-    r = _example(("-m", "torchmpi_b200.launch", "--nproc", "2"), EXAMPLE_ADAMW=bits)
+    r = _example(("-m", "torchmpi_b200.launch", "--nproc", "2"), EXAMPLE_ADAMW=bits, OMP_NUM_THREADS="2")
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-3000:]
 
 
