@@ -529,3 +529,21 @@ def test_64_bits_of_norms_and_mixed_devices():
     with pytest.raises(ValueError):
         adamw.grad_norm([a, torch.ones(5)])
     assert adamw.grad_norm([a.double()]).dtype == torch.float64
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_refused_step_changes_nothing(bits, device):
+    """The last of the parameters is refused, and the first ones, the counts, the averages and the norm are as they were."""
+    p = [torch.ones(300, device=device), torch.ones(5, 7, device=device)]
+    o = adamw.AdamW(p, bits=bits, max_norm=1.0)
+    for t in p:
+        t.grad = torch.full_like(t, 0.5)
+    o.step()
+    p[1].grad = None
+    p[1].data = p[1].data.t()
+    p[1].grad = torch.full_like(p[1], 2.0)
+    before = [t.clone() for t in (p[0], o.state[p[0]]["step"], *o.moments(), o.grad_norm)]
+    with pytest.raises(ValueError, match="changed"):
+        o.step()
+    assert all(torch.equal(a, b) for a, b in zip(before, (p[0], o.state[p[0]]["step"], *o.moments(), o.grad_norm)))

@@ -199,19 +199,22 @@ class AdamW:
 
     @torch.no_grad()
     def _step(self, options, rates) -> None:
+        for p, made in zip(self._params, self._made):          # all of them before anything changes
+            if p.grad is None:
+                continue
+            if (p.dtype, p.shape, self._order(p)) != made:
+                raise ValueError(f"AdamW: a parameter has changed: {p.dtype} {tuple(p.shape)} with strides {p.stride()}")
+            if p.grad.is_sparse or p.grad.shape != p.shape:
+                raise ValueError(f"AdamW: a gradient that is not its parameter's: {tuple(p.grad.shape)}")
         scale = self.grad_scale
         if self.max_norm is not None:
             grads = [p.grad for p in self._params if p.grad is not None]
             self._norm.copy_(abs(scale) * grad_norm(grads) if grads else torch.zeros(()))
             scale = scale * torch.clamp_max(self.max_norm / (self._norm + 1e-6), 1)
         which = [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
-        for p, i, made in zip(self._params, which, self._made):
+        for p, i in zip(self._params, which):
             if p.grad is None or not p.numel():
                 continue
-            if (p.dtype, p.shape, self._order(p)) != made:
-                raise ValueError(f"AdamW: a parameter has changed: {p.dtype} {tuple(p.shape)} with strides {p.stride()}")
-            if p.grad.is_sparse or p.grad.shape != p.shape:
-                raise ValueError(f"AdamW: a gradient that is not its parameter's: {tuple(p.grad.shape)}")
             st, (rate, b1, b2, eps, decay) = self.state[p], options[i]
             rate = float(rate if rates[i] is None else rates[i])
             st["step"] += 1
