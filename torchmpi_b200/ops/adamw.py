@@ -64,7 +64,8 @@ def _value_v(code: torch.Tensor, top: torch.Tensor) -> torch.Tensor:
 
 
 def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
-    """The 2-norm of all tensors together, a 0-dimensional fp32 tensor on their device (of 64 bits: fp64); nothing waits for it."""
+    """The 2-norm of all tensors together, a 0-dimensional fp32 tensor on their device (of 64 bits: fp64); nothing waits for it.  On the GPU squares are formed in fp32: elements
+    beyond 1e19 make the norm infinite (a clipped step then takes its gradients for zero), and those below 1e-23 count as zero in it."""
     tensors = [t.detach() for t in tensors]
     if not tensors:
         return torch.zeros(())
