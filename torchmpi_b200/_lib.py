@@ -227,6 +227,7 @@ _CUDA_PROTOS = {
     "tmpi_fp8_few_tokens": (_i, []),
     "tmpi_fp8_few": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "tmpi_fp8_product_workspace_bytes": (_sz, [_i, _i, _i]),
+    "tmpi_fp8_product_form": (_i, [_i, _i, _i, _ip, _ip]),
     "tmpi_fp8_product": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "tmpi_adamw_max_groups": (_i, []),
     "tmpi_adamw_step": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _vp]),

@@ -404,6 +404,7 @@ int tmpi_fp8_few(const void* x, int64_t ld, const void* q, const void* scale, co
 // c [M, N] = a b^T (+ bias), both in 8 bits, K columns; gelu: the GELU of the rounded sums, which go to z where it is given.  tmpi_fp8_product_sums: the same without
 // either, and db [M] = the columns' sums of `tiles` rows of sums [tiles, M] beside it.
 size_t tmpi_fp8_product_workspace_bytes(int M, int N, int K);
+int tmpi_fp8_product_form(int M, int N, int K, int* columns, int* slices);      // which form these sizes take: columns of a tile, slices of K
 int tmpi_fp8_product(const void* qa, const void* sa, const void* qb, const void* sb, const void* bias, void* c, void* z, int M, int N, int K, int gelu, int dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
 int tmpi_fp8_product_sums(const void* qa, const void* sa, const void* qb, const void* sb, void* c, const float* sums, int tiles, void* db, int M, int N, int K, int dtype,

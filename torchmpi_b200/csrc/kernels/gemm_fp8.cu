@@ -548,6 +548,14 @@ using namespace tmpi;
 
 extern "C" {
 
+int tmpi_fp8_product_form(int M, int N, int K, int* columns, int* slices) {
+  if (gemm8::too_large(M, N, K)) return fail(TMPI_ERR_INVALID, "fp8_product_form: %d x %d x %d", M, N, K);
+  const gemm8::Plan pl = gemm8::plan_of(M, N, fp8::blocks_of(K));
+  *columns = pl.bn;
+  *slices = pl.slices;
+  return TMPI_OK;
+}
+
 size_t tmpi_fp8_product_workspace_bytes(int M, int N, int K) {
   if (gemm8::too_large(M, N, K)) return 0;
   const gemm8::Plan pl = gemm8::plan_of(M, N, fp8::blocks_of(K));
