@@ -133,6 +133,7 @@ __device__ __forceinline__ uint32_t bytes(const float* r) {
 constexpr float LEAST = 7.888609052210118e-31f;          // 2^-100: what a share is divided by at least
 constexpr float LEAST_EPS = 1e-37f;                      // an element without any gradient is 0 / (0 + eps): stays, also with eps = 0
 constexpr float LEAST_EPS8 = 1e-18f;                     // of 8-bit states, which know no root below 1e-19
+constexpr float LEAST_DIVISOR = 2e-38f;                  // the least eps over a large rate: a subnormal divisor counts as zero in `rcp`, and 0 / 0 is no number
 
 // the largest magnitude of 128 elements, of which 128 / PER lanes have PER each; NaN if one is not finite
 template <int PER>
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(THREADS, 5) step_kernel(const __grid_constant_
         const float step = lr / -expm1f(t * g.log_beta1);
         const bool moves = step >= 1e-30f;
         unbias = moves ? rsqrtf(-expm1f(t * g.log_beta2)) / step : 0.f;
-        eps = moves ? fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step : __uint_as_float(0x7f800000u);
+        eps = moves ? fmaxf(fmaxf(g.eps, BITS == 8 ? LEAST_EPS8 : LEAST_EPS) / step, LEAST_DIVISOR) : __uint_as_float(0x7f800000u);
         keep = 1.f - lr * g.decay;
         b1 = g.beta1, b2 = g.beta2, a1 = g.rest1 * coefficient, a2 = sqrtf(g.rest2) * coefficient;
         unit_m = b1 * (1.f / 16129.f), unit_v = sqrtf(b2) * (1.f / 65025.f);
