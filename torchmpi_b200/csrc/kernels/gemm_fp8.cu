@@ -200,19 +200,30 @@ template <typename T> __device__ __forceinline__ float2 untwo(uint32_t w);
 template <> __device__ __forceinline__ float2 untwo<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 untwo<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// gelu of two rounded values, in a word of them
+// gelu of two rounded values, in a word of them; bf16 ones are `gelu_arguments`
 template <typename T>
 __device__ __forceinline__ uint32_t gelu_word(uint32_t w) {
+  const float2 f = untwo<T>(w);
   float y0, y1;
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) {          // results of 8 bits: the quicker form (gelu.cuh), whose Phi stops at 2^-60: from -1024 on (-inf too) nothing is left of z
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(w), "r"(0xc480c480u));
-    const float2 f = untwo<T>(w);
-    attn_util::unpack2(shared_gelu2(attn_util::pack2(__float_as_uint(f.x), __float_as_uint(f.y))), y0, y1);
-  } else {
-    const float2 f = untwo<T>(w);
-    gelu_value2(f.x, f.y, &y0, &y1);
-  }
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) attn_util::unpack2(shared_gelu2(attn_util::pack2(__float_as_uint(f.x), __float_as_uint(f.y))), y0, y1);          // results of 8 bits: the quicker form (gelu.cuh)
+  else gelu_value2(f.x, f.y, &y0, &y1);
   return two<T>(y0, y1);
+}
+// The Phi of that form stops at 2^-60: of what lies below -1024 nothing may be left, and -inf times nothing is no number.  Both are rare: a minimum for each word tells whether a thread has any.
+template <int WORDS>
+__device__ __forceinline__ void gelu_arguments(uint32_t (&w)[WORDS]) {
+  uint32_t least = w[0];
+#pragma unroll
+  for (int j = 1; j < WORDS; ++j) asm("min.bf16x2 %0, %0, %1;" : "+r"(least) : "r"(w[j]));
+  const float2 f = untwo<__nv_bfloat16>(least);
+  if (f.x < -1024.f || f.y < -1024.f) {
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) {
+      if ((w[j] & 0xffffu) == 0xff80u) w[j] |= 0x7fu;
+      if (w[j] >> 16 == 0xff80u) w[j] |= 0x7f0000u;
+      asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w[j]) : "r"(0xc480c480u));
+    }
+  }
 }
 
 // Four (two) groups of four warps in each CTA take the tile's slices of 32 columns in turn.  A warp has 32 rows of a slice: it stages them in shared memory and
@@ -300,6 +311,7 @@ __device__ __forceinline__ void epilogue(Shared* sh, unsigned char* staging, con
       if (MODE != WITH_GELU) put(0);
       if (MODE != PLAIN) {              // the GELU of what is rounded
         if constexpr (sizeof(T) == 2) {
+          if constexpr (std::is_same_v<T, __nv_bfloat16>) gelu_arguments(w);
 #pragma unroll
           for (int j = 0; j < WORDS; ++j) w[j] = gelu_word<T>(w[j]);
         } else {
