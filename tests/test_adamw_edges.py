@@ -29,3 +29,48 @@ def test_no_gradient_no_eps_at_any_rate(lr, beta1, dtype, bits, device):
     want = 1 - 2 * lr
     got = float((opt.state[p]["master"] if dtype != FP32 else p.detach())[3])
     assert abs(got - want) <= 2.0 ** -17 * (1 + 2 * lr)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype,grad_dtype,master", [(BF, FP32, True), (BF, FP32, False), (HALF, FP32, True), (HALF, FP32, False), (HALF, BF, True), (BF, HALF, False), (FP32, BF, True)])
+def test_gradients_of_another_type(dtype, grad_dtype, master, bits, device):
+    """A gradient counts as it is, not rounded to its parameter's type: 1 + 2^-12 is not 1, and what fp16 does not hold is not infinite.  Beside parameters with gradients of their own
+    type, transposed ones among them."""
+    gen = torch.Generator().manual_seed(6)
+    shapes = [(33, 20), (300,), (129,)]
+    ps = [torch.randn(s, generator=gen).to(dtype).to(device) for s in shapes]
+    ps[0] = ps[0].t().contiguous().t()
+    ps = [p.requires_grad_(True) for p in ps]
+    opt = adamw.AdamW(ps, lr=1e-2, weight_decay=0.1, eps=1e-6, bits=bits, master_weights=master, max_norm=1e9)
+    grads = [torch.randn(s, generator=gen) for s in shapes]
+    grads[1][:4] = torch.tensor([1 + 2.0 ** -12, 1e5 if dtype == HALF else 1.0, -(1 + 2.0 ** -9), 2.0 ** -10])
+    grads[1] = grads[1].to(grad_dtype)
+    grads[0], grads[2] = grads[0].to(grad_dtype), grads[2].to(dtype)
+    old = [p.detach().double().cpu() for p in ps]
+    for p, g in zip(ps, grads):
+        p.grad_dtype = None
+        p.grad = g.to(device)
+    version = ps[1]._version
+    opt.step()
+    assert ps[1]._version > version
+    want_norm = sum(float(g.double().square().sum()) for g in grads) ** 0.5
+    assert float(opt.grad_norm) == pytest.approx(want_norm, rel=1e-6)
+    for p, g, w in zip(ps, grads, old):
+        g = g.double()
+        m, v = 0.1 * g, 0.001 * g * g
+        want = w * (1 - 1e-3) - 1e-2 * g / (g.abs() + 1e-6)
+        info = torch.finfo(dtype)
+        assert int(opt.state[p]["step"]) == 1
+        if "master" in opt.state[p]:
+            assert ((opt.state[p]["master"].double().cpu() - want).abs() <= 2.0 ** -20 * (w.abs() + 0.2)).all()
+            assert torch.equal(p.detach(), opt.state[p]["master"].to(dtype))
+        assert ((p.detach().double().cpu() - want).abs() <= 2.0 ** -20 * (w.abs() + 0.2) + want.abs() * info.eps / 2 + info.smallest_normal * info.eps).all()
+        if bits == 32:
+            for got, x in zip(opt.moments(p), (m, v)):
+                assert ((got.double().cpu() - x).abs() <= 2.0 ** -20 * x.abs() + 1e-30).all()
+        else:
+            top = opt.state[p]["exp_avg_scale"].double().cpu()
+            flat = torch.empty_strided(p.shape, p.stride(), dtype=torch.float64).copy_(m).as_strided((p.numel(),), (1,))
+            pieces = torch.nn.functional.pad(flat, (0, -p.numel() % 128)).view(-1, 128).abs().amax(1)
+            assert ((top - pieces).abs() <= 2.0 ** -20 * pieces).all()

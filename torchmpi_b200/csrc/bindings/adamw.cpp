@@ -9,10 +9,10 @@
 namespace tmpi_bind {
 namespace {
 
-// The gradient in the order of the parameter's storage, of its type.
-Tensor in_order(const Tensor& g, const Tensor& p) {
-  if (g.scalar_type() == p.scalar_type() && g.strides() == p.strides()) return g;
-  Tensor c = at::empty_like(p);
+// A tensor of p's shape in the order of its storage, of the given type.
+Tensor in_order(const Tensor& g, const Tensor& p, at::ScalarType type) {
+  if (g.scalar_type() == type && g.strides() == p.strides()) return g;
+  Tensor c = at::empty_like(p, p.options().dtype(type));
   c.copy_(g);
   return c;
 }
@@ -50,6 +50,7 @@ struct AdamW {
       }
     }
     std::vector<Tensor> kept;                                        // gradients that had to be copied
+    std::vector<std::pair<Tensor, Tensor>> stepped;                  // parameters, and the fp32 tensors that are stepped in their place
     std::vector<tmpi_adamw_tensor_t> tables[3];
     for (size_t i = 0; i < params.size(); ++i) {
       const Tensor& p = params[i];
@@ -59,10 +60,15 @@ struct AdamW {
       TORCH_CHECK_VALUE(p.numel() == sizes[i] && p.scalar_type() == types[i] && in_same_order(p, strides[i]) && p.is_non_overlapping_and_dense(), "AdamW: a parameter has changed: ", p.scalar_type(), " ", p.sizes(),
                         " with strides ", p.strides());
       TORCH_CHECK_VALUE(!grad.is_sparse() && grad.layout() == at::kStrided && grad.device() == p.device() && grad.sizes() == p.sizes(), "AdamW: a gradient that is not its parameter's: ", grad.sizes());
-      const Tensor ordered = in_order(grad, p);
+      // A gradient of another type than its 16-bit parameter's counts as it is: the step is that of an fp32 parameter, the master or a copy, whose rounding the parameter becomes.
+      const bool other = grad.scalar_type() != types[i] && types[i] != at::kFloat;
+      const at::ScalarType type = other ? at::kFloat : types[i];
+      const Tensor ordered = in_order(grad, p, type);
       if (!ordered.is_same(grad)) kept.push_back(ordered);
-      const int code = p.scalar_type() == at::kBFloat16 ? 0 : p.scalar_type() == at::kHalf ? 1 : 2;
-      tables[code].push_back({p.data_ptr(), ordered.data_ptr(), places[i], sizes[i], (int)p.element_size(), group[i], (int)i});
+      const Tensor w = !other ? p : master.defined() ? master.slice(0, places[i], places[i] + sizes[i]).as_strided(p.sizes(), p.strides()) : in_order(p, p, type);
+      if (other) stepped.emplace_back(p, w);
+      const int code = type == at::kBFloat16 ? 0 : type == at::kHalf ? 1 : 2;
+      tables[code].push_back({w.data_ptr(), ordered.data_ptr(), places[i], sizes[i], (int)w.element_size(), group[i], (int)i});
     }
     tmpi_adamw_states_t s{};
     s.m = m.data_ptr(); s.v = v.data_ptr();
@@ -92,6 +98,7 @@ struct AdamW {
       check(tmpi_adamw_step(tables[c].data(), (int)tables[c].size(), g.data(), (int)g.size(), &s, bits, dtype_code(TYPES[c]), stream()));
       launched(ADAMW, 1);
     }
+    for (auto& [p, w] : stepped) p.copy_(w);
     for (const auto& p : params)
       if (p.grad().defined()) p.unsafeGetTensorImpl()->bump_version();          // written to, as autograd has to know
   }
