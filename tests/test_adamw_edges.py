@@ -74,3 +74,41 @@ def test_gradients_of_another_type(dtype, grad_dtype, master, bits, device):
             flat = torch.empty_strided(p.shape, p.stride(), dtype=torch.float64).copy_(m).as_strided((p.numel(),), (1,))
             pieces = torch.nn.functional.pad(flat, (0, -p.numel() % 128)).view(-1, 128).abs().amax(1)
             assert ((top - pieces).abs() <= 2.0 ** -20 * pieces).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("master", [True, False])
+def test_states_of_another_order(master, bits, device):
+    """Codes of 8 bits lie in the order of the parameter's storage: in another order, or of another shape, they are refused and nothing changes.  States of 32 bits are those of the elements."""
+    last = torch.channels_last
+
+    def made(memory_format, shape=(8, 16, 3, 3)):
+        p = torch.randn(shape, generator=torch.Generator().manual_seed(1)).to(BF).to(device).contiguous(memory_format=memory_format).requires_grad_(True)
+        return p, adamw.AdamW([p], lr=1e-2, bits=bits, master_weights=master)
+    p, one = made(last)
+    p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(2)).to(BF).to(device)
+    one.step()
+    saved = one.state_dict()
+    q, same = made(last)
+    same.load_state_dict(saved)
+    assert all(torch.equal(a, b) for a, b in zip(one.moments(p), same.moments(q)))
+    others = [made(torch.contiguous_format)]
+    if not (bits == 32 or master):                       # by their codes alone they could be another shape's
+        others.append(made(last, (16, 8, 3, 3)))
+    for q, other in others:
+        if bits == 8:
+            before = [t.clone() for t in (*other.moments(), other.state[q]["step"])]
+            with pytest.raises(ValueError, match="order"):
+                other.load_state_dict(saved)
+            assert all(torch.equal(a, b) for a, b in zip(before, (*other.moments(), other.state[q]["step"])))
+        else:
+            other.load_state_dict(saved)
+            assert all(torch.equal(a, b) for a, b in zip(one.moments(p), other.moments(q)))
+    saved.pop("layout", None)                            # a state without it is taken for one of the same order
+    q, same = made(last)
+    same.load_state_dict(saved)
+    assert all(torch.equal(a, b) for a, b in zip(one.moments(p), same.moments(q)))
+    one_row, saved = torch.zeros(6, 1, device=device).t().requires_grad_(True), None          # a dimension of one element has no order
+    a, b = adamw.AdamW([one_row], bits=bits), adamw.AdamW([torch.zeros(1, 6, device=device).requires_grad_(True)], bits=bits)
+    b.load_state_dict(a.state_dict())

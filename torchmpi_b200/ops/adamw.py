@@ -274,12 +274,14 @@ class AdamW:
 
     # ---- checkpointing
     def state_dict(self) -> dict:
-        """Options of the groups, and for each parameter its states, in the order of the groups (copies)."""
+        """Options of the groups, and for each parameter its states and, as ``layout``, its shape and order (the strides of its dimensions), in the order of the groups (copies)."""
         options = [{k: (v.clone() if isinstance(v, torch.Tensor) else v) for k, v in g.items() if k != "params"} for g in self.param_groups]
-        return {"bits": self.bits, "param_groups": options, "state": [{k: v.clone() for k, v in self.state[p].items()} for p in self._params]}
+        layout = [[list(shape), order] for _, shape, order in self._made]
+        return {"bits": self.bits, "param_groups": options, "layout": layout, "state": [{k: v.clone() for k, v in self.state[p].items()} for p in self._params]}
 
     def load_state_dict(self, state: dict) -> None:
-        """Loads a ``state_dict`` of an optimizer of the same parameters, number of bits and masters; anything else raises, and nothing has changed then."""
+        """Loads a ``state_dict`` of an optimizer of the same parameters, number of bits and masters; anything else raises, and nothing has changed then.  Codes of 8 bits are
+        those of parameters of the same order, too."""
         saved: Sequence[dict] = state["state"]
         if state["bits"] != self.bits or len(saved) != len(self._params) or len(state["param_groups"]) != len(self.param_groups):
             raise ValueError(f"AdamW: states of {state['bits']} bits for {len(saved)} parameters, not {self.bits} bits for {len(self._params)}")
@@ -287,6 +289,10 @@ class AdamW:
             mine = self.state[p]
             if set(st) != set(mine) or any(st[k].shape != mine[k].shape or st[k].dtype != mine[k].dtype for k in mine):
                 raise ValueError("AdamW: a parameter's states are not those of this optimizer's")
+        if self.bits == 8 and "layout" in state:
+            for (_, shape, order), (saved_shape, saved_order) in zip(self._made, state["layout"]):
+                if list(shape) != list(saved_shape) or order != list(saved_order):
+                    raise ValueError(f"AdamW: 8-bit states of a parameter {list(saved_shape)} in the order of strides {list(saved_order)}, not {list(shape)} and {order}")
         with torch.no_grad():
             for g, options in zip(self.param_groups, state["param_groups"]):
                 for k, v in options.items():
