@@ -112,3 +112,42 @@ def test_states_of_another_order(master, bits, device):
     one_row, saved = torch.zeros(6, 1, device=device).t().requires_grad_(True), None          # a dimension of one element has no order
     a, b = adamw.AdamW([one_row], bits=bits), adamw.AdamW([torch.zeros(1, 6, device=device).requires_grad_(True)], bits=bits)
     b.load_state_dict(a.state_dict())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("options", [dict(lr=-1.0), dict(betas=(0.9, 2.0)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(momentum=0.9), dict(lr=torch.tensor([0.1, 0.2])),
+                                     dict(betas=0.9)], ids=str)
+def test_options_that_are_none_are_not_loaded(options, device):
+    """Refused before anything has changed, the options of the groups before and the averages among it."""
+    ps = [torch.ones(5, device=device).requires_grad_(True) for _ in range(2)]
+    rate = torch.tensor(0.5, device=device)
+    opt = adamw.AdamW([{"params": ps[:1], "lr": 0.25}, {"params": ps[1:], "lr": rate}])
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    other = adamw.AdamW([{"params": [torch.ones(5, device=device).requires_grad_(True)], "lr": 0.125}, {"params": [torch.ones(5, device=device).requires_grad_(True)]}])
+    saved = other.state_dict()
+    saved["param_groups"][1].update(options)
+    before = [t.clone() for t in opt.moments()]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[1]["lr"] is rate and float(rate) == 0.5 and "momentum" not in opt.param_groups[1]
+    assert all(torch.equal(a, b) for a, b in zip(before, opt.moments())) and int(opt.state[ps[0]]["step"]) == 1
+    opt.step()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_loaded_learning_rate_of_another_form(device):
+    """One number of another type or shape is that number."""
+    rate = torch.tensor(0.5, device=device)
+    for lr in (rate, 0.125):
+        for saved_lr in (torch.tensor([0.25]), torch.tensor(0.25, dtype=torch.float64)):
+            p = torch.zeros(5, device=device).requires_grad_(True)
+            opt = adamw.AdamW([p], lr=lr)
+            state = opt.state_dict()
+            state["param_groups"][0]["lr"] = saved_lr
+            opt.load_state_dict(state)
+            p.grad = torch.ones_like(p)
+            opt.step()
+            assert torch.allclose(p.detach(), torch.full_like(p, -0.25), rtol=1e-6)
+    assert float(rate) == 0.25

@@ -168,9 +168,9 @@ class AdamW:
     def _has_master(self, p: torch.Tensor) -> bool:
         return self._master is not None and p.dtype != torch.float32
 
-    def _options(self):
+    def _options(self, groups: Optional[Sequence[dict]] = None):
         options, rates = [], []
-        for g in self.param_groups:
+        for g in self.param_groups if groups is None else groups:
             lr, (b1, b2), eps, decay = g["lr"], g["betas"], g["eps"], g["weight_decay"]
             on_device = isinstance(lr, torch.Tensor)
             if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and decay >= 0 and (on_device or lr >= 0)):
@@ -293,13 +293,17 @@ class AdamW:
             for (_, shape, order), (saved_shape, saved_order) in zip(self._made, state["layout"]):
                 if list(shape) != list(saved_shape) or order != list(saved_order):
                     raise ValueError(f"AdamW: 8-bit states of a parameter {list(saved_shape)} in the order of strides {list(saved_order)}, not {list(shape)} and {order}")
+        for g, options in zip(self.param_groups, state["param_groups"]):
+            if set(options) - (set(g) - {"params"}) or any(isinstance(v, torch.Tensor) and (k != "lr" or v.numel() != 1) for k, v in options.items()) or not isinstance(options.get("betas", ()), (tuple, list)):
+                raise ValueError(f"AdamW: a group's options are none: {options}")
+            self._options([{**g, **options}])
         with torch.no_grad():
             for g, options in zip(self.param_groups, state["param_groups"]):
                 for k, v in options.items():
                     if isinstance(v, torch.Tensor) and isinstance(g[k], torch.Tensor):
-                        g[k].copy_(v)                # where a captured step reads it
+                        g[k].copy_(v.reshape(g[k].shape))                # where a captured step reads it
                     else:
-                        g[k] = v.to(self._steps.device, copy=True) if isinstance(v, torch.Tensor) else v
+                        g[k] = v.to(self._steps.device, torch.float32, copy=True) if isinstance(v, torch.Tensor) else v
             for p, st in zip(self._params, saved):
                 for k, v in self.state[p].items():
                     v.copy_(st[k])
