@@ -151,3 +151,29 @@ def test_a_loaded_learning_rate_of_another_form(device):
             opt.step()
             assert torch.allclose(p.detach(), torch.full_like(p, -0.25), rtol=1e-6)
     assert float(rate) == 0.25
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_refused_step_keeps_the_rates(device):
+    """A step that is refused, for its rate or for a gradient, leaves the groups' rates too."""
+    ps = [torch.ones(5, device=device).requires_grad_(True) for _ in range(2)]
+    opt = adamw.AdamW([{"params": ps[:1], "lr": 0.25}, {"params": ps[1:], "lr": 0.5}])
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    calls = [lambda: opt.step(lr=-1.0)]
+    if device == "cuda":
+        calls.append(lambda: opt.step(lr=torch.tensor(0.1)))          # on the host
+
+    def of_another_order():
+        ps[1].grad = None
+        ps[1].data = torch.ones(7, device=device)
+        ps[1].grad = torch.ones(7, device=device)
+        opt.step(lr=0.125)
+    for call in (*calls, of_another_order):
+        with pytest.raises(ValueError):
+            call()
+        assert [g["lr"] for g in opt.param_groups] == [0.25, 0.5] and int(opt.state[ps[0]]["step"]) == 0
+    ps[1].data = torch.ones(5, device=device)
+    ps[1].grad = None
+    opt.step(lr=0.125)
+    assert [g["lr"] for g in opt.param_groups] == [0.125, 0.125]

@@ -188,15 +188,15 @@ class AdamW:
 
     # ---- one step
     def step(self, lr: Optional[Union[float, torch.Tensor]] = None) -> None:
-        """``lr``: the learning rate of all groups from now on."""
-        if lr is not None:
-            for g in self.param_groups:
-                g["lr"] = lr
-        options, rates = self._options()
+        """``lr``: the learning rate of all groups from now on, in the place of rates of their own and of tensors on the device."""
+        options, rates = self._options(None if lr is None else [{**g, "lr": lr} for g in self.param_groups])
         if self._native is not None:
             self._native.step(options, rates, self.max_norm, self.grad_scale)
         else:
             self._step(options, rates)
+        if lr is not None:                       # not by a step that was refused
+            for g in self.param_groups:
+                g["lr"] = lr
 
     @torch.no_grad()
     def _step(self, options, rates) -> None:
