@@ -177,3 +177,22 @@ def test_a_refused_step_keeps_the_rates(device):
     ps[1].grad = None
     opt.step(lr=0.125)
     assert [g["lr"] for g in opt.param_groups] == [0.125, 0.125]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_checkpoint_of_the_model_alone(bits, device, tmp_path):
+    """Loaded weights are those that the next step starts from, also where the file holds no optimizer."""
+    from torchmpi_b200.utils import checkpoint
+    torch.manual_seed(0)
+    a, b = (torch.nn.Linear(40, 30).to(BF).to(device) for _ in range(2))
+    checkpoint.save(str(tmp_path / "model.pt"), a)
+    opt = adamw.AdamW(b.parameters(), lr=1e-4, weight_decay=0.0, bits=bits)
+    checkpoint.load(str(tmp_path / "model.pt"), b, opt)
+    assert all(torch.equal(p, q) and torch.equal(opt.state[q]["master"], p.detach().float()) for p, q in zip(a.parameters(), b.parameters()))
+    for p in b.parameters():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    for p, q in zip(a.parameters(), b.parameters()):          # a first step is as long as its rate
+        want = p.detach().double() - 1e-4
+        assert ((opt.state[q]["master"].double() - want).abs() <= 2.0 ** -20 * (want.abs() + 1e-4)).all()

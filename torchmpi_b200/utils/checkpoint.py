@@ -6,7 +6,7 @@ rank 0: the model's ``state_dict`` (parameters are replicated, so rank 0's copy 
 when an optimizer is given, its state (of the fused one the gathered fp32 master weights and momentum, of AdamW averages, step counts and masters), and, when parameter
 servers are passed, the tensors they hold (pulled from their shards before the file is written).  ``load``
 restores them on every rank, re-synchronises the parameters from rank 0 and writes the saved tensors
-back into the parameter servers.
+back into the parameter servers.  An optimizer that the file holds nothing of takes its fp32 master weights anew from the parameters.
 """
 from __future__ import annotations
 
@@ -57,6 +57,8 @@ def load(path: str, model: torch.nn.Module, optimizer=None, synchronize: bool = 
         buckets = state["optimizer"].get("buckets")                # of the fused optimizer
         if hasattr(optimizer, "refresh_master") and buckets and buckets[0].get("master") is None:
             optimizer.refresh_master()
+    elif optimizer is not None and "optimizer" not in state and hasattr(optimizer, "refresh_master"):
+        optimizer.refresh_master()                                 # masters of the weights from before
     if parameter_servers and "parameter_servers" in state:
         if len(parameter_servers) != len(state["parameter_servers"]):
             raise ValueError("the checkpoint holds another number of parameter-server tensors")
