@@ -1,0 +1,58 @@
+"""The engine with an optimizer in the place of SGD: optimizers that were made earlier, and rates of the groups' own."""
+import pytest
+import torch
+
+from mp_util import run_ranks
+from torchmpi_b200.engine import AllReduceSGDEngine
+from torchmpi_b200.ops import adamw
+
+
+def _net(seed, dtype=torch.bfloat16):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(torch.nn.Linear(20, 150), torch.nn.ReLU(), torch.nn.Linear(150, 10)).to(dtype)
+
+
+def _data(seed, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    return [{"input": torch.randn(16, 20, generator=g).to(dtype), "target": torch.randint(0, 10, (16,), generator=g)} for _ in range(4)]
+
+
+class _Loss(torch.nn.Module):
+    def forward(self, x, target):
+        return torch.nn.functional.cross_entropy(x.float(), target)
+
+
+def _states(opt):
+    return [t.double().tolist() for p in opt.state for _, t in sorted(opt.state[p].items())]
+
+
+def _made_earlier(rank, world, bits):
+    """Every rank's optimizer has masters and averages of its own before the engine synchronises the parameters."""
+    import torchmpi_b200 as mpi
+    from torchmpi_b200 import nn as mpinn
+    mpi.start(with_cuda=False)
+    net = _net(rank)
+    opt = adamw.AdamW(net.parameters(), lr=0.01, bits=bits)
+    for s in _data(10 + rank)[: 2 + rank]:
+        opt.zero_grad()
+        _Loss()(net(s["input"]), s["target"]).backward()
+        opt.step()
+    opt.zero_grad()
+    before = [p.detach().clone() for p in net.parameters()], _states(opt)
+    engine = AllReduceSGDEngine(gradient_scale=1.0 / world, optimizer=lambda params: opt)
+    started = {}
+    engine.hooks["onStart"] = lambda state: started.update(weights=[p.detach().clone() for p in net.parameters()], states=_states(opt))
+    engine.train(net, _Loss(), _data(3), lr=0.01, maxepoch=1)
+    assert engine.own_optimizer is opt
+    if rank == 0:                                        # rank 0's are everybody's, as they were
+        assert all(torch.equal(a, b) for a, b in zip(started["weights"], before[0])) and started["states"] == before[1]
+    mpinn.check_with_allreduce(net)
+    out = [p.detach().float().reshape(-1).tolist() for p in net.parameters()], started["states"], _states(opt)
+    mpi.stop()
+    return out
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_an_optimizer_that_was_made_earlier(bits):
+    got = run_ranks(_made_earlier, 2, bits, timeout=300)
+    assert got[0] == got[1]

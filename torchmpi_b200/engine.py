@@ -11,6 +11,8 @@ the weight update, and writes the new weights to every peer - no NCCL call and
 no separate optimizer kernel.  ``fused=False`` (and every CPU run) takes the
 reference's shape: ``synchronize_gradients`` then a per-tensor update.  With ``optimizer`` (a function that makes one of the network's
 parameters, ``lambda params: ops.adamw.AdamW(params, bits=8)`` say) its ``step(lr)`` takes the place of that update, after the same synchronisation.
+It may hand back one that was made earlier (to resume, say): where that has a ``synchronize()``, all ranks start from rank 0's states, as they
+start from its parameters.
 
 Per sample:  onSample -> forward -> onForward -> criterion -> onForwardCriterion
 -> zero grads -> criterion backward -> onBackwardCriterion -> network backward
@@ -111,7 +113,8 @@ class AllReduceSGDEngine:
                                  grad_scale=self.gradient_scale, master_weights=self.master_weights,
                                  bucket_bytes=self.bucket_bytes, overlap=True)
             network._tmpi_buckets = self._opt.buckets
-        if len(runtime.intra_members(runtime.collective_span()[0])) > 1:
+        several = len(runtime.intra_members(runtime.collective_span()[0])) > 1
+        if several:
             # initial one-shot synchronisation of the parameters from rank 0
             mpinn.synchronize_parameters(network)
             if isinstance(criterion, torch.nn.Module):
@@ -120,6 +123,8 @@ class AllReduceSGDEngine:
             self._opt.refresh_master()
         if self.optimizer is not None:           # after the synchronisation: masters are copies of the parameters
             self.own_optimizer = self.optimizer([p for p in network.parameters() if p.requires_grad])
+            if several and hasattr(self.own_optimizer, "synchronize"):      # one that was made earlier may hold states of this rank's own
+                self.own_optimizer.synchronize()
 
     def _plain_update(self, params: Iterable[torch.nn.Parameter], lr: float) -> None:
         """w += -lr * g per tensor (torchnet's SGD step), with optional momentum / weight decay."""

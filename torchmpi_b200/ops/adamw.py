@@ -186,6 +186,13 @@ class AdamW:
                 if self._has_master(p):
                     self.state[p]["master"].copy_(p)
 
+    def synchronize(self, root: int = 0) -> None:
+        """Collective: makes every rank hold rank ``root``'s averages, step counts and masters, as the replicas of a model hold its parameters."""
+        from ..collectives import broadcast_tensor
+        for flat in (self._m, self._v, self._m_top, self._v_top, self._master, self._steps):
+            if flat is not None and flat.numel():
+                broadcast_tensor(root, flat)
+
     # ---- one step
     def step(self, lr: Optional[Union[float, torch.Tensor]] = None) -> None:
         """``lr``: the learning rate of all groups from now on, in the place of rates of their own and of tensors on the device."""
