@@ -56,3 +56,39 @@ def _made_earlier(rank, world, bits):
 def test_an_optimizer_that_was_made_earlier(bits):
     got = run_ranks(_made_earlier, 2, bits, timeout=300)
     assert got[0] == got[1]
+
+
+def _own_rates(rank, world):
+    import torchmpi_b200 as mpi
+    mpi.start(with_cuda=False)
+    net, rate = _net(0), torch.tensor(0.01)
+    before = [p.detach().clone() for p in net.parameters()]
+    made = lambda ps: adamw.AdamW([{"params": ps[:2], "lr": 0.0, "weight_decay": 0.0}, {"params": ps[2:], "lr": rate}])      # noqa: E731
+    engine = AllReduceSGDEngine(optimizer=made)
+    engine.train(net, _Loss(), _data(3), lr=None, maxepoch=1)
+    now = list(net.parameters())
+    assert all(torch.equal(a, b) for a, b in zip(now[:2], before[:2])) and not any(torch.equal(a, b) for a, b in zip(now[2:], before[2:]))
+    assert engine.own_optimizer.param_groups[0]["lr"] == 0.0 and engine.own_optimizer.param_groups[1]["lr"] is rate and float(rate) == torch.tensor(0.01).item()
+    engine.train(net, _Loss(), _data(3), lr=0.02, maxepoch=1, maxsteps=1)
+    assert [g["lr"] for g in engine.own_optimizer.param_groups] == [0.02, 0.02]
+    # nothing else has rates of its own
+    class Criterion(_Loss):
+        def __init__(self):
+            super().__init__()
+            self.scale = torch.nn.Parameter(torch.ones(()))
+
+        def forward(self, x, target):
+            return super().forward(x * self.scale, target)
+    before = [p.detach().clone() for p in net.parameters()]
+    for call in (lambda: AllReduceSGDEngine().train(net, _Loss(), _data(3), lr=None, maxepoch=1), lambda: engine.train(net, Criterion(), _data(3), lr=None, maxepoch=1)):
+        with pytest.raises(ValueError, match="lr"):
+            call()
+    assert all(torch.equal(a, b) for a, b in zip(net.parameters(), before))
+    criterion = Criterion()
+    engine.train(net, criterion, _data(3), lr=None, lrcriterion=0.1, maxepoch=1)
+    assert float(criterion.scale) != 1.0
+    mpi.stop()
+
+
+def test_rates_of_the_optimizers_own_groups():
+    run_ranks(_own_rates, 1, timeout=300)

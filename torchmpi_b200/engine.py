@@ -178,7 +178,7 @@ class AllReduceSGDEngine:
                         p.grad.mul_(self.gradient_scale)
             self.hook("onBackward", state)
             if self.own_optimizer is not None:
-                self.own_optimizer.step(state["lr"])
+                self.own_optimizer.step() if state["lr"] is None else self.own_optimizer.step(state["lr"])
             else:
                 self._plain_update(network.parameters(), state["lr"])
             if isinstance(criterion, torch.nn.Module) and any(True for _ in criterion.parameters()):
@@ -187,8 +187,13 @@ class AllReduceSGDEngine:
         self.hook("onUpdate", state)
         return loss
 
-    def train(self, network, criterion, iterator, lr: float, lrcriterion: Optional[float] = None,
+    def train(self, network, criterion, iterator, lr: Optional[float], lrcriterion: Optional[float] = None,
               maxepoch: int = 1000, maxsteps: Optional[int] = None):
+        """``lr``: the learning rate (``state["lr"]``, which a hook may change); with ``optimizer`` it replaces those of its groups, and None leaves them."""
+        if lr is None and self.optimizer is None:
+            raise ValueError("lr is None, which leaves an optimizer's own rates, but there is none")
+        if lr is None and lrcriterion is None and isinstance(criterion, torch.nn.Module) and any(True for _ in criterion.parameters()):
+            raise ValueError("lr is None and so is lrcriterion, the learning rate of the criterion's parameters")
         state = {"network": network, "criterion": criterion, "iterator": iterator, "lr": lr,
                  "lrcriterion": lr if lrcriterion is None else lrcriterion, "maxepoch": maxepoch,
                  "sample": None, "epoch": 0, "t": 0, "training": True}
