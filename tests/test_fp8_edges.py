@@ -46,3 +46,17 @@ def test_gelu_of_sums_beyond_the_type(T, device):
     want = torch.zeros(T, 24).double()
     want[1:3, 3], want[1:3, 4] = float("inf"), float("nan")
     assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(y.nan_to_num(0), want.nan_to_num(0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("T,N", [(5, 0), (0, 0), (0, 3)])
+def test_layers_without_outputs_or_tokens(T, N, gelu, device):
+    """Nothing comes of them, and the gradients are zeros of the inputs' shapes."""
+    x, w, b = (torch.randn(s, device=device).to(BF).requires_grad_() for s in ((T, 7), (N, 7), (N,)))
+    y = fp8.linear(x, w, b, gelu)
+    assert y.shape == (T, N) and y.dtype == BF
+    for t, d in zip((x, w, b), torch.autograd.grad(y.sum(), (x, w, b))):
+        assert d.shape == t.shape and d.dtype == t.dtype and not d.any()
+    kept = fp8.quantize(w.detach())
+    assert fp8.linear(x.detach(), kept, b.detach(), gelu).shape == (T, N) and fp8.matmul(fp8.quantize(x.detach()), kept).shape == (T, N)

@@ -188,13 +188,13 @@ class _Linear(torch.autograd.Function):
             raise RuntimeError("products in 8 bits can be differentiated once (no create_graph)")
         x, w, z = ctx.saved_tensors
         wide = torch.promote_types(x.dtype, torch.float32)
-        q = lambda t: _dequantize(_quantize(t), wide)      # noqa: E731
+        q = lambda t: _dequantize(_quantize(t), wide) if t.numel() else t.to(wide)      # noqa: E731
         dz = dy if z is None else (dy.to(wide) * _gelu_parts(z.to(wide))[1]).to(dy.dtype)
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
             dx = (q(dz) @ q(w.t()).t()).to(x.dtype)
         if ctx.needs_input_grad[1]:
-            dw = (q(dz.t()) @ q(x.t()).t()).to(w.dtype) if x.shape[0] else torch.zeros_like(w)
+            dw = (q(dz.t()) @ q(x.t()).t()).to(w.dtype)
         if ctx.bias and ctx.needs_input_grad[2]:
             db = dz.to(wide).sum(0).to(dy.dtype)
         return dx, dw, db, None
