@@ -166,7 +166,7 @@ __device__ __forceinline__ uint2 eight(const uint32_t* w, float inv) {
 
 // ---------------------------------------------------------------- along rows
 // Eight threads to a block of 128, sixteen elements each, two of a thread's pieces under way at a time (16 bytes by each thread, so that a warp's loads
-// are whole lines, took more instructions for an element and 25.7 us in place of 18.1 at 8192 x 4096; now 16.7).  Bound by memory and instructions alike (66 % of
+// are whole lines, took more instructions for an element and 25.7 us in place of 18.1 at 8192 x 4096; now 16.7 - 17.0, fp32 29.1; out of a cold L2 24.6 and 34.8, 65536 x 1024 41.0 and 63.5).  Bound by memory and instructions alike (66 % of
 // the issue slots, 0.92 of the copy rate).  VEC: rows start on 16-byte boundaries (else 8192 x 4001 takes 21.9, by elements it took 42).
 constexpr int ROW_THREADS = 256;
 struct Stride { int rows, pieces; };          // a launch's threads, as rows of pieces (or elements): what a thread's next piece lies further
@@ -236,7 +236,7 @@ constexpr int TILE = 128, TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32, RO
 // One matrix, or two in one launch (the input and the weight of a layer): the blocks from a's tiles on take b's.
 // GELU: x is the gradient behind a GELU of z; what is kept is x gelu'(z), rounded to T.  q, scale: along the rows, or null.  sums: the columns'
 // sums over this tile's rows, [row tiles, cols], or null; both are of a alone.  VEC: rows start on 16-byte boundaries.
-// 8192 x 4096 bf16: 24.9 us both ways (0.82 of the copy rate; 57 % of the issue slots, of a warp's time two fifths waiting for its loads), with the sums 26.8, with the GELU's
+// 8192 x 4096 bf16: 24.9 us both ways, out of a cold L2 28.6 (0.82 and 0.72 of the copy rate; along columns alone 18.3 and 24.6; fp32 34.9 and 38.9; 57 % of the issue slots, of a warp's time two fifths waiting for its loads), with the sums 26.8, with the GELU's
 // gradient and the sums 53 (0.58; 28 million warp instructions, by four warps to a scheduler).  40 us both ways where rows start anywhere (8192 x 4001).
 template <typename T> struct Matrix {
   const T* x;

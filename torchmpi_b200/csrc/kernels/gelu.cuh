@@ -79,7 +79,8 @@ __device__ __forceinline__ unsigned long long quick_cdf2(unsigned long long z, u
   unpack2(add2(pack2(__float_as_uint(ex2(x0)), __float_as_uint(ex2(x1))), both(1.f)), x0, x1);
   return pack2(__float_as_uint(rcp(x0)), __float_as_uint(rcp(x1)));
 }
-// The same with one reciprocal for two elements: 1 / a = b / (a b), 1 / b = a / (a b).  The exponents stop at 60 for that (Phi below 2^-60 is as good as 0).
+// The same with one reciprocal for two elements: 1 / a = b / (a b), 1 / b = a / (a b).  The exponents stop at 60 for that: Phi below 2^-60 is as good as 0 as
+// long as z is not below -1024, which the caller sees to.
 // For kernels that the special-function unit bounds.
 __device__ __forceinline__ unsigned long long shared_cdf2(unsigned long long z, unsigned long long t) {      // t = z^2
   using namespace attn_util;

@@ -13,8 +13,9 @@
 // 447, the scales lie from 448 on.  An epilogue reads the shared columns first and says so (`shared_free`), and the next tile's MMAs
 // wait for that alone, not for the whole accumulator.
 //
-// Measured (us, bf16 results): 8192^3 366 - 380, 2.9 - 3.0 PFLOP/s, bound by the MMAs and the power limit; 8192 x 4096 x 1024 plain 31 - 33, where the epilogue of 8 blocks of K's
-// tile takes as long as its MMAs, with the GELU 39, with the pre-activation beside it 46: bound by the epilogue.
+// Measured (us, bf16 results): 8192^3 366 - 380, 2.9 - 3.0 PFLOP/s, bound by the MMAs and the power limit; 8192 x 4096 x 1024 plain 31 - 33 (its MMAs alone
+// 21: of each tile 1.25 us are not hidden, for a cause that is not known; the epilogue's warps wait for the accumulator for half of their time), with the GELU 39 - 40, with the
+// pre-activation beside it 46 - 47: bound by the epilogue.  fp16 33, 42, 48; fp32 47, 45, 61, twice the bytes to store.
 //
 // Few tiles leave SMs idle: K is then cut into slices whose fp32 sums a second kernel adds, in order, and rounds (bit-reproducible).
 #include "fp8.cuh"

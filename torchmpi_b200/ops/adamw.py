@@ -6,8 +6,8 @@
     w = (1 - lr * weight_decay) w - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
 in fp32 (an element that never had a gradient stays, also with ``eps = 0``; with 8 bits ``eps`` counts as 1e-18 at least).  Parameters of 16 bits have fp32 masters (``master_weights=True``) that the step goes by and whose rounding the parameter becomes; without, the
-parameter itself is updated and rounded.  A gradient of another type than its parameter's (``grad_dtype``) counts as it is, at the price of a copy.  ``bits=8`` keeps ``m`` and the root of ``v`` as a byte an element with an fp32 scale for 128 (4.1 bytes an element
-less to read and to write than the 8 of 32 bits, each way): ``m = sign(c) c^2 top / 127^2``, ``sqrt(v) = c^2 top / 255^2``, where ``top`` is the block's
+parameter itself is updated and rounded.  A gradient of another type than its parameter's (``grad_dtype``) counts as it is, at the price of a copy.  ``bits=8`` keeps ``m`` and the root of ``v`` as a byte an element with an fp32 scale for 128 (2.06 bytes an element
+in the place of the 8 of 32 bits, to read and to write): ``m = sign(c) c^2 top / 127^2``, ``sqrt(v) = c^2 top / 255^2``, where ``top`` is the block's
 largest magnitude; a root that is not zero never becomes zero.  An average that changes by less than half a code in a step, its block's largest
 standing still, keeps its code.  A block with an element that is not finite becomes NaN.
 

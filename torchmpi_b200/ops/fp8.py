@@ -11,7 +11,9 @@ Q(x.T).T``, ``db`` the sums of ``dz``.  ``Q`` takes its blocks along the dimensi
 an element), ``w`` too, and ``z`` as it is.  With a ``Block8`` in the place of ``w`` (weights kept in 8 bits by a generating program) there is no
 backward pass; a few tokens (up to 32) then take one launch that is bound by reading the weights.
 
-Every result is bit-reproducible; tokens are independent of each other.  What the kernels do not take (CPU, 64 bits, tensors of several
+Every result is bit-reproducible (the bytes of ``scale`` behind a matrix' last row and block mean nothing and are not); tokens are independent of each other.  How many they are decides about the
+kernel and how it cuts K: the order of the sums, and in bf16 the form of the GELU's Phi (absolute error 1.5e-7 up to 32 tokens and where K is cut, else 1.4e-6; of the slope backward 1.4e-6), so that a token
+may round otherwise among others.  ``Phi(-inf) * -inf`` is NaN.  What the kernels do not take (CPU, 64 bits, tensors of several
 types, nothing to multiply) runs on PyTorch operations.  The reference has no such products (its models are Torch7's).
 """
 from __future__ import annotations
