@@ -115,7 +115,7 @@ def test_states_of_another_order(master, bits, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("options", [dict(lr=-1.0), dict(betas=(0.9, 2.0)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(momentum=0.9), dict(lr=torch.tensor([0.1, 0.2])),
+@pytest.mark.parametrize("options", [dict(lr=-1.0), dict(betas=(0.9, 2.0)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(eps=torch.tensor(0.1)), dict(lr=torch.tensor([0.1, 0.2])),
                                      dict(betas=0.9)], ids=str)
 def test_options_that_are_none_are_not_loaded(options, device):
     """Refused before anything has changed, the options of the groups before and the averages among it."""
@@ -131,9 +131,21 @@ def test_options_that_are_none_are_not_loaded(options, device):
     before = [t.clone() for t in opt.moments()]
     with pytest.raises(ValueError):
         opt.load_state_dict(saved)
-    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[1]["lr"] is rate and float(rate) == 0.5 and "momentum" not in opt.param_groups[1]
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[1]["lr"] is rate and float(rate) == 0.5 and opt.param_groups[1]["eps"] == 1e-8
     assert all(torch.equal(a, b) for a, b in zip(before, opt.moments())) and int(opt.state[ps[0]]["step"]) == 1
     opt.step()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_programs_own_entries_of_the_groups(device):
+    """What a schedule keeps beside the options is saved and loaded with them."""
+    made = lambda: adamw.AdamW([torch.ones(5, device=device).requires_grad_(True)], lr=0.5)      # noqa: E731
+    one, two = made(), made()
+    one.param_groups[0].update(initial_lr=0.25, curve=torch.arange(3))
+    two.load_state_dict(one.state_dict())
+    assert two.param_groups[0]["initial_lr"] == 0.25 and two.param_groups[0]["curve"].tolist() == [0, 1, 2]
+    two.load_state_dict(one.state_dict())
+    two.step()
 
 
 @pytest.mark.parametrize("device", DEVICES)

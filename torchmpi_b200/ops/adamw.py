@@ -301,16 +301,20 @@ class AdamW:
                 if list(shape) != list(saved_shape) or order != list(saved_order):
                     raise ValueError(f"AdamW: 8-bit states of a parameter {list(saved_shape)} in the order of strides {list(saved_order)}, not {list(shape)} and {order}")
         for g, options in zip(self.param_groups, state["param_groups"]):
-            if set(options) - (set(g) - {"params"}) or any(isinstance(v, torch.Tensor) and (k != "lr" or v.numel() != 1) for k, v in options.items()) or not isinstance(options.get("betas", ()), (tuple, list)):
-                raise ValueError(f"AdamW: a group's options are none: {options}")
-            self._options([{**g, **options}])
+            own = {k: options.get(k, g[k]) for k in ("lr", "betas", "eps", "weight_decay")}          # others are the program's
+            if any(isinstance(v, torch.Tensor) and (k != "lr" or v.numel() != 1) for k, v in own.items()) or not isinstance(own["betas"], (tuple, list)):
+                raise ValueError(f"AdamW: a group's options are none: {own}")
+            self._options([own])
         with torch.no_grad():
             for g, options in zip(self.param_groups, state["param_groups"]):
                 for k, v in options.items():
-                    if isinstance(v, torch.Tensor) and isinstance(g[k], torch.Tensor):
-                        g[k].copy_(v.reshape(g[k].shape))                # where a captured step reads it
-                    else:
-                        g[k] = v.to(self._steps.device, torch.float32, copy=True) if isinstance(v, torch.Tensor) else v
+                    if k == "lr" and isinstance(v, torch.Tensor):
+                        if isinstance(g[k], torch.Tensor):
+                            g[k].copy_(v.reshape(g[k].shape))                # where a captured step reads it
+                        else:
+                            g[k] = v.to(self._steps.device, torch.float32, copy=True)
+                    elif k != "params":
+                        g[k] = v.clone() if isinstance(v, torch.Tensor) else v
             for p, st in zip(self._params, saved):
                 for k, v in self.state[p].items():
                     v.copy_(st[k])
