@@ -60,3 +60,17 @@ def test_layers_without_outputs_or_tokens(T, N, gelu, device):
         assert d.shape == t.shape and d.dtype == t.dtype and not d.any()
     kept = fp8.quantize(w.detach())
     assert fp8.linear(x.detach(), kept, b.detach(), gelu).shape == (T, N) and fp8.matmul(fp8.quantize(x.detach()), kept).shape == (T, N)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, HALF, FP32])
+def test_the_slope_of_the_gelu(dtype, device):
+    """For one token and a gradient of ones the bias' gradient is the slope itself.  Phi is within 7.5e-8 (half of erf's 1.5e-7), its fp32 polynomial within 1.5e-7, the exponential within 2^-22 of itself and the reciprocal
+    within 2^-23: 6e-7 together, and the rounding."""
+    z = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(BF).float() if dtype == BF else torch.linspace(-9, 9, 40001)
+    z = z[z.abs() <= 9].to(dtype)
+    x, w, b = torch.zeros(1, 16, dtype=dtype, device=device), torch.zeros(z.numel(), 16, dtype=dtype, device=device), z.to(device).requires_grad_()
+    y = fp8.linear(x, w, b, gelu=True)
+    slope, = torch.autograd.grad(y, b, torch.ones_like(y))
+    want = ref.slope(z.double())
+    ref.close(slope, want, 6e-7 + ref.half_step(want, dtype) * (1 + 2.0 ** -10), "slope")
