@@ -208,3 +208,22 @@ def test_a_checkpoint_of_the_model_alone(bits, device, tmp_path):
     for p, q in zip(a.parameters(), b.parameters()):          # a first step is as long as its rate
         want = p.detach().double() - 1e-4
         assert ((opt.state[q]["master"].double() - want).abs() <= 2.0 ** -20 * (want.abs() + 1e-4)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_number_is_loaded_into_the_rate_on_the_device(device):
+    """A captured step reads the tensor: a saved rate that is a number goes into it."""
+    p = torch.zeros(5, device=device).requires_grad_(True)
+    rate = torch.tensor(0.5, device=device)
+    opt, other = adamw.AdamW([p], lr=rate), adamw.AdamW([torch.zeros(5, device=device).requires_grad_(True)], lr=0.25)
+    p.grad = torch.ones_like(p)
+    step = opt.step
+    if device == "cuda":
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+        step = graph.replay
+    opt.load_state_dict(other.state_dict())
+    assert opt.param_groups[0]["lr"] is rate and float(rate) == 0.25
+    step()
+    assert torch.allclose(p.detach(), torch.full_like(p, -0.25), rtol=1e-6)

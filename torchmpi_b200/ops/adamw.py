@@ -288,7 +288,7 @@ class AdamW:
 
     def load_state_dict(self, state: dict) -> None:
         """Loads a ``state_dict`` of an optimizer of the same parameters, number of bits and masters; anything else raises, and nothing has changed then.  Codes of 8 bits are
-        those of parameters of the same order, too."""
+        those of parameters of the same order, too.  A learning rate that is a tensor here stays that tensor and takes the saved value."""
         saved: Sequence[dict] = state["state"]
         if state["bits"] != self.bits or len(saved) != len(self._params) or len(state["param_groups"]) != len(self.param_groups):
             raise ValueError(f"AdamW: states of {state['bits']} bits for {len(saved)} parameters, not {self.bits} bits for {len(self._params)}")
@@ -308,11 +308,10 @@ class AdamW:
         with torch.no_grad():
             for g, options in zip(self.param_groups, state["param_groups"]):
                 for k, v in options.items():
-                    if k == "lr" and isinstance(v, torch.Tensor):
-                        if isinstance(g[k], torch.Tensor):
-                            g[k].copy_(v.reshape(g[k].shape))                # where a captured step reads it
-                        else:
-                            g[k] = v.to(self._steps.device, torch.float32, copy=True)
+                    if k == "lr" and isinstance(g[k], torch.Tensor):
+                        g[k].copy_(torch.as_tensor(v).reshape(g[k].shape))                # where a captured step reads it
+                    elif k == "lr" and isinstance(v, torch.Tensor):
+                        g[k] = v.to(self._steps.device, torch.float32, copy=True)
                     elif k != "params":
                         g[k] = v.clone() if isinstance(v, torch.Tensor) else v
             for p, st in zip(self._params, saved):
